@@ -278,6 +278,129 @@ RK_API int rk_cross_entropy_fwd_bwd(const void* logits, int64_t ld, int64_t voca
                                     int64_t rows, float grad_scale, const float* grad_scale_dev, float* loss_rows,
                                     void* dlogits, int64_t ldd, int dtype, int ignore_index, void* stream);
 
+/* ------------------------------------------------ Token log-probabilities
+ * For row r of logits [rows, ld] (vocab valid columns, dtype RK_F32/RK_BF16/
+ * RK_F16, any row stride >= vocab, no alignment rule) and z = x * inv_temp:
+ *   logprob[r] = z[label] - m - ln S,  m = max z,  S = sum exp(z - m)
+ *   entropy[r] = ln S - (sum exp(z - m) (z - m)) / S       (entropy may be NULL)
+ * and stats[r] = (m, ln S) (float2, 8-byte aligned, may be NULL) for the
+ * backward. fp32 math.
+ * A row whose label is ignore_index is not read and gets 0 everywhere; a label
+ * outside [0, vocab) sets RK_DEV_CE_LABEL and the row is treated as ignored.
+ * The backward writes, rounded once,
+ *   dlogits = ((d_logprob (1[j = label] - p_j)
+ *               - d_entropy p_j (ln p_j + entropy)) * inv_temp) * (*scale_dev)
+ * with p = exp(z - m - ln S), zero rows for ignored labels; d_entropy (with
+ * entropy, both or neither) and scale_dev (a device fp32 scalar) may be NULL.
+ * coef_stride is the element stride of d_logprob and d_entropy (1 for plain
+ * arrays, 2 for the interleaved coef of rk_policy_loss). dlogits may alias
+ * logits (same leading dimension). */
+RK_API int rk_token_logprob_fwd(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
+                                float inv_temp, int ignore_index, int dtype, float* logprob, float* entropy,
+                                float* stats, void* stream);
+RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
+                                float inv_temp, int ignore_index, int dtype, const float* stats, const float* entropy,
+                                const float* d_logprob, const float* d_entropy, int64_t coef_stride,
+                                const float* scale_dev, void* dlogits, int64_t ldd, void* stream);
+
+/* ------------------------------------------------ Clipped policy loss
+ * Per row with an action a in [0, vocab) (others as above), lp its
+ * log-probability and H its entropy:
+ *   ratio = exp(lp - old_logprobs[r]),  A = advantages[r / adv_group]
+ *   kl    = exp(d) - 1 - d with d = ref_logprobs[r] - lp   (0 without ref)
+ *   l     = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
+ *           + kl_coef kl - entropy_coef H
+ *   loss  = sum_r w_r l_r / D, w = weights (1 without), D = *denominator or the
+ *           sum of w over the rows with an action (loss 0 when that is 0)
+ * logprob and kl [rows] (kl may be NULL), entropy [rows] (required when
+ * entropy_coef != 0, else may be NULL), metrics fp32[4] = (loss, D, weighted
+ * share of rows where the clamped branch is taken, 0).
+ * With dlogits the gradient of grad_scale * (*grad_scale_dev) * loss is written
+ * in the same pass over the logits (they are read once while a row fits the
+ * shared memory of its CTAs; dlogits may alias logits with the same leading
+ * dimension). Without it, stats [rows] float2 and coef [rows] float2 =
+ * (dloss/dlp, dloss/dH), where given, are what rk_token_logprob_bwd needs.
+ * workspace: rk_policy_workspace(rows) bytes, 16-byte aligned. */
+typedef struct rk_policy_terms {
+  const float* old_logprobs;   /* [rows] */
+  const float* advantages;     /* [ceil(rows / adv_group)] */
+  const float* ref_logprobs;   /* [rows] or NULL */
+  const float* weights;        /* [rows] or NULL */
+  const float* denominator;    /* device scalar or NULL */
+  const float* grad_scale_dev; /* device scalar or NULL */
+  int64_t adv_group;
+  float clip_low, clip_high, kl_coef, entropy_coef, inv_temp, grad_scale;
+} rk_policy_terms;
+RK_API int64_t rk_policy_workspace(int64_t rows);
+RK_API int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* actions, int64_t rows,
+                          int ignore_index, int dtype, const rk_policy_terms* terms, float* logprob, float* kl,
+                          float* entropy, float* metrics, float* stats, float* coef, void* dlogits, int64_t ldd,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------ Paired preference loss
+ * logits [2 * pairs * length, ld]: the chosen sequences of all pairs, then the
+ * rejected ones; labels likewise (ignore_index on prompt and padding). Per
+ * sequence gap_s = sum_t (lp_t - ref_logprobs_t) over its labelled tokens (their
+ * mean with average != 0; 0 without any), rewards[s] = beta gap_s and, per pair,
+ * u = beta (gap_chosen - gap_rejected):
+ *   RK_PREF_SIGMOID  -(1 - smoothing) ln sigma(u) - smoothing ln sigma(-u)
+ *   RK_PREF_HINGE    max(0, 1 - u)
+ *   RK_PREF_SQUARED  (gap_chosen - gap_rejected - 1 / (2 beta))^2
+ * loss = the mean over pairs. logprob [rows], stats [rows] float2, coef [rows] =
+ * dloss/dlp. With dlogits, grad_scale * dloss/dlogits is written as well;
+ * without, stats and coef are what rk_token_logprob_bwd needs. workspace:
+ * rk_preference_workspace(pairs, length) bytes, 16-byte aligned. */
+enum { RK_PREF_SIGMOID = 0, RK_PREF_HINGE = 1, RK_PREF_SQUARED = 2 };
+typedef struct rk_preference_terms {
+  const float* ref_logprobs;   /* [2 * pairs * length] or NULL (0) */
+  const float* grad_scale_dev; /* device scalar or NULL */
+  float beta, smoothing, inv_temp, grad_scale;
+  int kind, average;
+} rk_preference_terms;
+RK_API int64_t rk_preference_workspace(int64_t pairs, int64_t length);
+RK_API int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t pairs,
+                              int64_t length, int ignore_index, int dtype, const rk_preference_terms* terms,
+                              float* logprob, float* rewards, float* loss, float* stats, float* coef, void* dlogits,
+                              int64_t ldd, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------ AdamW over many tensors
+ * The update of rk_adamw_step for a list of separate tensors (parameters of a
+ * module and their gradients where autograd left them), with moments in 32 or
+ * 8 bits. `tensors` is a host array, read during the call.
+ * 8-bit moments: blocks of 256 consecutive elements of a tensor share a scale,
+ *   exp_avg    int8  c: m = c |c| / 127^2 * exp_avg_scale     (scale = max |m|)
+ *   exp_avg_sq uint8 c: v = (c^2 / 255^2 * exp_avg_sq_scale)^2 (scale = max sqrt v)
+ * rounded to the nearest code in c, except that v > 0 never gets c = 0. The
+ * update itself uses the moments before they are rounded to codes.
+ * scalars: device fp32[8] as for rk_adamw_step ([0] lr, [1] step count,
+ * [2] gradient norm, [3] clip coefficient, [4..6] constants of the step):
+ * rk_adamw_multi_prepare reads the norm partials that rk_adamw_multi_sumsq left
+ * (parts = 0: no clipping, coefficient 1), counts the step in scalars[1] and
+ * derives the constants; rk_adamw_multi_step then updates every tensor.
+ * rk_adamw_multi_sumsq writes rk_adamw_multi_parts(n) partial sums of
+ * squares for its n tensors (fixed order, so norms are reproducible); the
+ * partials of several calls may be laid end to end for one prepare.
+ * dtypes: p and g each RK_F32, RK_BF16 or RK_F16; p, g and the moments 16-byte
+ * aligned (8-bit codes 8-byte), numel >= 0, contiguous. */
+typedef struct rk_adamw_tensor {
+  void* p;
+  const void* g;
+  void* exp_avg;           /* fp32, or int8 codes */
+  void* exp_avg_sq;        /* fp32, or uint8 codes */
+  float* exp_avg_scale;    /* [ceil(numel / 256)], 8-bit moments only */
+  float* exp_avg_sq_scale;
+  int64_t numel;
+} rk_adamw_tensor;
+RK_API int64_t rk_adamw_multi_parts(int64_t n);
+RK_API int rk_adamw_multi_sumsq(const rk_adamw_tensor* tensors, int64_t n, int g_dtype, float* partials, void* stream);
+RK_API int rk_adamw_multi_prepare(const float* partials, int64_t parts, float max_norm, float beta1, float beta2,
+                                  float weight_decay, float* scalars, void* stream);
+RK_API int rk_adamw_multi_step(const rk_adamw_tensor* tensors, int64_t n, int p_dtype, int g_dtype, int state_bits,
+                               const float* scalars, float beta1, float beta2, float eps, void* stream);
+/* The values 8-bit moments stand for: p (exp_avg) and g (exp_avg_sq) of each
+ * tensor are the destinations here, in out_dtype; the codes and scales are read. */
+RK_API int rk_adamw_multi_moments(const rk_adamw_tensor* tensors, int64_t n, int out_dtype, void* stream);
+
 /* ------------------------------------------------ Softmax head (fused CE)
  * The vocabulary head and its cross-entropy with no pass of their own over the
  * logits; together they replace the head Linear, F.cross_entropy(...,

@@ -77,6 +77,18 @@ SIGNATURES: dict[str, tuple] = {
     "rk_rmsnorm_bwd_fused": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _i, _f, _p, _p, _i, _p, _i64, _i64, _i64, _p]),
     "rk_rmsnorm_dw_reduce": (_i, [_p, _i64, _i64, _p, _i, _p]),
     "rk_cross_entropy_fwd_bwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _p, _p, _p, _i64, _i, _i, _p]),
+    "rk_token_logprob_fwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _i, _i, _p, _p, _p, _p]),
+    "rk_token_logprob_bwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _i, _i, _p, _p, _p, _p, _i64, _p, _p, _i64, _p]),
+    "rk_policy_workspace": (_i64, [_i64]),
+    "rk_policy_loss": (_i, [_p, _i64, _i64, _p, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p]),
+    "rk_preference_workspace": (_i64, [_i64, _i64]),
+    "rk_preference_loss": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64,
+                                _p]),
+    "rk_adamw_multi_parts": (_i64, [_i64]),
+    "rk_adamw_multi_sumsq": (_i, [_p, _i64, _i, _p, _p]),
+    "rk_adamw_multi_prepare": (_i, [_p, _i64, _f, _f, _f, _f, _p, _p]),
+    "rk_adamw_multi_step": (_i, [_p, _i64, _i, _i, _i, _p, _f, _f, _f, _p]),
+    "rk_adamw_multi_moments": (_i, [_p, _i64, _i, _p]),
     "rk_head_stats_width": (_i64, [_i64]),
     "rk_head_fprop": (_i, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i, _p]),
     "rk_head_loss": (_i, [_p, _i64, _p, _p, _i64, _i64, _f, _p, _p, _p, _p, _i64, _i, _p]),
@@ -107,7 +119,21 @@ class LayerGrads(ctypes.Structure):
     _fields_ = [("attn_norm", _p), ("qkv", _p), ("proj", _p), ("mlp_norm", _p), ("up", _p), ("down", _p)]
 
 
+class PolicyTerms(ctypes.Structure):
+    """rk_policy_terms of include/revk.h."""
+    _fields_ = [("old_logprobs", _p), ("advantages", _p), ("ref_logprobs", _p), ("weights", _p),
+                ("denominator", _p), ("grad_scale_dev", _p), ("adv_group", _i64), ("clip_low", _f),
+                ("clip_high", _f), ("kl_coef", _f), ("entropy_coef", _f), ("inv_temp", _f), ("grad_scale", _f)]
+
+
+class PreferenceTerms(ctypes.Structure):
+    """rk_preference_terms of include/revk.h."""
+    _fields_ = [("ref_logprobs", _p), ("grad_scale_dev", _p), ("beta", _f), ("smoothing", _f), ("inv_temp", _f),
+                ("grad_scale", _f), ("kind", _i), ("average", _i)]
+
+
 METHOD_MIDPOINT, METHOD_EULER = 0, 1
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
 def header_symbols() -> list[str]:

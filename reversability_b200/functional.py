@@ -593,3 +593,165 @@ def dgrad_swiglu_fusable(dy: torch.Tensor, w_down: torch.Tensor, u: torch.Tensor
 def swiglu_fusable(x: torch.Tensor, w_up: torch.Tensor) -> bool:
     return x.dtype in _TC_DTYPES and w_up.dtype == x.dtype and (w_up.shape[0] // 2) % 128 == 0 and \
         x.is_contiguous() and w_up.is_contiguous() and (x.shape[1] * 2) % 16 == 0
+
+
+# ------------------------------------------------------------------ token log-probabilities and their losses
+def token_rows(logits: torch.Tensor, labels: torch.Tensor, name: str = "labels") -> tuple[int, int, int, torch.Tensor]:
+    """Checks logits [..., V] against labels [...] and returns (rows, V, row stride, contiguous labels). The rows
+    must be evenly strided (any stride of at least V, no alignment rule) and the last dimension unit-stride."""
+    require_cuda(logits, labels)
+    if logits.dtype not in _lib.DTYPE_CODE:
+        raise ValueError(f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
+    if labels.dtype != torch.int64 or labels.device != logits.device or logits.dim() < 1 or \
+            labels.shape != logits.shape[:-1]:
+        raise ValueError(f"{name} must be int64 on the logits' device with shape {tuple(logits.shape[:-1])}")
+    V = logits.shape[-1]
+    if V < 1 or (V > 1 and logits.stride(-1) != 1):
+        raise ValueError("logits must have a non-empty, unit-stride last dimension")
+    rows, ld = 1, None
+    for size, stride in zip(reversed(logits.shape[:-1]), reversed(logits.stride()[:-1])):
+        if size != 1:
+            if ld is None:
+                ld = stride
+            elif stride != ld * rows and logits.numel():
+                raise ValueError("logits rows must be evenly strided (pass a contiguous tensor)")
+            rows *= size
+    if ld is None or rows <= 1:
+        ld = V
+    if ld < V and rows:
+        raise ValueError("logits rows overlap")
+    return rows, V, max(ld, V), labels.contiguous()
+
+
+def like_rows(logits: torch.Tensor, rows: int, ld: int) -> torch.Tensor:
+    """An uninitialised tensor of logits' shape and row stride (so both sides share their 16-byte phase)."""
+    V = logits.shape[-1]
+    if ld == V:
+        return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    return torch.empty((rows, ld), device=logits.device, dtype=logits.dtype)[:, :V].view(logits.shape)
+
+
+def row_values(t: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor | None:
+    """An fp32 contiguous array of one value a row (None passes)."""
+    if t is None:
+        return None
+    if t.device != like.device or t.shape != like.shape:
+        raise ValueError(f"{name} must be on the logits' device with shape {tuple(like.shape)}")
+    return t.detach().float().contiguous()
+
+
+def device_scalar(t, device, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.device != device or t.numel() != 1:
+        raise ValueError(f"{name} must be a scalar tensor on the logits' device")
+    return t.detach().float()
+
+
+def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0, ignore_index: int = -100,
+                      entropy: bool = False, want_stats: bool = True):
+    """(logprob, entropy or None, stats or None) of logits [..., V] at labels [...], fp32 in the shape of labels;
+    0 at ignore_index. stats [rows, 2] = (max, ln sum exp) of a row's scaled logits, for token_logprob_bwd."""
+    rows, V, ld, labels = token_rows(logits, labels)
+    logprob = torch.empty(labels.shape, device=logits.device, dtype=torch.float32)
+    h = torch.empty_like(logprob) if entropy else None
+    stats = torch.empty((rows, 2), device=logits.device, dtype=torch.float32) if want_stats else None
+    _lib.call("rk_token_logprob_fwd", logits.data_ptr(), ld, V, labels.data_ptr(), rows, 1.0 / temperature,
+              int(ignore_index), _lib.code(logits.dtype), logprob.data_ptr(), _lib.ptr(h), _lib.ptr(stats),
+              _lib.stream_ptr())
+    return logprob, h, stats
+
+
+def token_logprob_bwd(logits: torch.Tensor, labels: torch.Tensor, stats: torch.Tensor, d_logprob: torch.Tensor,
+                      entropy: torch.Tensor | None = None, d_entropy: torch.Tensor | None = None,
+                      temperature: float = 1.0, ignore_index: int = -100, coef_stride: int = 1,
+                      scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """d loss / d logits (in the logits' dtype, rounded once) from d loss / d logprob and, with `entropy`, d loss /
+    d entropy, times the device scalar `scale`. `out` may be the logits themselves."""
+    rows, V, ld, labels = token_rows(logits, labels)
+    out, ldd = gradient_rows(logits, out, rows, ld)
+    _lib.call("rk_token_logprob_bwd", logits.data_ptr(), ld, V, labels.data_ptr(), rows, 1.0 / temperature,
+              int(ignore_index), _lib.code(logits.dtype), stats.data_ptr(), _lib.ptr(entropy), d_logprob.data_ptr(),
+              _lib.ptr(d_entropy), coef_stride, _lib.ptr(scale), out.data_ptr(), ldd, _lib.stream_ptr())
+    return out
+
+
+def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld: int) -> tuple[torch.Tensor, int]:
+    """(gradient tensor, its row stride): a new one laid out like the logits, or a checked `out`."""
+    if out is None:
+        return like_rows(logits, rows, ld), ld
+    if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
+        raise ValueError("out must match the logits' shape, dtype and device")
+    if out.shape[-1] > 1 and out.stride(-1) != 1:
+        raise ValueError("out must have a unit-stride last dimension")
+    if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
+        raise ValueError("out may alias the logits only with the same strides")
+    return out, token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
+
+
+def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                ref_logprobs: torch.Tensor | None = None, weights: torch.Tensor | None = None,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                temperature: float = 1.0, ignore_index: int = -100, entropy: bool = False,
+                denominator: torch.Tensor | None = None, grad_scale: float = 1.0,
+                grad_scale_dev: torch.Tensor | None = None, want_grad: bool = True, want_coef: bool = False,
+                out: torch.Tensor | None = None):
+    """rk_policy_loss: (metrics [4], logprob, kl or None, entropy or None, dlogits or None, stats or None, coef or
+    None). advantages has the shape of actions or of its leading dimensions (one a sequence)."""
+    rows, V, ld, actions = token_rows(logits, actions, "actions")
+    dev = logits.device
+    old = row_values(old_logprobs, actions, "old_logprobs")
+    ref = row_values(ref_logprobs, actions, "ref_logprobs")
+    w = row_values(weights, actions, "weights")
+    lead = advantages.dim()
+    if advantages.device != dev or lead > actions.dim() or advantages.shape != actions.shape[:lead]:
+        raise ValueError("advantages must be on the logits' device with the shape of actions or of its leading "
+                         "dimensions")
+    group = max(1, actions.shape[lead:].numel())
+    adv = advantages.detach().float().contiguous()
+    denominator = device_scalar(denominator, dev, "denominator")
+    grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
+    n_ws = _lib.lib().rk_policy_workspace(rows) // 4
+    # one allocation for all, the pairs first (they are 8-byte aligned)
+    per_row = [2 * want_coef, 2 * want_coef, 1, int(ref is not None), int(entropy or entropy_coef != 0)]
+    buf = torch.empty(n_ws + 4 + rows * sum(per_row), device=dev, dtype=torch.float32)
+    ws, metrics, *parts = buf.split([n_ws, 4, *(rows * n for n in per_row)])
+    stats, coef, logprob, kl, h = (p if n else None for p, n in zip(parts, per_row))
+    dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
+    terms = _lib.PolicyTerms(old.data_ptr(), adv.data_ptr(), _lib.ptr(ref), _lib.ptr(w), _lib.ptr(denominator),
+                             _lib.ptr(grad_scale_dev), group, clip_low, clip_high, kl_coef, entropy_coef,
+                             1.0 / temperature, grad_scale)
+    _lib.call("rk_policy_loss", logits.data_ptr(), ld, V, actions.data_ptr(), rows, int(ignore_index),
+              _lib.code(logits.dtype), _lib.ctypes.byref(terms), logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h),
+              metrics.data_ptr(), _lib.ptr(stats), _lib.ptr(coef), _lib.ptr(dlogits), ldd, ws.data_ptr(), n_ws * 4,
+              _lib.stream_ptr())
+    shaped = (t if t is None else t.view(actions.shape) for t in (logprob, kl, h))
+    return metrics, *shaped, dlogits, stats, coef
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, kind: str,
+                    beta: float, label_smoothing: float = 0.0, average: bool = False, temperature: float = 1.0,
+                    ignore_index: int = -100, grad_scale: float = 1.0, grad_scale_dev: torch.Tensor | None = None,
+                    want_grad: bool = True, out: torch.Tensor | None = None):
+    """rk_preference_loss: (loss [1], logprob, rewards [2 * pairs], dlogits or None, stats, coef) for logits
+    [2 * pairs, length, V], chosen sequences first."""
+    if logits.dim() != 3 or logits.shape[0] % 2 or logits.shape[0] == 0:
+        raise ValueError("preference logits must be [2 * pairs, length, vocabulary], chosen sequences first")
+    if kind not in _lib.PREFERENCE_KINDS:
+        raise ValueError(f"kind must be one of {sorted(_lib.PREFERENCE_KINDS)}")
+    rows, V, ld, labels = token_rows(logits, labels)
+    dev = logits.device
+    seqs, length = labels.shape
+    ref = row_values(ref_logprobs, labels, "ref_logprobs")
+    grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
+    n_ws = -(-_lib.lib().rk_preference_workspace(seqs // 2, length) // 16) * 4
+    buf = torch.empty(n_ws + 4 + 4 * rows + seqs, device=dev, dtype=torch.float32)  # one allocation for all
+    ws, loss, stats, logprob, coef, rewards = buf.split([n_ws, 4, 2 * rows, rows, rows, seqs])
+    dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
+    terms = _lib.PreferenceTerms(_lib.ptr(ref), _lib.ptr(grad_scale_dev), beta, label_smoothing, 1.0 / temperature,
+                                 grad_scale, _lib.PREFERENCE_KINDS[kind], int(average))
+    _lib.call("rk_preference_loss", logits.data_ptr(), ld, V, labels.data_ptr(), seqs // 2, length, int(ignore_index),
+              _lib.code(logits.dtype), _lib.ctypes.byref(terms), logprob.data_ptr(), rewards.data_ptr(),
+              loss.data_ptr(), stats.data_ptr(), coef.data_ptr(), _lib.ptr(dlogits), ldd, ws.data_ptr(), n_ws * 4,
+              _lib.stream_ptr())
+    return loss, logprob.view(labels.shape), rewards, dlogits, stats, coef

@@ -1,0 +1,487 @@
+"""Token log-probabilities, clipped policy loss and paired preference loss
+(alignment.py) against their definitions in 64 bits, on the same inputs.
+
+Tolerances, derived from the arithmetic: a log-probability is
+(z - m) - ln S with z, m rounded to fp32 (relative 2^-24 each, so absolute
+2^-22 max|z|) and ln S within 2e-6 (exponentials within 2^-22 relative, a
+blocked fp32 sum). A probability then carries a relative error of 2e-5 as long
+as |ln p| < 60, and smaller ones round to nothing. A gradient is rounded once:
+half an ulp of its type on top of that."""
+import math
+
+import pytest
+import torch
+
+from reversability_b200 import _lib, alignment, functional as fn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+HALF_ULP = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SMALLEST = {torch.float32: 1e-36, torch.bfloat16: 1e-36, torch.float16: 6e-8}
+# (rows, vocabulary): single elements, warp and vector edges, the decoder's vocabulary, a large odd one
+SHAPES = [(1, 1), (3, 2), (5, 7), (64, 31), (70, 101), (9, 255), (300, 1000), (33, 4097), (17, 8209), (6, 50257), (3, 131075)]
+
+
+def _logits(rows, vocab, dtype, layout="plain", seed=0, scale=2.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    if layout == "plain":
+        x = torch.empty(rows, vocab, device=DEV, dtype=dtype)
+    elif layout == "padded":  # rows start on 128 bytes
+        x = torch.empty(rows, (vocab + 63) // 64 * 64, device=DEV, dtype=dtype)[:, :vocab]
+    else:  # "shifted": an odd row stride and a base that is no multiple of 16 bytes
+        width = vocab + 3 + vocab % 2
+        x = torch.empty(rows * width + 1, device=DEV, dtype=dtype)[1:].view(rows, width)[:, 1:1 + vocab]
+    x.copy_(torch.randn(rows, vocab, generator=g, device=DEV) * scale)
+    return x
+
+
+def _labels(rows, vocab, seed=0, ignored=0.3):
+    g = torch.Generator(device=DEV).manual_seed(100 + seed)
+    y = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    drop = torch.rand(rows, generator=g, device=DEV) < ignored
+    drop[0] = False
+    y[drop] = -100
+    return y
+
+
+def _rows64(x, y, temperature=1.0):
+    """fp64 (logp of all columns, lp at the label, entropy, valid) by torch's own log_softmax."""
+    logp = torch.log_softmax(x.double() / temperature, -1)
+    valid = y >= 0
+    lp = logp.gather(-1, y.clamp(min=0)[..., None])[..., 0] * valid
+    p = logp.exp()
+    h = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(-1) * valid
+    return logp, lp, h, valid
+
+
+def _lp_tol(x, temperature=1.0):
+    live = x.double().abs()
+    live = torch.where(live > 1e3, torch.zeros_like(live), live)  # masked columns do not count
+    return 2e-6 + 2.0 ** -22 * float(live.max()) / temperature
+
+
+def _check_grad(d, x, y, temperature, g_lp, g_h=None):
+    """d against g_lp ([j = y] - p) - g_h p (ln p + H), over the temperature, in 64 bits."""
+    logp, _, h, valid = _rows64(x, y, temperature)
+    p = logp.exp()
+    g = (torch.as_tensor(g_lp, device=DEV).double() * valid)[:, None]
+    want = -g * p
+    want.scatter_add_(1, y.clamp(min=0)[:, None], g)
+    size = g.abs() * p
+    size.scatter_add_(1, y.clamp(min=0)[:, None], g.abs() * p.gather(1, y.clamp(min=0)[:, None]))
+    if g_h is not None:
+        gh = (torch.as_tensor(g_h, device=DEV).double() * valid)[:, None]
+        want = want - gh * torch.where(p > 0, p * (logp + h[:, None]), torch.zeros_like(p))
+        size = size + gh.abs() * torch.where(p > 0, p * (logp.abs() + h[:, None] + 1), torch.zeros_like(p))
+    want, size = want / temperature, size / temperature
+    # the label's entry is g (1 - p): its error is that of p and fp32's own rounding of g
+    tol = HALF_ULP[d.dtype] * want.abs() + 2e-5 * size + 2.0 ** -22 * want.abs() + SMALLEST[d.dtype]
+    over = ((d.double() - want).abs() - tol).max()
+    assert float(over) <= 0, f"gradient off by {float(over):.3e} more than its tolerance"
+    assert not d[~valid].any(), "ignored rows must have zero gradients"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["plain", "padded", "shifted"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_token_logprobs_forward_and_backward(shape, layout, dtype):
+    rows, vocab = shape
+    for temperature in (1.0, 0.7):
+        x = _logits(rows, vocab, dtype, layout, seed=rows).requires_grad_()
+        y = _labels(rows, vocab)
+        _, lp64, h64, _ = _rows64(x.detach(), y, temperature)
+        lp, h = alignment.token_logprobs(x, y, temperature=temperature, entropy=True)
+        assert lp.dtype == h.dtype == torch.float32 and lp.requires_grad and h.requires_grad
+        tol = _lp_tol(x.detach(), temperature)
+        assert float((lp.detach().double() - lp64).abs().max()) <= tol
+        # the entropy is a mean of log-probabilities
+        assert float((h.detach().double() - h64).abs().max()) <= tol + 1e-5 * float(h64.max().clamp(min=1e-3))
+        g = torch.Generator(device=DEV).manual_seed(7)
+        a = torch.randn(rows, generator=g, device=DEV)
+        b = torch.randn(rows, generator=g, device=DEV)
+        d, = torch.autograd.grad([lp, h], x, [a, b], retain_graph=True)
+        _check_grad(d, x.detach(), y, temperature, a, b)
+        d, = torch.autograd.grad(lp, x, a)
+        _check_grad(d, x.detach(), y, temperature, a)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [5, 130, 3000, 50257])
+def test_masked_columns_infinities_and_nan(vocab, dtype):
+    """Columns at -inf or at the type's lowest value have probability 0 and no gradient; a NaN stays in its row, and
+    in an ignored row it is not read; +inf gives NaN as log_softmax does; large logits lose nothing to their size."""
+    rows = 8
+    x = _logits(rows, vocab, dtype, seed=3)
+    y = torch.randint(0, vocab // 2, (rows,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    half = vocab // 2 + 1
+    x[0, half:] = -math.inf
+    x[1, half:] = torch.finfo(dtype).min
+    x[2, vocab - 1] = math.nan
+    x[3] = math.nan
+    y[3] = -100
+    x[4, 0] = math.inf
+    x[5] = torch.finfo(dtype).min  # a row with nothing but masks of the lowest value: uniform
+    x[6] = -math.inf               # a row with nothing at all: NaN, as log_softmax gives
+    if dtype != torch.float16:
+        x[7] += 4096.0
+    x.requires_grad_()
+    lp, h = alignment.token_logprobs(x, y, entropy=True)
+    d, = torch.autograd.grad([lp, h], x, [torch.ones_like(lp), torch.full_like(h, 0.5)])
+    ok = torch.tensor([0, 1, 3, 5, 7], device=DEV)
+    _, lp64, h64, _ = _rows64(x.detach()[ok], y[ok])
+    lp64[2] = h64[2] = 0.0  # the ignored row
+    assert float((lp.detach()[ok].double() - lp64).abs().max()) <= 2e-6 + 2.0 ** -22 * (4200 if dtype != torch.float16 else 20)
+    assert float((h.detach()[ok].double() - h64).abs().max()) <= 2e-4
+    for r in (2, 4, 6):
+        assert math.isnan(float(lp.detach()[r])) and bool(d[r].isnan().any())
+    assert not d[3].any() and not d[0, half:].any() and not d[1, half:].any()
+    assert bool(d[ok].isfinite().all())
+    live = torch.tensor([0, 1, 5], device=DEV)
+    _check_grad(d[live], x.detach()[live], y[live], 1.0, torch.ones(3, device=DEV), torch.full((3,), 0.5, device=DEV))
+
+
+def test_label_out_of_range_sets_the_status_bit_and_is_ignored():
+    x = _logits(4, 33, torch.float32).requires_grad_()
+    y = torch.tensor([3, 33, -5, 0], device=DEV)
+    lp = alignment.token_logprobs(x, y)
+    assert _lib.device_status() == 1 << 2
+    d, = torch.autograd.grad(lp.sum(), x)
+    assert not d[1].any() and not d[2].any() and bool(d[0].any())
+    assert float(lp[1].detach()) == float(lp[2].detach()) == 0.0
+    old = torch.zeros(4, device=DEV)
+    alignment.policy_loss_and_grad(x, y, old, torch.ones(4, device=DEV))
+    assert _lib.device_status() == 1 << 2
+    _lib.device_status()
+
+
+def test_all_rows_ignored_and_no_rows():
+    x = _logits(6, 77, torch.bfloat16)
+    y = torch.full((6,), -100, device=DEV)
+    z = torch.zeros(6, device=DEV)
+    r, d = alignment.policy_loss_and_grad(x, y, z, z + 1, ref_logprobs=z, kl_coef=0.1, entropy_coef=0.1)
+    assert float(r.loss) == 0.0 and float(r.clip_fraction) == 0.0
+    assert not d.any() and not r.logprobs.any() and not r.kl.any() and not r.entropy.any()
+    e = torch.zeros(0, device=DEV)
+    none = torch.zeros(0, dtype=torch.int64, device=DEV)
+    r, d = alignment.policy_loss_and_grad(x[:0], none, e, e)
+    assert float(r.loss) == 0.0 and d.shape == (0, 77)
+    assert alignment.token_logprobs(x[:0], none).shape == (0,)
+    r, d = alignment.preference_loss_and_grad(torch.zeros(2, 0, 9, device=DEV), torch.zeros(2, 0, dtype=torch.int64, device=DEV), None)
+    assert abs(float(r.loss) - math.log(2)) < 1e-6 and d.shape == (2, 0, 9)
+    # pairs without a labelled token: gap 0, no gradient
+    y = torch.full((2, 3), -100, device=DEV)
+    r, d = alignment.preference_loss_and_grad(x.view(2, 3, 77), y, None, average=True)
+    assert abs(float(r.loss) - math.log(2)) < 1e-6 and not d.any() and not r.rewards.any()
+
+
+# ---------------------------------------------------------------- policy loss
+def _policy64(x, y, old, adv, ref, w, lo, hi, ckl, cent, temperature, denom, gscale):
+    z = x.double().requires_grad_()
+    logp = torch.log_softmax(z / temperature, -1)
+    valid = y >= 0
+    lp = logp.gather(1, y.clamp(min=0)[:, None])[:, 0]
+    p = logp.exp()
+    h = -(torch.where(p > 0, p * logp, torch.zeros_like(p))).sum(1)
+    ratio = (lp - old.double()).exp()
+    free, held = ratio * adv.double(), ratio.clamp(1 - lo, 1 + hi) * adv.double()
+    clipped = held < free
+    each = -torch.where(clipped, held, free) - cent * h
+    kl = torch.zeros_like(lp)
+    if ref is not None:
+        kl = (ref.double() - lp).exp() - 1 - (ref.double() - lp)
+        each = each + ckl * kl
+    ww = (torch.ones_like(lp) if w is None else w.double()) * valid
+    total = ww.sum() if denom is None else denom.double()
+    loss = (torch.where(valid, each, torch.zeros_like(each)) * ww).sum() / total
+    lp.retain_grad()
+    d, g_lp = torch.autograd.grad(loss * gscale, [z, lp])
+    return loss.detach(), lp.detach() * valid, kl.detach() * valid, h.detach() * valid, (clipped * ww).sum() / total, d, g_lp
+
+
+def _policy_inputs(rows, vocab, dtype, layout, seed=0):
+    x = _logits(rows, vocab, dtype, layout, seed)
+    y = _labels(rows, vocab, seed)
+    g = torch.Generator(device=DEV).manual_seed(seed + 9)
+    lp = _rows64(x, y)[1].float()
+    step = torch.linspace(-0.65, 0.65, rows, device=DEV)  # log ratios on both sides of both clip edges, none on one
+    old = lp - step
+    ref = lp + 0.3 * torch.randn(rows, generator=g, device=DEV)
+    adv = torch.randn(rows, generator=g, device=DEV)
+    adv[rows // 2] = 0.0
+    w = torch.rand(rows, generator=g, device=DEV) + 0.5
+    return x, y, old, adv, ref, w
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["plain", "padded", "shifted"])
+@pytest.mark.parametrize("shape", [(2, 3), (70, 101), (300, 1000), (33, 4097), (14, 50257), (3, 131075)])
+def test_policy_loss_both_forms(shape, layout, dtype):
+    rows, vocab = shape
+    x, y, old, adv, ref, w = _policy_inputs(rows, vocab, dtype, layout)
+    gscale = 1024.0 if dtype == torch.float16 else 1.0
+    for bonus, ckl, weights, temperature, given in ((0.0, 0.0, None, 1.0, False), (0.02, 0.1, w, 1.0, True),
+                                                    (0.0, 0.1, None, 1.3, False)):
+        denom = torch.full((), 3.0, device=DEV) if given else None
+        want = _policy64(x, y, old, adv, ref, weights, 0.2, 0.28, ckl, bonus, temperature, denom, gscale)
+        kw = dict(ref_logprobs=ref, weights=weights, clip_low=0.2, clip_high=0.28, kl_coef=ckl, entropy_coef=bonus,
+                  temperature=temperature, denominator=denom)
+        r, d = alignment.policy_loss_and_grad(x, y, old, adv, grad_scale=gscale, **kw)
+        xg = x.detach().requires_grad_()
+        r2 = alignment.policy_loss(xg, y, old, adv, **kw)
+        d2, = torch.autograd.grad(r2.loss * gscale, xg)
+        tol = _lp_tol(x, temperature)
+        size = float(adv.abs().max()) * 2 + 1
+        for got in (r, r2):
+            # a token's loss moves by about (|A| r + c) times the log-probability's error
+            assert abs(float(got.loss.detach()) - float(want[0])) <= 2 * size * tol * (rows / 3 if given else 1) + 1e-6
+            assert float((got.logprobs.double() - want[1]).abs().max()) <= tol
+            assert float((got.kl.double() - want[2]).abs().max()) <= 4 * tol
+            assert abs(float(got.clip_fraction) - float(want[4])) <= 1e-6 * (rows if given else 1)
+            if bonus:
+                assert float((got.entropy.double() - want[3]).abs().max()) <= tol + 1e-5 * float(want[3].max())
+            else:
+                assert got.entropy is None
+        ww = (y >= 0) if weights is None else w * (y >= 0)
+        total = float(ww.double().sum()) if denom is None else 3.0
+        g_h = -bonus * ww.double() * gscale / total if bonus else None
+        for got in (d, d2):
+            # the factor of a row (w/D)(A r + ...) is within 1e-5 of itself, beside the gradient's own tolerance
+            logp = _rows64(x, y, temperature)[0]
+            p = logp.exp()
+            err = (got.double() - want[5]).abs()
+            g = want[6].abs()[:, None]
+            hot = torch.zeros_like(p).scatter_(1, y.clamp(min=0)[:, None], 1.0)
+            span = (g + (w.double() * gscale / total * (1 + adv.double().abs()))[:, None] * 2) * (p + hot)
+            if g_h is not None:
+                span = span + g_h.abs()[:, None] * torch.where(p > 0, p * (logp.abs() + 12), torch.zeros_like(p))
+            lim = HALF_ULP[dtype] * want[5].abs() + 4e-5 * span / temperature + SMALLEST[dtype]
+            assert float((err - lim).max()) <= 0
+            assert not got[y < 0].any()
+    assert _lib.device_status() == 0
+
+
+def test_policy_loss_per_sequence_advantages_and_shapes():
+    B, T, V = 3, 5, 211
+    x, y, old, adv, ref, w = _policy_inputs(B * T, V, torch.float32, "plain")
+    per_seq = torch.tensor([0.5, -1.5, 2.0], device=DEV)
+    a, da = alignment.policy_loss_and_grad(x.view(B, T, V), y.view(B, T), old.view(B, T), per_seq)
+    b, db = alignment.policy_loss_and_grad(x, y, old, per_seq.repeat_interleave(T))
+    assert a.logprobs.shape == (B, T) and da.shape == (B, T, V) and a.kl is None and a.entropy is None
+    assert torch.equal(a.loss, b.loss) and torch.equal(da.view_as(db), db)
+    r = alignment.policy_loss(x.view(B, T, V), y.view(B, T), old.view(B, T), per_seq, entropy=True)
+    assert torch.equal(r.logprobs, a.logprobs) and r.entropy.shape == (B, T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9, 1000, 50257])
+def test_gradients_over_the_logits_in_place(vocab, dtype):
+    """out=logits: the same bits as a separate gradient, whatever the row alignment."""
+    rows = 37
+    for layout in ("plain", "padded", "shifted"):
+        x, y, old, adv, ref, w = _policy_inputs(rows, vocab, dtype, layout)
+        _, d = alignment.policy_loss_and_grad(x, y, old, adv, entropy_coef=0.01)
+        buf = _logits(rows, vocab, dtype, layout)
+        assert torch.equal(buf, x)
+        _, d2 = alignment.policy_loss_and_grad(buf, y, old, adv, entropy_coef=0.01, out=buf)
+        assert d2.data_ptr() == buf.data_ptr() and torch.equal(d, buf)
+        other = torch.full((rows, vocab + 5), 7.0, device=DEV, dtype=dtype)  # another stride than the logits'
+        alignment.policy_loss_and_grad(x, y, old, adv, entropy_coef=0.01, out=other[:, 3:3 + vocab])
+        assert torch.equal(other[:, 3:3 + vocab], d)
+        assert bool((other[:, :3] == 7.0).all()) and bool((other[:, 3 + vocab:] == 7.0).all())
+        pairs = x[:36].view(2, 18, vocab)
+        _, d = alignment.preference_loss_and_grad(pairs, y[:36].view(2, 18), None)
+        buf = _logits(rows, vocab, dtype, layout)
+        alignment.preference_loss_and_grad(buf[:36].view(2, 18, vocab), y[:36].view(2, 18), None,
+                                           out=buf[:36].view(2, 18, vocab))
+        assert torch.equal(buf[:36].view_as(d), d) and torch.equal(buf[36:], x[36:])
+
+
+def test_policy_gradient_agrees_with_differences():
+    """Central differences of the loss along a random sign vector, step e: the loss is fp32 (2^-23 |L| / e) and its
+    third derivative of order one (e^2 / 6)."""
+    rows, vocab, e = 24, 301, 5e-3
+    x, y, old, adv, ref, w = _policy_inputs(rows, vocab, torch.float32, "plain")
+    kw = dict(ref_logprobs=ref, kl_coef=0.1, entropy_coef=0.05, weights=w)
+    u = torch.randint(0, 2, x.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(5)).float() * 2 - 1
+    _, d = alignment.policy_loss_and_grad(x, y, old, adv, **kw)
+    up, down = (float(alignment.policy_loss_and_grad(x + s * e * u, y, old, adv, **kw)[0].loss) for s in (1, -1))
+    assert abs((up - down) / (2 * e) - float((d.double() * u).sum())) <= 3e-4
+
+
+# ---------------------------------------------------------------- preference loss
+def _preference64(x, y, ref, kind, beta, smoothing, average, temperature=1.0):
+    z = x.double().requires_grad_()
+    logp = torch.log_softmax(z / temperature, -1)
+    valid = y >= 0
+    lp = logp.gather(2, y.clamp(min=0)[..., None])[..., 0] * valid
+    gap = ((lp - (0 if ref is None else ref.double())) * valid).sum(1)
+    if average:
+        gap = gap / valid.sum(1).clamp(min=1)
+    n = x.shape[0] // 2
+    diff = gap[:n] - gap[n:]
+    u = beta * diff
+    if kind == "sigmoid":
+        ls = torch.nn.functional.logsigmoid
+        loss = -((1 - smoothing) * ls(u) + smoothing * ls(-u)).mean()
+    elif kind == "hinge":
+        loss = torch.relu(1 - u).mean()
+    else:
+        loss = (diff - 1 / (2 * beta)).square().mean()
+    d, g_lp = torch.autograd.grad(loss, [z, lp])
+    return loss.detach(), beta * gap.detach(), lp.detach(), d, g_lp * valid
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,beta,smoothing,average", [("sigmoid", 0.1, 0.0, False), ("sigmoid", 0.5, 0.2, True),
+                                                         ("hinge", 0.05, 0.0, False), ("squared", 0.1, 0.0, True),
+                                                         ("squared", 0.3, 0.0, False)])
+@pytest.mark.parametrize("shape", [(1, 1, 5), (3, 7, 101), (2, 33, 1000), (5, 130, 515), (1, 9, 50257)])
+def test_preference_loss_both_forms(shape, kind, beta, smoothing, average, dtype):
+    pairs, length, vocab = shape
+    rows = 2 * pairs * length
+    x = _logits(rows, vocab, dtype, "padded" if length % 2 else "plain").view(2 * pairs, length, vocab)
+    y = _labels(rows, vocab, ignored=0.4).view(2 * pairs, length)
+    if pairs > 2:
+        y[1] = -100  # a chosen sequence without a token
+    g = torch.Generator(device=DEV).manual_seed(4)
+    ref = _rows64(x, y)[1].float() + 0.3 * torch.randn(y.shape, generator=g, device=DEV)
+    ref = torch.where(y >= 0, ref, torch.full_like(ref, math.nan))  # not read where there is no label
+    clean = torch.nan_to_num(ref)
+    want = _preference64(x, y, clean, kind, beta, smoothing, average)
+    kw = dict(kind=kind, beta=beta, label_smoothing=smoothing, average=average)
+    r, d = alignment.preference_loss_and_grad(x, y, ref, **kw)
+    xg = x.detach().requires_grad_()
+    r2 = alignment.preference_loss(xg, y, ref, **kw)
+    d2, = torch.autograd.grad(r2.loss * 3.0, xg)
+    tol = _lp_tol(x)
+    # a gap sums at most `length` log-probabilities whose errors are independent or share a sign
+    gap_tol = (1 if average else length) * tol
+    slope = 2 * (float((want[1][:pairs] - want[1][pairs:]).abs().max()) / beta + 1 / (2 * beta)) if kind == "squared" else beta
+    for got, scale in ((r, 1.0), (r2, 1.0)):
+        assert float((got.logprobs.double() - want[2]).abs().max()) <= tol
+        assert float((got.rewards.double() - want[1]).abs().max()) <= beta * gap_tol + 1e-6
+        assert abs(float(got.loss.detach()) - float(want[0])) <= slope * 2 * gap_tol + 2.0 ** -22 * abs(float(want[0])) + 1e-7
+    for got, scale in ((d, 1.0), (d2, 3.0)):
+        # the row factors are those of 64 bits up to the slope's change over the gaps' error
+        p = _rows64(x, y)[0].exp()
+        hot = torch.zeros_like(p).scatter_(2, y.clamp(min=0)[..., None], 1.0)
+        per = want[4].abs()[..., None] * scale
+        bend = {"sigmoid": beta * beta / 4, "hinge": 0.0, "squared": 2.0}[kind] * 2 * gap_tol / pairs * scale
+        lim = HALF_ULP[dtype] * want[3].abs() * scale + (3e-5 * per + bend) * (p + hot) + SMALLEST[dtype]
+        assert float(((got.double() - want[3] * scale).abs() - lim).max()) <= 0
+        assert not got[y < 0].any()
+    assert _lib.device_status() == 0
+
+
+def test_preference_gradient_agrees_with_differences():
+    x = _logits(4 * 6, 53, torch.float32).view(4, 6, 53)
+    y = _labels(24, 53).view(4, 6)
+    u = torch.randint(0, 2, x.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(5)).float() * 2 - 1
+    for kind in ("sigmoid", "squared"):
+        _, d = alignment.preference_loss_and_grad(x, y, None, kind=kind, beta=0.5)
+        e = 5e-3
+        up, down = (float(alignment.preference_loss_and_grad(x + s * e * u, y, None, kind=kind, beta=0.5)[0].loss) for s in (1, -1))
+        slope = float((d.double() * u).sum())
+        # fp32 loss: 2^-23 L / e; the gaps are sums of a dozen terms of size up to 8 with third derivatives of order 10
+        assert abs((up - down) / (2 * e) - slope) <= 2.0 ** -22 * max(1.0, abs(up)) / e + 1e-3 * max(1.0, abs(slope))
+
+
+# ---------------------------------------------------------------- how they are called
+def test_other_stream_and_determinism():
+    x, y, old, adv, ref, w = _policy_inputs(300, 5000, torch.bfloat16, "plain")
+    a, da = alignment.policy_loss_and_grad(x, y, old, adv, ref_logprobs=ref, kl_coef=0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b, db = alignment.policy_loss_and_grad(x, y, old, adv, ref_logprobs=ref, kl_coef=0.1)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a.loss, b.loss) and torch.equal(da, db) and torch.equal(a.kl, b.kl)
+
+
+def test_captured_graph_replays_with_new_inputs():
+    x, y, old, adv, ref, w = _policy_inputs(40, 5000, torch.bfloat16, "plain")
+    alignment.policy_loss_and_grad(x, y, old, adv)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r, d = alignment.policy_loss_and_grad(x, y, old, adv)
+    x.copy_(_logits(40, 5000, torch.bfloat16, seed=8))
+    graph.replay()
+    r2, d2 = alignment.policy_loss_and_grad(x, y, old, adv)
+    assert torch.equal(r.loss, r2.loss) and torch.equal(d, d2)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose element offset passes 2^31: only the last few are labelled."""
+    rows, vocab = 43000, 50257
+    assert (rows - 1) * vocab > 2 ** 31
+    x = torch.empty(rows, vocab, device=DEV, dtype=torch.bfloat16)
+    x[-3:] = _logits(3, vocab, torch.bfloat16)
+    y = torch.full((rows,), -100, device=DEV)
+    y[-3:] = torch.tensor([5, 50256, 77], device=DEV)
+    lp = alignment.token_logprobs(x, y)
+    want = _rows64(x[-3:], y[-3:])[1]
+    assert float((lp[-3:].double() - want).abs().max()) <= _lp_tol(x[-3:])
+    old = lp - 0.1
+    tail = x[-3:].clone()
+    r, d = alignment.policy_loss_and_grad(x, y, old, torch.ones_like(lp), out=x)
+    _, small = alignment.policy_loss_and_grad(tail, y[-3:], old[-3:], torch.ones(3, device=DEV))
+    assert torch.equal(d[-3:], small) and not d[:-3].any()
+
+
+def test_model_path_preference_and_policy_through_the_head():
+    """backward_through_head on a reversible model: the preference loss's parameter gradients agree with autograd
+    over the model's logits, in fp32."""
+    import reversability_b200 as rb
+    torch.manual_seed(0)
+    model = rb.ReversibleLM(rb.ModelConfig(vocab_size=101, max_sequence_length=16, n_layers=2, n_heads=2, d_model=64,
+                                           d_ff=128), "midpoint").to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    ids = torch.randint(0, 101, (4, 16), generator=g, device=DEV)
+    y = torch.randint(0, 101, (4, 16), generator=g, device=DEV)
+    y[:, :5] = -100
+    loss = alignment.preference_loss(model(ids), y, None, beta=0.5).loss
+    loss.backward()
+    want = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    r = alignment.backward_through_head(
+        model, ids, lambda x, out: alignment.preference_loss_and_grad(x, y, None, beta=0.5, out=out), precision="fp32")
+    assert abs(float(r.loss) - float(loss)) <= 1e-6
+    for n, p in model.named_parameters():
+        assert float((p.grad - want[n]).norm()) <= 1e-5 * float(want[n].norm()), n
+    assert _lib.device_status() == 0
+
+
+def test_refusals():
+    x = _logits(6, 40, torch.float32)
+    y = torch.zeros(6, dtype=torch.int64, device=DEV)
+    f = torch.zeros(6, device=DEV)
+    bad = [
+        lambda: alignment.token_logprobs(x, y.int()),
+        lambda: alignment.token_logprobs(x, y[:5]),
+        lambda: alignment.token_logprobs(x.double(), y),
+        lambda: alignment.token_logprobs(x.t(), torch.zeros(40, dtype=torch.int64, device=DEV)),
+        lambda: alignment.token_logprobs(x[:1].expand(6, 40), y),
+        lambda: alignment.token_logprobs(x.view(2, 3, 40)[:, :2], torch.zeros(2, 2, dtype=torch.int64, device=DEV)),
+        lambda: alignment.token_logprobs(x, y, temperature=0.0),
+        lambda: alignment.token_logprobs(x, y.cpu()),
+        lambda: alignment.policy_loss(x, y, f[:5], f),
+        lambda: alignment.policy_loss(x, y, f, f[:5]),
+        lambda: alignment.policy_loss(x, y, f, f, kl_coef=0.1),
+        lambda: alignment.policy_loss(x, y, f, f, clip_low=-0.1),
+        lambda: alignment.policy_loss(x, y, f.clone().requires_grad_(), f),
+        lambda: alignment.policy_loss_and_grad(x, y, f, f, out=x.half()),
+        lambda: alignment.policy_loss_and_grad(x, y, f, f, denominator=f),
+        lambda: alignment.preference_loss(x, y, None),
+        lambda: alignment.preference_loss(x[:3].view(3, 1, 40), y[:3].view(3, 1), None),
+        lambda: alignment.preference_loss(x.view(2, 3, 40), y.view(2, 3), f),
+        lambda: alignment.preference_loss(x.view(2, 3, 40), y.view(2, 3), None, kind="other"),
+        lambda: alignment.preference_loss(x.view(2, 3, 40), y.view(2, 3), None, beta=0.0),
+        lambda: alignment.preference_loss(x.view(2, 3, 40), y.view(2, 3), None, kind="hinge", label_smoothing=0.1),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("no refusal:", k)
+    assert _lib.device_status() == 0

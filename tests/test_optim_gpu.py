@@ -1,0 +1,333 @@
+"""AdamW over many tensors (optim.py) against the update in 64 bits.
+
+Tolerances, derived from the arithmetic: each of m, v and p takes a handful of
+fp32 operations (2^-24 relative each) and an approximate root and quotient
+(2^-21 together), so one step is within 2^-20 of the moments' and the update's
+own size; errors of several steps add up. 8-bit codes are compared as codes:
+they may differ by one where the unrounded code lies within 1e-3 of a half."""
+import math
+
+import pytest
+import torch
+
+from reversability_b200 import _lib, optim
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SIZES = [1, 3, 4, 127, 255, 256, 257, 1000, 2047, 2048, 2049, 40961, 3 * 2048 * 7 + 5]
+HP = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+def _tensors(sizes, dtype=torch.float32, seed=0, offset=0, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [(torch.randn(n + offset, generator=g, device=DEV) * scale).to(dtype)[offset:] for n in sizes]
+
+
+def _params(sizes, dtype=torch.float32, offset=0):
+    return [torch.nn.Parameter(t) for t in _tensors(sizes, dtype, 1, offset, 0.1)]
+
+
+class Ref:
+    """The update in 64 bits over a list of tensors; 8-bit moments pass through their codes after each step."""
+
+    def __init__(self, params, bits=32, max_norm=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+        self.p = [p.detach().double().clone() for p in params]
+        self.m = [torch.zeros_like(p) for p in self.p]
+        self.v = [torch.zeros_like(p) for p in self.p]
+        self.bits, self.max_norm, self.t = bits, max_norm, 0
+        self.lr, self.betas, self.eps, self.wd = lr, betas, eps, weight_decay
+
+    def step(self, grads):
+        self.t += 1
+        b1, b2 = self.betas
+        g64 = [g.double() for g in grads]
+        self.norm = math.sqrt(sum(float((g * g).sum()) for g in g64))
+        coef = 1.0 if self.max_norm is None else min(1.0, self.max_norm / (self.norm + 1e-6))
+        for i, g in enumerate(g64):
+            g = g * coef
+            self.m[i] = b1 * self.m[i] + (1 - b1) * g
+            self.v[i] = b2 * self.v[i] + (1 - b2) * g * g
+            hat = self.m[i] / (1 - b1 ** self.t) / ((self.v[i] / (1 - b2 ** self.t)).sqrt() + self.eps)
+            self.p[i] = self.p[i] * (1 - self.lr * self.wd) - self.lr * hat
+
+
+def _codes64(m, v):
+    """Unrounded codes and scales of 8-bit moments for fp64 moments: (code of m, code of v, scales)."""
+    n = m.numel()
+    pad = -n % 256
+    mb = torch.nn.functional.pad(m, (0, pad)).view(-1, 256)
+    rb = torch.nn.functional.pad(v.sqrt(), (0, pad)).view(-1, 256)
+    ms, rs = mb.abs().amax(1), rb.amax(1)
+    safe = lambda t: torch.where(t > 0, t, torch.ones_like(t))[:, None]  # noqa: E731
+    cm = 127 * (mb.abs() / safe(ms)).sqrt() * mb.sign()
+    cv = 255 * (rb / safe(rs)).sqrt()
+    return cm.view(-1)[:n], torch.where(cv > 0, cv.clamp(min=1.0), cv).view(-1)[:n], ms, rs
+
+
+def _set(params, grads):
+    for p, g in zip(params, grads):
+        p.grad = g
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_32_bit_moments_against_64_bits(max_norm, offset):
+    params = _params(SIZES, offset=offset)
+    opt = optim.AdamW(params, max_norm=max_norm, **HP)
+    ref = Ref(params, max_norm=max_norm, **HP)
+    steps = 7
+    for k in range(steps):
+        grads = _tensors(SIZES, seed=10 + k, offset=offset)
+        _set(params, grads)
+        opt.step()
+        ref.step(grads)
+        if max_norm is not None:
+            assert abs(float(opt.grad_norm) - ref.norm) <= 1e-5 * ref.norm
+    # Adam's update is at most lr / (1 - b1) a step whatever the gradient's size; the clip coefficient
+    # carries the norm's 1e-6 but cancels in the update
+    for p, m, v, q in zip(ref.p, ref.m, ref.v, params):
+        st = opt.state[q]
+        assert float((q.detach().double() - p).abs().max()) <= steps * (2.0 ** -20 * HP["lr"] * 10 + 2.0 ** -23 * float(p.abs().max()))
+        assert float((st["exp_avg"].double() - m).abs().max()) <= steps * 3e-6 * float(m.abs().max())
+        assert float((st["exp_avg_sq"].double() - v).abs().max()) <= steps * 3e-6 * float(v.abs().max())
+
+
+def test_matches_torch_adamw_on_a_model():
+    torch.manual_seed(0)
+    a = torch.nn.Sequential(torch.nn.Linear(37, 300), torch.nn.GELU(), torch.nn.Linear(300, 11)).to(DEV)
+    b = torch.nn.Sequential(torch.nn.Linear(37, 300), torch.nn.GELU(), torch.nn.Linear(300, 11)).to(DEV)
+    b.load_state_dict(a.state_dict())
+    oa = optim.AdamW(a.parameters(), max_norm=1.0, **HP)
+    ob = torch.optim.AdamW(b.parameters(), **HP)
+    x = torch.randn(64, 37, device=DEV)
+    for k in range(5):
+        grads = [torch.randn(p.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(k)) for p in a.parameters()]
+        _set(a.parameters(), [g.clone() for g in grads])
+        _set(b.parameters(), [g.clone() for g in grads])
+        oa.step()
+        torch.nn.utils.clip_grad_norm_(b.parameters(), 1.0)
+        ob.step()
+        for pa, pb in zip(a.parameters(), b.parameters()):
+            assert float((pa - pb).abs().max()) <= 2.0 ** -18 * HP["lr"] * 10 * (k + 1) + 1e-7
+
+
+@pytest.mark.parametrize("p_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("g_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameter_and_gradient_types(bits, p_dtype, g_dtype):
+    params = _params([300, 2049, 7], p_dtype)
+    opt = optim.AdamW(params, state_bits=bits, **HP)
+    ref = Ref(params, **HP)
+    grads = _tensors([300, 2049, 7], g_dtype, seed=3)
+    if p_dtype == g_dtype:
+        _set(params, grads)
+        opt.step()
+    else:
+        opt.step(grads=grads)
+    ref.step(grads)
+    ulp = {torch.float32: 2.0 ** -23, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[p_dtype]
+    for p, q in zip(ref.p, params):
+        assert float(((q.detach().double() - p).abs() - ulp * p.abs()).max()) <= 2.0 ** -20 * HP["lr"] * 10
+        assert q.dtype == p_dtype
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_8_bit_moments_against_64_bits(offset):
+    """Each step is compared from the framework's own codes before it, so that errors do not pile up."""
+    params = _params(SIZES, offset=offset)
+    opt = optim.AdamW(params, state_bits=8, max_norm=0.7, **HP)
+    for k in range(4):
+        grads = _tensors(SIZES, seed=20 + k, offset=offset)
+        grads[5].zero_()  # a tensor whose gradient vanishes
+        if k == 0:
+            grads[7][10:200] = 0.0
+        ref = Ref(params, max_norm=0.7, **HP)
+        ref.t = k
+        if k:
+            ref.m, ref.v = ([t.double() for t in ts] for ts in zip(*opt.moments()))
+        _set(params, grads)
+        opt.step()
+        ref.step(grads)
+        for i, q in enumerate(params):
+            st = opt.state[q]
+            # coefficients and moments within 3e-6, so the update within 1e-5 of lr / (1 - b1)
+            assert float((q.detach().double() - ref.p[i]).abs().max()) <= 1e-5 * HP["lr"] * 10 + 2.0 ** -23 * float(ref.p[i].abs().max())
+            cm, cv, ms, rs = _codes64(ref.m[i], ref.v[i])
+            assert float((st["exp_avg_scale"].double() - ms).abs().max()) <= 1e-5 * float(ms.max())
+            assert float((st["exp_avg_sq_scale"].double() - rs).abs().max()) <= 1e-5 * float(rs.max())
+            assert float((st["exp_avg"].double() - cm).abs().max()) <= 0.5 + 1e-3
+            assert float((st["exp_avg_sq"].double() - cv).abs().max()) <= 0.5 + 1e-3
+            assert bool(((st["exp_avg_sq"] > 0) == (ref.v[i] > 0)).all())
+    # the decoded values: m = scale c|c| / 127^2, v = (scale c^2 / 255^2)^2, in fp32 and in bf16
+    for (m, v), (mb, vb), q in zip(opt.moments(), opt.moments(dtype=torch.bfloat16), params):
+        st, n = opt.state[q], q.numel()
+        c, d = st["exp_avg"].double(), st["exp_avg_sq"].double()
+        ms = st["exp_avg_scale"].double().repeat_interleave(256)[:n]
+        rs = st["exp_avg_sq_scale"].double().repeat_interleave(256)[:n]
+        want_m, want_v = ms * c * c.abs() / 127 ** 2, (rs * d * d / 255 ** 2) ** 2
+        assert float((m.double() - want_m).abs().max()) <= 2.0 ** -21 * float(want_m.abs().max())
+        assert float((v.double() - want_v).abs().max()) <= 2.0 ** -20 * float(want_v.max())
+        assert torch.equal(mb, m.bfloat16()) and torch.equal(vb, v.bfloat16())
+
+
+def test_8_bit_moments_follow_32_bits_over_many_steps():
+    """600 steps on noisy gradients of very different sizes: the 8-bit second moment's root follows the 32-bit one
+    within 25 % at nearly all elements, and no element's update runs away."""
+    n = 4096
+    a, b = torch.nn.Parameter(torch.zeros(n, device=DEV)), torch.nn.Parameter(torch.zeros(n, device=DEV))
+    hp = dict(lr=1e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.0)
+    oa, ob = optim.AdamW([a], state_bits=8, **hp), optim.AdamW([b], **hp)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    size = torch.exp(torch.randn(n, generator=g, device=DEV))
+    for _ in range(600):
+        grad = torch.randn(n, generator=g, device=DEV) * size
+        a.grad, b.grad = grad, grad
+        oa.step()
+        ob.step()
+    (_, v8), = oa.moments()
+    ratio = (v8 / ob.state[b]["exp_avg_sq"]).sqrt()
+    assert 0.97 <= float(ratio.mean()) <= 1.03
+    assert float(((ratio - 1).abs() < 0.25).float().mean()) >= 0.97
+    assert float((a - b).abs().max()) <= 0.1 and float(a.abs().max()) <= 0.6
+
+
+def test_zero_gradients_nan_and_infinity():
+    for bits in (32, 8):
+        p, q = _params([600, 600])
+        opt = optim.AdamW([p, q], state_bits=bits, **HP)
+        before = p.detach().clone()
+        p.grad, q.grad = torch.zeros_like(p), torch.zeros_like(q)
+        q.grad[300] = math.nan
+        q.grad[5] = math.inf
+        opt.step()
+        # nothing but decay where the gradient is zero
+        assert torch.allclose(p.detach(), before * (1 - HP["lr"] * HP["weight_decay"]), rtol=2.0 ** -22, atol=0)
+        assert bool(q[300].isnan()) and bool(q[100].isfinite()) and bool(q[599].isfinite())
+        if bits == 8:  # the scales of the blocks that saw them say so; the third block does not
+            m, v = opt.moments()[1]
+            assert not bool(m[256:512].isfinite().any() & m[300:301].isfinite().all())
+            assert bool(m[512:].isfinite().all()) and bool(v[512:].isfinite().all())
+    # a NaN norm shows in every parameter
+    p, q = _params([600, 600])
+    opt = optim.AdamW([p, q], max_norm=1.0, **HP)
+    p.grad, q.grad = torch.ones_like(p), torch.full_like(q, math.nan)
+    opt.step()
+    assert math.isnan(float(opt.grad_norm)) and bool(p.isnan().all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_one_launch_groups_and_missing_gradients(bits):
+    sizes = [(7 * i) % 900 + (0 if i % 13 == 5 else 1) for i in range(150)]
+    sizes[5] = 0
+    params = _params(sizes)
+    groups = [dict(params=params[:70], state_bits=bits), dict(params=params[70:], lr=3e-2, state_bits=32)]
+    opt = optim.AdamW(groups, max_norm=2.0, **HP)
+    grads = _tensors(sizes, seed=4)
+    _set(params, grads)
+    params[3].grad = None
+    params[100].grad = None
+    kept = [params[3].detach().clone(), params[100].detach().clone()]
+    live = [i for i in range(150) if i not in (3, 100)]
+    a = Ref([params[i] for i in live if i < 70], **HP)
+    b = Ref([params[i] for i in live if i >= 70], **dict(HP, lr=3e-2))
+    norm = math.sqrt(sum(float(grads[i].double().square().sum()) for i in live))
+    opt.step()
+    for r, idx in ((a, [i for i in live if i < 70]), (b, [i for i in live if i >= 70])):
+        r.step([grads[i].double() * min(1.0, 2.0 / (norm + 1e-6)) for i in idx])
+        for p, i in zip(r.p, idx):
+            if p.numel():
+                assert float((params[i].detach().double() - p).abs().max()) <= 1e-5 * r.lr * 10 + 2.0 ** -22
+    assert abs(float(opt.grad_norm) - norm) <= 1e-5 * norm
+    assert torch.equal(params[3], kept[0]) and torch.equal(params[100], kept[1])
+    assert len(opt.state[params[3]]) == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(bits, tmp_path):
+    params = _params([300, 2049], torch.bfloat16)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    opt = optim.AdamW(params, state_bits=bits, **HP)
+    for k in range(3):
+        _set(params, _tensors([300, 2049], torch.bfloat16, seed=k))
+        opt.step()
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    for p, q in zip(params, twin):
+        q.data.copy_(p.data)
+    other = optim.AdamW(twin, state_bits=bits, **dict(HP, lr=0.5))
+    other.load_state_dict(torch.load(tmp_path / "opt.pt", map_location="cpu"))
+    assert other.param_groups[0]["lr"] == HP["lr"]
+    for p, q in zip(params, twin):
+        for k, v in opt.state[p].items():
+            assert other.state[q][k].dtype == v.dtype and torch.equal(other.state[q][k], v)
+    grads = _tensors([300, 2049], torch.bfloat16, seed=9)
+    _set(params, grads)
+    _set(twin, grads)
+    opt.step()
+    other.step()
+    for p, q in zip(params, twin):
+        assert torch.equal(p, q)
+
+
+def test_captured_graph_counts_steps_and_takes_a_new_learning_rate():
+    params, twin = _params([300, 2049]), _params([300, 2049])
+    a, b = optim.AdamW(params, max_norm=1.0, **HP), optim.AdamW(twin, max_norm=1.0, **HP)
+    grads = _tensors([300, 2049], seed=2)
+    _set(params, grads)
+    _set(twin, grads)
+    a.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for lr in (1e-2, 1e-2, 3e-3):
+        a.param_groups[0]["lr"] = lr
+        a.sync_lr()
+        graph.replay()
+    for lr in (1e-2, 1e-2, 1e-2, 3e-3):
+        b.param_groups[0]["lr"] = lr
+        b.step()
+    for p, q in zip(params, twin):
+        assert torch.equal(p, q)
+    assert float(a.param_groups[0]["scalars"][1]) == 4.0
+
+
+def test_scheduler_closure_and_noncontiguous_gradient():
+    p = torch.nn.Parameter(torch.ones(20, 30, device=DEV))
+    q = torch.nn.Parameter(torch.ones(20, 30, device=DEV))
+    opt, ref = optim.AdamW([p], **HP), optim.AdamW([q], **HP)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+    g = torch.randn(30, 20, device=DEV).t()
+    p.grad, q.grad = g, g.contiguous()
+
+    def closure():
+        return torch.tensor(3.0)
+    assert float(opt.step(closure)) == 3.0
+    ref.step()
+    assert torch.equal(p, q)
+    sched.step()
+    opt.step()
+    ref.param_groups[0]["lr"] = HP["lr"] / 2
+    ref.step()
+    assert torch.equal(p, q)
+
+
+def test_refusals():
+    p = _params([10])[0]
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(max_norm=0.0)):
+        with pytest.raises(ValueError):
+            optim.AdamW([p], **kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(3))])
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(3, 4, device=DEV).t())])
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(3, device=DEV, dtype=torch.float64))])
+    opt = optim.AdamW([p], **HP)
+    with pytest.raises(ValueError):
+        opt.step(grads=[torch.zeros(9, device=DEV)])
+    with pytest.raises(ValueError):
+        opt.step(grads=[torch.zeros(10, device=DEV, dtype=torch.float64)])
+    opt8 = optim.AdamW([p], state_bits=8, **HP)
+    opt8.step(grads=[torch.zeros(10, device=DEV)])
+    with pytest.raises(ValueError):
+        opt8.moments(out=[])
+    assert _lib.device_status() == 0
