@@ -55,7 +55,8 @@ enum {
   RK_DEV_GEMM_TIMEOUT = 1u << 0,
   RK_DEV_ATTN_TIMEOUT = 1u << 1,
   RK_DEV_CE_LABEL = 1u << 2,    /* a cross-entropy label outside [0, vocab) and != ignore_index */
-  RK_DEV_EMB_INDEX = 1u << 3    /* an embedding id outside [0, vocab) */
+  RK_DEV_EMB_INDEX = 1u << 3,   /* an embedding id outside [0, vocab) */
+  RK_DEV_ROW_TIMEOUT = 1u << 4  /* a bounded wait of the token-loss row kernels gave up */
 };
 
 RK_API int rk_abi_version(void);
@@ -283,14 +284,15 @@ RK_API int rk_cross_entropy_fwd_bwd(const void* logits, int64_t ld, int64_t voca
  * RK_F16, any row stride >= vocab, no alignment rule) and z = x * inv_temp:
  *   logprob[r] = z[label] - m - ln S,  m = max z,  S = sum exp(z - m)
  *   entropy[r] = ln S - (sum exp(z - m) (z - m)) / S       (entropy may be NULL)
- * and stats[r] = (m, ln S) (float2, 8-byte aligned, may be NULL) for the
- * backward. fp32 math.
+ * and stats[r] (float2, 8-byte aligned, may be NULL) = (a reference value x_r of
+ * the row, sum 2^((x - x_r) c)) with c = inv_temp log2(e), for the backward. fp32
+ * math.
  * A row whose label is ignore_index is not read and gets 0 everywhere; a label
  * outside [0, vocab) sets RK_DEV_CE_LABEL and the row is treated as ignored.
  * The backward writes, rounded once,
  *   dlogits = ((d_logprob (1[j = label] - p_j)
  *               - d_entropy p_j (ln p_j + entropy)) * inv_temp) * (*scale_dev)
- * with p = exp(z - m - ln S), zero rows for ignored labels; d_entropy (with
+ * with p the softmax of z, zero rows for ignored labels; d_entropy (with
  * entropy, both or neither) and scale_dev (a device fp32 scalar) may be NULL.
  * coef_stride is the element stride of d_logprob and d_entropy (1 for plain
  * arrays, 2 for the interleaved coef of rk_policy_loss). dlogits may alias
@@ -316,9 +318,8 @@ RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, c
  * entropy_coef != 0, else may be NULL), metrics fp32[4] = (loss, D, weighted
  * share of rows where the clamped branch is taken, 0).
  * With dlogits the gradient of grad_scale * (*grad_scale_dev) * loss is written
- * in the same pass over the logits (they are read once while a row fits the
- * shared memory of its CTAs; dlogits may alias logits with the same leading
- * dimension). Without it, stats [rows] float2 and coef [rows] float2 =
+ * in the same pass over the logits (dlogits may alias logits with the same
+ * leading dimension). Without it, stats [rows] float2 and coef [rows] float2 =
  * (dloss/dlp, dloss/dH), where given, are what rk_token_logprob_bwd needs.
  * workspace: rk_policy_workspace(rows) bytes, 16-byte aligned. */
 typedef struct rk_policy_terms {

@@ -2,47 +2,29 @@
 // themselves, the clipped policy loss with a KL term, and the paired preference
 // loss, each with the gradient of the logits.
 //
-// A row's softmax is carried as (m, s, w): m = max z, s = sum exp(z - m),
-// w = sum exp(z - m)(z - m), merged online; then ln p_j = (z_j - m) - ln s and
-// the entropy is ln s - w / s. Keeping m and ln s apart (not their sum) keeps
-// ln p exact to fp32 when the logits are large. z = x * inv_temp in fp32; the
+// Everything is carried in base 2: with c = inv_temp log2(e) and a reference
+// value r of the row (an element within 2^8 of its maximum, so nothing
+// overflows), e_j = 2^(x_j c - r c), S = sum e_j, W = sum e_j log2 e_j:
+//   ln p_j = ln2 (x_j c - r c) - ln S,  entropy = ln S - ln2 W / S
+//   dx_j   = g_lp [j = label] + e_j (A + B (x_j c - r c)),
+//            A = (-g_lp - g_h (entropy - ln S)) / S, B = -g_h ln2 / S
+// x c - r c is one fused multiply-add with one rounding, whatever the size of
+// r; keeping r and S apart (not r + log S) keeps p exact when logits are large.
+// r is stored raw: where |r c| would overflow (a row with nothing but masks of
+// the type's lowest value) the exponent is formed as (x - r) c instead. Sums
+// are fp32 per thread over about a hundred terms, joined in a fixed order; the
 // gradient is rounded once, when it is stored.
+#include <type_traits>
 #include "vec.cuh"
 
 namespace rk {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-struct RowSum {
-  float m, s, w;
-};
-
-// Online merge of two partial sums; a part whose maximum is -inf is empty.
-template <bool ENT>
-__device__ __forceinline__ RowSum merge_rows(const RowSum& a, const RowSum& b) {
-  RowSum r;
-  r.m = fmaxf(a.m, b.m);
-  if (a.m != a.m || b.m != b.m) r.m = NAN;  // fmaxf drops a NaN
-  if (r.m == -INFINITY) return {-INFINITY, 0.f, 0.f};
-  const float da = a.m == -INFINITY ? 0.f : a.m - r.m, db = b.m == -INFINITY ? 0.f : b.m - r.m;
-  const float fa = a.m == -INFINITY ? 0.f : ex2_approx(da * kLog2e), fb = b.m == -INFINITY ? 0.f : ex2_approx(db * kLog2e);
-  r.s = fmaf(a.s, fa, b.s * fb);
-  // a part whose factor is 0 lies too far below to count (and da * s may overflow there)
-  r.w = ENT ? (fa > 0.f ? fmaf(da, a.s, a.w) * fa : 0.f) + (fb > 0.f ? fmaf(db, b.s, b.w) * fb : 0.f) : 0.f;
-  return r;
-}
-
-template <bool ENT>
-__device__ __forceinline__ RowSum warp_merge(RowSum v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const RowSum u = {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o),
-                      ENT ? __shfl_xor_sync(0xffffffffu, v.w, o) : 0.f};
-    v = merge_rows<ENT>(v, u);
-  }
-  return v;
-}
+constexpr float kHuge = 1e7f;       // |r c| from here on: the exponent as (x - r) c, as r c itself is rounded by more than 1
+constexpr float kFloor = -1e30f;    // the reference of a sum that has seen nothing finite
+constexpr float kLazy = 8.f;        // a thread's reference follows its maximum once that is 2^8 above
+constexpr float kTiny = -200.f;     // 2^-200 is 0 in fp32: exponents are clamped here where they are also a factor
 
 enum { ROW_LIVE = 0, ROW_IGNORED = 1, ROW_BAD = 2 };
 __device__ __forceinline__ int row_kind(int64_t label, int vocab, int ignore_index) {
@@ -50,107 +32,312 @@ __device__ __forceinline__ int row_kind(int64_t label, int vocab, int ignore_ind
   return label < 0 || label >= vocab ? ROW_BAD : ROW_LIVE;
 }
 
-// The row's sums over a whole CTA (every thread returns them).
-template <typename T, bool ENT>
-__device__ RowSum block_row_sum(const T* __restrict__ x, int vocab, float inv_temp, RowSum* sm) {
-  RowSum a = {-INFINITY, 0.f, 0.f};
-  for (int c = threadIdx.x; c < vocab; c += blockDim.x)
-    a = merge_rows<ENT>(a, {Dt<T>::to_f(x[c]) * inv_temp, 1.f, 0.f});
-  a = warp_merge<ENT>(a);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) sm[warp] = a;
-  __syncthreads();
-  RowSum r = lane < (int)(blockDim.x >> 5) ? sm[lane] : RowSum{-INFINITY, 0.f, 0.f};
-  r = warp_merge<ENT>(r);
-  __syncthreads();
+// ---------------------------------------------------------------- 16-byte vectors
+template <typename T>
+constexpr int kPer = 16 / (int)sizeof(T);
+
+// Pairs of floats in the packed fp32x2 arithmetic of sm_100 (one issue slot for two elements).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Exponents that are also a factor (entropy) are kept finite; a NaN stays one.
+__device__ __forceinline__ uint64_t clamp_pair(uint64_t t) {
+  float t0, t1;
+  unpair(t, t0, t1);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t0) : "f"(kTiny));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t1) : "f"(kTiny));
+  return pair(t0, t1);
+}
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
+  float t0, t1;
+  unpair(t, t0, t1);
+  return pair(ex2_approx(t0), ex2_approx(t1));
+}
 
-// Writes one row of gradients: g_lp ([j = label] - p_j) - g_h p_j (ln p_j + entropy), both factors already
-// times inv_temp and the outer scale.
-template <typename T, bool ENT>
-__device__ void block_row_grad(const T* x, T* dx, int vocab, int label, float inv_temp, float m, float ln_s,
-                               float entropy, float g_lp, float g_h) {
-  for (int c = threadIdx.x; c < vocab; c += blockDim.x) {
-    const float lp = (Dt<T>::to_f(x[c]) * inv_temp - m) - ln_s;
-    const float p = ex2_approx(lp * kLog2e);
-    float d = (c == label ? g_lp : 0.f) - g_lp * p;
-    if (ENT && p > 0.f) d -= g_h * p * (lp + entropy);  // p = 0 has lp = -inf
-    dx[c] = Dt<T>::from_f(d);
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, uint64_t (&p)[kPer<T> / 2]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4) {
+    p[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    p[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        p[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        p[i] = pair(f.x, f.y);
+      }
+    }
   }
 }
 template <typename T>
-__device__ void block_row_zero(T* dx, int vocab) {
-  for (int c = threadIdx.x; c < vocab; c += blockDim.x) dx[c] = Dt<T>::from_f(0.f);
-}
-
-// ---------------------------------------------------------------- token log-probabilities
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(512) logprob_fwd_kernel(const T* __restrict__ logits, int64_t ld, int vocab,
-                                                          const int64_t* __restrict__ labels, float inv_temp,
-                                                          int ignore_index, float* __restrict__ logprob,
-                                                          float* __restrict__ entropy, float2* __restrict__ stats,
-                                                          unsigned int* status) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ RowSum sm[32];
-  const int64_t row = blockIdx.x;
-  const int64_t label = labels[row];
-  const int kind = row_kind(label, vocab, ignore_index);
-  if (kind != ROW_LIVE) {
-    if (threadIdx.x == 0) {
-      if (kind == ROW_BAD) flag_error(status, RK_DEV_CE_LABEL);
-      logprob[row] = 0.f;
-      if (entropy) entropy[row] = 0.f;
-      if (stats) stats[row] = {0.f, 0.f};
+__device__ __forceinline__ uint4 pack(const uint64_t (&p)[kPer<T> / 2]) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+    float f[4];
+    unpair(p[0], f[0], f[1]);
+    unpair(p[1], f[2], f[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpair(p[i], a, b);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
     }
-    return;
   }
-  const T* x = logits + row * ld;
-  const RowSum r = block_row_sum<T, ENT>(x, vocab, inv_temp, sm);
-  if (threadIdx.x == 0) {
-    const float ln_s = logf(r.s);
-    logprob[row] = (Dt<T>::to_f(x[label]) * inv_temp - r.m) - ln_s;
-    if (ENT) entropy[row] = ln_s - r.w / r.s;
-    if (stats) stats[row] = {r.m, ln_s};
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Largest element of U vectors (NaNs do not count: they reach the sum through the exponential).
+template <typename T, int U>
+__device__ __forceinline__ float vec_max(const uint4 (&v)[U]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[u].x), __uint_as_float(v[u].y)),
+                         fmaxf(__uint_as_float(v[u].z), __uint_as_float(v[u].w))));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const T2* e = reinterpret_cast<const T2*>(&v[u]);
+      const T2 n = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
+      m = u ? __hmax2(m, n) : n;
+    }
+    return fmaxf(Dt<T>::to_f(m.x), Dt<T>::to_f(m.y));
   }
 }
 
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(512)
-    logprob_bwd_kernel(const T* logits, int64_t ld, int vocab, const int64_t* __restrict__ labels, float inv_temp,
-                       int ignore_index, const float2* __restrict__ stats, const float* __restrict__ entropy,
-                       const float* __restrict__ d_logprob, const float* __restrict__ d_entropy, int64_t coef_stride,
-                       const float* __restrict__ scale_dev, T* dlogits, int64_t ldd) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  const int64_t row = blockIdx.x;
-  const int64_t label = labels[row];
-  T* dx = dlogits + row * ldd;
-  if (row_kind(label, vocab, ignore_index) != ROW_LIVE) {
-    block_row_zero(dx, vocab);
-    return;
+// A row as head elements, 16-byte vectors and tail elements.
+template <typename T>
+struct RowSpan {
+  int head, nvec, tail;
+  __device__ __forceinline__ RowSpan(const T* x, int vocab) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15);
+    head = min(off ? (16 - off) / (int)sizeof(T) : 0, vocab);
+    nvec = (vocab - head) / kPer<T>;
+    tail = vocab - head - nvec * kPer<T>;
   }
-  const float scale = inv_temp * (scale_dev ? *scale_dev : 1.f);
-  const float2 st = stats[row];
-  block_row_grad<T, ENT>(logits + row * ld, dx, vocab, (int)label, inv_temp, st.x, st.y, ENT ? entropy[row] : 0.f,
-                         d_logprob[row * coef_stride] * scale, ENT ? d_entropy[row * coef_stride] * scale : 0.f);
+};
+
+// ---------------------------------------------------------------- row sums
+struct alignas(16) RowSum {
+  float r, m, s, w;  // raw reference, r c, sum 2^(x c - m), sum 2^(..) (x c - m)
+};
+__device__ __forceinline__ RowSum empty_sum() { return {-INFINITY, kFloor, 0.f, 0.f}; }
+
+// Moves a sum to the reference (r, m), m >= a.m.
+template <bool ENT>
+__device__ __forceinline__ void rebase(RowSum& a, float r, float m) {
+  const float d = a.m - m, f = ex2_approx(d);
+  if constexpr (ENT) a.w = f > 0.f ? fmaf(d, a.s, a.w) * f : 0.f;
+  a.s *= f;
+  a.r = r;
+  a.m = m;
 }
+
+// Adds U vectors at once: one look at their maximum, then U * kPer independent exponentials.
+template <typename T, bool ENT, int U>
+__device__ __forceinline__ void add_vectors(RowSum& a, const uint4 (&v)[U], float c) {
+  const float top = vec_max<T, U>(v);
+  if (top * c > a.m + kLazy) rebase<ENT>(a, top, top * c);
+  const uint64_t c2 = pair(c, c), m2 = pair(-a.m, -a.m);
+  uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint64_t p[kPer<T> / 2];
+    unpack<T>(v[u], p);
+#pragma unroll
+    for (int i = 0; i < kPer<T> / 2; ++i) {
+      uint64_t t = fma2(p[i], c2, m2);
+      if constexpr (ENT) t = clamp_pair(t);
+      const uint64_t e = exp2_pair(t);
+      s2[i & 1] = add2(s2[i & 1], e);
+      if constexpr (ENT) w2[i & 1] = fma2(e, t, w2[i & 1]);
+    }
+  }
+  float s0, s1;
+  unpair(add2(s2[0], s2[1]), s0, s1);
+  a.s += s0 + s1;
+  if constexpr (ENT) {
+    unpair(add2(w2[0], w2[1]), s0, s1);
+    a.w += s0 + s1;
+  }
+}
+template <bool ENT>
+__device__ __forceinline__ void add_element(RowSum& a, float x, float c) {
+  if (x * c > a.m + kLazy) rebase<ENT>(a, x, x * c);
+  float t = fmaf(x, c, -a.m);
+  if (ENT && t < kTiny) t = kTiny;
+  const float e = ex2_approx(t);
+  a.s += e;
+  if constexpr (ENT) a.w = fmaf(e, t, a.w);
+}
+// Joins the sums of the first N lanes (a power of two; the others hold empty ones) in a fixed order.
+template <bool ENT, int N = 32>
+__device__ __forceinline__ RowSum warp_join(RowSum a, float c) {
+  // r as an integer of the same order, so that one instruction finds the largest
+  const int b = __float_as_int(a.r), top = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
+  const float r = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
+  rebase<ENT>(a, r, fmaxf(r * c, kFloor));
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    if constexpr (ENT) a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  if constexpr (N < 32) {  // every lane returns the same sums: what follows branches on them as a warp
+    a.s = __shfl_sync(0xffffffffu, a.s, 0);
+    if constexpr (ENT) a.w = __shfl_sync(0xffffffffu, a.w, 0);
+  }
+  return a;
+}
+
+// One warp's sums of a whole row in the (x - r) c form, r its largest element: for rows whose reference overflows.
+template <typename T>
+__device__ __noinline__ RowSum warp_row_sum_far(const T* x, int vocab, float c) {
+  const int lane = threadIdx.x & 31;
+  RowSum a = {-INFINITY, 0.f, 0.f, 0.f};
+  for (int j = lane; j < vocab; j += 32) a.r = fmaxf(a.r, Dt<T>::to_f(x[j]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a.r = fmaxf(a.r, __shfl_xor_sync(0xffffffffu, a.r, o));
+  a.m = a.r * c;
+  for (int j = lane; j < vocab; j += 32) {
+    const float t = (Dt<T>::to_f(x[j]) - a.r) * c;
+    const float e = ex2_approx(t);
+    a.s += e;
+    a.w += e > 0.f ? e * t : e;  // e is 0 or NaN here
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  return a;
+}
+// Whether a finished row sum has to be formed again in that way (nothing finite seen, or r c out of range).
+__device__ __forceinline__ bool is_far(const RowSum& a) { return a.s == 0.f || !(fabsf(a.m) < kHuge); }
+__device__ __forceinline__ float exponent(float x, float c, const RowSum& a, bool far) {
+  return far ? (x - a.r) * c : fmaf(x, c, -a.m);
+}
+
+// ---------------------------------------------------------------- row gradients
+struct RowGrad {
+  float a, b, g;  // dx = e (a + b t), + g at the label; t = x c - m
+};
+__device__ __forceinline__ RowGrad row_grad(float s, float ln_s, float entropy, float g_lp, float g_h) {
+  const float inv = 1.f / s;
+  return {(-g_lp - g_h * (entropy - ln_s)) * inv, -g_h * kLn2 * inv, g_lp};
+}
+template <bool ENT>
+__device__ __forceinline__ float grad_element(float t, const RowGrad& k) {
+  if constexpr (ENT) {
+    t = t < kTiny ? kTiny : t;  // keeps a NaN
+    return ex2_approx(t) * fmaf(k.b, t, k.a);
+  }
+  return ex2_approx(t) * k.a;
+}
+// A vector's gradients, without the label's own term.
+template <typename T, bool ENT>
+__device__ __forceinline__ uint4 grad_vector(const uint4& v, float c, const RowSum& a, const RowGrad& k) {
+  uint64_t p[kPer<T> / 2];
+  unpack<T>(v, p);
+  const uint64_t c2 = pair(c, c), m2 = pair(-a.m, -a.m), ka = pair(k.a, k.a), kb = pair(k.b, k.b);
+#pragma unroll
+  for (int i = 0; i < kPer<T> / 2; ++i) {
+    uint64_t t = fma2(p[i], c2, m2);
+    if constexpr (ENT) t = clamp_pair(t);
+    p[i] = mul2(exp2_pair(t), ENT ? fma2(kb, t, ka) : ka);
+  }
+  return pack<T>(p);
+}
+// The same, element by element, for the vectors that hold the label and for rows whose reference overflows; `at` is
+// the column of the first element.
+template <typename T, bool ENT>
+__device__ __noinline__ uint4 grad_vector_any(uint4 v, float c, RowSum a, bool far, RowGrad k, int at, int label) {
+  T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+  for (int i = 0; i < kPer<T>; ++i)
+    e[i] = Dt<T>::from_f(grad_element<ENT>(exponent(Dt<T>::to_f(e[i]), c, a, far), k) + (at + i == label ? k.g : 0.f));
+  return v;
+}
+// Stores a vector at `p`, which has the phase of 16 bytes only if `vec`.
+template <typename T>
+__device__ __forceinline__ void store_vector(T* p, const uint4& v, bool vec) {
+  if (vec) {
+    __stcs(reinterpret_cast<uint4*>(p), v);
+  } else {
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < kPer<T>; ++i) p[i] = e[i];
+  }
+}
+
+// ---------------------------------------------------------------- what a row gives
+struct RowOut {
+  const int64_t* labels;
+  float* logprob;
+  float* entropy;  // NULL without ENT
+  float* kl;       // policy only, may be NULL
+  float2* stats;   // (r, S), may be NULL
+  float2* coef;    // policy only, may be NULL
+  float2* parts;   // policy only: (w l, w clipped)
+  const float* denom;
+  unsigned int* status;
+};
 
 // ---------------------------------------------------------------- policy loss
-// workspace: [0] the denominator, then per row (w l, w clipped)
 struct PolicyRow {
   float lp, kl, loss, clipped, g_lp, g_h;  // g_* without the outer scale and inv_temp
 };
-__device__ __forceinline__ PolicyRow policy_row(const rk_policy_terms& k, int64_t row, float lp, float entropy,
+struct PolicyIn {
+  float old, adv, ref, w;
+};
+__device__ __forceinline__ PolicyIn policy_in(const rk_policy_terms& k, int64_t row) {
+  return {k.old_logprobs[row], k.advantages[k.adv_group == 1 ? row : row / k.adv_group],
+          k.ref_logprobs ? k.ref_logprobs[row] : 0.f, k.weights ? k.weights[row] : 1.f};
+}
+__device__ __forceinline__ PolicyRow policy_row(const rk_policy_terms& k, const PolicyIn& in, float lp, float entropy,
                                                 float inv_d) {
   PolicyRow o;
-  const float adv = k.advantages[row / k.adv_group];
-  const float w = k.weights ? k.weights[row] : 1.f;
-  const float ratio = expf(lp - k.old_logprobs[row]);
+  const float adv = in.adv, w = in.w;
+  const float ratio = expf(lp - in.old);
   const float free = ratio * adv, held = fminf(fmaxf(ratio, 1.f - k.clip_low), 1.f + k.clip_high) * adv;
   const bool clipped = held < free;
   float kl = 0.f, dkl = 0.f;
   if (k.ref_logprobs) {
-    const float drift = k.ref_logprobs[row] - lp;
+    const float drift = in.ref - lp;
     const float em1 = expm1f(drift);
     kl = em1 - drift;
     dkl = -em1;
@@ -187,50 +374,500 @@ __global__ void __launch_bounds__(1024) policy_prepare_kernel(const int64_t* __r
   if (threadIdx.x == 0) *denom = k.denominator ? *k.denominator : (float)s;
 }
 
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(512)
-    policy_row_kernel(const T* logits, int64_t ld, int vocab, const int64_t* __restrict__ actions, int ignore_index,
-                      rk_policy_terms k, const float* __restrict__ denom, float2* __restrict__ parts,
-                      float* __restrict__ logprob, float* __restrict__ kl, float* __restrict__ entropy,
-                      float2* __restrict__ stats, float2* __restrict__ coef, T* dlogits, int64_t ldd,
-                      unsigned int* status) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ RowSum sm[32];
-  const int64_t row = blockIdx.x;
-  const int64_t label = actions[row];
-  const int kind = row_kind(label, vocab, ignore_index);
-  if (kind != ROW_LIVE) {
-    if (threadIdx.x == 0) {
-      if (kind == ROW_BAD) flag_error(status, RK_DEV_CE_LABEL);
-      logprob[row] = 0.f;
-      parts[row] = {0.f, 0.f};
-      if (kl) kl[row] = 0.f;
-      if (entropy) entropy[row] = 0.f;
-      if (stats) stats[row] = {0.f, 0.f};
-      if (coef) coef[row] = {0.f, 0.f};
+
+// ---------------------------------------------------------------- rows through a ring in shared memory
+// Persistent CTAs; a cluster of C CTAs takes a row, each a contiguous share of its 16-byte vectors. One warp
+// issues bulk copies of chunks (four vectors a thread) into a ring of seven, the other warps sum them as they land;
+// the CTA, then the cluster, joins its sums in a fixed order; and with a gradient the chunks, still in the ring, are
+// turned into it and stored, each slot refilled with the next row's chunk behind that. So the logits cross HBM once
+// each way. NT summing threads a CTA and 512 an SM: shorter rows take smaller rings and more CTAs, so that one
+// row's joins hide behind the others' sums. Of a row longer than its ring the first chunks are let go after the sums
+// and loaded again behind the others for the gradient: from L2, which holds the rows that are in work.
+constexpr int kUnroll = 4;     // vectors a thread takes of a chunk
+constexpr int kMaxSlots = 7;
+constexpr int kFreeSlots = 2;  // slots that a row longer than the ring leaves to the chunks that pass through
+constexpr int kMaxCluster = 8;
+constexpr int kMaxRowThreads = 512;
+constexpr int64_t chunk_bytes(int nt) { return (int64_t)nt * kUnroll * 16; }
+
+struct RingShared {
+  uint64_t full[kMaxSlots], empty[kMaxSlots], joined;
+  RowSum part[2][kMaxRowThreads / 32];
+  RowSum peer[2][kMaxCluster];
+  RowSum sum;
+  RowGrad grad;
+  int far;
+  int abort;
+};
+constexpr int ring_bytes(int nt, int slots) { return (int)(slots * chunk_bytes(nt)) + (int)sizeof(RingShared); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t out;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return (int)r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+// Waits of a CTA that has given up return at once: its threads go on through their rows, so that every barrier
+// still gets its arrivals, and the status word tells the host.
+__device__ __noinline__ bool ring_wait_long(uint32_t bar, uint32_t parity, unsigned int* status, volatile int* abort) {
+  return !*abort && mbar_wait(bar, parity, status, RK_DEV_ROW_TIMEOUT, abort);
+}
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsigned int* status, volatile int* abort) {
+  return mbar_try_wait(smem_u32(bar), parity) || ring_wait_long(smem_u32(bar), parity, status, abort);
+}
+template <int NT>
+__device__ __forceinline__ void row_bar() {
+  asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+}
+
+// Warp 0 of each CTA of the cluster: sends `mine` to every CTA and joins what all of them sent, in rank order.
+template <bool ENT>
+__device__ __forceinline__ RowSum cluster_join(RingShared& sh, const RowSum& mine, float c, int rank, int n, uint32_t& phase,
+                                               unsigned int* status) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // what any lane has read of the row is read before a peer learns that it may write
+  if (lane < n) {
+    const uint32_t dst = cluster_addr(smem_u32(&sh.peer[phase & 1][rank]), lane);
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(mine.r), "f"(mine.m), "f"(mine.s),
+                 "f"(mine.w)
+                 : "memory");
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     cluster_addr(smem_u32(&sh.joined), lane))
+                 : "memory");
+  }
+  bool there = false;
+  for (int i = 0; i < 256 && !there; ++i) there = try_wait_cluster(smem_u32(&sh.joined), phase & 1);
+  if (!there) {  // reading the timer costs more than the whole exchange, so only a long wait does
+    const uint64_t t0 = globaltimer();
+    while (!try_wait_cluster(smem_u32(&sh.joined), phase & 1)) {
+      if (*(volatile int*)&sh.abort) break;
+      if (globaltimer() - t0 > RK_WAIT_LIMIT_NS) {
+        flag_error(status, RK_DEV_ROW_TIMEOUT);
+        *(volatile int*)&sh.abort = 1;
+        break;
+      }
     }
-    if (dlogits) block_row_zero(dlogits + row * ldd, vocab);
+  }
+  const RowSum a = lane < n ? sh.peer[phase & 1][lane] : empty_sum();
+  ++phase;
+  return warp_join<ENT, kMaxCluster>(a, c);
+}
+
+// POLICY: the policy loss of the row, and with GRAD its gradient; else the log-probabilities alone. NT summing
+// threads, kSlots chunks in the ring, CTAS of them an SM.
+template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int kSlots, int CTAS>
+__global__ void __launch_bounds__(NT + 32, CTAS)
+    ring_row_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, float c, int ignore_index, int cluster, RowOut o,
+                    rk_policy_terms k, T* dlogits, int64_t ldd) {
+  constexpr int kWarps = NT / 32, kChunk = NT * kUnroll;  // warps that sum, vectors of a chunk
+  extern __shared__ __align__(128) unsigned char ring[];
+  RingShared& sh = *reinterpret_cast<RingShared*>(ring + kSlots * kChunk * 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = cluster > 1 ? cluster_rank() : 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.empty[i]), kWarps);
+    }
+    mbar_init(smem_u32(&sh.joined), cluster);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const int64_t first = blockIdx.x / cluster, step = gridDim.x / cluster;
+  volatile int* abort = &sh.abort;
+
+  if (warp == kWarps) {
+    if (lane == 0) {
+      int slot = 0;
+      uint32_t turn = 0;  // how often the ring has gone round
+      int64_t next = first < rows ? o.labels[first] : 0;
+      for (int64_t row = first; row < rows && !*abort; row += step) {
+        const int64_t label = next;
+        if (row + step < rows) next = o.labels[row + step];
+        if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
+        const T* x = logits + row * ld;
+        const RowSpan<T> sp(x, vocab);
+        const int chunks = (sp.nvec + kChunk - 1) / kChunk;
+        const int k0 = chunks * rank / cluster, n = chunks * (rank + 1) / cluster - k0;
+        const int again = GRAD && n > kSlots ? n - (kSlots - kFreeSlots) : 0;
+        for (int j = 0; j < n + again; ++j) {
+          const int ch = k0 + (j < n ? j : j - n);
+          if (turn && !ring_wait(&sh.empty[slot], (turn - 1) & 1, o.status, abort)) break;
+          const uint32_t bytes = 16u * (uint32_t)min(kChunk, sp.nvec - ch * kChunk);
+          const uint32_t bar = smem_u32(&sh.full[slot]);
+          mbar_arrive_expect_tx(bar, bytes);
+          bulk_load(smem_u32(ring) + slot * kChunk * 16, x + sp.head + (int64_t)ch * kChunk * kPer<T>, bytes, bar);
+          if (++slot == kSlots) {
+            slot = 0;
+            ++turn;
+          }
+        }
+      }
+      if (*abort) {  // nothing may still be on its way when the CTA ends
+        for (int i = 0; i < kSlots; ++i) {
+          const uint32_t filled = turn + (i < slot ? 1 : 0);
+          if (filled) {
+            const uint64_t t0 = globaltimer();
+            while (!mbar_try_wait(smem_u32(&sh.full[i]), (filled - 1) & 1) && globaltimer() - t0 < RK_WAIT_LIMIT_NS) {
+            }
+          }
+        }
+      }
+    }
+  } else {
+    int slot = 0;
+    uint32_t turn = 0, parity = 0, phase = 0;
+    float inv_d = 0.f, scale = 0.f;
+    if (POLICY && warp == 0) {
+      const float d = *o.denom;
+      inv_d = d != 0.f ? 1.f / d : 0.f;
+      scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
+    }
+    int64_t next = first < rows ? o.labels[first] : 0;
+    for (int64_t row = first; row < rows; row += step) {
+      const int64_t label = next;
+      if (row + step < rows) next = o.labels[row + step];
+      const int kind = row_kind(label, vocab, ignore_index);
+      T* dx = GRAD ? dlogits + row * ldd : nullptr;
+      if (kind != ROW_LIVE) {
+        if (threadIdx.x == 0 && rank == 0) {
+          if (kind == ROW_BAD) flag_error(o.status, RK_DEV_CE_LABEL);
+          o.logprob[row] = 0.f;
+          if (o.entropy) o.entropy[row] = 0.f;
+          if (o.stats) o.stats[row] = {0.f, 1.f};
+          if constexpr (POLICY) {
+            o.parts[row] = {0.f, 0.f};
+            if (o.kl) o.kl[row] = 0.f;
+            if (o.coef) o.coef[row] = {0.f, 0.f};
+          }
+        }
+        if constexpr (GRAD) {
+          const RowSpan<T> sz(dx, vocab);
+          const int v0 = (int)((int64_t)sz.nvec * rank / cluster), v1 = (int)((int64_t)sz.nvec * (rank + 1) / cluster);
+          for (int i = v0 + threadIdx.x; i < v1; i += NT)
+            __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
+          if (rank == 0 && (int)threadIdx.x < sz.head) dx[threadIdx.x] = Dt<T>::from_f(0.f);
+          if (rank == 0 && (int)threadIdx.x < sz.tail) dx[vocab - 1 - threadIdx.x] = Dt<T>::from_f(0.f);
+        }
+        continue;
+      }
+      const T* x = logits + row * ld;
+      const RowSpan<T> sp(x, vocab);
+      const int chunks = (sp.nvec + kChunk - 1) / kChunk;
+      const int k0 = chunks * rank / cluster, n = chunks * (rank + 1) / cluster - k0;
+      const int again = GRAD && n > kSlots ? n - (kSlots - kFreeSlots) : 0;  // chunks that pass through twice
+      // the elements before and behind the vectors: rank 0's first threads, the head in 0..7, the tail in 8..15
+      int edge = -1;
+      if (rank == 0 && threadIdx.x < 16) {
+        const int i = threadIdx.x & 7;
+        if (threadIdx.x < 8) edge = i < sp.head ? i : -1;
+        else edge = i < sp.tail ? vocab - 1 - i : -1;
+      }
+      const float xe = edge >= 0 ? Dt<T>::to_f(x[edge]) : 0.f;
+      const float xl = warp == 0 ? Dt<T>::to_f(x[label]) : 0.f;
+      PolicyIn in = {};
+      if (POLICY && warp == 0) in = policy_in(k, row);
+      RowSum a = empty_sum();
+      {
+        int s = slot;
+        uint32_t t = turn;
+        for (int j = 0; j < n; ++j) {
+          const int ch = k0 + j;
+          ring_wait(&sh.full[s], t & 1, o.status, abort);
+          const uint4* src = reinterpret_cast<const uint4*>(ring) + s * kChunk + threadIdx.x;
+          if ((ch + 1) * kChunk <= sp.nvec) {
+            uint4 v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];
+            add_vectors<T, ENT, kUnroll>(a, v, c);
+          } else {
+            for (int i = ch * kChunk + threadIdx.x; i < sp.nvec; i += NT, src += NT) {
+              const uint4 v[1] = {*src};
+              add_vectors<T, ENT, 1>(a, v, c);
+            }
+          }
+          const bool passes = !GRAD || j < again;
+          if (passes) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
+          }
+          if (++s == kSlots) {
+            s = 0;
+            ++t;
+          }
+          if (passes) {  // what stays in the ring begins behind it
+            slot = s;
+            turn = t;
+          }
+        }
+      }
+      if (edge >= 0) add_element<ENT>(a, xe, c);
+      a = warp_join<ENT>(a, c);
+      if (lane == 0) sh.part[parity][warp] = a;
+      row_bar<NT>();
+      if (warp == 0) {
+        a = warp_join<ENT, kWarps>(lane < kWarps ? sh.part[parity][lane] : empty_sum(), c);
+        if (cluster > 1) a = cluster_join<ENT>(sh, a, c, rank, cluster, phase, o.status);
+        const bool far = is_far(a);
+        if (far) {
+          a = warp_row_sum_far(x, vocab, c);
+          // no CTA of the cluster may write over the row before all have read it
+          if (cluster > 1) cluster_join<ENT>(sh, a, c, rank, cluster, phase, o.status);
+        }
+        const float ln_s = logf(a.s);
+        const float lp = fmaf(exponent(xl, c, a, far), kLn2, -ln_s);
+        const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
+        float g_lp = 0.f, g_h = 0.f;
+        if constexpr (POLICY) {
+          const PolicyRow q = policy_row(k, in, lp, h, inv_d);
+          g_lp = q.g_lp;
+          g_h = q.g_h;
+          if (lane == 0 && rank == 0) {
+            o.parts[row] = {q.loss, q.clipped};
+            if (o.kl) o.kl[row] = q.kl;
+            if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
+          }
+        }
+        if (lane == 0 && rank == 0) {
+          o.logprob[row] = lp;
+          if constexpr (ENT) o.entropy[row] = h;
+          if (o.stats) o.stats[row] = {a.r, a.s};
+        }
+        if (GRAD && lane == 0) {
+          sh.sum = a;
+          sh.far = far;
+          sh.grad = row_grad(a.s, ln_s, h, g_lp * scale, g_h * scale);
+        }
+      }
+      parity ^= 1;
+      if constexpr (GRAD) {
+        row_bar<NT>();
+        a = sh.sum;
+        const bool far = sh.far;
+        const RowGrad gk = sh.grad;
+        const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
+        const int hot = ((int)label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+        for (int j = again; j < n + again; ++j) {
+          const int ch = k0 + (j < n ? j : j - n);
+          if (j >= n) ring_wait(&sh.full[slot], turn & 1, o.status, abort);
+          const uint4* src = reinterpret_cast<const uint4*>(ring) + slot * kChunk + threadIdx.x;
+          const int i0 = ch * kChunk + (int)threadIdx.x;
+          uint4 v[kUnroll];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];  // past the row: what the slot held before, unused
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.empty[slot]));
+          T* to = dx + sp.head + (int64_t)i0 * kPer<T>;
+          if (vec && !far && (ch + 1) * kChunk <= sp.nvec && (unsigned)(hot - ch * kChunk) >= (unsigned)kChunk) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+              __stcs(reinterpret_cast<uint4*>(to) + u * NT, grad_vector<T, ENT>(v[u], c, a, gk));
+          } else {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+              const int i = i0 + u * NT;
+              if (i >= sp.nvec) break;
+              const uint4 g = far || i == hot ? grad_vector_any<T, ENT>(v[u], c, a, far, gk, sp.head + i * kPer<T>, (int)label)
+                                              : grad_vector<T, ENT>(v[u], c, a, gk);
+              store_vector(to + u * NT * kPer<T>, g, vec);
+            }
+          }
+          if (++slot == kSlots) {
+            slot = 0;
+            ++turn;
+          }
+        }
+        if (edge >= 0) {
+          const float t = exponent(xe, c, a, far);
+          dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, gk) + (edge == (int)label ? gk.g : 0.f));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (cluster > 1) cluster_sync();  // no CTA ends while another may still send to it
+}
+
+// ---------------------------------------------------------------- short rows: one warp each
+template <typename T, bool POLICY, bool GRAD, bool ENT>
+__global__ void __launch_bounds__(256)
+    warp_row_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, float c, int ignore_index, RowOut o,
+                    rk_policy_terms k, T* dlogits, int64_t ldd) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
+    const int64_t label = o.labels[row];
+    const int kind = row_kind(label, vocab, ignore_index);
+    T* dx = GRAD ? dlogits + row * ldd : nullptr;
+    if (kind != ROW_LIVE) {
+      if (lane == 0) {
+        if (kind == ROW_BAD) flag_error(o.status, RK_DEV_CE_LABEL);
+        o.logprob[row] = 0.f;
+        if (o.entropy) o.entropy[row] = 0.f;
+        if (o.stats) o.stats[row] = {0.f, 1.f};
+        if constexpr (POLICY) {
+          o.parts[row] = {0.f, 0.f};
+          if (o.kl) o.kl[row] = 0.f;
+          if (o.coef) o.coef[row] = {0.f, 0.f};
+        }
+      }
+      if constexpr (GRAD) {
+        const RowSpan<T> sz(dx, vocab);
+        for (int i = lane; i < sz.nvec; i += 32) __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
+        if (lane < sz.head) dx[lane] = Dt<T>::from_f(0.f);
+        if (lane < sz.tail) dx[vocab - 1 - lane] = Dt<T>::from_f(0.f);
+      }
+      continue;
+    }
+    const T* x = logits + row * ld;
+    const RowSpan<T> sp(x, vocab);
+    const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head);
+    int edge = -1;
+    if (lane < 8) edge = lane < sp.head ? lane : -1;
+    else if (lane < 16) edge = lane - 8 < sp.tail ? vocab - 1 - (lane - 8) : -1;
+    const float xe = edge >= 0 ? Dt<T>::to_f(x[edge]) : 0.f;
+    const float xl = Dt<T>::to_f(x[label]);
+    PolicyIn in = {};
+    if (POLICY) in = policy_in(k, row);
+    RowSum a = empty_sum();
+    int i = lane;
+    for (; i + 32 * (kUnroll - 1) < sp.nvec; i += 32 * kUnroll) {
+      uint4 v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u] = xv[i + 32 * u];
+      add_vectors<T, ENT, kUnroll>(a, v, c);
+    }
+    for (; i < sp.nvec; i += 32) {
+      const uint4 v[1] = {xv[i]};
+      add_vectors<T, ENT, 1>(a, v, c);
+    }
+    if (edge >= 0) add_element<ENT>(a, xe, c);
+    a = warp_join<ENT>(a, c);
+    const bool far = is_far(a);
+    if (far) a = warp_row_sum_far(x, vocab, c);
+    const float ln_s = logf(a.s);
+    const float lp = fmaf(exponent(xl, c, a, far), kLn2, -ln_s);
+    const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
+    float g_lp = 0.f, g_h = 0.f;
+    if constexpr (POLICY) {
+      const float d = *o.denom;
+      const PolicyRow q = policy_row(k, in, lp, h, d != 0.f ? 1.f / d : 0.f);
+      g_lp = q.g_lp;
+      g_h = q.g_h;
+      if (lane == 0) {
+        o.parts[row] = {q.loss, q.clipped};
+        if (o.kl) o.kl[row] = q.kl;
+        if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
+      }
+    }
+    if (lane == 0) {
+      o.logprob[row] = lp;
+      if constexpr (ENT) o.entropy[row] = h;
+      if (o.stats) o.stats[row] = {a.r, a.s};
+    }
+    if constexpr (GRAD) {
+      const float scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
+      const RowGrad gk = row_grad(a.s, ln_s, h, g_lp * scale, g_h * scale);
+      const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
+      __syncwarp();  // every lane has read the label's element and its own before any is written over
+      const int hot = ((int)label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+#pragma unroll 4
+      for (int i = lane; i < sp.nvec; i += 32) {
+        const int at = sp.head + i * kPer<T>;
+        const uint4 v = xv[i];
+        store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v, c, a, far, gk, at, (int)label)
+                                              : grad_vector<T, ENT>(v, c, a, gk), vec);
+      }
+      if (edge >= 0)
+        dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(xe, c, a, far), gk) + (edge == (int)label ? gk.g : 0.f));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradients from saved statistics
+// One CTA per (row, 8 K-element segment), four vectors a thread in flight.
+constexpr int kBwdThreads = 256, kBwdVecs = 4;
+
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kBwdThreads)
+    logprob_bwd_kernel(const T* logits, int64_t ld, int vocab, int segments, const int64_t* __restrict__ labels,
+                       float inv_temp, int ignore_index, const float2* __restrict__ stats,
+                       const float* __restrict__ entropy, const float* __restrict__ d_logprob,
+                       const float* __restrict__ d_entropy, int64_t coef_stride, const float* __restrict__ scale_dev,
+                       T* dlogits, int64_t ldd) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const int64_t row = blockIdx.x / segments;
+  const int seg = blockIdx.x % segments;
+  const int64_t label = labels[row];
+  const bool live = row_kind(label, vocab, ignore_index) == ROW_LIVE;
+  const T* x = logits + row * ld;
+  T* dx = dlogits + row * ldd;
+  const RowSpan<T> sp(live ? x : dx, vocab);
+  const int v0 = seg * kBwdThreads * kBwdVecs + threadIdx.x;
+  int edge = -1;
+  if (seg == 0 && threadIdx.x < 16) {
+    const int i = threadIdx.x & 7;
+    if (threadIdx.x < 8) edge = i < sp.head ? i : -1;
+    else edge = i < sp.tail ? vocab - 1 - i : -1;
+  }
+  if (!live) {
+#pragma unroll
+    for (int j = 0; j < kBwdVecs; ++j)
+      if (v0 + j * kBwdThreads < sp.nvec)
+        __stcs(reinterpret_cast<uint4*>(dx + sp.head) + v0 + j * kBwdThreads, make_uint4(0, 0, 0, 0));
+    if (edge >= 0) dx[edge] = Dt<T>::from_f(0.f);
     return;
   }
-  const T* x = logits + row * ld;
-  const float zl = Dt<T>::to_f(x[label]) * k.inv_temp;
-  const RowSum r = block_row_sum<T, ENT>(x, vocab, k.inv_temp, sm);
-  const float ln_s = logf(r.s), h = ENT ? ln_s - r.w / r.s : 0.f;
-  const float d = *denom;
-  const PolicyRow o = policy_row(k, row, (zl - r.m) - ln_s, h, d != 0.f ? 1.f / d : 0.f);
-  if (threadIdx.x == 0) {
-    logprob[row] = o.lp;
-    parts[row] = {o.loss, o.clipped};
-    if (kl) kl[row] = o.kl;
-    if (ENT) entropy[row] = h;
-    if (stats) stats[row] = {r.m, ln_s};
-    if (coef) coef[row] = {o.g_lp, o.g_h};
+  uint4 v[kBwdVecs];
+#pragma unroll
+  for (int j = 0; j < kBwdVecs; ++j)
+    if (v0 + j * kBwdThreads < sp.nvec) v[j] = reinterpret_cast<const uint4*>(x + sp.head)[v0 + j * kBwdThreads];
+  const float c = inv_temp * kLog2e;
+  const float scale = inv_temp * (scale_dev ? *scale_dev : 1.f);
+  const float2 st = stats[row];
+  const RowSum a = {st.x, st.x * c, st.y, 0.f};
+  const bool far = is_far(a);
+  const RowGrad k = row_grad(a.s, ENT ? logf(a.s) : 0.f, ENT ? entropy[row] : 0.f, d_logprob[row * coef_stride] * scale,
+                             ENT ? d_entropy[row * coef_stride] * scale : 0.f);
+  const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
+  const int hot = ((int)label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+#pragma unroll
+  for (int j = 0; j < kBwdVecs; ++j) {
+    const int i = v0 + j * kBwdThreads;
+    if (i < sp.nvec) {
+      const int at = sp.head + i * kPer<T>;
+      store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v[j], c, a, far, k, at, (int)label)
+                                            : grad_vector<T, ENT>(v[j], c, a, k), vec);
+    }
   }
-  if (dlogits) {
-    const float scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
-    block_row_grad<T, ENT>(x, dlogits + row * ldd, vocab, (int)label, k.inv_temp, r.m, ln_s, h, o.g_lp * scale,
-                           o.g_h * scale);
-  }
+  if (edge >= 0)
+    dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(Dt<T>::to_f(x[edge]), c, a, far), k) + (edge == (int)label ? k.g : 0.f));
 }
 
 __global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __restrict__ parts, int64_t rows,
@@ -329,20 +966,97 @@ bool shape_ok(int64_t ld, int64_t vocab, int64_t rows) {
   return rows >= 0 && rows < (1ll << 31) && vocab > 0 && vocab < (1ll << 31) && ld >= vocab;
 }
 
+// Row lengths in bytes at which the forms change; 4096 rows of 8192 x 16 bits (16 KB) and 8192 rows of 3000 (6 KB),
+// us, one warp a row / ring of 64 threads: sums 13.0 / 15.1 and 11.4 / 17.3, policy with gradient 44.0 / 35.5 and
+// 32.0 / 38.7 (a warp's second read of its row comes from L2 once 64 rows an SM exceed L1). Rings of 64 / 128 / 256
+// threads with gradient: 35.5 / 39.4 / 49.8 at 16 KB, 49 / 52 / 65 at 24 KB (the last size whose rows fit the first).
+// 256 KB rows (1500 x 131072 x 16 bits) with a ring of 256 threads twice an SM or of 512 once: 178 / 151, as the
+// larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
+constexpr int64_t kWarpRowSum = 20 * 1024, kWarpRowGrad = 8 * 1024;
+constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256);
+
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      v = 148;
+    return v;
+  }();
+  return n;
+}
+
+// CTAs that share a row: with few rows, enough to occupy an SM each while every CTA still has a chunk.
+int cluster_for(int64_t rows, int64_t bytes, int nt) {
+  const int64_t chunks = (bytes + chunk_bytes(nt) - 1) / chunk_bytes(nt);
+  int c = 1;
+  while (c < kMaxCluster && rows * c * 2 <= sm_count() && chunks >= 2 * c) c *= 2;
+  return c;
+}
+
+template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int SLOTS, int CTAS>
+int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, int ignore_index, const RowOut& o,
+                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+  static_assert(CTAS * (ring_bytes(NT, SLOTS) + 1024) <= 228 * 1024, "the rings of an SM's CTAs");
+  auto kernel = ring_row_kernel<T, POLICY, GRAD, ENT, NT, SLOTS, CTAS>;
+  const int st = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring_bytes(NT, SLOTS));
+  if (st) return st;
+  const int cluster = cluster_for(rows, vocab * (int64_t)sizeof(T), NT);
+  int64_t ctas = rows * cluster;
+  const int64_t most = (int64_t)CTAS * sm_count() / cluster * cluster;
+  if (ctas > most) ctas = most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(NT + 32);
+  cfg.dynamicSmemBytes = ring_bytes(NT, SLOTS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = rk_host::pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, x, ld, (int)vocab, rows, c, ignore_index, cluster, o, k, dx, ldd);
+  return rk_host::launch_status();
+}
+
+template <typename T, bool POLICY, bool GRAD, bool ENT>
+int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_temp, int ignore_index, const RowOut& o,
+                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+  const float c = inv_temp * kLog2e;
+  const int64_t bytes = vocab * (int64_t)sizeof(T);
+  if (bytes <= (GRAD ? kWarpRowGrad : kWarpRowSum)) {
+    const int64_t blocks = (rows + 7) / 8, most = (int64_t)sm_count() * 8;
+    rk_host::launch_k(warp_row_kernel<T, POLICY, GRAD, ENT>, (unsigned)(blocks < most ? blocks : most), 256, 0, s, x, ld,
+                      (int)vocab, rows, c, ignore_index, o, k, dx, ldd);
+    return rk_host::launch_status();
+  }
+  if (bytes <= kSmallRow) return launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+  if constexpr (GRAD) {
+    if (bytes <= kMidRow) return launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+    if (bytes <= kLongRow) return launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+    return launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+  } else {
+    return launch_ring<T, POLICY, GRAD, ENT, 256, 4, 3>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+  }
+}
+
 template <typename T>
 int logprob_fwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
                       float inv_temp, int ignore_index, float* logprob, float* entropy, float* stats,
                       cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
-  float2* st = reinterpret_cast<float2*>(stats);
-  unsigned int* status = rk_host::device_status_ptr();
-  if (entropy)
-    rk_host::launch_k(logprob_fwd_kernel<T, true>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, labels, inv_temp,
-                      ignore_index, logprob, entropy, st, status);
-  else
-    rk_host::launch_k(logprob_fwd_kernel<T, false>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, labels, inv_temp,
-                      ignore_index, logprob, entropy, st, status);
-  return rk_host::launch_status();
+  RowOut o = {};
+  o.labels = labels;
+  o.logprob = logprob;
+  o.entropy = entropy;
+  o.stats = reinterpret_cast<float2*>(stats);
+  o.status = rk_host::device_status_ptr();
+  const rk_policy_terms none = {};
+  if (entropy) return launch_rows<T, false, false, true>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, s);
+  return launch_rows<T, false, false, false>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, s);
 }
 
 template <typename T>
@@ -353,13 +1067,23 @@ int logprob_bwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64
   const T* x = static_cast<const T*>(logits);
   T* dx = static_cast<T*>(dlogits);
   const float2* st = reinterpret_cast<const float2*>(stats);
-  if (d_entropy)
-    rk_host::launch_k(logprob_bwd_kernel<T, true>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, labels, inv_temp,
-                      ignore_index, st, entropy, d_logprob, d_entropy, coef_stride, scale_dev, dx, ldd);
-  else
-    rk_host::launch_k(logprob_bwd_kernel<T, false>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, labels, inv_temp,
-                      ignore_index, st, entropy, d_logprob, d_entropy, coef_stride, scale_dev, dx, ldd);
-  return rk_host::launch_status();
+  const int64_t per = (int64_t)kBwdThreads * kBwdVecs * kPer<T>;
+  const int64_t segments = (vocab + per - 1) / per;
+  const int64_t block_rows = ((1ll << 31) - 1) / segments;  // rows of one launch
+  for (int64_t r = 0; r < rows; r += block_rows) {
+    const int64_t n = rows - r < block_rows ? rows - r : block_rows;
+    if (d_entropy)
+      rk_host::launch_k(logprob_bwd_kernel<T, true>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
+                        (int)segments, labels + r, inv_temp, ignore_index, st + r, entropy + r, d_logprob + r * coef_stride,
+                        d_entropy + r * coef_stride, coef_stride, scale_dev, dx + r * ldd, ldd);
+    else
+      rk_host::launch_k(logprob_bwd_kernel<T, false>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
+                        (int)segments, labels + r, inv_temp, ignore_index, st + r, nullptr, d_logprob + r * coef_stride,
+                        nullptr, coef_stride, scale_dev, dx + r * ldd, ldd);
+    const int e = rk_host::launch_status();
+    if (e) return e;
+  }
+  return RK_OK;
 }
 
 template <typename T>
@@ -374,15 +1098,23 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
   if (rows > 0) {
     const T* x = static_cast<const T*>(logits);
     T* dx = static_cast<T*>(dlogits);
-    float2 *S = reinterpret_cast<float2*>(stats), *C = reinterpret_cast<float2*>(coef);
-    unsigned int* status = rk_host::device_status_ptr();
+    RowOut o = {};
+    o.labels = actions;
+    o.logprob = logprob;
+    o.entropy = entropy;
+    o.kl = kl;
+    o.stats = reinterpret_cast<float2*>(stats);
+    o.coef = reinterpret_cast<float2*>(coef);
+    o.parts = parts;
+    o.denom = denom;
+    o.status = rk_host::device_status_ptr();
+    const float t = k.inv_temp;
     if (entropy)
-      rk_host::launch_k(policy_row_kernel<T, true>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, actions, ignore_index, k,
-                        denom, parts, logprob, kl, entropy, S, C, dx, ldd, status);
+      st = dx ? launch_rows<T, true, true, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s)
+              : launch_rows<T, true, false, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s);
     else
-      rk_host::launch_k(policy_row_kernel<T, false>, (unsigned)rows, 512, 0, s, x, ld, (int)vocab, actions, ignore_index,
-                        k, denom, parts, logprob, kl, entropy, S, C, dx, ldd, status);
-    st = rk_host::launch_status();
+      st = dx ? launch_rows<T, true, true, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s)
+              : launch_rows<T, true, false, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s);
     if (st) return st;
   }
   rk_host::launch_k(policy_reduce_kernel, 1, 1024, 0, s, parts, rows, denom, metrics);
@@ -425,6 +1157,7 @@ extern "C" int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t voca
   }
 }
 
+// Four scalars and the rows' loss terms.
 extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 8; }
 
 extern "C" int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* actions, int64_t rows,

@@ -651,7 +651,7 @@ def device_scalar(t, device, name: str) -> torch.Tensor | None:
 def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0, ignore_index: int = -100,
                       entropy: bool = False, want_stats: bool = True):
     """(logprob, entropy or None, stats or None) of logits [..., V] at labels [...], fp32 in the shape of labels;
-    0 at ignore_index. stats [rows, 2] = (max, ln sum exp) of a row's scaled logits, for token_logprob_bwd."""
+    0 at ignore_index. stats [rows, 2]: what token_logprob_bwd needs of a row (its reference value and sum)."""
     rows, V, ld, labels = token_rows(logits, labels)
     logprob = torch.empty(labels.shape, device=logits.device, dtype=torch.float32)
     h = torch.empty_like(logprob) if entropy else None
