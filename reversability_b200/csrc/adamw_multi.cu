@@ -20,75 +20,85 @@
 //
 // The tensor table travels as a kernel parameter: no host-to-device copy, no
 // device allocation, and a captured graph replays it.
+#include <type_traits>
 #include "vec.cuh"
 
 namespace rk {
 
-constexpr int kMultiCap = 64;       // tensors per launch: 64 x 56 bytes, below the 4 KB of a kernel's parameters
+constexpr int kMultiCap = 64;       // tensors per launch: 64 x 60 bytes, below the 4 KB of a kernel's parameters
 constexpr int kQBlock = 256;        // elements that share a scale
-constexpr int kChunk = 2048;        // elements per CTA: 8 warps, one scale block each
+constexpr int kWarps = 8;
+constexpr int kTile = kWarps * kQBlock;  // elements that a CTA takes at once
 constexpr int kMultiNormBlocks = 592;
+constexpr int kSumTiles = 4;        // tiles of a chunk of the norm: eight loads a thread in flight
 
 struct MultiTable {
   rk_adamw_tensor t[kMultiCap];
+  int start[kMultiCap + 1];  // first chunk of each tensor; start[n] = all chunks
   int n;
-  int64_t chunks;
+  int tiles;  // tiles of a chunk, which is what a CTA takes
 };
 
-// The tensor that holds chunk `c` of the launch, and the chunk's number within it.
-__device__ __forceinline__ int find_tensor(const MultiTable& tab, int64_t& c) {
-  int i = 0;
-  while (i + 1 < tab.n) {
-    const int64_t k = (tab.t[i].numel + kChunk - 1) / kChunk;
-    if (c < k) break;
-    c -= k;
-    ++i;
+// The tensor that holds chunk `c` of the launch.
+__device__ __forceinline__ int find_tensor(const MultiTable& tab, int c) {
+  int lo = 0, hi = tab.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (c >= tab.start[mid]) lo = mid;
+    else hi = mid;
   }
-  return i;
+  return lo;
 }
 
 __device__ __forceinline__ float sqrt_approx(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Four consecutive elements at `at`, those past n as zero; `vec` says that the tensor's base is aligned for it.
+// Four consecutive elements at p; where not all of them exist or p is not aligned for it (`left` >= 0), one by one,
+// the first `left` of them, the others zero.
+constexpr int kWhole = -1;
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t at, int64_t n, bool vec, float (&v)[4]) {
-  if (vec && at + 3 < n) {
-    load_vec<T, 4>(p + at, v);
+__device__ __forceinline__ void load4(const T* p, int left, float (&v)[4]) {
+  if (left == kWhole) {
+    load_vec<T, 4>(p, v);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = at + e < n ? Dt<T>::to_f(p[at + e]) : 0.f;
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? Dt<T>::to_f(p[e]) : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int64_t at, int64_t n, bool vec, const float (&v)[4]) {
-  if (vec && at + 3 < n) {
-    store_vec<T, 4>(p + at, v);
+__device__ __forceinline__ void store4(T* p, int left, const float (&v)[4]) {
+  if (left == kWhole) {
+    store_vec<T, 4>(p, v);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (at + e < n) p[at + e] = Dt<T>::from_f(v[e]);
+      if (e < left) p[e] = Dt<T>::from_f(v[e]);
   }
 }
-__device__ __forceinline__ uint32_t load4_codes(const void* p, int64_t at, int64_t n, bool vec) {
-  const uint8_t* q = static_cast<const uint8_t*>(p) + at;
-  if (vec && at + 3 < n) return *reinterpret_cast<const uint32_t*>(q);
+__device__ __forceinline__ uint32_t load4_codes(const uint8_t* p, int left) {
+  if (left == kWhole) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t w = 0;
+#pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (at + e < n) w |= (uint32_t)q[e] << (8 * e);
+    if (e < left) w |= (uint32_t)p[e] << (8 * e);
   return w;
 }
-__device__ __forceinline__ void store4_codes(void* p, int64_t at, int64_t n, bool vec, uint32_t w) {
-  uint8_t* q = static_cast<uint8_t*>(p) + at;
-  if (vec && at + 3 < n) {
-    *reinterpret_cast<uint32_t*>(q) = w;
+__device__ __forceinline__ void store4_codes(uint8_t* p, int left, uint32_t w) {
+  if (left == kWhole) {
+    *reinterpret_cast<uint32_t*>(p) = w;
     return;
   }
+#pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (at + e < n) q[e] = (uint8_t)(w >> (8 * e));
+    if (e < left) p[e] = (uint8_t)(w >> (8 * e));
 }
 // Byte e of a code word as a float, by placing it in the mantissa of 2^23 (one PRMT and one add;
 // conversion instructions run at a quarter of that rate).
@@ -137,65 +147,69 @@ __device__ __forceinline__ void adamw_element(const StepConst& k, float g, float
   m = fmaf(1.f - k.beta1, gi - m, m);
   v = fmaf(k.beta2, v, (1.f - k.beta2) * gi * gi);
   r = sqrt_approx(v);
-  p = fmaf(p, k.decay, -(k.step_size * __fdividef(m, fmaf(r, k.root, k.eps))));
+  p = fmaf(p, k.decay, -(k.step_size * m * rcp_approx(fmaf(r, k.root, k.eps))));
 }
 
+// Four codes from four rounded floats (their low bytes).
+__device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// One scale block of a tensor by one warp: lane l has elements 4 l .. 4 l + 3 of each half. WHOLE: all 256 exist and
+// every base is aligned for vectors.
 template <typename TP, typename TG, bool Q8>
-__global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant__ MultiTable tab,
-                                                          const float* __restrict__ scalars, float beta1, float beta2,
-                                                          float eps) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  const StepConst k = {scalars[3], scalars[4], 1.f / scalars[5], scalars[6], beta1, beta2, eps};
-  int64_t c = blockIdx.x;
-  const rk_adamw_tensor& t = tab.t[find_tensor(tab, c)];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n = t.numel;
-  const int64_t block = c * (kChunk / kQBlock) + warp;  // scale block of this warp
-  const int64_t base = block * kQBlock;
-  if (base >= n) return;
-  TP* P = static_cast<TP*>(t.p);
-  const TG* G = static_cast<const TG*>(t.g);
-  const bool pv = (reinterpret_cast<uintptr_t>(P) % (4 * sizeof(TP))) == 0;
-  const bool gv = (reinterpret_cast<uintptr_t>(G) % (4 * sizeof(TG))) == 0;
-  const uintptr_t state_bits = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq);
-  const bool sv = (state_bits % (Q8 ? 4 : 16)) == 0;
-  float p[2][4], g[2][4], m[2][4], v[2][4], r[2][4];
+struct BlockIn {
+  float p[2][4], m[2][4], v[2][4];
+  float g[2][4];
   uint32_t mc[2], vc[2];
+  float ms, vs;
+};
+__device__ __forceinline__ int left_of(const rk_adamw_tensor& t, int64_t at, bool whole) {
+  const int64_t have = t.numel - at;
+  return whole ? kWhole : (int)(have < 0 ? 0 : have > 4 ? 4 : have);
+}
+template <typename TP, typename TG, bool Q8, bool WHOLE>
+__device__ __forceinline__ void load_block(const rk_adamw_tensor& t, int64_t block, BlockIn<TP, TG, Q8>& in) {
+  const int64_t at = block * kQBlock + (threadIdx.x & 31) * 4;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t at = base + h * 128 + lane * 4;
-    load4(P, at, n, pv, p[h]);
-    load4(G, at, n, gv, g[h]);
+    const int left = left_of(t, at + h * 128, WHOLE);
+    load4(static_cast<const TP*>(t.p) + at + h * 128, left, in.p[h]);
+    load4(static_cast<const TG*>(t.g) + at + h * 128, left, in.g[h]);
     if constexpr (Q8) {
-      mc[h] = load4_codes(t.exp_avg, at, n, sv);
-      vc[h] = load4_codes(t.exp_avg_sq, at, n, sv);
+      in.mc[h] = load4_codes(static_cast<const uint8_t*>(t.exp_avg) + at + h * 128, left);
+      in.vc[h] = load4_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at + h * 128, left);
     } else {
-      load4(static_cast<const float*>(t.exp_avg), at, n, sv, m[h]);
-      load4(static_cast<const float*>(t.exp_avg_sq), at, n, sv, v[h]);
+      load4(static_cast<const float*>(t.exp_avg) + at + h * 128, left, in.m[h]);
+      load4(static_cast<const float*>(t.exp_avg_sq) + at + h * 128, left, in.v[h]);
     }
   }
+}
+template <typename TP, typename TG, bool Q8, bool WHOLE>
+__device__ __forceinline__ void update_block(const rk_adamw_tensor& t, int64_t block, BlockIn<TP, TG, Q8>& in,
+                                             const StepConst& k) {
+  const int64_t at = block * kQBlock + (threadIdx.x & 31) * 4;
   if constexpr (Q8) {
-    const float fm = t.exp_avg_scale[block] * (1.f / (127.f * 127.f));
-    const float fv = t.exp_avg_sq_scale[block] * (1.f / (255.f * 255.f));
+    const float fm = in.ms * (1.f / (127.f * 127.f)), fv = in.vs * (1.f / (255.f * 255.f));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) codes_to_moments(mc[h], vc[h], fm, fv, m[h], v[h]);
+    for (int h = 0; h < 2; ++h) codes_to_moments(in.mc[h], in.vc[h], fm, fv, in.m[h], in.v[h]);
   }
-  float mm = 0.f, rm = 0.f;
+  float mm = 0.f, rm = 0.f, r[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    const int left = left_of(t, at + h * 128, WHOLE);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      adamw_element(k, g[h][e], p[h][e], m[h][e], v[h][e], r[h][e]);
+      adamw_element(k, in.g[h][e], in.p[h][e], in.m[h][e], in.v[h][e], r[h][e]);
       if constexpr (Q8) {
-        mm = max_bits(mm, m[h][e]);
+        mm = max_bits(mm, in.m[h][e]);
         rm = max_bits(rm, r[h][e]);
       }
     }
-    const int64_t at = base + h * 128 + lane * 4;
-    store4(P, at, n, pv, p[h]);
+    store4(static_cast<TP*>(t.p) + at + h * 128, left, in.p[h]);
     if constexpr (!Q8) {
-      store4(static_cast<float*>(t.exp_avg), at, n, sv, m[h]);
-      store4(static_cast<float*>(t.exp_avg_sq), at, n, sv, v[h]);
+      store4(static_cast<float*>(t.exp_avg) + at + h * 128, left, in.m[h]);
+      store4(static_cast<float*>(t.exp_avg_sq) + at + h * 128, left, in.v[h]);
     }
   }
   if constexpr (Q8) {
@@ -204,22 +218,151 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
     const float im = code_factor(127.f * 127.f, mm), ir = code_factor(255.f * 255.f, rm);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t wm = 0, wv = 0;
+      const int left = left_of(t, at + h * 128, WHOLE);
+      uint32_t a[4], b[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = fminf(sqrt_approx(fabsf(m[h][e]) * im), 127.f);
-        const float b = fmaxf(fminf(sqrt_approx(r[h][e] * ir), 255.f), r[h][e] > 0.f ? 1.f : 0.f);
-        wm |= (round_bits(copysignf(a, m[h][e])) & 0xffu) << (8 * e);
-        wv |= (round_bits(b) & 0xffu) << (8 * e);
+      for (int e = 0; e < 4; ++e) {  // at most 127 and 255 up to rounding, which the nearest integer takes off
+        a[e] = round_bits(copysignf(sqrt_approx(fabsf(in.m[h][e]) * im), in.m[h][e]));
+        b[e] = round_bits(fmaxf(sqrt_approx(r[h][e] * ir), r[h][e] > 0.f ? 1.f : 0.f));
       }
-      const int64_t at = base + h * 128 + lane * 4;
-      store4_codes(t.exp_avg, at, n, sv, wm);
-      store4_codes(t.exp_avg_sq, at, n, sv, wv);
+      store4_codes(static_cast<uint8_t*>(t.exp_avg) + at + h * 128, left, pack_codes(a[0], a[1], a[2], a[3]));
+      store4_codes(static_cast<uint8_t*>(t.exp_avg_sq) + at + h * 128, left, pack_codes(b[0], b[1], b[2], b[3]));
     }
-    if (lane == 0) {
-      t.exp_avg_scale[block] = mm;
-      t.exp_avg_sq_scale[block] = rm;
+    in.ms = mm;
+    in.vs = rm;
+  }
+}
+
+// With 8-bit moments an element brings 10 bytes and takes 50 instructions: loads into registers in front of each
+// update kept too little in flight (4.6 TB/s; one block ahead, 4.9). So each lane copies its own elements of the next
+// blocks into its own places of shared memory (cp.async, no barrier needed) and takes them from there.
+constexpr int kStages = 4;
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* smem, const void* global) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(BYTES) : "memory");
+}
+template <typename TP, typename TG>
+struct Stage {  // of one CTA
+  TP p[2][256][4];
+  TG g[2][256][4];
+  uint32_t mc[2][256], vc[2][256];
+};
+template <typename TP, typename TG>
+__device__ __forceinline__ void stage_block(const rk_adamw_tensor& t, int64_t block, Stage<TP, TG>& st) {
+  const int64_t at = block * kQBlock + (threadIdx.x & 31) * 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    copy_async<4 * sizeof(TP)>(st.p[h][threadIdx.x], static_cast<const TP*>(t.p) + at + h * 128);
+    copy_async<4 * sizeof(TG)>(st.g[h][threadIdx.x], static_cast<const TG*>(t.g) + at + h * 128);
+    copy_async<4>(&st.mc[h][threadIdx.x], static_cast<const uint8_t*>(t.exp_avg) + at + h * 128);
+    copy_async<4>(&st.vc[h][threadIdx.x], static_cast<const uint8_t*>(t.exp_avg_sq) + at + h * 128);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unstage4(const T* p, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = Dt<T>::to_f(e[i]);
+  }
+}
+template <typename TP, typename TG>
+__device__ __forceinline__ void unstage_block(const Stage<TP, TG>& st, BlockIn<TP, TG, true>& in) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    unstage4(st.p[h][threadIdx.x], in.p[h]);
+    unstage4(st.g[h][threadIdx.x], in.g[h]);
+    in.mc[h] = st.mc[h][threadIdx.x];
+    in.vc[h] = st.vc[h][threadIdx.x];
+  }
+}
+template <typename TP, typename TG, bool Q8>
+constexpr int step_smem() { return Q8 ? kStages * (int)sizeof(Stage<TP, TG>) : 0; }
+
+// Whether p is aligned for four elements of `size` bytes.
+__device__ __forceinline__ bool vec_ok(const void* p, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & (4 * size - 1)) == 0;
+}
+
+template <typename TP, typename TG, bool Q8>
+__global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant__ MultiTable tab,
+                                                          const float* __restrict__ scalars, float beta1, float beta2,
+                                                          float eps) {
+  const int which = find_tensor(tab, blockIdx.x);
+  const rk_adamw_tensor& t = tab.t[which];
+  const bool vec = vec_ok(t.p, sizeof(TP)) && vec_ok(t.g, sizeof(TG)) && vec_ok(t.exp_avg, Q8 ? 1 : 4) &&
+                   vec_ok(t.exp_avg_sq, Q8 ? 1 : 4);
+  // 8-bit moments: a warp takes tab.tiles consecutive blocks, whose scales travel as one load and one store. 32-bit: the
+  // CTA's warps take neighbouring blocks (1874 against 1993 us at 456M elements)
+  const int64_t chunk = blockIdx.x - tab.start[which];
+  const int warp = threadIdx.x >> 5;
+  constexpr int kStep = Q8 ? 1 : kWarps;
+  const int64_t block = Q8 ? (chunk * kWarps + warp) * tab.tiles : chunk * tab.tiles * kWarps + warp;
+  const int64_t blocks = (t.numel + kQBlock - 1) / kQBlock, whole_blocks = vec ? t.numel / kQBlock : 0;
+  const auto before = [&](int64_t end) {  // how many of this warp's blocks lie before `end`
+    return (int)max((int64_t)0, min((int64_t)tab.tiles, (end - block + kStep - 1) / kStep));
+  };
+  const int todo = before(blocks), whole = before(whole_blocks);
+  const int lane = threadIdx.x & 31;
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const StepConst k = {scalars[3], scalars[4], 1.f / scalars[5], scalars[6], beta1, beta2, eps};
+  float ms = 0.f, vs = 0.f;
+  if (Q8 && lane < todo) {
+    ms = t.exp_avg_scale[block + lane];
+    vs = t.exp_avg_sq_scale[block + lane];
+  }
+  const auto update = [&](int i, BlockIn<TP, TG, Q8>& in, auto is_whole) {
+    if constexpr (Q8) {
+      in.ms = __shfl_sync(0xffffffffu, ms, i);
+      in.vs = __shfl_sync(0xffffffffu, vs, i);
     }
+    update_block<TP, TG, Q8, decltype(is_whole)::value>(t, block + i * kStep, in, k);
+    if (Q8 && lane == i) {
+      ms = in.ms;
+      vs = in.vs;
+    }
+  };
+  int i = 0;
+  if constexpr (Q8) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    Stage<TP, TG>* stages = reinterpret_cast<Stage<TP, TG>*>(smem);
+#pragma unroll
+    for (int j = 0; j < kStages - 1; ++j) {
+      if (j < whole) stage_block(t, block + j, stages[j]);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int at = 0;
+    for (; i < whole; ++i) {
+      BlockIn<TP, TG, Q8> now;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      unstage_block(stages[at], now);
+      if (i + kStages - 1 < whole) stage_block(t, block + i + kStages - 1, stages[at ? at - 1 : kStages - 1]);  // taken last
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      update(i, now, std::true_type{});
+      at = at + 1 < kStages ? at + 1 : 0;
+    }
+  } else {
+    for (; i < whole; ++i) {
+      BlockIn<TP, TG, Q8> now;
+      load_block<TP, TG, Q8, true>(t, block + i * kStep, now);
+      update(i, now, std::true_type{});
+    }
+  }
+  for (; i < todo; ++i) {
+    BlockIn<TP, TG, Q8> now;
+    load_block<TP, TG, Q8, false>(t, block + i * kStep, now);
+    update(i, now, std::false_type{});
+  }
+  if (Q8 && lane < todo) {
+    t.exp_avg_scale[block + lane] = ms;
+    t.exp_avg_sq_scale[block + lane] = vs;
   }
 }
 
@@ -229,16 +372,20 @@ __global__ void __launch_bounds__(256) sumsq_multi_kernel(const __grid_constant_
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ float red[8];
   float s = 0.f;
-  for (int64_t chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
-    int64_t c = chunk;
-    const rk_adamw_tensor& t = tab.t[find_tensor(tab, c)];
+  for (int chunk = blockIdx.x; chunk < tab.start[tab.n]; chunk += gridDim.x) {
+    const int which = find_tensor(tab, chunk);
+    const rk_adamw_tensor& t = tab.t[which];
     const TG* G = static_cast<const TG*>(t.g);
-    const bool gv = (reinterpret_cast<uintptr_t>(G) % (4 * sizeof(TG))) == 0;
-    float g[2][4];
+    const int64_t c0 = (int64_t)(chunk - tab.start[which]) * kSumTiles * kTile, at = c0 + threadIdx.x * 4;
+    const bool whole = vec_ok(G, sizeof(TG)) && c0 + kSumTiles * kTile <= t.numel;
+    float g[2 * kSumTiles][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load4(G, c * kChunk + h * 1024 + threadIdx.x * 4, t.numel, gv, g[h]);
+    for (int h = 0; h < 2 * kSumTiles; ++h) {
+      const int64_t have = t.numel - at - h * 1024;
+      load4(G + at + h * 1024, whole ? kWhole : (int)(have < 0 ? 0 : have > 4 ? 4 : have), g[h]);
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2 * kSumTiles; ++h)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = fmaf(g[h][e], g[h][e], s);
   }
@@ -284,31 +431,50 @@ __global__ void __launch_bounds__(256) prepare_multi_kernel(const float* __restr
   }
 }
 
+// A warp decodes a scale block, lane l its elements 8 l .. 8 l + 7, so that 16-bit values leave in 16-byte stores.
 template <typename TO>
 __global__ void __launch_bounds__(256) moments_multi_kernel(const __grid_constant__ MultiTable tab) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  int64_t c = blockIdx.x;
-  const rk_adamw_tensor& t = tab.t[find_tensor(tab, c)];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n = t.numel;
-  const int64_t block = c * (kChunk / kQBlock) + warp;
-  const int64_t base = block * kQBlock;
-  if (base >= n) return;
+  const int which = find_tensor(tab, blockIdx.x);
+  const rk_adamw_tensor& t = tab.t[which];
+  const int lane = threadIdx.x & 31;
   TO* M = static_cast<TO*>(t.p);
   TO* V = static_cast<TO*>(const_cast<void*>(t.g));
-  const uintptr_t out_bits = reinterpret_cast<uintptr_t>(M) | reinterpret_cast<uintptr_t>(V);
-  const bool ov = (out_bits % (4 * sizeof(TO))) == 0;
-  const uintptr_t state_bits = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq);
-  const bool sv = (state_bits % 4) == 0;
-  const float fm = t.exp_avg_scale[block] * (1.f / (127.f * 127.f));
-  const float fv = t.exp_avg_sq_scale[block] * (1.f / (255.f * 255.f));
+  const uint8_t* M8 = static_cast<const uint8_t*>(t.exp_avg);
+  const uint8_t* V8 = static_cast<const uint8_t*>(t.exp_avg_sq);
+  const bool vec = ((reinterpret_cast<uintptr_t>(M) | reinterpret_cast<uintptr_t>(V)) & 15) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(M8) | reinterpret_cast<uintptr_t>(V8)) & 7) == 0;
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * tab.tiles * (kTile / kQBlock) + (threadIdx.x >> 5);
+  pdl_wait();  // inputs are the previous kernel's outputs
+#pragma unroll 4
+  for (int tile = 0; tile < tab.tiles; ++tile) {
+    const int64_t block = first + tile * (kTile / kQBlock);
+    const int64_t at = block * kQBlock + lane * 8;
+    if (at >= t.numel) break;
+    const float fm = t.exp_avg_scale[block] * (1.f / (127.f * 127.f));
+    const float fv = t.exp_avg_sq_scale[block] * (1.f / (255.f * 255.f));
+    const int64_t have = t.numel - at;
+    if (vec && have >= 8) {
+      const uint2 mc = *reinterpret_cast<const uint2*>(M8 + at), vc = *reinterpret_cast<const uint2*>(V8 + at);
+      float m[2][4], v[2][4], o[8];
+      codes_to_moments(mc.x, vc.x, fm, fv, m[0], v[0]);
+      codes_to_moments(mc.y, vc.y, fm, fv, m[1], v[1]);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t at = base + h * 128 + lane * 4;
-    float m[4], v[4];
-    codes_to_moments(load4_codes(t.exp_avg, at, n, sv), load4_codes(t.exp_avg_sq, at, n, sv), fm, fv, m, v);
-    store4(M, at, n, ov, m);
-    store4(V, at, n, ov, v);
+      for (int e = 0; e < 8; ++e) o[e] = m[e >> 2][e & 3];
+      store_vec<TO, 8>(M + at, o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = v[e >> 2][e & 3];
+      store_vec<TO, 8>(V + at, o);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t rest = have - 4 * h;
+        const int left = (int)(rest < 0 ? 0 : rest > 4 ? 4 : rest);
+        float m[4], v[4];
+        codes_to_moments(load4_codes(M8 + at + 4 * h, left), load4_codes(V8 + at + 4 * h, left), fm, fv, m, v);
+        store4(M + at + 4 * h, left, m);
+        store4(V + at + 4 * h, left, v);
+      }
+    }
   }
 }
 
@@ -320,10 +486,23 @@ namespace {
 
 // Fills `tab` with up to kMultiCap tensors from `tensors[i..n)`, leaving out empty ones; returns the next index,
 // or -1 for a null pointer or a negative size.
+// Tiles of a chunk, that is consecutive blocks of a warp: 8, so that the warp writes its scales as whole 32-byte
+// sectors (written one by one, 4 bytes each, they cost 280 of 1376 us at 456M elements), but at least four CTAs for
+// each of about 150 SMs.
+// With 32-bit moments and for decoding 4 tiles are enough.
+int tiles_for(const rk_adamw_tensor* tensors, int64_t n, int most) {
+  int64_t all = 0;
+  for (int64_t i = 0; i < n; ++i) all += tensors[i].numel > 0 ? tensors[i].numel : 0;
+  int tiles = 1;
+  while (tiles < most && all >= (int64_t)600 * kTile * 2 * tiles) tiles *= 2;
+  return tiles;
+}
 enum { NEED_P = 1, NEED_STATE = 2, NEED_SCALES = 4 };
-int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, int64_t n, int needs) {
+int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, int64_t n, int needs, int tiles) {
   tab.n = 0;
-  tab.chunks = 0;
+  tab.start[0] = 0;
+  tab.tiles = tiles;
+  int64_t chunks = 0;
   for (; i < n && tab.n < kMultiCap; ++i) {
     const rk_adamw_tensor& t = tensors[i];
     if (t.numel < 0) return -1;
@@ -331,8 +510,14 @@ int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, i
     if (!t.g || ((needs & NEED_P) && !t.p) || ((needs & NEED_STATE) && (!t.exp_avg || !t.exp_avg_sq)) ||
         ((needs & NEED_SCALES) && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
       return -1;
+    const int64_t mine = (t.numel + tiles * kTile - 1) / (tiles * kTile);
+    if (chunks + mine >= (1ll << 31)) {
+      if (tab.n == 0) return -1;  // one tensor of more than 2^44 elements
+      break;
+    }
     tab.t[tab.n++] = t;
-    tab.chunks += (t.numel + kChunk - 1) / kChunk;
+    chunks += mine;
+    tab.start[tab.n] = (int)chunks;
   }
   return i;
 }
@@ -341,15 +526,18 @@ template <typename TP, typename TG>
 int step_typed(const rk_adamw_tensor* tensors, int64_t n, int bits, const float* scalars, float beta1, float beta2,
                float eps, cudaStream_t s) {
   MultiTable tab;
+  const int tiles = tiles_for(tensors, n, bits == 8 ? 8 : 4);
   for (int64_t i = 0; i < n;) {
-    i = fill_table(tab, tensors, i, n, NEED_P | NEED_STATE | (bits == 8 ? NEED_SCALES : 0));
+    i = fill_table(tab, tensors, i, n, NEED_P | NEED_STATE | (bits == 8 ? NEED_SCALES : 0), tiles);
     if (i < 0) return RK_ERR_ARG;
     if (tab.n == 0) continue;
-    if (tab.chunks >= (1ll << 31)) return RK_ERR_UNSUPPORTED;
-    if (bits == 8)
-      rk_host::launch_k(adamw_multi_kernel<TP, TG, true>, (unsigned)tab.chunks, 256, 0, s, tab, scalars, beta1, beta2, eps);
-    else
-      rk_host::launch_k(adamw_multi_kernel<TP, TG, false>, (unsigned)tab.chunks, 256, 0, s, tab, scalars, beta1, beta2, eps);
+    if (bits == 8) {
+      auto kernel = adamw_multi_kernel<TP, TG, true>;
+      const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), step_smem<TP, TG, true>());
+      if (e) return e;
+      rk_host::launch_k(kernel, (unsigned)tab.start[tab.n], 256, step_smem<TP, TG, true>(), s, tab, scalars, beta1, beta2, eps);
+    } else
+      rk_host::launch_k(adamw_multi_kernel<TP, TG, false>, (unsigned)tab.start[tab.n], 256, 0, s, tab, scalars, beta1, beta2, eps);
     const int st = rk_host::launch_status();
     if (st) return st;
   }
@@ -370,10 +558,11 @@ int step_g(const rk_adamw_tensor* tensors, int64_t n, int g_dtype, int bits, con
 template <typename TG>
 int sumsq_typed(const rk_adamw_tensor* tensors, int64_t n, float* partials, cudaStream_t s) {
   MultiTable tab;
+  const int tiles = kSumTiles;
   const int64_t end = rk_adamw_multi_parts(n);
   int64_t at = 0;
   for (int64_t i = 0; at < end;) {
-    i = fill_table(tab, tensors, i, n, 0);  // past the last tensor: an empty table, whose partials are 0
+    i = fill_table(tab, tensors, i, n, 0, tiles);  // past the last tensor: an empty table, whose partials are 0
     if (i < 0) return RK_ERR_ARG;
     rk_host::launch_k(sumsq_multi_kernel<TG>, kMultiNormBlocks, 256, 0, s, tab, partials + at);
     const int st = rk_host::launch_status();
@@ -386,12 +575,12 @@ int sumsq_typed(const rk_adamw_tensor* tensors, int64_t n, float* partials, cuda
 template <typename TO>
 int moments_typed(const rk_adamw_tensor* tensors, int64_t n, cudaStream_t s) {
   MultiTable tab;
+  const int tiles = tiles_for(tensors, n, 4);
   for (int64_t i = 0; i < n;) {
-    i = fill_table(tab, tensors, i, n, NEED_P | NEED_STATE | NEED_SCALES);
+    i = fill_table(tab, tensors, i, n, NEED_P | NEED_STATE | NEED_SCALES, tiles);
     if (i < 0) return RK_ERR_ARG;
     if (tab.n == 0) continue;
-    if (tab.chunks >= (1ll << 31)) return RK_ERR_UNSUPPORTED;
-    rk_host::launch_k(moments_multi_kernel<TO>, (unsigned)tab.chunks, 256, 0, s, tab);
+    rk_host::launch_k(moments_multi_kernel<TO>, (unsigned)tab.start[tab.n], 256, 0, s, tab);
     const int st = rk_host::launch_status();
     if (st) return st;
   }

@@ -20,10 +20,35 @@ QUANT_BLOCK = 256  # elements that share a scale in 8-bit moments
 _FIELDS = 7        # 8-byte fields of rk_adamw_tensor
 
 
-def _table(entries) -> tuple:
-    """rk_adamw_tensor array (every field is 8 bytes) from tuples of seven integers."""
-    flat = list(itertools.chain.from_iterable(entries))
-    return (ctypes.c_uint64 * len(flat))(*flat), len(flat) // _FIELDS
+class _Launch:
+    """The tensors of one group with one parameter and one gradient type: their rk_adamw_tensor array, whose moment
+    addresses and sizes stay from step to step while p and g are written anew in each."""
+
+    def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype):
+        self.index, self.bits, self.p_dtype, self.g_dtype = index, bits, p_dtype, g_dtype
+        self.p_code, self.g_code = _lib.code(p_dtype), _lib.code(g_dtype)
+        self.entries = []  # (parameter, its state, exp_avg, exp_avg_sq, elements)
+        self.table = None
+
+    def add(self, p: torch.Tensor, state: dict) -> None:
+        m, v = state["exp_avg"], state["exp_avg_sq"]
+        want = (torch.int8, torch.uint8) if self.bits == 8 else (torch.float32, torch.float32)
+        if (m.dtype, v.dtype) != want or m.numel() != p.numel() or v.numel() != p.numel() or \
+                not (m.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"{self.bits}-bit moments must be contiguous {want[0]} and {want[1]} of the parameter's size")
+        self.entries.append((p, state, m, v, p.numel()))
+
+    def finish(self) -> "_Launch":
+        flat = []
+        for p, state, m, v, n in self.entries:
+            scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if self.bits == 8 else (0, 0)
+            flat += (0, 0, m.data_ptr(), v.data_ptr(), *scales, n)
+        self.table = (ctypes.c_uint64 * len(flat))(*flat)
+        return self
+
+
+def _kind(found) -> tuple:
+    return found[0], str(found[1].dtype), str(found[2].dtype)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -35,9 +60,9 @@ class AdamW(torch.optim.Optimizer):
     max_norm: clip the gradients' global norm over all groups to it (torch.nn.utils.clip_grad_norm_ without its
     rescaling pass over the gradients); the norm of the last step is `grad_norm`, a device scalar.
 
-    A group counts one step for each step() that finds a gradient in it. Step count, learning rate and the derived constants live on the device, so a captured graph that contains
-    step() counts on when it is replayed; a learning rate changed in param_groups is copied there by the next
-    step() outside a graph, or by sync_lr()."""
+    A group counts one step for each step() that finds a gradient in it. Step count, learning rate and the derived
+    constants live on the device, so a captured graph that contains step() counts on when it is replayed; a learning
+    rate changed in param_groups is copied there by the next step() outside a graph, or by sync_lr()."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_norm: float | None = None):
@@ -45,9 +70,23 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("max_norm must be positive")
         self.max_norm = max_norm
         self.grad_norm = None  # the gradients' global norm before clipping in the last step (device scalar)
-        self._lr = {}  # group index -> the learning rate its device scalars hold
+        self._reset()
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       scalars=None))
+
+    def _reset(self) -> None:
+        self._launches = None  # the last step's plan
+        self._mixed = False    # whether a group's tensors are of several types
+        self._coded = None     # parameters with 8-bit moments and their table
+        self._lr = {}          # group index -> the learning rate its device scalars hold
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self.grad_norm = None
+        self._reset()
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
@@ -126,19 +165,39 @@ class AdamW(torch.optim.Optimizer):
             if key in state_dict["state"]:
                 self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
                                  for k, v in state_dict["state"][key].items()}
-        self._lr.clear()
+        self._reset()
 
-    def _entry(self, p: torch.Tensor, g: torch.Tensor, bits: int) -> tuple:
-        st = self._moments_of(p, bits)
-        m, v = st["exp_avg"], st["exp_avg_sq"]
-        if bits == 8:
-            if m.dtype != torch.int8 or v.dtype != torch.uint8:
-                raise ValueError("8-bit moments must be int8 and uint8 codes")
-            return (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
-                    st["exp_avg_sq_scale"].data_ptr(), p.numel())
-        if m.dtype != torch.float32 or v.dtype != torch.float32:
-            raise ValueError("32-bit moments must be fp32")
-        return p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, p.numel()
+    def _plan(self, found) -> list[_Launch]:
+        """The launches for (group index, parameter, gradient) triples."""
+        launches = {}
+        for index, p, g in found:
+            if p.dtype not in _lib.DTYPE_CODE or g.dtype not in _lib.DTYPE_CODE or not p.is_contiguous() or \
+                    g.numel() != p.numel():
+                raise ValueError("AdamW parameters must be contiguous fp32, bf16 or fp16 with gradients of their size")
+            bits = self.param_groups[index]["state_bits"]
+            key = index, p.dtype, g.dtype
+            if key not in launches:
+                launches[key] = _Launch(index, bits, p.dtype, g.dtype)
+            launches[key].add(p, self._moments_of(p, bits))
+        return [launch.finish() for launch in launches.values()]
+
+    def _fill(self, launches, found) -> bool:
+        """Writes the addresses of parameters and gradients into a plan's tables; False if the plan does not fit
+        (another set of gradients, other types or sizes, moments replaced)."""
+        if sum(len(launch.entries) for launch in launches) != len(found):
+            return False
+        it = iter(found)
+        for launch in launches:
+            table, at, p_dtype, g_dtype = launch.table, 0, launch.p_dtype, launch.g_dtype
+            for (p, state, m, v, n), (_, q, g) in zip(launch.entries, it):
+                if q is not p or p.dtype is not p_dtype or g.dtype is not g_dtype or p.numel() != n or \
+                        g.numel() != n or state["exp_avg"] is not m or state["exp_avg_sq"] is not v or \
+                        not p.is_contiguous():
+                    return False
+                table[at] = p.data_ptr()
+                table[at + 1] = g.data_ptr()
+                at += _FIELDS
+        return True
 
     # ---- the step
     @torch.no_grad()
@@ -149,75 +208,87 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        given = None if grads is None else iter(grads)
-        launches = []  # (group index, p dtype, g dtype, entries)
-        keep = []      # contiguous copies, alive until the launches are queued
-        for index, group in enumerate(self.param_groups):
-            bits, kinds = group["state_bits"], {}
-            for p in group["params"]:
-                g = p.grad if given is None else next(given, None)
+        found = []  # (group index, parameter, gradient) with contiguous gradients, alive until the launches are queued
+        if grads is None:
+            for index, group in enumerate(self.param_groups):
+                for p in group["params"]:
+                    g = p.grad  # autograd holds it to the parameter's type, shape and device
+                    if g is not None and p.numel():
+                        if g.layout is not torch.strided:
+                            raise ValueError("AdamW gradients must be dense")
+                        found.append((index, p, g if g.is_contiguous() else g.contiguous()))
+        else:
+            owners = [(index, p) for index, group in enumerate(self.param_groups) for p in group["params"]]
+            grads = list(grads)
+            if len(grads) != len(owners):
+                raise ValueError(f"grads must hold an entry for each of the {len(owners)} parameters")
+            for (index, p), g in zip(owners, grads):
                 if g is None:
                     continue
-                if g.layout != torch.strided or g.dtype not in _lib.DTYPE_CODE or g.device != p.device or \
+                if g.layout is not torch.strided or g.dtype not in _lib.DTYPE_CODE or g.device != p.device or \
                         g.shape != p.shape:
                     raise ValueError("AdamW gradients must be dense fp32, bf16 or fp16 in the parameters' shape and "
                                      "on their device")
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    keep.append(g)
                 if p.numel():
-                    kinds.setdefault((p.dtype, g.dtype), []).append(self._entry(p, g, bits))
-            launches += [(index, pd, gd, *_table(entries)) for (pd, gd), entries in kinds.items()]
-        if not launches:
+                    found.append((index, p, g if g.is_contiguous() else g.contiguous()))
+        if not found:
             return loss
+        if self._mixed:
+            found.sort(key=_kind)
+        launches = self._launches
+        if launches is None or not self._fill(launches, found):
+            found.sort(key=_kind)  # stable: by group and types, then in the order of the parameters
+            launches = self._launches = self._plan(found)
+            self._mixed = len({launch.index for launch in launches}) < len(launches)
+            self._coded = None
+            self._fill(launches, found)
         stream, lib = _lib.stream_ptr(), _lib.lib()
         partials, parts = None, 0
         if self.max_norm is not None:
-            counts = [lib.rk_adamw_multi_parts(n) for *_, n in launches]
+            counts = [lib.rk_adamw_multi_parts(len(launch.entries)) for launch in launches]
             parts = sum(counts)
-            partials = torch.empty(parts, device=self.param_groups[launches[0][0]]["params"][0].device,
-                                   dtype=torch.float32)
+            partials = torch.empty(parts, device=found[0][1].device, dtype=torch.float32)
             at = partials.data_ptr()
-            for (_, _, gd, table, n), count in zip(launches, counts):
-                _lib.call("rk_adamw_multi_sumsq", table, n, _lib.code(gd), at, stream)
+            for launch, count in zip(launches, counts):
+                _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
                 at += 4 * count
         scalars = {}
-        for index in dict.fromkeys(i for i, *_ in launches):
+        for index in dict.fromkeys(launch.index for launch in launches):
             group, scalars[index] = self.param_groups[index], self._group_scalars(index)
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_prepare", _lib.ptr(partials), parts, self.max_norm or 0.0, b1, b2,
                       group["weight_decay"], scalars[index].data_ptr(), stream)
         if self.max_norm is not None:
-            self.grad_norm = scalars[launches[0][0]][2]
-        for index, pd, gd, table, n in launches:
-            group = self.param_groups[index]
+            self.grad_norm = scalars[launches[0].index][2]
+        for launch in launches:
+            group = self.param_groups[launch.index]
             b1, b2 = group["betas"]
-            _lib.call("rk_adamw_multi_step", table, n, _lib.code(pd), _lib.code(gd), group["state_bits"],
-                      scalars[index].data_ptr(), b1, b2, group["eps"], stream)
+            _lib.call("rk_adamw_multi_step", launch.table, len(launch.entries), launch.p_code, launch.g_code, launch.bits,
+                      scalars[launch.index].data_ptr(), b1, b2, group["eps"], stream)
         return loss
 
     @torch.no_grad()
     def moments(self, out=None, dtype: torch.dtype = torch.float32) -> list:
         """The values that the 8-bit moments stand for: a pair (exp_avg, exp_avg_sq) for each parameter with 8-bit
         state, in the order of the parameters. out: pairs of contiguous tensors of one type to write into."""
-        params = [p for g in self.param_groups if g["state_bits"] == 8 for p in g["params"] if "exp_avg" in self.state[p]]
+        if self._coded is None:
+            coded = [(p, self.state[p]) for g in self.param_groups if g["state_bits"] == 8 for p in g["params"]
+                     if p in self.state and "exp_avg" in self.state[p]]
+            self._coded = [(p, st, p.numel()) for p, st in coded], (ctypes.c_uint64 * (_FIELDS * len(coded)))()
+        coded, table = self._coded
         if out is None:
-            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p in params]
-        if len(out) != len(params):
-            raise ValueError(f"out must hold {len(params)} pairs")
-        entries, kinds = [], set()
-        for p, (m, v) in zip(params, out):
-            if m.shape != p.shape or v.shape != p.shape or m.device != p.device or v.device != p.device or \
-                    not (m.is_contiguous() and v.is_contiguous()):
-                raise ValueError("out pairs must be contiguous in the parameters' shapes and on their device")
-            kinds |= {m.dtype, v.dtype}
-            st = self.state[p]
-            entries.append((m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
-                            st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr(), p.numel()))
-        if not entries:
+            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, _, _ in coded]
+        if len(out) != len(coded):
+            raise ValueError(f"out must hold {len(coded)} pairs")
+        if not coded:
             return out
-        if len(kinds) != 1:
-            raise ValueError("out tensors must share one type")
-        table, n = _table(entries)
-        _lib.call("rk_adamw_multi_moments", table, n, _lib.code(kinds.pop()), _lib.stream_ptr())
+        at, kind = 0, out[0][0].dtype
+        for (p, st, n), (m, v) in zip(coded, out):
+            if m.numel() != n or v.numel() != n or m.dtype is not kind or v.dtype is not kind or \
+                    not (m.is_cuda and v.is_cuda and m.is_contiguous() and v.is_contiguous()):
+                raise ValueError("out pairs must be contiguous CUDA tensors of one type and the parameters' sizes")
+            table[at:at + _FIELDS] = (m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
+                                      st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr(), n)
+            at += _FIELDS
+        _lib.call("rk_adamw_multi_moments", table, len(coded), _lib.code(kind), _lib.stream_ptr())
         return out
