@@ -296,10 +296,12 @@ RK_API int rk_cross_entropy_fwd_bwd(const void* logits, int64_t ld, int64_t voca
  * entropy, both or neither) and scale_dev (a device fp32 scalar) may be NULL.
  * coef_stride is the element stride of d_logprob and d_entropy (1 for plain
  * arrays, 2 for the interleaved coef of rk_policy_loss). dlogits may alias
- * logits (same leading dimension). */
+ * logits (same leading dimension). workspace of the forward:
+ * rk_token_logprob_workspace(rows) bytes (0 for few rows), 8-byte aligned. */
+RK_API int64_t rk_token_logprob_workspace(int64_t rows);
 RK_API int rk_token_logprob_fwd(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
                                 float inv_temp, int ignore_index, int dtype, float* logprob, float* entropy,
-                                float* stats, void* stream);
+                                float* stats, void* workspace, int64_t workspace_bytes, void* stream);
 RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
                                 float inv_temp, int ignore_index, int dtype, const float* stats, const float* entropy,
                                 const float* d_logprob, const float* d_entropy, int64_t coef_stride,
@@ -347,10 +349,11 @@ RK_API int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const i
  *   RK_PREF_SIGMOID  -(1 - smoothing) ln sigma(u) - smoothing ln sigma(-u)
  *   RK_PREF_HINGE    max(0, 1 - u)
  *   RK_PREF_SQUARED  (gap_chosen - gap_rejected - 1 / (2 beta))^2
- * loss = the mean over pairs. logprob [rows], stats [rows] float2, coef [rows] =
- * dloss/dlp. With dlogits, grad_scale * dloss/dlogits is written as well;
- * without, stats and coef are what rk_token_logprob_bwd needs. workspace:
- * rk_preference_workspace(pairs, length) bytes, 16-byte aligned. */
+ * loss = the mean over pairs. logprob [rows], stats [rows] float2. With dlogits,
+ * grad_scale * (*grad_scale_dev) * dloss/dlogits is written as well and coef
+ * [rows] is scratch; without, stats and coef = dloss/dlp are what
+ * rk_token_logprob_bwd needs. workspace: rk_preference_workspace(pairs, length)
+ * bytes, 16-byte aligned. */
 enum { RK_PREF_SIGMOID = 0, RK_PREF_HINGE = 1, RK_PREF_SQUARED = 2 };
 typedef struct rk_preference_terms {
   const float* ref_logprobs;   /* [2 * pairs * length] or NULL (0) */

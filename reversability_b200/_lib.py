@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import re
+import struct
 import threading
 from pathlib import Path
 
@@ -77,7 +78,8 @@ SIGNATURES: dict[str, tuple] = {
     "rk_rmsnorm_bwd_fused": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _i, _f, _p, _p, _i, _p, _i64, _i64, _i64, _p]),
     "rk_rmsnorm_dw_reduce": (_i, [_p, _i64, _i64, _p, _i, _p]),
     "rk_cross_entropy_fwd_bwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _p, _p, _p, _i64, _i, _i, _p]),
-    "rk_token_logprob_fwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _i, _i, _p, _p, _p, _p]),
+    "rk_token_logprob_workspace": (_i64, [_i64]),
+    "rk_token_logprob_fwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _i, _i, _p, _p, _p, _p, _i64, _p]),
     "rk_token_logprob_bwd": (_i, [_p, _i64, _i64, _p, _i64, _f, _i, _i, _p, _p, _p, _p, _i64, _p, _p, _i64, _p]),
     "rk_policy_workspace": (_i64, [_i64]),
     "rk_policy_loss": (_i, [_p, _i64, _i64, _p, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p]),
@@ -119,17 +121,10 @@ class LayerGrads(ctypes.Structure):
     _fields_ = [("attn_norm", _p), ("qkv", _p), ("proj", _p), ("mlp_norm", _p), ("up", _p), ("down", _p)]
 
 
-class PolicyTerms(ctypes.Structure):
-    """rk_policy_terms of include/revk.h."""
-    _fields_ = [("old_logprobs", _p), ("advantages", _p), ("ref_logprobs", _p), ("weights", _p),
-                ("denominator", _p), ("grad_scale_dev", _p), ("adv_group", _i64), ("clip_low", _f),
-                ("clip_high", _f), ("kl_coef", _f), ("entropy_coef", _f), ("inv_temp", _f), ("grad_scale", _f)]
-
-
-class PreferenceTerms(ctypes.Structure):
-    """rk_preference_terms of include/revk.h."""
-    _fields_ = [("ref_logprobs", _p), ("grad_scale_dev", _p), ("beta", _f), ("smoothing", _f), ("inv_temp", _f),
-                ("grad_scale", _f), ("kind", _i), ("average", _i)]
+# rk_policy_terms and rk_preference_terms of include/revk.h, field by field (packing bytes is a third of the time of
+# filling a ctypes structure)
+POLICY_TERMS = struct.Struct("@6Pq6f")
+PREFERENCE_TERMS = struct.Struct("@2P4f2i")
 
 
 METHOD_MIDPOINT, METHOD_EULER = 0, 1
@@ -188,6 +183,9 @@ def stream_ptr(device: torch.device | None = None) -> int:
     the innermost launch_on() stream."""
     if _launch_override:
         return _launch_override[-1]
+    if torch.cuda.is_initialized():  # the handle alone; building a Stream object takes several microseconds
+        index = torch._C._cuda_getDevice() if device is None or device.index is None else device.index
+        return torch._C._cuda_getCurrentRawStream(index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

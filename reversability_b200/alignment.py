@@ -89,6 +89,9 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     the pair (log-probabilities, entropies of the rows). Differentiable with respect to the logits."""
     _check_temperature(temperature)
     fn.require_cuda(logits, labels, what="token log-probabilities")
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        lp, h, _ = fn.token_logprob_fwd(logits, labels, temperature, ignore_index, entropy, want_stats=False)
+        return (lp, h) if entropy else lp
     return _TokenLogprobs.apply(logits, labels, float(temperature), int(ignore_index), bool(entropy))
 
 
@@ -98,7 +101,7 @@ class _Policy(torch.autograd.Function):
         want = ctx.needs_input_grad[0]
         metrics, lp, kl, h, _, stats, coef = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=want,
                                                             **args)
-        loss, _, clip, _ = metrics.unbind()
+        loss, clip = metrics[0], metrics[2]
         if want:
             ctx.save_for_backward(logits, actions, stats, coef, h if args["entropy_coef"] != 0 else None)
             ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
@@ -165,10 +168,9 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logpro
                         entropy, denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
     scale, scale_dev = _scale(grad_scale)
-    metrics, lp, kl, h, d, _, _ = fn.policy_loss(logits.detach(), actions, old_logprobs, advantages, grad_scale=scale,
+    metrics, lp, kl, h, d, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, grad_scale=scale,
                                                  grad_scale_dev=scale_dev, out=out, **args)
-    loss, _, clip, _ = metrics.unbind()
-    return PolicyLoss(loss, lp, kl, h, clip), d
+    return PolicyLoss(metrics[0], lp, kl, h, metrics[2]), d
 
 
 class _Preference(torch.autograd.Function):
@@ -179,7 +181,7 @@ class _Preference(torch.autograd.Function):
             ctx.save_for_backward(logits, labels, stats, coef)
             ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
         ctx.mark_non_differentiable(rewards, lp)
-        return loss[0], rewards, lp
+        return loss, rewards, lp
 
     @staticmethod
     @once_differentiable
@@ -226,9 +228,9 @@ def preference_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, ref_log
     args = _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index)
     fn.require_cuda(logits, labels, ref_logprobs, what="the preference loss")
     scale, scale_dev = _scale(grad_scale)
-    loss, lp, rewards, d, _, _ = fn.preference_loss(logits.detach(), labels, ref_logprobs, grad_scale=scale,
+    loss, lp, rewards, d, _, _ = fn.preference_loss(logits, labels, ref_logprobs, grad_scale=scale,
                                                     grad_scale_dev=scale_dev, out=out, **args)
-    return PreferenceLoss(loss[0], rewards, lp), d
+    return PreferenceLoss(loss, rewards, lp), d
 
 
 def backward_through_head(model, ids: torch.Tensor, loss_and_grad, precision: str = "bf16", reuse: bool = False):

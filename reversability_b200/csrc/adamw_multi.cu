@@ -343,6 +343,7 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
       BlockIn<TP, TG, Q8> now;
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       unstage_block(stages[at], now);
+      __syncwarp();  // orders the reads of the stage that is filled again
       if (i + kStages - 1 < whole) stage_block(t, block + i + kStages - 1, stages[at ? at - 1 : kStages - 1]);  // taken last
       asm volatile("cp.async.commit_group;" ::: "memory");
       update(i, now, std::true_type{});

@@ -313,9 +313,109 @@ struct RowOut {
   float2* stats;   // (r, S), may be NULL
   float2* coef;    // policy only, may be NULL
   float2* parts;   // policy only: (w l, w clipped)
-  const float* denom;
+  float* denom;    // policy only: the denominator, or with sum_here where it goes
+  bool sum_here;   // few rows: each CTA forms it by itself, which saves a launch
+  const int2* list;    // many rows: (row, label) of those with a label, the others behind; else NULL
   unsigned int* status;
 };
+
+// The outputs of a row without a label (label -1, or -2 if it is out of range).
+template <bool POLICY>
+__device__ __forceinline__ void unlabelled_row(const RowOut& o, int64_t row, int label) {
+  if (label == -2) flag_error(o.status, RK_DEV_CE_LABEL);
+  o.logprob[row] = 0.f;
+  if (o.entropy) o.entropy[row] = 0.f;
+  if (o.stats) o.stats[row] = {0.f, 1.f};
+  if constexpr (POLICY) {
+    o.parts[row] = {0.f, 0.f};
+    if (o.kl) o.kl[row] = 0.f;
+    if (o.coef) o.coef[row] = {0.f, 0.f};
+  }
+}
+__device__ __forceinline__ int checked_label(int64_t label, int vocab, int ignore_index) {
+  return label == ignore_index ? -1 : label < 0 || label >= vocab ? -2 : (int)label;
+}
+
+// The rows of one of `step` takers, the `first`-th: every step-th of the list (labelled rows first, so each taker has
+// as many of them as any other, whatever the mask), or without a list every step-th row. Reads one ahead.
+struct RowDeal {
+  const RowOut& o;
+  int64_t rows, at, step;
+  int vocab, ignore_index;
+  int64_t row;
+  int label;
+  int2 next;
+  __device__ __forceinline__ RowDeal(const RowOut& out, int64_t rows, int vocab, int ignore_index, int64_t first, int64_t step)
+      : o(out), rows(rows), at(first), step(step), vocab(vocab), ignore_index(ignore_index) {
+    if (at < rows) next = fetch(at);
+    settle();
+  }
+  __device__ __forceinline__ int2 fetch(int64_t i) const {
+    return o.list ? o.list[i] : make_int2((int)i, checked_label(o.labels[i], vocab, ignore_index));
+  }
+  __device__ __forceinline__ void settle() {
+    if (at >= rows) return;
+    row = next.x;
+    label = next.y;
+    if (at + step < rows) next = fetch(at + step);
+  }
+  __device__ __forceinline__ bool more() const { return at < rows; }
+  __device__ __forceinline__ void advance() {
+    at += step;
+    settle();
+  }
+};
+
+// Lists the rows, labelled ones in front, the others behind, both in order, and writes the outputs of the others; a CTA
+// for each 1024 rows, which counts those before its own by itself (a few loads a thread, where a second launch or a
+// chain of CTAs would take longer). With POLICY the last CTA, which sees all rows, also forms the denominator. Without
+// a list it does that alone.
+template <bool POLICY>
+__global__ void __launch_bounds__(1024) list_rows_kernel(int64_t rows, int vocab, int ignore_index, RowOut o,
+                                                         rk_policy_terms k, int2* __restrict__ list,
+                                                         float* __restrict__ denom) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  __shared__ int warp_before[32], warp_here[32];
+  __shared__ double warp_weight[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t base = list ? (int64_t)blockIdx.x * 1024 : (rows - 1) / 1024 * 1024;
+  const bool weigh = POLICY && base + 1024 >= rows;
+  double weight = 0.0;
+  int before = 0;
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < base; r += 1024) {
+    const bool live = checked_label(o.labels[r], vocab, ignore_index) >= 0;
+    before += live;
+    if (weigh && live) weight += k.weights ? (double)k.weights[r] : 1.0;
+  }
+  const int64_t row = base + threadIdx.x;
+  const int label = row < rows ? checked_label(o.labels[row], vocab, ignore_index) : -1;
+  const bool live = label >= 0;
+  const unsigned mask = __ballot_sync(0xffffffffu, live);
+  if (weigh && live) weight += k.weights ? (double)k.weights[row] : 1.0;
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (weigh) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, d);
+  }
+  if (lane == 0) {
+    warp_before[warp] = before;
+    warp_here[warp] = __popc(mask);
+    warp_weight[warp] = weight;
+  }
+  __syncthreads();
+  const int all_before = __reduce_add_sync(0xffffffffu, warp_before[lane] + (lane < warp ? warp_here[lane] : 0));
+  if (list && row < rows) {
+    const int64_t at = all_before + __popc(mask & ((1u << lane) - 1));  // labelled rows before this one
+    list[live ? at : rows - 1 - (row - at)] = make_int2((int)row, label);
+    if (!live) unlabelled_row<POLICY>(o, row, label);
+  }
+  if (weigh && threadIdx.x == 0) {
+    double s = 0.0;
+    for (int v = 0; v < 32; ++v) s += warp_weight[v];
+    *denom = k.denominator ? *k.denominator : (float)s;
+  }
+}
 
 // ---------------------------------------------------------------- policy loss
 struct PolicyRow {
@@ -363,15 +463,16 @@ __device__ double block_sum(double v) {
   return s;
 }
 
-__global__ void __launch_bounds__(1024) policy_prepare_kernel(const int64_t* __restrict__ actions, int64_t rows,
-                                                              int vocab, int ignore_index, rk_policy_terms k,
-                                                              float* __restrict__ denom) {
-  pdl_wait();  // inputs are the previous kernel's outputs
+// The sum of the weights of the rows that count, over one warp.
+__device__ __noinline__ float warp_denominator(const RowOut& o, const rk_policy_terms& k, int64_t rows, int vocab,
+                                                  int ignore_index) {
+  if (k.denominator) return *k.denominator;
   double s = 0.0;
-  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x)
-    if (row_kind(actions[r], vocab, ignore_index) == ROW_LIVE) s += k.weights ? (double)k.weights[r] : 1.0;
-  s = block_sum(s);
-  if (threadIdx.x == 0) *denom = k.denominator ? *k.denominator : (float)s;
+  for (int64_t r = threadIdx.x & 31; r < rows; r += 32)
+    if (row_kind(o.labels[r], vocab, ignore_index) == ROW_LIVE) s += k.weights ? (double)k.weights[r] : 1.0;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return (float)s;
 }
 
 
@@ -401,6 +502,13 @@ struct RingShared {
 };
 constexpr int ring_bytes(int nt, int slots) { return (int)(slots * chunk_bytes(nt)) + (int)sizeof(RingShared); }
 
+// A warp has read its part of a chunk: its slot may be filled again. The fence orders the reads before the copy that
+// follows, which writes through the other proxy; without it loads still queued behind stores read the new chunk.
+__device__ __forceinline__ void release_slot(uint64_t* empty) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(empty));
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
@@ -430,7 +538,7 @@ __device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) 
       : "memory");
   return ok;
 }
-// Waits of a CTA that has given up return at once: its threads go on through their rows, so that every barrier
+// Data waits of a CTA that has given up return at once: its threads go on through their rows, so that every barrier
 // still gets its arrivals, and the status word tells the host.
 __device__ __noinline__ bool ring_wait_long(uint32_t bar, uint32_t parity, unsigned int* status, volatile int* abort) {
   return !*abort && mbar_wait(bar, parity, status, RK_DEV_ROW_TIMEOUT, abort);
@@ -440,6 +548,7 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsign
 }
 template <int NT>
 __device__ __forceinline__ void row_bar() {
+  __syncwarp();
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
@@ -477,8 +586,9 @@ __device__ __forceinline__ RowSum cluster_join(RingShared& sh, const RowSum& min
 }
 
 // POLICY: the policy loss of the row, and with GRAD its gradient; else the log-probabilities alone. NT summing
-// threads, kSlots chunks in the ring, CTAS of them an SM.
-template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int kSlots, int CTAS>
+// threads, kSlots chunks in the ring, CTAS of them an SM. FITS: the ring holds a row's share (the loops without chunks
+// that pass twice take 548 us where the general ones take 565, 14848 x 50257 x 16 bits).
+template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int kSlots, int CTAS, bool FITS>
 __global__ void __launch_bounds__(NT + 32, CTAS)
     ring_row_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, float c, int ignore_index, int cluster, RowOut o,
                     rk_policy_terms k, T* dlogits, int64_t ldd) {
@@ -506,16 +616,13 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
     if (lane == 0) {
       int slot = 0;
       uint32_t turn = 0;  // how often the ring has gone round
-      int64_t next = first < rows ? o.labels[first] : 0;
-      for (int64_t row = first; row < rows && !*abort; row += step) {
-        const int64_t label = next;
-        if (row + step < rows) next = o.labels[row + step];
-        if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
-        const T* x = logits + row * ld;
+      for (RowDeal deal(o, rows, vocab, ignore_index, first, step); deal.more() && !*abort; deal.advance()) {
+        if (deal.label < 0) continue;
+        const T* x = logits + deal.row * ld;
         const RowSpan<T> sp(x, vocab);
         const int chunks = (sp.nvec + kChunk - 1) / kChunk;
         const int k0 = chunks * rank / cluster, n = chunks * (rank + 1) / cluster - k0;
-        const int again = GRAD && n > kSlots ? n - (kSlots - kFreeSlots) : 0;
+        const int again = GRAD && !FITS && n > kSlots ? n - (kSlots - kFreeSlots) : 0;
         for (int j = 0; j < n + again; ++j) {
           const int ch = k0 + (j < n ? j : j - n);
           if (turn && !ring_wait(&sh.empty[slot], (turn - 1) & 1, o.status, abort)) break;
@@ -545,28 +652,17 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
     uint32_t turn = 0, parity = 0, phase = 0;
     float inv_d = 0.f, scale = 0.f;
     if (POLICY && warp == 0) {
-      const float d = *o.denom;
+      const float d = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
+      if (o.sum_here && blockIdx.x == 0 && lane == 0) *o.denom = d;
       inv_d = d != 0.f ? 1.f / d : 0.f;
       scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
     }
-    int64_t next = first < rows ? o.labels[first] : 0;
-    for (int64_t row = first; row < rows; row += step) {
-      const int64_t label = next;
-      if (row + step < rows) next = o.labels[row + step];
-      const int kind = row_kind(label, vocab, ignore_index);
+    for (RowDeal deal(o, rows, vocab, ignore_index, first, step); deal.more(); deal.advance()) {
+      const int64_t row = deal.row;
+      const int label = deal.label;
       T* dx = GRAD ? dlogits + row * ldd : nullptr;
-      if (kind != ROW_LIVE) {
-        if (threadIdx.x == 0 && rank == 0) {
-          if (kind == ROW_BAD) flag_error(o.status, RK_DEV_CE_LABEL);
-          o.logprob[row] = 0.f;
-          if (o.entropy) o.entropy[row] = 0.f;
-          if (o.stats) o.stats[row] = {0.f, 1.f};
-          if constexpr (POLICY) {
-            o.parts[row] = {0.f, 0.f};
-            if (o.kl) o.kl[row] = 0.f;
-            if (o.coef) o.coef[row] = {0.f, 0.f};
-          }
-        }
+      if (label < 0) {
+        if (!o.list && threadIdx.x == 0 && rank == 0) unlabelled_row<POLICY>(o, row, label);
         if constexpr (GRAD) {
           const RowSpan<T> sz(dx, vocab);
           const int v0 = (int)((int64_t)sz.nvec * rank / cluster), v1 = (int)((int64_t)sz.nvec * (rank + 1) / cluster);
@@ -581,7 +677,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
       const RowSpan<T> sp(x, vocab);
       const int chunks = (sp.nvec + kChunk - 1) / kChunk;
       const int k0 = chunks * rank / cluster, n = chunks * (rank + 1) / cluster - k0;
-      const int again = GRAD && n > kSlots ? n - (kSlots - kFreeSlots) : 0;  // chunks that pass through twice
+      const int again = GRAD && !FITS && n > kSlots ? n - (kSlots - kFreeSlots) : 0;  // chunks that pass through twice
       // the elements before and behind the vectors: rank 0's first threads, the head in 0..7, the tail in 8..15
       int edge = -1;
       if (rank == 0 && threadIdx.x < 16) {
@@ -613,10 +709,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
             }
           }
           const bool passes = !GRAD || j < again;
-          if (passes) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
-          }
+          if (passes) release_slot(&sh.empty[s]);
           if (++s == kSlots) {
             s = 0;
             ++t;
@@ -672,7 +765,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
         const bool far = sh.far;
         const RowGrad gk = sh.grad;
         const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
-        const int hot = ((int)label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+        const int hot = (label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
         for (int j = again; j < n + again; ++j) {
           const int ch = k0 + (j < n ? j : j - n);
           if (j >= n) ring_wait(&sh.full[slot], turn & 1, o.status, abort);
@@ -681,19 +774,20 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
           uint4 v[kUnroll];
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];  // past the row: what the slot held before, unused
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.empty[slot]));
           T* to = dx + sp.head + (int64_t)i0 * kPer<T>;
           if (vec && !far && (ch + 1) * kChunk <= sp.nvec && (unsigned)(hot - ch * kChunk) >= (unsigned)kChunk) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-              __stcs(reinterpret_cast<uint4*>(to) + u * NT, grad_vector<T, ENT>(v[u], c, a, gk));
+            for (int u = 0; u < kUnroll; ++u) v[u] = grad_vector<T, ENT>(v[u], c, a, gk);
+            release_slot(&sh.empty[slot]);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) __stcs(reinterpret_cast<uint4*>(to) + u * NT, v[u]);
           } else {
+            release_slot(&sh.empty[slot]);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
               const int i = i0 + u * NT;
               if (i >= sp.nvec) break;
-              const uint4 g = far || i == hot ? grad_vector_any<T, ENT>(v[u], c, a, far, gk, sp.head + i * kPer<T>, (int)label)
+              const uint4 g = far || i == hot ? grad_vector_any<T, ENT>(v[u], c, a, far, gk, sp.head + i * kPer<T>, label)
                                               : grad_vector<T, ENT>(v[u], c, a, gk);
               store_vector(to + u * NT * kPer<T>, g, vec);
             }
@@ -705,7 +799,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
         }
         if (edge >= 0) {
           const float t = exponent(xe, c, a, far);
-          dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, gk) + (edge == (int)label ? gk.g : 0.f));
+          dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, gk) + (edge == label ? gk.g : 0.f));
         }
       }
     }
@@ -721,22 +815,16 @@ __global__ void __launch_bounds__(256)
                     rk_policy_terms k, T* dlogits, int64_t ldd) {
   pdl_wait();  // inputs are the previous kernel's outputs
   const int lane = threadIdx.x & 31;
+  float denom = 0.f;
+  if constexpr (POLICY) {
+    denom = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
+    if (o.sum_here && blockIdx.x == 0 && threadIdx.x == 0) *o.denom = denom;
+  }
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
-    const int64_t label = o.labels[row];
-    const int kind = row_kind(label, vocab, ignore_index);
+    const int label = checked_label(o.labels[row], vocab, ignore_index);
     T* dx = GRAD ? dlogits + row * ldd : nullptr;
-    if (kind != ROW_LIVE) {
-      if (lane == 0) {
-        if (kind == ROW_BAD) flag_error(o.status, RK_DEV_CE_LABEL);
-        o.logprob[row] = 0.f;
-        if (o.entropy) o.entropy[row] = 0.f;
-        if (o.stats) o.stats[row] = {0.f, 1.f};
-        if constexpr (POLICY) {
-          o.parts[row] = {0.f, 0.f};
-          if (o.kl) o.kl[row] = 0.f;
-          if (o.coef) o.coef[row] = {0.f, 0.f};
-        }
-      }
+    if (label < 0) {
+      if (lane == 0) unlabelled_row<POLICY>(o, row, label);
       if constexpr (GRAD) {
         const RowSpan<T> sz(dx, vocab);
         for (int i = lane; i < sz.nvec; i += 32) __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
@@ -776,8 +864,7 @@ __global__ void __launch_bounds__(256)
     const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
     float g_lp = 0.f, g_h = 0.f;
     if constexpr (POLICY) {
-      const float d = *o.denom;
-      const PolicyRow q = policy_row(k, in, lp, h, d != 0.f ? 1.f / d : 0.f);
+      const PolicyRow q = policy_row(k, in, lp, h, denom != 0.f ? 1.f / denom : 0.f);
       g_lp = q.g_lp;
       g_h = q.g_h;
       if (lane == 0) {
@@ -796,16 +883,16 @@ __global__ void __launch_bounds__(256)
       const RowGrad gk = row_grad(a.s, ln_s, h, g_lp * scale, g_h * scale);
       const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
       __syncwarp();  // every lane has read the label's element and its own before any is written over
-      const int hot = ((int)label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+      const int hot = (label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
 #pragma unroll 4
       for (int i = lane; i < sp.nvec; i += 32) {
         const int at = sp.head + i * kPer<T>;
         const uint4 v = xv[i];
-        store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v, c, a, far, gk, at, (int)label)
+        store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v, c, a, far, gk, at, label)
                                               : grad_vector<T, ENT>(v, c, a, gk), vec);
       }
       if (edge >= 0)
-        dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(xe, c, a, far), gk) + (edge == (int)label ? gk.g : 0.f));
+        dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(xe, c, a, far), gk) + (edge == label ? gk.g : 0.f));
     }
   }
 }
@@ -819,8 +906,8 @@ __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(const T* logits, int64_t ld, int vocab, int segments, const int64_t* __restrict__ labels,
                        float inv_temp, int ignore_index, const float2* __restrict__ stats,
                        const float* __restrict__ entropy, const float* __restrict__ d_logprob,
-                       const float* __restrict__ d_entropy, int64_t coef_stride, const float* __restrict__ scale_dev,
-                       T* dlogits, int64_t ldd) {
+                       const float* __restrict__ d_entropy, int64_t coef_stride, float scale_by,
+                       const float* __restrict__ scale_dev, T* dlogits, int64_t ldd) {
   pdl_wait();  // inputs are the previous kernel's outputs
   const int64_t row = blockIdx.x / segments;
   const int seg = blockIdx.x % segments;
@@ -849,7 +936,7 @@ __global__ void __launch_bounds__(kBwdThreads)
   for (int j = 0; j < kBwdVecs; ++j)
     if (v0 + j * kBwdThreads < sp.nvec) v[j] = reinterpret_cast<const uint4*>(x + sp.head)[v0 + j * kBwdThreads];
   const float c = inv_temp * kLog2e;
-  const float scale = inv_temp * (scale_dev ? *scale_dev : 1.f);
+  const float scale = inv_temp * scale_by * (scale_dev ? *scale_dev : 1.f);
   const float2 st = stats[row];
   const RowSum a = {st.x, st.x * c, st.y, 0.f};
   const bool far = is_far(a);
@@ -883,7 +970,7 @@ __global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __res
   a = block_sum(a);
   b = block_sum(b);
   if (threadIdx.x == 0) {
-    const float d = *denom;
+    const float d = denom ? *denom : 0.f;
     const double inv = d != 0.f ? 1.0 / d : 0.0;
     metrics[0] = (float)(a * inv);
     metrics[1] = d;
@@ -893,11 +980,33 @@ __global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __res
 }
 
 // ---------------------------------------------------------------- preference loss
-// One CTA per pair: the two sequences' gaps in a fixed order, the pair's loss and its rows' factors.
+// A sequence's gap is a sum of hundreds of differences, each small against its two log-probabilities: it is formed
+// in fp64 from the row's statistics, not from the log-probabilities rounded to fp32.
+__device__ __forceinline__ double gap_term(float xl, float r, float s, float inv_temp, const float* ref, int64_t row) {
+  return ((double)xl - (double)r) * (double)inv_temp - log((double)s) - (ref ? (double)ref[row] : 0.0);
+}
+struct PairLoss {
+  float loss, slope;  // slope = dloss / d gap_chosen
+};
+__device__ __forceinline__ PairLoss pair_loss_of(const rk_preference_terms& k, double gap_chosen, double gap_rejected) {
+  const float diff = (float)(gap_chosen - gap_rejected), u = k.beta * diff;
+  if (k.kind == RK_PREF_SIGMOID) {
+    const float tail = log1pf(expf(-fabsf(u)));
+    return {(1.f - k.smoothing) * (fmaxf(-u, 0.f) + tail) + k.smoothing * (fmaxf(u, 0.f) + tail),
+            k.beta * (k.smoothing / (1.f + expf(-u)) - (1.f - k.smoothing) / (1.f + expf(u)))};
+  }
+  if (k.kind == RK_PREF_HINGE) return {fmaxf(1.f - u, 0.f), u < 1.f ? -k.beta : 0.f};
+  const float off = diff - 0.5f / k.beta;
+  return {off * off, 2.f * off};
+}
+
+// After the rows' statistics: one CTA per pair forms the two gaps in a fixed order, the pair's loss and its rows' factors.
+template <typename T>
 __global__ void __launch_bounds__(256)
-    preference_pair_kernel(const int64_t* __restrict__ labels, int64_t pairs, int64_t length, int vocab,
-                           int ignore_index, rk_preference_terms k, const float* __restrict__ logprob,
-                           float* __restrict__ rewards, float* __restrict__ pair_loss, float* __restrict__ coef) {
+    preference_pair_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, int64_t pairs,
+                           int64_t length, int vocab, int ignore_index, rk_preference_terms k,
+                           const float2* __restrict__ stats, float* __restrict__ rewards, float* __restrict__ pair_loss,
+                           float* __restrict__ loss, float* __restrict__ coef) {
   pdl_wait();  // inputs are the previous kernel's outputs
   const int64_t pair = blockIdx.x;
   double gap[2], count[2];
@@ -905,55 +1014,38 @@ __global__ void __launch_bounds__(256)
     const int64_t base = (side * pairs + pair) * length;
     double g = 0.0, n = 0.0;
     for (int64_t t = threadIdx.x; t < length; t += blockDim.x) {
-      if (row_kind(labels[base + t], vocab, ignore_index) != ROW_LIVE) continue;
-      g += (double)logprob[base + t] - (k.ref_logprobs ? (double)k.ref_logprobs[base + t] : 0.0);
+      const int64_t row = base + t, label = labels[row];
+      if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
+      const float2 st = stats[row];
+      g += gap_term(Dt<T>::to_f(logits[row * ld + label]), st.x, st.y, k.inv_temp, k.ref_logprobs, row);
       n += 1.0;
     }
     gap[side] = block_sum(g);
     count[side] = block_sum(n);
     if (k.average) gap[side] /= fmax(count[side], 1.0);
   }
-  const float diff = (float)(gap[0] - gap[1]);
-  const float u = k.beta * diff;
-  float loss, slope;  // slope = dloss/d(gap_chosen)
-  if (k.kind == RK_PREF_SIGMOID) {
-    const float tail = log1pf(expf(-fabsf(u)));
-    loss = (1.f - k.smoothing) * (fmaxf(-u, 0.f) + tail) + k.smoothing * (fmaxf(u, 0.f) + tail);
-    slope = k.beta * (k.smoothing / (1.f + expf(-u)) - (1.f - k.smoothing) / (1.f + expf(u)));
-  } else if (k.kind == RK_PREF_HINGE) {
-    loss = fmaxf(1.f - u, 0.f);
-    slope = u < 1.f ? -k.beta : 0.f;
-  } else {
-    const float off = diff - 0.5f / k.beta;
-    loss = off * off;
-    slope = 2.f * off;
-  }
-  slope /= (float)pairs;
+  const PairLoss q = pair_loss_of(k, gap[0], gap[1]);
   if (threadIdx.x == 0) {
-    pair_loss[pair] = loss;
+    (pairs > 1 ? pair_loss + pair : loss)[0] = q.loss;
     rewards[pair] = k.beta * (float)gap[0];
     rewards[pairs + pair] = k.beta * (float)gap[1];
   }
   for (int side = 0; side < 2; ++side) {
     const int64_t base = (side * pairs + pair) * length;
-    const float s = (side ? -slope : slope) / (k.average ? (float)fmax(count[side], 1.0) : 1.f);
+    const float s = (side ? -q.slope : q.slope) / (float)pairs / (k.average ? (float)fmax(count[side], 1.0) : 1.f);
     for (int64_t t = threadIdx.x; t < length; t += blockDim.x)
       coef[base + t] = row_kind(labels[base + t], vocab, ignore_index) == ROW_LIVE ? s : 0.f;
   }
 }
 
-// loss = mean of the pair losses; scale_out = grad_scale * (*grad_scale_dev) for the gradient pass.
+// loss = mean of the pair losses.
 __global__ void __launch_bounds__(256) preference_reduce_kernel(const float* __restrict__ pair_loss, int64_t pairs,
-                                                                rk_preference_terms k, float* __restrict__ loss,
-                                                                float* __restrict__ scale_out) {
+                                                                float* __restrict__ loss) {
   pdl_wait();  // inputs are the previous kernel's outputs
   double s = 0.0;
   for (int64_t i = threadIdx.x; i < pairs; i += blockDim.x) s += pair_loss[i];
   s = block_sum(s);
-  if (threadIdx.x == 0) {
-    *loss = (float)(s / (double)pairs);
-    *scale_out = k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
-  }
+  if (threadIdx.x == 0) *loss = (float)(s / (double)pairs);
 }
 
 }  // namespace rk
@@ -965,6 +1057,12 @@ namespace {
 bool shape_ok(int64_t ld, int64_t vocab, int64_t rows) {
   return rows >= 0 && rows < (1ll << 31) && vocab > 0 && vocab < (1ll << 31) && ld >= vocab;
 }
+
+// Up to so many rows each CTA takes every n-th and sums the weights by itself (32 loads a lane, as long as the launch it
+// saves); beyond it the rows are listed first, as masks would load CTAs unevenly (a quarter of 14848 rows masked cost
+// 15 %); and with more rows than kListRows the loads even out by themselves.
+// The policy loss needs that launch for its denominator anyway; sums alone are worth its 4 us from about 60 us on.
+constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 
 // Row lengths in bytes at which the forms change; 4096 rows of 8192 x 16 bits (16 KB) and 8192 rows of 3000 (6 KB),
 // us, one warp a row / ring of 64 threads: sums 13.0 / 15.1 and 11.4 / 17.3, policy with gradient 44.0 / 35.5 and
@@ -993,11 +1091,11 @@ int cluster_for(int64_t rows, int64_t bytes, int nt) {
   return c;
 }
 
-template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int SLOTS, int CTAS>
+template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int SLOTS, int CTAS, bool FITS>
 int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, int ignore_index, const RowOut& o,
                 const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
   static_assert(CTAS * (ring_bytes(NT, SLOTS) + 1024) <= 228 * 1024, "the rings of an SM's CTAs");
-  auto kernel = ring_row_kernel<T, POLICY, GRAD, ENT, NT, SLOTS, CTAS>;
+  auto kernel = ring_row_kernel<T, POLICY, GRAD, ENT, NT, SLOTS, CTAS, FITS>;
   const int st = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring_bytes(NT, SLOTS));
   if (st) return st;
   const int cluster = cluster_for(rows, vocab * (int64_t)sizeof(T), NT);
@@ -1022,32 +1120,47 @@ int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, in
   return rk_host::launch_status();
 }
 
+// `list`: room for rows (row, label) pairs, `denom` for the denominator.
 template <typename T, bool POLICY, bool GRAD, bool ENT>
-int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_temp, int ignore_index, const RowOut& o,
-                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_temp, int ignore_index, RowOut o,
+                const rk_policy_terms& k, T* dx, int64_t ldd, int2* list, float* denom, cudaStream_t s) {
   const float c = inv_temp * kLog2e;
   const int64_t bytes = vocab * (int64_t)sizeof(T);
-  if (bytes <= (GRAD ? kWarpRowGrad : kWarpRowSum)) {
+  const bool by_warp = bytes <= (GRAD ? kWarpRowGrad : kWarpRowSum);
+  o.denom = denom;
+  o.sum_here = rows <= kFewRows;
+  const bool worth = POLICY || rows * bytes >= kListBytes;
+  o.list = rows > kFewRows && rows <= kListRows && !by_warp && worth ? list : nullptr;
+  if (rows > kFewRows && (o.list || POLICY)) {
+    rk_host::launch_k(list_rows_kernel<POLICY>, o.list ? (unsigned)((rows + 1023) / 1024) : 1, 1024, 0, s, rows, (int)vocab, ignore_index, o, k,
+                      const_cast<int2*>(o.list), denom);
+    const int st = rk_host::launch_status();
+    if (st) return st;
+  }
+  if (by_warp) {
     const int64_t blocks = (rows + 7) / 8, most = (int64_t)sm_count() * 8;
     rk_host::launch_k(warp_row_kernel<T, POLICY, GRAD, ENT>, (unsigned)(blocks < most ? blocks : most), 256, 0, s, x, ld,
                       (int)vocab, rows, c, ignore_index, o, k, dx, ldd);
     return rk_host::launch_status();
   }
-  if (bytes <= kSmallRow) return launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+  const auto ring = [&](auto launch) { return launch(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s); };
+  if (bytes <= kSmallRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8, true>);
   if constexpr (GRAD) {
-    if (bytes <= kMidRow) return launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
-    if (bytes <= kLongRow) return launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
-    return launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+    if (bytes <= kMidRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4, true>);
+    if (bytes <= 7 * chunk_bytes(256)) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, true>);
+    if (bytes <= kLongRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, false>);
+    return ring(launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1, false>);
   } else {
-    return launch_ring<T, POLICY, GRAD, ENT, 256, 4, 3>(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s);
+    return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 4, 3, true>);
   }
 }
 
 template <typename T>
 int logprob_fwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
-                      float inv_temp, int ignore_index, float* logprob, float* entropy, float* stats,
+                      float inv_temp, int ignore_index, float* logprob, float* entropy, float* stats, void* workspace,
                       cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
+  int2* list = static_cast<int2*>(workspace);
   RowOut o = {};
   o.labels = labels;
   o.logprob = logprob;
@@ -1055,15 +1168,15 @@ int logprob_fwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64
   o.stats = reinterpret_cast<float2*>(stats);
   o.status = rk_host::device_status_ptr();
   const rk_policy_terms none = {};
-  if (entropy) return launch_rows<T, false, false, true>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, s);
-  return launch_rows<T, false, false, false>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, s);
+  if (entropy) return launch_rows<T, false, false, true>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, s);
+  return launch_rows<T, false, false, false>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, s);
 }
 
 template <typename T>
 int logprob_bwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
                       float inv_temp, int ignore_index, const float* stats, const float* entropy,
-                      const float* d_logprob, const float* d_entropy, int64_t coef_stride, const float* scale_dev,
-                      void* dlogits, int64_t ldd, cudaStream_t s) {
+                      const float* d_logprob, const float* d_entropy, int64_t coef_stride, float scale_by,
+                      const float* scale_dev, void* dlogits, int64_t ldd, cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
   T* dx = static_cast<T*>(dlogits);
   const float2* st = reinterpret_cast<const float2*>(stats);
@@ -1075,11 +1188,11 @@ int logprob_bwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64
     if (d_entropy)
       rk_host::launch_k(logprob_bwd_kernel<T, true>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
                         (int)segments, labels + r, inv_temp, ignore_index, st + r, entropy + r, d_logprob + r * coef_stride,
-                        d_entropy + r * coef_stride, coef_stride, scale_dev, dx + r * ldd, ldd);
+                        d_entropy + r * coef_stride, coef_stride, scale_by, scale_dev, dx + r * ldd, ldd);
     else
       rk_host::launch_k(logprob_bwd_kernel<T, false>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
                         (int)segments, labels + r, inv_temp, ignore_index, st + r, nullptr, d_logprob + r * coef_stride,
-                        nullptr, coef_stride, scale_dev, dx + r * ldd, ldd);
+                        nullptr, coef_stride, scale_by, scale_dev, dx + r * ldd, ldd);
     const int e = rk_host::launch_status();
     if (e) return e;
   }
@@ -1092,9 +1205,8 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
                  float* coef, void* dlogits, int64_t ldd, void* workspace, cudaStream_t s) {
   float* denom = static_cast<float*>(workspace);
   float2* parts = reinterpret_cast<float2*>(denom + 4);
-  rk_host::launch_k(policy_prepare_kernel, 1, 1024, 0, s, actions, rows, (int)vocab, ignore_index, k, denom);
-  int st = rk_host::launch_status();
-  if (st) return st;
+  int2* list = reinterpret_cast<int2*>(parts + rows);
+  int st = RK_OK;
   if (rows > 0) {
     const T* x = static_cast<const T*>(logits);
     T* dx = static_cast<T*>(dlogits);
@@ -1106,36 +1218,42 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
     o.stats = reinterpret_cast<float2*>(stats);
     o.coef = reinterpret_cast<float2*>(coef);
     o.parts = parts;
-    o.denom = denom;
     o.status = rk_host::device_status_ptr();
     const float t = k.inv_temp;
     if (entropy)
-      st = dx ? launch_rows<T, true, true, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s)
-              : launch_rows<T, true, false, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s);
+      st = dx ? launch_rows<T, true, true, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s)
+              : launch_rows<T, true, false, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s);
     else
-      st = dx ? launch_rows<T, true, true, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s)
-              : launch_rows<T, true, false, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, s);
+      st = dx ? launch_rows<T, true, true, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s)
+              : launch_rows<T, true, false, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s);
     if (st) return st;
   }
-  rk_host::launch_k(policy_reduce_kernel, 1, 1024, 0, s, parts, rows, denom, metrics);
+  // without rows the denominator was not formed: the kernel takes it as 0
+  rk_host::launch_k(policy_reduce_kernel, 1, 1024, 0, s, parts, rows, rows > 0 ? denom : nullptr, metrics);
   return rk_host::launch_status();
 }
 
 }  // namespace
 
+extern "C" int64_t rk_token_logprob_workspace(int64_t rows) {
+  return rows > kFewRows && rows <= kListRows ? rows * 8 : 0;
+}
+
 extern "C" int rk_token_logprob_fwd(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t rows,
                                     float inv_temp, int ignore_index, int dtype, float* logprob, float* entropy,
-                                    float* stats, void* stream) {
+                                    float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!shape_ok(ld, vocab, rows)) return RK_ERR_ARG;
   if (!rk_host::dtype_ok(dtype)) return RK_ERR_DTYPE;
   if (rows == 0) return RK_OK;
-  if (!logits || !labels || !logprob) return RK_ERR_ARG;
-  if (!rk_host::aligned(stats, 8)) return RK_ERR_ALIGN;
+  const int64_t need = rk_token_logprob_workspace(rows);
+  if (!logits || !labels || !logprob || (need && !workspace)) return RK_ERR_ARG;
+  if (workspace_bytes < need) return RK_ERR_WORKSPACE;
+  if (!rk_host::aligned(stats, 8) || !rk_host::aligned(workspace, 8)) return RK_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case RK_F32: return logprob_fwd_typed<float>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, s);
-    case RK_BF16: return logprob_fwd_typed<__nv_bfloat16>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, s);
-    default: return logprob_fwd_typed<__half>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, s);
+    case RK_F32: return logprob_fwd_typed<float>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, workspace, s);
+    case RK_BF16: return logprob_fwd_typed<__nv_bfloat16>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, workspace, s);
+    default: return logprob_fwd_typed<__half>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, logprob, entropy, stats, workspace, s);
   }
 }
 
@@ -1151,14 +1269,14 @@ extern "C" int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t voca
   if (!rk_host::aligned(stats, 8)) return RK_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case RK_F32: return logprob_bwd_typed<float>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, scale_dev, dlogits, ldd, s);
-    case RK_BF16: return logprob_bwd_typed<__nv_bfloat16>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, scale_dev, dlogits, ldd, s);
-    default: return logprob_bwd_typed<__half>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, scale_dev, dlogits, ldd, s);
+    case RK_F32: return logprob_bwd_typed<float>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, 1.f, scale_dev, dlogits, ldd, s);
+    case RK_BF16: return logprob_bwd_typed<__nv_bfloat16>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, 1.f, scale_dev, dlogits, ldd, s);
+    default: return logprob_bwd_typed<__half>(logits, ld, vocab, labels, rows, inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, 1.f, scale_dev, dlogits, ldd, s);
   }
 }
 
-// Four scalars and the rows' loss terms.
-extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 8; }
+// Four scalars, the rows' loss terms and room for their list.
+extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 16; }
 
 extern "C" int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* actions, int64_t rows,
                               int ignore_index, int dtype, const rk_policy_terms* terms, float* logprob, float* kl,
@@ -1179,9 +1297,36 @@ extern "C" int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, con
   }
 }
 
+namespace {
+
+template <typename T>
+int preference_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t pairs, int64_t length,
+                     int ignore_index, int dtype, const rk_preference_terms& k, float* logprob, float* rewards, float* loss,
+                     float* stats, float* coef, void* dlogits, int64_t ldd, void* workspace, cudaStream_t s) {
+  const T* x = static_cast<const T*>(logits);
+  float2* st = reinterpret_cast<float2*>(stats);
+  const int64_t rows = 2 * pairs * length;
+  float* pair_loss = static_cast<float*>(workspace);
+  int e = rows ? logprob_fwd_typed<T>(logits, ld, vocab, labels, rows, k.inv_temp, ignore_index, logprob, nullptr, stats,
+                                        pair_loss + ((pairs + 3) & ~(int64_t)3), s)
+               : RK_OK;
+  if (e) return e;
+  rk_host::launch_k(preference_pair_kernel<T>, (unsigned)pairs, 256, 0, s, x, ld, labels, pairs, length, (int)vocab,
+                    ignore_index, k, st, rewards, pair_loss, loss, coef);
+  if ((e = rk_host::launch_status())) return e;
+  if (pairs > 1) {  // a single pair's loss is the mean already
+    rk_host::launch_k(preference_reduce_kernel, 1, 256, 0, s, pair_loss, pairs, loss);
+    if ((e = rk_host::launch_status())) return e;
+  }
+  if (!dlogits || !rows) return RK_OK;
+  return logprob_bwd_typed<T>(logits, ld, vocab, labels, rows, k.inv_temp, ignore_index, stats, nullptr, coef, nullptr, 1,
+                              k.grad_scale, k.grad_scale_dev, dlogits, ldd, s);
+}
+
+}  // namespace
+
 extern "C" int64_t rk_preference_workspace(int64_t pairs, int64_t length) {
-  (void)length;
-  return 16 + (pairs > 0 ? pairs : 0) * 4;
+  return pairs > 0 && length >= 0 ? 16 + pairs * 4 + rk_token_logprob_workspace(2 * pairs * length) : 0;
 }
 
 extern "C" int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* labels, int64_t pairs,
@@ -1189,7 +1334,7 @@ extern "C" int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab,
                                   float* logprob, float* rewards, float* loss, float* stats, float* coef,
                                   void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes,
                                   void* stream) {
-  if (pairs < 1 || length < 0 || length >= (1ll << 31) || pairs >= (1ll << 31) || !shape_ok(ld, vocab, 2 * pairs * length) ||
+  if (pairs < 1 || length < 0 || length >= (1ll << 30) || pairs >= (1ll << 31) || !shape_ok(ld, vocab, 2 * pairs * length) ||
       !terms || !rewards || !loss || !workspace || terms->kind < RK_PREF_SIGMOID || terms->kind > RK_PREF_SQUARED ||
       (dlogits && ldd < vocab))
     return RK_ERR_ARG;
@@ -1197,19 +1342,11 @@ extern "C" int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab,
   if (rows > 0 && (!logits || !labels || !logprob || !stats || !coef)) return RK_ERR_ARG;
   if (!rk_host::dtype_ok(dtype)) return RK_ERR_DTYPE;
   if (workspace_bytes < rk_preference_workspace(pairs, length)) return RK_ERR_WORKSPACE;
-  if (!rk_host::aligned(workspace, 16) || !rk_host::aligned(stats, 8) || !rk_host::aligned(coef, 8)) return RK_ERR_ALIGN;
+  if (!rk_host::aligned(workspace, 16) || !rk_host::aligned(stats, 8)) return RK_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* scale = static_cast<float*>(workspace);
-  float* pair_loss = scale + 4;
-  int st = rk_token_logprob_fwd(logits, ld, vocab, labels, rows, terms->inv_temp, ignore_index, dtype, logprob, nullptr,
-                                stats, stream);
-  if (st) return st;
-  rk_host::launch_k(preference_pair_kernel, (unsigned)pairs, 256, 0, s, labels, pairs, length, (int)vocab, ignore_index, *terms,
-                    logprob, rewards, pair_loss, coef);
-  if ((st = rk_host::launch_status())) return st;
-  rk_host::launch_k(preference_reduce_kernel, 1, 256, 0, s, pair_loss, pairs, *terms, loss, scale);
-  if ((st = rk_host::launch_status())) return st;
-  if (!dlogits) return RK_OK;
-  return rk_token_logprob_bwd(logits, ld, vocab, labels, rows, terms->inv_temp, ignore_index, dtype, stats, nullptr,
-                              coef, nullptr, 1, scale, dlogits, ldd, stream);
+  switch (dtype) {
+    case RK_F32: return preference_typed<float>(logits, ld, vocab, labels, pairs, length, ignore_index, dtype, *terms, logprob, rewards, loss, stats, coef, dlogits, ldd, workspace, s);
+    case RK_BF16: return preference_typed<__nv_bfloat16>(logits, ld, vocab, labels, pairs, length, ignore_index, dtype, *terms, logprob, rewards, loss, stats, coef, dlogits, ldd, workspace, s);
+    default: return preference_typed<__half>(logits, ld, vocab, labels, pairs, length, ignore_index, dtype, *terms, logprob, rewards, loss, stats, coef, dlogits, ldd, workspace, s);
+  }
 }

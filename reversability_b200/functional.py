@@ -7,6 +7,8 @@ CUDA (the reference's error convention, kernels.py:59-60, kernels_v3.py:54-57).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -16,7 +18,7 @@ _TC_DTYPES = (torch.bfloat16, torch.float16)
 
 def require_cuda(*tensors: torch.Tensor, what: str = "librevk kernels") -> None:
     for t in tensors:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise ValueError(f"{what} require CUDA tensors; no CPU fallback exists")
 
 
@@ -602,10 +604,12 @@ def token_rows(logits: torch.Tensor, labels: torch.Tensor, name: str = "labels")
     require_cuda(logits, labels)
     if logits.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
-    if labels.dtype != torch.int64 or labels.device != logits.device or logits.dim() < 1 or \
+    if labels.dtype is not torch.int64 or labels.get_device() != logits.get_device() or logits.dim() < 1 or \
             labels.shape != logits.shape[:-1]:
         raise ValueError(f"{name} must be int64 on the logits' device with shape {tuple(logits.shape[:-1])}")
     V = logits.shape[-1]
+    if V and logits.is_contiguous():
+        return labels.numel(), V, V, labels if labels.is_contiguous() else labels.contiguous()
     if V < 1 or (V > 1 and logits.stride(-1) != 1):
         raise ValueError("logits must have a non-empty, unit-stride last dimension")
     rows, ld = 1, None
@@ -635,9 +639,9 @@ def row_values(t: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.T
     """An fp32 contiguous array of one value a row (None passes)."""
     if t is None:
         return None
-    if t.device != like.device or t.shape != like.shape:
+    if t.get_device() != like.get_device() or t.shape != like.shape:
         raise ValueError(f"{name} must be on the logits' device with shape {tuple(like.shape)}")
-    return t.detach().float().contiguous()
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
 
 
 def device_scalar(t, device, name: str) -> torch.Tensor | None:
@@ -656,9 +660,11 @@ def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, temperature: f
     logprob = torch.empty(labels.shape, device=logits.device, dtype=torch.float32)
     h = torch.empty_like(logprob) if entropy else None
     stats = torch.empty((rows, 2), device=logits.device, dtype=torch.float32) if want_stats else None
+    n_ws = _lib.lib().rk_token_logprob_workspace(rows)
+    ws = torch.empty(n_ws, device=logits.device, dtype=torch.uint8) if n_ws else None
     _lib.call("rk_token_logprob_fwd", logits.data_ptr(), ld, V, labels.data_ptr(), rows, 1.0 / temperature,
-              int(ignore_index), _lib.code(logits.dtype), logprob.data_ptr(), _lib.ptr(h), _lib.ptr(stats),
-              _lib.stream_ptr())
+              int(ignore_index), _lib.code(logits.dtype), logprob.data_ptr(), _lib.ptr(h), _lib.ptr(stats), _lib.ptr(ws),
+              n_ws, _lib.stream_ptr())
     return logprob, h, stats
 
 
@@ -689,6 +695,16 @@ def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld:
     return out, token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
 
 
+@functools.lru_cache(maxsize=64)
+def _policy_workspace(rows: int) -> int:
+    return _lib.lib().rk_policy_workspace(rows)
+
+
+@functools.lru_cache(maxsize=64)
+def _preference_workspace(pairs: int, length: int) -> int:
+    return -(-_lib.lib().rk_preference_workspace(pairs, length) // 16) * 16
+
+
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
                 ref_logprobs: torch.Tensor | None = None, weights: torch.Tensor | None = None,
                 clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
@@ -703,37 +719,42 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     old = row_values(old_logprobs, actions, "old_logprobs")
     ref = row_values(ref_logprobs, actions, "ref_logprobs")
     w = row_values(weights, actions, "weights")
-    lead = advantages.dim()
-    if advantages.device != dev or lead > actions.dim() or advantages.shape != actions.shape[:lead]:
+    lead, group = advantages.dim(), 1
+    if advantages.get_device() != actions.get_device() or advantages.shape != actions.shape[:lead]:
         raise ValueError("advantages must be on the logits' device with the shape of actions or of its leading "
                          "dimensions")
-    group = max(1, actions.shape[lead:].numel())
-    adv = advantages.detach().float().contiguous()
+    if lead < actions.dim():
+        group = max(1, actions.shape[lead:].numel())
+    adv = row_values(advantages, advantages, "advantages")
     denominator = device_scalar(denominator, dev, "denominator")
     grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
-    n_ws = _lib.lib().rk_policy_workspace(rows) // 4
-    # one allocation for all, the pairs first (they are 8-byte aligned)
-    per_row = [2 * want_coef, 2 * want_coef, 1, int(ref is not None), int(entropy or entropy_coef != 0)]
-    buf = torch.empty(n_ws + 4 + rows * sum(per_row), device=dev, dtype=torch.float32)
-    ws, metrics, *parts = buf.split([n_ws, 4, *(rows * n for n in per_row)])
-    stats, coef, logprob, kl, h = (p if n else None for p, n in zip(parts, per_row))
+    want_h = entropy or entropy_coef != 0
+    # two allocations: metrics, workspace, and the pairs (8-byte aligned) in one, the values per token in the other
+    n_ws = _policy_workspace(rows)
+    aux = torch.empty(4 + n_ws // 4 + (4 * rows if want_coef else 0), device=dev, dtype=torch.float32)
+    at = aux.data_ptr()
+    ws, pairs = at + 16, at + 16 + n_ws
+    stats = coef = None
+    if want_coef:
+        stats, coef = aux[4 + n_ws // 4:].view(2, 2 * rows).unbind()
+    per_token = torch.empty((1 + (ref is not None) + want_h, *actions.shape), device=dev, dtype=torch.float32).unbind()
+    logprob, kl, h = per_token[0], per_token[1] if ref is not None else None, per_token[-1] if want_h else None
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
-    terms = _lib.PolicyTerms(old.data_ptr(), adv.data_ptr(), _lib.ptr(ref), _lib.ptr(w), _lib.ptr(denominator),
-                             _lib.ptr(grad_scale_dev), group, clip_low, clip_high, kl_coef, entropy_coef,
-                             1.0 / temperature, grad_scale)
+    terms = _lib.POLICY_TERMS.pack(old.data_ptr(), adv.data_ptr(), _lib.ptr(ref) or 0, _lib.ptr(w) or 0,
+                                   _lib.ptr(denominator) or 0, _lib.ptr(grad_scale_dev) or 0, group, clip_low, clip_high,
+                                   kl_coef, entropy_coef, 1.0 / temperature, grad_scale)
     _lib.call("rk_policy_loss", logits.data_ptr(), ld, V, actions.data_ptr(), rows, int(ignore_index),
-              _lib.code(logits.dtype), _lib.ctypes.byref(terms), logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h),
-              metrics.data_ptr(), _lib.ptr(stats), _lib.ptr(coef), _lib.ptr(dlogits), ldd, ws.data_ptr(), n_ws * 4,
+              _lib.code(logits.dtype), terms, logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h), at,
+              pairs if want_coef else None, pairs + 8 * rows if want_coef else None, _lib.ptr(dlogits), ldd, ws, n_ws,
               _lib.stream_ptr())
-    shaped = (t if t is None else t.view(actions.shape) for t in (logprob, kl, h))
-    return metrics, *shaped, dlogits, stats, coef
+    return aux[:4], logprob, kl, h, dlogits, stats, coef
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, kind: str,
                     beta: float, label_smoothing: float = 0.0, average: bool = False, temperature: float = 1.0,
                     ignore_index: int = -100, grad_scale: float = 1.0, grad_scale_dev: torch.Tensor | None = None,
                     want_grad: bool = True, out: torch.Tensor | None = None):
-    """rk_preference_loss: (loss [1], logprob, rewards [2 * pairs], dlogits or None, stats, coef) for logits
+    """rk_preference_loss: (loss, logprob, rewards [2 * pairs], dlogits or None, stats, coef) for logits
     [2 * pairs, length, V], chosen sequences first."""
     if logits.dim() != 3 or logits.shape[0] % 2 or logits.shape[0] == 0:
         raise ValueError("preference logits must be [2 * pairs, length, vocabulary], chosen sequences first")
@@ -744,14 +765,17 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     seqs, length = labels.shape
     ref = row_values(ref_logprobs, labels, "ref_logprobs")
     grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
-    n_ws = -(-_lib.lib().rk_preference_workspace(seqs // 2, length) // 16) * 4
-    buf = torch.empty(n_ws + 4 + 4 * rows + seqs, device=dev, dtype=torch.float32)  # one allocation for all
-    ws, loss, stats, logprob, coef, rewards = buf.split([n_ws, 4, 2 * rows, rows, rows, seqs])
+    n_ws = _preference_workspace(seqs // 2, length)
+    # two allocations: loss, workspace, statistics and factors in one, what is returned per token and sequence apart
+    aux = torch.empty(4 + n_ws // 4 + 3 * rows, device=dev, dtype=torch.float32)
+    logprob = torch.empty(labels.shape, device=dev, dtype=torch.float32)
+    rewards = torch.empty(seqs, device=dev, dtype=torch.float32)
+    stats, coef = aux[4 + n_ws // 4:].split([2 * rows, rows])
+    at = aux.data_ptr()
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
-    terms = _lib.PreferenceTerms(_lib.ptr(ref), _lib.ptr(grad_scale_dev), beta, label_smoothing, 1.0 / temperature,
-                                 grad_scale, _lib.PREFERENCE_KINDS[kind], int(average))
+    terms = _lib.PREFERENCE_TERMS.pack(_lib.ptr(ref) or 0, _lib.ptr(grad_scale_dev) or 0, beta, label_smoothing,
+                                       1.0 / temperature, grad_scale, _lib.PREFERENCE_KINDS[kind], int(average))
     _lib.call("rk_preference_loss", logits.data_ptr(), ld, V, labels.data_ptr(), seqs // 2, length, int(ignore_index),
-              _lib.code(logits.dtype), _lib.ctypes.byref(terms), logprob.data_ptr(), rewards.data_ptr(),
-              loss.data_ptr(), stats.data_ptr(), coef.data_ptr(), _lib.ptr(dlogits), ldd, ws.data_ptr(), n_ws * 4,
-              _lib.stream_ptr())
-    return loss, logprob.view(labels.shape), rewards, dlogits, stats, coef
+              _lib.code(logits.dtype), terms, logprob.data_ptr(), rewards.data_ptr(), at,
+              stats.data_ptr(), coef.data_ptr(), _lib.ptr(dlogits), ldd, at + 16, n_ws, _lib.stream_ptr())
+    return aux[0], logprob, rewards, dlogits, stats, coef

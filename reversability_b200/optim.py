@@ -27,28 +27,22 @@ class _Launch:
     def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype):
         self.index, self.bits, self.p_dtype, self.g_dtype = index, bits, p_dtype, g_dtype
         self.p_code, self.g_code = _lib.code(p_dtype), _lib.code(g_dtype)
-        self.entries = []  # (parameter, its state, exp_avg, exp_avg_sq, elements)
-        self.table = None
+        self.entries = []  # (parameter, its state, exp_avg, exp_avg_sq, elements, place among all parameters)
+        self.flat = []
 
-    def add(self, p: torch.Tensor, state: dict) -> None:
+    def add(self, p: torch.Tensor, g: torch.Tensor, state: dict, place: int) -> None:
         m, v = state["exp_avg"], state["exp_avg_sq"]
         want = (torch.int8, torch.uint8) if self.bits == 8 else (torch.float32, torch.float32)
         if (m.dtype, v.dtype) != want or m.numel() != p.numel() or v.numel() != p.numel() or \
                 not (m.is_contiguous() and v.is_contiguous()):
             raise ValueError(f"{self.bits}-bit moments must be contiguous {want[0]} and {want[1]} of the parameter's size")
-        self.entries.append((p, state, m, v, p.numel()))
+        scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if self.bits == 8 else (0, 0)
+        self.entries.append((p, state, m, v, p.numel(), place))
+        self.flat += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), *scales, p.numel())
 
     def finish(self) -> "_Launch":
-        flat = []
-        for p, state, m, v, n in self.entries:
-            scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if self.bits == 8 else (0, 0)
-            flat += (0, 0, m.data_ptr(), v.data_ptr(), *scales, n)
-        self.table = (ctypes.c_uint64 * len(flat))(*flat)
+        self.table = (ctypes.c_uint64 * len(self.flat))(*self.flat)
         return self
-
-
-def _kind(found) -> tuple:
-    return found[0], str(found[1].dtype), str(found[2].dtype)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -76,7 +70,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _reset(self) -> None:
         self._launches = None  # the last step's plan
-        self._mixed = False    # whether a group's tensors are of several types
+        self._idle = []        # (place, parameter) outside it
         self._coded = None     # parameters with 8-bit moments and their table
         self._lr = {}          # group index -> the learning rate its device scalars hold
 
@@ -168,36 +162,58 @@ class AdamW(torch.optim.Optimizer):
         self._reset()
 
     def _plan(self, found) -> list[_Launch]:
-        """The launches for (group index, parameter, gradient) triples."""
+        """The launches for (group index, parameter, gradient, place) tuples."""
         launches = {}
-        for index, p, g in found:
-            if p.dtype not in _lib.DTYPE_CODE or g.dtype not in _lib.DTYPE_CODE or not p.is_contiguous() or \
-                    g.numel() != p.numel():
-                raise ValueError("AdamW parameters must be contiguous fp32, bf16 or fp16 with gradients of their size")
+        for index, p, g, i in found:
+            if p.dtype not in _lib.DTYPE_CODE or not p.is_contiguous():
+                raise ValueError("AdamW parameters must be contiguous fp32, bf16 or fp16")
             bits = self.param_groups[index]["state_bits"]
             key = index, p.dtype, g.dtype
             if key not in launches:
                 launches[key] = _Launch(index, bits, p.dtype, g.dtype)
-            launches[key].add(p, self._moments_of(p, bits))
+            launches[key].add(p, g, self._moments_of(p, bits), i)
         return [launch.finish() for launch in launches.values()]
 
-    def _fill(self, launches, found) -> bool:
-        """Writes the addresses of parameters and gradients into a plan's tables; False if the plan does not fit
-        (another set of gradients, other types or sizes, moments replaced)."""
-        if sum(len(launch.entries) for launch in launches) != len(found):
-            return False
-        it = iter(found)
+    def _refill(self, launches, grads) -> bool:
+        """Writes the addresses of parameters and gradients into the last plan's tables; False if the plan does not fit
+        (another set of gradients, other types or sizes, moments replaced, a gradient that needs a copy)."""
+        for i, p in self._idle:
+            if (p.grad if grads is None else grads[i]) is not None and p.numel():
+                return False
         for launch in launches:
             table, at, p_dtype, g_dtype = launch.table, 0, launch.p_dtype, launch.g_dtype
-            for (p, state, m, v, n), (_, q, g) in zip(launch.entries, it):
-                if q is not p or p.dtype is not p_dtype or g.dtype is not g_dtype or p.numel() != n or \
-                        g.numel() != n or state["exp_avg"] is not m or state["exp_avg_sq"] is not v or \
-                        not p.is_contiguous():
+            for p, state, m, v, n, i in launch.entries:
+                g = p.grad if grads is None else grads[i]  # autograd holds .grad to the parameter's type, shape and device
+                if g is None or g.dtype is not g_dtype or p.dtype is not p_dtype or g.numel() != n or p.numel() != n or \
+                        state["exp_avg"] is not m or state["exp_avg_sq"] is not v or \
+                        not g.is_contiguous() or not p.is_contiguous():
+                    return False
+                if grads is not None and (g.shape != p.shape or g.get_device() != p.get_device()):
                     return False
                 table[at] = p.data_ptr()
                 table[at + 1] = g.data_ptr()
                 at += _FIELDS
         return True
+
+    def _collect(self, grads) -> list:
+        """Checks the gradients and plans the launches for them; returns what has to live until those are queued."""
+        found = []  # (group index, parameter, gradient, the parameter's place among all)
+        self._idle, self._coded = [], None
+        places = itertools.count()
+        for index, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                i = next(places)
+                g = p.grad if grads is None else grads[i]
+                if g is not None and (g.layout is not torch.strided or g.dtype not in _lib.DTYPE_CODE or
+                                      g.get_device() != p.get_device() or g.shape != p.shape):
+                    raise ValueError("AdamW gradients must be dense fp32, bf16 or fp16 in the parameters' shape and "
+                                     "on their device")
+                if g is None or not p.numel():
+                    self._idle.append((i, p))
+                else:
+                    found.append((index, p, g if g.is_contiguous() else g.contiguous(), i))
+        self._launches = self._plan(found)
+        return found
 
     # ---- the step
     @torch.no_grad()
@@ -208,46 +224,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        found = []  # (group index, parameter, gradient) with contiguous gradients, alive until the launches are queued
-        if grads is None:
-            for index, group in enumerate(self.param_groups):
-                for p in group["params"]:
-                    g = p.grad  # autograd holds it to the parameter's type, shape and device
-                    if g is not None and p.numel():
-                        if g.layout is not torch.strided:
-                            raise ValueError("AdamW gradients must be dense")
-                        found.append((index, p, g if g.is_contiguous() else g.contiguous()))
-        else:
-            owners = [(index, p) for index, group in enumerate(self.param_groups) for p in group["params"]]
+        if grads is not None:
             grads = list(grads)
-            if len(grads) != len(owners):
-                raise ValueError(f"grads must hold an entry for each of the {len(owners)} parameters")
-            for (index, p), g in zip(owners, grads):
-                if g is None:
-                    continue
-                if g.layout is not torch.strided or g.dtype not in _lib.DTYPE_CODE or g.device != p.device or \
-                        g.shape != p.shape:
-                    raise ValueError("AdamW gradients must be dense fp32, bf16 or fp16 in the parameters' shape and "
-                                     "on their device")
-                if p.numel():
-                    found.append((index, p, g if g.is_contiguous() else g.contiguous()))
-        if not found:
-            return loss
-        if self._mixed:
-            found.sort(key=_kind)
+            if len(grads) != sum(len(group["params"]) for group in self.param_groups):
+                raise ValueError("grads must hold an entry for each parameter")
+        keep = None
+        if self._launches is None or not self._refill(self._launches, grads):
+            keep = self._collect(grads)
         launches = self._launches
-        if launches is None or not self._fill(launches, found):
-            found.sort(key=_kind)  # stable: by group and types, then in the order of the parameters
-            launches = self._launches = self._plan(found)
-            self._mixed = len({launch.index for launch in launches}) < len(launches)
-            self._coded = None
-            self._fill(launches, found)
+        if not launches:
+            return loss
         stream, lib = _lib.stream_ptr(), _lib.lib()
         partials, parts = None, 0
         if self.max_norm is not None:
             counts = [lib.rk_adamw_multi_parts(len(launch.entries)) for launch in launches]
             parts = sum(counts)
-            partials = torch.empty(parts, device=found[0][1].device, dtype=torch.float32)
+            partials = torch.empty(parts, device=launches[0].entries[0][0].device, dtype=torch.float32)
             at = partials.data_ptr()
             for launch, count in zip(launches, counts):
                 _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
@@ -265,30 +257,36 @@ class AdamW(torch.optim.Optimizer):
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_step", launch.table, len(launch.entries), launch.p_code, launch.g_code, launch.bits,
                       scalars[launch.index].data_ptr(), b1, b2, group["eps"], stream)
+        del keep
         return loss
 
     @torch.no_grad()
     def moments(self, out=None, dtype: torch.dtype = torch.float32) -> list:
         """The values that the 8-bit moments stand for: a pair (exp_avg, exp_avg_sq) for each parameter with 8-bit
         state, in the order of the parameters. out: pairs of contiguous tensors of one type to write into."""
-        if self._coded is None:
-            coded = [(p, self.state[p]) for g in self.param_groups if g["state_bits"] == 8 for p in g["params"]
-                     if p in self.state and "exp_avg" in self.state[p]]
-            self._coded = [(p, st, p.numel()) for p, st in coded], (ctypes.c_uint64 * (_FIELDS * len(coded)))()
-        coded, table = self._coded
+        coded, table = self._coded or ((), None)
+        if table is None or any(st["exp_avg"] is not m for _, st, m, _ in coded):
+            coded = [(p, self.state[p], self.state[p]["exp_avg"], p.numel()) for g in self.param_groups
+                     if g["state_bits"] == 8 for p in g["params"] if p in self.state and "exp_avg" in self.state[p]]
+            flat = []
+            for p, st, m, n in coded:
+                flat += (0, 0, m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
+                         st["exp_avg_sq_scale"].data_ptr(), n)
+            table = (ctypes.c_uint64 * len(flat))(*flat)
+            self._coded = coded, table
         if out is None:
-            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, _, _ in coded]
+            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, *_ in coded]
         if len(out) != len(coded):
             raise ValueError(f"out must hold {len(coded)} pairs")
         if not coded:
             return out
         at, kind = 0, out[0][0].dtype
-        for (p, st, n), (m, v) in zip(coded, out):
+        for (_, _, _, n), (m, v) in zip(coded, out):
             if m.numel() != n or v.numel() != n or m.dtype is not kind or v.dtype is not kind or \
                     not (m.is_cuda and v.is_cuda and m.is_contiguous() and v.is_contiguous()):
                 raise ValueError("out pairs must be contiguous CUDA tensors of one type and the parameters' sizes")
-            table[at:at + _FIELDS] = (m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
-                                      st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr(), n)
+            table[at] = m.data_ptr()
+            table[at + 1] = v.data_ptr()
             at += _FIELDS
         _lib.call("rk_adamw_multi_moments", table, len(coded), _lib.code(kind), _lib.stream_ptr())
         return out

@@ -484,3 +484,36 @@ def test_refusals():
             call()
             print("no refusal:", k)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("shape,dtype", [((1500, 11003), torch.bfloat16), ((20011, 4301), torch.bfloat16),
+                                         ((1025, 6001), torch.float32), ((1300, 61), torch.float16)])
+@pytest.mark.parametrize("mask", ["blocks", "all", "none", "first"])
+def test_many_rows_with_uneven_masks(shape, dtype, mask):
+    """Row counts at which the rows are listed first: every labelled row is done once, every other is left at zero."""
+    rows, vocab = shape
+    x = _logits(rows, vocab, dtype, "padded")
+    y = _labels(rows, vocab, ignored=0.0)
+    if mask == "blocks":  # prompts and padding: runs of ignored rows, one label out of range
+        y[(torch.arange(rows, device=DEV) % 100) < 60] = -100
+        y[99] = vocab
+    elif mask == "all":
+        y[:] = -100
+    elif mask == "first":
+        y[1:] = -100
+    valid = (y >= 0) & (y < vocab)
+    clean = torch.where(valid, y, torch.full_like(y, -100))
+    lp = alignment.token_logprobs(x, y)
+    step = max(1, (1 << 27) // vocab)
+    want = torch.cat([_rows64(x[s:s + step], clean[s:s + step])[1] for s in range(0, rows, step)])
+    assert float((lp.double() - want).abs().max()) <= _lp_tol(x)
+    assert not lp[~valid].any()
+    old = torch.where(valid, lp, torch.zeros_like(lp))
+    r, d = alignment.policy_loss_and_grad(x, y, old, torch.ones_like(lp), grad_scale=float(rows))
+    n = max(int(valid.sum()), 1)
+    assert abs(float(r.loss) + (1.0 if valid.any() else 0.0)) <= 1e-5 and not d[~valid].any()
+    for s in range(0, rows, step):
+        _check_grad(d[s:s + step], x[s:s + step], clean[s:s + step], 1.0,
+                    torch.full((len(d[s:s + step]),), -float(rows) / n, device=DEV))
+    assert torch.equal(r.logprobs, lp) or float((r.logprobs - lp).abs().max()) <= 2e-6 + _lp_tol(x)
+    assert _lib.device_status() == (1 << 2 if mask == "blocks" else 0)
