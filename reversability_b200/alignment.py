@@ -62,12 +62,10 @@ def _check_constants(**tensors) -> None:
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, temperature, ignore_index, entropy):
-        want = ctx.needs_input_grad[0]
-        lp, h, stats = fn.token_logprob_fwd(logits, labels, temperature, ignore_index, entropy, want_stats=want)
-        if want:
-            ctx.save_for_backward(logits, labels, stats, h)
-            ctx.temperature, ctx.ignore_index = temperature, ignore_index
-            ctx.set_materialize_grads(False)
+        lp, h, stats = fn.token_logprob_fwd(logits, labels, temperature, ignore_index, entropy)
+        ctx.save_for_backward(logits, labels, stats, h)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.set_materialize_grads(False)
         return (lp, h) if entropy else lp
 
     @staticmethod
@@ -98,23 +96,23 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
 class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old, adv, args):
-        want = ctx.needs_input_grad[0]
-        metrics, lp, kl, h, _, stats, coef = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=want,
-                                                            **args)
-        loss, clip = metrics[0], metrics[2]
-        if want:
-            ctx.save_for_backward(logits, actions, stats, coef, h if args["entropy_coef"] != 0 else None)
-            ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
+        metrics, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=True, **args)
+        clip = metrics[2]
+        ctx.save_for_backward(logits, actions, pairs, h if args["entropy_coef"] != 0 else None)
+        ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in (lp, kl, h, clip) if t is not None))
-        return loss, lp, kl, h, clip
+        return metrics[0], lp, kl, h, clip
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, *_):
-        logits, actions, stats, coef, h = ctx.saved_tensors
-        flat = coef.view(-1)
-        d = fn.token_logprob_bwd(logits, actions, stats, flat, h, None if h is None else flat[1:], ctx.temperature,
-                                 ctx.ignore_index, coef_stride=2, scale=g.float())
+        if g is None:
+            return None, None, None, None, None
+        logits, actions, pairs, h = ctx.saved_tensors
+        coef = pairs.data_ptr() + 2 * pairs.numel()  # behind the statistics: half of the array's bytes
+        d = fn.token_logprob_bwd_at(logits, actions, pairs.data_ptr(), coef, 2, h, None if h is None else coef + 4,
+                                    ctx.temperature, ctx.ignore_index, g.float())
         return d, None, None, None, None
 
 
@@ -149,6 +147,9 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     _check_constants(old_logprobs=old_logprobs, advantages=advantages, ref_logprobs=ref_logprobs, weights=weights,
                      denominator=denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        metrics, lp, kl, h, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False, **args)
+        return PolicyLoss(metrics[0], lp, kl, h, metrics[2])
     return PolicyLoss(*_Policy.apply(logits, actions, old_logprobs, advantages, args))
 
 
@@ -168,7 +169,7 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logpro
                         entropy, denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
     scale, scale_dev = _scale(grad_scale)
-    metrics, lp, kl, h, d, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, grad_scale=scale,
+    metrics, lp, kl, h, d, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, grad_scale=scale,
                                                  grad_scale_dev=scale_dev, out=out, **args)
     return PolicyLoss(metrics[0], lp, kl, h, metrics[2]), d
 
@@ -176,19 +177,22 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logpro
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, args):
-        loss, lp, rewards, _, stats, coef = fn.preference_loss(logits, labels, ref, want_grad=False, **args)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, labels, stats, coef)
-            ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
+        loss, lp, rewards, _, rows = fn.preference_loss(logits, labels, ref, want_grad=False, **args)
+        ctx.save_for_backward(logits, labels, rows)
+        ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(rewards, lp)
         return loss, rewards, lp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, *_):
-        logits, labels, stats, coef = ctx.saved_tensors
-        d = fn.token_logprob_bwd(logits, labels, stats, coef, temperature=ctx.temperature,
-                                 ignore_index=ctx.ignore_index, scale=g.float())
+        if g is None:
+            return None, None, None, None
+        logits, labels, rows = ctx.saved_tensors
+        coef = rows.data_ptr() + 8 * (rows.numel() // 3)  # behind the statistics
+        d = fn.token_logprob_bwd_at(logits, labels, rows.data_ptr(), coef, 1, None, None, ctx.temperature,
+                                    ctx.ignore_index, g.float())
         return d, None, None, None
 
 
@@ -216,6 +220,9 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     args = _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index)
     _check_constants(ref_logprobs=ref_logprobs)
     fn.require_cuda(logits, labels, ref_logprobs, what="the preference loss")
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        loss, lp, rewards, _, _ = fn.preference_loss(logits, labels, ref_logprobs, want_grad=False, **args)
+        return PreferenceLoss(loss, rewards, lp)
     return PreferenceLoss(*_Preference.apply(logits, labels, ref_logprobs, args))
 
 
@@ -228,7 +235,7 @@ def preference_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, ref_log
     args = _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index)
     fn.require_cuda(logits, labels, ref_logprobs, what="the preference loss")
     scale, scale_dev = _scale(grad_scale)
-    loss, lp, rewards, d, _, _ = fn.preference_loss(logits, labels, ref_logprobs, grad_scale=scale,
+    loss, lp, rewards, d, _ = fn.preference_loss(logits, labels, ref_logprobs, grad_scale=scale,
                                                     grad_scale_dev=scale_dev, out=out, **args)
     return PreferenceLoss(loss, rewards, lp), d
 

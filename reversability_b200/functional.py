@@ -670,15 +670,22 @@ def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, temperature: f
 
 def token_logprob_bwd(logits: torch.Tensor, labels: torch.Tensor, stats: torch.Tensor, d_logprob: torch.Tensor,
                       entropy: torch.Tensor | None = None, d_entropy: torch.Tensor | None = None,
-                      temperature: float = 1.0, ignore_index: int = -100, coef_stride: int = 1,
-                      scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """d loss / d logits (in the logits' dtype, rounded once) from d loss / d logprob and, with `entropy`, d loss /
-    d entropy, times the device scalar `scale`. `out` may be the logits themselves."""
+                      temperature: float = 1.0, ignore_index: int = -100, scale: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """d loss / d logits (in the logits' dtype, rounded once) from contiguous fp32 d loss / d logprob and, with
+    `entropy`, d loss / d entropy, times the device scalar `scale`. `out` may be the logits themselves."""
+    return token_logprob_bwd_at(logits, labels, stats.data_ptr(), d_logprob.data_ptr(), 1, entropy, _lib.ptr(d_entropy),
+                                temperature, ignore_index, scale, out)
+
+
+def token_logprob_bwd_at(logits, labels, stats: int, d_logprob: int, coef_stride: int, entropy, d_entropy: int | None,
+                         temperature, ignore_index, scale, out=None) -> torch.Tensor:
+    """token_logprob_bwd with its row factors given by address (they may be interleaved)."""
     rows, V, ld, labels = token_rows(logits, labels)
     out, ldd = gradient_rows(logits, out, rows, ld)
     _lib.call("rk_token_logprob_bwd", logits.data_ptr(), ld, V, labels.data_ptr(), rows, 1.0 / temperature,
-              int(ignore_index), _lib.code(logits.dtype), stats.data_ptr(), _lib.ptr(entropy), d_logprob.data_ptr(),
-              _lib.ptr(d_entropy), coef_stride, _lib.ptr(scale), out.data_ptr(), ldd, _lib.stream_ptr())
+              ignore_index, _lib.code(logits.dtype), stats, _lib.ptr(entropy), d_logprob, d_entropy, coef_stride,
+              _lib.ptr(scale), out.data_ptr(), ldd, _lib.stream_ptr())
     return out
 
 
@@ -712,8 +719,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
                 denominator: torch.Tensor | None = None, grad_scale: float = 1.0,
                 grad_scale_dev: torch.Tensor | None = None, want_grad: bool = True, want_coef: bool = False,
                 out: torch.Tensor | None = None):
-    """rk_policy_loss: (metrics [4], logprob, kl or None, entropy or None, dlogits or None, stats or None, coef or
-    None). advantages has the shape of actions or of its leading dimensions (one a sequence)."""
+    """rk_policy_loss: (metrics [4], logprob, kl or None, entropy or None, dlogits or None, pairs or None), pairs
+    [2, rows, 2] being the rows' statistics and factors for the backward. advantages has the shape of actions or of its leading dimensions (one a sequence)."""
     rows, V, ld, actions = token_rows(logits, actions, "actions")
     dev = logits.device
     old = row_values(old_logprobs, actions, "old_logprobs")
@@ -733,10 +740,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     n_ws = _policy_workspace(rows)
     aux = torch.empty(4 + n_ws // 4 + (4 * rows if want_coef else 0), device=dev, dtype=torch.float32)
     at = aux.data_ptr()
-    ws, pairs = at + 16, at + 16 + n_ws
-    stats = coef = None
-    if want_coef:
-        stats, coef = aux[4 + n_ws // 4:].view(2, 2 * rows).unbind()
+    ws, pairs_at = at + 16, at + 16 + n_ws
     per_token = torch.empty((1 + (ref is not None) + want_h, *actions.shape), device=dev, dtype=torch.float32).unbind()
     logprob, kl, h = per_token[0], per_token[1] if ref is not None else None, per_token[-1] if want_h else None
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
@@ -745,17 +749,17 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
                                    kl_coef, entropy_coef, 1.0 / temperature, grad_scale)
     _lib.call("rk_policy_loss", logits.data_ptr(), ld, V, actions.data_ptr(), rows, int(ignore_index),
               _lib.code(logits.dtype), terms, logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h), at,
-              pairs if want_coef else None, pairs + 8 * rows if want_coef else None, _lib.ptr(dlogits), ldd, ws, n_ws,
+              pairs_at if want_coef else None, pairs_at + 8 * rows if want_coef else None, _lib.ptr(dlogits), ldd, ws, n_ws,
               _lib.stream_ptr())
-    return aux[:4], logprob, kl, h, dlogits, stats, coef
+    return aux[:4], logprob, kl, h, dlogits, aux[4 + n_ws // 4:] if want_coef else None
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, kind: str,
                     beta: float, label_smoothing: float = 0.0, average: bool = False, temperature: float = 1.0,
                     ignore_index: int = -100, grad_scale: float = 1.0, grad_scale_dev: torch.Tensor | None = None,
                     want_grad: bool = True, out: torch.Tensor | None = None):
-    """rk_preference_loss: (loss, logprob, rewards [2 * pairs], dlogits or None, stats, coef) for logits
-    [2 * pairs, length, V], chosen sequences first."""
+    """rk_preference_loss: (loss, logprob, rewards [2 * pairs], dlogits or None, rows' statistics [2 * rows] and factors
+    [rows] in one array) for logits [2 * pairs, length, V], chosen sequences first."""
     if logits.dim() != 3 or logits.shape[0] % 2 or logits.shape[0] == 0:
         raise ValueError("preference logits must be [2 * pairs, length, vocabulary], chosen sequences first")
     if kind not in _lib.PREFERENCE_KINDS:
@@ -770,12 +774,12 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     aux = torch.empty(4 + n_ws // 4 + 3 * rows, device=dev, dtype=torch.float32)
     logprob = torch.empty(labels.shape, device=dev, dtype=torch.float32)
     rewards = torch.empty(seqs, device=dev, dtype=torch.float32)
-    stats, coef = aux[4 + n_ws // 4:].split([2 * rows, rows])
     at = aux.data_ptr()
+    stats_at = at + 16 + n_ws
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
     terms = _lib.PREFERENCE_TERMS.pack(_lib.ptr(ref) or 0, _lib.ptr(grad_scale_dev) or 0, beta, label_smoothing,
                                        1.0 / temperature, grad_scale, _lib.PREFERENCE_KINDS[kind], int(average))
     _lib.call("rk_preference_loss", logits.data_ptr(), ld, V, labels.data_ptr(), seqs // 2, length, int(ignore_index),
               _lib.code(logits.dtype), terms, logprob.data_ptr(), rewards.data_ptr(), at,
-              stats.data_ptr(), coef.data_ptr(), _lib.ptr(dlogits), ldd, at + 16, n_ws, _lib.stream_ptr())
-    return aux[0], logprob, rewards, dlogits, stats, coef
+              stats_at, stats_at + 8 * rows, _lib.ptr(dlogits), ldd, at + 16, n_ws, _lib.stream_ptr())
+    return aux[0], logprob, rewards, dlogits, aux[4 + n_ws // 4:]
