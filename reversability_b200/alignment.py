@@ -96,13 +96,13 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
 class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old, adv, args):
-        metrics, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=True, **args)
-        clip = metrics[2]
+        loss, clip, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=True,
+                                                         **args)
         ctx.save_for_backward(logits, actions, pairs, h if args["entropy_coef"] != 0 else None)
         ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in (lp, kl, h, clip) if t is not None))
-        return metrics[0], lp, kl, h, clip
+        return loss, lp, kl, h, clip
 
     @staticmethod
     @once_differentiable
@@ -148,8 +148,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
                      denominator=denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
     if not (logits.requires_grad and torch.is_grad_enabled()):
-        metrics, lp, kl, h, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False, **args)
-        return PolicyLoss(metrics[0], lp, kl, h, metrics[2])
+        loss, clip, lp, kl, h, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False, **args)
+        return PolicyLoss(loss, lp, kl, h, clip)
     return PolicyLoss(*_Policy.apply(logits, actions, old_logprobs, advantages, args))
 
 
@@ -169,9 +169,9 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logpro
                         entropy, denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
     scale, scale_dev = _scale(grad_scale)
-    metrics, lp, kl, h, d, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, grad_scale=scale,
+    loss, clip, lp, kl, h, d, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, grad_scale=scale,
                                                  grad_scale_dev=scale_dev, out=out, **args)
-    return PolicyLoss(metrics[0], lp, kl, h, metrics[2]), d
+    return PolicyLoss(loss, lp, kl, h, clip), d
 
 
 class _Preference(torch.autograd.Function):

@@ -451,15 +451,21 @@ __device__ __forceinline__ PolicyRow policy_row(const rk_policy_terms& k, const 
   return o;
 }
 
-__device__ double block_sum(double v) {
-  __shared__ double red[32];
+// The sums of two values over the CTA, in a fixed order.
+__device__ double2 block_sum2(double a, double b) {
+  __shared__ double2 red[32];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = {a, b};
   __syncthreads();
-  double s = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += red[w];
-  __syncthreads();
+  double2 s = {0.0, 0.0};
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+    s.x += red[w].x;
+    s.y += red[w].y;
+  }
   return s;
 }
 
@@ -967,14 +973,13 @@ __global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __res
     a += v.x;
     b += v.y;
   }
-  a = block_sum(a);
-  b = block_sum(b);
+  const double2 sum = block_sum2(a, b);
   if (threadIdx.x == 0) {
     const float d = denom ? *denom : 0.f;
     const double inv = d != 0.f ? 1.0 / d : 0.0;
-    metrics[0] = (float)(a * inv);
+    metrics[0] = (float)(sum.x * inv);
     metrics[1] = d;
-    metrics[2] = (float)(b * inv);
+    metrics[2] = (float)(sum.y * inv);
     metrics[3] = 0.f;
   }
 }
@@ -1008,21 +1013,35 @@ __global__ void __launch_bounds__(256)
                            const float2* __restrict__ stats, float* __restrict__ rewards, float* __restrict__ pair_loss,
                            float* __restrict__ loss, float* __restrict__ coef) {
   pdl_wait();  // inputs are the previous kernel's outputs
+  __shared__ double red[2][8];
   const int64_t pair = blockIdx.x;
+  const int side = threadIdx.x >> 7, lane = threadIdx.x & 31;  // half of the CTA for each sequence
+  const int64_t base = (side * pairs + pair) * length;
+  double g = 0.0, n = 0.0;
+#pragma unroll 4
+  for (int64_t t = threadIdx.x & 127; t < length; t += 128) {
+    const int64_t row = base + t, label = labels[row];
+    if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
+    const float2 st = stats[row];
+    g += gap_term(Dt<T>::to_f(logits[row * ld + label]), st.x, st.y, k.inv_temp, k.ref_logprobs, row);
+    n += 1.0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    g += __shfl_xor_sync(0xffffffffu, g, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (lane == 0) {
+    red[0][threadIdx.x >> 5] = g;
+    red[1][threadIdx.x >> 5] = n;
+  }
+  __syncthreads();
   double gap[2], count[2];
-  for (int side = 0; side < 2; ++side) {
-    const int64_t base = (side * pairs + pair) * length;
-    double g = 0.0, n = 0.0;
-    for (int64_t t = threadIdx.x; t < length; t += blockDim.x) {
-      const int64_t row = base + t, label = labels[row];
-      if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
-      const float2 st = stats[row];
-      g += gap_term(Dt<T>::to_f(logits[row * ld + label]), st.x, st.y, k.inv_temp, k.ref_logprobs, row);
-      n += 1.0;
-    }
-    gap[side] = block_sum(g);
-    count[side] = block_sum(n);
-    if (k.average) gap[side] /= fmax(count[side], 1.0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    gap[i] = (red[0][4 * i] + red[0][4 * i + 1]) + (red[0][4 * i + 2] + red[0][4 * i + 3]);
+    count[i] = (red[1][4 * i] + red[1][4 * i + 1]) + (red[1][4 * i + 2] + red[1][4 * i + 3]);
+    if (k.average) gap[i] /= fmax(count[i], 1.0);
   }
   const PairLoss q = pair_loss_of(k, gap[0], gap[1]);
   if (threadIdx.x == 0) {
@@ -1030,12 +1049,9 @@ __global__ void __launch_bounds__(256)
     rewards[pair] = k.beta * (float)gap[0];
     rewards[pairs + pair] = k.beta * (float)gap[1];
   }
-  for (int side = 0; side < 2; ++side) {
-    const int64_t base = (side * pairs + pair) * length;
-    const float s = (side ? -q.slope : q.slope) / (float)pairs / (k.average ? (float)fmax(count[side], 1.0) : 1.f);
-    for (int64_t t = threadIdx.x; t < length; t += blockDim.x)
-      coef[base + t] = row_kind(labels[base + t], vocab, ignore_index) == ROW_LIVE ? s : 0.f;
-  }
+  const float s = (side ? -q.slope : q.slope) / (float)pairs / (k.average ? (float)fmax(count[side], 1.0) : 1.f);
+  for (int64_t t = threadIdx.x & 127; t < length; t += 128)
+    coef[base + t] = row_kind(labels[base + t], vocab, ignore_index) == ROW_LIVE ? s : 0.f;
 }
 
 // loss = mean of the pair losses.
@@ -1044,7 +1060,7 @@ __global__ void __launch_bounds__(256) preference_reduce_kernel(const float* __r
   pdl_wait();  // inputs are the previous kernel's outputs
   double s = 0.0;
   for (int64_t i = threadIdx.x; i < pairs; i += blockDim.x) s += pair_loss[i];
-  s = block_sum(s);
+  s = block_sum2(s, 0.0).x;
   if (threadIdx.x == 0) *loss = (float)(s / (double)pairs);
 }
 
@@ -1064,13 +1080,17 @@ bool shape_ok(int64_t ld, int64_t vocab, int64_t rows) {
 // The policy loss needs that launch for its denominator anyway; sums alone are worth its 4 us from about 60 us on.
 constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 
-// Row lengths in bytes at which the forms change; 4096 rows of 8192 x 16 bits (16 KB) and 8192 rows of 3000 (6 KB),
-// us, one warp a row / ring of 64 threads: sums 13.0 / 15.1 and 11.4 / 17.3, policy with gradient 44.0 / 35.5 and
-// 32.0 / 38.7 (a warp's second read of its row comes from L2 once 64 rows an SM exceed L1). Rings of 64 / 128 / 256
-// threads with gradient: 35.5 / 39.4 / 49.8 at 16 KB, 49 / 52 / 65 at 24 KB (the last size whose rows fit the first).
-// 256 KB rows (1500 x 131072 x 16 bits) with a ring of 256 threads twice an SM or of 512 once: 178 / 151, as the
-// larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
-constexpr int64_t kWarpRowSum = 20 * 1024, kWarpRowGrad = 8 * 1024;
+// Row lengths in bytes at which the forms change. us, one warp a row / ring of 64 / 128 / 256 threads:
+//   sums, 4096 rows: 22 KB bf16 18.5/19.0/20.5/27.3, 32 KB fp32 22.6/25.1/24.0/26.0, 40 KB fp32 28.6/32.3/28.7/29.9,
+//     48 KB bf16 38.2/36.9/37.4/43.5; 14848 of 100 KB bf16 -/243/241/263; 2047 of 128 KB fp32 -/76/46/43
+//   policy with gradient: 8192 rows of 6 KB bf16 32/39, 4096 of 16 KB 44/35.5/39/50, of 24 KB 72/49/52/65 (a warp's second
+//     read of its row comes from L2 once 64 rows an SM exceed L1)
+// So sums of 16-bit logits take rings of 128 threads eight times an SM (exponentials bound them, and 40 warps hide more),
+// fp32 ones, which HBM bounds, of 256 three times. With fewer rows than four an SM a warp's row takes too long alone, and
+// the larger CTAs are faster (64 rows of 100 KB: 5.5 / 6.6).
+// 256 KB rows (1500 x 131072 x 16 bits) with gradient and a ring of 256 threads twice an SM or of 512 once: 178 / 151, as
+// the larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
+constexpr int64_t kWarpRow = 4 * 1024, kWarpRowSum = 36 * 1024, kWarpRowGrad = 8 * 1024;
 constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256);
 
 int sm_count() {
@@ -1126,7 +1146,7 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
                 const rk_policy_terms& k, T* dx, int64_t ldd, int2* list, float* denom, cudaStream_t s) {
   const float c = inv_temp * kLog2e;
   const int64_t bytes = vocab * (int64_t)sizeof(T);
-  const bool by_warp = bytes <= (GRAD ? kWarpRowGrad : kWarpRowSum);
+  const bool by_warp = bytes <= (rows < 4 * sm_count() ? kWarpRow : GRAD ? kWarpRowGrad : kWarpRowSum);
   o.denom = denom;
   o.sum_here = rows <= kFewRows;
   const bool worth = POLICY || rows * bytes >= kListBytes;
@@ -1151,6 +1171,7 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
     if (bytes <= kLongRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, false>);
     return ring(launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1, false>);
   } else {
+    if (sizeof(T) == 2 && rows >= 4 * sm_count()) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 3, 8, true>);
     return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 4, 3, true>);
   }
 }

@@ -719,7 +719,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
                 denominator: torch.Tensor | None = None, grad_scale: float = 1.0,
                 grad_scale_dev: torch.Tensor | None = None, want_grad: bool = True, want_coef: bool = False,
                 out: torch.Tensor | None = None):
-    """rk_policy_loss: (metrics [4], logprob, kl or None, entropy or None, dlogits or None, pairs or None), pairs
+    """rk_policy_loss: (loss, clip fraction, logprob, kl or None, entropy or None, dlogits or None, pairs or None), pairs
     [2, rows, 2] being the rows' statistics and factors for the backward. advantages has the shape of actions or of its leading dimensions (one a sequence)."""
     rows, V, ld, actions = token_rows(logits, actions, "actions")
     dev = logits.device
@@ -751,7 +751,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
               _lib.code(logits.dtype), terms, logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h), at,
               pairs_at if want_coef else None, pairs_at + 8 * rows if want_coef else None, _lib.ptr(dlogits), ldd, ws, n_ws,
               _lib.stream_ptr())
-    return aux[:4], logprob, kl, h, dlogits, aux[4 + n_ws // 4:] if want_coef else None
+    return aux[0], aux[2], logprob, kl, h, dlogits, aux[4 + n_ws // 4:] if want_coef else None
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, kind: str,

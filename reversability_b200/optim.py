@@ -72,6 +72,8 @@ class AdamW(torch.optim.Optimizer):
         self._launches = None  # the last step's plan
         self._idle = []        # (place, parameter) outside it
         self._coded = None     # parameters with 8-bit moments and their table
+        self._partials = None  # the norm's workspace
+        self._norm_of = None   # the scalars that grad_norm is a view of
         self._lr = {}          # group index -> the learning rate its device scalars hold
 
     def __getstate__(self):
@@ -198,7 +200,7 @@ class AdamW(torch.optim.Optimizer):
     def _collect(self, grads) -> list:
         """Checks the gradients and plans the launches for them; returns what has to live until those are queued."""
         found = []  # (group index, parameter, gradient, the parameter's place among all)
-        self._idle, self._coded = [], None
+        self._idle, self._coded, self._partials = [], None, None
         places = itertools.count()
         for index, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -237,21 +239,24 @@ class AdamW(torch.optim.Optimizer):
         stream, lib = _lib.stream_ptr(), _lib.lib()
         partials, parts = None, 0
         if self.max_norm is not None:
-            counts = [lib.rk_adamw_multi_parts(len(launch.entries)) for launch in launches]
-            parts = sum(counts)
-            partials = torch.empty(parts, device=launches[0].entries[0][0].device, dtype=torch.float32)
+            if self._partials is None:  # as long as the plan: its size depends on the launches alone
+                parts = sum(lib.rk_adamw_multi_parts(len(launch.entries)) for launch in launches)
+                self._partials = torch.empty(parts, device=launches[0].entries[0][0].device, dtype=torch.float32)
+            partials, parts = self._partials, self._partials.numel()
             at = partials.data_ptr()
-            for launch, count in zip(launches, counts):
-                _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
-                at += 4 * count
+            for launch in launches:
+                n = len(launch.entries)
+                _lib.call("rk_adamw_multi_sumsq", launch.table, n, launch.g_code, at, stream)
+                at += 4 * lib.rk_adamw_multi_parts(n)
         scalars = {}
         for index in dict.fromkeys(launch.index for launch in launches):
             group, scalars[index] = self.param_groups[index], self._group_scalars(index)
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_prepare", _lib.ptr(partials), parts, self.max_norm or 0.0, b1, b2,
                       group["weight_decay"], scalars[index].data_ptr(), stream)
-        if self.max_norm is not None:
-            self.grad_norm = scalars[launches[0].index][2]
+        if self.max_norm is not None and self._norm_of is not scalars[launches[0].index]:
+            self._norm_of = scalars[launches[0].index]
+            self.grad_norm = self._norm_of[2]
         for launch in launches:
             group = self.param_groups[launch.index]
             b1, b2 = group["betas"]

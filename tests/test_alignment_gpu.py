@@ -512,8 +512,9 @@ def test_many_rows_with_uneven_masks(shape, dtype, mask):
     r, d = alignment.policy_loss_and_grad(x, y, old, torch.ones_like(lp), grad_scale=float(rows))
     n = max(int(valid.sum()), 1)
     assert abs(float(r.loss) + (1.0 if valid.any() else 0.0)) <= 1e-5 and not d[~valid].any()
+    # the factor at the log-probabilities that the loss itself reports (they may be sums in another order than `lp`)
+    g = -(r.logprobs.double() - old.double()).exp() * (float(rows) / n)
     for s in range(0, rows, step):
-        _check_grad(d[s:s + step], x[s:s + step], clean[s:s + step], 1.0,
-                    torch.full((len(d[s:s + step]),), -float(rows) / n, device=DEV))
+        _check_grad(d[s:s + step], x[s:s + step], clean[s:s + step], 1.0, g[s:s + step])
     assert torch.equal(r.logprobs, lp) or float((r.logprobs - lp).abs().max()) <= 2e-6 + _lp_tol(x)
     assert _lib.device_status() == (1 << 2 if mask == "blocks" else 0)
