@@ -251,6 +251,15 @@ __device__ __forceinline__ bool is_far(const RowSum& a) { return a.s == 0.f || !
 __device__ __forceinline__ float exponent(float x, float c, const RowSum& a, bool far) {
   return far ? (x - a.r) * c : fmaf(x, c, -a.m);
 }
+// The label's log-probability before it is rounded to fp32 (whose steps are 1e-6 at -10): losses are sums of many, in
+// which these roundings would show. With the sum's own c and m, so that their rounding cancels. The exponential unit's
+// results are 5e-8 low on average (5.0e-8 over [-16, -1], 2.2e-8 over [-1, 0], at most 1.4e-7), and a sum meets it again
+// where sums are joined: 8e-8 in all, but for the reference's own term, which is exact.
+constexpr double kUnitLow = 8e-8;
+__device__ __forceinline__ double label_logprob(float x, float c, const RowSum& a, bool far) {
+  const double t = far ? ((double)x - (double)a.r) * (double)c : fma((double)x, (double)c, -(double)a.m);
+  return t * 0.6931471805599453 - (log((double)a.s) + kUnitLow * (1.0 - (double)__fdividef(1.f, a.s)));
+}
 
 // ---------------------------------------------------------------- row gradients
 struct RowGrad {
@@ -313,6 +322,7 @@ struct RowOut {
   float2* stats;   // (r, S), may be NULL
   float2* coef;    // policy only, may be NULL
   float2* parts;   // policy only: (w l, w clipped)
+  float4* fine;    // policy only: (the label's logit, r, S, d(w l) / dlp), for finish_losses
   float* denom;    // policy only: the denominator, or with sum_here where it goes
   bool sum_here;   // few rows: each CTA forms it by itself, which saves a launch
   const int2* list;    // many rows: (row, label) of those with a label, the others behind; else NULL
@@ -419,7 +429,7 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(int64_t rows, int vocab
 
 // ---------------------------------------------------------------- policy loss
 struct PolicyRow {
-  float lp, kl, loss, clipped, g_lp, g_h;  // g_* without the outer scale and inv_temp
+  float kl, loss, slope, clipped, g_lp, g_h;  // slope = dloss / dlp; g_* without the outer scale and inv_temp
 };
 struct PolicyIn {
   float old, adv, ref, w;
@@ -442,13 +452,32 @@ __device__ __forceinline__ PolicyRow policy_row(const rk_policy_terms& k, const 
     kl = em1 - drift;
     dkl = -em1;
   }
-  o.lp = lp;
   o.kl = kl;
+  o.slope = w * ((clipped ? 0.f : -free) + k.kl_coef * dkl);
   o.loss = w * (k.kl_coef * kl - (clipped ? held : free) - k.entropy_coef * entropy);
   o.clipped = clipped ? w : 0.f;
-  o.g_lp = w * inv_d * ((clipped ? 0.f : -free) + k.kl_coef * dkl);
+  o.g_lp = o.slope * inv_d;
   o.g_h = -w * inv_d * k.entropy_coef;
   return o;
+}
+
+// What the reported log-probability was rounded by, times the loss's slope there; nothing for infinite terms.
+__device__ __forceinline__ float loss_rounding(float x, float c, const RowSum& a, bool far, float lp, float slope) {
+  const float more = slope * (float)(label_logprob(x, c, a, far) - (double)lp);
+  return fabsf(more) < INFINITY ? more : 0.f;
+}
+// Adds that to the loss terms of the first-th and every step-th row after it, of this warp. Behind the warp's last row,
+// a row a lane: within the rows, the logarithm in fp64 kept a whole CTA waiting (564 us in place of 544 at 14848 x 50257).
+__device__ __forceinline__ void finish_losses(const RowOut& o, int64_t first, int64_t step, int64_t rows, float c,
+                                              int vocab, int ignore_index) {
+  __syncwarp();
+  for (int64_t i = first + (threadIdx.x & 31) * step; i < rows; i += 32 * step) {
+    const int2 at = o.list ? o.list[i] : make_int2((int)i, checked_label(o.labels[i], vocab, ignore_index));
+    if (at.y < 0) continue;
+    const float4 f = o.fine[at.x];
+    const RowSum a = {f.y, f.y * c, f.z, 0.f};
+    o.parts[at.x].x += loss_rounding(f.x, c, a, is_far(a), o.logprob[at.x], f.w);
+  }
 }
 
 // The sums of two values over the CTA, in a fixed order.
@@ -749,6 +778,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
           g_h = q.g_h;
           if (lane == 0 && rank == 0) {
             o.parts[row] = {q.loss, q.clipped};
+            o.fine[row] = {xl, a.r, a.s, q.slope};
             if (o.kl) o.kl[row] = q.kl;
             if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
           }
@@ -809,6 +839,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
         }
       }
     }
+    if (POLICY && warp == 0 && rank == 0) finish_losses(o, first, step, rows, c, vocab, ignore_index);
   }
   __syncwarp();
   if (cluster > 1) cluster_sync();  // no CTA ends while another may still send to it
@@ -870,9 +901,10 @@ __global__ void __launch_bounds__(256)
     const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
     float g_lp = 0.f, g_h = 0.f;
     if constexpr (POLICY) {
-      const PolicyRow q = policy_row(k, in, lp, h, denom != 0.f ? 1.f / denom : 0.f);
+      PolicyRow q = policy_row(k, in, lp, h, denom != 0.f ? 1.f / denom : 0.f);
       g_lp = q.g_lp;
       g_h = q.g_h;
+      q.loss += loss_rounding(xl, c, a, far, lp, q.slope);
       if (lane == 0) {
         o.parts[row] = {q.loss, q.clipped};
         if (o.kl) o.kl[row] = q.kl;
@@ -985,11 +1017,6 @@ __global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __res
 }
 
 // ---------------------------------------------------------------- preference loss
-// A sequence's gap is a sum of hundreds of differences, each small against its two log-probabilities: it is formed
-// in fp64 from the row's statistics, not from the log-probabilities rounded to fp32.
-__device__ __forceinline__ double gap_term(float xl, float r, float s, float inv_temp, const float* ref, int64_t row) {
-  return ((double)xl - (double)r) * (double)inv_temp - log((double)s) - (ref ? (double)ref[row] : 0.0);
-}
 struct PairLoss {
   float loss, slope;  // slope = dloss / d gap_chosen
 };
@@ -1006,6 +1033,8 @@ __device__ __forceinline__ PairLoss pair_loss_of(const rk_preference_terms& k, d
 }
 
 // After the rows' statistics: one CTA per pair forms the two gaps in a fixed order, the pair's loss and its rows' factors.
+// A gap is a sum of hundreds of differences, each small against its two log-probabilities: it is formed in fp64 from the
+// rows' statistics, not from the log-probabilities rounded to fp32.
 template <typename T>
 __global__ void __launch_bounds__(256)
     preference_pair_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, int64_t pairs,
@@ -1017,13 +1046,15 @@ __global__ void __launch_bounds__(256)
   const int64_t pair = blockIdx.x;
   const int side = threadIdx.x >> 7, lane = threadIdx.x & 31;  // half of the CTA for each sequence
   const int64_t base = (side * pairs + pair) * length;
+  const float c = k.inv_temp * kLog2e;
   double g = 0.0, n = 0.0;
 #pragma unroll 4
   for (int64_t t = threadIdx.x & 127; t < length; t += 128) {
     const int64_t row = base + t, label = labels[row];
     if (row_kind(label, vocab, ignore_index) != ROW_LIVE) continue;
     const float2 st = stats[row];
-    g += gap_term(Dt<T>::to_f(logits[row * ld + label]), st.x, st.y, k.inv_temp, k.ref_logprobs, row);
+    const RowSum a = {st.x, st.x * c, st.y, 0.f};
+    g += label_logprob(Dt<T>::to_f(logits[row * ld + label]), c, a, is_far(a)) - (k.ref_logprobs ? (double)k.ref_logprobs[row] : 0.0);
     n += 1.0;
   }
 #pragma unroll
@@ -1171,7 +1202,9 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
     if (bytes <= kLongRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, false>);
     return ring(launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1, false>);
   } else {
-    if (sizeof(T) == 2 && rows >= 4 * sm_count()) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 3, 8, true>);
+    if constexpr (sizeof(T) == 2) {
+      if (rows >= 4 * sm_count()) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 3, 8, true>);
+    }
     return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 4, 3, true>);
   }
 }
@@ -1225,7 +1258,8 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
                  const rk_policy_terms& k, float* logprob, float* kl, float* entropy, float* metrics, float* stats,
                  float* coef, void* dlogits, int64_t ldd, void* workspace, cudaStream_t s) {
   float* denom = static_cast<float*>(workspace);
-  float2* parts = reinterpret_cast<float2*>(denom + 4);
+  float4* fine = reinterpret_cast<float4*>(denom + 4);
+  float2* parts = reinterpret_cast<float2*>(fine + rows);
   int2* list = reinterpret_cast<int2*>(parts + rows);
   int st = RK_OK;
   if (rows > 0) {
@@ -1239,6 +1273,7 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
     o.stats = reinterpret_cast<float2*>(stats);
     o.coef = reinterpret_cast<float2*>(coef);
     o.parts = parts;
+    o.fine = fine;
     o.status = rk_host::device_status_ptr();
     const float t = k.inv_temp;
     if (entropy)
@@ -1296,8 +1331,8 @@ extern "C" int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t voca
   }
 }
 
-// Four scalars, the rows' loss terms and room for their list.
-extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 16; }
+// Four scalars, what the rows' loss terms are finished from, these terms and room for the rows' list.
+extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 32; }
 
 extern "C" int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* actions, int64_t rows,
                               int ignore_index, int dtype, const rk_policy_terms* terms, float* logprob, float* kl,
