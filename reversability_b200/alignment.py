@@ -48,9 +48,11 @@ class PreferenceLoss(NamedTuple):
     logprobs: torch.Tensor
 
 
-def _check_temperature(temperature: float) -> None:
-    if not (math.isfinite(temperature) and temperature > 0):
+def _check_rows(temperature: float, ignore_index: int) -> None:
+    if not 1e-30 <= temperature <= 1e30:  # its reciprocal is an fp32 number
         raise ValueError("temperature must be finite and positive")
+    if not -2 ** 31 <= ignore_index < 2 ** 31:
+        raise ValueError("ignore_index must fit 32 bits")
 
 
 def _check_constants(**tensors) -> None:
@@ -85,7 +87,7 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
                    entropy: bool = False):
     """ln softmax(logits / temperature) at labels, fp32 in the shape of labels (0 at ignore_index); with `entropy`
     the pair (log-probabilities, entropies of the rows). Differentiable with respect to the logits."""
-    _check_temperature(temperature)
+    _check_rows(temperature, ignore_index)
     fn.require_cuda(logits, labels, what="token log-probabilities")
     if not (logits.requires_grad and torch.is_grad_enabled()):
         lp, h, _ = fn.token_logprob_fwd(logits, labels, temperature, ignore_index, entropy, want_stats=False)
@@ -118,7 +120,7 @@ class _Policy(torch.autograd.Function):
 
 def _policy_args(ref_logprobs, weights, clip_low, clip_high, kl_coef, entropy_coef, temperature, ignore_index, entropy,
                  denominator):
-    _check_temperature(temperature)
+    _check_rows(temperature, ignore_index)
     if not (0.0 <= clip_low and 0.0 <= clip_high):
         raise ValueError("clip_low and clip_high must not be negative")
     if kl_coef != 0 and ref_logprobs is None:
@@ -197,7 +199,7 @@ class _Preference(torch.autograd.Function):
 
 
 def _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index):
-    _check_temperature(temperature)
+    _check_rows(temperature, ignore_index)
     if not (math.isfinite(beta) and beta > 0):
         raise ValueError("beta must be finite and positive")
     if not 0.0 <= label_smoothing < 0.5:

@@ -20,6 +20,12 @@
 //
 // The tensor table travels as a kernel parameter: no host-to-device copy, no
 // device allocation, and a captured graph replays it.
+//
+// Bound: HBM, 28 bytes an element with fp32 parameters and gradients and 32-bit
+// moments, 16 and 1/16 with 8-bit ones. 456M parameters: 1871 us (6.8 TB/s) and
+// 1086 (6.75); their moments decoded to fp32 436 (6.3). The 20.3M decoder's 45
+// tensors with the norm for clipping: 105 (5.8 TB/s, three launches). A two-layer
+// test model's 14: 12 us, the launches' own.
 #include <type_traits>
 #include "vec.cuh"
 
@@ -367,6 +373,8 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
   }
 }
 
+// Squares of the gradients: fp32 per thread over its chunks, a partial sum a CTA, joined in fp64 below; the same order
+// every time. 20.3M gradients: 15 us cold (5.4 TB/s).
 template <typename TG>
 __global__ void __launch_bounds__(256) sumsq_multi_kernel(const __grid_constant__ MultiTable tab,
                                                           float* __restrict__ partial) {

@@ -608,6 +608,8 @@ def token_rows(logits: torch.Tensor, labels: torch.Tensor, name: str = "labels")
             labels.shape != logits.shape[:-1]:
         raise ValueError(f"{name} must be int64 on the logits' device with shape {tuple(logits.shape[:-1])}")
     V = logits.shape[-1]
+    if logits.get_device() != torch.cuda.current_device():
+        raise ValueError("logits must be on the current CUDA device")
     if V and logits.is_contiguous():
         return labels.numel(), V, V, labels if labels.is_contiguous() else labels.contiguous()
     if V < 1 or (V > 1 and logits.stride(-1) != 1):
@@ -699,7 +701,12 @@ def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld:
         raise ValueError("out must have a unit-stride last dimension")
     if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
         raise ValueError("out may alias the logits only with the same strides")
-    return out, token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
+    V = logits.shape[-1]
+    ldd = token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
+    gap = abs(out.data_ptr() - logits.data_ptr()) // out.element_size()
+    if rows and gap and gap < (rows - 1) * max(ld, ldd) + V and not (ld == ldd and V <= gap % ld <= ld - V):
+        raise ValueError("out overlaps the logits without being the same rows")
+    return out, ldd
 
 
 @functools.lru_cache(maxsize=64)

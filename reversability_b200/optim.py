@@ -27,22 +27,52 @@ class _Launch:
     def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype):
         self.index, self.bits, self.p_dtype, self.g_dtype = index, bits, p_dtype, g_dtype
         self.p_code, self.g_code = _lib.code(p_dtype), _lib.code(g_dtype)
-        self.entries = []  # (parameter, its state, exp_avg, exp_avg_sq, elements, place among all parameters)
+        # (parameter, elements, place among all parameters, its state, ((name, tensor, address) of each moment))
+        self.entries = []
         self.flat = []
 
     def add(self, p: torch.Tensor, g: torch.Tensor, state: dict, place: int) -> None:
-        m, v = state["exp_avg"], state["exp_avg_sq"]
-        want = (torch.int8, torch.uint8) if self.bits == 8 else (torch.float32, torch.float32)
-        if (m.dtype, v.dtype) != want or m.numel() != p.numel() or v.numel() != p.numel() or \
-                not (m.is_contiguous() and v.is_contiguous()):
-            raise ValueError(f"{self.bits}-bit moments must be contiguous {want[0]} and {want[1]} of the parameter's size")
-        scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if self.bits == 8 else (0, 0)
-        self.entries.append((p, state, m, v, p.numel(), place))
-        self.flat += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), *scales, p.numel())
+        n, blocks = p.numel(), -(-p.numel() // QUANT_BLOCK)
+        kinds = (("exp_avg", torch.int8, n), ("exp_avg_sq", torch.uint8, n), ("exp_avg_scale", torch.float32, blocks),
+                 ("exp_avg_sq_scale", torch.float32, blocks)) if self.bits == 8 else \
+            (("exp_avg", torch.float32, n), ("exp_avg_sq", torch.float32, n))
+        for name, dtype, size in kinds:
+            t = state[name]
+            if t.dtype is not dtype or t.numel() != size or not t.is_contiguous() or t.get_device() != p.get_device():
+                raise ValueError(f"{self.bits}-bit moments: {name} must be a contiguous {dtype} tensor of {size} elements "
+                                 "on the parameter's device")
+        held = tuple((name, state[name], state[name].data_ptr()) for name, _, _ in kinds)
+        self.entries.append((p, n, place, state, held))
+        self.flat += (p.data_ptr(), g.data_ptr(), *(at for _, _, at in held), *(0,) * (4 - len(held)), n)
 
     def finish(self) -> "_Launch":
         self.table = (ctypes.c_uint64 * len(self.flat))(*self.flat)
         return self
+
+    def moved(self) -> bool:
+        """Whether a moment is another tensor than when the table was made, or lies elsewhere."""
+        return any(state[name] is not t or t.data_ptr() != at
+                   for _, _, _, state, held in self.entries for name, t, at in held)
+
+    def refill(self, grads, device: int) -> bool:
+        """Writes the addresses of parameters and gradients into the table; False if it does not fit them or the
+        moments have moved."""
+        table, field, p_dtype, g_dtype = self.table, 0, self.p_dtype, self.g_dtype
+        for p, n, i, state, held in self.entries:
+            g = p.grad if grads is None else grads[i]  # autograd holds .grad to the parameter's shape
+            if g is None or g.dtype is not g_dtype or p.dtype is not p_dtype or p.numel() != n or \
+                    p.get_device() != device or g.get_device() != device or \
+                    not g.is_contiguous() or not p.is_contiguous():
+                return False
+            if grads is not None and g.shape != p.shape or grads is None and g.numel() != n:
+                return False
+            for name, t, at in held:
+                if state[name] is not t or t.data_ptr() != at:
+                    return False
+            table[field] = p.data_ptr()
+            table[field + 1] = g.data_ptr()
+            field += _FIELDS
+        return True
 
 
 class AdamW(torch.optim.Optimizer):
@@ -71,7 +101,7 @@ class AdamW(torch.optim.Optimizer):
     def _reset(self) -> None:
         self._launches = None  # the last step's plan
         self._idle = []        # (place, parameter) outside it
-        self._coded = None     # parameters with 8-bit moments and their table
+        self._coded = None     # the table of the parameters with 8-bit moments
         self._partials = None  # the norm's workspace
         self._norm_of = None   # the scalars that grad_norm is a view of
         self._lr = {}          # group index -> the learning rate its device scalars hold
@@ -182,25 +212,14 @@ class AdamW(torch.optim.Optimizer):
         for i, p in self._idle:
             if (p.grad if grads is None else grads[i]) is not None and p.numel():
                 return False
-        for launch in launches:
-            table, at, p_dtype, g_dtype = launch.table, 0, launch.p_dtype, launch.g_dtype
-            for p, state, m, v, n, i in launch.entries:
-                g = p.grad if grads is None else grads[i]  # autograd holds .grad to the parameter's type, shape and device
-                if g is None or g.dtype is not g_dtype or p.dtype is not p_dtype or g.numel() != n or p.numel() != n or \
-                        state["exp_avg"] is not m or state["exp_avg_sq"] is not v or \
-                        not g.is_contiguous() or not p.is_contiguous():
-                    return False
-                if grads is not None and (g.shape != p.shape or g.get_device() != p.get_device()):
-                    return False
-                table[at] = p.data_ptr()
-                table[at + 1] = g.data_ptr()
-                at += _FIELDS
-        return True
+        device = torch.cuda.current_device()
+        return all(launch.refill(grads, device) for launch in launches)
 
     def _collect(self, grads) -> list:
         """Checks the gradients and plans the launches for them; returns what has to live until those are queued."""
         found = []  # (group index, parameter, gradient, the parameter's place among all)
-        self._idle, self._coded, self._partials = [], None, None
+        self._launches, self._idle, self._coded, self._partials = None, [], None, None
+        device = torch.cuda.current_device()
         places = itertools.count()
         for index, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -212,6 +231,8 @@ class AdamW(torch.optim.Optimizer):
                                      "on their device")
                 if g is None or not p.numel():
                     self._idle.append((i, p))
+                elif p.get_device() != device:
+                    raise ValueError("AdamW parameters with gradients must be on the current CUDA device")
                 else:
                     found.append((index, p, g if g.is_contiguous() else g.contiguous(), i))
         self._launches = self._plan(found)
@@ -269,29 +290,29 @@ class AdamW(torch.optim.Optimizer):
     def moments(self, out=None, dtype: torch.dtype = torch.float32) -> list:
         """The values that the 8-bit moments stand for: a pair (exp_avg, exp_avg_sq) for each parameter with 8-bit
         state, in the order of the parameters. out: pairs of contiguous tensors of one type to write into."""
-        coded, table = self._coded or ((), None)
-        if table is None or any(st["exp_avg"] is not m for _, st, m, _ in coded):
-            coded = [(p, self.state[p], self.state[p]["exp_avg"], p.numel()) for g in self.param_groups
-                     if g["state_bits"] == 8 for p in g["params"] if p in self.state and "exp_avg" in self.state[p]]
-            flat = []
-            for p, st, m, n in coded:
-                flat += (0, 0, m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
-                         st["exp_avg_sq_scale"].data_ptr(), n)
-            table = (ctypes.c_uint64 * len(flat))(*flat)
-            self._coded = coded, table
+        coded = self._coded
+        if coded is None or coded.moved():
+            coded = _Launch(-1, 8, torch.float32, torch.float32)
+            for p in (p for g in self.param_groups if g["state_bits"] == 8 for p in g["params"]):
+                if p in self.state and "exp_avg" in self.state[p]:
+                    if p.get_device() != torch.cuda.current_device():
+                        raise ValueError("AdamW parameters must be on the current CUDA device")
+                    coded.add(p, p, self.state[p], 0)
+            self._coded = coded.finish()
         if out is None:
-            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, *_ in coded]
-        if len(out) != len(coded):
-            raise ValueError(f"out must hold {len(coded)} pairs")
-        if not coded:
+            out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, *_ in coded.entries]
+        if len(out) != len(coded.entries):
+            raise ValueError(f"out must hold {len(coded.entries)} pairs")
+        if not out:
             return out
-        at, kind = 0, out[0][0].dtype
-        for (_, _, _, n), (m, v) in zip(coded, out):
+        table, field, kind, device = coded.table, 0, out[0][0].dtype, torch.cuda.current_device()
+        for (_, n, *_), (m, v) in zip(coded.entries, out):
             if m.numel() != n or v.numel() != n or m.dtype is not kind or v.dtype is not kind or \
-                    not (m.is_cuda and v.is_cuda and m.is_contiguous() and v.is_contiguous()):
+                    m.get_device() != device or v.get_device() != device or \
+                    not (m.is_contiguous() and v.is_contiguous()):
                 raise ValueError("out pairs must be contiguous CUDA tensors of one type and the parameters' sizes")
-            table[at] = m.data_ptr()
-            table[at + 1] = v.data_ptr()
-            at += _FIELDS
-        _lib.call("rk_adamw_multi_moments", table, len(coded), _lib.code(kind), _lib.stream_ptr())
+            table[field] = m.data_ptr()
+            table[field + 1] = v.data_ptr()
+            field += _FIELDS
+        _lib.call("rk_adamw_multi_moments", table, len(out), _lib.code(kind), _lib.stream_ptr())
         return out

@@ -518,3 +518,20 @@ def test_many_rows_with_uneven_masks(shape, dtype, mask):
         _check_grad(d[s:s + step], x[s:s + step], clean[s:s + step], 1.0, g[s:s + step])
     assert torch.equal(r.logprobs, lp) or float((r.logprobs - lp).abs().max()) <= 2e-6 + _lp_tol(x)
     assert _lib.device_status() == (1 << 2 if mask == "blocks" else 0)
+
+
+def test_refuses_what_overlaps_and_constants_out_of_range():
+    buf = torch.randn(7, 100, device=DEV)
+    x, y, f = buf[:6, :40], torch.zeros(6, dtype=torch.int64, device=DEV), torch.zeros(6, device=DEV)
+    for out in (buf[:6, 1:41], buf[1:, :40], buf[:6, 39:79], buf.view(-1)[4:244].view(6, 40)):
+        with pytest.raises(ValueError):
+            alignment.policy_loss_and_grad(x, y, f, f, out=out)
+    for kw in (dict(temperature=1e-39), dict(temperature=float("inf")), dict(ignore_index=2 ** 31),
+               dict(ignore_index=-2 ** 31 - 1)):
+        with pytest.raises(ValueError):
+            alignment.token_logprobs(x, y, **kw)
+    keep = x.clone()
+    _, want = alignment.policy_loss_and_grad(x, y, f, f + 1)
+    _, d = alignment.policy_loss_and_grad(x, y, f, f + 1, out=buf[:6, 50:90])  # beside the logits in the same rows
+    assert torch.equal(d, want) and torch.equal(x, keep) and d.data_ptr() == buf[:6, 50:90].data_ptr()
+    assert _lib.device_status() == 0

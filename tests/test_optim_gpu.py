@@ -331,3 +331,58 @@ def test_refusals():
     with pytest.raises(ValueError):
         opt8.moments(out=[])
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_tensors_moved_between_steps(bits):
+    """Parameters and moments that get other memory between steps are found there."""
+    a, b = _params([300, 5000, 7]), _params([300, 5000, 7])
+    opt, ref = optim.AdamW(a, state_bits=bits, **HP), optim.AdamW(b, state_bits=bits, **HP)
+    held = []  # what the tensors left must not be handed out again
+    for k in range(4):
+        g = _tensors([300, 5000, 7], seed=20 + k)
+        opt.step(grads=g)
+        ref.step(grads=[t.clone() for t in g])
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+        for p in a:
+            for t in (p, *(t for t in opt.state[p].values() if isinstance(t, torch.Tensor))):
+                held.append(t.data)
+                t.data = t.data.clone()
+                held[-1].zero_()
+        if bits == 8:
+            for (m, v), (mr, vr) in zip(opt.moments(), ref.moments()):
+                assert torch.equal(m, mr) and torch.equal(v, vr)
+    state = opt.state[a[1]]
+    state["exp_avg_sq"] = state["exp_avg_sq"].clone()
+    g = _tensors([300, 5000, 7], seed=30)
+    opt.step(grads=g)
+    ref.step(grads=g)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_refuses_tensors_that_left_the_device():
+    p = _params([100])[0]
+    g = torch.ones(100, device=DEV)
+    opt = optim.AdamW([p], state_bits=8, **HP)
+    opt.step(grads=[g])
+    before = p.detach().clone()
+    for name in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+        t = opt.state[p][name]
+        there = t.data
+        t.data = there.cpu()
+        with pytest.raises(ValueError):
+            opt.step(grads=[g])
+        with pytest.raises(ValueError):
+            opt.moments()
+        t.data = there
+    there, p.data = p.data, p.data.cpu()
+    for h in (g, g.cpu()):
+        with pytest.raises(ValueError):
+            opt.step(grads=[h])
+    p.data = there
+    with pytest.raises(ValueError):
+        opt.step(grads=[g.cpu()])
+    assert torch.equal(p, before) and float(opt.param_groups[0]["scalars"][1]) == 1.0
+    opt.step(grads=[g])
+    assert not torch.equal(p, before) and _lib.device_status() == 0
