@@ -521,7 +521,7 @@ __device__ __noinline__ float warp_denominator(const RowOut& o, const rk_policy_
 // row's joins hide behind the others' sums. Of a row longer than its ring the first chunks are let go after the sums
 // and loaded again behind the others for the gradient: from L2, which holds the rows that are in work.
 constexpr int kUnroll = 4;     // vectors a thread takes of a chunk
-constexpr int kMaxSlots = 7;
+constexpr int kMaxSlots = 9;
 constexpr int kFreeSlots = 2;  // slots that a row longer than the ring leaves to the chunks that pass through
 constexpr int kMaxCluster = 8;
 constexpr int kMaxRowThreads = 512;
@@ -621,6 +621,104 @@ __device__ __forceinline__ RowSum cluster_join(RingShared& sh, const RowSum& min
   return warp_join<ENT, kMaxCluster>(a, c);
 }
 
+// A chunk into a thread's sums; src: the thread's first vector of it.
+template <typename T, bool ENT, int NT>
+__device__ __forceinline__ void sum_chunk(RowSum& a, const uint4* src, int tid, int ch, int nvec, float c) {
+  constexpr int kChunk = NT * kUnroll;
+  if ((ch + 1) * kChunk <= nvec) {
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];
+    add_vectors<T, ENT, kUnroll>(a, v, c);
+  } else {
+    for (int i = ch * kChunk + tid; i < nvec; i += NT, src += NT) {
+      const uint4 v[1] = {*src};
+      add_vectors<T, ENT, 1>(a, v, c);
+    }
+  }
+}
+// What a row's gradient is formed from, besides its elements.
+struct GradRow {
+  RowSum a;
+  RowGrad k;
+  bool far, vec;  // the (x - r) c form; whether dx has the phase of 16 bytes where x has it
+  int hot, label; // the vector that holds the label, if one does
+};
+// A chunk's gradients, and its slot released as soon as it is read.
+template <typename T, bool ENT, int NT>
+__device__ __forceinline__ void grad_chunk(const uint4* src, int tid, int ch, const RowSpan<T>& sp, T* dx, float c,
+                                           const GradRow& g, uint64_t* empty) {
+  constexpr int kChunk = NT * kUnroll;
+  const int i0 = ch * kChunk + tid;
+  uint4 v[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];  // past the row: what the slot held before, unused
+  T* to = dx + sp.head + (int64_t)i0 * kPer<T>;
+  if (g.vec && !g.far && (ch + 1) * kChunk <= sp.nvec && (unsigned)(g.hot - ch * kChunk) >= (unsigned)kChunk) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = grad_vector<T, ENT>(v[u], c, g.a, g.k);
+    release_slot(empty);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) __stcs(reinterpret_cast<uint4*>(to) + u * NT, v[u]);
+  } else {
+    release_slot(empty);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * NT;
+      if (i >= sp.nvec) break;
+      const uint4 d = g.far || i == g.hot
+                          ? grad_vector_any<T, ENT>(v[u], c, g.a, g.far, g.k, sp.head + i * kPer<T>, g.label)
+                          : grad_vector<T, ENT>(v[u], c, g.a, g.k);
+      store_vector(to + u * NT * kPer<T>, d, g.vec);
+    }
+  }
+}
+// The column of the element before or behind the vectors that thread `tid` takes, or -1: the head in 0..7, the tail in 8..15.
+template <typename T>
+__device__ __forceinline__ int edge_column(const RowSpan<T>& sp, int tid, int vocab) {
+  if (tid >= 16) return -1;
+  const int i = tid & 7;
+  if (tid < 8) return i < sp.head ? i : -1;
+  return i < sp.tail ? vocab - 1 - i : -1;
+}
+// A row without a label: zeros over the `rank`-th of n shares of its vectors, and rank 0 the elements around them.
+template <typename T, int NT>
+__device__ __forceinline__ void zero_row(T* dx, int tid, int vocab, int rank, int n) {
+  const RowSpan<T> sz(dx, vocab);
+  const int v0 = (int)((int64_t)sz.nvec * rank / n), v1 = (int)((int64_t)sz.nvec * (rank + 1) / n);
+  for (int i = v0 + tid; i < v1; i += NT) __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
+  if (rank == 0 && tid < sz.head) dx[tid] = Dt<T>::from_f(0.f);
+  if (rank == 0 && tid < sz.tail) dx[vocab - 1 - tid] = Dt<T>::from_f(0.f);
+}
+// One warp: what a row's sums give, and the factors of its gradient; `write`: this warp is the one that stores the former.
+template <bool POLICY, bool ENT>
+__device__ __forceinline__ RowGrad row_result(const RowOut& o, const rk_policy_terms& k, const PolicyIn& in, int64_t row,
+                                              const RowSum& a, bool far, float xl, float c, float inv_d, float scale,
+                                              bool write) {
+  const float ln_s = logf(a.s);
+  const float lp = fmaf(exponent(xl, c, a, far), kLn2, -ln_s);
+  const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
+  float g_lp = 0.f, g_h = 0.f;
+  write = write && (threadIdx.x & 31) == 0;
+  if constexpr (POLICY) {
+    const PolicyRow q = policy_row(k, in, lp, h, inv_d);
+    g_lp = q.g_lp;
+    g_h = q.g_h;
+    if (write) {
+      o.parts[row] = {q.loss, q.clipped};
+      o.fine[row] = {xl, a.r, a.s, q.slope};
+      if (o.kl) o.kl[row] = q.kl;
+      if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
+    }
+  }
+  if (write) {
+    o.logprob[row] = lp;
+    if constexpr (ENT) o.entropy[row] = h;
+    if (o.stats) o.stats[row] = {a.r, a.s};
+  }
+  return row_grad(a.s, ln_s, h, g_lp * scale, g_h * scale);
+}
+
 // POLICY: the policy loss of the row, and with GRAD its gradient; else the log-probabilities alone. NT summing
 // threads, kSlots chunks in the ring, CTAS of them an SM. FITS: the ring holds a row's share (the loops without chunks
 // that pass twice take 17 us less, 14848 x 50257 x 16 bits).
@@ -699,14 +797,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
       T* dx = GRAD ? dlogits + row * ldd : nullptr;
       if (label < 0) {
         if (!o.list && threadIdx.x == 0 && rank == 0) unlabelled_row<POLICY>(o, row, label);
-        if constexpr (GRAD) {
-          const RowSpan<T> sz(dx, vocab);
-          const int v0 = (int)((int64_t)sz.nvec * rank / cluster), v1 = (int)((int64_t)sz.nvec * (rank + 1) / cluster);
-          for (int i = v0 + threadIdx.x; i < v1; i += NT)
-            __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
-          if (rank == 0 && (int)threadIdx.x < sz.head) dx[threadIdx.x] = Dt<T>::from_f(0.f);
-          if (rank == 0 && (int)threadIdx.x < sz.tail) dx[vocab - 1 - threadIdx.x] = Dt<T>::from_f(0.f);
-        }
+        if constexpr (GRAD) zero_row<T, NT>(dx, threadIdx.x, vocab, rank, cluster);
         continue;
       }
       const T* x = logits + row * ld;
@@ -714,13 +805,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
       const int chunks = (sp.nvec + kChunk - 1) / kChunk;
       const int k0 = chunks * rank / cluster, n = chunks * (rank + 1) / cluster - k0;
       const int again = GRAD && !FITS && n > kSlots ? n - (kSlots - kFreeSlots) : 0;  // chunks that pass through twice
-      // the elements before and behind the vectors: rank 0's first threads, the head in 0..7, the tail in 8..15
-      int edge = -1;
-      if (rank == 0 && threadIdx.x < 16) {
-        const int i = threadIdx.x & 7;
-        if (threadIdx.x < 8) edge = i < sp.head ? i : -1;
-        else edge = i < sp.tail ? vocab - 1 - i : -1;
-      }
+      const int edge = rank == 0 ? edge_column(sp, threadIdx.x, vocab) : -1;
       const float xe = edge >= 0 ? Dt<T>::to_f(x[edge]) : 0.f;
       const float xl = warp == 0 ? Dt<T>::to_f(x[label]) : 0.f;
       PolicyIn in = {};
@@ -732,18 +817,7 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
         for (int j = 0; j < n; ++j) {
           const int ch = k0 + j;
           ring_wait(&sh.full[s], t & 1, o.status, abort);
-          const uint4* src = reinterpret_cast<const uint4*>(ring) + s * kChunk + threadIdx.x;
-          if ((ch + 1) * kChunk <= sp.nvec) {
-            uint4 v[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];
-            add_vectors<T, ENT, kUnroll>(a, v, c);
-          } else {
-            for (int i = ch * kChunk + threadIdx.x; i < sp.nvec; i += NT, src += NT) {
-              const uint4 v[1] = {*src};
-              add_vectors<T, ENT, 1>(a, v, c);
-            }
-          }
+          sum_chunk<T, ENT, NT>(a, reinterpret_cast<const uint4*>(ring) + s * kChunk + threadIdx.x, threadIdx.x, ch, sp.nvec, c);
           const bool passes = !GRAD || j < again;
           if (passes) release_slot(&sh.empty[s]);
           if (++s == kSlots) {
@@ -769,74 +843,31 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
           // no CTA of the cluster may write over the row before all have read it
           if (cluster > 1) cluster_join<ENT>(sh, a, c, rank, cluster, phase, o.status);
         }
-        const float ln_s = logf(a.s);
-        const float lp = fmaf(exponent(xl, c, a, far), kLn2, -ln_s);
-        const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
-        float g_lp = 0.f, g_h = 0.f;
-        if constexpr (POLICY) {
-          const PolicyRow q = policy_row(k, in, lp, h, inv_d);
-          g_lp = q.g_lp;
-          g_h = q.g_h;
-          if (lane == 0 && rank == 0) {
-            o.parts[row] = {q.loss, q.clipped};
-            o.fine[row] = {xl, a.r, a.s, q.slope};
-            if (o.kl) o.kl[row] = q.kl;
-            if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
-          }
-        }
-        if (lane == 0 && rank == 0) {
-          o.logprob[row] = lp;
-          if constexpr (ENT) o.entropy[row] = h;
-          if (o.stats) o.stats[row] = {a.r, a.s};
-        }
+        const RowGrad g = row_result<POLICY, ENT>(o, k, in, row, a, far, xl, c, inv_d, scale, rank == 0);
         if (GRAD && lane == 0) {
           sh.sum = a;
           sh.far = far;
-          sh.grad = row_grad(a.s, ln_s, h, g_lp * scale, g_h * scale);
+          sh.grad = g;
         }
       }
       parity ^= 1;
       if constexpr (GRAD) {
         row_bar<NT>();
-        a = sh.sum;
-        const bool far = sh.far;
-        const RowGrad gk = sh.grad;
-        const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
-        const int hot = (label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+        const GradRow g = {sh.sum, sh.grad, sh.far != 0, ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0,
+                           (label - sp.head) / kPer<T>, label};
         for (int j = again; j < n + again; ++j) {
           const int ch = k0 + (j < n ? j : j - n);
           if (j >= n) ring_wait(&sh.full[slot], turn & 1, o.status, abort);
-          const uint4* src = reinterpret_cast<const uint4*>(ring) + slot * kChunk + threadIdx.x;
-          const int i0 = ch * kChunk + (int)threadIdx.x;
-          uint4 v[kUnroll];
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u) v[u] = src[u * NT];  // past the row: what the slot held before, unused
-          T* to = dx + sp.head + (int64_t)i0 * kPer<T>;
-          if (vec && !far && (ch + 1) * kChunk <= sp.nvec && (unsigned)(hot - ch * kChunk) >= (unsigned)kChunk) {
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = grad_vector<T, ENT>(v[u], c, a, gk);
-            release_slot(&sh.empty[slot]);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) __stcs(reinterpret_cast<uint4*>(to) + u * NT, v[u]);
-          } else {
-            release_slot(&sh.empty[slot]);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-              const int i = i0 + u * NT;
-              if (i >= sp.nvec) break;
-              const uint4 g = far || i == hot ? grad_vector_any<T, ENT>(v[u], c, a, far, gk, sp.head + i * kPer<T>, label)
-                                              : grad_vector<T, ENT>(v[u], c, a, gk);
-              store_vector(to + u * NT * kPer<T>, g, vec);
-            }
-          }
+          grad_chunk<T, ENT, NT>(reinterpret_cast<const uint4*>(ring) + slot * kChunk + threadIdx.x, threadIdx.x, ch, sp, dx, c, g,
+                                 &sh.empty[slot]);
           if (++slot == kSlots) {
             slot = 0;
             ++turn;
           }
         }
         if (edge >= 0) {
-          const float t = exponent(xe, c, a, far);
-          dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, gk) + (edge == label ? gk.g : 0.f));
+          const float t = exponent(xe, c, g.a, g.far);
+          dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, g.k) + (edge == label ? g.k.g : 0.f));
         }
       }
     }
@@ -867,19 +898,14 @@ __global__ void __launch_bounds__(256)
     if (label < 0) {
       if (lane == 0) unlabelled_row<POLICY>(o, row, label);
       if constexpr (GRAD) {
-        const RowSpan<T> sz(dx, vocab);
-        for (int i = lane; i < sz.nvec; i += 32) __stcs(reinterpret_cast<uint4*>(dx + sz.head) + i, make_uint4(0, 0, 0, 0));
-        if (lane < sz.head) dx[lane] = Dt<T>::from_f(0.f);
-        if (lane < sz.tail) dx[vocab - 1 - lane] = Dt<T>::from_f(0.f);
+        zero_row<T, 32>(dx, lane, vocab, 0, 1);
       }
       continue;
     }
     const T* x = logits + row * ld;
     const RowSpan<T> sp(x, vocab);
     const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head);
-    int edge = -1;
-    if (lane < 8) edge = lane < sp.head ? lane : -1;
-    else if (lane < 16) edge = lane - 8 < sp.tail ? vocab - 1 - (lane - 8) : -1;
+    const int edge = edge_column(sp, lane, vocab);
     const float xe = edge >= 0 ? Dt<T>::to_f(x[edge]) : 0.f;
     const float xl = Dt<T>::to_f(x[label]);
     PolicyIn in = {};
@@ -961,12 +987,7 @@ __global__ void __launch_bounds__(kBwdThreads)
   T* dx = dlogits + row * ldd;
   const RowSpan<T> sp(live ? x : dx, vocab);
   const int v0 = seg * kBwdThreads * kBwdVecs + threadIdx.x;
-  int edge = -1;
-  if (seg == 0 && threadIdx.x < 16) {
-    const int i = threadIdx.x & 7;
-    if (threadIdx.x < 8) edge = i < sp.head ? i : -1;
-    else edge = i < sp.tail ? vocab - 1 - i : -1;
-  }
+  const int edge = seg == 0 ? edge_column(sp, threadIdx.x, vocab) : -1;
   if (!live) {
 #pragma unroll
     for (int j = 0; j < kBwdVecs; ++j)
@@ -1122,13 +1143,14 @@ constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 //     48 KB bf16 38.2/36.9/37.4/43.5; 14848 of 100 KB bf16 -/243/241/263; 2047 of 128 KB fp32 -/76/46/43
 //   policy with gradient: 8192 rows of 6 KB bf16 32/39, 4096 of 16 KB 44/35.5/39/50, of 24 KB 72/49/52/65 (a warp's second
 //     read of its row comes from L2 once 64 rows an SM exceed L1)
+//   policy, 4096 rows of 60 KB bf16: 128 threads and nine slots three times an SM 104, 256 and seven twice 114
 // So sums of 16-bit logits take rings of 128 threads eight times an SM (exponentials bound them, and 40 warps hide more),
 // fp32 ones, which HBM bounds, of 256 three times. With fewer rows than four an SM a warp's row takes too long alone, and
 // the larger CTAs are faster (64 rows of 100 KB: 5.5 / 6.6).
 // 256 KB rows (1500 x 131072 x 16 bits) with gradient and a ring of 256 threads twice an SM or of 512 once: 178 / 151, as
 // the larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
 constexpr int64_t kWarpRow = 4 * 1024, kWarpRowSum = 36 * 1024, kWarpRowGrad = 8 * 1024;
-constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256);
+constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kThirdRow = 9 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256);
 
 int sm_count() {
   static const int n = [] {
@@ -1204,6 +1226,7 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
   if (bytes <= kSmallRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8, true>);
   if constexpr (GRAD) {
     if (bytes <= kMidRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4, true>);
+    if (bytes <= kThirdRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 9, 3, true>);
     if (bytes <= 7 * chunk_bytes(256)) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, true>);
     if (bytes <= kLongRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, false>);
     return ring(launch_ring<T, POLICY, GRAD, ENT, 512, 7, 1, false>);
