@@ -513,13 +513,13 @@ __device__ __noinline__ float warp_denominator(const RowOut& o, const rk_policy_
 // turned into it and stored, each slot refilled with the next row's chunk behind that. So the logits cross HBM once
 // each way.
 // Bounds: HBM (14848 x 50257 x 16 bits: sums 231 us at the measured copy rate, with the gradient 462), and the exponential
-// unit, which takes an exponential for each element of a sum and one more for its gradient. Measured: sums 240 us (6.2
-// TB/s), with entropy 276; policy loss with its gradient 544 (5.5 TB/s;
-// 484 with the exponentials left out, so the unit's bursts are not hidden whole), with entropy 583. 2047 x 32003 x 32 bits,
-// which HBM alone bounds: 43 (6.1 TB/s) and 101.
-// NT summing threads a CTA and 512 an SM: shorter rows take smaller rings and more CTAs, so that one
-// row's joins hide behind the others' sums. Of a row longer than its ring the first chunks are let go after the sums
-// and loaded again behind the others for the gradient: from L2, which holds the rows that are in work.
+// unit, which takes an exponential for each element of a sum and one more for its gradient (331 us at full rate). Measured:
+// sums 240 us (6.2 TB/s), with entropy 276; policy loss with its gradient 544 (5.5 TB/s; 484 with the exponentials left
+// out), with entropy 583: the unit is 60 % busy, issue slots 47 %, and what waits waits for dependent results of four warps
+// a scheduler, which is what two such rings an SM leave room for. 2047 x 32003 x 32 bits, sums: 43 (6.1 TB/s).
+// NT summing threads a CTA: shorter rows take smaller rings and more CTAs, so that one row's joins hide behind the
+// others' sums. Of a row longer than its ring the first chunks are let go after the sums and loaded again behind the
+// others for the gradient: from L2, which holds the rows that are in work.
 constexpr int kUnroll = 4;     // vectors a thread takes of a chunk
 constexpr int kMaxSlots = 9;
 constexpr int kFreeSlots = 2;  // slots that a row longer than the ring leaves to the chunks that pass through
@@ -877,6 +877,169 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
   if (cluster > 1) cluster_sync();  // no CTA ends while another may still send to it
 }
 
+// ---------------------------------------------------------------- long fp32 rows: sums and gradients side by side
+// One CTA an SM, whose ring holds about two rows: half of its warps sum the row that has come while the other half turn
+// the one before it into its gradient, so that neither the copies nor the exponential unit wait for a row's joins. A row's
+// factors go from one half to the other through two places with a barrier each way. No circle of waits: the gradients of a
+// row wait for its sums alone, its sums for its chunks, these for the slots of rows before it, as a row fits the ring.
+// 2047 x 25000 x 32 bits: 72 us (5.7 TB/s), x 32003 96 (5.5), 2000 x 50257 142 (5.65).
+constexpr int kSplitThreads = 256, kSplitSlots = 14;
+struct SplitShared {
+  uint64_t full[kSplitSlots], empty[kSplitSlots], ready[2], taken[2];
+  RowSum part[2][kSplitThreads / 32];
+  RowSum sum[2];
+  RowGrad grad[2];
+  int far[2];
+  int abort;
+};
+constexpr int kSplitBytes = (int)(kSplitSlots * chunk_bytes(kSplitThreads)) + (int)sizeof(SplitShared);
+static_assert(kSplitBytes + 1024 <= 228 * 1024, "the ring of an SM's CTA");
+static_assert(kSplitSlots == 14, "kLongRow: rows that the ring holds");
+
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(2 * kSplitThreads + 32, 1)
+    split_row_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, float c, int ignore_index, RowOut o,
+                    rk_policy_terms k, T* dlogits, int64_t ldd) {
+  constexpr int NT = kSplitThreads, kWarps = NT / 32, kChunk = NT * kUnroll;
+  extern __shared__ __align__(128) unsigned char ring[];
+  SplitShared& sh = *reinterpret_cast<SplitShared*>(ring + kSplitSlots * kChunk * 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSplitSlots; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.empty[i]), kWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.ready[i]), 1);
+      mbar_init(smem_u32(&sh.taken[i]), kWarps);
+    }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  volatile int* abort = &sh.abort;
+  int slot = 0;
+  uint32_t turn = 0;  // how often the ring has gone round
+  const auto next_slot = [&] {
+    if (++slot == kSplitSlots) {
+      slot = 0;
+      ++turn;
+    }
+  };
+
+  if (warp == 2 * kWarps) {  // copies
+    if (lane == 0) {
+      for (RowDeal deal(o, rows, vocab, ignore_index, first, step); deal.more() && !*abort; deal.advance()) {
+        if (deal.label < 0) continue;
+        const T* x = logits + deal.row * ld;
+        const RowSpan<T> sp(x, vocab);
+        for (int ch = 0; ch * kChunk < sp.nvec; ++ch) {
+          if (turn && !ring_wait(&sh.empty[slot], (turn - 1) & 1, o.status, abort)) break;
+          const uint32_t bytes = 16u * (uint32_t)min(kChunk, sp.nvec - ch * kChunk);
+          const uint32_t bar = smem_u32(&sh.full[slot]);
+          mbar_arrive_expect_tx(bar, bytes);
+          bulk_load(smem_u32(ring) + slot * kChunk * 16, x + sp.head + (int64_t)ch * kChunk * kPer<T>, bytes, bar);
+          next_slot();
+        }
+      }
+      if (*abort) {  // nothing may still be on its way when the CTA ends
+        for (int i = 0; i < kSplitSlots; ++i) {
+          const uint32_t filled = turn + (i < slot ? 1 : 0);
+          if (filled) {
+            const uint64_t t0 = globaltimer();
+            while (!mbar_try_wait(smem_u32(&sh.full[i]), (filled - 1) & 1) && globaltimer() - t0 < RK_WAIT_LIMIT_NS) {
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < kWarps) {  // sums
+    float inv_d = 0.f, scale = 0.f;
+    if (warp == 0) {
+      const float d = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
+      if (o.sum_here && blockIdx.x == 0 && lane == 0) *o.denom = d;
+      inv_d = d != 0.f ? 1.f / d : 0.f;
+      scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
+    }
+    uint32_t done = 0;  // rows summed
+    for (RowDeal deal(o, rows, vocab, ignore_index, first, step); deal.more(); deal.advance()) {
+      const int64_t row = deal.row;
+      const int label = deal.label;
+      if (label < 0) {
+        if (!o.list && threadIdx.x == 0) unlabelled_row<true>(o, row, label);
+        continue;
+      }
+      const T* x = logits + row * ld;
+      const RowSpan<T> sp(x, vocab);
+      const int edge = edge_column(sp, threadIdx.x, vocab);
+      const float xe = edge >= 0 ? Dt<T>::to_f(x[edge]) : 0.f;
+      const float xl = warp == 0 ? Dt<T>::to_f(x[label]) : 0.f;
+      PolicyIn in = {};
+      if (warp == 0) in = policy_in(k, row);
+      RowSum a = empty_sum();
+      for (int ch = 0; ch * kChunk < sp.nvec; ++ch) {
+        ring_wait(&sh.full[slot], turn & 1, o.status, abort);
+        sum_chunk<T, ENT, NT>(a, reinterpret_cast<const uint4*>(ring) + slot * kChunk + threadIdx.x, threadIdx.x, ch, sp.nvec, c);
+        next_slot();
+      }
+      if (edge >= 0) add_element<ENT>(a, xe, c);
+      a = warp_join<ENT>(a, c);
+      const int at = done & 1;
+      if (lane == 0) sh.part[at][warp] = a;
+      row_bar<NT>();
+      if (warp == 0) {
+        a = warp_join<ENT, kWarps>(lane < kWarps ? sh.part[at][lane] : empty_sum(), c);
+        const bool far = is_far(a);
+        if (far) a = warp_row_sum_far(x, vocab, c);
+        const RowGrad g = row_result<true, ENT>(o, k, in, row, a, far, xl, c, inv_d, scale, true);
+        if (done >= 2) ring_wait(&sh.taken[at], ((done >> 1) - 1) & 1, o.status, abort);  // what the row before the last left
+        __syncwarp();
+        if (lane == 0) {
+          sh.sum[at] = a;
+          sh.far[at] = far;
+          sh.grad[at] = g;
+          mbar_arrive(smem_u32(&sh.ready[at]));
+        }
+      }
+      ++done;
+    }
+    if (warp == 0) finish_losses(o, first, step, rows, c, vocab, ignore_index);
+  } else {  // gradients
+    const int tid = threadIdx.x - NT;
+    uint32_t done = 0;
+    for (RowDeal deal(o, rows, vocab, ignore_index, first, step); deal.more(); deal.advance()) {
+      const int64_t row = deal.row;
+      const int label = deal.label;
+      T* dx = dlogits + row * ldd;
+      if (label < 0) {
+        zero_row<T, NT>(dx, tid, vocab, 0, 1);
+        continue;
+      }
+      const T* x = logits + row * ld;
+      const RowSpan<T> sp(x, vocab);
+      const int at = done & 1;
+      ring_wait(&sh.ready[at], (done >> 1) & 1, o.status, abort);
+      const GradRow g = {sh.sum[at], sh.grad[at], sh.far[at] != 0, ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0,
+                         (label - sp.head) / kPer<T>, label};
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.taken[at]));
+      ++done;
+      const int edge = edge_column(sp, tid, vocab);
+      if (edge >= 0) {
+        const float t = exponent(Dt<T>::to_f(x[edge]), c, g.a, g.far);
+        dx[edge] = Dt<T>::from_f(grad_element<ENT>(t, g.k) + (edge == label ? g.k.g : 0.f));
+      }
+      for (int ch = 0; ch * kChunk < sp.nvec; ++ch) {
+        ring_wait(&sh.full[slot], turn & 1, o.status, abort);  // complete, as the sums are; orders the copy's writes
+        grad_chunk<T, ENT, NT>(reinterpret_cast<const uint4*>(ring) + slot * kChunk + tid, tid, ch, sp, dx, c, g, &sh.empty[slot]);
+        next_slot();
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- short rows: one warp each
 // The same sums straight from global memory, four vectors a lane in flight, and for the gradient the row once more, from
 // L1 or L2. No join but the warp's own, which is what bounds short rows in a ring: 12001 x 1000 x 32 bits 8.8 us for the
@@ -967,8 +1130,8 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------- gradients from saved statistics
 // One CTA per (row, segment of 1024 vectors), four of them a thread in flight: no element depends on another, so many
-// small CTAs keep HBM busy by themselves. 14848 x 50257 x 16 bits: 443 us (6.7 TB/s, the copy rate), 2047 x 32003 x 32 bits
-// 72, with entropies 78.
+// small CTAs keep HBM busy by themselves. 14848 x 50257 x 16 bits: 445 to 470 us (6.4 to 6.7 TB/s, the copy rate), 2047 x
+// 32003 x 32 bits 78 (6.7).
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
 template <typename T, bool ENT>
@@ -1143,6 +1306,8 @@ constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 //     48 KB bf16 38.2/36.9/37.4/43.5; 14848 of 100 KB bf16 -/243/241/263; 2047 of 128 KB fp32 -/76/46/43
 //   policy with gradient: 8192 rows of 6 KB bf16 32/39, 4096 of 16 KB 44/35.5/39/50, of 24 KB 72/49/52/65 (a warp's second
 //     read of its row comes from L2 once 64 rows an SM exceed L1)
+//   policy, fp32, one ring / sums and gradients side by side: 4096 rows of 54 KB 87/91, 72 KB 115/105; 2047 of 100 KB 84/72;
+//     2000 of 200 KB 166/142; 300 of 72 KB 16/18. With 16-bit logits, whose exponentials bound both, 14848 of 100 KB 545/555
 //   policy, 4096 rows of 60 KB bf16: 128 threads and nine slots three times an SM 104, 256 and seven twice 114
 // So sums of 16-bit logits take rings of 128 threads eight times an SM (exponentials bound them, and 40 warps hide more),
 // fp32 ones, which HBM bounds, of 256 three times. With fewer rows than four an SM a warp's row takes too long alone, and
@@ -1150,7 +1315,8 @@ constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 // 256 KB rows (1500 x 131072 x 16 bits) with gradient and a ring of 256 threads twice an SM or of 512 once: 178 / 151, as
 // the larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
 constexpr int64_t kWarpRow = 4 * 1024, kWarpRowSum = 36 * 1024, kWarpRowGrad = 8 * 1024;
-constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kThirdRow = 9 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256);
+constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kThirdRow = 9 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256),
+                  kSplitRow = 4 * chunk_bytes(256);
 
 int sm_count() {
   static const int n = [] {
@@ -1199,6 +1365,17 @@ int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, in
   return rk_host::launch_status();
 }
 
+template <typename T, bool ENT>
+int launch_split(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, int ignore_index, const RowOut& o,
+                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+  auto kernel = split_row_kernel<T, ENT>;
+  const int st = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSplitBytes);
+  if (st) return st;
+  rk_host::launch_k(kernel, (unsigned)(rows < sm_count() ? rows : sm_count()), 2 * kSplitThreads + 32, kSplitBytes, s, x, ld,
+                    (int)vocab, rows, c, ignore_index, o, k, dx, ldd);
+  return rk_host::launch_status();
+}
+
 // `list`: room for rows (row, label) pairs, `denom` for the denominator.
 template <typename T, bool POLICY, bool GRAD, bool ENT>
 int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_temp, int ignore_index, RowOut o,
@@ -1226,6 +1403,9 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
   if (bytes <= kSmallRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8, true>);
   if constexpr (GRAD) {
     if (bytes <= kMidRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4, true>);
+    if constexpr (sizeof(T) == 4) {
+      if (bytes > kSplitRow && bytes <= kLongRow && rows >= 4 * sm_count()) return ring(launch_split<T, ENT>);
+    }
     if (bytes <= kThirdRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 9, 3, true>);
     if (bytes <= 7 * chunk_bytes(256)) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, true>);
     if (bytes <= kLongRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 256, 7, 2, false>);

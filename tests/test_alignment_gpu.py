@@ -535,3 +535,45 @@ def test_refuses_what_overlaps_and_constants_out_of_range():
     _, d = alignment.policy_loss_and_grad(x, y, f, f + 1, out=buf[:6, 50:90])  # beside the logits in the same rows
     assert torch.equal(d, want) and torch.equal(x, keep) and d.data_ptr() == buf[:6, 50:90].data_ptr()
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["plain", "padded", "shifted"])
+@pytest.mark.parametrize("shape,ignored", [((593, 16389), 0.3), ((1301, 25001), 0.0), ((2100, 17000), 0.97), ((600, 57343), 0.5)])
+def test_many_long_fp32_rows(shape, ignored, layout):
+    """Rows whose sums run beside the gradients of those before them: masks that leave few or uneven rows, masked
+    columns, a row of nothing but the lowest value, the gradient over the logits and in rows of another stride."""
+    rows, vocab = shape
+    x = _logits(rows, vocab, torch.float32, layout, seed=5)
+    y = _labels(rows, vocab, 5, ignored)
+    low = torch.finfo(torch.float32).min
+    x[1, vocab // 2:] = -math.inf
+    x[2, vocab // 2:] = low
+    x[rows - 1] = low
+    y[:3] = torch.tensor([7, 11, 0], device=DEV)
+    y[rows - 1] = vocab - 1
+    g = torch.Generator(device=DEV).manual_seed(3)
+    step = 290  # rows of one look at the 64-bit values
+    lp64 = torch.cat([_rows64(x[s:s + step], y[s:s + step])[1] for s in range(0, rows, step)])
+    old = (lp64 + 0.1 * torch.randn(rows, generator=g, device=DEV)).float()
+    adv = torch.randn(rows, generator=g, device=DEV)
+    kw = dict(clip_low=1.0, clip_high=10.0, entropy_coef=0.01, grad_scale=float(rows))
+    r, d = alignment.policy_loss_and_grad(x, y, old, adv, **kw)
+    valid = y >= 0
+    n = int(valid.sum())
+    assert float((r.logprobs.double() - lp64).abs().max()) <= _lp_tol(x)
+    scale = float(rows) / n
+    g_lp = -(r.logprobs.double() - old.double()).exp() * adv.double() * scale
+    g_h = torch.full_like(g_lp, -0.01 * scale)
+    for s in range(0, rows, step):
+        _check_grad(d[s:s + step], x[s:s + step], y[s:s + step], 1.0, g_lp[s:s + step], g_h[s:s + step])
+    assert not d[~valid].any()
+    again, d2 = alignment.policy_loss_and_grad(x, y, old, adv, **kw)
+    assert torch.equal(d, d2) and torch.equal(r.loss, again.loss)
+    other = torch.full((rows, vocab + 6), 7.0, device=DEV)
+    alignment.policy_loss_and_grad(x, y, old, adv, out=other[:, 3:3 + vocab], **kw)
+    assert torch.equal(other[:, 3:3 + vocab], d) and bool((other[:, :3] == 7.0).all()) and bool((other[:, 3 + vocab:] == 7.0).all())
+    buf = _logits(rows, vocab, torch.float32, layout)
+    buf.copy_(x)
+    _, d2 = alignment.policy_loss_and_grad(buf, y, old, adv, out=buf, **kw)
+    assert d2.data_ptr() == buf.data_ptr() and torch.equal(buf, d)
+    assert _lib.device_status() == 0
