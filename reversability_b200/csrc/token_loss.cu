@@ -320,10 +320,12 @@ struct RowOut {
   float* kl;       // policy only, may be NULL
   float2* stats;   // (r, S), may be NULL
   float2* coef;    // policy only, may be NULL
-  float2* parts;   // policy only: (w l, w clipped)
+  float2* parts;   // policy only: (w l, w clipped) of a row, for finish_losses
   float4* fine;    // policy only: (the label's logit, r, S, d(w l) / dlp), for finish_losses
-  float* denom;    // policy only: the denominator, or with sum_here where it goes
-  bool sum_here;   // few rows: each CTA forms it by itself, which saves a launch
+  double2* sums;   // policy only: these over the rows of a taker (a CTA, or a cluster)
+  const double* weights;  // policy only: sums of the weights of labelled rows, n_weights of them
+  int n_weights;          // 0: few rows, whose weights each CTA sums by itself, which saves a launch
+  float* denom;    // policy only: where the denominator goes
   const int2* list;    // many rows: (row, label) of those with a label, the others behind; else NULL
   unsigned int* status;
 };
@@ -336,7 +338,6 @@ __device__ __forceinline__ void unlabelled_row(const RowOut& o, int64_t row, int
   if (o.entropy) o.entropy[row] = 0.f;
   if (o.stats) o.stats[row] = {0.f, 1.f};
   if constexpr (POLICY) {
-    o.parts[row] = {0.f, 0.f};
     if (o.kl) o.kl[row] = 0.f;
     if (o.coef) o.coef[row] = {0.f, 0.f};
   }
@@ -374,33 +375,32 @@ struct RowDeal {
 
 // Lists the rows, labelled ones in front, the others behind, both in order, and writes the outputs of the others; a CTA
 // for each 1024 rows, which counts those before its own by itself (a few loads a thread, where a second launch or a
-// chain of CTAs would take longer). With POLICY the last CTA, which sees all rows, also forms the denominator. Without
-// a list it does that alone.
+// chain of CTAs would take longer). With POLICY each CTA also sums the weights of its labelled rows; without a list it
+// does that alone, over every gridDim-th 1024 rows.
 template <bool POLICY>
 __global__ void __launch_bounds__(1024) list_rows_kernel(int64_t rows, int vocab, int ignore_index, RowOut o,
-                                                         rk_policy_terms k, int2* __restrict__ list,
-                                                         float* __restrict__ denom) {
+                                                         const float* __restrict__ row_weights, int2* __restrict__ list,
+                                                         double* __restrict__ weights) {
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ int warp_before[32], warp_here[32];
   __shared__ double warp_weight[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t base = list ? (int64_t)blockIdx.x * 1024 : (rows - 1) / 1024 * 1024;
-  const bool weigh = POLICY && base + 1024 >= rows;
+  const int64_t base = (int64_t)blockIdx.x * 1024, row = base + threadIdx.x;
   double weight = 0.0;
-  int before = 0;
+  int before = 0, label = -1;
+  unsigned mask = 0;
+  if (list) {
 #pragma unroll 8
-  for (int64_t r = threadIdx.x; r < base; r += 1024) {
-    const bool live = checked_label(o.labels[r], vocab, ignore_index) >= 0;
-    before += live;
-    if (weigh && live) weight += k.weights ? (double)k.weights[r] : 1.0;
+    for (int64_t r = threadIdx.x; r < base; r += 1024) before += checked_label(o.labels[r], vocab, ignore_index) >= 0;
+    if (row < rows) label = checked_label(o.labels[row], vocab, ignore_index);
+    mask = __ballot_sync(0xffffffffu, label >= 0);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (POLICY && label >= 0) weight = row_weights ? (double)row_weights[row] : 1.0;
+  } else {
+    for (int64_t r = row; r < rows; r += (int64_t)gridDim.x * 1024)
+      if (checked_label(o.labels[r], vocab, ignore_index) >= 0) weight += row_weights ? (double)row_weights[r] : 1.0;
   }
-  const int64_t row = base + threadIdx.x;
-  const int label = row < rows ? checked_label(o.labels[row], vocab, ignore_index) : -1;
-  const bool live = label >= 0;
-  const unsigned mask = __ballot_sync(0xffffffffu, live);
-  if (weigh && live) weight += k.weights ? (double)k.weights[row] : 1.0;
-  before = __reduce_add_sync(0xffffffffu, before);
-  if (weigh) {
+  if constexpr (POLICY) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, d);
   }
@@ -410,16 +410,19 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(int64_t rows, int vocab
     warp_weight[warp] = weight;
   }
   __syncthreads();
-  const int all_before = __reduce_add_sync(0xffffffffu, warp_before[lane] + (lane < warp ? warp_here[lane] : 0));
-  if (list && row < rows) {
-    const int64_t at = all_before + __popc(mask & ((1u << lane) - 1));  // labelled rows before this one
-    list[live ? at : rows - 1 - (row - at)] = make_int2((int)row, label);
-    if (!live) unlabelled_row<POLICY>(o, row, label);
+  if (list) {
+    const int all_before = __reduce_add_sync(0xffffffffu, warp_before[lane] + (lane < warp ? warp_here[lane] : 0));
+    if (row < rows) {
+      const int64_t at = all_before + __popc(mask & ((1u << lane) - 1));  // labelled rows before this one
+      list[label >= 0 ? at : rows - 1 - (row - at)] = make_int2((int)row, label);
+      if (label < 0) unlabelled_row<POLICY>(o, row, label);
+    }
   }
-  if (weigh && threadIdx.x == 0) {
-    double s = 0.0;
-    for (int v = 0; v < 32; ++v) s += warp_weight[v];
-    *denom = k.denominator ? *k.denominator : (float)s;
+  if (POLICY && warp == 0) {
+    weight = warp_weight[lane];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, d);
+    if (lane == 0) weights[blockIdx.x] = weight;
   }
 }
 
@@ -462,18 +465,28 @@ __device__ __forceinline__ float loss_rounding(float x, float c, const RowSum& a
   const float more = slope * (float)(label_logprob(x, c, a, far) - (double)lp);
   return fabsf(more) < INFINITY ? more : 0.f;
 }
-// Adds that to the loss terms of the first-th and every step-th row after it, of this warp. Behind the warp's last row,
-// a row a lane: within the rows, the logarithm in fp64 kept a whole CTA waiting (564 us in place of 544 at 14848 x 50257).
+// Adds that to the loss terms of the first-th and every step-th row after it, of this warp, and sums these. Behind the
+// warp's last row, a row a lane: within the rows, the logarithm in fp64 kept a whole CTA waiting (564 us in place of 544 at
+// 14848 x 50257).
 __device__ __forceinline__ void finish_losses(const RowOut& o, int64_t first, int64_t step, int64_t rows, float c,
                                               int vocab, int ignore_index) {
   __syncwarp();
+  double loss = 0.0, clipped = 0.0;
   for (int64_t i = first + (threadIdx.x & 31) * step; i < rows; i += 32 * step) {
     const int2 at = o.list ? o.list[i] : make_int2((int)i, checked_label(o.labels[i], vocab, ignore_index));
     if (at.y < 0) continue;
     const float4 f = o.fine[at.x];
+    const float2 part = o.parts[at.x];
     const RowSum a = {f.y, f.y * c, f.z, 0.f};
-    o.parts[at.x].x += loss_rounding(f.x, c, a, is_far(a), o.logprob[at.x], f.w);
+    loss += (double)part.x + (double)loss_rounding(f.x, c, a, is_far(a), o.logprob[at.x], f.w);
+    clipped += (double)part.y;
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    loss += __shfl_xor_sync(0xffffffffu, loss, d);
+    clipped += __shfl_xor_sync(0xffffffffu, clipped, d);
+  }
+  if ((threadIdx.x & 31) == 0) o.sums[first] = {loss, clipped};
 }
 
 // The sums of two values over the CTA, in a fixed order.
@@ -494,21 +507,29 @@ __device__ double2 block_sum2(double a, double b) {
   return s;
 }
 
-// The sum of the weights of the rows that count, over one warp.
-__device__ __noinline__ float warp_denominator(const RowOut& o, const rk_policy_terms& k, int64_t rows, int vocab,
-                                                  int ignore_index) {
-  if (k.denominator) return *k.denominator;
+// The sum of the weights of the rows that count, over one warp, from sums[0 .. n) or, without them, from all rows.
+__device__ __noinline__ float warp_weight(const double* sums, int n, const int64_t* labels, const float* weights,
+                                          int64_t rows, int vocab, int ignore_index) {
   double s = 0.0;
-  for (int64_t r = threadIdx.x & 31; r < rows; r += 32)
-    if (checked_label(o.labels[r], vocab, ignore_index) >= 0) s += k.weights ? (double)k.weights[r] : 1.0;
+  if (n) {
+    for (int i = threadIdx.x & 31; i < n; i += 32) s += sums[i];
+  } else {
+    for (int64_t r = threadIdx.x & 31; r < rows; r += 32)
+      if (checked_label(labels[r], vocab, ignore_index) >= 0) s += weights ? (double)weights[r] : 1.0;
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   return (float)s;
 }
+__device__ __forceinline__ float warp_denominator(const RowOut& o, const rk_policy_terms& k, int64_t rows, int vocab,
+                                                  int ignore_index) {
+  return k.denominator ? *k.denominator
+                       : warp_weight(o.weights, o.n_weights, o.labels, k.weights, rows, vocab, ignore_index);
+}
 
 // ---------------------------------------------------------------- rows through a ring in shared memory
 // Persistent CTAs; a cluster of C CTAs takes a row, each a contiguous share of its 16-byte vectors. One warp
-// issues bulk copies of chunks (four vectors a thread) into a ring of seven, the other warps sum them as they land;
+// issues bulk copies of chunks (four vectors a thread) into a ring, the other warps sum them as they land;
 // the CTA, then the cluster, joins its sums in a fixed order; and with a gradient the chunks, still in the ring, are
 // turned into it and stored, each slot refilled with the next row's chunk behind that. So the logits cross HBM once
 // each way.
@@ -786,8 +807,8 @@ __global__ void __launch_bounds__(NT + 32, CTAS)
     uint32_t turn = 0, parity = 0, phase = 0;
     float inv_d = 0.f, scale = 0.f;
     if (POLICY && warp == 0) {
-      const float d = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
-      if (o.sum_here && blockIdx.x == 0 && lane == 0) *o.denom = d;
+      const float d = warp_denominator(o, k, rows, vocab, ignore_index);
+      if (blockIdx.x == 0 && lane == 0) *o.denom = d;
       inv_d = d != 0.f ? 1.f / d : 0.f;
       scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
     }
@@ -958,8 +979,8 @@ __global__ void __launch_bounds__(2 * kSplitThreads + 32, 1)
   } else if (warp < kWarps) {  // sums
     float inv_d = 0.f, scale = 0.f;
     if (warp == 0) {
-      const float d = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
-      if (o.sum_here && blockIdx.x == 0 && lane == 0) *o.denom = d;
+      const float d = warp_denominator(o, k, rows, vocab, ignore_index);
+      if (blockIdx.x == 0 && lane == 0) *o.denom = d;
       inv_d = d != 0.f ? 1.f / d : 0.f;
       scale = k.inv_temp * k.grad_scale * (k.grad_scale_dev ? *k.grad_scale_dev : 1.f);
     }
@@ -1051,9 +1072,10 @@ __global__ void __launch_bounds__(256)
   pdl_wait();  // inputs are the previous kernel's outputs
   const int lane = threadIdx.x & 31;
   float denom = 0.f;
+  double loss = 0.0, clipped = 0.0;  // over this warp's rows
   if constexpr (POLICY) {
-    denom = o.sum_here ? warp_denominator(o, k, rows, vocab, ignore_index) : *o.denom;
-    if (o.sum_here && blockIdx.x == 0 && threadIdx.x == 0) *o.denom = denom;
+    denom = warp_denominator(o, k, rows, vocab, ignore_index);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *o.denom = denom;
   }
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
     const int label = checked_label(o.labels[row], vocab, ignore_index);
@@ -1094,12 +1116,12 @@ __global__ void __launch_bounds__(256)
     const float h = ENT ? ln_s - kLn2 * a.w / a.s : 0.f;
     float g_lp = 0.f, g_h = 0.f;
     if constexpr (POLICY) {
-      PolicyRow q = policy_row(k, in, lp, h, denom != 0.f ? 1.f / denom : 0.f);
+      const PolicyRow q = policy_row(k, in, lp, h, denom != 0.f ? 1.f / denom : 0.f);
       g_lp = q.g_lp;
       g_h = q.g_h;
-      q.loss += loss_rounding(xl, c, a, far, lp, q.slope);
+      loss += (double)q.loss + (double)loss_rounding(xl, c, a, far, lp, q.slope);
+      clipped += (double)q.clipped;
       if (lane == 0) {
-        o.parts[row] = {q.loss, q.clipped};
         if (o.kl) o.kl[row] = q.kl;
         if (o.coef) o.coef[row] = {q.g_lp, q.g_h};
       }
@@ -1126,43 +1148,54 @@ __global__ void __launch_bounds__(256)
         dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(xe, c, a, far), gk) + (edge == label ? gk.g : 0.f));
     }
   }
+  if constexpr (POLICY) {
+    __shared__ double2 sums[8];
+    if (lane == 0) sums[threadIdx.x >> 5] = {loss, clipped};
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double2 all = sums[0];
+      for (int w = 1; w < 8; ++w) all = {all.x + sums[w].x, all.y + sums[w].y};
+      o.sums[blockIdx.x] = all;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- gradients from saved statistics
-// One CTA per (row, segment of 1024 vectors), four of them a thread in flight: no element depends on another, so many
+// No element depends on another: one CTA per (row, segment of 1024 vectors), four of them a thread in flight, so that many
 // small CTAs keep HBM busy by themselves. 14848 x 50257 x 16 bits: 445 to 470 us (6.4 to 6.7 TB/s, the copy rate), 2047 x
-// 32003 x 32 bits 78 (6.7).
+// 32003 x 32 bits 78 (6.7). Short rows, many of them: one warp each (16384 x 1001 x 16 bits 10 us in place of 31).
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(kBwdThreads)
-    logprob_bwd_kernel(const T* logits, int64_t ld, int vocab, int segments, const int64_t* __restrict__ labels,
-                       float inv_temp, int ignore_index, const float2* __restrict__ stats,
-                       const float* __restrict__ entropy, const float* __restrict__ d_logprob,
-                       const float* __restrict__ d_entropy, int64_t coef_stride, float scale_by,
-                       const float* __restrict__ scale_dev, T* dlogits, int64_t ldd) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  const int64_t row = blockIdx.x / segments;
-  const int seg = blockIdx.x % segments;
+// NT threads: a warp, with a row, or a CTA, with a segment of kBwdVecs vectors a thread.
+template <typename T, bool ENT, int NT>
+__device__ __forceinline__ void bwd_row(const T* logits, int64_t ld, int vocab, int64_t row, int seg, int tid,
+                                        const int64_t* __restrict__ labels, float inv_temp, int ignore_index,
+                                        const float2* __restrict__ stats, const float* __restrict__ entropy,
+                                        const float* __restrict__ d_logprob, const float* __restrict__ d_entropy,
+                                        int64_t coef_stride, float scale_by, const float* __restrict__ scale_dev,
+                                        T* dlogits, int64_t ldd) {
+  constexpr int kStep = NT * kBwdVecs;
   const int label = checked_label(labels[row], vocab, ignore_index);
-  const bool live = label >= 0;
   const T* x = logits + row * ld;
   T* dx = dlogits + row * ldd;
-  const RowSpan<T> sp(live ? x : dx, vocab);
-  const int v0 = seg * kBwdThreads * kBwdVecs + threadIdx.x;
-  const int edge = seg == 0 ? edge_column(sp, threadIdx.x, vocab) : -1;
-  if (!live) {
-#pragma unroll
-    for (int j = 0; j < kBwdVecs; ++j)
-      if (v0 + j * kBwdThreads < sp.nvec)
-        __stcs(reinterpret_cast<uint4*>(dx + sp.head) + v0 + j * kBwdThreads, make_uint4(0, 0, 0, 0));
+  const RowSpan<T> sp(label >= 0 ? x : dx, vocab);
+  const int v0 = seg * kStep, v1 = NT == 32 ? sp.nvec : min(v0 + kStep, sp.nvec);
+  const int edge = seg == 0 ? edge_column(sp, tid, vocab) : -1;
+  if (label < 0) {
+#pragma unroll 4
+    for (int i = v0 + tid; i < v1; i += NT) __stcs(reinterpret_cast<uint4*>(dx + sp.head) + i, make_uint4(0, 0, 0, 0));
     if (edge >= 0) dx[edge] = Dt<T>::from_f(0.f);
     return;
   }
+  const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
+  const int hot = (label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
   uint4 v[kBwdVecs];
+  const auto load = [&](int base) {
 #pragma unroll
-  for (int j = 0; j < kBwdVecs; ++j)
-    if (v0 + j * kBwdThreads < sp.nvec) v[j] = reinterpret_cast<const uint4*>(x + sp.head)[v0 + j * kBwdThreads];
+    for (int j = 0; j < kBwdVecs; ++j)
+      if (base + j * NT < v1) v[j] = reinterpret_cast<const uint4*>(x + sp.head)[base + j * NT];
+  };
+  load(v0 + tid);
   const float c = inv_temp * kLog2e;
   const float scale = inv_temp * scale_by * (scale_dev ? *scale_dev : 1.f);
   const float2 st = stats[row];
@@ -1170,28 +1203,58 @@ __global__ void __launch_bounds__(kBwdThreads)
   const bool far = is_far(a);
   const RowGrad k = row_grad(a.s, ENT ? logf(a.s) : 0.f, ENT ? entropy[row] : 0.f, d_logprob[row * coef_stride] * scale,
                              ENT ? d_entropy[row * coef_stride] * scale : 0.f);
-  const bool vec = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
-  const int hot = (label - sp.head) / kPer<T>;  // the vector that holds the label, if one does
+  const auto store = [&](int base) {
 #pragma unroll
-  for (int j = 0; j < kBwdVecs; ++j) {
-    const int i = v0 + j * kBwdThreads;
-    if (i < sp.nvec) {
-      const int at = sp.head + i * kPer<T>;
-      store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v[j], c, a, far, k, at, label)
-                                            : grad_vector<T, ENT>(v[j], c, a, k), vec);
+    for (int j = 0; j < kBwdVecs; ++j) {
+      const int i = base + j * NT;
+      if (i < v1) {
+        const int at = sp.head + i * kPer<T>;
+        store_vector(dx + at, far || i == hot ? grad_vector_any<T, ENT>(v[j], c, a, far, k, at, label)
+                                              : grad_vector<T, ENT>(v[j], c, a, k), vec);
+      }
+    }
+  };
+  store(v0 + tid);
+  if constexpr (NT == 32) {
+    for (int base = tid + kStep; base < v1; base += kStep) {
+      load(base);
+      store(base);
     }
   }
   if (edge >= 0)
     dx[edge] = Dt<T>::from_f(grad_element<ENT>(exponent(Dt<T>::to_f(x[edge]), c, a, far), k) + (edge == label ? k.g : 0.f));
 }
 
-__global__ void __launch_bounds__(1024) policy_reduce_kernel(const float2* __restrict__ parts, int64_t rows,
-                                                             const float* __restrict__ denom,
-                                                             float* __restrict__ metrics) {
+// BY_WARP: a warp a row; else a CTA a segment.
+template <typename T, bool ENT, bool BY_WARP>
+__global__ void __launch_bounds__(kBwdThreads)
+    logprob_bwd_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, int segments, const int64_t* __restrict__ labels,
+                       float inv_temp, int ignore_index, const float2* __restrict__ stats,
+                       const float* __restrict__ entropy, const float* __restrict__ d_logprob,
+                       const float* __restrict__ d_entropy, int64_t coef_stride, float scale_by,
+                       const float* __restrict__ scale_dev, T* dlogits, int64_t ldd) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  if constexpr (BY_WARP) {
+    const int64_t row = (int64_t)blockIdx.x * (kBwdThreads / 32) + (threadIdx.x >> 5);
+    if (row < rows)
+      bwd_row<T, ENT, 32>(logits, ld, vocab, row, 0, threadIdx.x & 31, labels, inv_temp, ignore_index, stats, entropy,
+                          d_logprob, d_entropy, coef_stride, scale_by, scale_dev, dlogits, ldd);
+  } else {
+    bwd_row<T, ENT, kBwdThreads>(logits, ld, vocab, blockIdx.x / segments, blockIdx.x % segments, threadIdx.x, labels,
+                                 inv_temp, ignore_index, stats, entropy, d_logprob, d_entropy, coef_stride, scale_by,
+                                 scale_dev, dlogits, ldd);
+  }
+}
+
+// The takers' sums over the denominator.
+__global__ void __launch_bounds__(256) policy_reduce_kernel(const double2* __restrict__ sums, int n,
+                                                            const float* __restrict__ denom,
+                                                            float* __restrict__ metrics) {
   pdl_wait();  // inputs are the previous kernel's outputs
   double a = 0.0, b = 0.0;
-  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) {
-    const float2 v = parts[r];
+#pragma unroll 5
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const double2 v = sums[i];
     a += v.x;
     b += v.y;
   }
@@ -1226,26 +1289,29 @@ __device__ __forceinline__ PairLoss pair_loss_of(const rk_preference_terms& k, d
 // A gap is a sum of hundreds of differences, each small against its two log-probabilities: it is formed in fp64 from the
 // rows' statistics, not from the log-probabilities rounded to fp32.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     preference_pair_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, int64_t pairs,
                            int64_t length, int vocab, int ignore_index, rk_preference_terms k,
                            const float2* __restrict__ stats, float* __restrict__ rewards, float* __restrict__ pair_loss,
                            float* __restrict__ loss, float* __restrict__ coef) {
   pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ double red[2][8];
+  __shared__ double red[2][32];
   const int64_t pair = blockIdx.x;
-  const int side = threadIdx.x >> 7, lane = threadIdx.x & 31;  // half of the CTA for each sequence
-  const int64_t base = (side * pairs + pair) * length;
+  const int half = blockDim.x >> 1, side = threadIdx.x >= half, tid = threadIdx.x - side * half, lane = threadIdx.x & 31;
+  const int64_t base = (side * pairs + pair) * length;  // half of the CTA for each sequence
   const float c = k.inv_temp * kLog2e;
   double g = 0.0, n = 0.0;
 #pragma unroll 4
-  for (int64_t t = threadIdx.x & 127; t < length; t += 128) {
-    const int64_t row = base + t, label = labels[row];
-    if (checked_label(label, vocab, ignore_index) < 0) continue;
+  for (int64_t t = tid; t < length; t += half) {
+    const int64_t row = base + t;
+    const int label = checked_label(labels[row], vocab, ignore_index);
     const float2 st = stats[row];
-    const RowSum a = {st.x, st.x * c, st.y, 0.f};
-    g += label_logprob(Dt<T>::to_f(logits[row * ld + label]), c, a, is_far(a)) - (k.ref_logprobs ? (double)k.ref_logprobs[row] : 0.0);
-    n += 1.0;
+    const double ref = k.ref_logprobs ? (double)k.ref_logprobs[row] : 0.0;
+    if (label >= 0) {
+      const RowSum a = {st.x, st.x * c, st.y, 0.f};
+      g += label_logprob(Dt<T>::to_f(logits[row * ld + label]), c, a, is_far(a)) - ref;
+      n += 1.0;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -1257,11 +1323,12 @@ __global__ void __launch_bounds__(256)
     red[1][threadIdx.x >> 5] = n;
   }
   __syncthreads();
-  double gap[2], count[2];
-#pragma unroll
+  double gap[2] = {0.0, 0.0}, count[2] = {0.0, 0.0};
   for (int i = 0; i < 2; ++i) {
-    gap[i] = (red[0][4 * i] + red[0][4 * i + 1]) + (red[0][4 * i + 2] + red[0][4 * i + 3]);
-    count[i] = (red[1][4 * i] + red[1][4 * i + 1]) + (red[1][4 * i + 2] + red[1][4 * i + 3]);
+    for (int w = i * (half >> 5); w < (i + 1) * (half >> 5); ++w) {
+      gap[i] += red[0][w];
+      count[i] += red[1][w];
+    }
     if (k.average) gap[i] /= fmax(count[i], 1.0);
   }
   const PairLoss q = pair_loss_of(k, gap[0], gap[1]);
@@ -1271,7 +1338,7 @@ __global__ void __launch_bounds__(256)
     rewards[pairs + pair] = k.beta * (float)gap[1];
   }
   const float s = (side ? -q.slope : q.slope) / (float)pairs / (k.average ? (float)fmax(count[side], 1.0) : 1.f);
-  for (int64_t t = threadIdx.x & 127; t < length; t += 128)
+  for (int64_t t = tid; t < length; t += half)
     coef[base + t] = checked_label(labels[base + t], vocab, ignore_index) >= 0 ? s : 0.f;
 }
 
@@ -1296,10 +1363,11 @@ bool shape_ok(int64_t ld, int64_t vocab, int64_t rows) {
 }
 
 // Up to so many rows each CTA takes every n-th and sums the weights by itself (32 loads a lane, as long as the launch it
-// saves); beyond it the rows are listed first, as masks would load CTAs unevenly (a quarter of 14848 rows masked cost
-// 15 %); and with more rows than kListRows the loads even out by themselves.
-// The policy loss needs that launch for its denominator anyway; sums alone are worth its 4 us from about 60 us on.
+// saves). Beyond it a launch sums the weights and, of rows that CTAs take, lists those with labels, as masks would load
+// CTAs unevenly (a quarter of 14848 rows masked cost 15 %); with more rows than kListRows the loads even out by
+// themselves. Sums alone are worth that launch's 4 us from about 60 us on.
 constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
+constexpr int kMaxWeights = 64;  // CTAs that sum weights: enough to load them, few enough for a warp to sum again
 
 // Row lengths in bytes at which the forms change. us, one warp a row / ring of 64 / 128 / 256 threads:
 //   sums, 4096 rows: 22 KB bf16 18.5/19.0/20.5/27.3, 32 KB fp32 22.6/25.1/24.0/26.0, 40 KB fp32 28.6/32.3/28.7/29.9,
@@ -1317,6 +1385,13 @@ constexpr int64_t kFewRows = 1024, kListRows = 32768, kListBytes = 400ll << 20;
 constexpr int64_t kWarpRow = 4 * 1024, kWarpRowSum = 36 * 1024, kWarpRowGrad = 8 * 1024;
 constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kThirdRow = 9 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256),
                   kSplitRow = 4 * chunk_bytes(256);
+// Gradients from statistics, us, a CTA / a warp a row: 16384 rows of 2 KB bf16 31/10, 6 KB 52/36, 10 KB 64/58, 14 KB 78/79,
+// fp32 12 KB 64/66; 1200 of 2 KB 3.9/2.9, of 8 KB 4.9/5.6; 100 of 12 KB 2.4/5.2. A warp loads 2 KB at once, so that with few
+// rows more than that takes it longer than a CTA.
+constexpr int64_t kBwdWarpRow = 12 * 1024, kBwdWarpOnce = 2 * 1024;
+// A pair's gaps by 256 threads / 1024, us for the whole loss without gradient of one pair of 64 tokens 4.8/6.3, of 512 7.8/7.2,
+// of 8192 69/29.
+constexpr int64_t kShortPair = 256;
 
 int sm_count() {
   static const int n = [] {
@@ -1338,7 +1413,7 @@ int cluster_for(int64_t rows, int64_t bytes, int nt) {
 
 template <typename T, bool POLICY, bool GRAD, bool ENT, int NT, int SLOTS, int CTAS, bool FITS>
 int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, int ignore_index, const RowOut& o,
-                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+                const rk_policy_terms& k, T* dx, int64_t ldd, int* takers, cudaStream_t s) {
   static_assert(CTAS * (ring_bytes(NT, SLOTS) + 1024) <= 228 * 1024, "the rings of an SM's CTAs");
   auto kernel = ring_row_kernel<T, POLICY, GRAD, ENT, NT, SLOTS, CTAS, FITS>;
   const int st = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring_bytes(NT, SLOTS));
@@ -1347,6 +1422,7 @@ int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, in
   int64_t ctas = rows * cluster;
   const int64_t most = (int64_t)CTAS * sm_count() / cluster * cluster;
   if (ctas > most) ctas = most;
+  *takers = (int)(ctas / cluster);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(NT + 32);
@@ -1367,39 +1443,44 @@ int launch_ring(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, in
 
 template <typename T, bool ENT>
 int launch_split(const T* x, int64_t ld, int64_t vocab, int64_t rows, float c, int ignore_index, const RowOut& o,
-                const rk_policy_terms& k, T* dx, int64_t ldd, cudaStream_t s) {
+                const rk_policy_terms& k, T* dx, int64_t ldd, int* takers, cudaStream_t s) {
   auto kernel = split_row_kernel<T, ENT>;
   const int st = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSplitBytes);
   if (st) return st;
-  rk_host::launch_k(kernel, (unsigned)(rows < sm_count() ? rows : sm_count()), 2 * kSplitThreads + 32, kSplitBytes, s, x, ld,
-                    (int)vocab, rows, c, ignore_index, o, k, dx, ldd);
+  *takers = (int)(rows < sm_count() ? rows : sm_count());
+  rk_host::launch_k(kernel, (unsigned)*takers, 2 * kSplitThreads + 32, kSplitBytes, s, x, ld, (int)vocab, rows, c,
+                    ignore_index, o, k, dx, ldd);
   return rk_host::launch_status();
 }
 
-// `list`: room for rows (row, label) pairs, `denom` for the denominator.
+// `list`: room for rows (row, label) pairs; `weights`: for kMaxWeights sums; *takers: how many of o.sums are written.
 template <typename T, bool POLICY, bool GRAD, bool ENT>
 int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_temp, int ignore_index, RowOut o,
-                const rk_policy_terms& k, T* dx, int64_t ldd, int2* list, float* denom, cudaStream_t s) {
+                const rk_policy_terms& k, T* dx, int64_t ldd, int2* list, double* weights, int* takers, cudaStream_t s) {
   const float c = inv_temp * kLog2e;
   const int64_t bytes = vocab * (int64_t)sizeof(T);
   const bool by_warp = bytes <= (rows < 4 * sm_count() ? kWarpRow : GRAD ? kWarpRowGrad : kWarpRowSum);
-  o.denom = denom;
-  o.sum_here = rows <= kFewRows;
   const bool worth = POLICY || rows * bytes >= kListBytes;
   o.list = rows > kFewRows && rows <= kListRows && !by_warp && worth ? list : nullptr;
-  if (rows > kFewRows && (o.list || POLICY)) {
-    rk_host::launch_k(list_rows_kernel<POLICY>, o.list ? (unsigned)((rows + 1023) / 1024) : 1, 1024, 0, s, rows, (int)vocab, ignore_index, o, k,
-                      const_cast<int2*>(o.list), denom);
+  const bool weigh = POLICY && !k.denominator && rows > kFewRows;
+  if (o.list || weigh) {
+    const int64_t blocks = (rows + 1023) / 1024;
+    const int grid = (int)(o.list || blocks < kMaxWeights ? blocks : kMaxWeights);
+    o.weights = weights;
+    o.n_weights = weigh ? grid : 0;
+    rk_host::launch_k(list_rows_kernel<POLICY>, (unsigned)grid, 1024, 0, s, rows, (int)vocab, ignore_index, o, k.weights,
+                      const_cast<int2*>(o.list), weights);
     const int st = rk_host::launch_status();
     if (st) return st;
   }
   if (by_warp) {
     const int64_t blocks = (rows + 7) / 8, most = (int64_t)sm_count() * 8;
-    rk_host::launch_k(warp_row_kernel<T, POLICY, GRAD, ENT>, (unsigned)(blocks < most ? blocks : most), 256, 0, s, x, ld,
-                      (int)vocab, rows, c, ignore_index, o, k, dx, ldd);
+    *takers = (int)(blocks < most ? blocks : most);
+    rk_host::launch_k(warp_row_kernel<T, POLICY, GRAD, ENT>, (unsigned)*takers, 256, 0, s, x, ld, (int)vocab, rows, c,
+                      ignore_index, o, k, dx, ldd);
     return rk_host::launch_status();
   }
-  const auto ring = [&](auto launch) { return launch(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, s); };
+  const auto ring = [&](auto launch) { return launch(x, ld, vocab, rows, c, ignore_index, o, k, dx, ldd, takers, s); };
   if (bytes <= kSmallRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 64, 6, 8, true>);
   if constexpr (GRAD) {
     if (bytes <= kMidRow) return ring(launch_ring<T, POLICY, GRAD, ENT, 128, 6, 4, true>);
@@ -1431,8 +1512,9 @@ int logprob_fwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64
   o.stats = reinterpret_cast<float2*>(stats);
   o.status = rk_host::device_status_ptr();
   const rk_policy_terms none = {};
-  if (entropy) return launch_rows<T, false, false, true>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, s);
-  return launch_rows<T, false, false, false>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, s);
+  int takers;
+  if (entropy) return launch_rows<T, false, false, true>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, &takers, s);
+  return launch_rows<T, false, false, false>(x, ld, vocab, rows, inv_temp, ignore_index, o, none, nullptr, 0, list, nullptr, &takers, s);
 }
 
 template <typename T>
@@ -1444,18 +1526,19 @@ int logprob_bwd_typed(const void* logits, int64_t ld, int64_t vocab, const int64
   T* dx = static_cast<T*>(dlogits);
   const float2* st = reinterpret_cast<const float2*>(stats);
   const int64_t per = (int64_t)kBwdThreads * kBwdVecs * kPer<T>;
+  const bool by_warp = vocab * (int64_t)sizeof(T) <= (rows >= 32 * sm_count() ? kBwdWarpRow : kBwdWarpOnce);
   const int64_t segments = (vocab + per - 1) / per;
-  const int64_t block_rows = ((1ll << 31) - 1) / segments;  // rows of one launch
+  const int64_t block_rows = by_warp ? 1ll << 31 : ((1ll << 31) - 1) / segments;  // rows of one launch
   for (int64_t r = 0; r < rows; r += block_rows) {
     const int64_t n = rows - r < block_rows ? rows - r : block_rows;
-    if (d_entropy)
-      rk_host::launch_k(logprob_bwd_kernel<T, true>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
-                        (int)segments, labels + r, inv_temp, ignore_index, st + r, entropy + r, d_logprob + r * coef_stride,
-                        d_entropy + r * coef_stride, coef_stride, scale_by, scale_dev, dx + r * ldd, ldd);
-    else
-      rk_host::launch_k(logprob_bwd_kernel<T, false>, (unsigned)(n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab,
-                        (int)segments, labels + r, inv_temp, ignore_index, st + r, nullptr, d_logprob + r * coef_stride,
-                        nullptr, coef_stride, scale_by, scale_dev, dx + r * ldd, ldd);
+    const auto launch = [&](auto kernel) {
+      rk_host::launch_k(kernel, (unsigned)(by_warp ? (n + 7) / 8 : n * segments), kBwdThreads, 0, s, x + r * ld, ld, (int)vocab, n,
+                        (int)segments, labels + r, inv_temp, ignore_index, st + r, d_entropy ? entropy + r : nullptr,
+                        d_logprob + r * coef_stride, d_entropy ? d_entropy + r * coef_stride : nullptr, coef_stride, scale_by,
+                        scale_dev, dx + r * ldd, ldd);
+    };
+    if (by_warp) d_entropy ? launch(logprob_bwd_kernel<T, true, true>) : launch(logprob_bwd_kernel<T, false, true>);
+    else d_entropy ? launch(logprob_bwd_kernel<T, true, false>) : launch(logprob_bwd_kernel<T, false, false>);
     const int e = rk_host::launch_status();
     if (e) return e;
   }
@@ -1467,9 +1550,12 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
                  const rk_policy_terms& k, float* logprob, float* kl, float* entropy, float* metrics, float* stats,
                  float* coef, void* dlogits, int64_t ldd, void* workspace, cudaStream_t s) {
   float* denom = static_cast<float*>(workspace);
-  float4* fine = reinterpret_cast<float4*>(denom + 4);
+  double* weights = reinterpret_cast<double*>(denom + 4);
+  double2* sums = reinterpret_cast<double2*>(weights + kMaxWeights);
+  float4* fine = reinterpret_cast<float4*>(sums + rows);
   float2* parts = reinterpret_cast<float2*>(fine + rows);
   int2* list = reinterpret_cast<int2*>(parts + rows);
+  int takers = 0;  // at most one a row
   int st = RK_OK;
   if (rows > 0) {
     const T* x = static_cast<const T*>(logits);
@@ -1483,18 +1569,20 @@ int policy_typed(const void* logits, int64_t ld, int64_t vocab, const int64_t* a
     o.coef = reinterpret_cast<float2*>(coef);
     o.parts = parts;
     o.fine = fine;
+    o.sums = sums;
+    o.denom = denom;
     o.status = rk_host::device_status_ptr();
     const float t = k.inv_temp;
     if (entropy)
-      st = dx ? launch_rows<T, true, true, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s)
-              : launch_rows<T, true, false, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s);
+      st = dx ? launch_rows<T, true, true, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, weights, &takers, s)
+              : launch_rows<T, true, false, true>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, weights, &takers, s);
     else
-      st = dx ? launch_rows<T, true, true, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s)
-              : launch_rows<T, true, false, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, denom, s);
+      st = dx ? launch_rows<T, true, true, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, weights, &takers, s)
+              : launch_rows<T, true, false, false>(x, ld, vocab, rows, t, ignore_index, o, k, dx, ldd, list, weights, &takers, s);
     if (st) return st;
   }
   // without rows the denominator was not formed: the kernel takes it as 0
-  rk_host::launch_k(policy_reduce_kernel, 1, 1024, 0, s, parts, rows, rows > 0 ? denom : nullptr, metrics);
+  rk_host::launch_k(policy_reduce_kernel, 1, 256, 0, s, sums, takers, rows > 0 ? denom : nullptr, metrics);
   return rk_host::launch_status();
 }
 
@@ -1540,8 +1628,8 @@ extern "C" int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t voca
   }
 }
 
-// Four scalars, what the rows' loss terms are finished from, these terms and room for the rows' list.
-extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + (rows > 0 ? rows : 0) * 32; }
+// Four scalars, the sums of weights and of losses, what the rows' losses are finished from, and room for the rows' list.
+extern "C" int64_t rk_policy_workspace(int64_t rows) { return 16 + kMaxWeights * 8 + (rows > 0 ? rows : 0) * 48; }
 
 extern "C" int rk_policy_loss(const void* logits, int64_t ld, int64_t vocab, const int64_t* actions, int64_t rows,
                               int ignore_index, int dtype, const rk_policy_terms* terms, float* logprob, float* kl,
@@ -1576,7 +1664,7 @@ int preference_typed(const void* logits, int64_t ld, int64_t vocab, const int64_
                                         pair_loss + ((pairs + 3) & ~(int64_t)3), s)
                : RK_OK;
   if (e) return e;
-  rk_host::launch_k(preference_pair_kernel<T>, (unsigned)pairs, 256, 0, s, x, ld, labels, pairs, length, (int)vocab,
+  rk_host::launch_k(preference_pair_kernel<T>, (unsigned)pairs, length > kShortPair ? 1024 : 256, 0, s, x, ld, labels, pairs, length, (int)vocab,
                     ignore_index, k, st, rewards, pair_loss, loss, coef);
   if ((e = rk_host::launch_status())) return e;
   if (pairs > 1) {  // a single pair's loss is the mean already
