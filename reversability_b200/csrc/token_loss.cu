@@ -1373,7 +1373,8 @@ constexpr int kMaxWeights = 64;  // CTAs that sum weights: enough to load them, 
 //   sums, 4096 rows: 22 KB bf16 18.5/19.0/20.5/27.3, 32 KB fp32 22.6/25.1/24.0/26.0, 40 KB fp32 28.6/32.3/28.7/29.9,
 //     48 KB bf16 38.2/36.9/37.4/43.5; 14848 of 100 KB bf16 -/243/241/263; 2047 of 128 KB fp32 -/76/46/43
 //   policy with gradient: 8192 rows of 6 KB bf16 32/39, 4096 of 16 KB 44/35.5/39/50, of 24 KB 72/49/52/65 (a warp's second
-//     read of its row comes from L2 once 64 rows an SM exceed L1)
+//     read of its row comes from L2 once 64 rows an SM exceed L1); warp / 64: 16384 of 10 KB bf16 93/98, of 12 KB 116/107, with
+//     entropies (which cost the ring's two warps more) 96/134 and 119/147, of 14 KB 144/158, of 20 KB 203/174; fp32 10 KB 85/79
 //   policy, fp32, one ring / sums and gradients side by side: 4096 rows of 54 KB 87/91, 72 KB 115/105; 2047 of 100 KB 84/72;
 //     2000 of 200 KB 166/142; 300 of 72 KB 16/18. With 16-bit logits, whose exponentials bound both, 14848 of 100 KB 545/555
 //   policy, 4096 rows of 60 KB bf16: 128 threads and nine slots three times an SM 104, 256 and seven twice 114
@@ -1383,6 +1384,8 @@ constexpr int kMaxWeights = 64;  // CTAs that sum weights: enough to load them, 
 // 256 KB rows (1500 x 131072 x 16 bits) with gradient and a ring of 256 threads twice an SM or of 512 once: 178 / 151, as
 // the larger ring keeps 5 of 8 chunks where the smaller keeps 5 of 16.
 constexpr int64_t kWarpRow = 4 * 1024, kWarpRowSum = 36 * 1024, kWarpRowGrad = 8 * 1024;
+template <typename T, bool ENT>
+constexpr int64_t kWarpRowMany = sizeof(T) == 4 ? kWarpRowGrad : ENT ? 14 * 1024 : 10 * 1024;  // from 32 rows an SM
 constexpr int64_t kSmallRow = 6 * chunk_bytes(64), kMidRow = 6 * chunk_bytes(128), kThirdRow = 9 * chunk_bytes(128), kLongRow = 14 * chunk_bytes(256),
                   kSplitRow = 4 * chunk_bytes(256);
 // Gradients from statistics, us, a CTA / a warp a row: 16384 rows of 2 KB bf16 31/10, 6 KB 52/36, 10 KB 64/58, 14 KB 78/79,
@@ -1459,7 +1462,7 @@ int launch_rows(const T* x, int64_t ld, int64_t vocab, int64_t rows, float inv_t
                 const rk_policy_terms& k, T* dx, int64_t ldd, int2* list, double* weights, int* takers, cudaStream_t s) {
   const float c = inv_temp * kLog2e;
   const int64_t bytes = vocab * (int64_t)sizeof(T);
-  const bool by_warp = bytes <= (rows < 4 * sm_count() ? kWarpRow : GRAD ? kWarpRowGrad : kWarpRowSum);
+  const bool by_warp = bytes <= (rows < 4 * sm_count() ? kWarpRow : !GRAD ? kWarpRowSum : rows < 32 * sm_count() ? kWarpRowGrad : kWarpRowMany<T, ENT>);
   const bool worth = POLICY || rows * bytes >= kListBytes;
   o.list = rows > kFewRows && rows <= kListRows && !by_warp && worth ? list : nullptr;
   const bool weigh = POLICY && !k.denominator && rows > kFewRows;

@@ -577,3 +577,69 @@ def test_many_long_fp32_rows(shape, ignored, layout):
     _, d2 = alignment.policy_loss_and_grad(buf, y, old, adv, out=buf, **kw)
     assert d2.data_ptr() == buf.data_ptr() and torch.equal(buf, d)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["plain", "shifted"])
+@pytest.mark.parametrize("vocab", [61, 1003, 3001, 5003])
+def test_many_short_rows(vocab, layout, dtype):
+    """Row counts at which short rows are taken by a warp each, and weights and losses are summed by many CTAs."""
+    rows = 5003
+    x = _logits(rows, vocab, dtype, layout, seed=2)
+    y = _labels(rows, vocab, 2)
+    _, lp64, h64, valid = _rows64(x, y)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    g_lp, g_h = (torch.randn(rows, generator=g, device=DEV) for _ in range(2))
+    xg = x.detach().requires_grad_()
+    lp, h = alignment.token_logprobs(xg, y, entropy=True)
+    d, = torch.autograd.grad([lp, h], xg, [g_lp, g_h])
+    assert float((lp.detach().double() - lp64).abs().max()) <= _lp_tol(x)
+    _check_grad(d, x, y, 1.0, g_lp, g_h)
+    assert not d[~valid].any()
+    d, = torch.autograd.grad(alignment.token_logprobs(xg, y), xg, g_lp)
+    _check_grad(d, x, y, 1.0, g_lp)
+    w = torch.rand(rows, generator=g, device=DEV) + 0.5
+    adv = torch.randn(rows, generator=g, device=DEV)
+    old = (lp64 + 0.1 * torch.randn(rows, generator=g, device=DEV)).float()
+    kw = dict(weights=w, clip_low=1.0, clip_high=10.0, entropy_coef=0.01)
+    r, d = alignment.policy_loss_and_grad(x, y, old, adv, grad_scale=float(rows), **kw)
+    r2 = alignment.policy_loss(xg, y, old, adv, **kw)
+    d2, = torch.autograd.grad(r2.loss * float(rows), xg)
+    ww = w.double() * valid
+    terms = (lp64 - old.double()).exp() * adv.double() + 0.01 * h64
+    want = -float((ww * terms).sum() / ww.sum())
+    size = float((ww * terms.abs()).sum() / ww.sum())
+    for got, grad in ((r, d), (r2, d2)):
+        # each term is as far off as the log-probability in its exponent
+        assert abs(float(got.loss.detach()) - want) <= 2 * _lp_tol(x) * (size + 1) + 1e-6
+        ratio = (got.logprobs.double() - old.double()).exp()
+        _check_grad(grad, x, y, 1.0, -ratio * adv.double() * ww * (rows / ww.sum()), -0.01 * ww * (rows / ww.sum()))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("pairs,length", [(1, 257), (2, 1030), (3, 256)])
+def test_preference_of_long_sequences(pairs, length):
+    vocab = 37
+    x = _logits(2 * pairs * length, vocab, torch.float32, seed=8)
+    y = _labels(2 * pairs * length, vocab, 8)
+    lp64 = _rows64(x, y)[1].view(2 * pairs, length)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    ref = (lp64 + 0.05 * torch.randn(2 * pairs, length, generator=g, device=DEV)).float()
+    x3, y2 = x.view(2 * pairs, length, vocab), y.view(2 * pairs, length)
+    for average in (False, True):
+        r, d = alignment.preference_loss_and_grad(x3, y2, ref, beta=0.2, average=average, grad_scale=float(pairs))
+        valid = (y2 >= 0).double()
+        n = valid.sum(1).clamp(min=1)
+        per = 1 / n if average else torch.ones_like(n)
+        gap = ((lp64 - ref.double()) * valid).sum(1) * per
+        diff = 0.2 * (gap[:pairs] - gap[pairs:])
+        want = torch.nn.functional.softplus(-diff)
+        # a gap is off by its tokens' log-probabilities, which are not rounded before they are summed
+        tol = _lp_tol(x) * float((n * per).max())
+        assert float((r.rewards.double() - 0.2 * gap).abs().max()) <= 0.2 * tol + 1e-6
+        assert abs(float(r.loss) - float(want.mean())) <= 0.4 * tol + 1e-6
+        # the slope at the reported rewards
+        slope = -0.2 * torch.sigmoid(r.rewards.double()[pairs:] - r.rewards.double()[:pairs])
+        g_lp = torch.cat([slope, -slope])[:, None] * per[:, None] * valid
+        _check_grad(d.view(-1, vocab), x, y, 1.0, g_lp.view(-1))
+    assert _lib.device_status() == 0
