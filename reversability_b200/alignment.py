@@ -96,26 +96,22 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
 
 
 class _Policy(torch.autograd.Function):
+    """The loss alone, formed before: what carries no gradient stays out of autograd, which costs it time for each tensor."""
+
     @staticmethod
-    def forward(ctx, logits, actions, old, adv, args):
-        loss, clip, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old, adv, want_grad=False, want_coef=True,
-                                                         **args)
-        ctx.save_for_backward(logits, actions, pairs, h if args["entropy_coef"] != 0 else None)
-        ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (lp, kl, h, clip) if t is not None))
-        return loss, lp, kl, h, clip
+    def forward(ctx, logits, made):
+        loss, actions, pairs, h, ctx.temperature, ctx.ignore_index = made
+        ctx.save_for_backward(logits, actions, pairs, h)
+        return loss.data  # no view of the metrics: they, and the loss itself, may be changed in place
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
-            return None, None, None, None, None
+    def backward(ctx, g):
         logits, actions, pairs, h = ctx.saved_tensors
         coef = pairs.data_ptr() + 2 * pairs.numel()  # behind the statistics: half of the array's bytes
         d = fn.token_logprob_bwd_at(logits, actions, pairs.data_ptr(), coef, 2, h, None if h is None else coef + 4,
                                     ctx.temperature, ctx.ignore_index, g.float())
-        return d, None, None, None, None
+        return d, None
 
 
 def _policy_args(ref_logprobs, weights, clip_low, clip_high, kl_coef, entropy_coef, temperature, ignore_index, entropy,
@@ -152,7 +148,11 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     if not (logits.requires_grad and torch.is_grad_enabled()):
         loss, clip, lp, kl, h, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False, **args)
         return PolicyLoss(loss, lp, kl, h, clip)
-    return PolicyLoss(*_Policy.apply(logits, actions, old_logprobs, advantages, args))
+    loss, clip, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False,
+                                                     want_coef=True, **args)
+    loss = _Policy.apply(logits, (loss, actions, pairs, h if args["entropy_coef"] != 0 else None, args["temperature"],
+                                  args["ignore_index"]))
+    return PolicyLoss(loss, lp, kl, h, clip)
 
 
 def _scale(grad_scale):
@@ -178,24 +178,19 @@ def policy_loss_and_grad(logits: torch.Tensor, actions: torch.Tensor, old_logpro
 
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, ref, args):
-        loss, lp, rewards, _, rows = fn.preference_loss(logits, labels, ref, want_grad=False, **args)
+    def forward(ctx, logits, made):
+        loss, labels, rows, ctx.temperature, ctx.ignore_index = made
         ctx.save_for_backward(logits, labels, rows)
-        ctx.temperature, ctx.ignore_index = args["temperature"], args["ignore_index"]
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(rewards, lp)
-        return loss, rewards, lp
+        return loss.data
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
-            return None, None, None, None
+    def backward(ctx, g):
         logits, labels, rows = ctx.saved_tensors
         coef = rows.data_ptr() + 8 * (rows.numel() // 3)  # behind the statistics
         d = fn.token_logprob_bwd_at(logits, labels, rows.data_ptr(), coef, 1, None, None, ctx.temperature,
                                     ctx.ignore_index, g.float())
-        return d, None, None, None
+        return d, None
 
 
 def _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index):
@@ -225,7 +220,9 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     if not (logits.requires_grad and torch.is_grad_enabled()):
         loss, lp, rewards, _, _ = fn.preference_loss(logits, labels, ref_logprobs, want_grad=False, **args)
         return PreferenceLoss(loss, rewards, lp)
-    return PreferenceLoss(*_Preference.apply(logits, labels, ref_logprobs, args))
+    loss, lp, rewards, _, rows = fn.preference_loss(logits, labels, ref_logprobs, want_grad=False, **args)
+    loss = _Preference.apply(logits, (loss, labels, rows, args["temperature"], args["ignore_index"]))
+    return PreferenceLoss(loss, rewards, lp)
 
 
 def preference_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, *,

@@ -743,22 +743,23 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     denominator = device_scalar(denominator, dev, "denominator")
     grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
     want_h = entropy or entropy_coef != 0
-    # two allocations: metrics, workspace, and the pairs (8-byte aligned) in one, the values per token in the other
+    # metrics and workspace in one allocation; what the backward keeps, apart from them, in another
     n_ws = _policy_workspace(rows)
-    aux = torch.empty(4 + n_ws // 4 + (4 * rows if want_coef else 0), device=dev, dtype=torch.float32)
-    at = aux.data_ptr()
-    ws, pairs_at = at + 16, at + 16 + n_ws
-    per_token = torch.empty((1 + (ref is not None) + want_h, *actions.shape), device=dev, dtype=torch.float32).unbind()
-    logprob, kl, h = per_token[0], per_token[1] if ref is not None else None, per_token[-1] if want_h else None
+    aux = torch.empty(4 + n_ws // 4, device=dev, dtype=torch.float32)
+    pairs = torch.empty(4 * rows, device=dev, dtype=torch.float32) if want_coef else None
+    at, pairs_at = aux.data_ptr(), _lib.ptr(pairs)
+    logprob = torch.empty(actions.shape, device=dev, dtype=torch.float32)
+    kl = torch.empty_like(logprob) if ref is not None else None
+    h = torch.empty_like(logprob) if want_h else None
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
     terms = _lib.POLICY_TERMS.pack(old.data_ptr(), adv.data_ptr(), _lib.ptr(ref) or 0, _lib.ptr(w) or 0,
                                    _lib.ptr(denominator) or 0, _lib.ptr(grad_scale_dev) or 0, group, clip_low, clip_high,
                                    kl_coef, entropy_coef, 1.0 / temperature, grad_scale)
     _lib.call("rk_policy_loss", logits.data_ptr(), ld, V, actions.data_ptr(), rows, int(ignore_index),
               _lib.code(logits.dtype), terms, logprob.data_ptr(), _lib.ptr(kl), _lib.ptr(h), at,
-              pairs_at if want_coef else None, pairs_at + 8 * rows if want_coef else None, _lib.ptr(dlogits), ldd, ws, n_ws,
+              pairs_at, pairs_at + 8 * rows if pairs_at else None, _lib.ptr(dlogits), ldd, at + 16, n_ws,
               _lib.stream_ptr())
-    return aux[0], aux[2], logprob, kl, h, dlogits, aux[4 + n_ws // 4:] if want_coef else None
+    return aux[0], aux[2], logprob, kl, h, dlogits, pairs
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: torch.Tensor | None, kind: str,
@@ -777,16 +778,17 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     ref = row_values(ref_logprobs, labels, "ref_logprobs")
     grad_scale_dev = device_scalar(grad_scale_dev, dev, "grad_scale")
     n_ws = _preference_workspace(seqs // 2, length)
-    # two allocations: loss, workspace, statistics and factors in one, what is returned per token and sequence apart
-    aux = torch.empty(4 + n_ws // 4 + 3 * rows, device=dev, dtype=torch.float32)
+    # loss and workspace in one allocation; what the backward keeps, apart from them, in another
+    aux = torch.empty(4 + n_ws // 4, device=dev, dtype=torch.float32)
+    kept = torch.empty(3 * rows, device=dev, dtype=torch.float32)
     logprob = torch.empty(labels.shape, device=dev, dtype=torch.float32)
     rewards = torch.empty(seqs, device=dev, dtype=torch.float32)
     at = aux.data_ptr()
-    stats_at = at + 16 + n_ws
+    stats_at = kept.data_ptr()
     dlogits, ldd = gradient_rows(logits, out, rows, ld) if want_grad else (None, V)
     terms = _lib.PREFERENCE_TERMS.pack(_lib.ptr(ref) or 0, _lib.ptr(grad_scale_dev) or 0, beta, label_smoothing,
                                        1.0 / temperature, grad_scale, _lib.PREFERENCE_KINDS[kind], int(average))
     _lib.call("rk_preference_loss", logits.data_ptr(), ld, V, labels.data_ptr(), seqs // 2, length, int(ignore_index),
               _lib.code(logits.dtype), terms, logprob.data_ptr(), rewards.data_ptr(), at,
               stats_at, stats_at + 8 * rows, _lib.ptr(dlogits), ldd, at + 16, n_ws, _lib.stream_ptr())
-    return aux[0], logprob, rewards, dlogits, aux[4 + n_ws // 4:]
+    return aux[0], logprob, rewards, dlogits, kept

@@ -643,3 +643,32 @@ def test_preference_of_long_sequences(pairs, length):
         g_lp = torch.cat([slope, -slope])[:, None] * per[:, None] * valid
         _check_grad(d.view(-1, vocab), x, y, 1.0, g_lp.view(-1))
     assert _lib.device_status() == 0
+
+
+def test_changing_what_was_returned_leaves_the_backward_alone():
+    """Metrics are often reduced in place over processes before the backward; what that reads lies apart from them. The
+    entropies, which the bonus's gradient is formed from, may not be changed."""
+    x, y, old, adv, ref, w = _policy_inputs(12, 50, torch.float32, "plain")
+
+    def policy(z):
+        return alignment.policy_loss(z, y, old, adv, ref_logprobs=ref, kl_coef=0.1, entropy_coef=0.01)
+
+    def preference(z):
+        return alignment.preference_loss(z.view(2, 6, 50), y.view(2, 6), None)
+    for make in (policy, preference):
+        a, b = (x.clone().requires_grad_() for _ in range(2))
+        want, = torch.autograd.grad(make(a).loss, a)
+        r = make(b)
+        for name, t in r._asdict().items():
+            if name != "entropy" and t is not None:
+                t.detach().mul_(3.0)
+        got, = torch.autograd.grad(r.loss, b, retain_graph=True)
+        assert torch.equal(got, want)
+        loss = r.loss
+        loss *= 0.5
+        half, = torch.autograd.grad(loss, b)
+        assert torch.equal(half, want * 0.5)
+    r = policy(x.clone().requires_grad_())
+    r.entropy.mul_(3.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        r.loss.backward()
