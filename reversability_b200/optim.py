@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import itertools
 import math
+import operator
 
 import torch
 
@@ -100,11 +101,12 @@ class AdamW(torch.optim.Optimizer):
 
     def _reset(self) -> None:
         self._launches = None  # the last step's plan
+        self._made_of = []     # (state_bits, parameters) of each group then
         self._idle = []        # (place, parameter) outside it
         self._coded = None     # the table of the parameters with 8-bit moments
         self._partials = None  # the norm's workspace
         self._norm_of = None   # the scalars that grad_norm is a view of
-        self._lr = {}          # group index -> the learning rate its device scalars hold
+        self._lr = {}          # group index -> (its device scalars, the learning rate they hold)
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm}
@@ -145,13 +147,15 @@ class AdamW(torch.optim.Optimizer):
             scalars = scalars.to(dev)
         if scalars is not group["scalars"]:
             group["scalars"] = scalars
-            self._lr.pop(index, None)
         lr = group["lr"]
         if isinstance(lr, torch.Tensor):
             scalars[0].copy_(lr)
-        elif self._lr.get(index) != lr:
-            scalars[0].fill_(lr)
-            self._lr[index] = lr
+            self._lr.pop(index, None)
+        else:
+            block, held = self._lr.get(index, (None, None))
+            if block is not scalars or held != lr:  # groups may be added, taken out or sorted by hand
+                scalars[0].fill_(lr)
+                self._lr[index] = scalars, lr
         return scalars
 
     def sync_lr(self) -> None:
@@ -200,6 +204,8 @@ class AdamW(torch.optim.Optimizer):
             if p.dtype not in _lib.DTYPE_CODE or not p.is_contiguous():
                 raise ValueError("AdamW parameters must be contiguous fp32, bf16 or fp16")
             bits = self.param_groups[index]["state_bits"]
+            if bits not in (8, 32):
+                raise ValueError("state_bits must be 8 or 32")
             key = index, p.dtype, g.dtype
             if key not in launches:
                 launches[key] = _Launch(index, bits, p.dtype, g.dtype)
@@ -208,7 +214,14 @@ class AdamW(torch.optim.Optimizer):
 
     def _refill(self, launches, grads) -> bool:
         """Writes the addresses of parameters and gradients into the last plan's tables; False if the plan does not fit
-        (another set of gradients, other types or sizes, moments replaced, a gradient that needs a copy)."""
+        (other groups or parameters, another set of gradients, other types or sizes, moments replaced, a gradient that
+        needs a copy)."""
+        if len(self._made_of) != len(self.param_groups):
+            return False
+        for group, (bits, params) in zip(self.param_groups, self._made_of):
+            now = group["params"]
+            if group["state_bits"] != bits or len(now) != len(params) or not all(map(operator.is_, now, params)):
+                return False
         for i, p in self._idle:
             if (p.grad if grads is None else grads[i]) is not None and p.numel():
                 return False
@@ -236,6 +249,7 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     found.append((index, p, g if g.is_contiguous() else g.contiguous(), i))
         self._launches = self._plan(found)
+        self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
 
     # ---- the step

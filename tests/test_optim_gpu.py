@@ -386,3 +386,38 @@ def test_refuses_tensors_that_left_the_device():
     assert torch.equal(p, before) and float(opt.param_groups[0]["scalars"][1]) == 1.0
     opt.step(grads=[g])
     assert not torch.equal(p, before) and _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_a_group_added_after_a_step(max_norm, given, bits):
+    """Layers unfrozen during tuning: their first update is that of a new optimizer, within the clip over all groups."""
+    sizes = [300, 2049, 7, 513]
+    params = _params(sizes)
+    opt = optim.AdamW(params[:2], max_norm=max_norm, state_bits=bits, **HP)
+    old, new = Ref(params[:2], **HP), Ref(params[2:], **dict(HP, lr=3e-2))
+    for k in range(2):  # within the second step the moments of 8 bits have been rounded once
+        grads = _tensors(sizes, seed=40 + k)
+        live = grads[:2] if k == 0 else grads
+        if k == 1:
+            opt.add_param_group(dict(params=params[2:], lr=3e-2))
+            if bits == 8:
+                old.m, old.v = ([t.double() for t in ts] for ts in zip(*opt.moments()))
+        norm = math.sqrt(sum(float(g.double().square().sum()) for g in live))
+        coef = 1.0 if max_norm is None else min(1.0, max_norm / (norm + 1e-6))
+        if given:
+            opt.step(grads=live)
+        else:
+            _set(params, live)
+            opt.step()
+        old.step([g.double() * coef for g in live[:2]])
+        if k == 1:
+            new.step([g.double() * coef for g in live[2:]])
+        if max_norm is not None:
+            assert abs(float(opt.grad_norm) - norm) <= 1e-5 * norm
+    for q, p, lr in [(q, p, HP["lr"]) for q, p in zip(params, old.p)] + [(q, p, 3e-2) for q, p in zip(params[2:], new.p)]:
+        # the tolerance of a step with 8-bit moments, twice
+        assert float((q.detach().double() - p).abs().max()) <= 2e-5 * lr * 10 + 2.0 ** -22 * float(p.abs().max())
+    if bits == 8:
+        assert len(opt.moments()) == 4

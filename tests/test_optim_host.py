@@ -1,0 +1,117 @@
+"""Host side of optim.AdamW on CPU tensors: the library calls are recorded
+instead of launched, so what is planned, allocated and refused is seen without
+a GPU."""
+import pytest
+import torch
+
+from reversability_b200 import _lib, optim
+
+
+class Recorder:
+    def __init__(self):
+        self.calls = []
+        self.capturing = False
+
+    def __call__(self, name, *args):
+        self.calls.append((name, args))
+
+    def named(self, name):
+        return [args for n, args in self.calls if n == name]
+
+    def stepped(self):
+        """The parameter addresses that the recorded steps would update."""
+        return [args[0][i * 7] for args in self.named("rk_adamw_multi_step") for i in range(args[1])]
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """A CPU tensor's device index is -1: so is the current device here."""
+    r = Recorder()
+    monkeypatch.setattr(optim.fn, "require_cuda", lambda *a, **k: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: r.capturing)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda device=None: 0)
+    monkeypatch.setattr(_lib, "call", r)
+    return r
+
+
+def _params(n, size=10):
+    return [torch.nn.Parameter(torch.zeros(size)) for _ in range(n)]
+
+
+def _grads(params):
+    return [torch.ones_like(p) for p in params]
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_a_group_added_after_a_step_is_updated(recorded, max_norm, given):
+    params = _params(3)
+    opt = optim.AdamW(params[:2], max_norm=max_norm)
+
+    def step(which):
+        if not given:
+            for p, g in zip(which, _grads(which)):
+                p.grad = g
+        recorded.calls.clear()
+        opt.step(grads=_grads(which) if given else None)
+    step(params[:2])
+    opt.add_param_group(dict(params=params[2:], state_bits=8))
+    step(params)
+    assert sorted(recorded.stepped()) == sorted(p.data_ptr() for p in params)
+    assert opt.state[params[2]]["exp_avg"].dtype is torch.int8
+    if max_norm:
+        assert sum(args[1] for args in recorded.named("rk_adamw_multi_sumsq")) == 3
+
+
+def test_parameters_put_into_a_group_by_hand(recorded):
+    params = _params(4)
+    opt = optim.AdamW(params[:2])
+    opt.step(grads=_grads(params[:2]))
+    group = opt.param_groups[0]
+    group["params"].append(params[2])
+    recorded.calls.clear()
+    opt.step(grads=_grads(params[:3]))
+    assert recorded.stepped() == [p.data_ptr() for p in params[:3]]
+    group["params"][1] = params[3]
+    recorded.calls.clear()
+    opt.step(grads=_grads(params[:3]))
+    assert recorded.stepped() == [params[i].data_ptr() for i in (0, 3, 2)]
+    del opt.param_groups[0]["params"][0]
+    recorded.calls.clear()
+    opt.step(grads=_grads(params[:2]))
+    assert recorded.stepped() == [params[i].data_ptr() for i in (3, 2)]
+
+
+def test_another_state_bits_is_noticed(recorded):
+    params = _params(2)
+    opt = optim.AdamW([dict(params=params[:1]), dict(params=params[1:])])
+    opt.step(grads=_grads(params))
+    for bits in (8, 16):  # the moments are there in 32 bits; 16 there is not
+        opt.param_groups[1]["state_bits"] = bits
+        with pytest.raises(ValueError, match="bit"):
+            opt.step(grads=_grads(params))
+    opt.param_groups[1]["state_bits"] = 8
+    opt.state[params[1]].clear()
+    recorded.calls.clear()
+    opt.step(grads=_grads(params))
+    assert [args[4] for args in recorded.named("rk_adamw_multi_step")] == [32, 8]
+
+
+def test_groups_that_change_places_keep_their_learning_rates(recorded):
+    params = _params(2)
+    opt = optim.AdamW([dict(params=params[:1], lr=1.0), dict(params=params[1:], lr=2.0)])
+    opt.step(grads=_grads(params))
+    opt.param_groups.reverse()
+    opt.param_groups[0]["lr"], opt.param_groups[1]["lr"] = 1.0, 2.0
+    opt.step(grads=_grads(params)[::-1])
+    assert [float(g["scalars"][0]) for g in opt.param_groups] == [1.0, 2.0]
+
+
+def test_a_number_after_a_learning_rate_tensor(recorded):
+    params = _params(1)
+    opt = optim.AdamW(params, lr=1.0)
+    for lr in (1.0, torch.tensor(2.0), 1.0):
+        opt.param_groups[0]["lr"] = lr
+        opt.step(grads=_grads(params))
+        assert float(opt.param_groups[0]["scalars"][0]) == float(lr)
