@@ -7,6 +7,7 @@ parameters and gradients lie where PyTorch put them.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import itertools
 import math
@@ -21,6 +22,17 @@ QUANT_BLOCK = 256  # elements that share a scale in 8-bit moments
 _FIELDS = 7        # 8-byte fields of rk_adamw_tensor
 
 
+def _seen(state) -> tuple[list, list]:
+    """The parameters and their entries in an optimizer's state."""
+    return list(state), list(state.values())
+
+
+def _same(seen, state) -> bool:
+    """Whether these are still the same objects in the same order (a comparison would look into the tensors)."""
+    return len(seen[0]) == len(state) and all(map(operator.is_, seen[0], state)) and \
+        all(map(operator.is_, seen[1], state.values()))
+
+
 class _Launch:
     """The tensors of one group with one parameter and one gradient type: their rk_adamw_tensor array, whose moment
     addresses and sizes stay from step to step while p and g are written anew in each."""
@@ -28,50 +40,64 @@ class _Launch:
     def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype):
         self.index, self.bits, self.p_dtype, self.g_dtype = index, bits, p_dtype, g_dtype
         self.p_code, self.g_code = _lib.code(p_dtype), _lib.code(g_dtype)
-        # (parameter, elements, place among all parameters, its state, ((name, tensor, address) of each moment))
-        self.entries = []
+        self.entries = []  # (parameter, elements, place among all parameters)
         self.flat = []
+        # of each entry its state, of all entries the moments (held, so that nothing else can lie there) and their addresses
+        self.names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if bits == 8 else 2]
+        self.of_state = operator.itemgetter(*self.names)
+        self.states, self.moments, self.at = [], [], []
 
     def add(self, p: torch.Tensor, g: torch.Tensor, state: dict, place: int) -> None:
         n, blocks = p.numel(), -(-p.numel() // QUANT_BLOCK)
-        kinds = (("exp_avg", torch.int8, n), ("exp_avg_sq", torch.uint8, n), ("exp_avg_scale", torch.float32, blocks),
-                 ("exp_avg_sq_scale", torch.float32, blocks)) if self.bits == 8 else \
-            (("exp_avg", torch.float32, n), ("exp_avg_sq", torch.float32, n))
-        for name, dtype, size in kinds:
-            t = state[name]
-            if t.dtype is not dtype or t.numel() != size or not t.is_contiguous() or t.get_device() != p.get_device():
+        kinds = ((torch.int8, n), (torch.uint8, n), (torch.float32, blocks), (torch.float32, blocks)) if self.bits == 8 else \
+            ((torch.float32, n), (torch.float32, n))
+        for name, (dtype, size) in zip(self.names, kinds):
+            t = state.get(name)
+            if t is None or t.dtype is not dtype or t.numel() != size or not t.is_contiguous() or \
+                    t.get_device() != p.get_device():
                 raise ValueError(f"{self.bits}-bit moments: {name} must be a contiguous {dtype} tensor of {size} elements "
                                  "on the parameter's device")
-        held = tuple((name, state[name], state[name].data_ptr()) for name, _, _ in kinds)
-        self.entries.append((p, n, place, state, held))
-        self.flat += (p.data_ptr(), g.data_ptr(), *(at for _, _, at in held), *(0,) * (4 - len(held)), n)
+        moments = self.of_state(state)
+        at = [t.data_ptr() for t in moments]
+        self.entries.append((p, n, place))
+        self.states.append(state)
+        self.moments += moments
+        self.at += at
+        self.flat += (p.data_ptr(), g.data_ptr(), *at, *(0,) * (4 - len(at)), n)
 
     def finish(self) -> "_Launch":
-        self.table = (ctypes.c_uint64 * len(self.flat))(*self.flat)
+        self.parts = _lib.lib().rk_adamw_multi_parts(len(self.entries))  # of the norm's partial sums
+        self.words = array.array("Q", self.flat)
+        self.table = (ctypes.c_uint64 * len(self.flat)).from_buffer(self.words) if self.flat else None
         return self
 
     def moved(self) -> bool:
-        """Whether a moment is another tensor than when the table was made, or lies elsewhere."""
-        return any(state[name] is not t or t.data_ptr() != at
-                   for _, _, _, state, held in self.entries for name, t, at in held)
+        """Whether a moment lies elsewhere than when the table was made."""
+        of_state = self.of_state
+        try:
+            return [t.data_ptr() for state in self.states for t in of_state(state)] != self.at
+        except KeyError:
+            return True
 
     def refill(self, grads, device: int) -> bool:
         """Writes the addresses of parameters and gradients into the table; False if it does not fit them or the
         moments have moved."""
-        table, field, p_dtype, g_dtype = self.table, 0, self.p_dtype, self.g_dtype
-        for p, n, i, state, held in self.entries:
+        if self.moved():
+            return False
+        words, field, p_dtype, g_dtype = self.words, 0, self.p_dtype, self.g_dtype
+        for p, n, i in self.entries:
             g = p.grad if grads is None else grads[i]  # autograd holds .grad to the parameter's shape
             if g is None or g.dtype is not g_dtype or p.dtype is not p_dtype or p.numel() != n or \
-                    p.get_device() != device or g.get_device() != device or \
-                    not g.is_contiguous() or not p.is_contiguous():
+                    g.get_device() != device or not g.is_contiguous() or not p.is_contiguous():
                 return False
             if grads is not None and g.shape != p.shape or grads is None and g.numel() != n:
                 return False
-            for name, t, at in held:
-                if state[name] is not t or t.data_ptr() != at:
+            at = p.data_ptr()
+            if at != words[field]:  # no two devices share an address
+                if p.get_device() != device:
                     return False
-            table[field] = p.data_ptr()
-            table[field + 1] = g.data_ptr()
+                words[field] = at
+            words[field + 1] = g.data_ptr()
             field += _FIELDS
         return True
 
@@ -102,8 +128,10 @@ class AdamW(torch.optim.Optimizer):
     def _reset(self) -> None:
         self._launches = None  # the last step's plan
         self._made_of = []     # (state_bits, parameters) of each group then
+        self._state_of = ()    # the optimizer's state then
         self._idle = []        # (place, parameter) outside it
         self._coded = None     # the table of the parameters with 8-bit moments
+        self._coded_of = ()    # the optimizer's state when it was made
         self._partials = None  # the norm's workspace
         self._norm_of = None   # the scalars that grad_norm is a view of
         self._lr = {}          # group index -> (its device scalars, the learning rate they hold)
@@ -149,7 +177,7 @@ class AdamW(torch.optim.Optimizer):
             group["scalars"] = scalars
         lr = group["lr"]
         if isinstance(lr, torch.Tensor):
-            scalars[0].copy_(lr)
+            scalars[0].copy_(lr.detach())
             self._lr.pop(index, None)
         else:
             block, held = self._lr.get(index, (None, None))
@@ -222,12 +250,15 @@ class AdamW(torch.optim.Optimizer):
             now = group["params"]
             if group["state_bits"] != bits or len(now) != len(params) or not all(map(operator.is_, now, params)):
                 return False
+        if not _same(self._state_of, self.state):
+            return False
         for i, p in self._idle:
             if (p.grad if grads is None else grads[i]) is not None and p.numel():
                 return False
         device = torch.cuda.current_device()
         return all(launch.refill(grads, device) for launch in launches)
 
+    @torch.no_grad()
     def _collect(self, grads) -> list:
         """Checks the gradients and plans the launches for them; returns what has to live until those are queued."""
         found = []  # (group index, parameter, gradient, the parameter's place among all)
@@ -249,11 +280,11 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     found.append((index, p, g if g.is_contiguous() else g.contiguous(), i))
         self._launches = self._plan(found)
+        self._state_of = _seen(self.state)
         self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
 
     # ---- the step
-    @torch.no_grad()
     def step(self, closure=None, *, grads=None):
         """One update. grads: gradients in the order of the parameters over all groups (None where there is none),
         instead of the parameters' .grad; they may have another floating type than the parameters."""
@@ -271,18 +302,17 @@ class AdamW(torch.optim.Optimizer):
         launches = self._launches
         if not launches:
             return loss
-        stream, lib = _lib.stream_ptr(), _lib.lib()
+        stream = _lib.stream_ptr()
         partials, parts = None, 0
         if self.max_norm is not None:
             if self._partials is None:  # as long as the plan: its size depends on the launches alone
-                parts = sum(lib.rk_adamw_multi_parts(len(launch.entries)) for launch in launches)
+                parts = sum(launch.parts for launch in launches)
                 self._partials = torch.empty(parts, device=launches[0].entries[0][0].device, dtype=torch.float32)
             partials, parts = self._partials, self._partials.numel()
             at = partials.data_ptr()
             for launch in launches:
-                n = len(launch.entries)
-                _lib.call("rk_adamw_multi_sumsq", launch.table, n, launch.g_code, at, stream)
-                at += 4 * lib.rk_adamw_multi_parts(n)
+                _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
+                at += 4 * launch.parts
         scalars = {}
         for index in dict.fromkeys(launch.index for launch in launches):
             group, scalars[index] = self.param_groups[index], self._group_scalars(index)
@@ -305,14 +335,14 @@ class AdamW(torch.optim.Optimizer):
         """The values that the 8-bit moments stand for: a pair (exp_avg, exp_avg_sq) for each parameter with 8-bit
         state, in the order of the parameters. out: pairs of contiguous tensors of one type to write into."""
         coded = self._coded
-        if coded is None or coded.moved():
+        if coded is None or not _same(self._coded_of, self.state) or coded.moved():
             coded = _Launch(-1, 8, torch.float32, torch.float32)
             for p in (p for g in self.param_groups if g["state_bits"] == 8 for p in g["params"]):
                 if p in self.state and "exp_avg" in self.state[p]:
                     if p.get_device() != torch.cuda.current_device():
                         raise ValueError("AdamW parameters must be on the current CUDA device")
                     coded.add(p, p, self.state[p], 0)
-            self._coded = coded.finish()
+            self._coded, self._coded_of = coded.finish(), _seen(self.state)
         if out is None:
             out = [(torch.empty_like(p, dtype=dtype), torch.empty_like(p, dtype=dtype)) for p, *_ in coded.entries]
         if len(out) != len(coded.entries):

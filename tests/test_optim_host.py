@@ -115,3 +115,40 @@ def test_a_number_after_a_learning_rate_tensor(recorded):
         opt.param_groups[0]["lr"] = lr
         opt.step(grads=_grads(params))
         assert float(opt.param_groups[0]["scalars"][0]) == float(lr)
+
+
+def _used(recorded, opt, params):
+    """Whether the last step was given the moments that the optimizer's state holds."""
+    args, = recorded.named("rk_adamw_multi_step")
+    for i, p in enumerate(params):
+        names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if args[4] == 8 else 2]
+        assert [args[0][i * 7 + 2 + k] for k in range(len(names))] == [opt.state[p][name].data_ptr() for name in names]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_that_is_replaced_or_dropped(recorded, bits):
+    params, held = _params(3), []
+
+    def step():
+        recorded.calls.clear()
+        opt.step(grads=_grads(params))
+        _used(recorded, opt, params)
+    opt = optim.AdamW(params, state_bits=bits)
+    step()
+    for change in (lambda: opt.state.clear(), lambda: opt.state.pop(params[1]), lambda: opt.state[params[2]].clear(),
+                   lambda: opt.state.update({params[0]: {k: v.clone() for k, v in opt.state[params[0]].items()}}),
+                   lambda: opt.state[params[0]].update(exp_avg_sq=opt.state[params[0]]["exp_avg_sq"].clone())):
+        if bits == 8:
+            opt.moments()
+        held.append([dict(s) for s in opt.state.values()])  # so that nothing new lies where something was
+        change()
+        if bits == 8 and all(opt.state.get(p) for p in params):
+            recorded.calls.clear()
+            opt.moments()
+            (table, n, *_), = recorded.named("rk_adamw_multi_moments")
+            assert [table[i * 7 + 3] for i in range(n)] == [opt.state[p]["exp_avg_sq"].data_ptr() for p in params]
+        step()
+    del opt.state[params[0]]["exp_avg"]  # not a whole state
+    opt.state[params[0]]["exp_avg"] = torch.zeros(9)
+    with pytest.raises(ValueError, match="exp_avg"):
+        step()
