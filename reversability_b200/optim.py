@@ -113,7 +113,9 @@ class AdamW(torch.optim.Optimizer):
 
     A group counts one step for each step() that finds a gradient in it. Step count, learning rate and the derived
     constants live on the device, so a captured graph that contains step() counts on when it is replayed; a learning
-    rate changed in param_groups is copied there by the next step() outside a graph, or by sync_lr()."""
+    rate changed in param_groups is copied there by the next step() outside a graph, or by sync_lr(), and never by a
+    capture, except that a rate given as a tensor on the device is read from that tensor by each replay. What a step()
+    makes for itself cannot be captured: take a first step, with the same gradients, outside the graph."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_norm: float | None = None):
@@ -121,6 +123,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("max_norm must be positive")
         self.max_norm = max_norm
         self.grad_norm = None  # the gradients' global norm before clipping in the last step (device scalar)
+        self._captured = {}    # by id, what captured graphs go on reading
         self._reset()
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       scalars=None))
@@ -142,6 +145,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         self.grad_norm = None
+        self._captured = {}
         self._reset()
 
     def add_param_group(self, param_group) -> None:
@@ -168,26 +172,34 @@ class AdamW(torch.optim.Optimizer):
         """fp32[8] of the group on its device: [0] lr, [1] steps taken, [2] gradient norm, [3] clip coefficient."""
         group = self.param_groups[index]
         dev = group["params"][0].device
-        scalars = group["scalars"]
-        if scalars is None:
-            scalars = torch.zeros(8, device=dev, dtype=torch.float32)
-        elif scalars.device != dev:
-            scalars = scalars.to(dev)
-        if scalars is not group["scalars"]:
+        scalars, capturing = group["scalars"], torch.cuda.is_current_stream_capturing()
+        if scalars is None or scalars.device != dev:
+            self._uncaptured(capturing)
+            scalars = torch.zeros(8, device=dev, dtype=torch.float32) if scalars is None else scalars.to(dev)
             group["scalars"] = scalars
         lr = group["lr"]
         if isinstance(lr, torch.Tensor):
-            scalars[0].copy_(lr.detach())
+            if not capturing or lr.device == dev:
+                scalars[0].copy_(lr.detach())
+            if capturing:
+                self._captured[id(lr)] = lr
             self._lr.pop(index, None)
-        else:
+        elif not capturing:  # a fill in a graph would put this rate back with every replay
             block, held = self._lr.get(index, (None, None))
             if block is not scalars or held != lr:  # groups may be added, taken out or sorted by hand
                 scalars[0].fill_(lr)
                 self._lr[index] = scalars, lr
         return scalars
 
+    def _uncaptured(self, capturing: bool) -> None:
+        """Moments and scalars made in a capture would start from zero again with every replay."""
+        if capturing:
+            raise RuntimeError("AdamW: a first step cannot be captured; take one with these gradients outside the graph")
+
     def sync_lr(self) -> None:
         """Copies the groups' learning rates to the device (for graph replays; step() does it by itself)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.sync_lr: a captured copy would put these rates back with every replay")
         for i, group in enumerate(self.param_groups):
             if group["params"]:
                 self._group_scalars(i)
@@ -202,6 +214,7 @@ class AdamW(torch.optim.Optimizer):
     def _moments_of(self, p: torch.Tensor, bits: int) -> dict:
         state = self.state[p]
         if "exp_avg" not in state:
+            self._uncaptured(torch.cuda.is_current_stream_capturing())
             if bits == 32:
                 state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
@@ -303,6 +316,7 @@ class AdamW(torch.optim.Optimizer):
         if not launches:
             return loss
         stream = _lib.stream_ptr()
+        scalars = {index: self._group_scalars(index) for index in dict.fromkeys(launch.index for launch in launches)}
         partials, parts = None, 0
         if self.max_norm is not None:
             if self._partials is None:  # as long as the plan: its size depends on the launches alone
@@ -313,12 +327,11 @@ class AdamW(torch.optim.Optimizer):
             for launch in launches:
                 _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
                 at += 4 * launch.parts
-        scalars = {}
-        for index in dict.fromkeys(launch.index for launch in launches):
-            group, scalars[index] = self.param_groups[index], self._group_scalars(index)
+        for index, block in scalars.items():
+            group = self.param_groups[index]
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_prepare", _lib.ptr(partials), parts, self.max_norm or 0.0, b1, b2,
-                      group["weight_decay"], scalars[index].data_ptr(), stream)
+                      group["weight_decay"], block.data_ptr(), stream)
         if self.max_norm is not None and self._norm_of is not scalars[launches[0].index]:
             self._norm_of = scalars[launches[0].index]
             self.grad_norm = self._norm_of[2]

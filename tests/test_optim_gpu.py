@@ -421,3 +421,53 @@ def test_a_group_added_after_a_step(max_norm, given, bits):
         assert float((q.detach().double() - p).abs().max()) <= 2e-5 * lr * 10 + 2.0 ** -22 * float(p.abs().max())
     if bits == 8:
         assert len(opt.moments()) == 4
+
+
+@pytest.mark.parametrize("tensor_rate", [False, True])
+def test_learning_rates_around_a_capture(tensor_rate):
+    """A rate changed before a capture, between replays and behind them: each update takes the rate that was last copied
+    to the device, a graph recorded with a rate on the device the one that is there."""
+    params, twin = _params([300, 2049]), _params([300, 2049])
+    a, b = optim.AdamW(params, max_norm=1.0, **HP), optim.AdamW(twin, max_norm=1.0, **HP)
+    grads = _tensors([300, 2049], seed=2)
+    rate = torch.tensor(5e-3, device=DEV, dtype=torch.float64) if tensor_rate else 5e-3
+    taken = []
+
+    def step():
+        a.step(grads=grads)
+        taken.append(float(a.param_groups[0]["lr"]))
+    step()
+    a.param_groups[0]["lr"] = rate
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(grads=grads)
+    step()  # takes the rate that was set before the capture
+    for lr in (7e-3, 2e-3):
+        if tensor_rate:
+            rate.fill_(lr)
+        else:
+            a.param_groups[0]["lr"] = lr
+            a.sync_lr()
+        graph.replay()
+        graph.replay()
+        taken += [lr, lr]
+    step()
+    for lr in taken:
+        b.param_groups[0]["lr"] = lr
+        b.step(grads=grads)
+    for p, q in zip(params, twin):
+        assert torch.equal(p, q)
+    assert float(a.param_groups[0]["scalars"][1]) == len(taken) == 7.0
+
+
+def test_a_first_step_is_not_captured():
+    p, q = _params([300, 2049])
+    opt = optim.AdamW([p, q], **HP)
+    g = _tensors([300, 2049], seed=2)
+    opt.step(grads=[g[0], None])
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step(grads=g)
+    before = q.detach().clone()
+    opt.step(grads=g)
+    assert not torch.equal(q, before) and bool(q.isfinite().all())

@@ -1,6 +1,8 @@
 """Host side of optim.AdamW on CPU tensors: the library calls are recorded
 instead of launched, so what is planned, allocated and refused is seen without
 a GPU."""
+import weakref
+
 import pytest
 import torch
 
@@ -152,3 +154,53 @@ def test_state_that_is_replaced_or_dropped(recorded, bits):
     opt.state[params[0]]["exp_avg"] = torch.zeros(9)
     with pytest.raises(ValueError, match="exp_avg"):
         step()
+
+
+def test_a_capture_does_not_write_the_learning_rate(recorded):
+    params = _params(1)
+    opt = optim.AdamW(params, lr=1.0)
+    opt.step(grads=_grads(params))
+    scalars = opt.param_groups[0]["scalars"]
+    opt.param_groups[0]["lr"] = 2.0
+    recorded.capturing = True
+    opt.step(grads=_grads(params))
+    assert float(scalars[0]) == 1.0
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.sync_lr()
+    recorded.capturing = False
+    opt.step(grads=_grads(params))  # nor does a capture note it as written
+    assert float(scalars[0]) == 2.0
+    rate = torch.tensor(3.0)  # a tensor on the parameters' device: replays read it, so it is kept
+    opt.param_groups[0]["lr"] = rate
+    recorded.capturing = True
+    opt.step(grads=_grads(params))
+    assert float(scalars[0]) == 3.0
+    gone = weakref.ref(rate)
+    opt.param_groups[0]["lr"] = 2.0
+    del rate
+    assert gone() is not None
+
+
+def test_a_first_step_is_not_captured(recorded):
+    params = _params(3)
+    opt = optim.AdamW([dict(params=params[:2]), dict(params=params[2:])])
+    g = _grads(params)
+    recorded.capturing = True
+    with pytest.raises(RuntimeError, match="first step"):
+        opt.step(grads=[g[0], None, None])
+    recorded.capturing = False
+    opt.step(grads=[g[0], None, None])
+    recorded.capturing = True
+    opt.step(grads=[g[0], None, None])
+    for grads in ([g[0], g[1], None], [g[0], None, g[2]]):
+        with pytest.raises(RuntimeError, match="first step"):
+            opt.step(grads=grads)
+    opt.step(grads=[g[0], None, None])
+    for name in ("exp_avg", "exp_avg_sq"):
+        opt.state[params[2]][name] = torch.zeros(10)
+    with pytest.raises(RuntimeError, match="first step"):  # its group has no count yet
+        opt.step(grads=g[:1] + [None] + g[2:])
+    recorded.capturing = False
+    opt.step(grads=g)
+    recorded.capturing = True
+    opt.step(grads=g)
