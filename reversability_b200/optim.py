@@ -123,7 +123,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("max_norm must be positive")
         self.max_norm = max_norm
         self.grad_norm = None  # the gradients' global norm before clipping in the last step (device scalar)
-        self._captured = {}    # by id, what captured graphs go on reading
+        self._captured = {}    # by id, what captured graphs go on reading and writing
+        self._partials = []    # workspaces of the norm, the last one in use
         self._reset()
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       scalars=None))
@@ -135,7 +136,6 @@ class AdamW(torch.optim.Optimizer):
         self._idle = []        # (place, parameter) outside it
         self._coded = None     # the table of the parameters with 8-bit moments
         self._coded_of = ()    # the optimizer's state when it was made
-        self._partials = None  # the norm's workspace
         self._norm_of = None   # the scalars that grad_norm is a view of
         self._lr = {}          # group index -> (its device scalars, the learning rate they hold)
 
@@ -145,7 +145,8 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         self.grad_norm = None
-        self._captured = {}
+        self.__dict__.setdefault("_captured", {})  # load_state_dict comes here too
+        self.__dict__.setdefault("_partials", [])
         self._reset()
 
     def add_param_group(self, param_group) -> None:
@@ -275,7 +276,7 @@ class AdamW(torch.optim.Optimizer):
     def _collect(self, grads) -> list:
         """Checks the gradients and plans the launches for them; returns what has to live until those are queued."""
         found = []  # (group index, parameter, gradient, the parameter's place among all)
-        self._launches, self._idle, self._coded, self._partials = None, [], None, None
+        self._launches, self._idle, self._coded = None, [], None
         device = torch.cuda.current_device()
         places = itertools.count()
         for index, group in enumerate(self.param_groups):
@@ -297,6 +298,20 @@ class AdamW(torch.optim.Optimizer):
         self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
 
+    def _norm_workspace(self, parts: int, device: torch.device) -> torch.Tensor:
+        """At least `parts` floats. A workspace is never given back: a captured graph or another stream may still write
+        to it."""
+        if not self._partials or self._partials[-1].numel() < parts or self._partials[-1].device != device:
+            self._partials.append(torch.empty(parts, device=device, dtype=torch.float32))
+        return self._partials[-1]
+
+    def _keep_for_replays(self, launches, scalars=()) -> None:
+        """Holds the moments and scalars whose addresses a capture is about to record: a state that is loaded or put in
+        their place must not leave replays with memory that belongs to others. Parameters and gradients are the
+        caller's to hold, as with any captured graph."""
+        for t in itertools.chain(scalars, *(launch.moments for launch in launches)):
+            self._captured[id(t)] = t
+
     # ---- the step
     def step(self, closure=None, *, grads=None):
         """One update. grads: gradients in the order of the parameters over all groups (None where there is none),
@@ -317,12 +332,12 @@ class AdamW(torch.optim.Optimizer):
             return loss
         stream = _lib.stream_ptr()
         scalars = {index: self._group_scalars(index) for index in dict.fromkeys(launch.index for launch in launches)}
+        if torch.cuda.is_current_stream_capturing():
+            self._keep_for_replays(launches, scalars.values())
         partials, parts = None, 0
         if self.max_norm is not None:
-            if self._partials is None:  # as long as the plan: its size depends on the launches alone
-                parts = sum(launch.parts for launch in launches)
-                self._partials = torch.empty(parts, device=launches[0].entries[0][0].device, dtype=torch.float32)
-            partials, parts = self._partials, self._partials.numel()
+            parts = sum(launch.parts for launch in launches)
+            partials = self._norm_workspace(parts, launches[0].entries[0][0].device)
             at = partials.data_ptr()
             for launch in launches:
                 _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
@@ -371,5 +386,7 @@ class AdamW(torch.optim.Optimizer):
             table[field] = m.data_ptr()
             table[field + 1] = v.data_ptr()
             field += _FIELDS
+        if torch.cuda.is_current_stream_capturing():
+            self._keep_for_replays([coded])
         _lib.call("rk_adamw_multi_moments", table, len(out), _lib.code(kind), _lib.stream_ptr())
         return out

@@ -471,3 +471,26 @@ def test_a_first_step_is_not_captured():
     before = q.detach().clone()
     opt.step(grads=g)
     assert not torch.equal(q, before) and bool(q.isfinite().all())
+
+
+def test_an_eager_step_with_other_gradients_between_replays():
+    """The plan of an eager step leaves a captured graph its workspace: replays give the gradients' norm and write to
+    nothing that was allocated since."""
+    params = _params([300, 2049])
+    opt = optim.AdamW(params, max_norm=1.0, **HP)
+    grads = _tensors([300, 2049], seed=2)
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    opt.step(grads=grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(grads=grads)
+    opt.step(grads=[grads[0], None])
+    opt.step(grads=[grads[0].bfloat16(), grads[1]])
+    others = [torch.full((n,), 7.0, device=DEV) for n in (128, 512, 592, 600, 1184, 4096) for _ in range(20)]
+    for _ in range(2):
+        graph.replay()
+        assert abs(float(opt.param_groups[0]["scalars"][2]) - norm) <= 1e-5 * norm
+    assert all(bool((t == 7.0).all()) for t in others)
+    opt.step(grads=grads)
+    assert abs(float(opt.grad_norm) - norm) <= 1e-5 * norm
+    assert all(bool(p.isfinite().all()) for p in params)

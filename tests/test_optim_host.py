@@ -204,3 +204,60 @@ def test_a_first_step_is_not_captured(recorded):
     opt.step(grads=g)
     recorded.capturing = True
     opt.step(grads=g)
+
+
+def test_the_workspace_of_the_norm_outlives_plans(recorded, monkeypatch):
+    """What a captured graph has been given stays where it is when the plan is made anew, also a smaller or a larger one."""
+    params, made, empty = _params(70), [], torch.empty
+
+    def allocate(*args, **kwargs):
+        t = empty(*args, **kwargs)
+        made.append((weakref.ref(t), t.data_ptr(), t.data_ptr() + 4 * t.numel()))
+        return t
+    monkeypatch.setattr(torch, "empty", allocate)
+
+    def inside(a, b):
+        return any(r() is not None and first <= a and b <= end for r, first, end in made)
+    opt = optim.AdamW(params, max_norm=1.0)
+    g = _grads(params)
+    opt.step(grads=g)
+    recorded.capturing = True
+    recorded.calls.clear()
+    opt.step(grads=g)
+    recorded.capturing = False
+    at = [args[3] for args in recorded.named("rk_adamw_multi_sumsq")]
+    prepare, = recorded.named("rk_adamw_multi_prepare")
+    assert at[0] == prepare[0] and inside(at[0], at[0] + 4 * prepare[1])
+
+    def some(n, dtype=torch.float32):
+        return [x.to(dtype) if i < n else None for i, x in enumerate(g)]
+    for grads in (some(3), some(70), some(69), some(70, torch.bfloat16), [x.bfloat16() if i % 2 else x for i, x in enumerate(g)]):
+        recorded.calls.clear()
+        opt.step(grads=grads)
+        calls = recorded.named("rk_adamw_multi_sumsq")
+        (begin, parts, *_), = recorded.named("rk_adamw_multi_prepare")
+        assert parts == sum(_lib.lib().rk_adamw_multi_parts(args[1]) for args in calls)  # no part that nothing has written
+        ends = [args[3] + 4 * _lib.lib().rk_adamw_multi_parts(args[1]) for args in calls]
+        assert [args[3] for args in calls] == [begin] + ends[:-1]
+        assert inside(begin, ends[-1])
+    more = _params(70)
+    opt.add_param_group(dict(params=more))
+    opt.step(grads=g + _grads(more))
+    opt.load_state_dict(opt.state_dict())
+    opt.step(grads=g + _grads(more))
+    assert inside(at[0], at[0] + 4 * prepare[1])
+
+
+def test_what_a_capture_has_seen_outlives_the_state(recorded):
+    params = _params(2)
+    opt = optim.AdamW([dict(params=params[:1]), dict(params=params[1:], state_bits=8)])
+    opt.step(grads=_grads(params))
+    recorded.capturing = True
+    opt.step(grads=_grads(params))
+    opt.moments()
+    recorded.capturing = False
+    seen = [weakref.ref(t) for s in opt.state.values() for t in s.values()]
+    seen += [weakref.ref(group["scalars"]) for group in opt.param_groups]
+    opt.load_state_dict(opt.state_dict())
+    opt.step(grads=_grads(params))
+    assert all(r() is not None for r in seen)
