@@ -20,6 +20,7 @@ from . import functional as fn
 
 QUANT_BLOCK = 256  # elements that share a scale in 8-bit moments
 _FIELDS = 7        # 8-byte fields of rk_adamw_tensor
+_NO_RATE = (None, None)
 
 
 def _seen(state) -> tuple[list, list]:
@@ -34,11 +35,12 @@ def _same(seen, state) -> bool:
 
 
 class _Launch:
-    """The tensors of one group with one parameter and one gradient type: their rk_adamw_tensor array, whose moment
-    addresses and sizes stay from step to step while p and g are written anew in each."""
+    """The tensors of one group with one parameter and one gradient type and one count of steps: their rk_adamw_tensor
+    array, whose moment addresses and sizes stay from step to step while p and g are written anew in each."""
 
-    def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype):
+    def __init__(self, index: int, bits: int, p_dtype: torch.dtype, g_dtype: torch.dtype, block: torch.Tensor | None = None):
         self.index, self.bits, self.p_dtype, self.g_dtype = index, bits, p_dtype, g_dtype
+        self.block, self.counter = block, (index, id(block))  # the scalars that count their steps, None for the group's
         self.p_code, self.g_code = _lib.code(p_dtype), _lib.code(g_dtype)
         self.entries = []  # (parameter, elements, place among all parameters)
         self.flat = []
@@ -111,8 +113,12 @@ class AdamW(torch.optim.Optimizer):
     max_norm: clip the gradients' global norm over all groups to it (torch.nn.utils.clip_grad_norm_ without its
     rescaling pass over the gradients); the norm of the last step is `grad_norm`, a device scalar.
 
-    A group counts one step for each step() that finds a gradient in it. Step count, learning rate and the derived
-    constants live on the device, so a captured graph that contains step() counts on when it is replayed; a learning
+    Each tensor counts the steps that found a gradient for it. Tensors that have always stepped together share their
+    scalars: the group's (param_groups[i]["scalars"], which hold its learning rate too) or, for those that came in late
+    or were left out of a step, a copy of their own (state[p]["scalars"]), with a launch of its own. A captured graph
+    counts the tensors together that it was captured with.
+
+    Step count, learning rate and the derived constants live on the device, so a captured graph that contains step() counts on when it is replayed; a learning
     rate changed in param_groups is copied there by the next step() outside a graph, or by sync_lr(), and never by a
     capture, except that a rate given as a tensor on the device is read from that tensor by each replay. What a step()
     makes for itself cannot be captured: take a first step, with the same gradients, outside the graph."""
@@ -137,7 +143,8 @@ class AdamW(torch.optim.Optimizer):
         self._coded = None     # the table of the parameters with 8-bit moments
         self._coded_of = ()    # the optimizer's state when it was made
         self._norm_of = None   # the scalars that grad_norm is a view of
-        self._lr = {}          # group index -> (its device scalars, the learning rate they hold)
+        self._lr = {}          # by id, device scalars and the learning rate that they hold
+        self._counted = {}     # by id, the groups' scalars that steps have counted in
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm}
@@ -173,28 +180,67 @@ class AdamW(torch.optim.Optimizer):
         """fp32[8] of the group on its device: [0] lr, [1] steps taken, [2] gradient norm, [3] clip coefficient."""
         group = self.param_groups[index]
         dev = group["params"][0].device
-        scalars, capturing = group["scalars"], torch.cuda.is_current_stream_capturing()
+        scalars = group["scalars"]
         if scalars is None or scalars.device != dev:
-            self._uncaptured(capturing)
+            self._uncaptured()
             scalars = torch.zeros(8, device=dev, dtype=torch.float32) if scalars is None else scalars.to(dev)
             group["scalars"] = scalars
-        lr = group["lr"]
+        return self._with_rate(scalars, group["lr"])
+
+    def _with_rate(self, scalars: torch.Tensor, lr) -> torch.Tensor:
+        """The scalars, holding this learning rate."""
         if isinstance(lr, torch.Tensor):
-            if not capturing or lr.device == dev:
+            capturing = torch.cuda.is_current_stream_capturing()
+            if not capturing or lr.device == scalars.device:
                 scalars[0].copy_(lr.detach())
             if capturing:
                 self._captured[id(lr)] = lr
-            self._lr.pop(index, None)
-        elif not capturing:  # a fill in a graph would put this rate back with every replay
-            block, held = self._lr.get(index, (None, None))
-            if block is not scalars or held != lr:  # groups may be added, taken out or sorted by hand
-                scalars[0].fill_(lr)
-                self._lr[index] = scalars, lr
+            self._lr.pop(id(scalars), None)
+        elif self._lr.get(id(scalars), _NO_RATE)[1] != lr and not torch.cuda.is_current_stream_capturing():
+            scalars[0].fill_(lr)  # in a graph it would put this rate back with every replay
+            self._lr[id(scalars)] = scalars, lr
         return scalars
 
-    def _uncaptured(self, capturing: bool) -> None:
-        """Moments and scalars made in a capture would start from zero again with every replay."""
-        if capturing:
+    def _all_scalars(self, index: int) -> list[torch.Tensor]:
+        """The group's scalars and those that its tensors have of their own."""
+        group = self.param_groups[index]
+        own = (self.state[p]["scalars"] for p in group["params"] if p in self.state and "scalars" in self.state[p])
+        blocks = {id(t): t for t in (self._group_scalars(index), *own)}
+        return [self._with_rate(t, group["lr"]) for t in blocks.values()]
+
+    def _count(self, found) -> None:
+        """Parts the counts of tensors that no longer step together, before a step with these (group index, parameter,
+        gradient, place) tuples: those of a block that are left out go on with a copy of it; those without moments start
+        from zero, on the group's scalars if none has stepped there."""
+        live = {id(p) for _, p, _, _ in found}
+        for index, group in enumerate(self.param_groups):
+            blocks, new = {}, []
+            for p in group["params"]:
+                state = self.state.get(p)
+                if state and "exp_avg" in state:
+                    block = state.get("scalars")
+                    blocks.setdefault(id(block), (block, [], []))[1 if id(p) in live else 2].append(state)
+                elif id(p) in live:
+                    new.append(p)
+            for block, steps, rests in blocks.values():
+                if steps and rests:
+                    self._uncaptured()
+                    copy = (self._group_scalars(index) if block is None else block).clone()
+                    for state in rests:
+                        state["scalars"] = copy
+            if new and group["scalars"] is not None:
+                if blocks:
+                    self._uncaptured()
+                    block = torch.zeros(8, device=new[0].device, dtype=torch.float32)
+                    for p in new:
+                        self.state[p]["scalars"] = block
+                elif id(group["scalars"]) in self._counted:  # all moments have been dropped
+                    self._uncaptured()
+                    group["scalars"] = None
+
+    def _uncaptured(self) -> None:
+        """Moments and scalars made in a capture would start anew with every replay."""
+        if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: a first step cannot be captured; take one with these gradients outside the graph")
 
     def sync_lr(self) -> None:
@@ -203,19 +249,21 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW.sync_lr: a captured copy would put these rates back with every replay")
         for i, group in enumerate(self.param_groups):
             if group["params"]:
-                self._group_scalars(i)
+                self._all_scalars(i)
 
     def set_step(self, step: int) -> None:
         """Sets the number of steps already taken (bias correction), as when moments come from elsewhere."""
         for i, group in enumerate(self.param_groups):
             if group["params"]:
-                self._group_scalars(i)[1].fill_(float(step))
+                for scalars in self._all_scalars(i):
+                    scalars[1].fill_(float(step))
+        self._counted, self._launches = {}, None  # no step has counted on from here
 
     # ---- state
     def _moments_of(self, p: torch.Tensor, bits: int) -> dict:
         state = self.state[p]
         if "exp_avg" not in state:
-            self._uncaptured(torch.cuda.is_current_stream_capturing())
+            self._uncaptured()
             if bits == 32:
                 state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
@@ -233,10 +281,15 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         saved = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         own = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        copies = {}  # what tensors share stays shared
+
+        def copy(v, device):
+            if not isinstance(v, torch.Tensor):
+                return v
+            return copies.setdefault((id(v), device), v.detach().to(device, copy=True))
         for key, p in zip(saved, own):
             if key in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in state_dict["state"][key].items()}
+                self.state[p] = {k: copy(v, p.device) for k, v in state_dict["state"][key].items()}
         self._reset()
 
     def _plan(self, found) -> list[_Launch]:
@@ -248,9 +301,12 @@ class AdamW(torch.optim.Optimizer):
             bits = self.param_groups[index]["state_bits"]
             if bits not in (8, 32):
                 raise ValueError("state_bits must be 8 or 32")
-            key = index, p.dtype, g.dtype
+            block = self.state[p].get("scalars")
+            if block is not None and block.device != p.device:
+                raise ValueError("scalars must be on the parameter's device")
+            key = index, id(block), p.dtype, g.dtype
             if key not in launches:
-                launches[key] = _Launch(index, bits, p.dtype, g.dtype)
+                launches[key] = _Launch(index, bits, p.dtype, g.dtype, block)
             launches[key].add(p, g, self._moments_of(p, bits), i)
         return [launch.finish() for launch in launches.values()]
 
@@ -293,7 +349,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("AdamW parameters with gradients must be on the current CUDA device")
                 else:
                     found.append((index, p, g if g.is_contiguous() else g.contiguous(), i))
+        self._count(found)
         self._launches = self._plan(found)
+        for launch in self._launches:
+            if launch.block is None:
+                block = self._group_scalars(launch.index)
+                self._counted[id(block)] = block
         self._state_of = _seen(self.state)
         self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
@@ -331,7 +392,11 @@ class AdamW(torch.optim.Optimizer):
         if not launches:
             return loss
         stream = _lib.stream_ptr()
-        scalars = {index: self._group_scalars(index) for index in dict.fromkeys(launch.index for launch in launches)}
+        scalars = {}
+        for launch in launches:
+            if launch.counter not in scalars:
+                scalars[launch.counter] = self._group_scalars(launch.index) if launch.block is None else \
+                    self._with_rate(launch.block, self.param_groups[launch.index]["lr"])
         if torch.cuda.is_current_stream_capturing():
             self._keep_for_replays(launches, scalars.values())
         partials, parts = None, 0
@@ -342,19 +407,19 @@ class AdamW(torch.optim.Optimizer):
             for launch in launches:
                 _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
                 at += 4 * launch.parts
-        for index, block in scalars.items():
+        for (index, _), block in scalars.items():
             group = self.param_groups[index]
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_prepare", _lib.ptr(partials), parts, self.max_norm or 0.0, b1, b2,
                       group["weight_decay"], block.data_ptr(), stream)
-        if self.max_norm is not None and self._norm_of is not scalars[launches[0].index]:
-            self._norm_of = scalars[launches[0].index]
+        if self.max_norm is not None and self._norm_of is not scalars[launches[0].counter]:
+            self._norm_of = scalars[launches[0].counter]
             self.grad_norm = self._norm_of[2]
         for launch in launches:
             group = self.param_groups[launch.index]
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_step", launch.table, len(launch.entries), launch.p_code, launch.g_code, launch.bits,
-                      scalars[launch.index].data_ptr(), b1, b2, group["eps"], stream)
+                      scalars[launch.counter].data_ptr(), b1, b2, group["eps"], stream)
         del keep
         return loss
 

@@ -494,3 +494,44 @@ def test_an_eager_step_with_other_gradients_between_replays():
     opt.step(grads=grads)
     assert abs(float(opt.grad_norm) - norm) <= 1e-5 * norm
     assert all(bool(p.isfinite().all()) for p in params)
+
+
+def test_tensors_that_come_late_or_rest_follow_torch_adamw():
+    """Each tensor's bias correction goes by its own steps: against torch.optim.AdamW, whose fp32 arithmetic is as far off
+    as this one's, with the default betas, over steps that leave out changing tensors."""
+    sizes = [300, 2049, 7, 513, 1000]
+    a, b = _params(sizes), _params(sizes)
+    hp = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    oa, ob = optim.AdamW(a, **hp), torch.optim.AdamW(b, **hp)
+    live = [(0, 1), (0, 1), (0, 1, 2), (0, 2), (3,), (0, 1, 2, 3, 4), (1, 4), (0, 1, 2, 3, 4), (0, 1, 2, 3, 4), (2, 3)]
+    for k, now in enumerate(live):
+        grads = _tensors(sizes, seed=60 + k)
+        for i in range(5):
+            a[i].grad = b[i].grad = grads[i] if i in now else None
+        oa.step()
+        ob.step()
+        for p, q in zip(a, b):
+            # as in the test beside torch's on a model; an update is at most lr / (1 - b1), and a first one 1 / (1 - b1^t)
+            assert float((p - q).detach().abs().max()) <= 2.0 ** -18 * hp["lr"] * 10 * (k + 1) + 1e-7
+    steps = [float(oa.state[p].get("scalars", oa.param_groups[0]["scalars"])[1]) for p in a]
+    assert steps == [sum(i in now for now in live) for i in range(5)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_late_tensors_survive_a_round_trip(bits, tmp_path):
+    sizes = [300, 2049, 7]
+    params = _params(sizes)
+    opt = optim.AdamW(params, state_bits=bits, max_norm=1.0, **HP)
+    for k, now in enumerate([(0,), (0, 1), (1, 2), (0, 1, 2)]):
+        grads = _tensors(sizes, seed=k)
+        opt.step(grads=[g if i in now else None for i, g in enumerate(grads)])
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = optim.AdamW(twin, state_bits=bits, max_norm=1.0, **HP)
+    other.load_state_dict(torch.load(tmp_path / "opt.pt", map_location="cpu"))
+    for k in range(2):
+        grads = _tensors(sizes, seed=10 + k)
+        opt.step(grads=grads)
+        other.step(grads=[g.clone() for g in grads])
+    assert all(torch.equal(p, q) for p, q in zip(params, twin))
+    assert float(opt.grad_norm) == float(other.grad_norm)

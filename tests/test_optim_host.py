@@ -121,8 +121,9 @@ def test_a_number_after_a_learning_rate_tensor(recorded):
 
 def _used(recorded, opt, params):
     """Whether the last step was given the moments that the optimizer's state holds."""
-    args, = recorded.named("rk_adamw_multi_step")
-    for i, p in enumerate(params):
+    given = {args[0][i * 7]: (args, i) for args in recorded.named("rk_adamw_multi_step") for i in range(args[1])}
+    for p in params:
+        args, i = given[p.data_ptr()]
         names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if args[4] == 8 else 2]
         assert [args[0][i * 7 + 2 + k] for k in range(len(names))] == [opt.state[p][name].data_ptr() for name in names]
 
@@ -235,7 +236,7 @@ def test_the_workspace_of_the_norm_outlives_plans(recorded, monkeypatch):
         recorded.calls.clear()
         opt.step(grads=grads)
         calls = recorded.named("rk_adamw_multi_sumsq")
-        (begin, parts, *_), = recorded.named("rk_adamw_multi_prepare")
+        (begin, parts), = {args[:2] for args in recorded.named("rk_adamw_multi_prepare")}
         assert parts == sum(_lib.lib().rk_adamw_multi_parts(args[1]) for args in calls)  # no part that nothing has written
         ends = [args[3] + 4 * _lib.lib().rk_adamw_multi_parts(args[1]) for args in calls]
         assert [args[3] for args in calls] == [begin] + ends[:-1]
@@ -261,3 +262,87 @@ def test_what_a_capture_has_seen_outlives_the_state(recorded):
     opt.load_state_dict(opt.state_dict())
     opt.step(grads=_grads(params))
     assert all(r() is not None for r in seen)
+
+
+def _counts(recorded, opt):
+    """Lets the recorded prepares count, as they do on the device; the counts of all parameters with moments."""
+    blocks = {t.data_ptr(): t for t in [g["scalars"] for g in opt.param_groups if g["scalars"] is not None]
+              + [s["scalars"] for s in opt.state.values() if "scalars" in s]}
+    for args in recorded.named("rk_adamw_multi_prepare"):
+        blocks[args[6]][1] += 1
+    recorded.calls.clear()
+    return [float(opt.state[p].get("scalars", g["scalars"])[1]) for g in opt.param_groups for p in g["params"]
+            if "exp_avg" in opt.state.get(p, ())]
+
+
+def test_each_tensor_counts_its_own_steps(recorded):
+    params = _params(5)
+    opt = optim.AdamW([dict(params=params[:4]), dict(params=params[4:])])
+    want, g = [0.0] * 5, _grads(params)
+    for live in ((0, 1, 4), (0, 1), (0, 1, 2), (2, 3), (0, 1, 2, 3, 4), (0, 3), (0, 1, 2, 3, 4), (4,), (0, 1, 2, 3, 4)):
+        opt.step(grads=[x if i in live else None for i, x in enumerate(g)])
+        want = [w + (i in live) for i, w in enumerate(want)]
+        launches = len(recorded.named("rk_adamw_multi_step"))
+        assert launches == len(recorded.named("rk_adamw_multi_prepare")) >= len({(i == 4, want[i]) for i in live})
+        assert _counts(recorded, opt) == [w for w in want if w]
+    again = optim.AdamW([dict(params=params[:4]), dict(params=params[4:])])
+    again.load_state_dict(opt.state_dict())
+    opt.step(grads=g)
+    launches = len(recorded.named("rk_adamw_multi_step"))
+    recorded.calls.clear()
+    again.step(grads=g)
+    assert len(recorded.named("rk_adamw_multi_step")) == launches  # who counted together still does
+    assert _counts(recorded, again) == [w + 1 for w in want]
+    again.set_step(7)
+    again.step(grads=g)
+    assert _counts(recorded, again) == [8.0] * 5
+    again.param_groups[0]["lr"] = 0.5
+    again.sync_lr()
+    assert all(float(again.state[p].get("scalars", again.param_groups[0]["scalars"])[0]) == 0.5 for p in params[:4])
+
+
+def test_tensors_that_step_together_stay_in_one_launch(recorded):
+    params = _params(6)
+    opt = optim.AdamW(params)
+    g = _grads(params)
+    opt.step(grads=g[:4] + [None, None])
+    for _ in range(3):  # two frozen from here on
+        recorded.calls.clear()
+        opt.step(grads=[None, None] + g[2:4] + [None, None])
+        assert len(recorded.named("rk_adamw_multi_step")) == 1
+    recorded.calls.clear()
+    opt.step(grads=g)  # three histories: the frozen, those that went on, those that are new
+    assert len(recorded.named("rk_adamw_multi_step")) == 3
+
+
+def test_dropped_moments_start_from_zero(recorded):
+    params = _params(2)
+    opt = optim.AdamW(params)
+    for _ in range(3):
+        opt.step(grads=_grads(params))
+    assert _counts(recorded, opt) == [3.0, 3.0]
+    opt.state.clear()
+    opt.step(grads=_grads(params))
+    assert _counts(recorded, opt) == [1.0, 1.0]
+    opt.state.pop(params[1])
+    opt.step(grads=_grads(params))
+    assert _counts(recorded, opt) == [2.0, 1.0]
+    by_hand = optim.AdamW(params)
+    for p in params:
+        by_hand.state[p].update(exp_avg=torch.zeros(10), exp_avg_sq=torch.zeros(10))
+    by_hand.step(grads=[None, torch.ones(10)])
+    assert _counts(recorded, by_hand) == [0.0, 1.0]
+    fresh = optim.AdamW(params)
+    fresh.set_step(40)  # before the first step: moments from elsewhere, or none yet
+    fresh.step(grads=_grads(params))
+    assert _counts(recorded, fresh) == [41.0, 41.0]
+
+
+def test_a_capture_does_not_part_counts(recorded):
+    params = _params(2)
+    opt = optim.AdamW(params)
+    opt.step(grads=_grads(params))
+    recorded.capturing = True
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step(grads=[torch.ones(10), None])
+    assert "scalars" not in opt.state[params[1]]
