@@ -277,7 +277,13 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer.load_state_dict, but the moments keep their saved types (the base class would
-        cast codes and fp32 moments to the parameters' type)."""
+        cast codes and fp32 moments to the parameters' type). Refuses the state of another optimizer."""
+        for group in state_dict["param_groups"]:
+            missing = {"lr", "betas", "eps", "weight_decay", "state_bits", "scalars"} - set(group)
+            if missing:
+                raise ValueError("not the state of an optim.AdamW of this package: its groups have no " +
+                                 ", ".join(sorted(missing)) + ". To take over moments from another optimizer, put them into "
+                                 "state[p] as fp32 exp_avg and exp_avg_sq and call set_step()")
         super().load_state_dict(state_dict)
         saved = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         own = itertools.chain.from_iterable(g["params"] for g in self.param_groups)

@@ -346,3 +346,27 @@ def test_a_capture_does_not_part_counts(recorded):
     with pytest.raises(RuntimeError, match="captured"):
         opt.step(grads=[torch.ones(10), None])
     assert "scalars" not in opt.state[params[1]]
+
+
+def test_the_state_of_another_optimizer_is_refused(recorded):
+    params = _params(2)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    other = torch.optim.AdamW(params)
+    other.step()
+    opt = optim.AdamW(params, lr=0.5)
+    opt.step()
+    before = [dict(s) for s in opt.state.values()]
+    with pytest.raises(ValueError, match="scalars, state_bits"):
+        opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5 and all(a[k] is s[k] for a, s in zip(before, opt.state.values()) for k in a)
+    opt.step()
+    # the way that the refusal names
+    new = optim.AdamW(params)
+    for p in params:
+        new.state[p].update({k: other.state[p][k].clone() for k in ("exp_avg", "exp_avg_sq")})
+    new.set_step(int(other.state[params[0]]["step"]))
+    recorded.calls.clear()
+    new.step()
+    _used(recorded, new, params)
+    assert _counts(recorded, new) == [2.0, 2.0]
