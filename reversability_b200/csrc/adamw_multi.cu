@@ -147,12 +147,17 @@ struct StepConst {
   float coef, step_size, root, decay, beta1, beta2, eps;
 };
 
-// One element: m and v become the new moments, r = sqrt(v), p the new parameter.
+// One element: m and v become the new moments, r = sqrt(v), p the new parameter. The approximate root and reciprocal are
+// within 2^-22 together and leave the update as near to 64 bits as exact ones do the plain fp32 form (0.97 times its rms
+// error; exact ones 0.90, at 14 % more time with 8-bit moments). DENORMAL: the root of a denormal v too, which otherwise
+// counts as 0, and with a small eps the update as infinite.
+template <bool DENORMAL>
 __device__ __forceinline__ void adamw_element(const StepConst& k, float g, float& p, float& m, float& v, float& r) {
   const float gi = g * k.coef;
   m = fmaf(1.f - k.beta1, gi - m, m);
   v = fmaf(k.beta2, v, (1.f - k.beta2) * gi * gi);
-  r = sqrt_approx(v);
+  if constexpr (DENORMAL) asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  else r = sqrt_approx(v);
   p = fmaf(p, k.decay, -(k.step_size * m * rcp_approx(fmaf(r, k.root, k.eps))));
 }
 
@@ -191,7 +196,7 @@ __device__ __forceinline__ void load_block(const rk_adamw_tensor& t, int64_t blo
     }
   }
 }
-template <typename TP, typename TG, bool Q8, bool WHOLE>
+template <typename TP, typename TG, bool Q8, bool WHOLE, bool DENORMAL>
 __device__ __forceinline__ void update_block(const rk_adamw_tensor& t, int64_t block, BlockIn<TP, TG, Q8>& in,
                                              const StepConst& k) {
   const int64_t at = block * kQBlock + (threadIdx.x & 31) * 4;
@@ -206,7 +211,7 @@ __device__ __forceinline__ void update_block(const rk_adamw_tensor& t, int64_t b
     const int left = left_of(t, at + h * 128, WHOLE);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      adamw_element(k, in.g[h][e], in.p[h][e], in.m[h][e], in.v[h][e], r[h][e]);
+      adamw_element<DENORMAL>(k, in.g[h][e], in.p[h][e], in.m[h][e], in.v[h][e], r[h][e]);
       if constexpr (Q8) {
         mm = max_bits(mm, in.m[h][e]);
         rm = max_bits(rm, r[h][e]);
@@ -297,7 +302,7 @@ __device__ __forceinline__ bool vec_ok(const void* p, int size) {
   return (reinterpret_cast<uintptr_t>(p) & (4 * size - 1)) == 0;
 }
 
-template <typename TP, typename TG, bool Q8>
+template <typename TP, typename TG, bool Q8, bool DENORMAL>
 __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant__ MultiTable tab,
                                                           const float* __restrict__ scalars, float beta1, float beta2,
                                                           float eps) {
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
       in.ms = __shfl_sync(0xffffffffu, ms, i);
       in.vs = __shfl_sync(0xffffffffu, vs, i);
     }
-    update_block<TP, TG, Q8, decltype(is_whole)::value>(t, block + i * kStep, in, k);
+    update_block<TP, TG, Q8, decltype(is_whole)::value, DENORMAL>(t, block + i * kStep, in, k);
     if (Q8 && lane == i) {
       ms = in.ms;
       vs = in.vs;
@@ -539,6 +544,11 @@ int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, i
   return i;
 }
 
+// Below it the kernels take the root of a denormal second moment: it is at most 1e-19, 1e-17 once it is corrected for
+// beta2 = 0.9999, so beside a larger eps nothing is lost with it. 456M elements with 8-bit moments, us without and with:
+// fp32 1086/1086, bf16 gradients 978/980, bf16 parameters too 849/880. With 32-bit moments, 1869/1869, always.
+constexpr float kSmallEps = 1e-10f;
+
 template <typename TP, typename TG>
 int step_typed(const rk_adamw_tensor* tensors, int64_t n, int bits, const float* scalars, float beta1, float beta2,
                float eps, cudaStream_t s) {
@@ -549,12 +559,12 @@ int step_typed(const rk_adamw_tensor* tensors, int64_t n, int bits, const float*
     if (i < 0) return RK_ERR_ARG;
     if (tab.n == 0) continue;
     if (bits == 8) {
-      auto kernel = adamw_multi_kernel<TP, TG, true>;
+      auto kernel = eps < kSmallEps ? adamw_multi_kernel<TP, TG, true, true> : adamw_multi_kernel<TP, TG, true, false>;
       const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kernel), step_smem<TP, TG, true>());
       if (e) return e;
       rk_host::launch_k(kernel, (unsigned)tab.start[tab.n], 256, step_smem<TP, TG, true>(), s, tab, scalars, beta1, beta2, eps);
     } else
-      rk_host::launch_k(adamw_multi_kernel<TP, TG, false>, (unsigned)tab.start[tab.n], 256, 0, s, tab, scalars, beta1, beta2, eps);
+      rk_host::launch_k(adamw_multi_kernel<TP, TG, false, true>, (unsigned)tab.start[tab.n], 256, 0, s, tab, scalars, beta1, beta2, eps);
     const int st = rk_host::launch_status();
     if (st) return st;
   }

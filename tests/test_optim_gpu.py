@@ -535,3 +535,45 @@ def test_late_tensors_survive_a_round_trip(bits, tmp_path):
         other.step(grads=[g.clone() for g in grads])
     assert all(torch.equal(p, q) for p, q in zip(params, twin))
     assert float(opt.grad_norm) == float(other.grad_norm)
+
+
+def test_an_update_is_as_near_to_64_bits_as_the_plain_form():
+    """The kernel rounds no more often than the plain fp32 form, operation by operation (products fused into sums round
+    less): over many elements its error is that form's, to a tenth. The betas are exact in fp32, parameters 0, so
+    that the update itself is what is rounded last."""
+    n, b1, b2, lr, eps, step = 1 << 18, 0.875, 0.96875, 1e-2, 1e-8, 40
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    g, m, v = (torch.randn(n, generator=gen, device=DEV) for _ in range(3))
+    v = v.square() + 1e-3
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = optim.AdamW([p], lr=lr, betas=(b1, b2), eps=eps, weight_decay=0.0)
+    opt.state[p].update(exp_avg=m.clone(), exp_avg_sq=v.clone())
+    opt.set_step(step - 1)
+    opt.step(grads=[g])
+    a, s = lr / (1 - b1 ** step), math.sqrt(1 - b2 ** step)
+    ours = opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"], p.detach()
+    mp = m + (1 - b1) * (g - m)
+    vp = b2 * v + (1 - b2) * g * g
+    plain = mp, vp, -a * (mp / (vp.sqrt() / s + eps))
+    m64, g64, v64 = m.double(), g.double(), v.double()
+    me = b1 * m64 + (1 - b1) * g64
+    ve = b2 * v64 + (1 - b2) * g64 * g64
+    exact = me, ve, -a * (me / (ve.sqrt() / s + eps))
+    for got, other, want in zip(ours, plain, exact):
+        off, its = ((t.double() - want).square().mean().sqrt() for t in (got, other))
+        assert float(off) <= 1.1 * float(its) + 1e-12 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_whose_squares_are_denormal(bits):
+    """eps = 0 and gradients of 3e-20: the second moment is a denormal of 15 bits, so its root is within 2^-16 and the
+    first update within that of lr, instead of infinite."""
+    n = 512
+    g = torch.full((n,), 3e-20, device=DEV)
+    g[::2] = -3e-20
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = optim.AdamW([p], lr=1e-2, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0, state_bits=bits)
+    for k in range(3):  # the same gradient: bias-corrected moments stay g and g^2, 8-bit codes are exact at a block's largest
+        opt.step(grads=[g])
+        # a code's own rounding (2^-22) and what three roundings of a denormal leave
+        assert float((p.detach() + (k + 1) * 1e-2 * g.sign()).abs().max()) <= (k + 1) * 1e-2 * 2.0 ** -13
