@@ -380,7 +380,8 @@ RK_API int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab, con
  * [2] gradient norm, [3] clip coefficient, [4..6] constants of the step):
  * rk_adamw_multi_prepare reads the norm partials that rk_adamw_multi_sumsq left
  * (parts = 0: no clipping, coefficient 1), counts the step in scalars[1] and
- * derives the constants; rk_adamw_multi_step then updates every tensor.
+ * derives the constants; rk_adamw_multi_step then updates every tensor. Both
+ * take the betas in 64 bits: 1 - beta formed from a float would be off by 1e-5.
  * rk_adamw_multi_sumsq writes rk_adamw_multi_parts(n) partial sums of
  * squares for its n tensors (fixed order, so norms are reproducible); the
  * partials of several calls may be laid end to end for one prepare.
@@ -397,10 +398,10 @@ typedef struct rk_adamw_tensor {
 } rk_adamw_tensor;
 RK_API int64_t rk_adamw_multi_parts(int64_t n);
 RK_API int rk_adamw_multi_sumsq(const rk_adamw_tensor* tensors, int64_t n, int g_dtype, float* partials, void* stream);
-RK_API int rk_adamw_multi_prepare(const float* partials, int64_t parts, float max_norm, float beta1, float beta2,
+RK_API int rk_adamw_multi_prepare(const float* partials, int64_t parts, float max_norm, double beta1, double beta2,
                                   float weight_decay, float* scalars, void* stream);
 RK_API int rk_adamw_multi_step(const rk_adamw_tensor* tensors, int64_t n, int p_dtype, int g_dtype, int state_bits,
-                               const float* scalars, float beta1, float beta2, float eps, void* stream);
+                               const float* scalars, double beta1, double beta2, float eps, void* stream);
 /* The values 8-bit moments stand for: p (exp_avg) and g (exp_avg_sq) of each
  * tensor are the destinations here, in out_dtype; the codes and scales are read. */
 RK_API int rk_adamw_multi_moments(const rk_adamw_tensor* tensors, int64_t n, int out_dtype, void* stream);

@@ -28,6 +28,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple] = {
@@ -88,8 +89,8 @@ SIGNATURES: dict[str, tuple] = {
                                 _p]),
     "rk_adamw_multi_parts": (_i64, [_i64]),
     "rk_adamw_multi_sumsq": (_i, [_p, _i64, _i, _p, _p]),
-    "rk_adamw_multi_prepare": (_i, [_p, _i64, _f, _f, _f, _f, _p, _p]),
-    "rk_adamw_multi_step": (_i, [_p, _i64, _i, _i, _i, _p, _f, _f, _f, _p]),
+    "rk_adamw_multi_prepare": (_i, [_p, _i64, _f, _d, _d, _f, _p, _p]),
+    "rk_adamw_multi_step": (_i, [_p, _i64, _i, _i, _i, _p, _d, _d, _f, _p]),
     "rk_adamw_multi_moments": (_i, [_p, _i64, _i, _p]),
     "rk_head_stats_width": (_i64, [_i64]),
     "rk_head_fprop": (_i, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i, _p]),

@@ -54,7 +54,7 @@ int ensure_smem_attr(const void* kernel, int bytes) {
 }
 }  // namespace rk_host
 
-extern "C" int rk_abi_version(void) { return 1; }
+extern "C" int rk_abi_version(void) { return 2; }  // 2: rk_adamw_multi_prepare and _step take the betas in 64 bits
 
 extern "C" unsigned long long rk_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 

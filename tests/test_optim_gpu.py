@@ -577,3 +577,42 @@ def test_gradients_whose_squares_are_denormal(bits):
         opt.step(grads=[g])
         # a code's own rounding (2^-22) and what three roundings of a denormal leave
         assert float((p.detach() + (k + 1) * 1e-2 * g.sign()).abs().max()) <= (k + 1) * 1e-2 * 2.0 ** -13
+
+
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.9, 0.95), (0.8, 0.9999), (0.5, 0.3), (0.0, 0.0)])
+def test_moments_take_the_betas_in_64_bits(betas):
+    """One step from given moments. exp_avg_sq: its weights and their products are rounded 2^-24 four times, its sums
+    twice, all terms positive; exp_avg: a difference, its product and a sum, of the size of both terms."""
+    n, (b1, b2) = 1 << 16, betas
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    g, m, v = (torch.randn(n, generator=gen, device=DEV) for _ in range(3))
+    v = v.square() * 3
+    v[::7] = 0.0
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = optim.AdamW([p], betas=betas, weight_decay=0.0)
+    opt.state[p].update(exp_avg=m.clone(), exp_avg_sq=v.clone())
+    opt.set_step(3)
+    opt.step(grads=[g])
+    m64, g64, v64 = m.double(), g.double(), v.double()
+    me = b1 * m64 + (1 - b1) * g64
+    ve = b2 * v64 + (1 - b2) * g64 * g64
+    assert float(((opt.state[p]["exp_avg_sq"].double() - ve).abs() - 6 * 2.0 ** -24 * ve).max()) <= 0
+    lim = 4 * 2.0 ** -24 * (m64.abs() + g64.abs())
+    assert float(((opt.state[p]["exp_avg"].double() - me).abs() - lim).max()) <= 0
+
+
+def test_default_betas_against_64_bits():
+    """The class's own betas from the first step on: each step adds its six roundings to exp_avg_sq (which are at most
+    those of the sum so far) and as many to the update, whose bias corrections are formed in 64 bits."""
+    params = _params([300, 2049])
+    opt, ref = optim.AdamW(params, lr=1e-2), Ref(params, lr=1e-2)
+    for k in range(1, 31):
+        grads = _tensors([300, 2049], seed=70 + k)
+        opt.step(grads=grads)
+        ref.step(grads)
+        for p, m, v, q in zip(ref.p, ref.m, ref.v, params):
+            st = opt.state[q]
+            assert float(((st["exp_avg_sq"].double() - v).abs() - 6 * k * 2.0 ** -24 * v).max()) <= 0
+            assert float((st["exp_avg"].double() - m).abs().max()) <= 4 * k * 2.0 ** -24 * 10
+            # the update is at most lr |m| / sqrt(v), both corrected: here below 10 lr; p itself is rounded each step
+            assert float((q.detach().double() - p).abs().max()) <= k * (2.0 ** -20 * 1e-2 * 10 + 2.0 ** -24)
