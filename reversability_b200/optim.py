@@ -140,6 +140,7 @@ class AdamW(torch.optim.Optimizer):
         self._made_of = []     # (state_bits, parameters) of each group then
         self._state_of = ()    # the optimizer's state then
         self._idle = []        # (place, parameter) outside it
+        self._updated = []     # the parameters in it
         self._coded = None     # the table of the parameters with 8-bit moments
         self._coded_of = ()    # the optimizer's state when it was made
         self._norm_of = None   # the scalars that grad_norm is a view of
@@ -361,6 +362,7 @@ class AdamW(torch.optim.Optimizer):
             if launch.block is None:
                 block = self._group_scalars(launch.index)
                 self._counted[id(block)] = block
+        self._updated = [p for _, p, _, _ in found]
         self._state_of = _seen(self.state)
         self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
@@ -426,6 +428,8 @@ class AdamW(torch.optim.Optimizer):
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_step", launch.table, len(launch.entries), launch.p_code, launch.g_code, launch.bits,
                       scalars[launch.counter].data_ptr(), b1, b2, group["eps"], stream)
+        # the kernels wrote past autograd: a graph kept from before must not take the new values for the old ones
+        torch.autograd.graph.increment_version(self._updated)
         del keep
         return loss
 

@@ -370,3 +370,14 @@ def test_the_state_of_another_optimizer_is_refused(recorded):
     new.step()
     _used(recorded, new, params)
     assert _counts(recorded, new) == [2.0, 2.0]
+
+
+def test_a_graph_kept_over_a_step_notices(recorded):
+    p, q, r = params = _params(3)
+    opt = optim.AdamW(params)
+    for _ in range(2):  # with a new plan and with the one that is there
+        a, b = (p * q).sum(), (r * r).sum()
+        opt.step(grads=[torch.ones(10), None, None])
+        b.backward()  # what was not updated may still be used
+        with pytest.raises(RuntimeError, match="inplace"):
+            a.backward()
