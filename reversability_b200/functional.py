@@ -692,7 +692,8 @@ def token_logprob_bwd_at(logits, labels, stats: int, d_logprob: int, coef_stride
 
 
 def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld: int) -> tuple[torch.Tensor, int]:
-    """(gradient tensor, its row stride): a new one laid out like the logits, or a checked `out`."""
+    """(gradient tensor, its row stride): a new one laid out like the logits, or a checked `out`, of which autograd is
+    told that it is written (a loss that saved it must not take the gradients for its logits)."""
     if out is None:
         return like_rows(logits, rows, ld), ld
     if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
@@ -706,6 +707,7 @@ def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld:
     gap = abs(out.data_ptr() - logits.data_ptr()) // out.element_size()
     if rows and gap and gap < (rows - 1) * max(ld, ldd) + V and not (ld == ldd and V <= gap % ld <= ld - V):
         raise ValueError("out overlaps the logits without being the same rows")
+    torch.autograd.graph.increment_version(out)
     return out, ldd
 
 

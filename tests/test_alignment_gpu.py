@@ -672,3 +672,25 @@ def test_changing_what_was_returned_leaves_the_backward_alone():
     r.entropy.mul_(3.0)
     with pytest.raises(RuntimeError, match="inplace"):
         r.loss.backward()
+
+
+def test_a_loss_that_saved_the_logits_notices_gradients_written_over_them():
+    x, y, old, adv, ref, w = _policy_inputs(12, 50, torch.float32, "plain")
+    others = torch.zeros_like(x)
+    for write in (lambda z: alignment.policy_loss_and_grad(z.detach(), y, old, adv, out=z.detach()),
+                  lambda z: alignment.preference_loss_and_grad(z.detach().view(2, 6, 50), y.view(2, 6), None,
+                                                               out=z.detach().view(2, 6, 50))):
+        for loss in (lambda z: alignment.token_logprobs(z, y).sum(), lambda z: alignment.policy_loss(z, y, old, adv).loss,
+                     lambda z: alignment.preference_loss(z.view(2, 6, 50), y.view(2, 6), None).loss):
+            z = x.clone().requires_grad_()
+            kept = loss(z)
+            write(z)
+            with pytest.raises(RuntimeError, match="inplace"):
+                kept.backward()
+    z = x.clone().requires_grad_()
+    kept = alignment.token_logprobs(z, y).sum()
+    alignment.policy_loss_and_grad(z.detach(), y, old, adv, out=others)  # the logits stay as they are
+    kept.backward()
+    with torch.inference_mode():  # such tensors have no such count
+        z = x.clone()
+        alignment.policy_loss_and_grad(z, y, old, adv, out=z)
