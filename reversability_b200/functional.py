@@ -700,10 +700,10 @@ def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld:
         raise ValueError("out must match the logits' shape, dtype and device")
     if out.shape[-1] > 1 and out.stride(-1) != 1:
         raise ValueError("out must have a unit-stride last dimension")
-    if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
-        raise ValueError("out may alias the logits only with the same strides")
     V = logits.shape[-1]
     ldd = token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
+    if out.data_ptr() == logits.data_ptr() and rows and ldd != ld:  # strides of dimensions of size 1 say nothing
+        raise ValueError("out may alias the logits only with the same strides")
     gap = abs(out.data_ptr() - logits.data_ptr()) // out.element_size()
     if rows and gap and gap < (rows - 1) * max(ld, ldd) + V and not (ld == ldd and V <= gap % ld <= ld - V):
         raise ValueError("out overlaps the logits without being the same rows")

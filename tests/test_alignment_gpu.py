@@ -694,3 +694,23 @@ def test_a_loss_that_saved_the_logits_notices_gradients_written_over_them():
     with torch.inference_mode():  # such tensors have no such count
         z = x.clone()
         alignment.policy_loss_and_grad(z, y, old, adv, out=z)
+
+
+def test_out_may_name_the_same_rows_by_other_strides():
+    """Dimensions of size 1 may have any stride; rows that start together and lie apart otherwise are refused."""
+    full = torch.randn(2, 4, 60, device=DEV)
+    y, f = torch.tensor([[3]], device=DEV), torch.zeros(1, 1, device=DEV)
+    x = full[:1, :1]
+    _, want = alignment.policy_loss_and_grad(x, y, f, f + 1)
+    same = full.view(8, 60)[:1].view(1, 1, 60).as_strided((1, 1, 60), (60, 7, 1))
+    assert same.stride() != x.stride()
+    _, d = alignment.policy_loss_and_grad(x, y, f, f + 1, out=same)
+    assert torch.equal(x, want) and d.data_ptr() == x.data_ptr()
+    y, f = torch.zeros(1, 2, dtype=torch.int64, device=DEV), torch.zeros(1, 2, device=DEV)
+    x = full.view(8, 60)[:3:2][None]
+    _, want = alignment.policy_loss_and_grad(x, y, f, f + 1)
+    same = full.view(8, 60).as_strided((1, 2, 60), (9999, 120, 1))
+    alignment.policy_loss_and_grad(x, y, f, f + 1, out=same)
+    assert torch.equal(x, want)
+    with pytest.raises(ValueError, match="strides"):
+        alignment.policy_loss_and_grad(x, y, f, f + 1, out=full.view(8, 60)[:2][None])
