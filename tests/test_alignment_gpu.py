@@ -714,3 +714,60 @@ def test_out_may_name_the_same_rows_by_other_strides():
     assert torch.equal(x, want)
     with pytest.raises(ValueError, match="strides"):
         alignment.policy_loss_and_grad(x, y, f, f + 1, out=full.view(8, 60)[:2][None])
+
+
+def _check_policy_rows(x, y, layout, seed, entropy_coef=0.01):
+    """The policy loss with its gradient against 64 bits, again (the same bits), over the logits and in rows of another
+    stride. The rows' factors are the kernel's own: an exponential (2 ulp) and six roundings, 10 * 2^-24."""
+    rows, vocab = x.shape
+    dtype = x.dtype
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    step = max(1, (1 << 24) // vocab)
+    lp64 = torch.cat([_rows64(x[s:s + step], y[s:s + step])[1] for s in range(0, rows, step)])
+    old = (lp64 + 0.1 * torch.randn(rows, generator=g, device=DEV)).float()
+    adv = torch.randn(rows, generator=g, device=DEV)
+    kw = dict(clip_low=1.0, clip_high=10.0, entropy_coef=entropy_coef, grad_scale=float(rows))
+    r, d = alignment.policy_loss_and_grad(x, y, old, adv, **kw)
+    valid = y >= 0
+    assert float((r.logprobs.double() - lp64).abs().max()) <= _lp_tol(x)
+    scale = float(rows) / int(valid.sum())
+    g_lp = -(r.logprobs.double() - old.double()).exp() * adv.double() * scale
+    g_h = torch.full_like(g_lp, -entropy_coef * scale)
+    for s in range(0, rows, step):
+        logp, _, h, _ = _rows64(x[s:s + step], y[s:s + step])
+        p, at = logp.exp(), y[s:s + step].clamp(min=0)[:, None]
+        gl, gh = ((t[s:s + step] * valid[s:s + step])[:, None] for t in (g_lp, g_h))
+        inner = torch.where(p > 0, p * (logp + h[:, None]), torch.zeros_like(p))
+        want = (-gl * p - gh * inner).scatter_add_(1, at, gl)
+        near = gl.abs() * p + gh.abs() * torch.where(p > 0, p * (logp.abs() + h[:, None] + 1), torch.zeros_like(p))
+        near.scatter_add_(1, at, gl.abs() * p.gather(1, at))
+        # as in _check_grad, and the factor's own error where it stands alone
+        lim = (HALF_ULP[dtype] + 2.0 ** -22) * want.abs() + 2e-5 * near + SMALLEST[dtype]
+        lim.scatter_add_(1, at, 10 * 2.0 ** -24 * gl.abs())
+        assert float(((d[s:s + step].double() - want).abs() - lim).max()) <= 0
+    assert not d[~valid].any()
+    again, d2 = alignment.policy_loss_and_grad(x, y, old, adv, **kw)
+    assert torch.equal(d, d2) and torch.equal(r.loss, again.loss)
+    other = torch.full((rows, vocab + 6), 7.0, device=DEV, dtype=dtype)
+    alignment.policy_loss_and_grad(x, y, old, adv, out=other[:, 3:3 + vocab], **kw)
+    assert torch.equal(other[:, 3:3 + vocab], d) and bool((other[:, :3] == 7.0).all()) and bool((other[:, 3 + vocab:] == 7.0).all())
+    buf = _logits(rows, vocab, dtype, layout)
+    buf.copy_(x)
+    _, d2 = alignment.policy_loss_and_grad(buf, y, old, adv, out=buf, **kw)
+    assert d2.data_ptr() == buf.data_ptr() and torch.equal(buf, d)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["plain", "shifted"])
+@pytest.mark.parametrize("rows,vocab", [(5, 131075), (9, 50257), (2, 300007)])
+def test_few_long_rows_of_the_lowest_value(rows, vocab, layout, dtype):
+    """Rows that a cluster shares and forms again relative to their largest element, while the gradient goes over the logits."""
+    x = _logits(rows, vocab, dtype, layout, seed=9)
+    y = _labels(rows, vocab, 9, 0.0)
+    for r in range(0, rows, 2):
+        x[r] = torch.finfo(dtype).min
+    if dtype != torch.float16:
+        x[1] -= 3e7  # a finite reference beyond what x c is exact for
+        x[1, vocab // 2] = x[1].max()
+    _check_policy_rows(x, y, layout, 3)
