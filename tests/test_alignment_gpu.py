@@ -758,6 +758,23 @@ def _check_policy_rows(x, y, layout, seed, entropy_coef=0.01):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("layout", ["plain", "shifted"])
+@pytest.mark.parametrize("rows,vocab,dtype", [(200, 131075, torch.bfloat16), (200, 131075, torch.float16), (200, 131075, torch.float32),
+                                              (500, 50257, torch.float32), (400, 100003, torch.bfloat16), (310, 114689, torch.float16)])
+def test_rows_longer_than_their_ring(rows, vocab, dtype, layout):
+    """Rows whose first chunks pass through the ring twice, several of them a CTA: the second time while the rest of the
+    row is written over. Uneven masks, masked columns, a row of nothing but the lowest value."""
+    x = _logits(rows, vocab, dtype, layout, seed=6)
+    y = _labels(rows, vocab, 6)
+    y[150:190] = -100
+    y[:4] = torch.tensor([7, 11, vocab // 3, vocab - 1], device=DEV)
+    x[1, vocab // 2:] = -math.inf
+    x[2, vocab // 2:] = torch.finfo(dtype).min
+    x[3] = torch.finfo(dtype).min
+    for bonus in (0.01, 0.0):
+        _check_policy_rows(x, y, layout, 7, bonus)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", ["plain", "shifted"])
 @pytest.mark.parametrize("rows,vocab", [(5, 131075), (9, 50257), (2, 300007)])
