@@ -257,7 +257,10 @@ __device__ __forceinline__ float exponent(float x, float c, const RowSum& a, boo
 // The label's log-probability before it is rounded to fp32 (whose steps are 1e-6 at -10): losses are sums of many, in
 // which these roundings would show. With the sum's own c and m, so that their rounding cancels. The exponential unit's
 // results are 5e-8 low on average (5.0e-8 over [-16, -1], 2.2e-8 over [-1, 0], at most 1.4e-7), and a sum meets it again
-// where sums are joined: 8e-8 in all, but for the reference's own term, which is exact.
+// where sums are joined: 8e-8 in all, but for the reference's own term, which is exact. Mean errors left over rows of 1000
+// to 50257 normal logits: -4e-8 to 7e-8 at spreads of 0.01 to 2, where they were 4e-8 to 1.5e-7; wider ones are 1.3e-8 of the
+// label's distance from the row's mean under p further off, by the rounding of c. Rows of equal logits, whose exponentials
+// are exact, become up to 1e-7 too low.
 constexpr double kUnitLow = 8e-8;
 __device__ __forceinline__ double label_logprob(float x, float c, const RowSum& a, bool far) {
   const double t = far ? ((double)x - (double)a.r) * (double)c : fma((double)x, (double)c, -(double)a.m);

@@ -788,3 +788,29 @@ def test_few_long_rows_of_the_lowest_value(rows, vocab, layout, dtype):
         x[1] -= 3e7  # a finite reference beyond what x c is exact for
         x[1, vocab // 2] = x[1].max()
     _check_policy_rows(x, y, layout, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [101, 1000, 8192, 50257])
+def test_losses_have_no_bias_of_the_exponential_unit(vocab, dtype):
+    """Mean signed error of the log-probabilities that enter a preference loss, seen through rewards of sequences of one
+    token whose reference is the 64-bit value rounded to fp32. What is taken out for the exponential unit is 8e-8: the
+    mean may be no further off than that, beside 2^-26 (the rounding of log2 e) of the label's distance from the mean
+    logit under p and, where exponentials are exact, 2^-24 of a logit in base 2 (the rounding of the reference)."""
+    rows = 4096 if vocab < 20000 else 1024
+    for spread in (0.0, 0.01, 0.1, 0.5, 1.0, 2.0, 4.0, 8.0):
+        g = torch.Generator(device=DEV).manual_seed(1)
+        x = (torch.randn(rows, vocab, generator=g, device=DEV) * spread + 0.37).to(dtype)
+        y = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+        lp, far = [], []
+        for s in range(0, rows, 256):
+            z = x[s:s + 256].double()
+            logp = torch.log_softmax(z, -1)
+            lp.append(logp.gather(1, y[s:s + 256, None])[:, 0])
+            far.append((logp.exp() * z).sum(1) - z.gather(1, y[s:s + 256, None])[:, 0])
+        lp, far = torch.cat(lp), torch.cat(far)
+        ref = lp.float()
+        r = alignment.preference_loss(x.view(rows, 1, vocab), y.view(rows, 1), ref.view(rows, 1), beta=1.0)
+        mean = float((r.rewards.double() - (lp - ref.double())).mean())
+        tied = 2.0 ** -24 * 0.37 * 1.4427 if spread == 0.0 else 0.0
+        assert abs(mean) <= 8e-8 + 2.0 ** -26 * abs(float(far.mean())) + tied
