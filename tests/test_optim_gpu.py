@@ -616,3 +616,22 @@ def test_default_betas_against_64_bits():
             assert float((st["exp_avg"].double() - m).abs().max()) <= 4 * k * 2.0 ** -24 * 10
             # the update is at most lr |m| / sqrt(v), both corrected: here below 10 lr; p itself is rounded each step
             assert float((q.detach().double() - p).abs().max()) <= k * (2.0 ** -20 * 1e-2 * 10 + 2.0 ** -24)
+
+
+def test_scales_of_8_bit_blocks_mark_nan_and_infinity():
+    """A block that saw either has scales, and so decoded moments, that are not finite; its neighbours' are."""
+    q = _params([1300])[0]
+    opt = optim.AdamW([q], state_bits=8, **HP)
+    g = _tensors([1300], seed=1)[0]
+    g[5], g[300], g[1290] = math.inf, math.nan, -math.inf
+    for _ in range(2):  # and it stays so
+        opt.step(grads=[g])
+        (m, v), = opt.moments()
+        st = opt.state[q]
+        for name, values in (("exp_avg_scale", m), ("exp_avg_sq_scale", v)):
+            assert st[name].isfinite().tolist() == [False, False, True, True, True, False]
+            for block in range(6):
+                finite = values[block * 256:(block + 1) * 256].isfinite()
+                assert bool(finite.all() if block in (2, 3, 4) else ~finite.any())
+        g = _tensors([1300], seed=2)[0]
+    assert bool(q[512:1280].isfinite().all()) and not bool(q[[5, 300, 1290]].isfinite().any())
