@@ -86,17 +86,17 @@ class _Launch:
         moments have moved."""
         if self.moved():
             return False
-        words, field, p_dtype, g_dtype = self.words, 0, self.p_dtype, self.g_dtype
+        words, field, g_dtype = self.words, 0, self.g_dtype
         for p, n, i in self.entries:
             g = p.grad if grads is None else grads[i]  # autograd holds .grad to the parameter's shape
-            if g is None or g.dtype is not g_dtype or p.dtype is not p_dtype or p.numel() != n or \
-                    g.get_device() != device or not g.is_contiguous() or not p.is_contiguous():
+            if g is None or g.dtype is not g_dtype or p.numel() != n or g.get_device() != device or \
+                    not g.is_contiguous() or not p.is_contiguous():
                 return False
             if grads is not None and g.shape != p.shape or grads is None and g.numel() != n:
                 return False
             at = p.data_ptr()
-            if at != words[field]:  # no two devices share an address
-                if p.get_device() != device:
+            if at != words[field]:  # memory that it did not leave is of one type, and no two devices share an address
+                if p.dtype is not self.p_dtype or p.get_device() != device:
                     return False
                 words[field] = at
             words[field + 1] = g.data_ptr()
@@ -141,6 +141,7 @@ class AdamW(torch.optim.Optimizer):
         self._state_of = ()    # the optimizer's state then
         self._idle = []        # (place, parameter) outside it
         self._updated = []     # the parameters in it
+        self._parts = None     # (address, size) of the norm's workspace for it
         self._coded = None     # the table of the parameters with 8-bit moments
         self._coded_of = ()    # the optimizer's state when it was made
         self._norm_of = None   # the scalars that grad_norm is a view of
@@ -180,10 +181,10 @@ class AdamW(torch.optim.Optimizer):
     def _group_scalars(self, index: int) -> torch.Tensor:
         """fp32[8] of the group on its device: [0] lr, [1] steps taken, [2] gradient norm, [3] clip coefficient."""
         group = self.param_groups[index]
-        dev = group["params"][0].device
-        scalars = group["scalars"]
-        if scalars is None or scalars.device != dev:
+        scalars, first = group["scalars"], group["params"][0]
+        if scalars is None or scalars.get_device() != first.get_device():
             self._uncaptured()
+            dev = first.device
             scalars = torch.zeros(8, device=dev, dtype=torch.float32) if scalars is None else scalars.to(dev)
             group["scalars"] = scalars
         return self._with_rate(scalars, group["lr"])
@@ -333,7 +334,10 @@ class AdamW(torch.optim.Optimizer):
             if (p.grad if grads is None else grads[i]) is not None and p.numel():
                 return False
         device = torch.cuda.current_device()
-        return all(launch.refill(grads, device) for launch in launches)
+        for launch in launches:
+            if not launch.refill(grads, device):
+                return False
+        return True
 
     @torch.no_grad()
     def _collect(self, grads) -> list:
@@ -362,7 +366,7 @@ class AdamW(torch.optim.Optimizer):
             if launch.block is None:
                 block = self._group_scalars(launch.index)
                 self._counted[id(block)] = block
-        self._updated = [p for _, p, _, _ in found]
+        self._updated, self._parts = [p for _, p, _, _ in found], None
         self._state_of = _seen(self.state)
         self._made_of = [(group["state_bits"], list(group["params"])) for group in self.param_groups]
         return found
@@ -407,18 +411,20 @@ class AdamW(torch.optim.Optimizer):
                     self._with_rate(launch.block, self.param_groups[launch.index]["lr"])
         if torch.cuda.is_current_stream_capturing():
             self._keep_for_replays(launches, scalars.values())
-        partials, parts = None, 0
+        norm = None, 0
         if self.max_norm is not None:
-            parts = sum(launch.parts for launch in launches)
-            partials = self._norm_workspace(parts, launches[0].entries[0][0].device)
-            at = partials.data_ptr()
+            if self._parts is None:
+                parts = sum(launch.parts for launch in launches)
+                self._parts = self._norm_workspace(parts, self._updated[0].device).data_ptr(), parts
+            norm = self._parts
+            at = norm[0]
             for launch in launches:
                 _lib.call("rk_adamw_multi_sumsq", launch.table, len(launch.entries), launch.g_code, at, stream)
                 at += 4 * launch.parts
         for (index, _), block in scalars.items():
             group = self.param_groups[index]
             b1, b2 = group["betas"]
-            _lib.call("rk_adamw_multi_prepare", _lib.ptr(partials), parts, self.max_norm or 0.0, b1, b2,
+            _lib.call("rk_adamw_multi_prepare", *norm, self.max_norm or 0.0, b1, b2,
                       group["weight_decay"], block.data_ptr(), stream)
         if self.max_norm is not None and self._norm_of is not scalars[launches[0].counter]:
             self._norm_of = scalars[launches[0].counter]
