@@ -385,8 +385,10 @@ RK_API int rk_preference_loss(const void* logits, int64_t ld, int64_t vocab, con
  * rk_adamw_multi_sumsq writes rk_adamw_multi_parts(n) partial sums of
  * squares for its n tensors (fixed order, so norms are reproducible); the
  * partials of several calls may be laid end to end for one prepare.
- * dtypes: p and g each RK_F32, RK_BF16 or RK_F16; p, g and the moments 16-byte
- * aligned (8-bit codes 8-byte), numel >= 0, contiguous. */
+ * dtypes: p and g each RK_F32, RK_BF16 or RK_F16; numel >= 0, contiguous, any
+ * alignment that the elements have themselves (a tensor of which an array is not
+ * aligned to four elements, or to 16 bytes for rk_adamw_multi_moments' outputs
+ * and 8 for its codes, is taken element by element, which is slower). */
 typedef struct rk_adamw_tensor {
   void* p;
   const void* g;

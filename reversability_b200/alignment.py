@@ -16,8 +16,9 @@ advantage inputs are constants, and asking for their gradients raises.
 
 The autograd forms save the logits and two numbers a row and form the gradient
 in the backward, with the upstream factor applied before the one rounding, so a
-loss scaler works with fp16 logits; the *_and_grad forms read the logits once
-instead of twice and may write the gradient over them (`out=logits`).
+loss scaler works with fp16 logits; the *_and_grad forms may write the gradient over
+them (`out=logits`), and that of the policy loss reads them once instead of
+twice (a preference pair's factor is known only after all its rows are read).
 """
 from __future__ import annotations
 

@@ -22,10 +22,10 @@
 // device allocation, and a captured graph replays it.
 //
 // Bound: HBM, 28 bytes an element with fp32 parameters and gradients and 32-bit
-// moments, 16 and 1/16 with 8-bit ones. 456M parameters: 1871 us (6.8 TB/s) and
-// 1086 (6.75); their moments decoded to fp32 436 (6.3). The 20.3M decoder's 45
-// tensors with the norm for clipping: 105 (5.8 TB/s, three launches). A two-layer
-// test model's 14: 12 us, the launches' own.
+// moments, 16 and 1/16 with 8-bit ones. 456M parameters: 1872 us (6.8 TB/s) and
+// 1086 (6.75), with bf16 parameters and gradients 822 (5.6); their moments decoded
+// 431 (6.4). The 20.3M decoder's 45 tensors with the norm for clipping: 104 (5.5
+// TB/s, three launches). A two-layer test model's 14: 12 us, the launches' own.
 #include <type_traits>
 #include "vec.cuh"
 
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
   const bool vec = vec_ok(t.p, sizeof(TP)) && vec_ok(t.g, sizeof(TG)) && vec_ok(t.exp_avg, Q8 ? 1 : 4) &&
                    vec_ok(t.exp_avg_sq, Q8 ? 1 : 4);
   // 8-bit moments: a warp takes tab.tiles consecutive blocks, whose scales travel as one load and one store. 32-bit: the
-  // CTA's warps take neighbouring blocks (1874 against 1993 us at 456M elements)
+  // CTA's warps take neighbouring blocks (1872 against 1993 us at 456M elements)
   const int64_t chunk = blockIdx.x - tab.start[which];
   const int warp = threadIdx.x >> 5;
   constexpr int kStep = Q8 ? 1 : kWarps;
@@ -514,8 +514,6 @@ using namespace rk;
 
 namespace {
 
-// Fills `tab` with up to kMultiCap tensors from `tensors[i..n)`, leaving out empty ones; returns the next index,
-// or -1 for a null pointer or a negative size.
 // Tiles of a chunk, that is consecutive blocks of a warp: 8, so that the warp writes its scales as whole 32-byte
 // sectors (written one by one, 4 bytes each, they cost 280 of 1376 us at 456M elements), but at least four CTAs for
 // each of about 150 SMs.
@@ -528,6 +526,8 @@ int tiles_for(const rk_adamw_tensor* tensors, int64_t n, int most) {
   return tiles;
 }
 enum { NEED_P = 1, NEED_STATE = 2, NEED_SCALES = 4 };
+// Fills `tab` with up to kMultiCap tensors from `tensors[i..n)`, leaving out empty ones; returns the next index,
+// or -1 for a null pointer or a negative size.
 int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, int64_t n, int needs, int tiles) {
   tab.n = 0;
   tab.start[0] = 0;
@@ -554,8 +554,7 @@ int64_t fill_table(MultiTable& tab, const rk_adamw_tensor* tensors, int64_t i, i
 
 // Below it the kernels take the root of a denormal second moment: it is at most 1e-19, 1e-17 once it is corrected for
 // beta2 = 0.9999, so beside a larger eps nothing is lost with it. 456M elements with 8-bit moments, us without and with:
-// fp32 1086/1086, bf16 gradients 978/980, bf16 parameters too 849/880. With 32-bit moments, 1869/1869, always. (These
-// with v' as a sum of two products; see Weights.)
+// fp32 1086/1087, bf16 gradients 978/980, bf16 parameters too 822/857. With 32-bit moments 1870 either way, so always.
 constexpr float kSmallEps = 1e-10f;
 
 template <typename TP, typename TG>

@@ -12,8 +12,10 @@
 // r; keeping r and S apart (not r + log S) keeps p exact when logits are large.
 // r is stored raw: where |r c| would overflow (a row with nothing but masks of
 // the type's lowest value) the exponent is formed as (x - r) c instead. Sums
-// are fp32 per thread over about a hundred terms, joined in a fixed order; the
-// gradient is rounded once, when it is stored.
+// are fp32: a thread adds up partial sums of 16 (fp32) or 32 terms, 13 of them
+// at 50257 columns of 16 bits and 32 at 131072 (18 where a warp has the row),
+// and those of threads are joined in a fixed order; the gradient is rounded
+// once, when it is stored.
 #include <type_traits>
 #include "vec.cuh"
 
@@ -1070,8 +1072,11 @@ __global__ void __launch_bounds__(2 * kSplitThreads + 32, 1)
 
 // ---------------------------------------------------------------- short rows: one warp each
 // The same sums straight from global memory, four vectors a lane in flight, and for the gradient the row once more, from
-// L1 or L2. No join but the warp's own, which is what bounds short rows in a ring: 12001 x 1000 x 32 bits 8.8 us for the
-// sums (5.5 TB/s, half of it from L2), 30 with the gradient.
+// L1 or L2. No join but the warp's own, which is what bounds short rows in a ring: 12001 x 1000 x 32 bits 8.9 us for the
+// sums (5.4 TB/s, half of it from L2), 27 with the gradient. That is more than sums and gradients from statistics take as
+// two launches (20): the policy's logarithm in fp64 stands in each row (1.4 us of the 27 at 12001 rows, 1.7 of 32 at 16384
+// x 1001), twice as many CTAs are launched as fit an SM with 64 registers (25.1 with four, but 32.7 in place of 32.4 at
+// 16384 x 1001), and no load of the next row is under way while this one is finished.
 template <typename T, bool POLICY, bool GRAD, bool ENT>
 __global__ void __launch_bounds__(256)
     warp_row_kernel(const T* logits, int64_t ld, int vocab, int64_t rows, float c, int ignore_index, RowOut o,
@@ -1385,7 +1390,8 @@ constexpr int kMaxWeights = 64;  // CTAs that sum weights: enough to load them, 
 //   policy, fp32, one ring / sums and gradients side by side: 4096 rows of 54 KB 87/91, 72 KB 115/105; 2047 of 100 KB 84/72;
 //     2000 of 200 KB 166/142; 300 of 72 KB 16/18. With 16-bit logits, whose exponentials bound both, 14848 of 100 KB 545/555
 //   policy, 4096 rows of 60 KB bf16: 128 threads and nine slots three times an SM 104, 256 and seven twice 114
-// So sums of 16-bit logits take rings of 128 threads eight times an SM (exponentials bound them, and 40 warps hide more),
+// So sums of 16-bit logits take rings of 128 threads eight times an SM (exponentials bound them, and 40 warps hide more
+// than the 28 to 92 bytes cost that the forms with entropies or a policy's terms spill at 48 registers),
 // fp32 ones, which HBM bounds, of 256 three times. With fewer rows than four an SM a warp's row takes too long alone, and
 // the larger CTAs are faster (64 rows of 100 KB: 5.5 / 6.6).
 // 256 KB rows (1500 x 131072 x 16 bits) with gradient and a ring of 256 threads twice an SM or of 512 once: 178 / 151, as

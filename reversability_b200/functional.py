@@ -729,7 +729,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
                 grad_scale_dev: torch.Tensor | None = None, want_grad: bool = True, want_coef: bool = False,
                 out: torch.Tensor | None = None):
     """rk_policy_loss: (loss, clip fraction, logprob, kl or None, entropy or None, dlogits or None, pairs or None), pairs
-    [2, rows, 2] being the rows' statistics and factors for the backward. advantages has the shape of actions or of its leading dimensions (one a sequence)."""
+    [2, rows, 2] being the rows' statistics and factors for the backward. advantages has the shape of actions or of its
+    leading dimensions (one a sequence)."""
     rows, V, ld, actions = token_rows(logits, actions, "actions")
     dev = logits.device
     old = row_values(old_logprobs, actions, "old_logprobs")
