@@ -118,10 +118,11 @@ class AdamW(torch.optim.Optimizer):
     or were left out of a step, a copy of their own (state[p]["scalars"]), with a launch of its own. A captured graph
     counts the tensors together that it was captured with.
 
-    Step count, learning rate and the derived constants live on the device, so a captured graph that contains step() counts on when it is replayed; a learning
-    rate changed in param_groups is copied there by the next step() outside a graph, or by sync_lr(), and never by a
-    capture, except that a rate given as a tensor on the device is read from that tensor by each replay. What a step()
-    makes for itself cannot be captured: take a first step, with the same gradients, outside the graph."""
+    Step count, learning rate and the derived constants live on the device, so a captured graph that contains step()
+    counts on when it is replayed; a learning rate changed in param_groups is copied there by the next step() outside a
+    graph, or by sync_lr(), and never by a capture, except that a rate given as a tensor on the device is read from that
+    tensor by each replay. What a step() makes for itself cannot be captured: take a first step, with the same
+    gradients, outside the graph."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_norm: float | None = None):
@@ -299,6 +300,10 @@ class AdamW(torch.optim.Optimizer):
             if key in state_dict["state"]:
                 self.state[p] = {k: copy(v, p.device) for k, v in state_dict["state"][key].items()}
         self._reset()
+        for group in self.param_groups:
+            if group["scalars"] is not None and any("exp_avg" in self.state.get(p, ()) for p in group["params"]):
+                group["scalars"] = scalars = group["scalars"].to(group["params"][0].device)
+                self._counted[id(scalars)] = scalars
 
     def _plan(self, found) -> list[_Launch]:
         """The launches for (group index, parameter, gradient, place) tuples."""

@@ -327,6 +327,10 @@ def test_dropped_moments_start_from_zero(recorded):
     opt.state.pop(params[1])
     opt.step(grads=_grads(params))
     assert _counts(recorded, opt) == [2.0, 1.0]
+    opt.load_state_dict(opt.state_dict())
+    opt.state.clear()
+    opt.step(grads=_grads(params))
+    assert _counts(recorded, opt) == [1.0, 1.0]
     by_hand = optim.AdamW(params)
     for p in params:
         by_hand.state[p].update(exp_avg=torch.zeros(10), exp_avg_sq=torch.zeros(10))
