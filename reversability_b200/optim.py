@@ -145,7 +145,7 @@ class AdamW(torch.optim.Optimizer):
         self._parts = None     # (address, size) of the norm's workspace for it
         self._coded = None     # the table of the parameters with 8-bit moments
         self._coded_of = ()    # the optimizer's state when it was made
-        self._norm_of = None   # the scalars that grad_norm is a view of
+        self._norm_of = None   # the address of the scalars that grad_norm is a view of
         self._lr = {}          # by id, device scalars and the learning rate that they hold
         self._counted = {}     # by id, the groups' scalars that steps have counted in
 
@@ -431,9 +431,10 @@ class AdamW(torch.optim.Optimizer):
             b1, b2 = group["betas"]
             _lib.call("rk_adamw_multi_prepare", *norm, self.max_norm or 0.0, b1, b2,
                       group["weight_decay"], block.data_ptr(), stream)
-        if self.max_norm is not None and self._norm_of is not scalars[launches[0].counter]:
-            self._norm_of = scalars[launches[0].counter]
-            self.grad_norm = self._norm_of[2]
+        if self.max_norm is not None:
+            block = scalars[launches[0].counter]
+            if block.data_ptr() != self._norm_of:
+                self._norm_of, self.grad_norm = block.data_ptr(), block[2]
         for launch in launches:
             group = self.param_groups[launch.index]
             b1, b2 = group["betas"]

@@ -385,3 +385,19 @@ def test_a_graph_kept_over_a_step_notices(recorded):
         b.backward()  # what was not updated may still be used
         with pytest.raises(RuntimeError, match="inplace"):
             a.backward()
+
+
+def test_grad_norm_follows_scalars_that_move(recorded):
+    params = _params(2)
+    opt = optim.AdamW(params, max_norm=1.0)
+    opt.step(grads=[torch.ones(10), None])
+    for _ in range(2):
+        opt.step(grads=_grads(params))
+        first = opt.state[params[0]].get("scalars", opt.param_groups[0]["scalars"])
+        first[2] = 3.0
+        assert float(opt.grad_norm) == 3.0
+        first.data = first.data.clone()
+        opt.step(grads=_grads(params))
+        first[2] = 4.0
+        assert float(opt.grad_norm) == 4.0
+        opt.step(grads=[None, torch.ones(10)])
