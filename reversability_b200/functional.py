@@ -704,8 +704,9 @@ def gradient_rows(logits: torch.Tensor, out: torch.Tensor | None, rows: int, ld:
     ldd = token_rows(out, torch.empty(out.shape[:-1], device=out.device, dtype=torch.int64))[2]
     if out.data_ptr() == logits.data_ptr() and rows and ldd != ld:  # strides of dimensions of size 1 say nothing
         raise ValueError("out may alias the logits only with the same strides")
-    gap = abs(out.data_ptr() - logits.data_ptr()) // out.element_size()
-    if rows and gap and gap < (rows - 1) * max(ld, ldd) + V and not (ld == ldd and V <= gap % ld <= ld - V):
+    gap = (out.data_ptr() - logits.data_ptr()) // out.element_size()
+    first = (rows - 1) * (ld if gap > 0 else ldd) + V  # elements from the start of the one that lies first to its end
+    if rows and gap and abs(gap) < first and not (ld == ldd and V <= abs(gap) % ld <= ld - V):
         raise ValueError("out overlaps the logits without being the same rows")
     torch.autograd.graph.increment_version(out)
     return out, ldd

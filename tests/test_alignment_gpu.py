@@ -814,3 +814,18 @@ def test_losses_have_no_bias_of_the_exponential_unit(vocab, dtype):
         mean = float((r.rewards.double() - (lp - ref.double())).mean())
         tied = 2.0 ** -24 * 0.37 * 1.4427 if spread == 0.0 else 0.0
         assert abs(mean) <= 8e-8 + 2.0 ** -26 * abs(float(far.mean())) + tied
+
+
+def test_out_beside_the_logits_with_wider_rows():
+    """Neighbours in memory, as an allocator hands them out, are not refused for the stride of the one behind."""
+    buf = torch.randn(2000, device=DEV)
+    y, f = torch.zeros(6, dtype=torch.int64, device=DEV), torch.zeros(6, device=DEV)
+    narrow, wide = (lambda at: buf[at:at + 240].view(6, 40)), (lambda at: buf[at:at + 360].view(6, 60)[:, :40])
+    for x, out in ((narrow(0), wide(240)), (wide(0), narrow(340)), (wide(240), narrow(0)), (narrow(340), wide(0))):
+        keep = x.clone()
+        _, want = alignment.policy_loss_and_grad(x, y, f, f + 1)
+        _, d = alignment.policy_loss_and_grad(x, y, f, f + 1, out=out)
+        assert torch.equal(d, want) and torch.equal(x, keep) and d.data_ptr() == out.data_ptr()
+    for x, out in ((narrow(0), wide(239)), (wide(0), narrow(339)), (wide(239), narrow(0)), (narrow(339), wide(0))):
+        with pytest.raises(ValueError, match="overlaps"):
+            alignment.policy_loss_and_grad(x, y, f, f + 1, out=out)
