@@ -88,6 +88,39 @@ RK_API int rk_rmsnorm_bwd(const void* x, int x_dtype, int64_t ldx, const float* 
                    int dy_dtype, int64_t lddy, void* dx, int dx_dtype, int64_t lddx, float* dw, int accumulate_dw,
                    float* dw_partial, int64_t workspace_bytes, int64_t rows, int64_t width, void* stream);
 
+/* ------------------------------------------------------------------ layer norm
+ * No counterpart in the reference (its decoder has RMSNorm only).
+ * y = (x - mu) * s * w + b, mu = mean_c x, s = rsqrt(mean_c (x - mu)^2 + eps).
+ * x, y: [rows, width] with row strides ldx, ldy (elements), any alignment;
+ * x in fp32 with y in any type, or x in 16 bits with y in the same type or
+ * fp32. w, b: [width] in param_dtype, each may be NULL (1 and 0). stats
+ * (may be NULL): fp32 pairs (mu, s) per row, 8-byte aligned. width <= 16384. */
+RK_API int rk_layernorm_fwd(const void* x, int x_dtype, int64_t ldx, const void* w, const void* b, int param_dtype,
+                            void* y, int y_dtype, int64_t ldy, float* stats, int64_t rows, int64_t width, float eps,
+                            void* stream);
+/* With n = (x - mu) s and g = dy: dx = s (g w - mean(g w) - n mean(g w n)) in
+ * x's type, dw = sum_rows g n and db = sum_rows g in param_dtype; each of dx,
+ * dw, db may be NULL. dw and db are set (not accumulated), to zero for zero
+ * rows, and are the same bits every run. workspace (fp32, of
+ * rk_layernorm_bwd_workspace(rows, width) bytes) is needed with dw or db. */
+RK_API int64_t rk_layernorm_bwd_workspace(int64_t rows, int64_t width);
+RK_API int rk_layernorm_bwd(const void* x, int x_dtype, int64_t ldx, const void* w, int param_dtype, const float* stats,
+                            const void* dy, int dy_dtype, int64_t lddy, void* dx, int64_t lddx, void* dw, void* db,
+                            float* workspace, int64_t workspace_bytes, int64_t rows, int64_t width, void* stream);
+
+/* ------------------------------------------------------------------ dropout
+ * No counterpart in the reference (reversible.py:82-83 refuses dropout: the
+ * mask could not be replayed). y_i = residual_i + (word_i >= round(p 2^32) ?
+ * x_i / (1 - p) : 0) for i < n, where word_i is number i % 4 of the Philox
+ * 4x32-10 block of counter (i / 4, offset) under key seed: the same (seed,
+ * offset) gives the same mask, whatever the type, so the backward is the same
+ * call on the gradient without a residual. A dropped x_i is not used (NaN
+ * there does not spread). seed_dev (may be NULL): the seed in device memory,
+ * read when the kernel runs. residual (may be NULL) is in y's type; y in x's
+ * type or fp32, and for fp32 x without a residual in any type. */
+RK_API int rk_dropout(const void* x, int x_dtype, const void* residual, void* y, int y_dtype, int64_t n, double p,
+                      uint64_t seed, const int64_t* seed_dev, uint64_t offset, void* stream);
+
 /* Residual add fused into RMSNorm: s = x + a (fp32), y = rmsnorm(s) * w
  * (model.py:67-68, reversible.py:18: mlp_norm(x + attention)). x fp32, a in
  * a_dtype, y in y_dtype, rows contiguous (ld = width, width % 4 == 0).

@@ -26,6 +26,7 @@ DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
+_u64 = ctypes.c_uint64
 _i = ctypes.c_int
 _f = ctypes.c_float
 _d = ctypes.c_double
@@ -40,6 +41,10 @@ SIGNATURES: dict[str, tuple] = {
     "rk_rmsnorm_bwd_workspace": (_i64, [_i64, _i64]),
     "rk_rmsnorm_bwd": (_i, [_p, _i, _i64, _p, _p, _p, _i, _i64, _p, _i, _i64, _p, _i, _p, _i64, _i64, _i64, _p]),
     "rk_rmsnorm_bwd_noalloc": (_i, [_p, _i, _i64, _p, _p, _p, _i, _i64, _p, _i, _i64, _p, _i, _i64, _i64, _p]),
+    "rk_layernorm_fwd": (_i, [_p, _i, _i64, _p, _p, _i, _p, _i, _i64, _p, _i64, _i64, _f, _p]),
+    "rk_layernorm_bwd_workspace": (_i64, [_i64, _i64]),
+    "rk_layernorm_bwd": (_i, [_p, _i, _i64, _p, _i, _p, _p, _i, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p]),
+    "rk_dropout": (_i, [_p, _i, _p, _p, _i, _i64, _d, _u64, _p, _u64, _p]),
     "rk_swiglu_fwd": (_i, [_p, _p, _i, _i64, _i64, _p]),
     "rk_swiglu_bwd": (_i, [_p, _p, _p, _i, _i64, _i64, _p]),
     "rk_reconstruct_midpoint": (_i, [_p, _p, _i, _f, _p, _i64, _p]),

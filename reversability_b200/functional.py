@@ -73,6 +73,120 @@ def rmsnorm_bwd(x: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dy: t
     return dx, dw
 
 
+# ------------------------------------------------------------------ layer norm
+def _on_current_device(t: torch.Tensor, name: str, *others: torch.Tensor | None) -> None:
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} must be on the current CUDA device")
+    for o in others:
+        if o is not None and o.get_device() != t.get_device():
+            raise ValueError(f"all tensors must be on {name}'s device")
+
+
+def even_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """(t or a contiguous copy of it, rows, width, row stride): rows of unit-stride elements an even distance apart
+    are taken as they lie, anything else is copied."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // width if width else 0, width, width
+    rows, ld = 1, None
+    even = width == 1 or t.stride(-1) == 1
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size != 1:
+            if ld is None:
+                ld = stride
+            even = even and stride == ld * rows
+            rows *= size
+    if even and (ld is None or ld >= width):
+        return t, rows, width, width if ld is None else ld
+    return t.contiguous(), rows, width, width
+
+
+def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None):
+    """(weight, bias, dtype code): contiguous [width] vectors of one type, fp32 or x's."""
+    dtype = None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.dtype not in (torch.float32, x.dtype):
+                raise ValueError(f"layer norm {name} must be [width] in fp32 or the input's type")
+            if dtype is not None and t.dtype != dtype:
+                raise ValueError("layer norm weight and bias must share a type")
+            dtype = t.dtype
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    return weight, bias, _lib.code(dtype or torch.float32)
+
+
+def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                  out_dtype: torch.dtype | None = None, want_stats: bool = True):
+    """y = (x - mean) * rsqrt(var + eps) * weight + bias over the last dim; returns (y, stats [rows, 2] or None)."""
+    require_cuda(x, weight, bias, what="layer norm kernels")
+    out_dtype = out_dtype or x.dtype
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("layer norm needs a non-empty last dimension")
+    if x.dtype != torch.float32 and out_dtype not in (x.dtype, torch.float32):
+        raise ValueError("layer norm of 16-bit inputs gives their type or fp32")
+    _on_current_device(x, "the input", weight, bias)
+    weight, bias, pcode = _norm_params(x, weight, bias)
+    xr, rows, width, ld = even_rows(x)
+    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32) if want_stats else None
+    _lib.call("rk_layernorm_fwd", xr.data_ptr(), _lib.code(x.dtype), ld, _lib.ptr(weight), _lib.ptr(bias), pcode,
+              y.data_ptr(), _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, float(eps), _lib.stream_ptr())
+    return y, stats
+
+
+def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+                  param_dtype: torch.dtype = torch.float32, want_dx: bool = True, want_dw: bool = True,
+                  want_db: bool = True):
+    """(dx in x's type, dweight, dbias in param_dtype; None where not wanted) of layernorm_fwd."""
+    require_cuda(x, weight, stats, dy, what="layer norm kernels")
+    _on_current_device(x, "the input", weight, stats, dy)
+    weight, _, _ = _norm_params(x, weight, None)
+    if weight is not None and weight.dtype != param_dtype:
+        raise ValueError("parameter gradients come in the weight's type")
+    xr, rows, width, ldx = even_rows(x)
+    dyr, _, _, lddy = even_rows(dy)
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
+    dw = torch.empty(width, device=x.device, dtype=param_dtype) if want_dw else None
+    db = torch.empty(width, device=x.device, dtype=param_dtype) if want_db else None
+    n_ws = _lib.lib().rk_layernorm_bwd_workspace(rows, width) if want_dw or want_db else 0
+    ws = torch.empty(n_ws // 4, device=x.device, dtype=torch.float32) if n_ws else None
+    _lib.call("rk_layernorm_bwd", xr.data_ptr(), _lib.code(x.dtype), ldx, _lib.ptr(weight), _lib.code(param_dtype),
+              stats.data_ptr(), dyr.data_ptr(), _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw),
+              _lib.ptr(db), _lib.ptr(ws), n_ws, rows, width, _lib.stream_ptr())
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------ dropout
+def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0, residual: torch.Tensor | None = None,
+            out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """residual + (kept ? x / (1 - p) : 0) with the mask of (seed, offset), a function of the element's position in
+    row-major order. seed: a whole number or an int64 device scalar."""
+    require_cuda(x, residual, what="dropout kernels")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("the dropout probability must be in [0, 1]")
+    if not 0 <= offset < 2 ** 64:
+        raise ValueError("the dropout offset must fit 64 bits")
+    on_device = isinstance(seed, torch.Tensor)
+    if on_device:
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError("a dropout seed on the device must be one int64 number")
+    elif not -2 ** 63 <= seed < 2 ** 64:
+        raise ValueError("the dropout seed must fit 64 bits")
+    if residual is not None and (residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32)):
+        raise ValueError("the dropout residual must have the input's shape and its type or fp32")
+    _on_current_device(x, "the input", residual, seed if on_device else None)
+    out_dtype = out_dtype or (x.dtype if residual is None else residual.dtype)
+    if residual is not None and out_dtype != residual.dtype:
+        raise ValueError("dropout with a residual gives the residual's type")
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    _lib.call("rk_dropout", x.data_ptr(), _lib.code(x.dtype), _lib.ptr(residual), y.data_ptr(), _lib.code(out_dtype),
+              x.numel(), float(p), 0 if on_device else seed & (2 ** 64 - 1), seed.data_ptr() if on_device else None,
+              offset, _lib.stream_ptr())
+    return y
+
+
 # ------------------------------------------------------------------ SwiGLU
 def swiglu_fwd(u: torch.Tensor) -> torch.Tensor:
     require_cuda(u)

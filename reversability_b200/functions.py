@@ -105,6 +105,71 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float | None) -> torch.Tenso
     return RMSNormFn.apply(x.contiguous(), w, float(eps))
 
 
+class LayerNormFn(torch.autograd.Function):
+    """Keeps the input and two numbers a row."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, out_dtype):
+        y, stats = fn.layernorm_fwd(x, w, b, eps, out_dtype)
+        ctx.save_for_backward(x, w, stats)
+        ctx.param_dtype = (w if w is not None else b).dtype if w is not None or b is not None else torch.float32
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, w, stats = ctx.saved_tensors
+        dx, dw, db = fn.layernorm_bwd(x, w, stats, gy, ctx.param_dtype, *ctx.needs_input_grad[:3])
+        return dx, dw, db, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """F.layer_norm over the last dimension (at most 16384 wide): statistics in fp32, weight and bias (each may be
+    None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise (any type for fp32 x, fp32 for
+    16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in its input's type under
+    autocast. The gradients of weight and bias are sums in a fixed order."""
+    fn.require_cuda(x, weight, bias, what="layer norm kernels")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
+    return fn.layernorm_fwd(x, weight, bias, float(eps), out_dtype, want_stats=False)[0]
+
+
+class DropoutFn(torch.autograd.Function):
+    """Keeps no mask: the backward generates it anew from (seed, offset)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        on_device = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(*((seed,) if on_device else ()))
+        ctx.seed = None if on_device else seed
+        ctx.p, ctx.offset, ctx.dtype = p, offset, x.dtype
+        return fn.dropout(x, p, seed, offset, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
+        dx = fn.dropout(gy, ctx.p, seed, ctx.offset, out_dtype=ctx.dtype) if ctx.needs_input_grad[0] else None
+        return dx, gy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, *, offset: int = 0,
+            residual: torch.Tensor | None = None, training: bool = True) -> torch.Tensor:
+    """Dropout whose mask is a function of (seed, offset) and the element's position and is never stored: a
+    recompute, an inverse or a backward with the same two numbers drops the same elements. Each is dropped with
+    probability round(p 2^32) / 2^32, the others scaled by 1 / (1 - p); with `residual` (x's shape, its type or fp32)
+    the result is added to it, in its type. Give every call of a step its own offset and every step its own seed (or
+    the other way round). seed may be an int64 scalar on the device, which a captured step's replays read anew;
+    change it in place only after the backward. What is dropped is not used: NaN there does not spread."""
+    fn.require_cuda(x, residual, what="dropout kernels")
+    if not training:
+        p = 0.0
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return DropoutFn.apply(x, residual, float(p), seed, offset)
+    return fn.dropout(x, float(p), seed, offset, residual)
+
+
 class SwiGLUFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u):

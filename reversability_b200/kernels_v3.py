@@ -1,4 +1,5 @@
-"""Fused RMSNorm — drop-in for src/reversibility/kernels_v3.py.
+"""Fused RMSNorm — drop-in for src/reversibility/kernels_v3.py — and the same
+switch for nn.LayerNorm modules (enable_layernorm), which the reference lacks.
 
 Same contract as the reference FusedRMSNorm (kernels_v3.py:51-74): CUDA fp32
 residuals and fp32 weight only ("CUDA FP32" in the error), contiguous input,
@@ -38,4 +39,21 @@ def enable_rmsnorm(model):
         return FusedRMSNorm.apply(x, self.weight, eps)
     for module in model.modules():
         if isinstance(module, torch.nn.RMSNorm):
+            module.forward = types.MethodType(forward, module)
+
+
+def enable_layernorm(model):
+    """Route every nn.LayerNorm of a model through functions.layer_norm (output in the input's type)."""
+    from .functions import layer_norm
+
+    def forward(self, x):
+        n = len(self.normalized_shape)
+        if tuple(x.shape[-n:]) != tuple(self.normalized_shape):
+            raise ValueError(f'Expected trailing dimensions {tuple(self.normalized_shape)}')
+        if n == 1:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        weight, bias = (None if t is None else t.flatten() for t in (self.weight, self.bias))
+        return layer_norm(x.flatten(-n), weight, bias, self.eps).view(x.shape)
+    for module in model.modules():
+        if isinstance(module, torch.nn.LayerNorm):
             module.forward = types.MethodType(forward, module)
