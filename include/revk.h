@@ -340,6 +340,34 @@ RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, c
                                 const float* d_logprob, const float* d_entropy, int64_t coef_stride,
                                 const float* scale_dev, void* dlogits, int64_t ldd, void* stream);
 
+/* ------------------------------------------------ Cross-entropy from hidden states, in pieces of the vocabulary
+ * Replaces the head Linear and F.cross_entropy together (model.py:104,
+ * train_baseline.py:262) where the logits must not be kept: z = hidden W^T,
+ * loss_r = ln sum_j exp z_rj - z_r,label, with dz = (softmax z - onehot) g_r,
+ * dx = dz W, dW = dz^T hidden. hidden [M, K] (row stride ldh, any alignment)
+ * and w [V, K] (16-byte aligned, ldw a multiple of 8) in bf16 or f16, labels
+ * int64 [M]. A row whose label is ignore_index is not read, loses 0 and gets a
+ * zero gradient; a label outside [0, V) sets RK_DEV_CE_LABEL and counts as
+ * ignored. reduction 0: loss[M] per row; 1: their sum, loss[1]; 2: their mean
+ * over the rows that count (0 if none does).
+ * kept (rk_linear_ce_kept(M) bytes, 16-byte aligned) carries the listed rows
+ * and their log-sum-exps to the backward, which does not write it. Workspaces
+ * are 256-byte aligned; the backward's holds dz of one piece of the vocabulary
+ * (up to 512 MB, one 256-column tile at least). */
+RK_API int64_t rk_linear_ce_kept(int64_t M);
+RK_API int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K);
+RK_API int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K);
+RK_API int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                            int64_t ignore_index, int64_t M, int64_t V, int64_t K, int dtype, int reduction, float* loss,
+                            void* kept, void* workspace, int64_t workspace_bytes, void* stream);
+/* grad: fp32, d / d loss (one number, or M for reduction 0), device memory. dx
+ * [M, K] and dw [V, K] (each may be NULL) in any of the three types, set, not
+ * accumulated; the same bits every run. */
+RK_API int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const void* kept, int64_t M,
+                            int64_t V, int64_t K, int dtype, int reduction, const float* grad, void* dx, int64_t lddx,
+                            int dx_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
 /* ------------------------------------------------ Clipped policy loss
  * Per row with an action a in [0, vocab) (others as above), lp its
  * log-probability and H its entropy:

@@ -92,6 +92,12 @@ SIGNATURES: dict[str, tuple] = {
     "rk_preference_workspace": (_i64, [_i64, _i64]),
     "rk_preference_loss": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64,
                                 _p]),
+    "rk_linear_ce_kept": (_i64, [_i64]),
+    "rk_linear_ce_fwd_workspace": (_i64, [_i64, _i64, _i64]),
+    "rk_linear_ce_bwd_workspace": (_i64, [_i64, _i64, _i64]),
+    "rk_linear_ce_fwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _p, _p, _p, _i64, _p]),
+    "rk_linear_ce_bwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i, _i, _p, _p, _i64, _i, _p, _i64, _i, _p, _i64,
+                              _p]),
     "rk_adamw_multi_parts": (_i64, [_i64]),
     "rk_adamw_multi_sumsq": (_i, [_p, _i64, _i, _p, _p]),
     "rk_adamw_multi_prepare": (_i, [_p, _i64, _f, _d, _d, _f, _p, _p]),

@@ -1,0 +1,1096 @@
+// Cross entropy from hidden states in pieces of the vocabulary: neither the
+// logits nor anything of their size outlives a piece.
+//
+//   z = x W^T,  loss_r = ln sum_j exp z_rj - z_r,label
+//   dz = (softmax z - [j = label]) g_r,  dx = dz W,  dW = dz^T x
+//
+// Rows whose label is ignored are left out before anything is multiplied: the
+// others are listed and gathered (a padded or masked row costs nothing, and
+// what lies in it cannot spread). Forward: one GEMM over the whole vocabulary
+// whose epilogue keeps a running maximum and sum of exponentials in registers
+// and writes no logits; a row keeps one number, its log-sum-exp. Backward, for
+// each piece of the vocabulary: the logits again, turned in the epilogue into
+// dz / scale (16 bits; the scale of the loss, with which fp16 would underflow, is
+// applied to the fp32 results) in a workspace of rows x
+// piece; then the two gradient GEMMs read it: dx adds up over the pieces in
+// fp32, dW of the piece is final and leaves in the weight's type.
+//
+// Bound by the tensor cores: 2 M V K operations forward, 6 M V K backward (one
+// third of it the logits again). All four GEMMs are one kernel: CTA pairs
+// (cta_group::2) on 256 x 256 tiles, each CTA loading its 128 rows of A and
+// half of B by TMA (32 KB a 64-wide k block for 4.2 MFLOP, where a single
+// CTA's 128 x 256 tile takes 48 KB and is bound by L2), one thread of the pair
+// issuing tcgen05.mma into double-buffered tensor memory, sixteen epilogue
+// warps a CTA. Sums over sliced reductions are added in a fixed order: no
+// atomics, the same bits every run.
+#include <cudaTypedefs.h>
+#include <mutex>
+#include <type_traits>
+#include "vec.cuh"
+
+namespace rk {
+
+constexpr int kTile = 256;  // rows and columns of a pair's output tile
+constexpr int kHalf = 128;  // of them a CTA's rows of A and rows of B
+constexpr int kKb = 64;     // reduction elements of a stage
+constexpr float kLog2e = 1.4426950408889634f;
+
+// STATS: running (max, sum exp) per row; DLOGITS: dz of a piece, 16 bits; ADD: fp32 tiles stored or added, A K-major
+// (dx); OUTER: the same with A MN-major (slices of dW); OUTER_T: A MN-major, scaled and stored in 16 bits (dW).
+enum { STATS = 0, DLOGITS = 1, ADD = 2, OUTER = 3, OUTER_T = 4 };
+
+constexpr int kEpiWarps = 16;
+constexpr int kCeThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kStageBytes = 2 * kHalf * kKb * 2;  // A and B of one CTA
+__host__ __device__ constexpr uint32_t ce_out_bytes(int m) {
+  return m == STATS ? 0 : (m == ADD || m == OUTER) ? kEpiWarps * 4096 : kEpiWarps * 2048;
+}
+__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : (m == ADD || m == OUTER) ? 5 : 6; }
+__host__ __device__ constexpr uint32_t ce_smem(int m) {
+  return 1024 + ce_stages(m) * kStageBytes + ce_out_bytes(m) + (2 * ce_stages(m) + 6) * 8 + 16;
+}
+
+struct CeArgs {
+  const int* count;  // rows that are not ignored (device memory)
+  int vocab, width;  // V, K
+  int tiles_n;       // column tiles of the output
+  int kb;            // k blocks of the reduction (ADD: of the piece; OUTER: given by count)
+  int slices;        // ADD, OUTER: slices of the reduction
+  int segments;      // STATS: segments of the vocabulary when all of rows_tiles row tiles are there
+  int row_tiles;     // row tiles if no row is ignored (OUTER: vocabulary tiles of the piece)
+  int unit_cap;      // STATS: row tiles x segments at most
+  int v0;            // first vocabulary entry of the piece
+  int slice_rows;    // ADD, OUTER: rows between slices in the output
+  int add;           // ADD: add to what is there
+  float2* part;      // STATS: [unit][4 column groups][256 rows]
+  float* xlabel;     // STATS: logit at the label, per listed row
+  const int* label;  // labels of the listed rows
+  const float2* rowc;  // DLOGITS: per listed row (-lse log2 e, factor of dz)
+  const float* scale;  // OUTER_T
+  unsigned int* status;
+};
+
+// The tiles that a CTA pair visits, in order. STATS: units of one row tile and a run of column tiles, so that a row's
+// running values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
+template <int MODE>
+struct CeWalk {
+  int unit, units, step, tiles_m, segments;
+  int nt, nt_end;
+  int m0, n0, kb0, kb1, slice;
+  bool first, last;
+  __device__ CeWalk(const CeArgs& g, int pair, int pairs) {
+    const int rows = *g.count;
+    tiles_m = (MODE == OUTER || MODE == OUTER_T) ? g.row_tiles : (rows + kTile - 1) / kTile;
+    segments = 1;
+    if (MODE == STATS) {
+      segments = tiles_m == g.row_tiles ? g.segments : g.unit_cap / (tiles_m > 0 ? tiles_m : 1);
+      if (segments > g.tiles_n) segments = g.tiles_n;
+      units = tiles_m * segments;
+    } else {
+      units = tiles_m * g.tiles_n * g.slices;
+    }
+    unit = pair;
+    step = pairs;
+    kb_all = (MODE == OUTER || MODE == OUTER_T) ? (rows + kKb - 1) / kKb : g.kb;
+    if (unit < units) begin(g);
+  }
+  int kb_all;
+  __device__ bool more() const { return unit < units; }
+  __device__ void begin(const CeArgs& g) {
+    slice = 0;
+    kb0 = 0;
+    kb1 = kb_all;
+    if (MODE == STATS) {  // segment-major
+      const int seg = unit / tiles_m;
+      m0 = (unit - seg * tiles_m) * kTile;
+      nt = (int)((int64_t)seg * g.tiles_n / segments);
+      nt_end = (int)((int64_t)(seg + 1) * g.tiles_n / segments);
+    } else if (MODE == DLOGITS) {  // row tiles fastest: they share the weight's tile
+      nt = unit / tiles_m;
+      m0 = (unit - nt * tiles_m) * kTile;
+      nt_end = nt + 1;
+    } else {  // column tiles fastest: they share A's tile
+      const int per = tiles_m * g.tiles_n;
+      slice = unit / per;
+      const int t = unit - slice * per;
+      const int mt = t / g.tiles_n;
+      m0 = mt * kTile;
+      nt = t - mt * g.tiles_n;
+      nt_end = nt + 1;
+      kb0 = (int)((int64_t)slice * kb_all / g.slices);
+      kb1 = (int)((int64_t)(slice + 1) * kb_all / g.slices);
+    }
+    n0 = nt * kTile;
+    first = true;
+    last = nt + 1 == nt_end;
+  }
+  __device__ void next(const CeArgs& g) {
+    if (MODE == STATS && nt + 1 < nt_end) {
+      ++nt;
+      n0 += kTile;
+      first = false;
+      last = nt + 1 == nt_end;
+      return;
+    }
+    unit += step;
+    if (unit < units) begin(g);
+  }
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of this shared-memory location in the pair's first CTA.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t a) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+  return r;
+}
+// Load into this CTA's shared memory, completion counted on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* tmap, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs when all MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void store_2d(const void* tmap, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src),
+               "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void reduce_add_2d(const void* tmap, uint32_t src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   tmap),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t d;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+template <int MODE, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
+    ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmC, const CeArgs g, const uint32_t idesc) {
+  constexpr int STAGES = ce_stages(MODE);
+  constexpr bool A_MN = MODE == OUTER || MODE == OUTER_T;
+  constexpr bool B_MN = MODE == ADD || A_MN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sOut = smem + STAGES * kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + ce_out_bytes(MODE));
+  const uint32_t full0 = smem_u32(bars);           // first CTA: both CTAs' loads of a stage have landed
+  const uint32_t empty0 = full0 + 8 * STAGES;      // each CTA: the MMAs reading a stage are done
+  const uint32_t tfull0 = empty0 + 8 * STAGES;     // each CTA: accumulator b is complete
+  const uint32_t tempty0 = tfull0 + 16;            // first CTA: both CTAs' epilogues have read accumulator b
+  const uint32_t drain = tempty0 + 16;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  volatile int* s_consumed = reinterpret_cast<volatile int*>(s_tmem + 2);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull0 + 8 * b, 1);
+      mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    *s_abort = 0;
+    *s_consumed = 0;
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (MODE != STATS) tma_prefetch_desc(&tmC);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(s_tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are set up before either signals the other's
+  tc_fence_after();
+  const uint32_t tmem_base = *s_tmem;
+  pdl_wait();  // inputs are the previous kernels' outputs
+
+  int issued = 0;
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ producer (each CTA its own halves)
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (CeWalk<MODE> w(g, pair, pairs); w.more() && ok; w.next(g)) {
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = leader_addr(full0 + 8 * stage);
+        if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * kStageBytes);
+        const uint32_t a = smem_u32(smem + stage * kStageBytes), b = a + kHalf * kKb * 2;
+        const int k0 = kb * kKb, ra = w.m0 + rank * kHalf, rb = w.n0 + rank * kHalf;
+        if constexpr (A_MN) {
+          tma_load_pair(a, &tmA, fb, ra, k0);
+          tma_load_pair(a + 8192, &tmA, fb, ra + 64, k0);
+        } else {
+          tma_load_pair(a, &tmA, fb, k0, ra);
+        }
+        if constexpr (B_MN) {
+          const int ky = MODE == ADD ? g.v0 + k0 : k0;
+          tma_load_pair(b, &tmB, fb, rb, ky);
+          tma_load_pair(b + 8192, &tmB, fb, rb + 64, ky);
+        } else {
+          tma_load_pair(b, &tmB, fb, k0, g.v0 + rb);
+        }
+        ++issued;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // the last stages' releases arrive before the CTA may end
+    for (int i = 0; ok && i < STAGES && i < issued; ++i) {
+      const int at = issued - 1 - i;
+      ok = mbar_wait(empty0 + 8 * (at % STAGES), (uint32_t)((at / STAGES) & 1), g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ------------------------------------------------------------ MMA issuer (the pair's first CTA)
+    int stage = 0, acc = 0, consumed = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (CeWalk<MODE> w(g, pair, pairs); w.more() && ok; w.next(g)) {
+      if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem_base + acc * kTile;
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        if (!mbar_wait(full0 + 8 * stage, phase, g.status, RK_DEV_GEMM_TIMEOUT, s_abort)) {
+          ok = false;
+          break;
+        }
+        ++consumed;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + stage * kStageBytes), b = a + kHalf * kKb * 2;
+#pragma unroll
+        for (int j = 0; j < kKb / 16; ++j) {
+          const uint64_t ad = A_MN ? smem_desc_sw128(a + j * 2048, 8192, 1024) : smem_desc_sw128(a + j * 32, 16, 1024);
+          const uint64_t bd = B_MN ? smem_desc_sw128(b + j * 2048, 8192, 1024) : smem_desc_sw128(b + j * 32, 16, 1024);
+          umma_pair(d, ad, bd, idesc, (kb > w.kb0 || j > 0) ? 1u : 0u);
+        }
+        umma_commit_pair(empty0 + 8 * stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      umma_commit_pair(tfull0 + 8 * acc);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    *s_consumed = consumed;
+    if (!ok && consumed) {  // the MMAs already issued finish before tensor memory is released
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain) : "memory");
+      mbar_wait(drain, 0, g.status, RK_DEV_GEMM_TIMEOUT, nullptr);
+    }
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------ epilogue: one row a thread, 64 of the tile's columns
+    const int quarter = warp & 3;       // tensor-memory lanes of this warp
+    const int ew = warp - 2;
+    const int cg = ew >> 2;             // its group of 64 columns
+    const int local = rank * kHalf + quarter * 32 + lane;  // row of the tile
+    uint8_t* buf = sOut + ew * (ce_out_bytes(MODE) / kEpiWarps);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const int rows = MODE == STATS || MODE == DLOGITS ? *g.count : 0;
+    float run_m = -INFINITY, run_s = 0.f;  // STATS: reference and sum of exp(z - reference), z in units of log 2
+    int label = -1;
+    const float scale = MODE == OUTER_T ? *g.scale : 1.f;
+    for (CeWalk<MODE> w(g, pair, pairs); w.more(); w.next(g)) {
+      float2 rc = make_float2(0.f, 0.f);
+      if (MODE == STATS || MODE == DLOGITS) {
+        const int row = w.m0 + local;
+        if (MODE == STATS && w.first) {
+          run_m = -INFINITY;
+          run_s = 0.f;
+        }
+        if (w.first) label = row < rows ? __ldg(g.label + row) : -1;
+        if (MODE == DLOGITS && row < rows) rc = __ldg(g.rowc + row);
+      }
+      bool ok = mbar_wait(tfull0 + 8 * acc, acc_phase, g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTile + cg * 64;
+#pragma unroll 1
+      for (int ch = 0; ch < 2; ++ch) {
+        uint32_t r[32];
+        tmem_ld_32cols_nowait(t_row + ch * 32, r);
+        tmem_ld_wait();
+        if (ch == 1) {  // read: the MMA thread may reuse this accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(leader_addr(tempty0 + 8 * acc));
+        }
+        const int c0 = w.n0 + cg * 64 + ch * 32;  // first column of the chunk
+        float* v = reinterpret_cast<float*>(r);
+        if ((MODE == ADD || A_MN) && w.kb0 >= w.kb1) {  // an empty slice: nothing was accumulated
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0u;
+        }
+        if constexpr (MODE == STATS) {
+          const int valid = g.vocab - c0;
+          if (valid < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (k >= valid) v[k] = -INFINITY;
+          }
+          const int li = label - c0;
+          if (li >= 0 && li < 32) {
+            float xl = 0.f;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) xl = li == k ? v[k] : xl;
+            g.xlabel[w.m0 + local] = xl;
+          }
+          float m = v[0];
+#pragma unroll
+          for (int k = 1; k < 32; ++k) m = fmaxf(m, v[k]);
+          m *= kLog2e;
+          // the reference follows the maximum only when that is 2^8 above it: sums stay below 2^40
+          if (m > run_m + 8.f) {
+            run_s *= run_m == -INFINITY ? 0.f : ex2_approx(run_m - m);
+            run_m = m;
+          }
+          const float ref = run_m == -INFINITY ? 0.f : -run_m;
+          const float2 l2 = make_float2(kLog2e, kLog2e), ref2 = make_float2(ref, ref);
+          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 t = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), l2, ref2);
+            s2[k & 1] = __fadd2_rn(s2[k & 1], make_float2(ex2_approx(t.x), ex2_approx(t.y)));
+          }
+          run_s += (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
+        } else if constexpr (MODE == DLOGITS) {
+          const float2 l2 = make_float2(kLog2e, kLog2e), ref2 = make_float2(rc.x, rc.x);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 t = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), l2, ref2);
+            v[2 * k] = ex2_approx(t.x) * rc.y;
+            v[2 * k + 1] = ex2_approx(t.y) * rc.y;
+          }
+          const int li = label - (g.v0 + c0);
+          if (li >= 0 && li < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (li == k) v[k] -= rc.y;
+          }
+          const int valid = g.vocab - (g.v0 + c0);
+          if (valid < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (k >= valid) v[k] = 0.f;
+          }
+        } else if constexpr (MODE == OUTER_T) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] *= scale;
+        }
+        if constexpr (MODE != STATS) {
+          if (lane == 0) stores_read();  // the warp's box is free
+          __syncwarp();
+          const int y = w.slice * g.slice_rows + w.m0 + rank * kHalf + quarter * 32;
+          if constexpr (MODE == ADD || MODE == OUTER) {  // 32 rows of 128 bytes, 128-byte swizzle
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+                  make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && c0 < g.width) {
+              if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(buf), c0, y);
+              else store_2d(&tmC, smem_u32(buf), c0, y);
+              stores_commit();
+            }
+          } else {  // 32 rows of 64 bytes, 64-byte swizzle
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) p[k] = pack_pair<T>(v[2 * k], v[2 * k + 1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+                  make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            const int yy = MODE == OUTER_T ? g.v0 + y : y;
+            if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && yy < g.vocab))) {
+              store_2d(&tmC, smem_u32(buf), c0, yy);
+              stores_commit();
+            }
+          }
+        }
+      }
+      if (MODE == STATS && w.last)
+        g.part[((int64_t)w.unit * 4 + cg) * kTile + local] = make_float2(run_m, run_s);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (MODE != STATS && lane == 0) stores_done();
+  }
+
+  __syncthreads();
+  if (*s_abort && threadIdx.x == 0) {
+    // Loads in flight land before shared memory is given up. The first CTA's barriers count both CTAs' loads; loads
+    // that its barriers no longer follow land within the time waited here.
+    if (rank == 0)
+      for (int i = *s_consumed; i < issued; ++i)
+        mbar_wait(full0 + 8 * (i % STAGES), (uint32_t)((i / STAGES) & 1), g.status, RK_DEV_GEMM_TIMEOUT, nullptr);
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 1000000ull) {
+    }
+  }
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still signal or read it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- rows
+// One CTA lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
+// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored.
+__global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
+                                                       int64_t ignore, int* __restrict__ head, int* __restrict__ pos,
+                                                       int* __restrict__ label, int* __restrict__ rows_of,
+                                                       unsigned int* status) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  __shared__ int sums[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0, turn = 0;
+  bool bad = false;
+  for (int64_t r0 = 0; r0 < rows; r0 += 4096, turn ^= 1) {
+    int64_t lab[4];
+    const int64_t r = r0 + (int64_t)threadIdx.x * 4;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lab[e] = r + e < rows ? labels[r + e] : ignore;
+      if (lab[e] != ignore && (lab[e] < 0 || lab[e] >= vocab)) bad = true;
+      if (lab[e] == ignore || lab[e] < 0 || lab[e] >= vocab) lab[e] = -1;
+      n += lab[e] >= 0;
+    }
+    int scan = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) sums[turn][warp] = scan;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      const int s = sums[turn][w];
+      if (w < warp) before += s;
+      all += s;
+    }
+    int at = base + before + scan - n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (r + e < rows) pos[r + e] = lab[e] >= 0 ? at : -1;
+      if (lab[e] >= 0) {
+        label[at] = (int)lab[e];
+        rows_of[at] = (int)(r + e);
+        ++at;
+      }
+    }
+    base += all;
+  }
+  if (bad) flag_error(status, RK_DEV_CE_LABEL);
+  if (threadIdx.x == 0) {
+    head[0] = base;
+    head[1] = 0;  // CTAs of the finish kernel that are done
+  }
+}
+
+// Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x, int64_t ldx, int width, int64_t pitch,
+                                                        const int* __restrict__ head, const int* __restrict__ rows_of,
+                                                        T* __restrict__ out) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const int count = head[0];
+  const int end = (count + kTile - 1) / kTile * kTile;
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += gridDim.x * 8) {
+    const T* src = i < count ? x + (int64_t)rows_of[i] * ldx : nullptr;
+    T* dst = out + (int64_t)i * pitch;
+    for (int c = (threadIdx.x & 31) * V; c < width; c += 32 * V) {
+      if constexpr (V == 8) {
+        *reinterpret_cast<uint4*>(dst + c) =
+            src ? __ldg(reinterpret_cast<const uint4*>(src + c)) : make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        dst[c] = src ? src[c] : Dt<T>::from_f(0.f);
+      }
+    }
+  }
+}
+
+// A warp per row joins the partial (reference, sum) pairs: log-sum-exp, loss. The last CTA to finish adds the CTAs'
+// sums in order (64 bits). reduction: 0 a loss per row, 1 their sum, 2 their mean (0 over no rows).
+__global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part, int tiles_n, int segments_all,
+                                                        int row_tiles, int unit_cap, const float* __restrict__ xlabel,
+                                                        const int* __restrict__ pos, int* __restrict__ head,
+                                                        float* __restrict__ lse, int64_t rows, int reduction,
+                                                        double* __restrict__ sums, float* __restrict__ loss) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  __shared__ float row_loss[8];
+  __shared__ double block_sum[8];
+  __shared__ int is_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int count = head[0];
+  const int tiles_m = (count + kTile - 1) / kTile;
+  int segments = tiles_m == row_tiles ? segments_all : unit_cap / (tiles_m > 0 ? tiles_m : 1);
+  if (segments > tiles_n) segments = tiles_n;
+  const int64_t r = (int64_t)blockIdx.x * 8 + warp;
+  float l = 0.f;
+  const int i = r < rows ? pos[r] : -1;
+  if (i >= 0) {
+    const int mt = i / kTile, local = i - mt * kTile;
+    float m = -INFINITY;
+    for (int k = lane; k < segments * 4; k += 32)
+      m = fmaxf(m, part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = 0.f;
+    for (int k = lane; k < segments * 4; k += 32) {
+      const float2 p = part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local];
+      s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const double total = (double)m * 0.6931471805599453 + log((double)s);
+    l = (float)(total - (double)xlabel[i]);
+    if (lane == 0) lse[i] = (float)total;
+  }
+  if (reduction == 0) {
+    if (lane == 0 && r < rows) loss[r] = l;
+    return;
+  }
+  if (lane == 0) row_loss[warp] = l;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int k = 0; k < 8; ++k) s += (double)row_loss[k];
+    sums[blockIdx.x] = s;
+    __threadfence();
+    is_last = atomicAdd(head + 1, 1) == (int)gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!is_last) return;
+  double s = 0.0;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) s += __ldcg(sums + b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) block_sum[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int k = 0; k < 8; ++k) s += block_sum[k];
+    if (reduction == 2) s = count ? s / count : 0.0;
+    loss[0] = (float)s;
+  }
+}
+
+// Factors of the backward: rowc[i] = (-lse log2 e, f_i) with dz = scale * f_i * (softmax - onehot). One gradient for
+// all rows: f = 1 and scale is that gradient (over the count for a mean). One a row: scale is a power of two near the
+// largest of them and f_i = g_i / scale, exactly. In fp16 `boost` moves a power of two from the scale to the factors, so
+// that probabilities down to 2^-37 are held.
+__global__ void __launch_bounds__(1024) ce_factor_kernel(const float* __restrict__ lse, const int* __restrict__ head,
+                                                         const int* __restrict__ rows_of, const float* __restrict__ grad,
+                                                         int reduction, float boost, float2* __restrict__ rowc,
+                                                         float* __restrict__ scale) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  __shared__ float top[32];
+  const int count = head[0];
+  const int lane = threadIdx.x & 31;
+  float unit = 1.f;
+  if (reduction == 0) {  // every CTA for itself: the gradients are few
+    float m = 0.f;
+    for (int i = threadIdx.x; i < count; i += 1024) m = fmaxf(m, fabsf(grad[rows_of[i]]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) top[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = top[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (m > 0.f && m < INFINITY) {
+      int e;
+      frexpf(m, &e);
+      e = e < -100 ? -100 : e > 100 ? 100 : e;  // the scale and its reciprocal are normal numbers
+      unit = ldexpf(1.f, e);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = unit / boost;
+  } else if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *scale = (reduction == 2 ? grad[0] / (float)(count > 0 ? count : 1) : grad[0]) / boost;
+  }
+  for (int i = blockIdx.x * 1024 + threadIdx.x; i < count; i += gridDim.x * 1024)
+    rowc[i] = make_float2(-lse[i] * kLog2e, (reduction == 0 ? grad[rows_of[i]] / unit : 1.f) * boost);
+}
+
+// out[r] = scale * sum of the slices of row pos[r] (zeros where that is -1), or of row r without pos, in slice order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) ce_reduce_kernel(const float* __restrict__ part, int slices, int64_t slice_rows,
+                                                        int64_t pitch, const int* __restrict__ pos,
+                                                        const float* __restrict__ scale, T* __restrict__ out,
+                                                        int64_t ldo, int64_t rows, int width) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const float f = *scale;
+  const int64_t per = (width + V - 1) / V, n = rows * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / per;
+    const int c = (int)(t - r * per) * V;
+    const int64_t i = pos ? pos[r] : r;
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+    if (i >= 0) {
+      for (int k = 0; k < slices; ++k) {
+        float v[V];
+        load_vec<float, V>(part + ((int64_t)k * slice_rows + i) * pitch + c, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += v[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] *= f;
+    }
+    store_vec<T, V>(out + r * ldo + c, s);
+  }
+}
+
+}  // namespace rk
+
+using namespace rk;
+
+namespace {
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [rows, inner] with row pitch ld (elements), boxes of box_inner x box_rows.
+bool tensor_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, int dtype, uint32_t box_inner,
+                uint32_t box_rows) {
+  auto fn = tensor_map_fn();
+  if (!fn) return false;
+  const int64_t esz = rk_host::dtype_size(dtype);
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * esz)};
+  cuuint32_t box[2] = {box_inner, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType dt = dtype == RK_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : dtype == RK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_inner * esz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int kPairs = 74;  // CTA pairs of a B200's 148 SMs
+constexpr int64_t kPieceBytes = 512ll << 20;  // dz of one piece
+
+// How the work of (M rows, V, K) is cut. Pure arithmetic, the same for the workspace queries and the calls.
+struct CePlan {
+  int64_t M, V, K, Mp, Kp, Kq;  // Mp: rows in whole tiles; Kp, Kq: pitch of the gathered rows and of fp32 rows
+  int tiles_m, tiles_v, tiles_k, kb_k;
+  int segments, unit_cap;
+  int piece_tiles;  // vocabulary tiles of a piece
+  int dx_slices, dw_slices;
+};
+
+// Shares of a wave of kPairs tiles that `tiles` slices-many times fill, as time: waves over slices.
+double wave_time(int64_t tiles, int64_t slices) { return (double)ceil_div(tiles * slices, kPairs) / (double)slices; }
+
+CePlan make_plan(int64_t M, int64_t V, int64_t K) {
+  CePlan p{};
+  p.M = M;
+  p.V = V;
+  p.K = K;
+  p.Mp = up(M, kTile);
+  p.Kp = up(K, 8);
+  p.Kq = up(K, 4);
+  p.tiles_m = (int)(p.Mp / kTile);
+  p.tiles_v = (int)ceil_div(V, kTile);
+  p.tiles_k = (int)ceil_div(K, kTile);
+  p.kb_k = (int)ceil_div(K, kKb);
+  // segments of the vocabulary: full waves, long runs
+  double best = 1e30;
+  const int most = (int)(ceil_div(8 * kPairs, p.tiles_m) < p.tiles_v ? ceil_div(8 * kPairs, p.tiles_m) : p.tiles_v);
+  p.segments = 1;
+  for (int s = 1; s <= most; ++s) {
+    const double t = (double)(ceil_div((int64_t)p.tiles_m * s, kPairs) * ceil_div(p.tiles_v, s)) + 0.02 * s;
+    if (t < best) {
+      best = t;
+      p.segments = s;
+    }
+  }
+  p.unit_cap = p.tiles_m * p.segments > 8 * kPairs ? p.tiles_m * p.segments : 8 * kPairs;
+  // pieces: as few as the workspace allows, the count (and the slices of dW) with the fullest waves
+  const int64_t fit = kPieceBytes / (p.Mp * 2 * kTile) > 1 ? kPieceBytes / (p.Mp * 2 * kTile) : 1;
+  const int fewest = (int)ceil_div(p.tiles_v, fit);
+  best = 1e30;
+  for (int n = fewest; n <= fewest + 4 && n <= p.tiles_v; ++n) {
+    const int tiles = (int)ceil_div(p.tiles_v, n);
+    const int rest = p.tiles_v - (int)(ceil_div(p.tiles_v, tiles) - 1) * tiles;  // of the last piece
+    for (int s = 1; s <= 16 && (s == 1 || p.Mp / kKb / s >= 16); ++s) {
+      const double t = (ceil_div(p.tiles_v, tiles) - 1) * wave_time((int64_t)tiles * p.tiles_k, s) +
+                       wave_time((int64_t)rest * p.tiles_k, s) + 0.02 * (n + (s > 1 ? s : 0));
+      if (t < best) {
+        best = t;
+        p.piece_tiles = tiles;
+        p.dw_slices = s;
+      }
+    }
+  }
+  best = 1e30;
+  const int kb_piece = p.piece_tiles * (kTile / kKb);
+  p.dx_slices = 1;
+  for (int s = 1; s <= 16 && (s == 1 || kb_piece / s >= 16); ++s) {
+    const double t = wave_time((int64_t)p.tiles_m * p.tiles_k, s) + 0.02 * s;
+    if (t < best) {
+      best = t;
+      p.dx_slices = s;
+    }
+  }
+  return p;
+}
+
+// Kept from forward to backward (4-byte words): [count, done, -, -], pos [M], rows_of [M], lse [M], label [M].
+struct CeKept {
+  int *head, *pos, *rows_of, *label;
+  float* lse;
+};
+CeKept kept_of(int* k, int64_t M) { return {k, k + 4, k + 4 + M, k + 4 + 3 * M, reinterpret_cast<float*>(k + 4 + 2 * M)}; }
+
+struct Arena {
+  char* base;
+  int64_t at;
+  void* take(int64_t bytes) {
+    void* p = base ? base + at : nullptr;
+    at += up(bytes, 1024);
+    return p;
+  }
+};
+
+struct FwdSpace {
+  void* x;
+  float2* part;
+  float* xlabel;
+  double* sums;
+};
+int64_t fwd_space(const CePlan& p, char* base, FwdSpace* f) {
+  Arena a{base, 0};
+  f->x = a.take(p.Mp * p.Kp * 2);
+  f->part = static_cast<float2*>(a.take((int64_t)p.unit_cap * 4 * kTile * 8));
+  f->xlabel = static_cast<float*>(a.take(p.M * 4));
+  f->sums = static_cast<double*>(a.take(ceil_div(p.M, 8) * 8));
+  return a.at;
+}
+
+struct BwdSpace {
+  void *x, *dz;
+  float2* rowc;
+  float *scale, *dx, *dw;
+};
+// fp32 slices of dW are used unless each tile can leave in the weight's type at once.
+bool dw_direct(const CePlan& p, const void* dw, int64_t lddw, int dw_dtype, int dtype) {
+  return p.dw_slices == 1 && dw_dtype == dtype && rk_host::aligned(dw, 16) && (lddw * 2) % 16 == 0;
+}
+int64_t bwd_space(const CePlan& p, char* base, BwdSpace* b) {
+  Arena a{base, 0};
+  b->x = a.take(p.Mp * p.Kp * 2);
+  b->dz = a.take(p.Mp * p.piece_tiles * kTile * 2);
+  b->rowc = static_cast<float2*>(a.take(p.M * 8));
+  b->scale = static_cast<float*>(a.take(4));
+  b->dx = static_cast<float*>(a.take((int64_t)p.dx_slices * p.Mp * p.Kq * 4));
+  b->dw = static_cast<float*>(a.take((int64_t)p.dw_slices * p.piece_tiles * kTile * p.Kq * 4));
+  return a.at;
+}
+
+template <int MODE, typename T>
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CeArgs& g, int dtype, int64_t tiles,
+           cudaStream_t s) {
+  constexpr bool a_mn = MODE == OUTER || MODE == OUTER_T, b_mn = MODE == ADD || a_mn;
+  static_assert(ce_smem(MODE) <= 232448, "shared memory over the per-block limit");
+  auto kern = ce_gemm_kernel<MODE, T>;
+  if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)ce_smem(MODE))) return e;
+  const int pairs = tiles < kPairs ? (int)tiles : kPairs;
+  rk_host::launch_k(kern, 2 * pairs, kCeThreads, ce_smem(MODE), s, ta, tb, tc, g,
+                    idesc_f16(kTile, kTile, dtype == RK_BF16 ? 1 : 0, a_mn ? 1 : 0, b_mn ? 1 : 0));
+  return rk_host::launch_status();
+}
+
+template <typename T>
+int gather_typed(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, cudaStream_t s) {
+  const bool vec = p.K % 8 == 0 && rk_host::aligned(x, 16) && (p.M <= 1 || ldx % 8 == 0);
+  const int64_t blocks = ceil_div(p.Mp, 8);
+  const unsigned grid = (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
+  if (vec)
+    rk_host::launch_k(ce_gather_kernel<T, 8>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
+                      k.rows_of, static_cast<T*>(out));
+  else
+    rk_host::launch_k(ce_gather_kernel<T, 1>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
+                      k.rows_of, static_cast<T*>(out));
+  return rk_host::launch_status();
+}
+int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, int dtype, cudaStream_t s) {
+  return dtype == RK_BF16 ? gather_typed<__nv_bfloat16>(x, ldx, p, k, out, s) : gather_typed<__half>(x, ldx, p, k, out, s);
+}
+
+template <typename T>
+int reduce_typed(const float* part, int slices, int64_t slice_rows, int64_t pitch, const int* pos, const float* scale,
+                 void* out, int64_t ldo, int64_t rows, int64_t width, cudaStream_t s) {
+  const bool vec = width % 4 == 0 && ldo % 4 == 0 && rk_host::aligned(out, 4 * sizeof(T));
+  int64_t blocks = ceil_div(rows * ceil_div(width, vec ? 4 : 1), 256);
+  if (blocks > 148 * 16) blocks = 148 * 16;
+  if (vec)
+    rk_host::launch_k(ce_reduce_kernel<T, 4>, (unsigned)blocks, 256, 0, s, part, slices, slice_rows, pitch, pos, scale,
+                      static_cast<T*>(out), ldo, rows, (int)width);
+  else
+    rk_host::launch_k(ce_reduce_kernel<T, 1>, (unsigned)blocks, 256, 0, s, part, slices, slice_rows, pitch, pos, scale,
+                      static_cast<T*>(out), ldo, rows, (int)width);
+  return rk_host::launch_status();
+}
+int reduce(const float* part, int slices, int64_t slice_rows, int64_t pitch, const int* pos, const float* scale, void* out,
+           int64_t ldo, int64_t rows, int64_t width, int dtype, cudaStream_t s) {
+  if (dtype == RK_F32) return reduce_typed<float>(part, slices, slice_rows, pitch, pos, scale, out, ldo, rows, width, s);
+  if (dtype == RK_BF16)
+    return reduce_typed<__nv_bfloat16>(part, slices, slice_rows, pitch, pos, scale, out, ldo, rows, width, s);
+  return reduce_typed<__half>(part, slices, slice_rows, pitch, pos, scale, out, ldo, rows, width, s);
+}
+
+bool sizes_ok(int64_t M, int64_t V, int64_t K) {
+  return M >= 0 && V > 0 && K > 0 && M < (1ll << 30) && V < (1ll << 30) && K < (1ll << 24);
+}
+
+}  // namespace
+
+extern "C" int64_t rk_linear_ce_kept(int64_t M) { return M < 0 ? 0 : (4 + 4 * M) * 4; }
+
+extern "C" int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K) {
+  if (!sizes_ok(M, V, K) || M == 0) return 0;
+  FwdSpace f;
+  return fwd_space(make_plan(M, V, K), nullptr, &f);
+}
+
+extern "C" int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K) {
+  if (!sizes_ok(M, V, K) || M == 0) return 0;
+  BwdSpace b;
+  return bwd_space(make_plan(M, V, K), nullptr, &b);
+}
+
+extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                                int64_t ignore_index, int64_t M, int64_t V, int64_t K, int dtype, int reduction,
+                                float* loss, void* kept, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (dtype != RK_BF16 && dtype != RK_F16) return RK_ERR_DTYPE;
+  if (!sizes_ok(M, V, K) || (M > 1 && ldh < K) || (V > 1 && ldw < K) || reduction < 0 || reduction > 2 || !kept ||
+      (M && (!hidden || !w || !labels)) || (!loss && (M || reduction)))
+    return RK_ERR_ARG;
+  if (!rk_host::aligned(w, 16) || (V > 1 && ldw % 8) || !rk_host::aligned(kept, 16)) return RK_ERR_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (cudaMemsetAsync(kept, 0, 16, s) != cudaSuccess) return RK_ERR_LAUNCH;
+    if (reduction && cudaMemsetAsync(loss, 0, 4, s) != cudaSuccess) return RK_ERR_LAUNCH;
+    return RK_OK;
+  }
+  if (V == 1) ldw = up(K, 8);  // one row: its pitch says nothing
+  const CePlan p = make_plan(M, V, K);
+  FwdSpace f;
+  if (!workspace || workspace_bytes < fwd_space(p, nullptr, &f)) return RK_ERR_WORKSPACE;
+  if (!rk_host::aligned(workspace, 256)) return RK_ERR_ALIGN;
+  fwd_space(p, static_cast<char*>(workspace), &f);
+  const CeKept k = kept_of(static_cast<int*>(kept), M);
+  unsigned int* status = rk_host::device_status_ptr();
+  rk_host::launch_k(ce_list_kernel, 1, 1024, 0, s, labels, M, V, ignore_index, k.head, k.pos, k.label, k.rows_of, status);
+  int st = rk_host::launch_status();
+  if (st != RK_OK) return st;
+  if ((st = gather(hidden, ldh, p, k, f.x, dtype, s)) != RK_OK) return st;
+  CUtensorMap ta, tb;
+  if (!tensor_map(&ta, f.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&tb, w, K, V, ldw, dtype, kKb, kHalf))
+    return RK_ERR_LAUNCH;
+  CeArgs g{};
+  g.count = k.head;
+  g.vocab = (int)V;
+  g.width = (int)K;
+  g.tiles_n = p.tiles_v;
+  g.kb = p.kb_k;
+  g.slices = 1;
+  g.segments = p.segments;
+  g.row_tiles = p.tiles_m;
+  g.unit_cap = p.unit_cap;
+  g.part = f.part;
+  g.xlabel = f.xlabel;
+  g.label = k.label;
+  g.status = status;
+  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, g, dtype, p.unit_cap, s)) != RK_OK) return st;
+  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 8), 256, 0, s, f.part, p.tiles_v, p.segments, p.tiles_m,
+                    p.unit_cap, f.xlabel, k.pos, k.head, k.lse, M, reduction, f.sums, loss);
+  return rk_host::launch_status();
+}
+
+extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const void* kept, int64_t M,
+                                int64_t V, int64_t K, int dtype, int reduction, const float* grad, void* dx, int64_t lddx,
+                                int dx_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  if ((dtype != RK_BF16 && dtype != RK_F16) || !rk_host::dtype_ok(dx_dtype) || !rk_host::dtype_ok(dw_dtype))
+    return RK_ERR_DTYPE;
+  if (!sizes_ok(M, V, K) || (M > 1 && (ldh < K || (dx && lddx < K))) || (V > 1 && (ldw < K || (dw && lddw < K))) ||
+      reduction < 0 || reduction > 2 || !kept || (M && (!hidden || !w)) || (!grad && (M || reduction)))
+    return RK_ERR_ARG;
+  if (!rk_host::aligned(w, 16) || (V > 1 && ldw % 8) || !rk_host::aligned(kept, 16)) return RK_ERR_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (V == 1) ldw = lddw = up(K, 8);  // one row: its pitch says nothing
+  if (M == 0) {
+    if (dw && cudaMemset2DAsync(dw, lddw * rk_host::dtype_size(dw_dtype), 0, K * rk_host::dtype_size(dw_dtype), V, s) !=
+                  cudaSuccess)
+      return RK_ERR_LAUNCH;
+    return RK_OK;
+  }
+  if (M == 1 && lddx < K) lddx = K;
+  if (!dx && !dw) return RK_OK;
+  const CePlan p = make_plan(M, V, K);
+  BwdSpace b;
+  if (!workspace || workspace_bytes < bwd_space(p, nullptr, &b)) return RK_ERR_WORKSPACE;
+  if (!rk_host::aligned(workspace, 256)) return RK_ERR_ALIGN;
+  bwd_space(p, static_cast<char*>(workspace), &b);
+  const CeKept k = kept_of(const_cast<int*>(static_cast<const int*>(kept)), M);
+  float* scale = b.scale;
+  int st = gather(hidden, ldh, p, k, b.x, dtype, s);
+  if (st != RK_OK) return st;
+  const int64_t fblocks = ceil_div(M, 4096);
+  rk_host::launch_k(ce_factor_kernel, (unsigned)(fblocks < 64 ? fblocks : 64), 1024, 0, s, k.lse, k.head, k.rows_of, grad,
+                    reduction, dtype == RK_F16 ? 8192.f : 1.f, b.rowc, scale);
+  if ((st = rk_host::launch_status()) != RK_OK) return st;
+  const int64_t pitch = (int64_t)p.piece_tiles * kTile;  // of dz
+  const bool direct = dw && dw_direct(p, dw, lddw, dw_dtype, dtype);
+  CUtensorMap x_k, x_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out, dw_out;
+  if (!tensor_map(&x_k, b.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&x_mn, b.x, K, p.Mp, p.Kp, dtype, 64, kKb) ||
+      !tensor_map(&w_k, w, K, V, ldw, dtype, kKb, kHalf) || !tensor_map(&w_mn, w, K, V, ldw, dtype, 64, kKb) ||
+      !tensor_map(&dz_out, b.dz, pitch, p.Mp, pitch, dtype, 32, 32) ||
+      !tensor_map(&dz_k, b.dz, pitch, p.Mp, pitch, dtype, kKb, kHalf) ||
+      !tensor_map(&dz_mn, b.dz, pitch, p.Mp, pitch, dtype, 64, kKb) ||
+      !tensor_map(&dx_out, b.dx, K, (int64_t)p.dx_slices * p.Mp, p.Kq, RK_F32, 32, 32))
+    return RK_ERR_LAUNCH;
+  if (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dtype, 32, 32)
+             : !tensor_map(&dw_out, b.dw, K, (int64_t)p.dw_slices * pitch, p.Kq, RK_F32, 32, 32))
+    return RK_ERR_LAUNCH;
+  CeArgs g{};
+  g.count = k.head;
+  g.vocab = (int)V;
+  g.width = (int)K;
+  g.label = k.label;
+  g.rowc = b.rowc;
+  g.scale = scale;
+  g.status = rk_host::device_status_ptr();
+  for (int t0 = 0; t0 < p.tiles_v; t0 += p.piece_tiles) {
+    const int tiles = p.tiles_v - t0 < p.piece_tiles ? p.tiles_v - t0 : p.piece_tiles;
+    const int64_t v0 = (int64_t)t0 * kTile;
+    const int64_t live = V - v0 < (int64_t)tiles * kTile ? V - v0 : (int64_t)tiles * kTile;
+    g.v0 = (int)v0;
+    g.slices = 1;
+    g.tiles_n = tiles;
+    g.kb = p.kb_k;
+    g.row_tiles = p.tiles_m;
+    g.slice_rows = 0;
+    st = dtype == RK_BF16 ? launch<DLOGITS, __nv_bfloat16>(x_k, w_k, dz_out, g, dtype, (int64_t)p.tiles_m * tiles, s)
+                          : launch<DLOGITS, __half>(x_k, w_k, dz_out, g, dtype, (int64_t)p.tiles_m * tiles, s);
+    if (st != RK_OK) return st;
+    if (dx) {
+      g.tiles_n = p.tiles_k;
+      g.kb = (int)ceil_div(live, kKb);
+      g.slices = p.dx_slices;
+      g.slice_rows = (int)p.Mp;
+      g.add = t0 > 0;
+      st = launch<ADD, float>(dz_k, w_mn, dx_out, g, dtype, (int64_t)p.tiles_m * p.tiles_k * p.dx_slices, s);
+      if (st != RK_OK) return st;
+    }
+    if (dw) {
+      g.tiles_n = p.tiles_k;
+      g.row_tiles = tiles;
+      g.slices = p.dw_slices;
+      g.slice_rows = direct ? 0 : (int)pitch;
+      const int64_t n = (int64_t)tiles * p.tiles_k * p.dw_slices;
+      if (!direct) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, g, dtype, n, s);
+      else if (dtype == RK_BF16) st = launch<OUTER_T, __nv_bfloat16>(dz_mn, x_mn, dw_out, g, dtype, n, s);
+      else st = launch<OUTER_T, __half>(dz_mn, x_mn, dw_out, g, dtype, n, s);
+      if (st != RK_OK) return st;
+      if (!direct) {
+        char* out = static_cast<char*>(dw) + v0 * lddw * (int64_t)rk_host::dtype_size(dw_dtype);
+        if ((st = reduce(b.dw, p.dw_slices, pitch, p.Kq, nullptr, scale, out, lddw, live, K, dw_dtype, s)) != RK_OK)
+          return st;
+      }
+    }
+  }
+  if (!dx) return RK_OK;
+  return reduce(b.dx, p.dx_slices, p.Mp, p.Kq, k.pos, scale, dx, lddx, M, K, dx_dtype, s);
+}

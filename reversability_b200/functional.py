@@ -438,6 +438,127 @@ def head_wgrad(st: HeadState, hidden: torch.Tensor, dw: torch.Tensor | None = No
     return dw
 
 
+# ------------------------------------------------------------------ cross-entropy in pieces of the vocabulary
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_PIECE_BYTES = 512 << 20  # fp32: logits of the rows taken at a time
+
+
+def _linear_ce_check(hidden, weight, labels, reduction):
+    require_cuda(hidden, weight, labels, what="the head loss")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or 0 in weight.shape:
+        raise ValueError("the head loss takes hidden [..., d] and a non-empty weight [vocabulary, d]")
+    if hidden.dtype != weight.dtype or hidden.dtype not in _lib.DTYPE_CODE:
+        raise ValueError("hidden and weight must share a type: fp32, bf16 or fp16")
+    if labels.dtype != torch.int64 or labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels must be int64 of shape {tuple(hidden.shape[:-1])}")
+    _on_current_device(hidden, "hidden", weight, labels)
+
+
+@functools.lru_cache(maxsize=64)
+def _linear_ce_bytes(M: int, V: int, K: int) -> tuple[int, int, int]:
+    lib = _lib.lib()
+    return lib.rk_linear_ce_kept(M), lib.rk_linear_ce_fwd_workspace(M, V, K), lib.rk_linear_ce_bwd_workspace(M, V, K)
+
+
+def _head_weight(weight: torch.Tensor) -> torch.Tensor:
+    return _tma_ready(weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous())
+
+
+def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                  reduction: str = "mean"):
+    """(loss, kept): the cross-entropy of hidden [..., d] @ weight[V, d].T at labels [...] without its logits, fp32; kept
+    is what linear_ce_bwd needs beside the inputs."""
+    _linear_ce_check(hidden, weight, labels, reduction)
+    labels = labels.contiguous()
+    V, K = weight.shape
+    loss = torch.empty(labels.shape if reduction == "none" else (), device=hidden.device, dtype=torch.float32)
+    if hidden.dtype == torch.float32:
+        return _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss)
+    x, M, _, ld = even_rows(hidden)
+    w = _head_weight(weight)
+    n_kept, n_ws, _ = _linear_ce_bytes(M, V, K)
+    kept = torch.empty(n_kept // 4, device=hidden.device, dtype=torch.int32)
+    ws = torch.empty(n_ws, device=hidden.device, dtype=torch.uint8)
+    _lib.call("rk_linear_ce_fwd", x.data_ptr(), ld, w.data_ptr(), _ld(w), labels.data_ptr(), int(ignore_index), M, V, K,
+              _lib.code(hidden.dtype), _REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n_ws,
+              _lib.stream_ptr())
+    return loss, kept
+
+
+def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor, grad: torch.Tensor,
+                  reduction: str = "mean", want_dx: bool = True, want_dw: bool = True,
+                  dx_dtype: torch.dtype | None = None, dw_dtype: torch.dtype | None = None):
+    """(d hidden, d weight) for the loss's gradient (a device scalar; one a row with reduction "none"), in the inputs'
+    types unless others are given; None where not wanted."""
+    V, K = weight.shape
+    grad = grad.detach().float().contiguous()
+    if grad.device != hidden.device or grad.numel() != (hidden.shape[:-1].numel() if reduction == "none" else 1):
+        raise ValueError("the loss's gradient must be on hidden's device, one number or one a row")
+    dx = torch.empty(hidden.shape, device=hidden.device, dtype=dx_dtype or hidden.dtype) if want_dx else None
+    dw = torch.empty((V, K), device=hidden.device, dtype=dw_dtype or weight.dtype) if want_dw else None
+    if hidden.dtype == torch.float32:
+        return _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw)
+    _on_current_device(hidden, "hidden", weight, kept)
+    x, M, _, ld = even_rows(hidden)
+    w = _head_weight(weight)
+    n_ws = _linear_ce_bytes(M, V, K)[2]
+    ws = torch.empty(n_ws, device=hidden.device, dtype=torch.uint8)
+    _lib.call("rk_linear_ce_bwd", x.data_ptr(), ld, w.data_ptr(), _ld(w), kept.data_ptr(), M, V, K,
+              _lib.code(hidden.dtype), _REDUCTIONS[reduction], grad.data_ptr(), _lib.ptr(dx), K,
+              _lib.code(dx.dtype) if want_dx else 0, _lib.ptr(dw), K, _lib.code(dw.dtype) if want_dw else 0,
+              ws.data_ptr(), n_ws, _lib.stream_ptr())
+    return dx, dw
+
+
+def _f32_chunks(hidden: torch.Tensor, labels: torch.Tensor, V: int):
+    """(first row, rows, logits buffer) of the row chunks whose fp32 logits fit _PIECE_BYTES."""
+    rows = labels.numel()
+    step = min(rows, max(1, _PIECE_BYTES // (4 * V)))
+    logits = torch.empty((step, V), device=hidden.device, dtype=torch.float32)
+    for s in range(0, rows, max(step, 1)):
+        yield s, min(step, rows - s), logits
+
+
+def _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss):
+    """fp32 parity configuration: pieces of the rows, on the CUDA-core GEMM and the token-loss kernels."""
+    V = weight.shape[0]
+    x, y = hidden.reshape(-1, hidden.shape[-1]), labels.view(-1)
+    valid = (y != ignore_index) & (y >= 0) & (y < V)
+    rows = torch.empty(y.shape, device=x.device, dtype=torch.float32)
+    w = weight.contiguous()
+    for s, n, logits in _f32_chunks(x, y, V):
+        linear_fwd(x[s:s + n].contiguous(), w, out=logits[:n])
+        rows[s:s + n] = token_logprob_fwd(logits[:n], torch.where(valid[s:s + n], y[s:s + n], -100), want_stats=False)[0]
+    rows.neg_()
+    if reduction == "none":
+        loss.copy_(rows.view(loss.shape))
+    else:
+        total = rows.sum(dtype=torch.float64)
+        loss.copy_(total / valid.sum().clamp(min=1) if reduction == "mean" else total)
+    return loss, torch.where(valid, y, -100)
+
+
+def _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw):
+    V, K = weight.shape
+    x, w = hidden.reshape(-1, K), weight.contiguous()
+    valid = kept >= 0
+    up = grad.view(-1) if reduction == "none" else grad.expand(kept.shape)
+    up = torch.where(valid, -up / valid.sum().clamp(min=1) if reduction == "mean" else -up, 0.0)
+    total = None if dw is None else torch.zeros((V, K), device=x.device, dtype=torch.float32)
+    for s, n, logits in _f32_chunks(x, kept, V):
+        xc = x[s:s + n].masked_fill(~valid[s:s + n, None], 0.0)  # what lies in an ignored row does not spread
+        z = linear_fwd(xc, w, out=logits[:n])
+        stats = token_logprob_fwd(z, kept[s:s + n])[2]
+        d = token_logprob_bwd(z, kept[s:s + n], stats, up[s:s + n].contiguous(), out=z)
+        if dx is not None:
+            dx.view(-1, K)[s:s + n] = linear_dgrad(d, w)
+        if total is not None:
+            linear_wgrad(d, xc, dw=total, accumulate=True)
+    return dx, total if dw is None or dw.dtype == torch.float32 else total.to(dw.dtype)
+
+
 # ------------------------------------------------------------------ attention
 def attention_fwd(qkv: torch.Tensor, n_heads: int, out: torch.Tensor | None = None):
     """Causal attention over packed qkv [B, T, 3*D]; returns (o [B, T, D], lse [B, H, T])."""

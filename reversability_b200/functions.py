@@ -187,3 +187,39 @@ def swiglu(u: torch.Tensor) -> torch.Tensor:
     """silu(gate) * value over u = [gate | value] (model.py:55-56)."""
     fn.require_cuda(u)
     return SwiGLUFn.apply(u.contiguous())
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """Keeps the inputs and one number a row; the backward forms the logits again, a piece of the vocabulary at a time."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, ignore_index, reduction):
+        loss, kept = fn.linear_ce_fwd(hidden, weight, labels, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, kept)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        hidden, weight, kept = ctx.saved_tensors
+        dx, dw = fn.linear_ce_bwd(hidden, weight, kept, g, ctx.reduction, *ctx.needs_input_grad[:2])
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """F.cross_entropy(F.linear(hidden, weight), labels) without the logits (model.py:104, train_baseline.py:262): hidden
+    [..., d], weight [V, d] of one type, int64 labels [...]; the loss in fp32, 'mean' over the labels that count (0 if
+    none does), 'sum', or 'none' (one a label). Rows labelled ignore_index cost nothing, are not read and get zero
+    gradients; a label outside [0, V) sets the library's device status and counts as ignored. The gradients come in the
+    inputs' types, rounded once from fp32 sums over 16-bit softmax terms (fp16: scaled inside, so a mean over many rows
+    does not underflow before the gradients themselves do). Under autocast both inputs are cast as F.linear's are."""
+    fn.require_cuda(hidden, weight, labels, what="the head loss")
+    low = autocast_dtype(hidden.device.type)
+    if low is not None:
+        with torch.autocast(hidden.device.type, enabled=False):
+            hidden, weight = hidden.to(low), weight.to(low)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return LinearCrossEntropyFn.apply(hidden, weight, labels, int(ignore_index), reduction)
+    return fn.linear_ce_fwd(hidden, weight, labels, int(ignore_index), reduction)[0]

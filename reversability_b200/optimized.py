@@ -23,7 +23,7 @@ from torch.utils._pytree import tree_map
 from . import _lib, functional as fn
 from .reversible import stack_backward, stack_forward
 
-_LOSS_BACKENDS = ("torch", "triton", "cuda")
+_LOSS_BACKENDS = ("torch", "triton", "cuda", "pieces")
 
 
 class ReusedMidpoint(torch.autograd.Function):
@@ -138,6 +138,27 @@ def head_chunks_backward(hidden, weight, labels, denominator, chunk_tokens, comp
     return total, dhidden, dw
 
 
+def head_pieces_backward(hidden, weight, labels, denominator, compute, scaler=None):
+    """head_chunks_backward's loss and gradients in pieces of the vocabulary instead of the tokens (loss_backend
+    "pieces"): all tokens at once, no logits kept, rows labelled -100 left out of the products, and each part of the
+    weight gradient written once instead of added to for every chunk."""
+    fn.require_cuda(hidden, weight, labels)
+    scale = torch.ones((), device=hidden.device, dtype=torch.float32)
+    if scaler is not None:
+        scale = scaler.scale(scale)
+    x, w = hidden.to(compute), weight.detach().to(compute)
+    total, kept = fn.linear_ce_fwd(x, w, labels, reduction="sum")
+    dhidden, dw = fn.linear_ce_bwd(x, w, kept, scale / denominator, "sum", dx_dtype=torch.float32,
+                                   dw_dtype=torch.float32)
+    return total, dhidden, dw
+
+
+def _head_backward(hidden, weight, labels, denominator, chunk_tokens, compute, scaler, loss_backend):
+    if loss_backend == "pieces":
+        return head_pieces_backward(hidden, weight, labels, denominator, compute, scaler)
+    return head_chunks_backward(hidden, weight, labels, denominator, chunk_tokens, compute, scaler)
+
+
 def _accumulate_grad(param, g):
     if param.grad is None:
         param.grad = g.to(param.dtype)
@@ -150,7 +171,8 @@ def chunked_backward(model, ids, labels, denominator, chunk_tokens, scaler=None,
     """optimized.py:70-101: one core forward, the vocabulary head in chunks of
     `chunk_tokens` tokens against the detached hidden state, one core backward.
     loss_backend 'torch', 'triton' (the reference names) and 'cuda' all run the
-    librevk head; returns the fp32 loss sum."""
+    librevk head; 'pieces' takes all tokens at once and the vocabulary in pieces
+    (head_pieces_backward; chunk_tokens is not used). Returns the fp32 loss sum."""
     if chunk_tokens <= 0 or denominator <= 0:
         raise ValueError("Chunk size and normalization denominator must be positive")
     if loss_backend not in _LOSS_BACKENDS:
@@ -159,8 +181,8 @@ def chunked_backward(model, ids, labels, denominator, chunk_tokens, scaler=None,
         hidden = hidden_states(model, ids, reuse)
     weight = model.lm_head.weight
     flat = hidden.detach().reshape(-1, hidden.shape[-1])
-    total, dhidden, dw = head_chunks_backward(flat, weight, labels.reshape(-1), denominator, chunk_tokens,
-                                              compute_dtype(ids.device, precision, weight.dtype), scaler)
+    total, dhidden, dw = _head_backward(flat, weight, labels.reshape(-1), denominator, chunk_tokens,
+                                        compute_dtype(ids.device, precision, weight.dtype), scaler, loss_backend)
     _accumulate_grad(weight, dw)
     with amp_context(ids.device, precision):
         hidden.backward(dhidden.view(hidden.shape).to(hidden.dtype))

@@ -21,8 +21,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import functional as fn
-from .optimized import (ReusedMidpoint, _LOSS_BACKENDS, _accumulate_grad, amp_context, compute_dtype,
-                        head_chunks_backward, hidden_states)
+from .optimized import (ReusedMidpoint, _LOSS_BACKENDS, _accumulate_grad, _head_backward, amp_context, compute_dtype,
+                        hidden_states)
 from .reversible import stack_backward, stack_forward
 
 
@@ -154,7 +154,7 @@ def cached_head_backward(model, ids, labels, denominator, chunk_tokens, scaler=N
     """optimized_v3.py:151-192: the installed core once, the vocabulary head in
     token chunks with the head weight cast once for the call, the head
     gradient accumulated in fp32 and added to the tied weight's .grad, then one
-    core backward. Returns the fp32 loss sum."""
+    core backward. loss_backend as for chunked_backward. Returns the fp32 loss sum."""
     if reuse or chunk_tokens < 1 or denominator < 1:
         raise ValueError('Use installed core mode and positive normalization/chunk')
     if loss_backend not in _LOSS_BACKENDS:
@@ -163,8 +163,8 @@ def cached_head_backward(model, ids, labels, denominator, chunk_tokens, scaler=N
         hidden = hidden_states(model, ids)
     weight = model.lm_head.weight
     flat = hidden.detach().reshape(-1, hidden.shape[-1])
-    total, dhidden, dw = head_chunks_backward(flat, weight, labels.reshape(-1), denominator, chunk_tokens,
-                                              compute_dtype(ids.device, precision, weight.dtype), scaler)
+    total, dhidden, dw = _head_backward(flat, weight, labels.reshape(-1), denominator, chunk_tokens,
+                                        compute_dtype(ids.device, precision, weight.dtype), scaler, loss_backend)
     _accumulate_grad(weight, dw)
     with amp_context(ids.device, precision):
         hidden.backward(dhidden.view(hidden.shape).to(hidden.dtype))
