@@ -91,10 +91,14 @@ RK_API int rk_rmsnorm_bwd(const void* x, int x_dtype, int64_t ldx, const float* 
 /* ------------------------------------------------------------------ layer norm
  * No counterpart in the reference (its decoder has RMSNorm only).
  * y = (x - mu) * s * w + b, mu = mean_c x, s = rsqrt(mean_c (x - mu)^2 + eps).
- * x, y: [rows, width] with row strides ldx, ldy (elements), any alignment;
- * x in fp32 with y in any type, or x in 16 bits with y in the same type or
- * fp32. w, b: [width] in param_dtype, each may be NULL (1 and 0). stats
- * (may be NULL): fp32 pairs (mu, s) per row, 8-byte aligned. width <= 16384. */
+ * x, y: [rows, width] with row strides ldx, ldy (elements), at any address, but
+ * every row of y (and of dy and dx below) lies as many elements behind a
+ * multiple of 16 / sizeof(x element) elements as the row of x does, else
+ * RK_ERR_ALIGN; contiguous arrays from 32-byte boundaries do. x in fp32 with y
+ * in any type, or x in 16 bits with y in the same type or fp32. w, b: [width]
+ * in param_dtype, each may be NULL (1 and 0). stats (may be NULL): fp32 pairs
+ * (mu, s) per row, 8-byte aligned. width <= 16384. Up to 15 bytes in front of
+ * a row and behind it are read where other rows of the same array surround it. */
 RK_API int rk_layernorm_fwd(const void* x, int x_dtype, int64_t ldx, const void* w, const void* b, int param_dtype,
                             void* y, int y_dtype, int64_t ldy, float* stats, int64_t rows, int64_t width, float eps,
                             void* stream);

@@ -4,247 +4,398 @@
 //   dx = s (g w - mean(g w) - n mean(g w n)),  dw = sum_rows g n,  db = sum_rows g
 //
 // Bound by memory: forward x in and y out, backward x and dy in and dx out; a
-// row is read once and stays in registers (packed as it was read) through its
-// sums, the mean first and then the squares about it, so a large mean costs
-// no digits. Rows of up to 1024 elements belong to a warp, wider ones to a
-// CTA with 16 elements a thread. The column sums of the backward stay in
-// registers over all rows that a warp (CTA) visits; warps of a CTA add theirs
-// in shared memory, CTAs leave one partial row each and a second kernel adds
-// those in a fixed order: no atomics, the same bits every run.
+// row is read once. Rows of up to 1024 elements belong to a warp, wider ones
+// to a CTA with 16 (from 8192 on 32) elements a thread; warps (CTAs) walk over
+// rows, and each lane copies its own elements of the next rows into shared
+// memory asynchronously while the current row is summed, the mean first and
+// then the squares about it, so a large mean costs no digits. (With rows loaded
+// into registers as they were needed the backward of 32768 x 1024 bf16 took
+// 152 us: eight warps an SM, each waiting for its row.) Arithmetic is on pairs
+// (fp32x2), or instructions would bound it: 16-bit rows leave some 14 of them
+// an element at full bandwidth, forward, and 20 backward.
+//
+// A lane's elements are vectors of 16 bytes of x at 16-byte boundaries, also
+// where rows start between those: then the first and last vector of a row are
+// used in part. The rows that a CTA visits all start equally far from a
+// boundary (their distance is a multiple of 8 rows), so a lane's columns are
+// the same in each, its parameters stay in registers or shared memory, and so
+// do the column sums of the backward. At the end warps of a CTA add their
+// sums in shared memory, CTAs leave one partial row each and a second kernel
+// adds those in a fixed order: no atomics, the same bits every run.
 #include "vec.cuh"
 
 namespace rk {
 
-// Per-column parameters in fp32 or the activations' type; `p` null: the value `fill` everywhere.
+// Per-column parameters in fp32 or 16 bits; `p` null: one value everywhere.
 struct NormParam {
   const void* p;
   int dtype;
-  int vec;  // the base allows vector loads
 };
+__device__ __forceinline__ float param_at(const NormParam& q, int c, int width, float fill) {
+  if (!q.p || (unsigned)c >= (unsigned)width) return fill;
+  if (q.dtype == RK_F32) return __ldg(static_cast<const float*>(q.p) + c);
+  if (q.dtype == RK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(q.p)[c]);
+  return __half2float(static_cast<const __half*>(q.p)[c]);
+}
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) RowPack {
   T e[V];
 };
 
-// V elements of a row from column c on, zero behind the row's end; read once, so L1 keeps the parameters instead.
-template <typename T, int V>
-__device__ __forceinline__ RowPack<T, V> load_pack(const T* __restrict__ row, int c, int width) {
-  RowPack<T, V> r;
-  if (V > 1 && c + V <= width) {
-    static_assert(V == 1 || sizeof(T) * V == 16, "packs of 16 bytes");
-    uint32_t* d = reinterpret_cast<uint32_t*>(&r);
-    if constexpr (V > 1)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                   : "l"(row + c));
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 32) {
+    copy_async<16>(dst, src);
+    copy_async<16>(dst + 16, static_cast<const char*>(src) + 16);
+  } else if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) r.e[e] = c + e < width ? row[c + e] : Dt<T>::from_f(0.f);
+    static_assert(BYTES == 8, "packs of 8, 16 or 32 bytes");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
   }
-  return r;
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void param_vec(const T* p, bool vec, int c, int width, float fill, float (&o)[V]) {
-  if (vec && c + V <= width) {
-    load_vec<T, V>(p + c, o);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = c + e < width ? Dt<T>::to_f(p[c + e]) : fill;
-  }
-}
-template <int V>
-__device__ __forceinline__ void load_param(const NormParam& q, int c, int width, float fill, float (&o)[V]) {
-  if (!q.p) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = fill;
-  } else if (q.dtype == RK_F32) {
-    param_vec<V>(static_cast<const float*>(q.p), q.vec, c, width, fill, o);
-  } else if (q.dtype == RK_BF16) {
-    param_vec<V>(static_cast<const __nv_bfloat16*>(q.p), q.vec, c, width, fill, o);
-  } else {
-    param_vec<V>(static_cast<const __half*>(q.p), q.vec, c, width, fill, o);
-  }
-}
-
+// Starts the copy of V elements of a row from column c on into this lane's slot. `whole`: all of them lie in the
+// matrix, those of an edge vector outside the row too; else what is outside the row is not touched.
 template <typename T, int V>
-__device__ __forceinline__ void store_part(T* __restrict__ row, int c, int width, const float (&v)[V]) {
-  if (c + V <= width) {
-    store_vec<T, V>(row + c, v);
+__device__ __forceinline__ void fetch(RowPack<T, V>* slot, const T* __restrict__ row, int c, int width, bool whole) {
+  if (whole) {
+    copy_async<V * (int)sizeof(T)>(smem_u32(slot), row + c);
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (c + e < width) row[c + e] = Dt<T>::from_f(v[e]);
+      slot->e[e] = (unsigned)(c + e) < (unsigned)width ? row[c + e] : Dt<T>::from_f(0.f);
   }
 }
 
-__device__ __forceinline__ float lanes_sum(float v) {
+// The pairs of a slot; in an edge vector what is outside the row is zero.
+template <typename T, int V>
+__device__ __forceinline__ void read_slot(const RowPack<T, V>* slot, bool edge, int c, int width, float2 (&v)[V / 2]) {
+  const RowPack<T, V> r = *slot;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int k = 0; k < V / 2; ++k) v[k] = make_float2(Dt<T>::to_f(r.e[2 * k]), Dt<T>::to_f(r.e[2 * k + 1]));
+  if (edge) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if ((unsigned)(c + 2 * k) >= (unsigned)width) v[k].x = 0.f;
+      if ((unsigned)(c + 2 * k + 1) >= (unsigned)width) v[k].y = 0.f;
+    }
+  }
 }
 
-// Sum over the row's threads, the same value in all of them. CTA rows: one barrier; `red` is one of several buffers
+template <typename T, int V>
+__device__ __forceinline__ void store_part(T* __restrict__ row, bool edge, int c, int width, const float2 (&v)[V / 2]) {
+  float o[V];
+#pragma unroll
+  for (int k = 0; k < V / 2; ++k) {
+    o[2 * k] = v[k].x;
+    o[2 * k + 1] = v[k].y;
+  }
+  if (!edge) {
+    store_vec<T, V>(row + c, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if ((unsigned)(c + e) < (unsigned)width) row[c + e] = Dt<T>::from_f(o[e]);
+  }
+}
+
+// Sums over the row's threads, the same values in all of them. CTA rows: one barrier; `red` is one of several buffers
 // used in turn, so a buffer is written again only after a barrier that follows its last read.
-template <bool WARP>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  v = lanes_sum(v);
+template <bool WARP, bool TWO>
+__device__ __forceinline__ float2 row_sums(float2 v, float2* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    if (TWO) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
   if (WARP) return v;
-  const int warps = blockDim.x >> 5;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  return lanes_sum((int)(threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.f);
+  v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x & 31] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {  // at most 16 warps
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    if (TWO) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  return make_float2(__shfl_sync(0xffffffffu, v.x, 0), TWO ? __shfl_sync(0xffffffffu, v.y, 0) : 0.f);
 }
 
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+// Rows in flight: the one at work and up to two being copied, in at most 100 KB a CTA (the widest rows, whose
+// parameters take up to 128 KB beside them: one).
+__host__ __device__ constexpr int norm_depth(int elements, int bytes_per_element, bool warp) {
+  const int row = elements * bytes_per_element * (warp ? 256 : 512);
+  return !warp && elements > 16 ? 1 : 3 * row <= 100 * 1024 ? 3 : 2;
+}
+// Parameters in registers (CTA rows of 16 elements a thread) or in shared memory, as they meet the lanes' vectors.
+__host__ __device__ constexpr bool norm_param_regs(int elements, bool warp) { return !warp && elements <= 16; }
+
+// What a thread does in every row that it visits.
+template <typename Tx, int V, int NV, bool WARP>
+struct RowWalk {
+  int T, t;            // threads of a row, and this one's place
+  int ph;              // elements between a row's start and the 16-byte boundary (of x) before it
+  int64_t row, step;
+  uint32_t edge;       // bit j: vector j lies partly outside the row
+  __device__ RowWalk(const Tx* x, int64_t ldx, int width) {
+    T = WARP ? 32 : blockDim.x;
+    t = WARP ? threadIdx.x & 31 : threadIdx.x;
+    if (WARP) {  // a CTA's rows are equal mod 8
+      row = (blockIdx.x & 7) + 8 * ((int64_t)(blockIdx.x >> 3) * 8 + (threadIdx.x >> 5));
+      step = (int64_t)gridDim.x * 8;
+    } else {
+      row = blockIdx.x;
+      step = gridDim.x;
+    }
+    // the CTA's first row speaks for all that it visits
+    const int64_t first = WARP ? blockIdx.x & 7 : blockIdx.x;
+    ph = (int)((reinterpret_cast<uintptr_t>(x + first * ldx) / sizeof(Tx)) % V);
+    edge = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (col(j) < width && (col(j) < 0 || col(j) + V > width)) edge |= 1u << j;
+  }
+  __device__ __forceinline__ int col(int j) const { return (j * T + t) * V - ph; }
+};
+
 template <typename Tx, typename Ty, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024)
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 2) : 1)
     layernorm_fwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const NormParam b,
                          Ty* __restrict__ y, int64_t ldy, float2* __restrict__ stats, int64_t rows, int width,
                          float eps) {
+  constexpr int D = norm_depth(NV * V, (int)sizeof(Tx), WARP), H = V / 2;
+  constexpr bool REGS = norm_param_regs(NV * V, WARP);
+  extern __shared__ uint4 shared[];  // [D][NV][threads] packs of x, then parameters: [2][NV][T] vectors of floats
+  __shared__ float2 red[WARP ? 1 : 4][16];
   pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ float red[WARP ? 1 : 2][32];
-  const int T = WARP ? 32 : blockDim.x;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= rows) return;
-  RowPack<Tx, V> v[NV];
+  RowWalk<Tx, V, NV, WARP> r(x, ldx, width);
+  RowPack<Tx, V>* mine = reinterpret_cast<RowPack<Tx, V>*>(shared) + threadIdx.x;
+  float2* params = reinterpret_cast<float2*>(reinterpret_cast<RowPack<Tx, V>*>(shared) + D * NV * blockDim.x);
+  auto start = [&](int64_t row, int d) {
+    if (row < rows) {
+      const Tx* src = x + row * ldx;
+      const bool inner = row > 0 && row + 1 < rows;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) v[j] = load_pack<Tx, V>(x + row * ldx, (j * T + t) * V, width);
-  float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) sum += Dt<Tx>::to_f(v[j].e[e]);
-  const float mean = row_sum<WARP>(sum, red[0]) / (float)width;
-  float sq = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float d = Dt<Tx>::to_f(v[j].e[e]) - mean;
-      if ((j * T + t) * V + e < width) sq += d * d;
+      for (int j = 0; j < NV; ++j)
+        if (r.col(j) < width)
+          fetch<Tx, V>(mine + (d * NV + j) * blockDim.x, src, r.col(j), width, inner || !(r.edge >> j & 1));
     }
-  const float rstd = rsqrtf(row_sum<WARP>(sq, red[WARP ? 0 : 1]) / (float)width + eps);
-  if (stats && t == 0) stats[row] = make_float2(mean, rstd);
+    copies_commit();
+  };
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * T + t) * V;
-    if (c >= width) break;
-    float wv[V], bv[V], o[V];
-    load_param<V>(w, c, width, 1.f, wv);
-    load_param<V>(b, c, width, 0.f, bv);
+  for (int d = 0; d < D; ++d)
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = fmaf((Dt<Tx>::to_f(v[j].e[e]) - mean) * rstd, wv[e], bv[e]);
-    store_part<Ty, V>(y + row * ldy, c, width, o);
+    for (int j = 0; j < NV; ++j)
+      if (r.col(j) >= width) mine[(d * NV + j) * blockDim.x] = RowPack<Tx, V>{};
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) start(r.row + d * r.step, d);
+  float2 wr[REGS ? NV : 1][H], br[REGS ? NV : 1][H];
+  if constexpr (REGS) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const int c = r.col(j) + 2 * k;
+        wr[j][k] = make_float2(param_at(w, c, width, 1.f), param_at(w, c + 1, width, 1.f));
+        br[j][k] = make_float2(param_at(b, c, width, 0.f), param_at(b, c + 1, width, 0.f));
+      }
+  } else {
+    for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x) {
+      const int c = 2 * i - r.ph;
+      params[i] = make_float2(param_at(w, c, width, 1.f), param_at(w, c + 1, width, 1.f));
+      params[NV * r.T * H + i] = make_float2(param_at(b, c, width, 0.f), param_at(b, c + 1, width, 0.f));
+    }
+    __syncthreads();
   }
+  const float inv = 1.f / (float)width;
+  int d = 0, turn = 0;
+  for (int64_t row = r.row; row < rows; row += r.step, turn ^= 1) {
+    start(row + (D - 1) * r.step, d == 0 ? D - 1 : d - 1);
+    copies_wait<D - 1>();
+    float2 v[NV][H];
+    float2 sum = both(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      read_slot<Tx, V>(mine + (d * NV + j) * blockDim.x, r.edge >> j & 1, r.col(j), width, v[j]);
+#pragma unroll
+      for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][k]);
+    }
+    const float mean = row_sums<WARP, false>(make_float2(sum.x + sum.y, 0.f), red[WARP ? 0 : 2 * turn]).x * inv;
+    float2 sq = both(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int k = 0; k < H; ++k) v[j][k] = __fadd2_rn(v[j][k], both(-mean));
+      if (r.col(j) >= width || (r.edge >> j & 1)) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          if ((unsigned)(r.col(j) + 2 * k) >= (unsigned)width) v[j][k].x = 0.f;
+          if ((unsigned)(r.col(j) + 2 * k + 1) >= (unsigned)width) v[j][k].y = 0.f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][k], v[j][k], sq);
+    }
+    const float rstd =
+        rsqrtf(row_sums<WARP, false>(make_float2(sq.x + sq.y, 0.f), red[WARP ? 0 : 2 * turn + 1]).x * inv + eps);
+    if (stats && r.t == 0) stats[row] = make_float2(mean, rstd);
+    Ty* dst = y + row * ldy;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (r.col(j) >= width) break;
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const int at = (j * r.T + r.t) * H + k;
+        v[j][k] = __ffma2_rn(__fmul2_rn(v[j][k], both(rstd)), REGS ? wr[j][k] : params[at],
+                             REGS ? br[j][k] : params[NV * r.T * H + at]);
+      }
+      store_part<Ty, V>(dst, r.edge >> j & 1, r.col(j), width, v[j]);
+    }
+    d = d + 1 == D ? 0 : d + 1;
+  }
+  copies_wait<0>();
 }
 
 // partial: [gridDim.x][2][width] fp32 (dw, then db), or null when neither is wanted; dx may be null.
 template <typename Tx, typename Tg, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024)
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2) : 1)
     layernorm_bwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const float2* __restrict__ stats,
                          const Tg* __restrict__ dy, int64_t lddy, Tx* __restrict__ dx, int64_t lddx,
                          float* __restrict__ partial, int64_t rows, int width) {
+  constexpr int D = norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), WARP), H = V / 2;
+  constexpr bool REGS = norm_param_regs(NV * V, WARP);
+  // [D][NV][threads] packs of x, then of dy, then the weight [NV][T] vectors; at the end (WARP) [8][2][width] column sums
+  extern __shared__ uint4 shared[];
+  __shared__ float2 red[WARP ? 1 : 2][16];
   pdl_wait();  // inputs are the previous kernel's outputs
-  extern __shared__ float shared[];  // WARP: [8][2][width] column sums; else 4 x 32 row sums
-  const int T = WARP ? 32 : blockDim.x;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t first = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = WARP ? (int64_t)gridDim.x * 8 : gridDim.x;
-  float dw[NV][V], db[NV][V];
+  RowWalk<Tx, V, NV, WARP> r(x, ldx, width);
+  RowPack<Tx, V>* ring_x = reinterpret_cast<RowPack<Tx, V>*>(shared);
+  RowPack<Tg, V>* ring_g = reinterpret_cast<RowPack<Tg, V>*>(ring_x + D * NV * blockDim.x);
+  float2* params = reinterpret_cast<float2*>(ring_g + D * NV * blockDim.x);
+  RowPack<Tx, V>* mine_x = ring_x + threadIdx.x;
+  RowPack<Tg, V>* mine_g = ring_g + threadIdx.x;
+  auto start = [&](int64_t row, int d) {
+    if (row < rows) {
+      const Tx* src = x + row * ldx;
+      const Tg* src_g = dy + row * lddy;
+      const bool inner = row > 0 && row + 1 < rows;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.f;
-  int turn = 0;
-  for (int64_t row = first; row < rows; row += step, turn ^= 1) {
-    RowPack<Tx, V> xv[NV];
-    RowPack<Tg, V> gv[NV];
-    const float2 st = __ldg(stats + row);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * T + t) * V;
-      xv[j] = load_pack<Tx, V>(x + row * ldx, c, width);
-      if constexpr (V == 1 || sizeof(Tg) * V == 16) {
-        gv[j] = load_pack<Tg, V>(dy + row * lddy, c, width);
-      } else {  // a pack of x spans half of or two 16-byte packs of dy
-        float f[V];
-        if (c + V <= width) {
-          load_vec<Tg, V>(dy + row * lddy + c, f);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) f[e] = c + e < width ? Dt<Tg>::to_f(dy[row * lddy + c + e]) : 0.f;
+      for (int j = 0; j < NV; ++j)
+        if (r.col(j) < width) {
+          fetch<Tx, V>(mine_x + (d * NV + j) * blockDim.x, src, r.col(j), width, inner || !(r.edge >> j & 1));
+          fetch<Tg, V>(mine_g + (d * NV + j) * blockDim.x, src_g, r.col(j), width, inner || !(r.edge >> j & 1));
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) gv[j].e[e] = Dt<Tg>::from_f(f[e]);
-      }
     }
-    float s1 = 0.f, s2 = 0.f;
+    copies_commit();
+  };
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * T + t) * V;
-      float wv[V];
-      load_param<V>(w, c, width, 1.f, wv);
+  for (int d = 0; d < D; ++d)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {  // behind the row's end g = 0
-        const float g = Dt<Tg>::to_f(gv[j].e[e]), n = (Dt<Tx>::to_f(xv[j].e[e]) - st.x) * st.y;
-        const float gw = g * wv[e];
-        s1 += gw;
-        s2 = fmaf(gw, n, s2);
-        dw[j][e] = fmaf(g, n, dw[j][e]);
-        db[j][e] += g;
+    for (int j = 0; j < NV; ++j)
+      if (r.col(j) >= width) {
+        mine_x[(d * NV + j) * blockDim.x] = RowPack<Tx, V>{};
+        mine_g[(d * NV + j) * blockDim.x] = RowPack<Tg, V>{};
       }
-    }
-    if (dx) {
-      const float m1 = row_sum<WARP>(s1, shared + 64 * turn) / (float)width;
-      const float m2 = row_sum<WARP>(s2, shared + 64 * turn + 32) / (float)width;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = (j * T + t) * V;
-        if (c >= width) break;
-        float wv[V], o[V];
-        load_param<V>(w, c, width, 1.f, wv);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float n = (Dt<Tx>::to_f(xv[j].e[e]) - st.x) * st.y;
-          o[e] = st.y * (Dt<Tg>::to_f(gv[j].e[e]) * wv[e] - m1 - n * m2);
-        }
-        store_part<Tx, V>(dx + row * lddx, c, width, o);
-      }
-    }
-  }
-  if (!partial) return;
-  float* out = partial + (int64_t)blockIdx.x * 2 * width;
-  if (!WARP) {
+  for (int d = 0; d < D - 1; ++d) start(r.row + d * r.step, d);
+  float2 wr[REGS ? NV : 1][H];
+  if constexpr (REGS) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int c = (j * T + t) * V + e;
-        if (c < width) {
-          out[c] = dw[j][e];
-          out[width + c] = db[j][e];
-        }
+      for (int k = 0; k < H; ++k) {
+        const int c = r.col(j) + 2 * k;
+        wr[j][k] = make_float2(param_at(w, c, width, 1.f), param_at(w, c + 1, width, 1.f));
       }
-    return;
+  } else {
+    for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x)
+      params[i] = make_float2(param_at(w, 2 * i - r.ph, width, 1.f), param_at(w, 2 * i - r.ph + 1, width, 1.f));
+    __syncthreads();
   }
-  float* mine = shared + (threadIdx.x >> 5) * 2 * width;
+  float2 dw[NV][H], db[NV][H];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int k = 0; k < H; ++k) dw[j][k] = db[j][k] = both(0.f);
+  const float inv = 1.f / (float)width;
+  float2 next = r.row < rows ? __ldg(stats + r.row) : both(0.f);
+  int d = 0, turn = 0;
+  for (int64_t row = r.row; row < rows; row += r.step, turn ^= 1) {
+    const float2 st = next;
+    if (row + r.step < rows) next = __ldg(stats + row + r.step);
+    start(row + (D - 1) * r.step, d == 0 ? D - 1 : d - 1);
+    copies_wait<D - 1>();
+    const float2 rs = both(st.y), mu = both(-st.x);
+    float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {  // outside the row g = 0 (and x, but for edges of rows with a mean that is not finite)
+      float2 xv[H], gv[H];
+      const bool edge = r.edge >> j & 1;
+      read_slot<Tx, V>(mine_x + (d * NV + j) * blockDim.x, edge, r.col(j), width, xv);
+      read_slot<Tg, V>(mine_g + (d * NV + j) * blockDim.x, edge, r.col(j), width, gv);
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
+        const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[(j * r.T + r.t) * H + k]);
+        s1 = __fadd2_rn(s1, gw);
+        s2 = __ffma2_rn(gw, n, s2);
+        dw[j][k] = __ffma2_rn(gv[k], n, dw[j][k]);
+        db[j][k] = __fadd2_rn(db[j][k], gv[k]);
+      }
+    }
+    if (dx) {
+      const float2 m = row_sums<WARP, true>(make_float2(s1.x + s1.y, s2.x + s2.y), red[WARP ? 0 : turn]);
+      asm volatile("" ::: "memory");  // the row is read from shared memory again: kept, its registers would spill
+      // dx = s g w - s m1 - s m2 n
+      const float2 a = both(-st.y * (m.x * inv)), c2 = both(-st.y * (m.y * inv));
+      Tx* dst = dx + row * lddx;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (r.col(j) >= width) break;
+        float2 xv[H], gv[H];
+        const bool edge = r.edge >> j & 1;
+        read_slot<Tx, V>(mine_x + (d * NV + j) * blockDim.x, false, 0, width, xv);
+        read_slot<Tg, V>(mine_g + (d * NV + j) * blockDim.x, false, 0, width, gv);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
+          const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[(j * r.T + r.t) * H + k]);
+          xv[k] = __ffma2_rn(gw, rs, __ffma2_rn(n, c2, a));
+        }
+        store_part<Tx, V>(dst, edge, r.col(j), width, xv);
+      }
+    }
+    d = d + 1 == D ? 0 : d + 1;
+  }
+  copies_wait<0>();
+  if (!partial) return;
+  float* out = partial + (int64_t)blockIdx.x * 2 * width;
+  float* sums = reinterpret_cast<float*>(shared) + (threadIdx.x >> 5) * 2 * width;
+  if (WARP) __syncthreads();  // ring and weight are not read any more
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = (j * T + t) * V + e;
-      if (c < width) {
-        mine[c] = dw[j][e];
-        mine[width + c] = db[j][e];
+      const int c = r.col(j) + e;
+      if ((unsigned)c < (unsigned)width) {
+        (WARP ? sums : out)[c] = e & 1 ? dw[j][e / 2].y : dw[j][e / 2].x;
+        (WARP ? sums : out)[width + c] = e & 1 ? db[j][e / 2].y : db[j][e / 2].x;
       }
     }
+  if (!WARP) return;
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += shared[k * 2 * width + c];
+    for (int k = 0; k < 8; ++k) s += reinterpret_cast<float*>(shared)[k * 2 * width + c];
     out[c] = s;
   }
 }
@@ -278,27 +429,25 @@ using namespace rk;
 
 namespace {
 
-constexpr int kMaxWidth = 16384;  // 16 elements a thread, 1024 threads
+constexpr int kMaxWidth = 16384;  // 32 elements a thread, 512 threads
 constexpr int kWarpWidth = 1024;  // 32 elements a lane
+constexpr int kCtaWidth = 8192;   // 16 elements a thread, 512 threads
 
-NormParam make_param(const void* p, int dtype, bool vec16) {
-  // a vector of 4 or 8 parameters is read in 16-byte (fp32) or 8/16-byte pieces
-  return NormParam{p, dtype, vec16 && rk_host::aligned(p, 16) ? 1 : 0};
+// Threads of a row's CTA: `per` elements each, whole warps.
+int cta_threads(int64_t elements, int per) { return (int)((elements + per * 32 - 1) / (per * 32) * 32); }
+
+// CTAs for warps' rows, at most `most` of them: a multiple of 8, eight warps each.
+int64_t warp_ctas(int64_t rows, int64_t most) {
+  const int64_t want = (rows + 63) / 64 * 8;
+  return want < most / 8 * 8 ? want : most / 8 * 8;
 }
 
-// Threads of a row's CTA: 16 elements each (scalar rows the same), whole warps.
-int cta_threads(int64_t width) { return (int)((width + 16 * 32 - 1) / (16 * 32) * 32); }
-
-bool rows_vec(const void* p, int64_t ld, size_t size, int64_t rows, size_t bytes) {
-  return rk_host::aligned(p, bytes) && (rows <= 1 || (ld * size) % bytes == 0);
-}
-
-// CTAs of the backward: as many as fit the SMs at once (rows permitting), so partial rows stay few.
-int64_t bwd_ctas(int64_t rows, int64_t width) {
-  const bool warp = width <= kWarpWidth;
-  const int64_t most = warp ? 148 * (width <= 512 ? 4 : 2) : 148 * (width <= 4096 ? 4 : width <= 8192 ? 2 : 1);
-  const int64_t want = warp ? (rows + 7) / 8 : rows;
-  return want < most ? want : most;
+// CTAs of the backward for rows of `span` elements from boundary to boundary: as many as the SMs hold at once, so
+// partial rows stay few; a multiple of 8 where a CTA visits more than one row.
+int64_t bwd_ctas(int64_t rows, int64_t span) {
+  if (span <= kWarpWidth) return warp_ctas(rows, 148 * (span <= 256 ? 3 : 2));
+  const int64_t most = 148 * (span <= 2560 ? 4 : span <= 5120 ? 2 : 1) / 8 * 8;
+  return rows < most ? rows : most;
 }
 
 struct NormArgs {
@@ -311,6 +460,7 @@ struct NormArgs {
   float* partial;
   int64_t rows;
   int width;
+  int span;  // elements between the boundaries around a row, at most
   float eps;
   bool backward;
   cudaStream_t s;
@@ -318,54 +468,58 @@ struct NormArgs {
 
 template <typename Tx, typename To, int V, int NV, bool WARP>
 int launch(const NormArgs& a) {
+  const int threads = WARP ? 256 : cta_threads(a.span, NV * V);
+  const size_t params = norm_param_regs(NV * V, WARP) ? 0 : (size_t)NV * V * (WARP ? 32 : threads) * 4;
   if (!a.backward) {
-    const int64_t grid = WARP ? (a.rows + 7) / 8 : a.rows;
-    if (grid >= (1ll << 31)) return RK_ERR_UNSUPPORTED;
-    rk_host::launch_k(layernorm_fwd_kernel<Tx, To, V, NV, WARP>, (unsigned)grid, WARP ? 256 : cta_threads(a.width), 0, a.s,
-                      static_cast<const Tx*>(a.x), a.ldx, a.w, a.b, static_cast<To*>(a.out), a.ldo, a.stats, a.rows,
-                      a.width, a.eps);
+    auto kern = layernorm_fwd_kernel<Tx, To, V, NV, WARP>;
+    const int bytes = NV * V * (int)sizeof(Tx);
+    const size_t smem = (size_t)norm_depth(NV * V, (int)sizeof(Tx), WARP) * bytes * threads + 2 * params;
+    if (smem > 46 * 1024)  // beside 1 KB of row sums
+      if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
+    const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (WARP ? NV * V <= 16 ? 1024 : 512 : 512) / threads;
+    const int64_t most = 148 * (fit < held ? fit : held);
+    const int64_t grid = WARP ? warp_ctas(a.rows, most) : a.rows < most ? a.rows : most / 8 * 8;
+    rk_host::launch_k(kern, (unsigned)grid, threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w, a.b,
+                      static_cast<To*>(a.out), a.ldo, a.stats, a.rows, a.width, a.eps);
     return rk_host::launch_status();
   }
   auto kern = layernorm_bwd_kernel<Tx, To, V, NV, WARP>;
-  const size_t smem = WARP ? (a.partial ? (size_t)16 * a.width * 4 : 0) : 512;
-  if (smem > 48 * 1024)
+  const int bytes = NV * V * (int)(sizeof(Tx) + sizeof(To));
+  size_t smem = (size_t)norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(To)), WARP) * bytes * threads + params;
+  if (WARP && smem < (size_t)16 * a.width * 4) smem = (size_t)16 * a.width * 4;
+  if (smem > 46 * 1024)
     if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
-  rk_host::launch_k(kern, (unsigned)bwd_ctas(a.rows, a.width), WARP ? 256 : cta_threads(a.width), smem, a.s,
-                    static_cast<const Tx*>(a.x), a.ldx, a.w, a.stats, static_cast<const To*>(a.dy), a.lddy,
-                    static_cast<Tx*>(a.out), a.ldo, a.partial, a.rows, a.width);
+  rk_host::launch_k(kern, (unsigned)bwd_ctas(a.rows, a.span), threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w,
+                    a.stats, static_cast<const To*>(a.dy), a.lddy, static_cast<Tx*>(a.out), a.ldo, a.partial, a.rows,
+                    a.width);
   return rk_host::launch_status();
 }
 
-// Vectors of 16 bytes of x where every row allows them, single elements otherwise.
 template <typename Tx, typename To>
-int dispatch(const NormArgs& a, bool vec) {
+int dispatch(const NormArgs& a) {
   constexpr int V = 16 / (int)sizeof(Tx);
-  const int w = a.width;
-  if (w > kWarpWidth) {
-    if (vec) return launch<Tx, To, V, 16 / V, false>(a);
-    return launch<Tx, To, 1, 16, false>(a);
-  }
-  if (!vec) return w <= 256 ? launch<Tx, To, 1, 8, true>(a) : launch<Tx, To, 1, 32, true>(a);
-  if (w <= 32 * V) return launch<Tx, To, V, 1, true>(a);
-  if (w <= 64 * V) return launch<Tx, To, V, 2, true>(a);
+  if (a.span > kCtaWidth) return launch<Tx, To, V, 32 / V, false>(a);
+  if (a.span > kWarpWidth) return launch<Tx, To, V, 16 / V, false>(a);
+  if (a.span <= 32 * V) return launch<Tx, To, V, 1, true>(a);
+  if (a.span <= 64 * V) return launch<Tx, To, V, 2, true>(a);
   if constexpr (V == 4)
-    if (w > 128 * V) return launch<Tx, To, V, 8, true>(a);
+    if (a.span > 128 * V) return launch<Tx, To, V, 8, true>(a);
   return launch<Tx, To, V, 4, true>(a);
 }
 
 // x in fp32: the other side in any type; x in 16 bits: the same type or fp32.
-int dispatch_types(const NormArgs& a, int x_dtype, int o_dtype, bool vec) {
+int dispatch_types(const NormArgs& a, int x_dtype, int o_dtype) {
   if (x_dtype == RK_F32) {
-    if (o_dtype == RK_F32) return dispatch<float, float>(a, vec);
-    if (o_dtype == RK_BF16) return dispatch<float, __nv_bfloat16>(a, vec);
-    return dispatch<float, __half>(a, vec);
+    if (o_dtype == RK_F32) return dispatch<float, float>(a);
+    if (o_dtype == RK_BF16) return dispatch<float, __nv_bfloat16>(a);
+    return dispatch<float, __half>(a);
   }
   if (x_dtype == RK_BF16) {
-    if (o_dtype == RK_BF16) return dispatch<__nv_bfloat16, __nv_bfloat16>(a, vec);
-    if (o_dtype == RK_F32) return dispatch<__nv_bfloat16, float>(a, vec);
+    if (o_dtype == RK_BF16) return dispatch<__nv_bfloat16, __nv_bfloat16>(a);
+    if (o_dtype == RK_F32) return dispatch<__nv_bfloat16, float>(a);
   } else {
-    if (o_dtype == RK_F16) return dispatch<__half, __half>(a, vec);
-    if (o_dtype == RK_F32) return dispatch<__half, float>(a, vec);
+    if (o_dtype == RK_F16) return dispatch<__half, __half>(a);
+    if (o_dtype == RK_F32) return dispatch<__half, float>(a);
   }
   return RK_ERR_DTYPE;
 }
@@ -375,10 +529,19 @@ bool types_ok(int x_dtype, int o_dtype, int p_dtype) {
          (x_dtype == RK_F32 || o_dtype == RK_F32 || x_dtype == o_dtype);
 }
 
-// Bytes that V elements (16 bytes of x) take on the other side: its rows must allow vectors of that size, 16 at most.
-size_t other_bytes(int x_dtype, int o_dtype) {
-  const size_t b = 16 / rk_host::dtype_size(x_dtype) * rk_host::dtype_size(o_dtype);
-  return b < 16 ? b : 16;
+// Whether every row of `p` (row stride ld) is as far from a boundary, in elements, as the row of x.
+bool same_phase(const void* x, int64_t ldx, int x_dtype, const void* p, int64_t ld, int dtype, int64_t rows) {
+  const int64_t size = (int64_t)rk_host::dtype_size(x_dtype), other = (int64_t)rk_host::dtype_size(dtype), v = 16 / size;
+  if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(p) % other) return false;
+  const int64_t a = (int64_t)(reinterpret_cast<uintptr_t>(x) / size), b = (int64_t)(reinterpret_cast<uintptr_t>(p) / other);
+  return a % v == b % v && (rows <= 1 || ldx % v == ld % v);
+}
+
+// Elements between the 16-byte boundaries around a row: all rows start equally far from one, or anywhere.
+int row_span(const void* x, int64_t ldx, int x_dtype, int64_t rows, int64_t width) {
+  const int64_t size = (int64_t)rk_host::dtype_size(x_dtype), v = 16 / size;
+  const int64_t ph = rows <= 1 || ldx % v == 0 ? (int64_t)(reinterpret_cast<uintptr_t>(x) / size) % v : v - 1;
+  return (int)((width + ph + v - 1) / v * v);
 }
 
 }  // namespace
@@ -392,26 +555,27 @@ extern "C" int rk_layernorm_fwd(const void* x, int x_dtype, int64_t ldx, const v
   if (rows == 0) return RK_OK;
   if (!x || !y) return RK_ERR_ARG;
   if (stats && !rk_host::aligned(stats, 8)) return RK_ERR_ALIGN;
-  const bool vec = rows_vec(x, ldx, rk_host::dtype_size(x_dtype), rows, 16) &&
-                   rows_vec(y, ldy, rk_host::dtype_size(y_dtype), rows, other_bytes(x_dtype, y_dtype));
+  if (!same_phase(x, ldx, x_dtype, y, ldy, y_dtype, rows)) return RK_ERR_ALIGN;
   NormArgs a{};
   a.x = x;
   a.ldx = ldx;
-  a.w = make_param(w, param_dtype, vec);
-  a.b = make_param(b, param_dtype, vec);
+  a.w = NormParam{w, param_dtype};
+  a.b = NormParam{b, param_dtype};
   a.out = y;
   a.ldo = ldy;
   a.stats = reinterpret_cast<float2*>(stats);
   a.rows = rows;
   a.width = (int)width;
+  a.span = row_span(x, ldx, x_dtype, rows, width);
   a.eps = eps;
   a.s = static_cast<cudaStream_t>(stream);
-  return dispatch_types(a, x_dtype, y_dtype, vec);
+  return dispatch_types(a, x_dtype, y_dtype);
 }
 
 extern "C" int64_t rk_layernorm_bwd_workspace(int64_t rows, int64_t width) {
   if (rows <= 0 || width <= 0) return 0;
-  return bwd_ctas(rows, width) * 2 * width * (int64_t)sizeof(float);
+  const int64_t a = bwd_ctas(rows, width), b = bwd_ctas(rows, width + 14);  // the spans there may be
+  return (a > b ? a : b) * 2 * width * (int64_t)sizeof(float);
 }
 
 extern "C" int rk_layernorm_bwd(const void* x, int x_dtype, int64_t ldx, const void* w, int param_dtype,
@@ -426,29 +590,31 @@ extern "C" int rk_layernorm_bwd(const void* x, int x_dtype, int64_t ldx, const v
   if (rows && (!x || !dy || !stats)) return RK_ERR_ARG;
   if (rows && !rk_host::aligned(stats, 8)) return RK_ERR_ALIGN;
   if (columns && rows && (!workspace || workspace_bytes < rk_layernorm_bwd_workspace(rows, width))) return RK_ERR_WORKSPACE;
+  int parts = 0;  // no rows: the columns' sums are zeros
   if (rows && (dx || columns)) {
-    const size_t xs = rk_host::dtype_size(x_dtype);
-    const bool vec = rows_vec(x, ldx, xs, rows, 16) && (!dx || rows_vec(dx, lddx, xs, rows, 16)) &&
-                     rows_vec(dy, lddy, rk_host::dtype_size(dy_dtype), rows, other_bytes(x_dtype, dy_dtype));
+    if (!same_phase(x, ldx, x_dtype, dy, lddy, dy_dtype, rows) ||
+        (dx && !same_phase(x, ldx, x_dtype, dx, lddx, x_dtype, rows)))
+      return RK_ERR_ALIGN;
     NormArgs a{};
     a.backward = true;
     a.x = x;
     a.ldx = ldx;
     a.dy = dy;
     a.lddy = lddy;
-    a.w = make_param(w, param_dtype, vec);
+    a.w = NormParam{w, param_dtype};
     a.out = dx;
     a.ldo = lddx;
     a.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
     a.partial = columns ? workspace : nullptr;
     a.rows = rows;
     a.width = (int)width;
+    a.span = row_span(x, ldx, x_dtype, rows, width);
     a.s = s;
-    const int st = dispatch_types(a, x_dtype, dy_dtype, vec);
+    parts = (int)bwd_ctas(rows, a.span);
+    const int st = dispatch_types(a, x_dtype, dy_dtype);
     if (st != RK_OK) return st;
   }
   if (!columns) return RK_OK;
-  const int parts = rows ? (int)bwd_ctas(rows, width) : 0;  // no rows: zeros
   const unsigned grid = (unsigned)((2 * width + 31) / 32);
   if (param_dtype == RK_F32)
     rk_host::launch_k(layernorm_columns_kernel<float>, grid, 1024, 0, s, workspace, parts, (int)width,

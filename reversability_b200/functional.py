@@ -101,6 +101,16 @@ def even_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     return t.contiguous(), rows, width, width
 
 
+def _norm_rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, int, int, int]:
+    """even_rows of a tensor whose rows start as far from multiples of `per` elements as those of a new contiguous one
+    (what the layer norm's vectors need); others are copied."""
+    rows_of = even_rows(t)
+    r, rows, width, ld = rows_of
+    if r.data_ptr() // t.element_size() % per == 0 and (rows <= 1 or (ld - width) % per == 0):
+        return rows_of
+    return t.clone(memory_format=torch.contiguous_format), rows, width, width
+
+
 def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None):
     """(weight, bias, dtype code): contiguous [width] vectors of one type, fp32 or x's."""
     dtype = None
@@ -126,7 +136,7 @@ def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tens
         raise ValueError("layer norm of 16-bit inputs gives their type or fp32")
     _on_current_device(x, "the input", weight, bias)
     weight, bias, pcode = _norm_params(x, weight, bias)
-    xr, rows, width, ld = even_rows(x)
+    xr, rows, width, ld = _norm_rows(x, 16 // x.element_size())
     y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
     stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32) if want_stats else None
     _lib.call("rk_layernorm_fwd", xr.data_ptr(), _lib.code(x.dtype), ld, _lib.ptr(weight), _lib.ptr(bias), pcode,
@@ -143,8 +153,9 @@ def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Ten
     weight, _, _ = _norm_params(x, weight, None)
     if weight is not None and weight.dtype != param_dtype:
         raise ValueError("parameter gradients come in the weight's type")
-    xr, rows, width, ldx = even_rows(x)
-    dyr, _, _, lddy = even_rows(dy)
+    per = 16 // x.element_size()
+    xr, rows, width, ldx = _norm_rows(x, per)
+    dyr, _, _, lddy = _norm_rows(dy, per)
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
     dw = torch.empty(width, device=x.device, dtype=param_dtype) if want_dw else None
     db = torch.empty(width, device=x.device, dtype=param_dtype) if want_db else None
