@@ -164,16 +164,23 @@ struct RowWalk {
       if (col(j) < width && (col(j) < 0 || col(j) + V > width)) edge |= 1u << j;
   }
   __device__ __forceinline__ int col(int j) const { return (j * T + t) * V - ph; }
+  // Place of pair k of vector (j, t) among the parameters in shared memory: 16-byte pieces, lane beside lane.
+  __device__ __forceinline__ int param(int j, int k) const { return ((j * (V / 4) + k / 2) * T + t) * 2 + k % 2; }
+  // Column of the pair at place i.
+  __device__ __forceinline__ int param_col(int i) const {
+    const int piece = i / (2 * T), j = piece / (V / 4);
+    return (j * T + i / 2 % T) * V + (piece - j * (V / 4)) * 4 + i % 2 * 2 - ph;
+  }
 };
 
 template <typename Tx, typename Ty, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 2) : 1)
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 3) : 1)
     layernorm_fwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const NormParam b,
                          Ty* __restrict__ y, int64_t ldy, float2* __restrict__ stats, int64_t rows, int width,
                          float eps) {
   constexpr int D = norm_depth(NV * V, (int)sizeof(Tx), WARP), H = V / 2;
   constexpr bool REGS = norm_param_regs(NV * V, WARP);
-  extern __shared__ uint4 shared[];  // [D][NV][threads] packs of x, then parameters: [2][NV][T] vectors of floats
+  extern __shared__ uint4 shared[];  // [D][NV][threads] packs of x, then weight and bias, NV * T * V floats each
   __shared__ float2 red[WARP ? 1 : 4][16];
   pdl_wait();  // inputs are the previous kernel's outputs
   RowWalk<Tx, V, NV, WARP> r(x, ldx, width);
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 2
       }
   } else {
     for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x) {
-      const int c = 2 * i - r.ph;
+      const int c = r.param_col(i);
       params[i] = make_float2(param_at(w, c, width, 1.f), param_at(w, c + 1, width, 1.f));
       params[NV * r.T * H + i] = make_float2(param_at(b, c, width, 0.f), param_at(b, c + 1, width, 0.f));
     }
@@ -253,7 +260,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 2
       if (r.col(j) >= width) break;
 #pragma unroll
       for (int k = 0; k < H; ++k) {
-        const int at = (j * r.T + r.t) * H + k;
+        const int at = r.param(j, k);
         v[j][k] = __ffma2_rn(__fmul2_rn(v[j][k], both(rstd)), REGS ? wr[j][k] : params[at],
                              REGS ? br[j][k] : params[NV * r.T * H + at]);
       }
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
                          float* __restrict__ partial, int64_t rows, int width) {
   constexpr int D = norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), WARP), H = V / 2;
   constexpr bool REGS = norm_param_regs(NV * V, WARP);
-  // [D][NV][threads] packs of x, then of dy, then the weight [NV][T] vectors; at the end (WARP) [8][2][width] column sums
+  // [D][NV][threads] packs of x, then of dy, then the weight; at the end (WARP) [8][2][width] column sums
   extern __shared__ uint4 shared[];
   __shared__ float2 red[WARP ? 1 : 2][16];
   pdl_wait();  // inputs are the previous kernel's outputs
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
       }
   } else {
     for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x)
-      params[i] = make_float2(param_at(w, 2 * i - r.ph, width, 1.f), param_at(w, 2 * i - r.ph + 1, width, 1.f));
+      params[i] = make_float2(param_at(w, r.param_col(i), width, 1.f), param_at(w, r.param_col(i) + 1, width, 1.f));
     __syncthreads();
   }
   float2 dw[NV][H], db[NV][H];
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
-        const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[(j * r.T + r.t) * H + k]);
+        const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[r.param(j, k)]);
         s1 = __fadd2_rn(s1, gw);
         s2 = __ffma2_rn(gw, n, s2);
         dw[j][k] = __ffma2_rn(gv[k], n, dw[j][k]);
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
 #pragma unroll
         for (int k = 0; k < H; ++k) {
           const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
-          const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[(j * r.T + r.t) * H + k]);
+          const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[r.param(j, k)]);
           xv[k] = __ffma2_rn(gw, rs, __ffma2_rn(n, c2, a));
         }
         store_part<Tx, V>(dst, edge, r.col(j), width, xv);
@@ -476,7 +483,7 @@ int launch(const NormArgs& a) {
     const size_t smem = (size_t)norm_depth(NV * V, (int)sizeof(Tx), WARP) * bytes * threads + 2 * params;
     if (smem > 46 * 1024)  // beside 1 KB of row sums
       if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
-    const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (WARP ? NV * V <= 16 ? 1024 : 512 : 512) / threads;
+    const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (WARP ? NV * V <= 16 ? 1024 : 768 : 512) / threads;
     const int64_t most = 148 * (fit < held ? fit : held);
     const int64_t grid = WARP ? warp_ctas(a.rows, most) : a.rows < most ? a.rows : most / 8 * 8;
     rk_host::launch_k(kern, (unsigned)grid, threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w, a.b,
