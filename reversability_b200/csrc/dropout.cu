@@ -9,85 +9,137 @@
 //   kept  iff word i >= round(p 2^32);  y_i = residual_i + (kept ? x_i / (1 - p) : 0)
 //
 // Bound by memory for fp32 and with a residual. In 16 bits without one an
-// element moves 4 bytes and costs 5 wide multiplies and about 9 other
-// instructions, about two thirds of the issue slots at full bandwidth.
+// element moves 4 bytes and costs 4.5 wide multiplies and about 10 other
+// instructions, some two thirds of the issue slots at full bandwidth: what is
+// the same for all blocks of a thread (round keys, the second counter word's
+// first product, the first word's second) is formed once, pairs are scaled and
+// rounded by one instruction.
+#include <type_traits>
 #include "vec.cuh"
 
 namespace rk {
 
-__device__ __forceinline__ uint4 philox10(uint64_t block, uint64_t offset, uint64_t key) {
-  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-  uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+
+// The generator for blocks that share the upper half of their number.
+struct Philox {
+  uint32_t k0[10], k1[10];
+  uint32_t c3k1, l1k0, h2k1, l2;  // parts of rounds 1 and 2
+  __device__ __forceinline__ Philox(uint32_t block_hi, uint64_t offset, uint64_t key) {
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
-    c1 = (uint32_t)b;
-    c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    for (int r = 0; r < 10; ++r) {
+      k0[r] = (uint32_t)key + r * kPhiloxW0;
+      k1[r] = (uint32_t)(key >> 32) + r * kPhiloxW1;
+    }
+    const uint64_t b = (uint64_t)(uint32_t)offset * kPhiloxM1;  // round 1 of words 2 and 3
+    const uint64_t a = (uint64_t)((uint32_t)(b >> 32) ^ block_hi ^ k0[0]) * kPhiloxM0;  // round 2 of word 0
+    c3k1 = (uint32_t)(offset >> 32) ^ k1[0];
+    l1k0 = (uint32_t)b ^ k0[1];
+    h2k1 = (uint32_t)(a >> 32) ^ k1[1];
+    l2 = (uint32_t)a;
   }
-  return make_uint4(c0, c1, c2, c3);
-}
+  __device__ __forceinline__ void block(uint32_t block_lo, uint32_t (&w)[4]) const {
+    const uint64_t a1 = (uint64_t)block_lo * kPhiloxM0;
+    const uint64_t b2 = (uint64_t)((uint32_t)(a1 >> 32) ^ c3k1) * kPhiloxM1;
+    uint32_t c0 = (uint32_t)(b2 >> 32) ^ l1k0, c1 = (uint32_t)b2, c2 = (uint32_t)a1 ^ h2k1, c3 = l2;
+#pragma unroll
+    for (int r = 2; r < 10; ++r) {
+      const uint64_t a = (uint64_t)c0 * kPhiloxM0, b = (uint64_t)c2 * kPhiloxM1;
+      c0 = (uint32_t)(b >> 32) ^ c1 ^ k0[r];
+      c2 = (uint32_t)(a >> 32) ^ c3 ^ k1[r];
+      c1 = (uint32_t)b;
+      c3 = (uint32_t)a;
+    }
+    w[0] = c0;
+    w[1] = c1;
+    w[2] = c2;
+    w[3] = c3;
+  }
+};
 
 struct DropArgs {
   int64_t n;
   uint64_t seed, offset;
   const int64_t* seed_dev;  // used instead of seed when not null
-  uint32_t below;           // words up to this one drop ...
-  uint32_t all;             // ... unless all bits are set here: nothing drops
+  uint32_t border;          // words from this one on keep their element
   float scale;
 };
 
-// V consecutive elements from i0 on (a multiple of 4): elements at or past n are not touched.
-template <typename Tx, typename Tr, typename Ty, int V, bool RES, bool VEC>
-__device__ __forceinline__ void drop_chunk(const Tx* __restrict__ x, const Tr* __restrict__ res, Ty* __restrict__ y,
-                                           int64_t i0, const DropArgs& a, uint64_t key) {
-  float v[V], o[V];
-  const bool whole = VEC && i0 + V <= a.n;
-  if (whole) {
-    load_vec<Tx, V>(x + i0, v);
-    if (RES) load_vec<Tr, V>(res + i0, o);
+// Two values rounded to a pair of 16-bit ones.
+template <typename T>
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  uint32_t d;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_rounded(T* __restrict__ p, const float (&v)[V]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t r[V / 2];
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) r[k] = round_pair<T>(v[2 * k], v[2 * k + 1]);
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
   } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[e] = i0 + e < a.n ? Dt<Tx>::to_f(x[i0 + e]) : 0.f;
-      if (RES) o[e] = i0 + e < a.n ? Dt<Tr>::to_f(res[i0 + e]) : 0.f;
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < V / 4; ++q) {
-    const uint4 w = philox10((uint64_t)(i0 >> 2) + q, a.offset, key);
-    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {  // a dropped value is not used, whatever it is
-      const float kept = (word[e] | a.all) > a.below ? v[q * 4 + e] * a.scale : 0.f;
-      o[q * 4 + e] = RES ? o[q * 4 + e] + kept : kept;
-    }
-  }
-  if (whole) {
-    store_vec<Ty, V>(y + i0, o);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (i0 + e < a.n) y[i0 + e] = Dt<Ty>::from_f(o[e]);
+    store_vec<T, V>(p, v);
   }
 }
 
 constexpr int kDropThreads = 256, kDropUnroll = 2;
 
+// A thread takes kDropUnroll vectors of V elements, all loads before the words are formed. A CTA's elements are an
+// aligned power of two, so the upper half of the block number is the same for all of them. The last CTA, and tensors
+// that do not start on vector boundaries (VEC false), go element by element.
 template <typename Tx, typename Tr, typename Ty, bool RES, bool VEC>
 __global__ void __launch_bounds__(kDropThreads)
     dropout_kernel(const Tx* __restrict__ x, const Tr* __restrict__ res, Ty* __restrict__ y, const DropArgs a) {
   pdl_wait();  // inputs are the previous kernel's outputs
-  constexpr int V = VEC ? 16 / (int)sizeof(Tx) : 4;
-  const uint64_t key = a.seed_dev ? (uint64_t)__ldg(a.seed_dev) : a.seed;
-  const int64_t c0 = (int64_t)blockIdx.x * (kDropThreads * kDropUnroll) + threadIdx.x;
+  constexpr int V = 16 / (int)sizeof(Tx);
+  constexpr int PER = kDropThreads * kDropUnroll * V;
+  static_assert((PER & (PER - 1)) == 0, "a power of two");
+  const int64_t base = (int64_t)blockIdx.x * PER;
+  const Philox gen((uint32_t)(base >> 34), a.offset, a.seed_dev ? (uint64_t)__ldg(a.seed_dev) : a.seed);
+  const bool whole = VEC && base + PER <= a.n;
+  float v[kDropUnroll][V], o[kDropUnroll][V];
 #pragma unroll
   for (int u = 0; u < kDropUnroll; ++u) {
-    const int64_t i0 = (c0 + u * kDropThreads) * V;
-    if (i0 < a.n) drop_chunk<Tx, Tr, Ty, V, RES, VEC>(x, res, y, i0, a, key);
+    const int64_t i0 = base + (u * kDropThreads + threadIdx.x) * V;
+    if (whole) {
+      load_vec<Tx, V>(x + i0, v[u]);
+      if (RES) load_vec<Tr, V>(res + i0, o[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[u][e] = i0 + e < a.n ? Dt<Tx>::to_f(x[i0 + e]) : 0.f;
+        if (RES) o[u][e] = i0 + e < a.n ? Dt<Tr>::to_f(res[i0 + e]) : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kDropUnroll; ++u) {
+    const int64_t i0 = base + (u * kDropThreads + threadIdx.x) * V;
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      uint32_t w[4];
+      gen.block((uint32_t)(i0 >> 2) + q, w);
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {  // a dropped value is not used, whatever it is
+        const int k = q * 4 + e;
+        const float2 s = __fmul2_rn(make_float2(v[u][k], v[u][k + 1]), make_float2(a.scale, a.scale));
+        const float2 kept = make_float2(w[e] >= a.border ? s.x : 0.f, w[e + 1] >= a.border ? s.y : 0.f);
+        const float2 r = RES ? __fadd2_rn(make_float2(o[u][k], o[u][k + 1]), kept) : kept;
+        o[u][k] = r.x;
+        o[u][k + 1] = r.y;
+      }
+    }
+    if (whole) {
+      store_rounded<Ty, V>(y + i0, o[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i0 + e < a.n) y[i0 + e] = Dt<Ty>::from_f(o[u][e]);
+    }
   }
 }
 
@@ -103,7 +155,7 @@ int launch(const void* x, const void* res, void* y, const DropArgs& a, cudaStrea
   constexpr int V = 16 / (int)sizeof(Tx);
   auto fits = [](const void* p, size_t bytes) { return rk_host::aligned(p, bytes < 16 ? bytes : 16); };
   const bool vec = fits(x, 16) && fits(y, V * sizeof(Ty)) && (!RES || fits(res, V * sizeof(Tr)));
-  const int64_t per = (int64_t)kDropThreads * kDropUnroll * (vec ? V : 4);
+  const int64_t per = (int64_t)kDropThreads * kDropUnroll * V;
   const int64_t grid = (a.n + per - 1) / per;
   if (grid >= (1ll << 31)) return RK_ERR_UNSUPPORTED;
   const Tx* xp = static_cast<const Tx*>(x);
@@ -143,10 +195,15 @@ extern "C" int rk_dropout(const void* x, int x_dtype, const void* residual, void
   uint64_t words = (uint64_t)border;       // rounded to the nearest even whole number
   const double rest = border - (double)words;
   if (rest > 0.5 || (rest == 0.5 && (words & 1))) ++words;
-  a.all = words ? 0u : 0xffffffffu;
-  a.below = words ? (uint32_t)(words - 1) : 0u;
-  a.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (words >> 32) {  // everything drops
+    const size_t bytes = (size_t)n * rk_host::dtype_size(y_dtype);
+    const cudaError_t e = residual ? cudaMemcpyAsync(y, residual, bytes, cudaMemcpyDeviceToDevice, s)
+                                   : cudaMemsetAsync(y, 0, bytes, s);
+    return e == cudaSuccess ? RK_OK : RK_ERR_LAUNCH;
+  }
+  a.border = (uint32_t)words;
+  a.scale = (float)(1.0 / (1.0 - p));
   if (x_dtype == RK_BF16) return launch16<__nv_bfloat16>(x, residual, y, y_dtype, a, s);
   if (x_dtype == RK_F16) return launch16<__half>(x, residual, y, y_dtype, a, s);
   if (y_dtype == RK_F32)
