@@ -8,12 +8,15 @@
 //            as 1, 2, 3", SC 2011);
 //   kept  iff word i >= round(p 2^32);  y_i = residual_i + (kept ? x_i / (1 - p) : 0)
 //
-// Bound by memory for fp32 and with a residual. In 16 bits without one an
-// element moves 4 bytes and costs 4.5 wide multiplies and about 10 other
-// instructions, some two thirds of the issue slots at full bandwidth: what is
-// the same for all blocks of a thread (round keys, the second counter word's
-// first product, the first word's second) is formed once, pairs are scaled and
-// rounded by one instruction.
+// Bound by memory for fp32 and with a residual; in 16 bits without one, where
+// an element moves 4 bytes, by the integer pipes: 20 instructions an element, a
+// quarter of them wide multiplies, half of the rest on the half-rate logic
+// pipe. 134M bf16 elements take 115 us (4.7 TB/s; 163 us with one vector after
+// the other and nothing shared): what is the same for all blocks of a thread
+// (round keys, the second counter word's first product, the first word's
+// second) is formed once, pairs are scaled and rounded by one instruction, and
+// the next tile is loaded before this one's words are formed. 4 CTAs an SM and
+// two vectors a thread: 5 and 6 CTAs 117 and 119 us, one vector 127, four 118.
 #include <type_traits>
 #include "vec.cuh"
 
@@ -86,59 +89,98 @@ __device__ __forceinline__ void store_rounded(T* __restrict__ p, const float (&v
   }
 }
 
-constexpr int kDropThreads = 256, kDropUnroll = 2;
+constexpr int kDropThreads = 256, kDropCtas = 4;
+// Vectors a thread takes at a time: two, one where the residual takes twice the registers.
+__host__ __device__ constexpr int drop_unroll(int size_x, int size_res) { return size_res > size_x ? 1 : 2; }
 
-// A thread takes kDropUnroll vectors of V elements, all loads before the words are formed. A CTA's elements are an
-// aligned power of two, so the upper half of the block number is the same for all of them. The last CTA, and tensors
-// that do not start on vector boundaries (VEC false), go element by element.
-template <typename Tx, typename Tr, typename Ty, bool RES, bool VEC>
-__global__ void __launch_bounds__(kDropThreads)
-    dropout_kernel(const Tx* __restrict__ x, const Tr* __restrict__ res, Ty* __restrict__ y, const DropArgs a) {
-  pdl_wait();  // inputs are the previous kernel's outputs
-  constexpr int V = 16 / (int)sizeof(Tx);
-  constexpr int PER = kDropThreads * kDropUnroll * V;
-  static_assert((PER & (PER - 1)) == 0, "a power of two");
-  const int64_t base = (int64_t)blockIdx.x * PER;
-  const Philox gen((uint32_t)(base >> 34), a.offset, a.seed_dev ? (uint64_t)__ldg(a.seed_dev) : a.seed);
-  const bool whole = VEC && base + PER <= a.n;
-  float v[kDropUnroll][V], o[kDropUnroll][V];
-#pragma unroll
-  for (int u = 0; u < kDropUnroll; ++u) {
-    const int64_t i0 = base + (u * kDropThreads + threadIdx.x) * V;
-    if (whole) {
-      load_vec<Tx, V>(x + i0, v[u]);
-      if (RES) load_vec<Tr, V>(res + i0, o[u]);
+// V elements of T as they lie in memory.
+template <typename T, int V>
+struct Packed {
+  uint4 q[(V * sizeof(T) + 15) / 16];  // 8 bytes: half of one
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    if constexpr (V * sizeof(T) == 8) {
+      const uint2 h = __ldg(reinterpret_cast<const uint2*>(p));
+      q[0] = make_uint4(h.x, h.y, 0u, 0u);
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[u][e] = i0 + e < a.n ? Dt<Tx>::to_f(x[i0 + e]) : 0.f;
-        if (RES) o[u][e] = i0 + e < a.n ? Dt<Tr>::to_f(res[i0 + e]) : 0.f;
-      }
+      for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     }
   }
+  __device__ __forceinline__ float2 pair(int k) const {
+    const T* e = reinterpret_cast<const T*>(q);
+    return make_float2(Dt<T>::to_f(e[2 * k]), Dt<T>::to_f(e[2 * k + 1]));
+  }
+};
+
+// CTAs walk over tiles of a few vectors of V elements a thread and load the next tile before they form this
+// one's words. A tile is an aligned power of two of elements, so the upper half of the block number is the same for
+// all of it. What is left behind the last whole tile, and tensors that do not start on vector boundaries (VEC false),
+// go element by element.
+template <typename Tx, typename Tr, typename Ty, bool RES, bool VEC>
+__global__ void __launch_bounds__(kDropThreads, kDropCtas)
+    dropout_kernel(const Tx* __restrict__ x, const Tr* __restrict__ res, Ty* __restrict__ y, const DropArgs a) {
+  pdl_wait();  // inputs are the previous kernel's outputs
+  constexpr int V = 16 / (int)sizeof(Tx), U = drop_unroll((int)sizeof(Tx), RES ? (int)sizeof(Tr) : 0);
+  constexpr int PER = kDropThreads * U * V;
+  static_assert((PER & (PER - 1)) == 0, "a power of two");
+  const uint64_t key = a.seed_dev ? (uint64_t)__ldg(a.seed_dev) : a.seed;
+  const int64_t whole = VEC ? a.n / PER : 0, tiles = (a.n + PER - 1) / PER;
+  int64_t tile = blockIdx.x;
+  Packed<Tx, V> vx[U], nx[U];
+  Packed<Tr, V> vr[U], nr[U];
+  auto load = [&](int64_t t, Packed<Tx, V>(&px)[U], Packed<Tr, V>(&pr)[U]) {
 #pragma unroll
-  for (int u = 0; u < kDropUnroll; ++u) {
-    const int64_t i0 = base + (u * kDropThreads + threadIdx.x) * V;
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      uint32_t w[4];
-      gen.block((uint32_t)(i0 >> 2) + q, w);
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {  // a dropped value is not used, whatever it is
-        const int k = q * 4 + e;
-        const float2 s = __fmul2_rn(make_float2(v[u][k], v[u][k + 1]), make_float2(a.scale, a.scale));
-        const float2 kept = make_float2(w[e] >= a.border ? s.x : 0.f, w[e + 1] >= a.border ? s.y : 0.f);
-        const float2 r = RES ? __fadd2_rn(make_float2(o[u][k], o[u][k + 1]), kept) : kept;
-        o[u][k] = r.x;
-        o[u][k + 1] = r.y;
-      }
+    for (int u = 0; u < U; ++u) {
+      const int64_t i0 = t * PER + (u * kDropThreads + threadIdx.x) * V;
+      px[u].load(x + i0);
+      if (RES) pr[u].load(res + i0);
     }
-    if (whole) {
-      store_rounded<Ty, V>(y + i0, o[u]);
-    } else {
+  };
+  if (tile < whole) load(tile, vx, vr);
+  while (tile < whole) {
+    const uint32_t hi = (uint32_t)((tile * PER) >> 34);
+    const Philox gen(hi, a.offset, key);
+    do {
+      const int64_t next = tile + gridDim.x;
+      if (next < whole) load(next, nx, nr);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (i0 + e < a.n) y[i0 + e] = Dt<Ty>::from_f(o[u][e]);
+      for (int u = 0; u < U; ++u) {
+        const int64_t i0 = tile * PER + (u * kDropThreads + threadIdx.x) * V;
+        float o[V];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          uint32_t w[4];
+          gen.block((uint32_t)(i0 >> 2) + q, w);
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {  // a dropped value is not used, whatever it is
+            const int k = q * 4 + e;
+            const float2 s = __fmul2_rn(vx[u].pair(k / 2), make_float2(a.scale, a.scale));
+            const float2 kept = make_float2(w[e] >= a.border ? s.x : 0.f, w[e + 1] >= a.border ? s.y : 0.f);
+            const float2 r = RES ? __fadd2_rn(vr[u].pair(k / 2), kept) : kept;
+            o[k] = r.x;
+            o[k + 1] = r.y;
+          }
+        }
+        store_rounded<Ty, V>(y + i0, o);
+        vx[u] = nx[u];
+        vr[u] = nr[u];
+      }
+      tile = next;
+    } while (tile < whole && (uint32_t)((tile * PER) >> 34) == hi);
+  }
+  for (; tile < tiles; tile += gridDim.x) {
+    const Philox gen((uint32_t)((tile * PER) >> 34), a.offset, key);
+#pragma unroll
+    for (int u = threadIdx.x; u < PER / 4; u += kDropThreads) {
+      const int64_t i0 = tile * PER + u * 4;
+      uint32_t w[4];
+      if (i0 < a.n) gen.block((uint32_t)(i0 >> 2), w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i0 + e < a.n) {
+          const float kept = w[e] >= a.border ? Dt<Tx>::to_f(x[i0 + e]) * a.scale : 0.f;
+          y[i0 + e] = Dt<Ty>::from_f(RES ? Dt<Tr>::to_f(res[i0 + e]) + kept : kept);
+        }
     }
   }
 }
@@ -155,9 +197,9 @@ int launch(const void* x, const void* res, void* y, const DropArgs& a, cudaStrea
   constexpr int V = 16 / (int)sizeof(Tx);
   auto fits = [](const void* p, size_t bytes) { return rk_host::aligned(p, bytes < 16 ? bytes : 16); };
   const bool vec = fits(x, 16) && fits(y, V * sizeof(Ty)) && (!RES || fits(res, V * sizeof(Tr)));
-  const int64_t per = (int64_t)kDropThreads * kDropUnroll * V;
-  const int64_t grid = (a.n + per - 1) / per;
-  if (grid >= (1ll << 31)) return RK_ERR_UNSUPPORTED;
+  const int64_t per = (int64_t)kDropThreads * drop_unroll((int)sizeof(Tx), RES ? (int)sizeof(Tr) : 0) * V;
+  const int64_t tiles = (a.n + per - 1) / per;
+  const int64_t grid = tiles < 148 * kDropCtas ? tiles : 148 * kDropCtas;
   const Tx* xp = static_cast<const Tx*>(x);
   const Tr* rp = static_cast<const Tr*>(res);
   Ty* yp = static_cast<Ty*>(y);

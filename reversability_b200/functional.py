@@ -82,6 +82,13 @@ def _on_current_device(t: torch.Tensor, name: str, *others: torch.Tensor | None)
             raise ValueError(f"all tensors must be on {name}'s device")
 
 
+def _new(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous uninitialised tensor of t's shape (the cheapest call for it: they are most of a small pass's time)."""
+    if t.dtype is dtype and t.is_contiguous():
+        return torch.empty_like(t)
+    return t.new_empty(t.shape, dtype=dtype)
+
+
 def even_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """(t or a contiguous copy of it, rows, width, row stride): rows of unit-stride elements an even distance apart
     are taken as they lie, anything else is copied."""
@@ -137,11 +144,16 @@ def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tens
     _on_current_device(x, "the input", weight, bias)
     weight, bias, pcode = _norm_params(x, weight, bias)
     xr, rows, width, ld = _norm_rows(x, 16 // x.element_size())
-    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
-    stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32) if want_stats else None
+    y = _new(x, out_dtype)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     _lib.call("rk_layernorm_fwd", xr.data_ptr(), _lib.code(x.dtype), ld, _lib.ptr(weight), _lib.ptr(bias), pcode,
               y.data_ptr(), _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, float(eps), _lib.stream_ptr())
     return y, stats
+
+
+@functools.lru_cache(maxsize=64)
+def _layernorm_workspace(rows: int, width: int) -> int:
+    return _lib.lib().rk_layernorm_bwd_workspace(rows, width)
 
 
 def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
@@ -156,11 +168,11 @@ def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Ten
     per = 16 // x.element_size()
     xr, rows, width, ldx = _norm_rows(x, per)
     dyr, _, _, lddy = _norm_rows(dy, per)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
-    dw = torch.empty(width, device=x.device, dtype=param_dtype) if want_dw else None
-    db = torch.empty(width, device=x.device, dtype=param_dtype) if want_db else None
-    n_ws = _lib.lib().rk_layernorm_bwd_workspace(rows, width) if want_dw or want_db else 0
-    ws = torch.empty(n_ws // 4, device=x.device, dtype=torch.float32) if n_ws else None
+    dx = _new(x, x.dtype) if want_dx else None
+    dw = x.new_empty(width, dtype=param_dtype) if want_dw else None
+    db = x.new_empty(width, dtype=param_dtype) if want_db else None
+    n_ws = _layernorm_workspace(rows, width) if want_dw or want_db else 0
+    ws = x.new_empty(n_ws // 4, dtype=torch.float32) if n_ws else None
     _lib.call("rk_layernorm_bwd", xr.data_ptr(), _lib.code(x.dtype), ldx, _lib.ptr(weight), _lib.code(param_dtype),
               stats.data_ptr(), dyr.data_ptr(), _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw),
               _lib.ptr(db), _lib.ptr(ws), n_ws, rows, width, _lib.stream_ptr())
@@ -191,7 +203,7 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
         raise ValueError("dropout with a residual gives the residual's type")
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
-    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    y = _new(x, out_dtype)
     _lib.call("rk_dropout", x.data_ptr(), _lib.code(x.dtype), _lib.ptr(residual), y.data_ptr(), _lib.code(out_dtype),
               x.numel(), float(p), 0 if on_device else seed & (2 ** 64 - 1), seed.data_ptr() if on_device else None,
               offset, _lib.stream_ptr())
@@ -484,14 +496,14 @@ def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
     _linear_ce_check(hidden, weight, labels, reduction)
     labels = labels.contiguous()
     V, K = weight.shape
-    loss = torch.empty(labels.shape if reduction == "none" else (), device=hidden.device, dtype=torch.float32)
+    loss = hidden.new_empty(labels.shape if reduction == "none" else (), dtype=torch.float32)
     if hidden.dtype == torch.float32:
         return _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss)
     x, M, _, ld = even_rows(hidden)
     w = _head_weight(weight)
     n_kept, n_ws, _ = _linear_ce_bytes(M, V, K)
-    kept = torch.empty(n_kept // 4, device=hidden.device, dtype=torch.int32)
-    ws = torch.empty(n_ws, device=hidden.device, dtype=torch.uint8)
+    kept = labels.new_empty(n_kept // 4, dtype=torch.int32)
+    ws = labels.new_empty(n_ws, dtype=torch.uint8)
     _lib.call("rk_linear_ce_fwd", x.data_ptr(), ld, w.data_ptr(), _ld(w), labels.data_ptr(), int(ignore_index), M, V, K,
               _lib.code(hidden.dtype), _REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n_ws,
               _lib.stream_ptr())
@@ -507,8 +519,8 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
     grad = grad.detach().float().contiguous()
     if grad.device != hidden.device or grad.numel() != (hidden.shape[:-1].numel() if reduction == "none" else 1):
         raise ValueError("the loss's gradient must be on hidden's device, one number or one a row")
-    dx = torch.empty(hidden.shape, device=hidden.device, dtype=dx_dtype or hidden.dtype) if want_dx else None
-    dw = torch.empty((V, K), device=hidden.device, dtype=dw_dtype or weight.dtype) if want_dw else None
+    dx = _new(hidden, dx_dtype or hidden.dtype) if want_dx else None
+    dw = _new(weight, dw_dtype or weight.dtype) if want_dw else None
     if hidden.dtype == torch.float32:
         return _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw)
     _on_current_device(hidden, "hidden", weight, kept)
