@@ -52,6 +52,7 @@ __host__ __device__ constexpr uint32_t ce_smem(int m) {
 
 struct CeArgs {
   const int* count;  // rows that are not ignored (device memory)
+  int in_place_rows;  // with this count the hidden states are read where they are (-1: never)
   int vocab, width;  // V, K
   int tiles_n;       // column tiles of the output
   int kb;            // k blocks of the reduction (ADD: of the piece; OUTER: given by count)
@@ -204,7 +205,8 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
 template <int MODE, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const __grid_constant__ CUtensorMap tmC, const CeArgs g, const uint32_t idesc) {
+                   const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmX, const CeArgs g,
+                   const uint32_t idesc) {
   constexpr int STAGES = ce_stages(MODE);
   constexpr bool A_MN = MODE == OUTER || MODE == OUTER_T;
   constexpr bool B_MN = MODE == ADD || A_MN;
@@ -257,6 +259,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
   int issued = 0;
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ producer (each CTA its own halves)
+    // hidden states: gathered, or themselves where every row is listed
+    const bool in_place = *g.count == g.in_place_rows;
+    const CUtensorMap* mapA = (MODE == STATS || MODE == DLOGITS) && in_place ? &tmX : &tmA;
+    const CUtensorMap* mapB = A_MN && in_place ? &tmX : &tmB;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -271,17 +277,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
         const uint32_t a = smem_u32(smem + stage * kStageBytes), b = a + kHalf * kKb * 2;
         const int k0 = kb * kKb, ra = w.m0 + rank * kHalf, rb = w.n0 + rank * kHalf;
         if constexpr (A_MN) {
-          tma_load_pair(a, &tmA, fb, ra, k0);
-          tma_load_pair(a + 8192, &tmA, fb, ra + 64, k0);
+          tma_load_pair(a, mapA, fb, ra, k0);
+          tma_load_pair(a + 8192, mapA, fb, ra + 64, k0);
         } else {
-          tma_load_pair(a, &tmA, fb, k0, ra);
+          tma_load_pair(a, mapA, fb, k0, ra);
         }
         if constexpr (B_MN) {
           const int ky = MODE == ADD ? g.v0 + k0 : k0;
-          tma_load_pair(b, &tmB, fb, rb, ky);
-          tma_load_pair(b + 8192, &tmB, fb, rb + 64, ky);
+          tma_load_pair(b, mapB, fb, rb, ky);
+          tma_load_pair(b + 8192, mapB, fb, rb + 64, ky);
         } else {
-          tma_load_pair(b, &tmB, fb, k0, g.v0 + rb);
+          tma_load_pair(b, mapB, fb, k0, g.v0 + rb);
         }
         ++issued;
         if (++stage == STAGES) {
@@ -505,7 +511,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 
 // ---------------------------------------------------------------- rows
 // One CTA lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
-// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored.
+// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. Each warp takes 1024
+// consecutive labels at a time, all loads first; a row's place is the number of those that count before it.
 __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
                                                        int64_t ignore, int* __restrict__ head, int* __restrict__ pos,
                                                        int* __restrict__ label, int* __restrict__ rows_of,
@@ -513,43 +520,43 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ int sums[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t below = (1u << lane) - 1u;
   int base = 0, turn = 0;
   bool bad = false;
-  for (int64_t r0 = 0; r0 < rows; r0 += 4096, turn ^= 1) {
-    int64_t lab[4];
-    const int64_t r = r0 + (int64_t)threadIdx.x * 4;
+  for (int64_t r0 = 0; r0 < rows; r0 += 32768, turn ^= 1) {
+    const int64_t r = r0 + warp * 1024 + lane;
+    int lab[32];
     int n = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      lab[e] = r + e < rows ? labels[r + e] : ignore;
-      if (lab[e] != ignore && (lab[e] < 0 || lab[e] >= vocab)) bad = true;
-      if (lab[e] == ignore || lab[e] < 0 || lab[e] >= vocab) lab[e] = -1;
-      n += lab[e] >= 0;
+    for (int j = 0; j < 32; ++j) {
+      const int64_t v = r + j * 32 < rows ? labels[r + j * 32] : ignore;
+      const bool counts = v != ignore && v >= 0 && v < vocab;
+      bad |= v != ignore && !counts;
+      lab[j] = counts ? (int)v : -1;
     }
-    int scan = n;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) n += __popc(__ballot_sync(0xffffffffu, lab[j] >= 0));
+    if (lane == 0) sums[turn][warp] = n;
+    __syncthreads();
+    int before = sums[turn][lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += v;
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
     }
-    if (lane == 31) sums[turn][warp] = scan;
-    __syncthreads();
-    int before = 0, all = 0;
+    const int all = __shfl_sync(0xffffffffu, before, 31);
+    int at = base + __shfl_sync(0xffffffffu, before, warp) - n;
 #pragma unroll
-    for (int w = 0; w < 32; ++w) {
-      const int s = sums[turn][w];
-      if (w < warp) before += s;
-      all += s;
-    }
-    int at = base + before + scan - n;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (r + e < rows) pos[r + e] = lab[e] >= 0 ? at : -1;
-      if (lab[e] >= 0) {
-        label[at] = (int)lab[e];
-        rows_of[at] = (int)(r + e);
-        ++at;
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t votes = __ballot_sync(0xffffffffu, lab[j] >= 0);
+      const int i = at + __popc(votes & below);
+      const int64_t row = r + j * 32;
+      if (row < rows) pos[row] = lab[j] >= 0 ? i : -1;
+      if (lab[j] >= 0) {
+        label[i] = lab[j];
+        rows_of[i] = (int)row;
       }
+      at += __popc(votes);
     }
     base += all;
   }
@@ -560,13 +567,15 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
   }
 }
 
-// Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows.
+// Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows. Nothing to do if all rows are
+// listed and the GEMMs can read them where they are.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x, int64_t ldx, int width, int64_t pitch,
                                                         const int* __restrict__ head, const int* __restrict__ rows_of,
-                                                        T* __restrict__ out) {
+                                                        T* __restrict__ out, int in_place_rows) {
   pdl_wait();  // inputs are the previous kernel's outputs
   const int count = head[0];
+  if (count == in_place_rows) return;
   const int end = (count + kTile - 1) / kTile * kTile;
   for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += gridDim.x * 8) {
     const T* src = i < count ? x + (int64_t)rows_of[i] * ldx : nullptr;
@@ -582,15 +591,17 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x,
   }
 }
 
-// A warp per row joins the partial (reference, sum) pairs: log-sum-exp, loss. The last CTA to finish adds the CTAs'
-// sums in order (64 bits). reduction: 0 a loss per row, 1 their sum, 2 their mean (0 over no rows).
+// Joins the partial (reference, sum) pairs of 32 rows a CTA: log-sum-exp, loss. Lanes are rows (the pairs of
+// neighbouring rows lie side by side), warps take every eighth pair. The last CTA to finish adds the CTAs' sums in
+// order (64 bits). reduction: 0 a loss per row, 1 their sum, 2 their mean (0 over no rows).
 __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part, int tiles_n, int segments_all,
                                                         int row_tiles, int unit_cap, const float* __restrict__ xlabel,
-                                                        const int* __restrict__ pos, int* __restrict__ head,
-                                                        float* __restrict__ lse, int64_t rows, int reduction,
-                                                        double* __restrict__ sums, float* __restrict__ loss) {
+                                                        const int* __restrict__ pos, const int* __restrict__ rows_of,
+                                                        int* __restrict__ head, float* __restrict__ lse, int64_t rows,
+                                                        int reduction, double* __restrict__ sums,
+                                                        float* __restrict__ loss) {
   pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ float row_loss[8];
+  __shared__ float2 joined[8][32];
   __shared__ double block_sum[8];
   __shared__ int is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -598,54 +609,65 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   const int tiles_m = (count + kTile - 1) / kTile;
   int segments = tiles_m == row_tiles ? segments_all : unit_cap / (tiles_m > 0 ? tiles_m : 1);
   if (segments > tiles_n) segments = tiles_n;
-  const int64_t r = (int64_t)blockIdx.x * 8 + warp;
-  float l = 0.f;
-  const int i = r < rows ? pos[r] : -1;
-  if (i >= 0) {
-    const int mt = i / kTile, local = i - mt * kTile;
-    float m = -INFINITY;
-    for (int k = lane; k < segments * 4; k += 32)
-      m = fmaxf(m, part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = 0.f;
-    for (int k = lane; k < segments * 4; k += 32) {
+  const int64_t r = (int64_t)blockIdx.x * 32 + lane;  // listed row; also a row whose loss is cleared if it is not
+  float m = -INFINITY, s = 0.f;
+  if (r < count) {
+    const int mt = (int)r / kTile, local = (int)r - mt * kTile;
+#pragma unroll 4
+    for (int k = warp; k < segments * 4; k += 8) {
       const float2 p = part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local];
+      if (p.x > m) {
+        s *= m == -INFINITY ? 1.f : exp2f(m - p.x);  // a sum without a reference is 0, or not a number
+        m = p.x;
+      }
       s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const double total = (double)m * 0.6931471805599453 + log((double)s);
-    l = (float)(total - (double)xlabel[i]);
-    if (lane == 0) lse[i] = (float)total;
   }
-  if (reduction == 0) {
-    if (lane == 0 && r < rows) loss[r] = l;
-    return;
-  }
-  if (lane == 0) row_loss[warp] = l;
+  joined[warp][lane] = make_float2(m, s);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int k = 0; k < 8; ++k) s += (double)row_loss[k];
-    sums[blockIdx.x] = s;
-    __threadfence();
-    is_last = atomicAdd(head + 1, 1) == (int)gridDim.x - 1;
-    __threadfence();
+  double l = 0.0;
+  if (warp == 0) {
+    if (r < count) {
+#pragma unroll
+      for (int k = 1; k < 8; ++k) m = fmaxf(m, joined[k][lane].x);
+      s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float2 p = joined[k][lane];
+        s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+      }
+      const double total = (double)m * 0.6931471805599453 + log((double)s);
+      const float row_loss = (float)(total - (double)xlabel[r]);
+      lse[r] = (float)total;
+      if (reduction == 0) loss[rows_of[r]] = row_loss;
+      l = (double)row_loss;
+    }
+    if (reduction == 0 && r < rows && pos[r] < 0) loss[r] = 0.f;
+  }
+  if (reduction == 0) return;
+  if (warp == 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      sums[blockIdx.x] = l;
+      __threadfence();
+      is_last = atomicAdd(head + 1, 1) == (int)gridDim.x - 1;
+      __threadfence();
+    }
   }
   __syncthreads();
   if (!is_last) return;
-  double s = 0.0;
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) s += __ldcg(sums + b);
+  double a = 0.0;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) a += __ldcg(sums + b);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) block_sum[warp] = s;
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (lane == 0) block_sum[warp] = a;
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = 0.0;
-    for (int k = 0; k < 8; ++k) s += block_sum[k];
-    if (reduction == 2) s = count ? s / count : 0.0;
-    loss[0] = (float)s;
+    a = 0.0;
+    for (int k = 0; k < 8; ++k) a += block_sum[k];
+    if (reduction == 2) a = count ? a / count : 0.0;
+    loss[0] = (float)a;
   }
 }
 
@@ -768,8 +790,12 @@ struct CePlan {
   int dx_slices, dw_slices;
 };
 
-// Shares of a wave of kPairs tiles that `tiles` slices-many times fill, as time: waves over slices.
-double wave_time(int64_t tiles, int64_t slices) { return (double)ceil_div(tiles * slices, kPairs) / (double)slices; }
+// Model of the work in microseconds, for choosing among cuts: a k block of a 256 x 256 tile takes a pair about 0.35, a
+// tile 1.5 more, a kernel 3, and fp32 slices are moved at 5 TB/s.
+double waves_us(int64_t tiles, int64_t slices, int64_t kb) {
+  return (double)ceil_div(tiles * slices, kPairs) * (0.35 * (double)ceil_div(kb, slices) + 1.5) + 3.0;
+}
+double moved_us(double bytes) { return bytes / 5e6 + 3.0; }
 
 CePlan make_plan(int64_t M, int64_t V, int64_t K) {
   CePlan p{};
@@ -795,16 +821,23 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
     }
   }
   p.unit_cap = p.tiles_m * p.segments > 8 * kPairs ? p.tiles_m * p.segments : 8 * kPairs;
-  // pieces: as few as the workspace allows, the count (and the slices of dW) with the fullest waves
+  // pieces: as few as the workspace allows or a few more, and slices of dW, by the model
   const int64_t fit = kPieceBytes / (p.Mp * 2 * kTile) > 1 ? kPieceBytes / (p.Mp * 2 * kTile) : 1;
   const int fewest = (int)ceil_div(p.tiles_v, fit);
+  const int kb_rows = (int)(p.Mp / kKb);
   best = 1e30;
   for (int n = fewest; n <= fewest + 4 && n <= p.tiles_v; ++n) {
     const int tiles = (int)ceil_div(p.tiles_v, n);
-    const int rest = p.tiles_v - (int)(ceil_div(p.tiles_v, tiles) - 1) * tiles;  // of the last piece
-    for (int s = 1; s <= 16 && (s == 1 || p.Mp / kKb / s >= 16); ++s) {
-      const double t = (ceil_div(p.tiles_v, tiles) - 1) * wave_time((int64_t)tiles * p.tiles_k, s) +
-                       wave_time((int64_t)rest * p.tiles_k, s) + 0.02 * (n + (s > 1 ? s : 0));
+    const int whole = (int)ceil_div(p.tiles_v, tiles) - 1, rest = p.tiles_v - whole * tiles;
+    for (int s = 1; s <= 16 && (s == 1 || kb_rows / s >= 16); ++s) {
+      double t = 0;
+      for (int last = 0; last < 2; ++last) {
+        const int64_t v = last ? rest : tiles;
+        t += (last ? 1 : whole) *
+             (waves_us((int64_t)p.tiles_m * v, 1, p.kb_k) + waves_us(v * p.tiles_k, s, kb_rows) +
+              (s > 1 ? moved_us((double)v * kTile * (double)K * (8.0 * s + 2.0)) : 0.0) +
+              waves_us((int64_t)p.tiles_m * p.tiles_k, 1, v * (kTile / kKb)) + (double)p.Mp * (double)K * 4.0 / 5e6);
+      }
       if (t < best) {
         best = t;
         p.piece_tiles = tiles;
@@ -813,10 +846,11 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
     }
   }
   best = 1e30;
-  const int kb_piece = p.piece_tiles * (kTile / kKb);
+  const int kb_piece = p.piece_tiles * (kTile / kKb), pieces = (int)ceil_div(p.tiles_v, p.piece_tiles);
   p.dx_slices = 1;
   for (int s = 1; s <= 16 && (s == 1 || kb_piece / s >= 16); ++s) {
-    const double t = wave_time((int64_t)p.tiles_m * p.tiles_k, s) + 0.02 * s;
+    const double t = pieces * (waves_us((int64_t)p.tiles_m * p.tiles_k, s, kb_piece) +
+                               s * (double)p.Mp * (double)K * 8.0 / 5e6) + moved_us((double)p.Mp * (double)K * 4.0 * s);
     if (t < best) {
       best = t;
       p.dx_slices = s;
@@ -853,7 +887,7 @@ int64_t fwd_space(const CePlan& p, char* base, FwdSpace* f) {
   f->x = a.take(p.Mp * p.Kp * 2);
   f->part = static_cast<float2*>(a.take((int64_t)p.unit_cap * 4 * kTile * 8));
   f->xlabel = static_cast<float*>(a.take(p.M * 4));
-  f->sums = static_cast<double*>(a.take(ceil_div(p.M, 8) * 8));
+  f->sums = static_cast<double*>(a.take(ceil_div(p.M, 32) * 8));
   return a.at;
 }
 
@@ -878,33 +912,39 @@ int64_t bwd_space(const CePlan& p, char* base, BwdSpace* b) {
 }
 
 template <int MODE, typename T>
-int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CeArgs& g, int dtype, int64_t tiles,
-           cudaStream_t s) {
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CUtensorMap& tx, const CeArgs& g,
+           int dtype, int64_t tiles, cudaStream_t s) {
   constexpr bool a_mn = MODE == OUTER || MODE == OUTER_T, b_mn = MODE == ADD || a_mn;
   static_assert(ce_smem(MODE) <= 232448, "shared memory over the per-block limit");
   auto kern = ce_gemm_kernel<MODE, T>;
   if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)ce_smem(MODE))) return e;
   const int pairs = tiles < kPairs ? (int)tiles : kPairs;
-  rk_host::launch_k(kern, 2 * pairs, kCeThreads, ce_smem(MODE), s, ta, tb, tc, g,
+  rk_host::launch_k(kern, 2 * pairs, kCeThreads, ce_smem(MODE), s, ta, tb, tc, tx, g,
                     idesc_f16(kTile, kTile, dtype == RK_BF16 ? 1 : 0, a_mn ? 1 : 0, b_mn ? 1 : 0));
   return rk_host::launch_status();
 }
 
 template <typename T>
-int gather_typed(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, cudaStream_t s) {
+int gather_typed(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, bool in_place, cudaStream_t s) {
   const bool vec = p.K % 8 == 0 && rk_host::aligned(x, 16) && (p.M <= 1 || ldx % 8 == 0);
   const int64_t blocks = ceil_div(p.Mp, 8);
   const unsigned grid = (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
   if (vec)
     rk_host::launch_k(ce_gather_kernel<T, 8>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
-                      k.rows_of, static_cast<T*>(out));
+                      k.rows_of, static_cast<T*>(out), in_place ? (int)p.M : -1);
   else
     rk_host::launch_k(ce_gather_kernel<T, 1>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
-                      k.rows_of, static_cast<T*>(out));
+                      k.rows_of, static_cast<T*>(out), in_place ? (int)p.M : -1);
   return rk_host::launch_status();
 }
-int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, int dtype, cudaStream_t s) {
-  return dtype == RK_BF16 ? gather_typed<__nv_bfloat16>(x, ldx, p, k, out, s) : gather_typed<__half>(x, ldx, p, k, out, s);
+int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, int dtype, bool in_place,
+           cudaStream_t s) {
+  return dtype == RK_BF16 ? gather_typed<__nv_bfloat16>(x, ldx, p, k, out, in_place, s)
+                          : gather_typed<__half>(x, ldx, p, k, out, in_place, s);
+}
+// Whether TMA can read the hidden states themselves.
+bool readable(const void* x, int64_t ldx, const CePlan& p) {
+  return rk_host::aligned(x, 16) && (p.M == 1 || ldx % 8 == 0);
 }
 
 template <typename T>
@@ -974,11 +1014,15 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   rk_host::launch_k(ce_list_kernel, 1, 1024, 0, s, labels, M, V, ignore_index, k.head, k.pos, k.label, k.rows_of, status);
   int st = rk_host::launch_status();
   if (st != RK_OK) return st;
-  if ((st = gather(hidden, ldh, p, k, f.x, dtype, s)) != RK_OK) return st;
-  CUtensorMap ta, tb;
+  const bool in_place = readable(hidden, ldh, p);
+  if ((st = gather(hidden, ldh, p, k, f.x, dtype, in_place, s)) != RK_OK) return st;
+  CUtensorMap ta, tb, tx;
   if (!tensor_map(&ta, f.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&tb, w, K, V, ldw, dtype, kKb, kHalf))
     return RK_ERR_LAUNCH;
+  tx = ta;
+  if (in_place && !tensor_map(&tx, hidden, K, M, M == 1 ? p.Kp : ldh, dtype, kKb, kHalf)) return RK_ERR_LAUNCH;
   CeArgs g{};
+  g.in_place_rows = in_place ? (int)M : -1;
   g.count = k.head;
   g.vocab = (int)V;
   g.width = (int)K;
@@ -992,9 +1036,9 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   g.xlabel = f.xlabel;
   g.label = k.label;
   g.status = status;
-  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, g, dtype, p.unit_cap, s)) != RK_OK) return st;
-  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 8), 256, 0, s, f.part, p.tiles_v, p.segments, p.tiles_m,
-                    p.unit_cap, f.xlabel, k.pos, k.head, k.lse, M, reduction, f.sums, loss);
+  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, p.unit_cap, s)) != RK_OK) return st;
+  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, p.tiles_v, p.segments,
+                    p.tiles_m, p.unit_cap, f.xlabel, k.pos, k.rows_of, k.head, k.lse, M, reduction, f.sums, loss);
   return rk_host::launch_status();
 }
 
@@ -1025,7 +1069,8 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   bwd_space(p, static_cast<char*>(workspace), &b);
   const CeKept k = kept_of(const_cast<int*>(static_cast<const int*>(kept)), M);
   float* scale = b.scale;
-  int st = gather(hidden, ldh, p, k, b.x, dtype, s);
+  const bool in_place = readable(hidden, ldh, p);
+  int st = gather(hidden, ldh, p, k, b.x, dtype, in_place, s);
   if (st != RK_OK) return st;
   const int64_t fblocks = ceil_div(M, 4096);
   rk_host::launch_k(ce_factor_kernel, (unsigned)(fblocks < 64 ? fblocks : 64), 1024, 0, s, k.lse, k.head, k.rows_of, grad,
@@ -1033,7 +1078,7 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   if ((st = rk_host::launch_status()) != RK_OK) return st;
   const int64_t pitch = (int64_t)p.piece_tiles * kTile;  // of dz
   const bool direct = dw && dw_direct(p, dw, lddw, dw_dtype, dtype);
-  CUtensorMap x_k, x_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out, dw_out;
+  CUtensorMap x_k, x_mn, in_k, in_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out, dw_out;
   if (!tensor_map(&x_k, b.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&x_mn, b.x, K, p.Mp, p.Kp, dtype, 64, kKb) ||
       !tensor_map(&w_k, w, K, V, ldw, dtype, kKb, kHalf) || !tensor_map(&w_mn, w, K, V, ldw, dtype, 64, kKb) ||
       !tensor_map(&dz_out, b.dz, pitch, p.Mp, pitch, dtype, 32, 32) ||
@@ -1041,10 +1086,17 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
       !tensor_map(&dz_mn, b.dz, pitch, p.Mp, pitch, dtype, 64, kKb) ||
       !tensor_map(&dx_out, b.dx, K, (int64_t)p.dx_slices * p.Mp, p.Kq, RK_F32, 32, 32))
     return RK_ERR_LAUNCH;
+  in_k = x_k;
+  in_mn = x_mn;
+  const int64_t ldi = M == 1 ? p.Kp : ldh;
+  if (in_place && (!tensor_map(&in_k, hidden, K, M, ldi, dtype, kKb, kHalf) ||
+                   !tensor_map(&in_mn, hidden, K, M, ldi, dtype, 64, kKb)))
+    return RK_ERR_LAUNCH;
   if (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dtype, 32, 32)
              : !tensor_map(&dw_out, b.dw, K, (int64_t)p.dw_slices * pitch, p.Kq, RK_F32, 32, 32))
     return RK_ERR_LAUNCH;
   CeArgs g{};
+  g.in_place_rows = in_place ? (int)M : -1;
   g.count = k.head;
   g.vocab = (int)V;
   g.width = (int)K;
@@ -1062,8 +1114,8 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
     g.kb = p.kb_k;
     g.row_tiles = p.tiles_m;
     g.slice_rows = 0;
-    st = dtype == RK_BF16 ? launch<DLOGITS, __nv_bfloat16>(x_k, w_k, dz_out, g, dtype, (int64_t)p.tiles_m * tiles, s)
-                          : launch<DLOGITS, __half>(x_k, w_k, dz_out, g, dtype, (int64_t)p.tiles_m * tiles, s);
+    st = dtype == RK_BF16 ? launch<DLOGITS, __nv_bfloat16>(x_k, w_k, dz_out, in_k, g, dtype, (int64_t)p.tiles_m * tiles, s)
+                          : launch<DLOGITS, __half>(x_k, w_k, dz_out, in_k, g, dtype, (int64_t)p.tiles_m * tiles, s);
     if (st != RK_OK) return st;
     if (dx) {
       g.tiles_n = p.tiles_k;
@@ -1071,7 +1123,7 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
       g.slices = p.dx_slices;
       g.slice_rows = (int)p.Mp;
       g.add = t0 > 0;
-      st = launch<ADD, float>(dz_k, w_mn, dx_out, g, dtype, (int64_t)p.tiles_m * p.tiles_k * p.dx_slices, s);
+      st = launch<ADD, float>(dz_k, w_mn, dx_out, dz_k, g, dtype, (int64_t)p.tiles_m * p.tiles_k * p.dx_slices, s);
       if (st != RK_OK) return st;
     }
     if (dw) {
@@ -1080,9 +1132,9 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
       g.slices = p.dw_slices;
       g.slice_rows = direct ? 0 : (int)pitch;
       const int64_t n = (int64_t)tiles * p.tiles_k * p.dw_slices;
-      if (!direct) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, g, dtype, n, s);
-      else if (dtype == RK_BF16) st = launch<OUTER_T, __nv_bfloat16>(dz_mn, x_mn, dw_out, g, dtype, n, s);
-      else st = launch<OUTER_T, __half>(dz_mn, x_mn, dw_out, g, dtype, n, s);
+      if (!direct) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
+      else if (dtype == RK_BF16) st = launch<OUTER_T, __nv_bfloat16>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
+      else st = launch<OUTER_T, __half>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       if (st != RK_OK) return st;
       if (!direct) {
         char* out = static_cast<char*>(dw) + v0 * lddw * (int64_t)rk_host::dtype_size(dw_dtype);
