@@ -57,9 +57,7 @@ struct CeArgs {
   int tiles_n;       // column tiles of the output
   int kb;            // k blocks of the reduction (ADD: of the piece; OUTER: given by count)
   int slices;        // ADD, OUTER: slices of the reduction
-  int segments;      // STATS: segments of the vocabulary when all of rows_tiles row tiles are there
-  int row_tiles;     // row tiles if no row is ignored (OUTER: vocabulary tiles of the piece)
-  int unit_cap;      // STATS: row tiles x segments at most
+  int row_tiles;     // OUTER: vocabulary tiles of the piece
   int v0;            // first vocabulary entry of the piece
   int slice_rows;    // ADD, OUTER: rows between slices in the output
   int add;           // ADD: add to what is there
@@ -70,6 +68,25 @@ struct CeArgs {
   const float* scale;  // OUTER_T
   unsigned int* status;
 };
+
+constexpr int kPairs = 74;  // CTA pairs of a B200's 148 SMs
+
+// Segments that the vocabulary's tiles are cut into when there are tiles_m row tiles: full waves of pairs, at most eight
+// of them unless there are more row tiles.
+__host__ __device__ inline int stats_segments(int tiles_m, int tiles_n) {
+  int best = 1;
+  int64_t cost = ((int64_t)tiles_m + kPairs - 1) / kPairs * tiles_n;
+  for (int k = 1; k <= 8 && tiles_m > 0; ++k) {
+    const int s = kPairs * k / tiles_m < tiles_n ? kPairs * k / tiles_m : tiles_n;
+    if (s < 1) continue;
+    const int64_t c = (int64_t)((tiles_m * s + kPairs - 1) / kPairs) * ((tiles_n + s - 1) / s);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
 
 // The tiles that a CTA pair visits, in order. STATS: units of one row tile and a run of column tiles, so that a row's
 // running values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
@@ -84,8 +101,7 @@ struct CeWalk {
     tiles_m = (MODE == OUTER || MODE == OUTER_T) ? g.row_tiles : (rows + kTile - 1) / kTile;
     segments = 1;
     if (MODE == STATS) {
-      segments = tiles_m == g.row_tiles ? g.segments : g.unit_cap / (tiles_m > 0 ? tiles_m : 1);
-      if (segments > g.tiles_n) segments = g.tiles_n;
+      segments = stats_segments(tiles_m, g.tiles_n);
       units = tiles_m * segments;
     } else {
       units = tiles_m * g.tiles_n * g.slices;
@@ -511,8 +527,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 
 // ---------------------------------------------------------------- rows
 // One CTA lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
-// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. Each warp takes 1024
-// consecutive labels at a time, all loads first; a row's place is the number of those that count before it.
+// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. The warps share the
+// rows (1024 each at most at a time), all loads first; a row's place is the number of those that count before it.
 __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
                                                        int64_t ignore, int* __restrict__ head, int* __restrict__ pos,
                                                        int* __restrict__ label, int* __restrict__ rows_of,
@@ -523,19 +539,21 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
   const uint32_t below = (1u << lane) - 1u;
   int base = 0, turn = 0;
   bool bad = false;
-  for (int64_t r0 = 0; r0 < rows; r0 += 32768, turn ^= 1) {
-    const int64_t r = r0 + warp * 1024 + lane;
+  const int each = rows >= 32768 ? 32 : (int)((rows + 1023) / 1024);  // of 32 rows
+  for (int64_t r0 = 0; r0 < rows; r0 += 1024 * each, turn ^= 1) {
+    const int64_t r = r0 + warp * 32 * each + lane;
     int lab[32];
     int n = 0;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      const int64_t v = r + j * 32 < rows ? labels[r + j * 32] : ignore;
+      const int64_t v = j < each && r + j * 32 < rows ? labels[r + j * 32] : ignore;
       const bool counts = v != ignore && v >= 0 && v < vocab;
       bad |= v != ignore && !counts;
       lab[j] = counts ? (int)v : -1;
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) n += __popc(__ballot_sync(0xffffffffu, lab[j] >= 0));
+    for (int j = 0; j < 32; ++j)
+      if (j < each) n += __popc(__ballot_sync(0xffffffffu, lab[j] >= 0));
     if (lane == 0) sums[turn][warp] = n;
     __syncthreads();
     int before = sums[turn][lane];
@@ -548,6 +566,7 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
     int at = base + __shfl_sync(0xffffffffu, before, warp) - n;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
+      if (j >= each) break;
       const uint32_t votes = __ballot_sync(0xffffffffu, lab[j] >= 0);
       const int i = at + __popc(votes & below);
       const int64_t row = r + j * 32;
@@ -594,12 +613,11 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x,
 // Joins the partial (reference, sum) pairs of 32 rows a CTA: log-sum-exp, loss. Lanes are rows (the pairs of
 // neighbouring rows lie side by side), warps take every eighth pair. The last CTA to finish adds the CTAs' sums in
 // order (64 bits). reduction: 0 a loss per row, 1 their sum, 2 their mean (0 over no rows).
-__global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part, int tiles_n, int segments_all,
-                                                        int row_tiles, int unit_cap, const float* __restrict__ xlabel,
-                                                        const int* __restrict__ pos, const int* __restrict__ rows_of,
-                                                        int* __restrict__ head, float* __restrict__ lse, int64_t rows,
-                                                        int reduction, double* __restrict__ sums,
-                                                        float* __restrict__ loss) {
+__global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part, int tiles_n,
+                                                        const float* __restrict__ xlabel, const int* __restrict__ pos,
+                                                        const int* __restrict__ rows_of, int* __restrict__ head,
+                                                        float* __restrict__ lse, int64_t rows, int reduction,
+                                                        double* __restrict__ sums, float* __restrict__ loss) {
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ float2 joined[8][32];
   __shared__ double block_sum[8];
@@ -607,29 +625,52 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int count = head[0];
   const int tiles_m = (count + kTile - 1) / kTile;
-  int segments = tiles_m == row_tiles ? segments_all : unit_cap / (tiles_m > 0 ? tiles_m : 1);
-  if (segments > tiles_n) segments = tiles_n;
+  const int pairs = stats_segments(tiles_m, tiles_n) * 4;
   const int64_t r = (int64_t)blockIdx.x * 32 + lane;  // listed row; also a row whose loss is cleared if it is not
   float m = -INFINITY, s = 0.f;
-  if (r < count) {
-    const int mt = (int)r / kTile, local = (int)r - mt * kTile;
+  // adds a pair to (m, s); a sum without a reference is 0, or not a number
+  auto join = [&](float2 p) {
+    if (p.x > m) {
+      s *= m == -INFINITY ? 1.f : exp2f(m - p.x);
+      m = p.x;
+    }
+    s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+  };
+  if (pairs <= 64) {
+    if (r < count) {
+      const int mt = (int)r / kTile, local = (int)r - mt * kTile;
 #pragma unroll 4
-    for (int k = warp; k < segments * 4; k += 8) {
-      const float2 p = part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local];
-      if (p.x > m) {
-        s *= m == -INFINITY ? 1.f : exp2f(m - p.x);  // a sum without a reference is 0, or not a number
-        m = p.x;
+      for (int k = warp; k < pairs; k += 8)
+        join(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
+    }
+    joined[warp][lane] = make_float2(m, s);
+  } else {  // few rows with many pairs each: a warp takes four rows, lanes are pairs
+    for (int e = 0; e < 4; ++e) {
+      const int64_t row = (int64_t)blockIdx.x * 32 + warp * 4 + e;
+      m = -INFINITY;
+      s = 0.f;
+      if (row < count) {
+        const int mt = (int)row / kTile, local = (int)row - mt * kTile;
+#pragma unroll 4
+        for (int k = lane; k < pairs; k += 32)
+          join(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
       }
-      s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float2 p = make_float2(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+        join(p);
+      }
+      if (lane == 0) joined[0][warp * 4 + e] = make_float2(m, s);
+      if (lane < 7) joined[1 + lane][warp * 4 + e] = make_float2(-INFINITY, 0.f);
     }
   }
-  joined[warp][lane] = make_float2(m, s);
   __syncthreads();
   double l = 0.0;
   if (warp == 0) {
     if (r < count) {
+      m = -INFINITY;
 #pragma unroll
-      for (int k = 1; k < 8; ++k) m = fmaxf(m, joined[k][lane].x);
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, joined[k][lane].x);
       s = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -778,14 +819,13 @@ bool tensor_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows,
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int kPairs = 74;  // CTA pairs of a B200's 148 SMs
 constexpr int64_t kPieceBytes = 512ll << 20;  // dz of one piece
 
 // How the work of (M rows, V, K) is cut. Pure arithmetic, the same for the workspace queries and the calls.
 struct CePlan {
   int64_t M, V, K, Mp, Kp, Kq;  // Mp: rows in whole tiles; Kp, Kq: pitch of the gathered rows and of fp32 rows
   int tiles_m, tiles_v, tiles_k, kb_k;
-  int segments, unit_cap;
+  int units;        // row tiles x segments of the forward, at most
   int piece_tiles;  // vocabulary tiles of a piece
   int dx_slices, dw_slices;
 };
@@ -809,18 +849,8 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
   p.tiles_v = (int)ceil_div(V, kTile);
   p.tiles_k = (int)ceil_div(K, kTile);
   p.kb_k = (int)ceil_div(K, kKb);
-  // segments of the vocabulary: full waves, long runs
-  double best = 1e30;
-  const int most = (int)(ceil_div(8 * kPairs, p.tiles_m) < p.tiles_v ? ceil_div(8 * kPairs, p.tiles_m) : p.tiles_v);
-  p.segments = 1;
-  for (int s = 1; s <= most; ++s) {
-    const double t = (double)(ceil_div((int64_t)p.tiles_m * s, kPairs) * ceil_div(p.tiles_v, s)) + 0.02 * s;
-    if (t < best) {
-      best = t;
-      p.segments = s;
-    }
-  }
-  p.unit_cap = p.tiles_m * p.segments > 8 * kPairs ? p.tiles_m * p.segments : 8 * kPairs;
+  p.units = p.tiles_m > 8 * kPairs ? p.tiles_m : 8 * kPairs;  // whatever the number of rows that count
+  double best;
   // pieces: as few as the workspace allows or a few more, and slices of dW, by the model
   const int64_t fit = kPieceBytes / (p.Mp * 2 * kTile) > 1 ? kPieceBytes / (p.Mp * 2 * kTile) : 1;
   const int fewest = (int)ceil_div(p.tiles_v, fit);
@@ -885,7 +915,7 @@ struct FwdSpace {
 int64_t fwd_space(const CePlan& p, char* base, FwdSpace* f) {
   Arena a{base, 0};
   f->x = a.take(p.Mp * p.Kp * 2);
-  f->part = static_cast<float2*>(a.take((int64_t)p.unit_cap * 4 * kTile * 8));
+  f->part = static_cast<float2*>(a.take((int64_t)p.units * 4 * kTile * 8));
   f->xlabel = static_cast<float*>(a.take(p.M * 4));
   f->sums = static_cast<double*>(a.take(ceil_div(p.M, 32) * 8));
   return a.at;
@@ -1029,16 +1059,13 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   g.tiles_n = p.tiles_v;
   g.kb = p.kb_k;
   g.slices = 1;
-  g.segments = p.segments;
-  g.row_tiles = p.tiles_m;
-  g.unit_cap = p.unit_cap;
   g.part = f.part;
   g.xlabel = f.xlabel;
   g.label = k.label;
   g.status = status;
-  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, p.unit_cap, s)) != RK_OK) return st;
-  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, p.tiles_v, p.segments,
-                    p.tiles_m, p.unit_cap, f.xlabel, k.pos, k.rows_of, k.head, k.lse, M, reduction, f.sums, loss);
+  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, kPairs, s)) != RK_OK) return st;
+  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, p.tiles_v, f.xlabel, k.pos,
+                    k.rows_of, k.head, k.lse, M, reduction, f.sums, loss);
   return rk_host::launch_status();
 }
 
