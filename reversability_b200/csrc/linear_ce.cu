@@ -192,8 +192,10 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+// What it orders are reads of tensor memory, which tcgen05.fence and the barrier itself do; a release at cluster scope
+// would be a full fence (the forward of 14848 x 50257 x 256 took 363 us with it).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void store_2d(const void* tmap, uint32_t src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src),
@@ -209,6 +211,12 @@ __device__ __forceinline__ void reduce_add_2d(const void* tmap, uint32_t src, in
 __device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
@@ -398,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
         if (ch == 1) {  // read: the MMA thread may reuse this accumulator
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(leader_addr(tempty0 + 8 * acc));
+          if (lane == 0) mbar_arrive_pair(leader_addr(tempty0 + 8 * acc));
         }
         const int c0 = w.n0 + cg * 64 + ch * 32;  // first column of the chunk
         float* v = reinterpret_cast<float*>(r);
@@ -420,9 +428,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
             for (int k = 0; k < 32; ++k) xl = li == k ? v[k] : xl;
             g.xlabel[w.m0 + local] = xl;
           }
-          float m = v[0];
+          float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int k = 1; k < 32; ++k) m = fmaxf(m, v[k]);
+          for (int k = 4; k < 28; k += 2) m4[(k / 2) & 3] = max3(m4[(k / 2) & 3], v[k], v[k + 1]);
+          float m = max3(max3(m4[0], m4[1], max3(m4[2], v[28], v[29])), m4[3], fmaxf(v[30], v[31]));
           m *= kLog2e;
           // the reference follows the maximum only when that is 2^8 above it: sums stay below 2^40
           if (m > run_m + 8.f) {
