@@ -43,9 +43,9 @@ constexpr int kEpiWarps = 16;
 constexpr int kCeThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kStageBytes = 2 * kHalf * kKb * 2;  // A and B of one CTA
 __host__ __device__ constexpr uint32_t ce_out_bytes(int m) {
-  return m == STATS ? 0 : (m == ADD || m == OUTER) ? kEpiWarps * 4096 : kEpiWarps * 2048;
+  return m == STATS ? 0 : kEpiWarps * 4096;  // a warp: one box of 32 x 32 fp32, or two of 16 bits
 }
-__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : (m == ADD || m == OUTER) ? 5 : 6; }
+__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : 5; }
 __host__ __device__ constexpr uint32_t ce_smem(int m) {
   return 1024 + ce_stages(m) * kStageBytes + ce_out_bytes(m) + (2 * ce_stages(m) + 6) * 8 + 16;
 }
@@ -88,8 +88,8 @@ __host__ __device__ inline int stats_segments(int tiles_m, int tiles_n) {
   return best;
 }
 
-// The tiles that a CTA pair visits, in order. STATS: units of one row tile and a run of column tiles, so that a row's
-// running values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
+// The tiles that a CTA pair visits, in order. STATS and DLOGITS: units of one row tile and a run of column tiles, so
+// that a row's values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
 template <int MODE>
 struct CeWalk {
   int unit, units, step, tiles_m, segments;
@@ -100,7 +100,7 @@ struct CeWalk {
     const int rows = *g.count;
     tiles_m = (MODE == OUTER || MODE == OUTER_T) ? g.row_tiles : (rows + kTile - 1) / kTile;
     segments = 1;
-    if (MODE == STATS) {
+    if (MODE == STATS || MODE == DLOGITS) {
       segments = stats_segments(tiles_m, g.tiles_n);
       units = tiles_m * segments;
     } else {
@@ -117,15 +117,11 @@ struct CeWalk {
     slice = 0;
     kb0 = 0;
     kb1 = kb_all;
-    if (MODE == STATS) {  // segment-major
+    if (MODE == STATS || MODE == DLOGITS) {  // segment-major
       const int seg = unit / tiles_m;
       m0 = (unit - seg * tiles_m) * kTile;
       nt = (int)((int64_t)seg * g.tiles_n / segments);
       nt_end = (int)((int64_t)(seg + 1) * g.tiles_n / segments);
-    } else if (MODE == DLOGITS) {  // row tiles fastest: they share the weight's tile
-      nt = unit / tiles_m;
-      m0 = (unit - nt * tiles_m) * kTile;
-      nt_end = nt + 1;
     } else {  // column tiles fastest: they share A's tile
       const int per = tiles_m * g.tiles_n;
       slice = unit / per;
@@ -142,7 +138,7 @@ struct CeWalk {
     last = nt + 1 == nt_end;
   }
   __device__ void next(const CeArgs& g) {
-    if (MODE == STATS && nt + 1 < nt_end) {
+    if ((MODE == STATS || MODE == DLOGITS) && nt + 1 < nt_end) {
       ++nt;
       n0 += kTile;
       first = false;
@@ -209,13 +205,30 @@ __device__ __forceinline__ void reduce_add_2d(const void* tmap, uint32_t src, in
                : "memory");
 }
 __device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
+__device__ __forceinline__ float chunk_max(const float* v) {
+  float m = v[0];
+#pragma unroll
+  for (int k = 1; k < 32; ++k) m = fmaxf(m, v[k]);
+  return m;
+}
+// Sum of exp(v) relative to 2^ref.
+__device__ __forceinline__ float chunk_sum(const float* v, float ref) {
+  const float2 l2 = make_float2(kLog2e, kLog2e);
+  const float r = ref == -INFINITY ? 0.f : -ref;
+  const float2 r2 = make_float2(r, r);
+  float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float2 t = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), l2, r2);
+    s[k & 1] = __fadd2_rn(s[k & 1], make_float2(ex2_approx(t.x), ex2_approx(t.y)));
+  }
+  return (s[0].x + s[1].x) + (s[0].y + s[1].y);
 }
 
 template <typename T>
@@ -381,33 +394,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     const int rows = MODE == STATS || MODE == DLOGITS ? *g.count : 0;
     float run_m = -INFINITY, run_s = 0.f;  // STATS: reference and sum of exp(z - reference), z in units of log 2
     int label = -1;
+    float2 rc = make_float2(0.f, 0.f);
     const float scale = MODE == OUTER_T ? *g.scale : 1.f;
     for (CeWalk<MODE> w(g, pair, pairs); w.more(); w.next(g)) {
-      float2 rc = make_float2(0.f, 0.f);
-      if (MODE == STATS || MODE == DLOGITS) {
+      if ((MODE == STATS || MODE == DLOGITS) && w.first) {
         const int row = w.m0 + local;
-        if (MODE == STATS && w.first) {
-          run_m = -INFINITY;
-          run_s = 0.f;
-        }
-        if (w.first) label = row < rows ? __ldg(g.label + row) : -1;
-        if (MODE == DLOGITS && row < rows) rc = __ldg(g.rowc + row);
+        run_m = -INFINITY;
+        run_s = 0.f;
+        label = row < rows ? __ldg(g.label + row) : -1;
+        if (MODE == DLOGITS) rc = row < rows ? __ldg(g.rowc + row) : make_float2(0.f, 0.f);
       }
       bool ok = mbar_wait(tfull0 + 8 * acc, acc_phase, g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTile + cg * 64;
-#pragma unroll 1
+      uint32_t both[2][32];
+      tmem_ld_32cols_nowait(t_row, both[0]);
+      tmem_ld_32cols_nowait(t_row + 32, both[1]);
+      tmem_ld_wait();
+      tc_fence_before();  // read: the MMA thread may reuse this accumulator
+      __syncwarp();
+      if (lane == 0) mbar_arrive_pair(leader_addr(tempty0 + 8 * acc));
+#pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
-        uint32_t r[32];
-        tmem_ld_32cols_nowait(t_row + ch * 32, r);
-        tmem_ld_wait();
-        if (ch == 1) {  // read: the MMA thread may reuse this accumulator
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_pair(leader_addr(tempty0 + 8 * acc));
-        }
+        uint32_t(&r)[32] = both[ch];
         const int c0 = w.n0 + cg * 64 + ch * 32;  // first column of the chunk
         float* v = reinterpret_cast<float*>(r);
         if ((MODE == ADD || A_MN) && w.kb0 >= w.kb1) {  // an empty slice: nothing was accumulated
@@ -428,25 +439,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
             for (int k = 0; k < 32; ++k) xl = li == k ? v[k] : xl;
             g.xlabel[w.m0 + local] = xl;
           }
-          float m4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-          for (int k = 4; k < 28; k += 2) m4[(k / 2) & 3] = max3(m4[(k / 2) & 3], v[k], v[k + 1]);
-          float m = max3(max3(m4[0], m4[1], max3(m4[2], v[28], v[29])), m4[3], fmaxf(v[30], v[31]));
-          m *= kLog2e;
-          // the reference follows the maximum only when that is 2^8 above it: sums stay below 2^40
-          if (m > run_m + 8.f) {
-            run_s *= run_m == -INFINITY ? 0.f : ex2_approx(run_m - m);
+          // Sums are formed against a reference that some earlier logit of the row set, without looking at these first:
+          // fp32 holds terms of up to 2^64, and only a sum beyond that takes a new reference (the largest logit so far).
+          if (run_m == -INFINITY) run_m = chunk_max(v) * kLog2e;
+          float part = chunk_sum(v, run_m);
+          if (part > 0x1p64f) {
+            const float m = chunk_max(v) * kLog2e;
+            run_s *= ex2_approx(run_m - m);
             run_m = m;
+            part = chunk_sum(v, m);
           }
-          const float ref = run_m == -INFINITY ? 0.f : -run_m;
-          const float2 l2 = make_float2(kLog2e, kLog2e), ref2 = make_float2(ref, ref);
-          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float2 t = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), l2, ref2);
-            s2[k & 1] = __fadd2_rn(s2[k & 1], make_float2(ex2_approx(t.x), ex2_approx(t.y)));
-          }
-          run_s += (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
+          run_s += part;
         } else if constexpr (MODE == DLOGITS) {
           const float2 l2 = make_float2(kLog2e, kLog2e), ref2 = make_float2(rc.x, rc.x);
 #pragma unroll
@@ -472,19 +475,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
           for (int k = 0; k < 32; ++k) v[k] *= scale;
         }
         if constexpr (MODE != STATS) {
-          if (lane == 0) stores_read();  // the warp's box is free
+          constexpr bool wide = MODE == ADD || MODE == OUTER;
+          if (lane == 0) {  // a box of the warp is free: all stores have read theirs, or all but the last
+            if (wide) stores_read<0>();
+            else stores_read<1>();
+          }
           __syncwarp();
+          uint8_t* box = wide ? buf : buf + ch * 2048;
           const int y = w.slice * g.slice_rows + w.m0 + rank * kHalf + quarter * 32;
-          if constexpr (MODE == ADD || MODE == OUTER) {  // 32 rows of 128 bytes, 128-byte swizzle
+          if constexpr (wide) {  // 32 rows of 128 bytes, 128-byte swizzle
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+              *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) =
                   make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && c0 < g.width) {
-              if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(buf), c0, y);
-              else store_2d(&tmC, smem_u32(buf), c0, y);
+              if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(box), c0, y);
+              else store_2d(&tmC, smem_u32(box), c0, y);
               stores_commit();
             }
           } else {  // 32 rows of 64 bytes, 64-byte swizzle
@@ -493,13 +501,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
             for (int k = 0; k < 16; ++k) p[k] = pack_pair<T>(v[2 * k], v[2 * k + 1]);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+              *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
                   make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
             fence_proxy_async_smem();
             __syncwarp();
             const int yy = MODE == OUTER_T ? g.v0 + y : y;
             if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && yy < g.vocab))) {
-              store_2d(&tmC, smem_u32(buf), c0, yy);
+              store_2d(&tmC, smem_u32(box), c0, yy);
               stores_commit();
             }
           }
