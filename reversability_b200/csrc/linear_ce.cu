@@ -43,9 +43,10 @@ constexpr int kEpiWarps = 16;
 constexpr int kCeThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kStageBytes = 2 * kHalf * kKb * 2;  // A and B of one CTA
 __host__ __device__ constexpr uint32_t ce_out_bytes(int m) {
-  return m == STATS ? 0 : kEpiWarps * 4096;  // a warp: one box of 32 x 32 fp32, or two of 16 bits
+  return m == STATS ? 0 : (m == ADD || m == OUTER) ? kEpiWarps * 4096 : kEpiWarps * 2048;  // a box of 32 rows of 128 bytes a warp
 }
-__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : 5; }
+// As many as fit. (Boxes of both chunks, 128 bytes a row, with five stages: dz of 14848 x 50257 x 256 404 us for 393.)
+__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : (m == ADD || m == OUTER) ? 5 : 6; }
 __host__ __device__ constexpr uint32_t ce_smem(int m) {
   return 1024 + ce_stages(m) * kStageBytes + ce_out_bytes(m) + (2 * ce_stages(m) + 6) * 8 + 16;
 }
@@ -88,8 +89,9 @@ __host__ __device__ inline int stats_segments(int tiles_m, int tiles_n) {
   return best;
 }
 
-// The tiles that a CTA pair visits, in order. STATS and DLOGITS: units of one row tile and a run of column tiles, so
-// that a row's values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
+// The tiles that a CTA pair visits, in order. STATS: units of one row tile and a run of column tiles, so that a row's
+// running values stay in registers; units of the same segment run side by side and share the weight's tiles in L2.
+// DLOGITS: equal shares of the tiles, column tiles fastest (a piece of the weight stays in L2).
 template <int MODE>
 struct CeWalk {
   int unit, units, step, tiles_m, segments;
@@ -100,7 +102,7 @@ struct CeWalk {
     const int rows = *g.count;
     tiles_m = (MODE == OUTER || MODE == OUTER_T) ? g.row_tiles : (rows + kTile - 1) / kTile;
     segments = 1;
-    if (MODE == STATS || MODE == DLOGITS) {
+    if (MODE == STATS) {
       segments = stats_segments(tiles_m, g.tiles_n);
       units = tiles_m * segments;
     } else {
@@ -108,6 +110,12 @@ struct CeWalk {
     }
     unit = pair;
     step = pairs;
+    if (MODE == DLOGITS) {
+      const int64_t all = units;
+      unit = (int)(all * pair / pairs);
+      units = (int)(all * (pair + 1) / pairs);
+      step = 1;
+    }
     kb_all = (MODE == OUTER || MODE == OUTER_T) ? (rows + kKb - 1) / kKb : g.kb;
     if (unit < units) begin(g);
   }
@@ -117,11 +125,17 @@ struct CeWalk {
     slice = 0;
     kb0 = 0;
     kb1 = kb_all;
-    if (MODE == STATS || MODE == DLOGITS) {  // segment-major
+    first = true;
+    if (MODE == STATS) {  // segment-major
       const int seg = unit / tiles_m;
       m0 = (unit - seg * tiles_m) * kTile;
       nt = (int)((int64_t)seg * g.tiles_n / segments);
       nt_end = (int)((int64_t)(seg + 1) * g.tiles_n / segments);
+    } else if (MODE == DLOGITS) {
+      const int mt = unit / g.tiles_n;
+      m0 = mt * kTile;
+      nt = unit - mt * g.tiles_n;
+      nt_end = nt + 1;
     } else {  // column tiles fastest: they share A's tile
       const int per = tiles_m * g.tiles_n;
       slice = unit / per;
@@ -134,19 +148,20 @@ struct CeWalk {
       kb1 = (int)((int64_t)(slice + 1) * kb_all / g.slices);
     }
     n0 = nt * kTile;
-    first = true;
     last = nt + 1 == nt_end;
   }
   __device__ void next(const CeArgs& g) {
-    if ((MODE == STATS || MODE == DLOGITS) && nt + 1 < nt_end) {
+    if (MODE == STATS && nt + 1 < nt_end) {
       ++nt;
       n0 += kTile;
       first = false;
       last = nt + 1 == nt_end;
       return;
     }
+    const int row = m0;
     unit += step;
     if (unit < units) begin(g);
+    if (MODE == DLOGITS) first = m0 != row;
   }
 };
 
@@ -205,10 +220,7 @@ __device__ __forceinline__ void reduce_add_2d(const void* tmap, uint32_t src, in
                : "memory");
 }
 __device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void stores_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 __device__ __forceinline__ float chunk_max(const float* v) {
@@ -476,40 +488,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
         }
         if constexpr (MODE != STATS) {
           constexpr bool wide = MODE == ADD || MODE == OUTER;
-          if (lane == 0) {  // a box of the warp is free: all stores have read theirs, or all but the last
-            if (wide) stores_read<0>();
-            else stores_read<1>();
-          }
+          if (lane == 0) stores_read();  // the warp's box is free
           __syncwarp();
-          uint8_t* box = wide ? buf : buf + ch * 2048;
           const int y = w.slice * g.slice_rows + w.m0 + rank * kHalf + quarter * 32;
           if constexpr (wide) {  // 32 rows of 128 bytes, 128-byte swizzle
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+              *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) * 16)) =
                   make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && c0 < g.width) {
-              if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(box), c0, y);
-              else store_2d(&tmC, smem_u32(box), c0, y);
-              stores_commit();
-            }
           } else {  // 32 rows of 64 bytes, 64-byte swizzle
-            uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) p[k] = pack_pair<T>(v[2 * k], v[2 * k + 1]);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
-                  make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            const int yy = MODE == OUTER_T ? g.v0 + y : y;
-            if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && yy < g.vocab))) {
-              store_2d(&tmC, smem_u32(box), c0, yy);
-              stores_commit();
-            }
+              *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+                  make_uint4(pack_pair<T>(v[8 * j], v[8 * j + 1]), pack_pair<T>(v[8 * j + 2], v[8 * j + 3]),
+                             pack_pair<T>(v[8 * j + 4], v[8 * j + 5]), pack_pair<T>(v[8 * j + 6], v[8 * j + 7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          const int yy = MODE == OUTER_T ? g.v0 + y : y;
+          if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && (MODE != OUTER_T || yy < g.vocab)))) {
+            if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(buf), c0, yy);
+            else store_2d(&tmC, smem_u32(buf), c0, yy);
+            stores_commit();
           }
         }
       }
@@ -543,22 +543,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 }
 
 // ---------------------------------------------------------------- rows
-// One CTA lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
-// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. The warps share the
-// rows (1024 each at most at a time), all loads first; a row's place is the number of those that count before it.
-__global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab,
-                                                       int64_t ignore, int* __restrict__ head, int* __restrict__ pos,
-                                                       int* __restrict__ label, int* __restrict__ rows_of,
-                                                       unsigned int* status) {
+// A cluster lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
+// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. The warps share the rows
+// (1024 each at most at a time), all loads first; a row's place is the number of those that count before it, its CTA's
+// share of that read from the other CTAs' shared memory.
+constexpr int kListCtas = 8;
+__global__ void __cluster_dims__(kListCtas, 1, 1) __launch_bounds__(1024)
+    ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab, int64_t ignore, int* __restrict__ head,
+                   int* __restrict__ pos, int* __restrict__ label, int* __restrict__ rows_of, unsigned int* status) {
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ int sums[2][32];
+  __shared__ int total[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = (int)cluster_rank();
   const uint32_t below = (1u << lane) - 1u;
   int base = 0, turn = 0;
   bool bad = false;
-  const int each = rows >= 32768 ? 32 : (int)((rows + 1023) / 1024);  // of 32 rows
-  for (int64_t r0 = 0; r0 < rows; r0 += 1024 * each, turn ^= 1) {
-    const int64_t r = r0 + warp * 32 * each + lane;
+  const int64_t share = (rows + 1024 * kListCtas - 1) / (1024 * kListCtas);
+  const int each = share >= 32 ? 32 : (int)share;  // a warp's rows at a time, in units of 32
+  for (int64_t r0 = 0; r0 < rows; r0 += (int64_t)1024 * kListCtas * each, turn ^= 1) {
+    const int64_t r = r0 + (int64_t)(rank * 32 + warp) * 32 * each + lane;
     int lab[32];
     int n = 0;
 #pragma unroll
@@ -579,8 +583,22 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
       const int v = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += v;
     }
-    const int all = __shfl_sync(0xffffffffu, before, 31);
-    int at = base + __shfl_sync(0xffffffffu, before, warp) - n;
+    if (threadIdx.x == 31) total[turn] = before;
+    int at = __shfl_sync(0xffffffffu, before, warp) - n;
+    cluster_sync();
+    int all = 0, ahead = 0;
+#pragma unroll
+    for (int c = 0; c < kListCtas; ++c) {
+      int v;
+      asm volatile(
+          "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+          : "=r"(v)
+          : "r"(smem_u32(&total[turn])), "r"(c)
+          : "memory");
+      all += v;
+      if (c < rank) ahead += v;
+    }
+    at += base + ahead;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       if (j >= each) break;
@@ -597,10 +615,11 @@ __global__ void __launch_bounds__(1024) ce_list_kernel(const int64_t* __restrict
     base += all;
   }
   if (bad) flag_error(status, RK_DEV_CE_LABEL);
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && rank == 0) {
     head[0] = base;
     head[1] = 0;  // CTAs of the finish kernel that are done
   }
+  cluster_sync();  // the others may still read this CTA's total
 }
 
 // Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows. Nothing to do if all rows are
@@ -815,7 +834,7 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_fn() {
   return fn;
 }
 
-// [rows, inner] with row pitch ld (elements), boxes of box_inner x box_rows.
+// [rows, inner] with row pitch ld (elements), boxes of box_inner (64 or 128 bytes) x box_rows.
 bool tensor_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, int dtype, uint32_t box_inner,
                 uint32_t box_rows) {
   auto fn = tensor_map_fn();
@@ -829,8 +848,7 @@ bool tensor_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows,
                                  : dtype == RK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            box_inner * esz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            box_inner * esz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -1058,7 +1076,7 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   fwd_space(p, static_cast<char*>(workspace), &f);
   const CeKept k = kept_of(static_cast<int*>(kept), M);
   unsigned int* status = rk_host::device_status_ptr();
-  rk_host::launch_k(ce_list_kernel, 1, 1024, 0, s, labels, M, V, ignore_index, k.head, k.pos, k.label, k.rows_of, status);
+  rk_host::launch_k(ce_list_kernel, kListCtas, 1024, 0, s, labels, M, V, ignore_index, k.head, k.pos, k.label, k.rows_of, status);
   int st = rk_host::launch_status();
   if (st != RK_OK) return st;
   const bool in_place = readable(hidden, ldh, p);
