@@ -72,21 +72,23 @@ struct CeArgs {
 
 constexpr int kPairs = 74;  // CTA pairs of a B200's 148 SMs
 
-// Segments that the vocabulary's tiles are cut into when there are tiles_m row tiles: full waves of pairs, at most eight
-// of them unless there are more row tiles.
-__host__ __device__ inline int stats_segments(int tiles_m, int tiles_n) {
-  int best = 1;
-  int64_t cost = ((int64_t)tiles_m + kPairs - 1) / kPairs * tiles_n;
-  for (int k = 1; k <= 8 && tiles_m > 0; ++k) {
-    const int s = kPairs * k / tiles_m < tiles_n ? kPairs * k / tiles_m : tiles_n;
-    if (s < 1) continue;
-    const int64_t c = (int64_t)((tiles_m * s + kPairs - 1) / kPairs) * ((tiles_n + s - 1) / s);
-    if (c < cost) {
+// Segments that the vocabulary's tiles are cut into when there are tiles_m row tiles, so that waves of pairs are full: at
+// most eight waves unless there are more row tiles. Called by a warp: a lane a number of waves.
+__device__ __forceinline__ int stats_segments(uint32_t tiles_m, uint32_t tiles_n) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t seg = 1;
+  if (lane > 0 && lane <= 8 && tiles_m > 0 && kPairs * lane >= tiles_m) seg = min(kPairs * lane / tiles_m, tiles_n);
+  float cost = (float)((tiles_m * seg + kPairs - 1) / kPairs) * (float)((tiles_n + seg - 1) / seg);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float c = __shfl_xor_sync(0xffffffffu, cost, o);
+    const uint32_t k = __shfl_xor_sync(0xffffffffu, seg, o);
+    if (c < cost || (c == cost && k < seg)) {
       cost = c;
-      best = s;
+      seg = k;
     }
   }
-  return best;
+  return (int)seg;
 }
 
 // The tiles that a CTA pair visits, in order. STATS: units of one row tile and a run of column tiles, so that a row's
@@ -103,7 +105,7 @@ struct CeWalk {
     tiles_m = (MODE == OUTER || MODE == OUTER_T) ? g.row_tiles : (rows + kTile - 1) / kTile;
     segments = 1;
     if (MODE == STATS) {
-      segments = stats_segments(tiles_m, g.tiles_n);
+      segments = g.count[2];
       units = tiles_m * segments;
     } else {
       units = tiles_m * g.tiles_n * g.slices;
@@ -543,83 +545,85 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 }
 
 // ---------------------------------------------------------------- rows
-// A cluster lists the rows whose label counts: pos[r] = place in the list or -1, label[i] and rows_of[i] of listed row i.
-// Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored. The warps share the rows
-// (1024 each at most at a time), all loads first; a row's place is the number of those that count before it, its CTA's
-// share of that read from the other CTAs' shared memory.
-constexpr int kListCtas = 8;
-__global__ void __cluster_dims__(kListCtas, 1, 1) __launch_bounds__(1024)
+// Lets the next kernel's prologue start now: it still waits for this one's end before it reads anything.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// CTAS CTAs (one, or a cluster) list the rows whose label counts: pos[r] = place in the list or -1, label[i] and
+// rows_of[i] of listed row i. Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored.
+// Each warp has its share of the rows and reads it twice, to count and to write; a row's place is the number of those
+// that count before it, the other CTAs' part of that read from their shared memory.
+template <int CTAS>
+__global__ void __launch_bounds__(1024)
     ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab, int64_t ignore, int* __restrict__ head,
                    int* __restrict__ pos, int* __restrict__ label, int* __restrict__ rows_of, unsigned int* status) {
+  pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
-  __shared__ int sums[2][32];
-  __shared__ int total[2];
+  __shared__ int sums[32];
+  __shared__ int total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = (int)cluster_rank();
-  const uint32_t below = (1u << lane) - 1u;
-  int base = 0, turn = 0;
+  const int rank = CTAS > 1 ? (int)cluster_rank() : 0;
+  const int64_t each = (rows + 1024 * CTAS - 1) / (1024 * CTAS) * 32;  // a warp's rows
+  const int64_t from = (rank * 32 + warp) * each, to = from + each < rows ? from + each : rows;
   bool bad = false;
-  const int64_t share = (rows + 1024 * kListCtas - 1) / (1024 * kListCtas);
-  const int each = share >= 32 ? 32 : (int)share;  // a warp's rows at a time, in units of 32
-  for (int64_t r0 = 0; r0 < rows; r0 += (int64_t)1024 * kListCtas * each, turn ^= 1) {
-    const int64_t r = r0 + (int64_t)(rank * 32 + warp) * 32 * each + lane;
-    int lab[32];
-    int n = 0;
+  int n = 0;
+#pragma unroll 4
+  for (int64_t r = from + lane; r < to; r += 32) {
+    const int64_t v = __ldg(labels + r);
+    const bool counts = v != ignore && v >= 0 && v < vocab;
+    bad |= v != ignore && !counts;
+    n += counts;
+  }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int64_t v = j < each && r + j * 32 < rows ? labels[r + j * 32] : ignore;
-      const bool counts = v != ignore && v >= 0 && v < vocab;
-      bad |= v != ignore && !counts;
-      lab[j] = counts ? (int)v : -1;
-    }
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if (lane == 0) sums[warp] = n;
+  __syncthreads();
+  int before = sums[lane];
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < each) n += __popc(__ballot_sync(0xffffffffu, lab[j] >= 0));
-    if (lane == 0) sums[turn][warp] = n;
-    __syncthreads();
-    int before = sums[turn][lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += v;
-    }
-    if (threadIdx.x == 31) total[turn] = before;
-    int at = __shfl_sync(0xffffffffu, before, warp) - n;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  int all = __shfl_sync(0xffffffffu, before, 31);
+  int at = __shfl_sync(0xffffffffu, before, warp) - n;
+  if constexpr (CTAS > 1) {
+    if (threadIdx.x == 0) total = all;
     cluster_sync();
-    int all = 0, ahead = 0;
+    all = 0;
 #pragma unroll
-    for (int c = 0; c < kListCtas; ++c) {
+    for (int c = 0; c < CTAS; ++c) {
       int v;
       asm volatile(
           "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
           : "=r"(v)
-          : "r"(smem_u32(&total[turn])), "r"(c)
+          : "r"(smem_u32(&total)), "r"(c)
           : "memory");
       all += v;
-      if (c < rank) ahead += v;
+      if (c < rank) at += v;
     }
-    at += base + ahead;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (j >= each) break;
-      const uint32_t votes = __ballot_sync(0xffffffffu, lab[j] >= 0);
-      const int i = at + __popc(votes & below);
-      const int64_t row = r + j * 32;
-      if (row < rows) pos[row] = lab[j] >= 0 ? i : -1;
-      if (lab[j] >= 0) {
-        label[i] = lab[j];
-        rows_of[i] = (int)row;
-      }
-      at += __popc(votes);
+  }
+#pragma unroll 4
+  for (int64_t r = from; r < to; r += 32) {
+    const int64_t v = r + lane < to ? __ldg(labels + r + lane) : ignore;
+    const bool counts = v != ignore && v >= 0 && v < vocab;
+    const uint32_t votes = __ballot_sync(0xffffffffu, counts);
+    const int i = at + __popc(votes & ((1u << lane) - 1u));
+    if (r + lane < to) pos[r + lane] = counts ? i : -1;
+    if (counts) {
+      label[i] = (int)v;
+      rows_of[i] = (int)(r + lane);
     }
-    base += all;
+    at += __popc(votes);
   }
   if (bad) flag_error(status, RK_DEV_CE_LABEL);
-  if (threadIdx.x == 0 && rank == 0) {
-    head[0] = base;
-    head[1] = 0;  // CTAs of the finish kernel that are done
+  if (warp == 0 && rank == 0) {
+    const int segments = stats_segments((all + kTile - 1) / kTile, (uint32_t)((vocab + kTile - 1) / kTile));
+    if (lane == 0) {
+      head[0] = all;
+      head[1] = 0;  // CTAs of the finish kernel that are done
+      head[2] = segments;
+    }
   }
-  cluster_sync();  // the others may still read this CTA's total
+  if constexpr (CTAS > 1) cluster_sync();  // the others may still read this CTA's total
 }
 
 // Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows. Nothing to do if all rows are
@@ -628,6 +632,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x, int64_t ldx, int width, int64_t pitch,
                                                         const int* __restrict__ head, const int* __restrict__ rows_of,
                                                         T* __restrict__ out, int in_place_rows) {
+  pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
   const int count = head[0];
   if (count == in_place_rows) return;
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x,
 // Joins the partial (reference, sum) pairs of 32 rows a CTA: log-sum-exp, loss. Lanes are rows (the pairs of
 // neighbouring rows lie side by side), warps take every eighth pair. The last CTA to finish adds the CTAs' sums in
 // order (64 bits). reduction: 0 a loss per row, 1 their sum, 2 their mean (0 over no rows).
-__global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part, int tiles_n,
+__global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict__ part,
                                                         const float* __restrict__ xlabel, const int* __restrict__ pos,
                                                         const int* __restrict__ rows_of, int* __restrict__ head,
                                                         float* __restrict__ lse, int64_t rows, int reduction,
@@ -661,16 +666,16 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int count = head[0];
   const int tiles_m = (count + kTile - 1) / kTile;
-  const int pairs = stats_segments(tiles_m, tiles_n) * 4;
+  const int pairs = head[2] * 4;
   const int64_t r = (int64_t)blockIdx.x * 32 + lane;  // listed row; also a row whose loss is cleared if it is not
   float m = -INFINITY, s = 0.f;
   // adds a pair to (m, s); a sum without a reference is 0, or not a number
   auto join = [&](float2 p) {
     if (p.x > m) {
-      s *= m == -INFINITY ? 1.f : exp2f(m - p.x);
+      s *= m == -INFINITY ? 1.f : ex2_approx(m - p.x);
       m = p.x;
     }
-    s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+    s += p.x == -INFINITY ? p.y : p.y * ex2_approx(p.x - m);
   };
   if (pairs <= 64) {
     if (r < count) {
@@ -711,9 +716,9 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float2 p = joined[k][lane];
-        s += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
+        s += p.x == -INFINITY ? p.y : p.y * ex2_approx(p.x - m);
       }
-      const double total = (double)m * 0.6931471805599453 + log((double)s);
+      const double total = (double)m * 0.6931471805599453 + (double)logf(s);
       const float row_loss = (float)(total - (double)xlabel[r]);
       lse[r] = (float)total;
       if (reduction == 0) loss[rows_of[r]] = row_loss;
@@ -725,13 +730,15 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   if (warp == 0) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) {
+    if (lane == 0 && gridDim.x == 1) loss[0] = (float)(reduction == 2 && count ? l / count : l);
+    if (lane == 0 && gridDim.x > 1) {
       sums[blockIdx.x] = l;
       __threadfence();
       is_last = atomicAdd(head + 1, 1) == (int)gridDim.x - 1;
       __threadfence();
     }
   }
+  if (gridDim.x == 1) return;
   __syncthreads();
   if (!is_last) return;
   double a = 0.0;
@@ -756,6 +763,7 @@ __global__ void __launch_bounds__(1024) ce_factor_kernel(const float* __restrict
                                                          const int* __restrict__ rows_of, const float* __restrict__ grad,
                                                          int reduction, float boost, float2* __restrict__ rowc,
                                                          float* __restrict__ scale) {
+  pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ float top[32];
   const int count = head[0];
@@ -924,7 +932,7 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
   return p;
 }
 
-// Kept from forward to backward (4-byte words): [count, done, -, -], pos [M], rows_of [M], lse [M], label [M].
+// Kept from forward to backward (4-byte words): [count, done, segments, -], pos [M], rows_of [M], lse [M], label [M].
 struct CeKept {
   int *head, *pos, *rows_of, *label;
   float* lse;
@@ -1007,6 +1015,28 @@ int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* o
   return dtype == RK_BF16 ? gather_typed<__nv_bfloat16>(x, ldx, p, k, out, in_place, s)
                           : gather_typed<__half>(x, ldx, p, k, out, in_place, s);
 }
+// One CTA for up to 4096 rows (its launch is the cheaper one), a cluster of eight for more.
+int list_rows(const int64_t* labels, int64_t ignore, const CePlan& p, const CeKept& k, unsigned int* status,
+              cudaStream_t s) {
+  if (p.M <= 4096) {
+    rk_host::launch_k(ce_list_kernel<1>, 1, 1024, 0, s, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status);
+    return rk_host::launch_status();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = 8;
+  cfg.blockDim = 1024;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = rk_host::pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 8;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, ce_list_kernel<8>, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status);
+  return rk_host::launch_status();
+}
 // Whether TMA can read the hidden states themselves.
 bool readable(const void* x, int64_t ldx, const CePlan& p) {
   return rk_host::aligned(x, 16) && (p.M == 1 || ldx % 8 == 0);
@@ -1076,8 +1106,7 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   fwd_space(p, static_cast<char*>(workspace), &f);
   const CeKept k = kept_of(static_cast<int*>(kept), M);
   unsigned int* status = rk_host::device_status_ptr();
-  rk_host::launch_k(ce_list_kernel, kListCtas, 1024, 0, s, labels, M, V, ignore_index, k.head, k.pos, k.label, k.rows_of, status);
-  int st = rk_host::launch_status();
+  int st = list_rows(labels, ignore_index, p, k, status, s);
   if (st != RK_OK) return st;
   const bool in_place = readable(hidden, ldh, p);
   if ((st = gather(hidden, ldh, p, k, f.x, dtype, in_place, s)) != RK_OK) return st;
@@ -1099,7 +1128,7 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   g.label = k.label;
   g.status = status;
   if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, kPairs, s)) != RK_OK) return st;
-  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, p.tiles_v, f.xlabel, k.pos,
+  rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, f.xlabel, k.pos,
                     k.rows_of, k.head, k.lse, M, reduction, f.sums, loss);
   return rk_host::launch_status();
 }
