@@ -348,19 +348,20 @@ RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, c
  * Replaces the head Linear and F.cross_entropy together (model.py:104,
  * train_baseline.py:262) where the logits must not be kept: z = hidden W^T,
  * loss_r = ln sum_j exp z_rj - z_r,label, with dz = (softmax z - onehot) g_r,
- * dx = dz W, dW = dz^T hidden. hidden [M, K] (row stride ldh, any alignment)
- * and w [V, K] (16-byte aligned, ldw a multiple of 8) in bf16 or f16, labels
- * int64 [M]. A row whose label is ignore_index is not read, loses 0 and gets a
+ * dx = dz W, dW = dz^T hidden. hidden [M, K] and w [V, K] (row strides ldh and
+ * ldw, any alignment) in bf16 or f16, labels int64 [M]. A row whose label is ignore_index is not read, loses 0 and gets a
  * zero gradient; a label outside [0, V) sets RK_DEV_CE_LABEL and counts as
  * ignored. reduction 0: loss[M] per row; 1: their sum, loss[1]; 2: their mean
  * over the rows that count (0 if none does).
  * kept (rk_linear_ce_kept(M) bytes, 16-byte aligned) carries the listed rows
  * and their log-sum-exps to the backward, which does not write it. Workspaces
  * are 256-byte aligned; the backward's holds dz of one piece of the vocabulary
- * (up to 512 MB, one 256-column tile at least). */
+ * (up to 512 MB, one 256-column tile at least). copy_w: whether w is copied
+ * into the workspace, which it is unless it is 16-byte aligned with ldw a
+ * multiple of 8. */
 RK_API int64_t rk_linear_ce_kept(int64_t M);
-RK_API int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K);
-RK_API int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K);
+RK_API int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w);
+RK_API int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w);
 RK_API int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
                             int64_t ignore_index, int64_t M, int64_t V, int64_t K, int dtype, int reduction, float* loss,
                             void* kept, void* workspace, int64_t workspace_bytes, void* stream);

@@ -93,8 +93,8 @@ SIGNATURES: dict[str, tuple] = {
     "rk_preference_loss": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64,
                                 _p]),
     "rk_linear_ce_kept": (_i64, [_i64]),
-    "rk_linear_ce_fwd_workspace": (_i64, [_i64, _i64, _i64]),
-    "rk_linear_ce_bwd_workspace": (_i64, [_i64, _i64, _i64]),
+    "rk_linear_ce_fwd_workspace": (_i64, [_i64, _i64, _i64, _i]),
+    "rk_linear_ce_bwd_workspace": (_i64, [_i64, _i64, _i64, _i]),
     "rk_linear_ce_fwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _p, _p, _p, _i64, _p]),
     "rk_linear_ce_bwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i, _i, _p, _p, _i64, _i, _p, _i64, _i, _p, _i64,
                               _p]),

@@ -626,27 +626,88 @@ __global__ void __launch_bounds__(1024)
   if constexpr (CTAS > 1) cluster_sync();  // the others may still read this CTA's total
 }
 
-// Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows. Nothing to do if all rows are
-// listed and the GEMMs can read them where they are.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) ce_gather_kernel(const T* __restrict__ x, int64_t ldx, int width, int64_t pitch,
-                                                        const int* __restrict__ head, const int* __restrict__ rows_of,
-                                                        T* __restrict__ out, int in_place_rows) {
+// One row of 16-bit elements to a 16-byte boundary, by a warp. The source may start anywhere: a vector of the result is cut
+// out of the two aligned ones that hold it, unless those reach behind the array's end or before its start.
+__device__ __forceinline__ void copy_row(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst, int width,
+                                         const uint16_t* first, const uint16_t* end) {
+  const int shift = (int)(reinterpret_cast<uintptr_t>(src) & 15) / 2;  // elements behind a boundary
+  for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) {
+    const uint16_t* lo = src + c - shift;
+    if (lo >= first && lo + (shift ? 16 : 8) <= end) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(lo));
+      uint4 o = a;
+      if (shift) {
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(lo) + 1);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t x = 0, y = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)  // words (shift / 2 + k) and the one behind it
+            if (q == shift >> 1) {
+              x = w[q + k];
+              y = w[q + k + 1];
+            }
+          r[k] = shift & 1 ? __funnelshift_r(x, y, 16) : x;
+        }
+        o = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+      *reinterpret_cast<uint4*>(dst + c) = o;  // the pitch has room for whole vectors
+    } else {
+      for (int e = 0; e < 8 && c + e < width; ++e) dst[c + e] = src[c + e];
+    }
+  }
+}
+
+// Rows of any pitch and address to rows that TMA can read (the weight's).
+__global__ void __launch_bounds__(256) ce_copy_kernel(const uint16_t* __restrict__ w, int64_t ldw, int64_t rows, int width,
+                                                      int64_t pitch, uint16_t* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();  // inputs are the previous kernel's outputs
+  const uint16_t* end = w + (rows - 1) * ldw + width;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (int64_t)gridDim.x * 8)
+    copy_row(w + i * ldw, out + i * pitch, width, w, end);
+}
+
+struct FactorArgs {
+  const float* lse;    // null: no factors are wanted (forward)
+  const float* grad;   // the loss's gradient: one, or one a row (reduction 0)
+  int reduction;
+  float boost;
+  float2* rowc;
+  float* scale;        // reduction 0: already there (ce_scale_kernel)
+};
+
+// Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows; not if all rows are listed and
+// the GEMMs can read them where they are. For the backward also the rows' factors: rowc[i] = (-lse log2 e, f_i) with
+// dz = scale f_i (softmax - onehot). One gradient for all rows: f = boost and scale is that gradient (over the count for
+// a mean) / boost. One a row: scale is a power of two near the largest of them / boost and f_i = g_i / scale, exactly. In
+// fp16 `boost` is a power of two above 1, so that probabilities down to 2^-37 are held.
+__global__ void __launch_bounds__(256) ce_gather_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows, int width,
+                                                        int64_t pitch, const int* __restrict__ head,
+                                                        const int* __restrict__ rows_of, uint16_t* __restrict__ out,
+                                                        int in_place_rows, const FactorArgs f) {
   pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
   const int count = head[0];
+  if (f.lse) {
+    float each = f.boost;
+    if (f.reduction == 0) each = 1.f / *f.scale;
+    else if (blockIdx.x == 0 && threadIdx.x == 0)
+      *f.scale = (f.reduction == 2 ? f.grad[0] / (float)(count > 0 ? count : 1) : f.grad[0]) / f.boost;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256)
+      f.rowc[i] = make_float2(-f.lse[i] * kLog2e, f.reduction == 0 ? f.grad[rows_of[i]] * each : each);
+  }
   if (count == in_place_rows) return;
-  const int end = (count + kTile - 1) / kTile * kTile;
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += gridDim.x * 8) {
-    const T* src = i < count ? x + (int64_t)rows_of[i] * ldx : nullptr;
-    T* dst = out + (int64_t)i * pitch;
-    for (int c = (threadIdx.x & 31) * V; c < width; c += 32 * V) {
-      if constexpr (V == 8) {
-        *reinterpret_cast<uint4*>(dst + c) =
-            src ? __ldg(reinterpret_cast<const uint4*>(src + c)) : make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        dst[c] = src ? src[c] : Dt<T>::from_f(0.f);
-      }
+  const int64_t end = ((int64_t)count + kTile - 1) / kTile * kTile;
+  const uint16_t* behind = x + (rows - 1) * ldx + width;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += (int64_t)gridDim.x * 8) {
+    uint16_t* dst = out + i * pitch;
+    if (i < count) {
+      copy_row(x + (int64_t)rows_of[i] * ldx, dst, width, x, behind);
+    } else {
+      for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
 }
@@ -755,71 +816,68 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   }
 }
 
-// Factors of the backward: rowc[i] = (-lse log2 e, f_i) with dz = scale * f_i * (softmax - onehot). One gradient for
-// all rows: f = 1 and scale is that gradient (over the count for a mean). One a row: scale is a power of two near the
-// largest of them and f_i = g_i / scale, exactly. In fp16 `boost` moves a power of two from the scale to the factors, so
-// that probabilities down to 2^-37 are held.
-__global__ void __launch_bounds__(1024) ce_factor_kernel(const float* __restrict__ lse, const int* __restrict__ head,
-                                                         const int* __restrict__ rows_of, const float* __restrict__ grad,
-                                                         int reduction, float boost, float2* __restrict__ rowc,
-                                                         float* __restrict__ scale) {
+// The scale of the backward when each row has a gradient: a power of two near the largest of them, over boost.
+__global__ void __launch_bounds__(1024) ce_scale_kernel(const int* __restrict__ head, const int* __restrict__ rows_of,
+                                                        const float* __restrict__ grad, float boost,
+                                                        float* __restrict__ scale) {
   pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ float top[32];
   const int count = head[0];
   const int lane = threadIdx.x & 31;
-  float unit = 1.f;
-  if (reduction == 0) {  // every CTA for itself: the gradients are few
-    float m = 0.f;
-    for (int i = threadIdx.x; i < count; i += 1024) m = fmaxf(m, fabsf(grad[rows_of[i]]));
+  float m = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += 1024) m = fmaxf(m, fabsf(grad[rows_of[i]]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) top[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = top[lane];
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) top[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = top[lane];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (threadIdx.x == 0) {
+    float unit = 1.f;
     if (m > 0.f && m < INFINITY) {
       int e;
       frexpf(m, &e);
-      e = e < -100 ? -100 : e > 100 ? 100 : e;  // the scale and its reciprocal are normal numbers
-      unit = ldexpf(1.f, e);
+      unit = ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);  // the scale and its reciprocal are normal numbers
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = unit / boost;
-  } else if (blockIdx.x == 0 && threadIdx.x == 0) {
-    *scale = (reduction == 2 ? grad[0] / (float)(count > 0 ? count : 1) : grad[0]) / boost;
+    *scale = unit / boost;
   }
-  for (int i = blockIdx.x * 1024 + threadIdx.x; i < count; i += gridDim.x * 1024)
-    rowc[i] = make_float2(-lse[i] * kLog2e, (reduction == 0 ? grad[rows_of[i]] / unit : 1.f) * boost);
 }
 
-// out[r] = scale * sum of the slices of row pos[r] (zeros where that is -1), or of row r without pos, in slice order.
-template <typename T, int V>
+// out[r] = scale * sum of the slices of row pos[r] (zeros where that is -1), or of row r without pos, in slice order. A
+// warp takes a row; VEC: rows of out allow stores of four elements.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) ce_reduce_kernel(const float* __restrict__ part, int slices, int64_t slice_rows,
                                                         int64_t pitch, const int* __restrict__ pos,
                                                         const float* __restrict__ scale, T* __restrict__ out,
                                                         int64_t ldo, int64_t rows, int width) {
   pdl_wait();  // inputs are the previous kernel's outputs
   const float f = *scale;
-  const int64_t per = (width + V - 1) / V, n = rows * per;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-    const int64_t r = t / per;
-    const int c = (int)(t - r * per) * V;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     const int64_t i = pos ? pos[r] : r;
-    float s[V];
+#pragma unroll 2
+    for (int c = (threadIdx.x & 31) * 4; c < width; c += 128) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      if (i >= 0) {
+        for (int k = 0; k < slices; ++k) {
+          float v[4];
+          load_vec<float, 4>(part + ((int64_t)k * slice_rows + i) * pitch + c, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = 0.f;
-    if (i >= 0) {
-      for (int k = 0; k < slices; ++k) {
-        float v[V];
-        load_vec<float, V>(part + ((int64_t)k * slice_rows + i) * pitch + c, v);
+          for (int e = 0; e < 4; ++e) s[e] += v[e];
+        }
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e] += v[e];
+        for (int e = 0; e < 4; ++e) s[e] *= f;
       }
+      if (VEC) {
+        store_vec<T, 4>(out + r * ldo + c, s);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[e] *= f;
+        for (int e = 0; e < 4; ++e)
+          if (c + e < width) out[r * ldo + c + e] = Dt<T>::from_f(s[e]);
+      }
     }
-    store_vec<T, V>(out + r * ldo + c, s);
   }
 }
 
@@ -881,7 +939,9 @@ double waves_us(int64_t tiles, int64_t slices, int64_t kb) {
 double moved_us(double bytes) { return bytes / 5e6 + 3.0; }
 
 CePlan make_plan(int64_t M, int64_t V, int64_t K) {
-  CePlan p{};
+  static thread_local CePlan p{};  // of the last sizes asked for: the choice takes some microseconds
+  if (p.M == M && p.V == V && p.K == K) return p;
+  p = CePlan{};
   p.M = M;
   p.V = V;
   p.K = K;
@@ -949,14 +1009,17 @@ struct Arena {
   }
 };
 
+bool w_ready(const void* w, int64_t ldw, int64_t V) { return rk_host::aligned(w, 16) && (V == 1 || ldw % 8 == 0); }
+
 struct FwdSpace {
-  void* x;
+  void *x, *w;
   float2* part;
   float* xlabel;
   double* sums;
 };
-int64_t fwd_space(const CePlan& p, char* base, FwdSpace* f) {
+int64_t fwd_space(const CePlan& p, bool copy_w, char* base, FwdSpace* f) {
   Arena a{base, 0};
+  f->w = a.take(copy_w ? p.V * p.Kp * 2 : 0);
   f->x = a.take(p.Mp * p.Kp * 2);
   f->part = static_cast<float2*>(a.take((int64_t)p.units * 4 * kTile * 8));
   f->xlabel = static_cast<float*>(a.take(p.M * 4));
@@ -965,7 +1028,7 @@ int64_t fwd_space(const CePlan& p, char* base, FwdSpace* f) {
 }
 
 struct BwdSpace {
-  void *x, *dz;
+  void *x, *w, *dz;
   float2* rowc;
   float *scale, *dx, *dw;
 };
@@ -973,8 +1036,9 @@ struct BwdSpace {
 bool dw_direct(const CePlan& p, const void* dw, int64_t lddw, int dw_dtype, int dtype) {
   return p.dw_slices == 1 && dw_dtype == dtype && rk_host::aligned(dw, 16) && (lddw * 2) % 16 == 0;
 }
-int64_t bwd_space(const CePlan& p, char* base, BwdSpace* b) {
+int64_t bwd_space(const CePlan& p, bool copy_w, char* base, BwdSpace* b) {
   Arena a{base, 0};
+  b->w = a.take(copy_w ? p.V * p.Kp * 2 : 0);
   b->x = a.take(p.Mp * p.Kp * 2);
   b->dz = a.take(p.Mp * p.piece_tiles * kTile * 2);
   b->rowc = static_cast<float2*>(a.take(p.M * 8));
@@ -997,23 +1061,26 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
   return rk_host::launch_status();
 }
 
-template <typename T>
-int gather_typed(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, bool in_place, cudaStream_t s) {
-  const bool vec = p.K % 8 == 0 && rk_host::aligned(x, 16) && (p.M <= 1 || ldx % 8 == 0);
+int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, bool in_place, const FactorArgs& f,
+           cudaStream_t s) {
   const int64_t blocks = ceil_div(p.Mp, 8);
   const unsigned grid = (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
-  if (vec)
-    rk_host::launch_k(ce_gather_kernel<T, 8>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
-                      k.rows_of, static_cast<T*>(out), in_place ? (int)p.M : -1);
-  else
-    rk_host::launch_k(ce_gather_kernel<T, 1>, grid, 256, 0, s, static_cast<const T*>(x), ldx, (int)p.K, p.Kp, k.head,
-                      k.rows_of, static_cast<T*>(out), in_place ? (int)p.M : -1);
+  rk_host::launch_k(ce_gather_kernel, grid, 256, 0, s, static_cast<const uint16_t*>(x), ldx, p.M, (int)p.K, p.Kp, k.head,
+                    k.rows_of, static_cast<uint16_t*>(out), in_place ? (int)p.M : -1, f);
   return rk_host::launch_status();
 }
-int gather(const void* x, int64_t ldx, const CePlan& p, const CeKept& k, void* out, int dtype, bool in_place,
-           cudaStream_t s) {
-  return dtype == RK_BF16 ? gather_typed<__nv_bfloat16>(x, ldx, p, k, out, in_place, s)
-                          : gather_typed<__half>(x, ldx, p, k, out, in_place, s);
+// The weight as TMA can read it: itself, or a copy in `space` (whose pitch then replaces ldw).
+int weight_rows(const void*& w, int64_t& ldw, const CePlan& p, void* space, cudaStream_t s) {
+  if (w_ready(w, ldw, p.V)) {
+    if (p.V == 1) ldw = p.Kp;  // one row: its pitch says nothing
+    return RK_OK;
+  }
+  const int64_t blocks = ceil_div(p.V, 8);
+  rk_host::launch_k(ce_copy_kernel, (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s,
+                    static_cast<const uint16_t*>(w), ldw, p.V, (int)p.K, p.Kp, static_cast<uint16_t*>(space));
+  w = space;
+  ldw = p.Kp;
+  return rk_host::launch_status();
 }
 // One CTA for up to 4096 rows (its launch is the cheaper one), a cluster of eight for more.
 int list_rows(const int64_t* labels, int64_t ignore, const CePlan& p, const CeKept& k, unsigned int* status,
@@ -1046,14 +1113,10 @@ template <typename T>
 int reduce_typed(const float* part, int slices, int64_t slice_rows, int64_t pitch, const int* pos, const float* scale,
                  void* out, int64_t ldo, int64_t rows, int64_t width, cudaStream_t s) {
   const bool vec = width % 4 == 0 && ldo % 4 == 0 && rk_host::aligned(out, 4 * sizeof(T));
-  int64_t blocks = ceil_div(rows * ceil_div(width, vec ? 4 : 1), 256);
-  if (blocks > 148 * 16) blocks = 148 * 16;
-  if (vec)
-    rk_host::launch_k(ce_reduce_kernel<T, 4>, (unsigned)blocks, 256, 0, s, part, slices, slice_rows, pitch, pos, scale,
-                      static_cast<T*>(out), ldo, rows, (int)width);
-  else
-    rk_host::launch_k(ce_reduce_kernel<T, 1>, (unsigned)blocks, 256, 0, s, part, slices, slice_rows, pitch, pos, scale,
-                      static_cast<T*>(out), ldo, rows, (int)width);
+  const int64_t blocks = ceil_div(rows, 8);
+  auto kern = vec ? ce_reduce_kernel<T, true> : ce_reduce_kernel<T, false>;
+  rk_host::launch_k(kern, (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s, part, slices, slice_rows, pitch, pos,
+                    scale, static_cast<T*>(out), ldo, rows, (int)width);
   return rk_host::launch_status();
 }
 int reduce(const float* part, int slices, int64_t slice_rows, int64_t pitch, const int* pos, const float* scale, void* out,
@@ -1072,16 +1135,16 @@ bool sizes_ok(int64_t M, int64_t V, int64_t K) {
 
 extern "C" int64_t rk_linear_ce_kept(int64_t M) { return M < 0 ? 0 : (4 + 4 * M) * 4; }
 
-extern "C" int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K) {
+extern "C" int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w) {
   if (!sizes_ok(M, V, K) || M == 0) return 0;
   FwdSpace f;
-  return fwd_space(make_plan(M, V, K), nullptr, &f);
+  return fwd_space(make_plan(M, V, K), copy_w != 0, nullptr, &f);
 }
 
-extern "C" int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K) {
+extern "C" int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w) {
   if (!sizes_ok(M, V, K) || M == 0) return 0;
   BwdSpace b;
-  return bwd_space(make_plan(M, V, K), nullptr, &b);
+  return bwd_space(make_plan(M, V, K), copy_w != 0, nullptr, &b);
 }
 
 extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
@@ -1091,25 +1154,26 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   if (!sizes_ok(M, V, K) || (M > 1 && ldh < K) || (V > 1 && ldw < K) || reduction < 0 || reduction > 2 || !kept ||
       (M && (!hidden || !w || !labels)) || (!loss && (M || reduction)))
     return RK_ERR_ARG;
-  if (!rk_host::aligned(w, 16) || (V > 1 && ldw % 8) || !rk_host::aligned(kept, 16)) return RK_ERR_ALIGN;
+  if (!rk_host::aligned(kept, 16) || !rk_host::aligned(hidden, 2) || !rk_host::aligned(w, 2)) return RK_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M == 0) {
     if (cudaMemsetAsync(kept, 0, 16, s) != cudaSuccess) return RK_ERR_LAUNCH;
     if (reduction && cudaMemsetAsync(loss, 0, 4, s) != cudaSuccess) return RK_ERR_LAUNCH;
     return RK_OK;
   }
-  if (V == 1) ldw = up(K, 8);  // one row: its pitch says nothing
   const CePlan p = make_plan(M, V, K);
   FwdSpace f;
-  if (!workspace || workspace_bytes < fwd_space(p, nullptr, &f)) return RK_ERR_WORKSPACE;
+  const bool copy_w = !w_ready(w, ldw, V);
+  if (!workspace || workspace_bytes < fwd_space(p, copy_w, nullptr, &f)) return RK_ERR_WORKSPACE;
   if (!rk_host::aligned(workspace, 256)) return RK_ERR_ALIGN;
-  fwd_space(p, static_cast<char*>(workspace), &f);
+  fwd_space(p, copy_w, static_cast<char*>(workspace), &f);
   const CeKept k = kept_of(static_cast<int*>(kept), M);
   unsigned int* status = rk_host::device_status_ptr();
   int st = list_rows(labels, ignore_index, p, k, status, s);
   if (st != RK_OK) return st;
   const bool in_place = readable(hidden, ldh, p);
-  if ((st = gather(hidden, ldh, p, k, f.x, dtype, in_place, s)) != RK_OK) return st;
+  if ((st = gather(hidden, ldh, p, k, f.x, in_place, FactorArgs{}, s)) != RK_OK) return st;
+  if ((st = weight_rows(w, ldw, p, f.w, s)) != RK_OK) return st;
   CUtensorMap ta, tb, tx;
   if (!tensor_map(&ta, f.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&tb, w, K, V, ldw, dtype, kKb, kHalf))
     return RK_ERR_LAUNCH;
@@ -1142,9 +1206,9 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   if (!sizes_ok(M, V, K) || (M > 1 && (ldh < K || (dx && lddx < K))) || (V > 1 && (ldw < K || (dw && lddw < K))) ||
       reduction < 0 || reduction > 2 || !kept || (M && (!hidden || !w)) || (!grad && (M || reduction)))
     return RK_ERR_ARG;
-  if (!rk_host::aligned(w, 16) || (V > 1 && ldw % 8) || !rk_host::aligned(kept, 16)) return RK_ERR_ALIGN;
+  if (!rk_host::aligned(kept, 16) || !rk_host::aligned(hidden, 2) || !rk_host::aligned(w, 2)) return RK_ERR_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (V == 1) ldw = lddw = up(K, 8);  // one row: its pitch says nothing
+  if (V == 1) lddw = up(K, 8);  // one row: its pitch says nothing
   if (M == 0) {
     if (dw && cudaMemset2DAsync(dw, lddw * rk_host::dtype_size(dw_dtype), 0, K * rk_host::dtype_size(dw_dtype), V, s) !=
                   cudaSuccess)
@@ -1155,18 +1219,21 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   if (!dx && !dw) return RK_OK;
   const CePlan p = make_plan(M, V, K);
   BwdSpace b;
-  if (!workspace || workspace_bytes < bwd_space(p, nullptr, &b)) return RK_ERR_WORKSPACE;
+  const bool copy_w = !w_ready(w, ldw, V);
+  if (!workspace || workspace_bytes < bwd_space(p, copy_w, nullptr, &b)) return RK_ERR_WORKSPACE;
   if (!rk_host::aligned(workspace, 256)) return RK_ERR_ALIGN;
-  bwd_space(p, static_cast<char*>(workspace), &b);
+  bwd_space(p, copy_w, static_cast<char*>(workspace), &b);
   const CeKept k = kept_of(const_cast<int*>(static_cast<const int*>(kept)), M);
   float* scale = b.scale;
   const bool in_place = readable(hidden, ldh, p);
-  int st = gather(hidden, ldh, p, k, b.x, dtype, in_place, s);
-  if (st != RK_OK) return st;
-  const int64_t fblocks = ceil_div(M, 4096);
-  rk_host::launch_k(ce_factor_kernel, (unsigned)(fblocks < 64 ? fblocks : 64), 1024, 0, s, k.lse, k.head, k.rows_of, grad,
-                    reduction, dtype == RK_F16 ? 8192.f : 1.f, b.rowc, scale);
-  if ((st = rk_host::launch_status()) != RK_OK) return st;
+  const FactorArgs f{k.lse, grad, reduction, dtype == RK_F16 ? 8192.f : 1.f, b.rowc, scale};
+  int st = RK_OK;
+  if (reduction == 0) {
+    rk_host::launch_k(ce_scale_kernel, 1, 1024, 0, s, k.head, k.rows_of, grad, f.boost, scale);
+    if ((st = rk_host::launch_status()) != RK_OK) return st;
+  }
+  if ((st = gather(hidden, ldh, p, k, b.x, in_place, f, s)) != RK_OK) return st;
+  if ((st = weight_rows(w, ldw, p, b.w, s)) != RK_OK) return st;
   const int64_t pitch = (int64_t)p.piece_tiles * kTile;  // of dz
   const bool direct = dw && dw_direct(p, dw, lddw, dw_dtype, dtype);
   CUtensorMap x_k, x_mn, in_k, in_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out, dw_out;

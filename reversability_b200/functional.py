@@ -480,13 +480,18 @@ def _linear_ce_check(hidden, weight, labels, reduction):
 
 
 @functools.lru_cache(maxsize=64)
-def _linear_ce_bytes(M: int, V: int, K: int) -> tuple[int, int, int]:
+def _linear_ce_bytes(M: int, V: int, K: int, copy_w: bool) -> tuple[int, int, int]:
     lib = _lib.lib()
-    return lib.rk_linear_ce_kept(M), lib.rk_linear_ce_fwd_workspace(M, V, K), lib.rk_linear_ce_bwd_workspace(M, V, K)
+    return (lib.rk_linear_ce_kept(M), lib.rk_linear_ce_fwd_workspace(M, V, K, copy_w),
+            lib.rk_linear_ce_bwd_workspace(M, V, K, copy_w))
 
 
-def _head_weight(weight: torch.Tensor) -> torch.Tensor:
-    return _tma_ready(weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous())
+def _head_weight(weight: torch.Tensor) -> tuple[torch.Tensor, int, bool]:
+    """(weight with unit-stride rows, row stride, whether the library has to copy it to rows that TMA can read)."""
+    if weight.stride(1) != 1 or (weight.stride(0) < weight.shape[1] and weight.shape[0] > 1):
+        weight = weight.contiguous()
+    ld = weight.stride(0) if weight.shape[0] > 1 else weight.shape[1]
+    return weight, ld, weight.data_ptr() % 16 != 0 or (weight.shape[0] > 1 and ld % 8 != 0)
 
 
 def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
@@ -500,11 +505,11 @@ def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
     if hidden.dtype == torch.float32:
         return _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss)
     x, M, _, ld = even_rows(hidden)
-    w = _head_weight(weight)
-    n_kept, n_ws, _ = _linear_ce_bytes(M, V, K)
+    w, ldw, copy_w = _head_weight(weight)
+    n_kept, n_ws, _ = _linear_ce_bytes(M, V, K, copy_w)
     kept = labels.new_empty(n_kept // 4, dtype=torch.int32)
     ws = labels.new_empty(n_ws, dtype=torch.uint8)
-    _lib.call("rk_linear_ce_fwd", x.data_ptr(), ld, w.data_ptr(), _ld(w), labels.data_ptr(), int(ignore_index), M, V, K,
+    _lib.call("rk_linear_ce_fwd", x.data_ptr(), ld, w.data_ptr(), ldw, labels.data_ptr(), int(ignore_index), M, V, K,
               _lib.code(hidden.dtype), _REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n_ws,
               _lib.stream_ptr())
     return loss, kept
@@ -525,10 +530,10 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
         return _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw)
     _on_current_device(hidden, "hidden", weight, kept)
     x, M, _, ld = even_rows(hidden)
-    w = _head_weight(weight)
-    n_ws = _linear_ce_bytes(M, V, K)[2]
+    w, ldw, copy_w = _head_weight(weight)
+    n_ws = _linear_ce_bytes(M, V, K, copy_w)[2]
     ws = torch.empty(n_ws, device=hidden.device, dtype=torch.uint8)
-    _lib.call("rk_linear_ce_bwd", x.data_ptr(), ld, w.data_ptr(), _ld(w), kept.data_ptr(), M, V, K,
+    _lib.call("rk_linear_ce_bwd", x.data_ptr(), ld, w.data_ptr(), ldw, kept.data_ptr(), M, V, K,
               _lib.code(hidden.dtype), _REDUCTIONS[reduction], grad.data_ptr(), _lib.ptr(dx), K,
               _lib.code(dx.dtype) if want_dx else 0, _lib.ptr(dw), K, _lib.code(dw.dtype) if want_dw else 0,
               ws.data_ptr(), n_ws, _lib.stream_ptr())
