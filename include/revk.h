@@ -352,7 +352,7 @@ RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, c
  * ldw, any alignment) in bf16 or f16, labels int64 [M]. A row whose label is ignore_index is not read, loses 0 and gets a
  * zero gradient; a label outside [0, V) sets RK_DEV_CE_LABEL and counts as
  * ignored. reduction 0: loss[M] per row; 1: their sum, loss[1]; 2: their mean
- * over the rows that count (0 if none does).
+ * over the rows that count (0 if none does). M < 2^26, V < 2^30, K < 2^24.
  * kept (rk_linear_ce_kept(M) bytes, 16-byte aligned) carries the listed rows
  * and their log-sum-exps to the backward, which does not write it. Workspaces
  * are 256-byte aligned; the backward's holds dz of one piece of the vocabulary

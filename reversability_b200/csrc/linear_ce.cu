@@ -1128,7 +1128,7 @@ int reduce(const float* part, int slices, int64_t slice_rows, int64_t pitch, con
 }
 
 bool sizes_ok(int64_t M, int64_t V, int64_t K) {
-  return M >= 0 && V > 0 && K > 0 && M < (1ll << 30) && V < (1ll << 30) && K < (1ll << 24);
+  return M >= 0 && V > 0 && K > 0 && M < (1ll << 26) && V < (1ll << 30) && K < (1ll << 24);
 }
 
 }  // namespace

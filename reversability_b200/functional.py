@@ -187,14 +187,16 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
     require_cuda(x, residual, what="dropout kernels")
     if not 0.0 <= p <= 1.0:
         raise ValueError("the dropout probability must be in [0, 1]")
+    offset, on_device = int(offset), isinstance(seed, torch.Tensor)
     if not 0 <= offset < 2 ** 64:
         raise ValueError("the dropout offset must fit 64 bits")
-    on_device = isinstance(seed, torch.Tensor)
     if on_device:
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ValueError("a dropout seed on the device must be one int64 number")
-    elif not -2 ** 63 <= seed < 2 ** 64:
-        raise ValueError("the dropout seed must fit 64 bits")
+    else:
+        seed = int(seed)
+        if not -2 ** 63 <= seed < 2 ** 64:
+            raise ValueError("the dropout seed must fit 64 bits")
     if residual is not None and (residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32)):
         raise ValueError("the dropout residual must have the input's shape and its type or fp32")
     _on_current_device(x, "the input", residual, seed if on_device else None)

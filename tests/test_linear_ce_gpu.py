@@ -22,7 +22,8 @@ SMALLEST = {F32: 1e-36, BF16: 1e-36, F16: 3e-8}
 E = 2.0 ** -24
 # (rows, vocabulary, width): one of each, tile and k-block edges, several pieces, a slice of every reduction
 SHAPES = [(1, 1, 1), (1, 2, 8), (3, 7, 5), (5, 300, 33), (130, 1000, 64), (257, 4099, 72), (600, 513, 256), (1000, 2000, 328),
-          (64, 50257, 256), (300, 257, 1024), (2500, 1500, 96), (40, 700, 2056), (5000, 300, 40)]
+          (64, 50257, 256), (300, 257, 1024), (2500, 1500, 96), (40, 700, 2056), (5000, 300, 40),
+          (256, 256, 64), (512, 512, 128), (257, 257, 65), (9000, 600, 520), (3, 20000, 24)]
 
 
 def _inputs(M, V, K, dtype, seed=0, ignored=0.3):
@@ -275,6 +276,43 @@ def test_refusals():
                        (lambda: fx.linear_cross_entropy(x, w, y.cpu()), "CUDA")):
         with pytest.raises(ValueError, match=match):
             bad()
+
+
+def test_two_streams_and_two_graphs_at_once():
+    """Calls of different sizes in flight together, then two captured steps replayed in turn: each as if alone."""
+    cases = [_inputs(700, 1500, 64, BF16, 1), _inputs(300, 4000, 136, BF16, 2)]
+
+    def step(x, w, y):
+        loss = fx.linear_cross_entropy(x, w, y)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for k, c in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(*c))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(s, t) for r in got[k] for s, t in zip(r, want[k]))
+    graphs, outs = [], []
+    for x, w, y in cases:
+        leaves = (x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_())  # no eager graph holds them
+        with torch.cuda.stream(streams[0]):
+            step(*leaves, y)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*leaves, y))
+        graphs.append((graph, leaves, y))
+    for _ in range(3):
+        for graph, _, _ in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(s, t) for s, t in zip(outs[k], want[k]))
+    assert _lib.device_status() == 0
 
 
 def test_captured_and_replayed():

@@ -18,7 +18,8 @@ SMALLEST = {F32: 1e-36, BF16: 1e-36, F16: 3e-8}
 E = 2.0 ** -24
 # (rows, width): one element, warp, vector and CTA edges, more rows than the backward has CTAs, the widest
 SHAPES = [(1, 1), (3, 2), (5, 7), (9, 8), (17, 31), (33, 256), (70, 257), (10, 1000), (6, 1024), (5, 1025), (3, 4097),
-          (3, 8192), (2, 16384), (5000, 333), (7000, 64), (1500, 768), (700, 1536)]
+          (3, 8192), (2, 16384), (5000, 333), (7000, 64), (1500, 768), (700, 1536),
+          (100, 1017), (100, 1019), (1400, 1501), (310, 5003), (160, 8191), (150, 10007)]
 
 
 def _rows(rows, width, dtype, layout="plain", seed=0, shift=0.5):
@@ -152,6 +153,23 @@ def test_layer_norm_gradients_are_the_same_bits_every_run():
     runs = [torch.autograd.grad(fx.layer_norm(x, w, b), (x, w, b), g) for _ in range(3)]
     for r in runs[1:]:
         assert all(torch.equal(s, t) for s, t in zip(r, runs[0]))
+
+
+def test_layer_norm_on_two_streams_at_once():
+    inputs = [(_rows(3000, 640, BF16, seed=k).requires_grad_(), _rows(3000, 640, BF16, seed=9 + k)) for k in range(2)]
+    w, b = _params(640, F32)
+    want = [torch.autograd.grad(fx.layer_norm(x, w, b), (x, w, b), g) for x, g in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for k, (x, g) in enumerate(inputs):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(torch.autograd.grad(fx.layer_norm(x, w, b), (x, w, b), g))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(s, t) for s, t in zip(r, want[k]))
 
 
 def test_layer_norm_gradient_against_differences():
