@@ -184,7 +184,9 @@ def check(code: int, name: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    code = getattr(_lib or lib(), name)(*args)
+    if code != 0:
+        check(code, name)
 
 
 _launch_override: list[int] = []  # stack of stream handles set by launch_on()

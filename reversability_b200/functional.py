@@ -75,10 +75,11 @@ def rmsnorm_bwd(x: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dy: t
 
 # ------------------------------------------------------------------ layer norm
 def _on_current_device(t: torch.Tensor, name: str, *others: torch.Tensor | None) -> None:
-    if t.get_device() != torch.cuda.current_device():
+    index = t.get_device()
+    if index != torch.cuda.current_device():
         raise ValueError(f"{name} must be on the current CUDA device")
     for o in others:
-        if o is not None and o.get_device() != t.get_device():
+        if o is not None and o.get_device() != index:
             raise ValueError(f"all tensors must be on {name}'s device")
 
 
@@ -118,42 +119,78 @@ def _norm_rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, int, int, int]:
     return t.clone(memory_format=torch.contiguous_format), rows, width, width
 
 
+def _norm_param(x: torch.Tensor, t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != x.shape[-1] or (t.dtype is not torch.float32 and t.dtype != x.dtype):
+        raise ValueError(f"layer norm {name} must be [width] in fp32 or the input's type")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None):
     """(weight, bias, dtype code): contiguous [width] vectors of one type, fp32 or x's."""
-    dtype = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.dtype not in (torch.float32, x.dtype):
-                raise ValueError(f"layer norm {name} must be [width] in fp32 or the input's type")
-            if dtype is not None and t.dtype != dtype:
-                raise ValueError("layer norm weight and bias must share a type")
-            dtype = t.dtype
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    return weight, bias, _lib.code(dtype or torch.float32)
+    if weight is not None:
+        weight = _norm_param(x, weight, "weight")
+    if bias is not None:
+        bias = _norm_param(x, bias, "bias")
+        if weight is not None and bias.dtype != weight.dtype:
+            raise ValueError("layer norm weight and bias must share a type")
+    one = bias if weight is None else weight
+    return weight, bias, 0 if one is None else _lib.code(one.dtype)
+
+
+def _fast_rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, int, int, int]:
+    if t.is_contiguous() and t.data_ptr() % 32 == 0 and t.shape[-1]:
+        width = t.shape[-1]
+        return t, t.numel() // width, width, width
+    return _norm_rows(t, per)
+
+
+def layernorm_fwd_rows(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                       out_dtype: torch.dtype | None = None, want_stats: bool = True):
+    """layernorm_fwd that also returns what its backward can use again: (y, stats, weight, (rows of x, their number,
+    width, stride, dtype code, parameters' dtype code))."""
+    require_cuda(x, weight, bias, what="layer norm kernels")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("layer norm needs a non-empty last dimension")
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif x.dtype is not torch.float32 and out_dtype not in (x.dtype, torch.float32):
+        raise ValueError("layer norm of 16-bit inputs gives their type or fp32")
+    _on_current_device(x, "the input", weight, bias)
+    weight, bias, pcode = _norm_params(x, weight, bias)
+    xr, rows, width, ld = _fast_rows(x, 16 // x.element_size())
+    xcode = _lib.code(x.dtype)
+    y = _new(x, out_dtype)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
+    _lib.call("rk_layernorm_fwd", xr.data_ptr(), xcode, ld, _lib.ptr(weight), _lib.ptr(bias), pcode, y.data_ptr(),
+              _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, eps, _lib.stream_ptr())
+    return y, stats, weight, (xr, rows, width, ld, xcode, pcode)
 
 
 def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
                   out_dtype: torch.dtype | None = None, want_stats: bool = True):
     """y = (x - mean) * rsqrt(var + eps) * weight + bias over the last dim; returns (y, stats [rows, 2] or None)."""
-    require_cuda(x, weight, bias, what="layer norm kernels")
-    out_dtype = out_dtype or x.dtype
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError("layer norm needs a non-empty last dimension")
-    if x.dtype != torch.float32 and out_dtype not in (x.dtype, torch.float32):
-        raise ValueError("layer norm of 16-bit inputs gives their type or fp32")
-    _on_current_device(x, "the input", weight, bias)
-    weight, bias, pcode = _norm_params(x, weight, bias)
-    xr, rows, width, ld = _norm_rows(x, 16 // x.element_size())
-    y = _new(x, out_dtype)
-    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
-    _lib.call("rk_layernorm_fwd", xr.data_ptr(), _lib.code(x.dtype), ld, _lib.ptr(weight), _lib.ptr(bias), pcode,
-              y.data_ptr(), _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, float(eps), _lib.stream_ptr())
-    return y, stats
+    return layernorm_fwd_rows(x, weight, bias, float(eps), out_dtype, want_stats)[:2]
 
 
 @functools.lru_cache(maxsize=64)
 def _layernorm_workspace(rows: int, width: int) -> int:
     return _lib.lib().rk_layernorm_bwd_workspace(rows, width)
+
+
+def layernorm_bwd_rows(x_rows: tuple, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+                       param_dtype: torch.dtype, want_dx: bool, want_dw: bool, want_db: bool):
+    """layernorm_bwd from layernorm_fwd_rows' results, which were checked there."""
+    xr, rows, width, ldx, xcode, pcode = x_rows
+    dyr, _, _, lddy = _fast_rows(dy, 16 // xr.element_size())
+    dx = _new(xr, xr.dtype) if want_dx else None
+    dw = (xr.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_dw else None
+    db = (xr.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_db else None
+    n_ws = _layernorm_workspace(rows, width) if want_dw or want_db else 0
+    ws = stats.new_empty(n_ws // 4) if n_ws else None
+    _lib.call("rk_layernorm_bwd", xr.data_ptr(), xcode, ldx, _lib.ptr(weight), pcode, stats.data_ptr(), dyr.data_ptr(),
+              _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), n_ws, rows, width,
+              _lib.stream_ptr())
+    return dx, dw, db
 
 
 def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
@@ -165,18 +202,11 @@ def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Ten
     weight, _, _ = _norm_params(x, weight, None)
     if weight is not None and weight.dtype != param_dtype:
         raise ValueError("parameter gradients come in the weight's type")
-    per = 16 // x.element_size()
-    xr, rows, width, ldx = _norm_rows(x, per)
-    dyr, _, _, lddy = _norm_rows(dy, per)
-    dx = _new(x, x.dtype) if want_dx else None
-    dw = x.new_empty(width, dtype=param_dtype) if want_dw else None
-    db = x.new_empty(width, dtype=param_dtype) if want_db else None
-    n_ws = _layernorm_workspace(rows, width) if want_dw or want_db else 0
-    ws = x.new_empty(n_ws // 4, dtype=torch.float32) if n_ws else None
-    _lib.call("rk_layernorm_bwd", xr.data_ptr(), _lib.code(x.dtype), ldx, _lib.ptr(weight), _lib.code(param_dtype),
-              stats.data_ptr(), dyr.data_ptr(), _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw),
-              _lib.ptr(db), _lib.ptr(ws), n_ws, rows, width, _lib.stream_ptr())
-    return dx, dw, db
+    xr, rows, width, ldx = _norm_rows(x, 16 // x.element_size())
+    if dy.shape != x.shape or stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError("layer norm backward takes dy of the input's shape and the forward's stats")
+    x_rows = (xr, rows, width, ldx, _lib.code(x.dtype), _lib.code(param_dtype))
+    return layernorm_bwd_rows(x_rows, weight, stats, dy, param_dtype, want_dx, want_dw, want_db)
 
 
 # ------------------------------------------------------------------ dropout
@@ -203,12 +233,20 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0
     out_dtype = out_dtype or (x.dtype if residual is None else residual.dtype)
     if residual is not None and out_dtype != residual.dtype:
         raise ValueError("dropout with a residual gives the residual's type")
+    return dropout_checked(x, float(p), seed, offset, residual, out_dtype)
+
+
+def dropout_checked(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int, residual: torch.Tensor | None,
+                    out_dtype: torch.dtype) -> torch.Tensor:
+    """dropout of arguments that were checked."""
     x = x.contiguous()
-    residual = None if residual is None else residual.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
+    on_device = isinstance(seed, torch.Tensor)
     y = _new(x, out_dtype)
     _lib.call("rk_dropout", x.data_ptr(), _lib.code(x.dtype), _lib.ptr(residual), y.data_ptr(), _lib.code(out_dtype),
-              x.numel(), float(p), 0 if on_device else seed & (2 ** 64 - 1), seed.data_ptr() if on_device else None,
-              offset, _lib.stream_ptr())
+              x.numel(), p, 0 if on_device else seed & 0xFFFFFFFFFFFFFFFF, seed.data_ptr() if on_device else None, offset,
+              _lib.stream_ptr())
     return y
 
 

@@ -105,21 +105,31 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float | None) -> torch.Tenso
     return RMSNormFn.apply(x.contiguous(), w, float(eps))
 
 
+def once(backward):
+    """once_differentiable, whose context costs some microseconds, only where a graph of the backward is recorded."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class LayerNormFn(torch.autograd.Function):
     """Keeps the input and two numbers a row."""
 
     @staticmethod
     def forward(ctx, x, w, b, eps, out_dtype):
-        y, stats = fn.layernorm_fwd(x, w, b, eps, out_dtype)
-        ctx.save_for_backward(x, w, stats)
-        ctx.param_dtype = (w if w is not None else b).dtype if w is not None or b is not None else torch.float32
+        y, stats, weight, (xr, *ctx.rows) = fn.layernorm_fwd_rows(x, w, b, eps, out_dtype)
+        ctx.save_for_backward(xr, weight, stats)
+        ctx.param_dtype = torch.float32 if w is None and b is None else (b if w is None else w).dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gy):
-        x, w, stats = ctx.saved_tensors
-        dx, dw, db = fn.layernorm_bwd(x, w, stats, gy, ctx.param_dtype, *ctx.needs_input_grad[:3])
+        xr, weight, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = fn.layernorm_bwd_rows((xr, *ctx.rows), weight, stats, gy, ctx.param_dtype, need[0], need[1], need[2])
         return dx, dw, db, None, None
 
 
@@ -129,10 +139,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise (any type for fp32 x, fp32 for
     16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in its input's type under
     autocast. The gradients of weight and bias are sums in a fixed order."""
-    fn.require_cuda(x, weight, bias, what="layer norm kernels")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
-    return fn.layernorm_fwd(x, weight, bias, float(eps), out_dtype, want_stats=False)[0]
+    return fn.layernorm_fwd_rows(x, weight, bias, float(eps), out_dtype, False)[0]
 
 
 class DropoutFn(torch.autograd.Function):
@@ -140,18 +150,22 @@ class DropoutFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset):
-        on_device = isinstance(seed, torch.Tensor)
-        ctx.save_for_backward(*((seed,) if on_device else ()))
-        ctx.seed = None if on_device else seed
-        ctx.p, ctx.offset, ctx.dtype = p, offset, x.dtype
-        return fn.dropout(x, p, seed, offset, residual)
+        y = fn.dropout(x, p, seed, offset, residual)
+        if isinstance(seed, torch.Tensor):
+            ctx.save_for_backward(seed)
+            seed = None
+        ctx.args = p, seed, int(offset), x.dtype
+        return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gy):
-        seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
-        dx = fn.dropout(gy, ctx.p, seed, ctx.offset, out_dtype=ctx.dtype) if ctx.needs_input_grad[0] else None
-        return dx, gy if ctx.needs_input_grad[1] else None, None, None, None
+        p, seed, offset, dtype = ctx.args
+        need = ctx.needs_input_grad
+        dx = None
+        if need[0]:
+            dx = fn.dropout_checked(gy, p, ctx.saved_tensors[0] if seed is None else int(seed), offset, None, dtype)
+        return dx, gy if need[1] else None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, *, offset: int = 0,
@@ -162,7 +176,6 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, *, offset: int 
     the result is added to it, in its type. Give every call of a step its own offset and every step its own seed (or
     the other way round). seed may be an int64 scalar on the device, which a captured step's replays read anew;
     change it in place only after the backward. What is dropped is not used: NaN there does not spread."""
-    fn.require_cuda(x, residual, what="dropout kernels")
     if not training:
         p = 0.0
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
@@ -200,10 +213,11 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, g):
         hidden, weight, kept = ctx.saved_tensors
-        dx, dw = fn.linear_ce_bwd(hidden, weight, kept, g, ctx.reduction, *ctx.needs_input_grad[:2])
+        need = ctx.needs_input_grad
+        dx, dw = fn.linear_ce_bwd(hidden, weight, kept, g, ctx.reduction, need[0], need[1])
         return dx, dw, None, None, None
 
 
@@ -215,10 +229,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     gradients; a label outside [0, V) sets the library's device status and counts as ignored. The gradients come in the
     inputs' types, rounded once from fp32 sums over 16-bit softmax terms (fp16: scaled inside, so a mean over many rows
     does not underflow before the gradients themselves do). Under autocast both inputs are cast as F.linear's are."""
-    fn.require_cuda(hidden, weight, labels, what="the head loss")
-    low = autocast_dtype(hidden.device.type)
+    low = autocast_dtype("cuda")
     if low is not None:
-        with torch.autocast(hidden.device.type, enabled=False):
+        with torch.autocast("cuda", enabled=False):
             hidden, weight = hidden.to(low), weight.to(low)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return LinearCrossEntropyFn.apply(hidden, weight, labels, int(ignore_index), reduction)
