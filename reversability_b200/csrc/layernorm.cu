@@ -22,6 +22,10 @@
 // do the column sums of the backward. At the end warps of a CTA add their
 // sums in shared memory, CTAs leave one partial row each and a second kernel
 // adds those in a fixed order: no atomics, the same bits every run.
+//
+// 32768 x 1024 bf16: forward 28 us (4.8 TB/s), backward 52 + 3 us (3.9 TB/s);
+// 14848 x 256 fp32 to bf16: 5.9 and 9.3 + 3.2 us in L2; 2047 x 5001 fp32: 22.7
+// (3.6 TB/s) and 35 + 5.6 us (3.5 TB/s; by single elements 33 and 80 + 5).
 #include "vec.cuh"
 
 namespace rk {
