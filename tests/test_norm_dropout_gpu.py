@@ -393,3 +393,12 @@ def test_kernels_run_on_the_stream_that_is_current():
     y2 = fx.layer_norm(fx.dropout(leaf, 0.1, 5))
     assert torch.equal(y, y2) and torch.equal(dx, torch.autograd.grad(y2, leaf, g)[0])
     assert fn is not None and _lib.device_status() == 0
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 16, device=DEV, requires_grad=True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    for y in (fx.layer_norm(x, w), fx.dropout(x, 0.5, 3)):
+        dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
