@@ -76,6 +76,30 @@ struct CeArgs {
   const float2* rowc;  // DLOGITS: per listed row (-lse log2 e, factor of dz)
   const float* scale;  // OUTER_T
   unsigned int* status;
+  // STATS with loss set (few rows): the last CTA to finish joins the rows and writes lse and loss
+  int* head;
+  const int *pos, *rows_of;
+  float *lse, *loss;
+  int rows, reduction;
+};
+constexpr int kFewRows = 32;
+
+// A row's sum of exponentials relative to 2^m. A sum without a reference (m = -inf) is 0, or not a number.
+struct RowSum {
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ void add(float2 p) {
+    if (p.x > m) {
+      s *= m == -INFINITY ? 1.f : ex2_approx(m - p.x);
+      m = p.x;
+    }
+    s += p.x == -INFINITY ? p.y : p.y * ex2_approx(p.x - m);
+  }
+  __device__ __forceinline__ void add_lanes() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      add(make_float2(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o)));
+  }
+  __device__ __forceinline__ double lse() const { return (double)m * 0.6931471805599453 + (double)logf(s); }
 };
 
 constexpr int kPairs = 74;  // CTA pairs of a B200's 148 SMs
@@ -262,6 +286,50 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
+}
+
+// The end of a forward over at most kFewRows rows: the last CTA joins each row's partial pairs, a warp a row, and adds the
+// losses. (A kernel of its own costs a launch and 4 us more of 25.)
+__device__ __noinline__ void join_few_rows(const CeArgs& g) {
+  __shared__ float row_loss[kFewRows];
+  __shared__ int is_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    is_last = atomicAdd(g.head + 1, 1) == (int)gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!is_last) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int count = *g.count, pairs = g.count[2] * 4;
+  for (int r = warp; r < kFewRows; r += kCeThreads / 32) {
+    float l = 0.f;
+    if (r < count) {
+      RowSum a;
+#pragma unroll 4
+      for (int k = lane; k < pairs; k += 32) a.add(__ldcg(g.part + k * kTile + r));
+      a.add_lanes();
+      const double total = a.lse();
+      l = (float)(total - (double)__ldcg(g.xlabel + r));
+      if (lane == 0) {
+        g.lse[r] = (float)total;
+        if (g.reduction == 0) g.loss[g.rows_of[r]] = l;
+      }
+    }
+    if (lane == 0) row_loss[r] = l;
+  }
+  if (g.reduction == 0) {
+    if ((int)threadIdx.x < g.rows && g.pos[threadIdx.x] < 0) g.loss[threadIdx.x] = 0.f;
+    return;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    double a = (double)row_loss[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (lane == 0) g.loss[0] = (float)(g.reduction == 2 && count ? a / count : a);
+  }
 }
 
 template <int MODE, typename T>
@@ -536,6 +604,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     }
     if (MODE != STATS && lane == 0) stores_done();
   }
+  if constexpr (MODE == STATS) {
+    if (g.loss) join_few_rows(g);
+  }
 
   __syncthreads();
   if (*s_abort && threadIdx.x == 0) {
@@ -557,6 +628,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 }
 
 // ---------------------------------------------------------------- rows
+// One row of 16-bit elements to a 16-byte boundary, by a warp. The source may start anywhere: a vector of the result is cut
+// out of the two aligned ones that hold it, unless those reach behind the array's end or before its start.
+__device__ __forceinline__ void copy_row(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst, int width,
+                                         const uint16_t* first, const uint16_t* end) {
+  const int shift = (int)(reinterpret_cast<uintptr_t>(src) & 15) / 2;  // elements behind a boundary
+  for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) {
+    const uint16_t* lo = src + c - shift;
+    if (lo >= first && lo + (shift ? 16 : 8) <= end) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(lo));
+      uint4 o = a;
+      if (shift) {
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(lo) + 1);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t x = 0, y = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)  // words (shift / 2 + k) and the one behind it
+            if (q == shift >> 1) {
+              x = w[q + k];
+              y = w[q + k + 1];
+            }
+          r[k] = shift & 1 ? __funnelshift_r(x, y, 16) : x;
+        }
+        o = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+      *reinterpret_cast<uint4*>(dst + c) = o;  // the pitch has room for whole vectors
+    } else {
+      for (int e = 0; e < 8 && c + e < width; ++e) dst[c + e] = src[c + e];
+    }
+  }
+}
+
+// Hidden states that the listing kernel gathers itself (forward, few rows; rows behind the last are left as they are: a
+// row's logits depend on no other row).
+struct FewRows {
+  const uint16_t* x;  // null: not this kernel's business
+  int64_t ldx, pitch;
+  int width, in_place_rows;
+  uint16_t* out;
+};
+
 // CTAS CTAs (one, or a cluster) list the rows whose label counts: pos[r] = place in the list or -1, label[i] and
 // rows_of[i] of listed row i. Labels outside [0, vocab) that are not ignore_index set an error bit and count as ignored.
 // Each warp has its share of the rows and reads it twice, to count and to write; a row's place is the number of those
@@ -564,7 +678,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 template <int CTAS>
 __global__ void __launch_bounds__(1024)
     ce_list_kernel(const int64_t* __restrict__ labels, int64_t rows, int64_t vocab, int64_t ignore, int* __restrict__ head,
-                   int* __restrict__ pos, int* __restrict__ label, int* __restrict__ rows_of, unsigned int* status) {
+                   int* __restrict__ pos, int* __restrict__ label, int* __restrict__ rows_of, unsigned int* status,
+                   const FewRows few) {
   pdl_trigger();
   pdl_wait();  // inputs are the previous kernel's outputs
   __shared__ int sums[32];
@@ -632,40 +747,13 @@ __global__ void __launch_bounds__(1024)
       head[2] = segments;
     }
   }
-  if constexpr (CTAS > 1) cluster_sync();  // the others may still read this CTA's total
-}
-
-// One row of 16-bit elements to a 16-byte boundary, by a warp. The source may start anywhere: a vector of the result is cut
-// out of the two aligned ones that hold it, unless those reach behind the array's end or before its start.
-__device__ __forceinline__ void copy_row(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst, int width,
-                                         const uint16_t* first, const uint16_t* end) {
-  const int shift = (int)(reinterpret_cast<uintptr_t>(src) & 15) / 2;  // elements behind a boundary
-  for (int c = (threadIdx.x & 31) * 8; c < width; c += 256) {
-    const uint16_t* lo = src + c - shift;
-    if (lo >= first && lo + (shift ? 16 : 8) <= end) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(lo));
-      uint4 o = a;
-      if (shift) {
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(lo) + 1);
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        uint32_t r[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t x = 0, y = 0;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)  // words (shift / 2 + k) and the one behind it
-            if (q == shift >> 1) {
-              x = w[q + k];
-              y = w[q + k + 1];
-            }
-          r[k] = shift & 1 ? __funnelshift_r(x, y, 16) : x;
-        }
-        o = make_uint4(r[0], r[1], r[2], r[3]);
-      }
-      *reinterpret_cast<uint4*>(dst + c) = o;  // the pitch has room for whole vectors
-    } else {
-      for (int e = 0; e < 8 && c + e < width; ++e) dst[c + e] = src[c + e];
-    }
+  if constexpr (CTAS > 1) {
+    cluster_sync();  // the others may still read this CTA's total
+  } else if (few.x && all != few.in_place_rows) {
+    __syncthreads();
+    const uint16_t* behind = few.x + (rows - 1) * few.ldx + few.width;
+    for (int i = warp; i < all; i += 32)
+      copy_row(few.x + (int64_t)rows_of[i] * few.ldx, few.out + i * few.pitch, few.width, few.x, behind);
   }
 }
 
@@ -738,40 +826,27 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   const int tiles_m = (count + kTile - 1) / kTile;
   const int pairs = head[2] * 4;
   const int64_t r = (int64_t)blockIdx.x * 32 + lane;  // listed row; also a row whose loss is cleared if it is not
-  float m = -INFINITY, s = 0.f;
-  // adds a pair to (m, s); a sum without a reference is 0, or not a number
-  auto join = [&](float2 p) {
-    if (p.x > m) {
-      s *= m == -INFINITY ? 1.f : ex2_approx(m - p.x);
-      m = p.x;
-    }
-    s += p.x == -INFINITY ? p.y : p.y * ex2_approx(p.x - m);
-  };
   if (pairs <= 64) {
+    RowSum a;
     if (r < count) {
       const int mt = (int)r / kTile, local = (int)r - mt * kTile;
 #pragma unroll 4
       for (int k = warp; k < pairs; k += 8)
-        join(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
+        a.add(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
     }
-    joined[warp][lane] = make_float2(m, s);
+    joined[warp][lane] = make_float2(a.m, a.s);
   } else {  // few rows with many pairs each: a warp takes four rows, lanes are pairs
     for (int e = 0; e < 4; ++e) {
       const int64_t row = (int64_t)blockIdx.x * 32 + warp * 4 + e;
-      m = -INFINITY;
-      s = 0.f;
+      RowSum a;
       if (row < count) {
         const int mt = (int)row / kTile, local = (int)row - mt * kTile;
 #pragma unroll 4
         for (int k = lane; k < pairs; k += 32)
-          join(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
+          a.add(part[(((int64_t)(k >> 2) * tiles_m + mt) * 4 + (k & 3)) * kTile + local]);
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float2 p = make_float2(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
-        join(p);
-      }
-      if (lane == 0) joined[0][warp * 4 + e] = make_float2(m, s);
+      a.add_lanes();
+      if (lane == 0) joined[0][warp * 4 + e] = make_float2(a.m, a.s);
       if (lane < 7) joined[1 + lane][warp * 4 + e] = make_float2(-INFINITY, 0.f);
     }
   }
@@ -779,16 +854,10 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   double l = 0.0;
   if (warp == 0) {
     if (r < count) {
-      m = -INFINITY;
+      RowSum a;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, joined[k][lane].x);
-      s = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float2 p = joined[k][lane];
-        s += p.x == -INFINITY ? p.y : p.y * ex2_approx(p.x - m);
-      }
-      const double total = (double)m * 0.6931471805599453 + (double)logf(s);
+      for (int k = 0; k < 8; ++k) a.add(joined[k][lane]);
+      const double total = a.lse();
       const float row_loss = (float)(total - (double)xlabel[r]);
       lse[r] = (float)total;
       if (reduction == 0) loss[rows_of[r]] = row_loss;
@@ -800,15 +869,13 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   if (warp == 0) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0 && gridDim.x == 1) loss[0] = (float)(reduction == 2 && count ? l / count : l);
-    if (lane == 0 && gridDim.x > 1) {
+    if (lane == 0) {
       sums[blockIdx.x] = l;
       __threadfence();
       is_last = atomicAdd(head + 1, 1) == (int)gridDim.x - 1;
       __threadfence();
     }
   }
-  if (gridDim.x == 1) return;
   __syncthreads();
   if (!is_last) return;
   double a = 0.0;
@@ -1095,9 +1162,10 @@ int weight_rows(const void*& w, int64_t& ldw, const CePlan& p, void* space, cuda
 }
 // One CTA for up to 4096 rows (its launch is the cheaper one), a cluster of eight for more.
 int list_rows(const int64_t* labels, int64_t ignore, const CePlan& p, const CeKept& k, unsigned int* status,
-              cudaStream_t s) {
+              const FewRows& few, cudaStream_t s) {
   if (p.M <= 4096) {
-    rk_host::launch_k(ce_list_kernel<1>, 1, 1024, 0, s, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status);
+    rk_host::launch_k(ce_list_kernel<1>, 1, 1024, 0, s, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status,
+                      few);
     return rk_host::launch_status();
   }
   cudaLaunchConfig_t cfg = {};
@@ -1112,7 +1180,7 @@ int list_rows(const int64_t* labels, int64_t ignore, const CePlan& p, const CeKe
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, ce_list_kernel<8>, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status);
+  cudaLaunchKernelEx(&cfg, ce_list_kernel<8>, labels, p.M, p.V, ignore, k.head, k.pos, k.label, k.rows_of, status, few);
   return rk_host::launch_status();
 }
 // Whether TMA can read the hidden states themselves.
@@ -1180,10 +1248,14 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   fwd_space(p, copy_w, static_cast<char*>(workspace), &f);
   const CeKept k = kept_of(static_cast<int*>(kept), M);
   unsigned int* status = rk_host::device_status_ptr();
-  int st = list_rows(labels, ignore_index, p, k, status, s);
+  const bool in_place = readable(hidden, ldh, p), few = M <= kFewRows;
+  FewRows own{};
+  if (few)
+    own = FewRows{static_cast<const uint16_t*>(hidden), ldh, p.Kp, (int)K, in_place ? (int)M : -1,
+                  static_cast<uint16_t*>(f.x)};
+  int st = list_rows(labels, ignore_index, p, k, status, own, s);
   if (st != RK_OK) return st;
-  const bool in_place = readable(hidden, ldh, p);
-  if ((st = gather(hidden, ldh, p, k, f.x, in_place, FactorArgs{}, s)) != RK_OK) return st;
+  if (!few && (st = gather(hidden, ldh, p, k, f.x, in_place, FactorArgs{}, s)) != RK_OK) return st;
   if ((st = weight_rows(w, ldw, p, f.w, s)) != RK_OK) return st;
   CUtensorMap ta, tb, tx;
   if (!tensor_map(&ta, f.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&tb, w, K, V, ldw, dtype, kKb, kHalf))
@@ -1202,7 +1274,17 @@ extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, 
   g.xlabel = f.xlabel;
   g.label = k.label;
   g.status = status;
-  if ((st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, kPairs, s)) != RK_OK) return st;
+  if (few) {
+    g.head = k.head;
+    g.pos = k.pos;
+    g.rows_of = k.rows_of;
+    g.lse = k.lse;
+    g.loss = loss;
+    g.rows = (int)M;
+    g.reduction = reduction;
+  }
+  st = launch<STATS, __nv_bfloat16>(ta, tb, ta, tx, g, dtype, kPairs, s);
+  if (few || st != RK_OK) return st;
   rk_host::launch_k(ce_finish_kernel, (unsigned)ceil_div(M, 32), 256, 0, s, f.part, f.xlabel, k.pos,
                     k.rows_of, k.head, k.lse, M, reduction, f.sums, loss);
   return rk_host::launch_status();
