@@ -23,7 +23,8 @@ E = 2.0 ** -24
 # (rows, vocabulary, width): one of each, tile and k-block edges, several pieces, a slice of every reduction
 SHAPES = [(1, 1, 1), (1, 2, 8), (3, 7, 5), (5, 300, 33), (130, 1000, 64), (257, 4099, 72), (600, 513, 256), (1000, 2000, 328),
           (64, 50257, 256), (300, 257, 1024), (2500, 1500, 96), (40, 700, 2056), (5000, 300, 40),
-          (256, 256, 64), (512, 512, 128), (257, 257, 65), (9000, 600, 520), (3, 20000, 24)]
+          (256, 256, 64), (512, 512, 128), (257, 257, 65), (9000, 600, 520), (3, 20000, 24), (32, 900, 40),
+          (33, 900, 40), (300000, 64, 16), (20, 300, 8200)]
 
 
 def _inputs(M, V, K, dtype, seed=0, ignored=0.3):
@@ -207,6 +208,31 @@ def test_gradient_against_differences():
                 moved.append(value(*args))
             # 16-bit terms: 11 (or 6) roundings of at most 2^-8 |up p v| and the result's own
             assert abs((moved[0] - moved[1]) / (2 * step) - got.view(-1)[k]) < 0.06
+
+
+def test_a_weight_past_32_bits():
+    """More than 2^31 weight elements: losses and gradients where the last rows are labels."""
+    V, K = 4_200_001, 520
+    w = torch.empty(V, K, device=DEV, dtype=BF16).normal_(std=0.02).requires_grad_()
+    y = torch.tensor([V - 1, 5, V - 2], device=DEV)
+    x = torch.randn(3, K, device=DEV).to(BF16).requires_grad_()
+    rows = fx.linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(rows.sum(), (x, w))
+    X = x.detach().double()
+    z = torch.cat([X @ w.detach()[s:s + 300_000].double().T for s in range(0, V, 300_000)], 1)
+    lse = torch.logsumexp(z, 1)
+    assert (rows.double() - (lse - z.gather(1, y[:, None])[:, 0])).abs().max() < 1e-4
+    for s in (0, 4_129_800, V - 1000):  # 2^31 elements lie before row 4129777
+        p = torch.exp(z[:, s:s + 1000] - lse[:, None])
+        for r in range(3):
+            if s <= y[r] < s + 1000:
+                p[r, y[r] - s] -= 1
+        want = p.T @ X
+        # three terms rounded to 16 bits, and the result
+        tol = 2.0 ** -8 * (p.T.abs() @ X.abs()) + 2.0 ** -8 * want.abs() + 1e-12
+        assert ((dw[s:s + 1000].double() - want).abs() <= tol).all()
+    # dx is the mean of 4 million small rows less one row: that row, within what the others can add
+    assert ((dx.double() + w.detach()[y].double()).abs() < 0.02).all()
 
 
 def test_large_logits():

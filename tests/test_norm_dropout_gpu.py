@@ -402,3 +402,22 @@ def test_second_derivatives_are_refused():
         dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             dx.sum().backward()
+
+
+def test_layer_norm_past_32_bits():
+    """More than 2^31 elements: the last rows are those of a short call, and the column sums those of equal rows."""
+    rows, width = (1 << 21) + 5, 1024
+    x = torch.zeros(rows, width, device=DEV, dtype=BF16)
+    x[-3:] = _rows(3, width, BF16)
+    g = torch.zeros_like(x)
+    g[-3:] = _rows(3, width, BF16, seed=1)
+    w, b = _params(width, F32)
+    x.requires_grad_()
+    y = fx.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    short = x.detach()[-3:].clone().requires_grad_()
+    ys = fx.layer_norm(short, w, b)
+    sx, sw, sb = torch.autograd.grad(ys, (short, w, b), g[-3:])
+    assert torch.equal(y[-3:], ys) and torch.equal(dx[-3:], sx) and not dx[:-3].any()
+    # three terms a column, added in another order: two roundings of half an ulp each way
+    assert torch.allclose(dw, sw, rtol=0, atol=4 * E * float(sw.abs().max()) * 3) and torch.allclose(db, sb, rtol=0, atol=4 * E * 30)
