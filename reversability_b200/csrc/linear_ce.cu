@@ -53,10 +53,18 @@ constexpr uint32_t kStageBytes = 2 * kHalf * kKb * 2;  // A and B of one CTA
 __host__ __device__ constexpr uint32_t ce_out_bytes(int m) {
   return m == STATS ? 0 : (m == ADD || m == OUTER) ? kEpiWarps * 4096 : kEpiWarps * 2048;  // a box of 32 rows of 128 bytes a warp
 }
-// As many as fit. (Boxes of both chunks, 128 bytes a row, with five stages: dz of 14848 x 50257 x 256 404 us for 393.)
-__host__ __device__ constexpr int ce_stages(int m) { return m == STATS ? 7 : (m == ADD || m == OUTER) ? 5 : 6; }
-__host__ __device__ constexpr uint32_t ce_smem(int m) {
-  return 1024 + ce_stages(m) * kStageBytes + ce_out_bytes(m) + (2 * ce_stages(m) + 6) * 8 + 16;
+// Row tiles of A that stay in shared memory (STATS, DLOGITS, up to `res` k blocks): only the weight streams, half of the
+// bytes from L2, whose 10 TB/s bound these two at K = 256 otherwise.
+constexpr int kResKb = 4;
+__host__ __device__ constexpr uint32_t ce_stage_bytes(int res) { return res ? kStageBytes / 2 : kStageBytes; }
+__host__ __device__ constexpr uint32_t ce_res_bytes(int res) { return res * (kStageBytes / 2); }
+// As many stages as fit. (Boxes of both chunks, 128 bytes a row, with five stages: dz of 14848 x 50257 x 256 404 us for 393.)
+__host__ __device__ constexpr int ce_stages(int m, int res) {
+  return (int)((224 * 1024 - ce_out_bytes(m) - ce_res_bytes(res)) / ce_stage_bytes(res));
+}
+__host__ __device__ constexpr uint32_t ce_smem(int m, int res) {
+  return 1024 + ce_res_bytes(res) + ce_stages(m, res) * ce_stage_bytes(res) + ce_out_bytes(m) +
+         (2 * ce_stages(m, res) + 8) * 8 + 16;
 }
 
 struct CeArgs {
@@ -182,7 +190,7 @@ struct CeWalk {
       kb1 = (int)((int64_t)(slice + 1) * kb_all / g.slices);
     }
     n0 = nt * kTile;
-    last = nt + 1 == nt_end;
+    last = MODE == DLOGITS ? nt + 1 == g.tiles_n || unit + 1 == units : nt + 1 == nt_end;
   }
   __device__ void next(const CeArgs& g) {
     if (MODE == STATS && nt + 1 < nt_end) {
@@ -332,24 +340,30 @@ __device__ __noinline__ void join_few_rows(const CeArgs& g) {
   }
 }
 
-template <int MODE, typename T>
+template <int MODE, typename T, int RES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmX, const CeArgs g,
                    const uint32_t idesc) {
-  constexpr int STAGES = ce_stages(MODE);
+  static_assert(RES == 0 || MODE == STATS || MODE == DLOGITS, "runs of tiles with the same rows");
+  constexpr int STAGES = ce_stages(MODE, RES);
+  constexpr uint32_t STAGE = ce_stage_bytes(RES);
   constexpr bool A_MN = MODE == OUTER || MODE == OUTER_T;
   constexpr bool B_MN = MODE == ADD || A_MN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sOut = smem + STAGES * kStageBytes;
+  uint8_t* sA = smem;  // RES: the resident row tile
+  uint8_t* sRing = smem + ce_res_bytes(RES);
+  uint8_t* sOut = sRing + STAGES * STAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + ce_out_bytes(MODE));
   const uint32_t full0 = smem_u32(bars);           // first CTA: both CTAs' loads of a stage have landed
   const uint32_t empty0 = full0 + 8 * STAGES;      // each CTA: the MMAs reading a stage are done
   const uint32_t tfull0 = empty0 + 8 * STAGES;     // each CTA: accumulator b is complete
   const uint32_t tempty0 = tfull0 + 16;            // first CTA: both CTAs' epilogues have read accumulator b
   const uint32_t drain = tempty0 + 16;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  const uint32_t afull = drain + 8;                // RES, first CTA: both CTAs' resident rows have landed
+  const uint32_t aempty = afull + 8;               // RES, each CTA: the MMAs reading them are done
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 8);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_consumed = reinterpret_cast<volatile int*>(s_tmem + 2);
   const int warp = threadIdx.x >> 5;
@@ -367,6 +381,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
       mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);
     }
     mbar_init(drain, 1);
+    mbar_init(afull, 1);
+    mbar_init(aempty, 1);
     fence_mbar_init();
     *s_abort = 0;
     *s_consumed = 0;
@@ -387,7 +403,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
   pdl_trigger();  // all CTAs of this grid are resident: the next one's take the SMs as these leave them
   pdl_wait();  // inputs are the previous kernels' outputs
 
-  int issued = 0;
+  int issued = 0, issued_a = 0;
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ producer (each CTA its own halves)
     // hidden states: gathered, or themselves where every row is listed
@@ -398,19 +414,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     uint32_t phase = 0;
     bool ok = true;
     for (CeWalk<MODE> w(g, pair, pairs); w.more() && ok; w.next(g)) {
+      if (RES && w.first) {  // new rows, once the products of the last ones are done
+        ok = mbar_wait(aempty, (uint32_t)(issued_a & 1) ^ 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
+        if (!ok) break;
+        if (rank == 0) mbar_arrive_expect_tx(afull, 2 * w.kb1 * kHalf * kKb * 2);
+        for (int kb = 0; kb < w.kb1; ++kb)
+          tma_load_pair(smem_u32(sA + kb * kHalf * kKb * 2), mapA, leader_addr(afull), kb * kKb, w.m0 + rank * kHalf);
+        ++issued_a;
+      }
       for (int kb = w.kb0; kb < w.kb1; ++kb) {
         if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort)) {
           ok = false;
           break;
         }
         const uint32_t fb = leader_addr(full0 + 8 * stage);
-        if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * kStageBytes);
-        const uint32_t a = smem_u32(smem + stage * kStageBytes), b = a + kHalf * kKb * 2;
+        if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * STAGE);
+        const uint32_t a = smem_u32(sRing + stage * STAGE), b = RES ? a : a + kHalf * kKb * 2;
         const int k0 = kb * kKb, ra = w.m0 + rank * kHalf, rb = w.n0 + rank * kHalf;
         if constexpr (A_MN) {
           tma_load_pair(a, mapA, fb, ra, k0);
           tma_load_pair(a + 8192, mapA, fb, ra + 64, k0);
-        } else {
+        } else if constexpr (RES == 0) {
           tma_load_pair(a, mapA, fb, k0, ra);
         }
         if constexpr (B_MN) {
@@ -432,12 +456,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
       const int at = issued - 1 - i;
       ok = mbar_wait(empty0 + 8 * (at % STAGES), (uint32_t)((at / STAGES) & 1), g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
     }
+    if (RES && ok && issued_a) mbar_wait(aempty, (uint32_t)(issued_a - 1) & 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
   } else if (warp == 1 && lane == 0 && rank == 0) {
     // ------------------------------------------------------------ MMA issuer (the pair's first CTA)
     int stage = 0, acc = 0, consumed = 0;
-    uint32_t phase = 0, acc_phase = 0;
+    uint32_t phase = 0, acc_phase = 0, a_phase = 0;
     bool ok = true;
     for (CeWalk<MODE> w(g, pair, pairs); w.more() && ok; w.next(g)) {
+      if (RES && w.first) {
+        ok = mbar_wait(afull, a_phase, g.status, RK_DEV_GEMM_TIMEOUT, s_abort);
+        if (!ok) break;
+        a_phase ^= 1;
+      }
       if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, g.status, RK_DEV_GEMM_TIMEOUT, s_abort)) {
         ok = false;
         break;
@@ -451,7 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
         }
         ++consumed;
         tc_fence_after();
-        const uint32_t a = smem_u32(smem + stage * kStageBytes), b = a + kHalf * kKb * 2;
+        const uint32_t ring = smem_u32(sRing + stage * STAGE);
+        const uint32_t a = RES ? smem_u32(sA + kb * kHalf * kKb * 2) : ring, b = RES ? ring : ring + kHalf * kKb * 2;
 #pragma unroll
         for (int j = 0; j < kKb / 16; ++j) {
           const uint64_t ad = A_MN ? smem_desc_sw128(a + j * 2048, 8192, 1024) : smem_desc_sw128(a + j * 32, 16, 1024);
@@ -466,6 +497,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
       }
       if (!ok) break;
       umma_commit_pair(tfull0 + 8 * acc);
+      if (RES && w.last) umma_commit_pair(aempty);
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -612,6 +644,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
   if (*s_abort && threadIdx.x == 0) {
     // Loads in flight land before shared memory is given up. The first CTA's barriers count both CTAs' loads; loads
     // that its barriers no longer follow land within the time waited here.
+    if (RES && rank == 0 && issued_a)
+      mbar_wait(afull, (uint32_t)(issued_a - 1) & 1, g.status, RK_DEV_GEMM_TIMEOUT, nullptr);
     if (rank == 0)
       for (int i = *s_consumed; i < issued; ++i)
         mbar_wait(full0 + 8 * (i % STAGES), (uint32_t)((i / STAGES) & 1), g.status, RK_DEV_GEMM_TIMEOUT, nullptr);
@@ -1126,15 +1160,18 @@ int64_t bwd_space(const CePlan& p, bool copy_w, char* base, BwdSpace* b) {
   return a.at;
 }
 
-template <int MODE, typename T>
+template <int MODE, typename T, int RES = 0>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CUtensorMap& tx, const CeArgs& g,
            int dtype, int64_t tiles, cudaStream_t s) {
   constexpr bool a_mn = MODE == OUTER || MODE == OUTER_T, b_mn = MODE == ADD || a_mn;
-  static_assert(ce_smem(MODE) <= 232448, "shared memory over the per-block limit");
-  auto kern = ce_gemm_kernel<MODE, T>;
-  if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)ce_smem(MODE))) return e;
+  constexpr uint32_t smem = ce_smem(MODE, RES);
+  static_assert(smem <= 232448 - 256, "shared memory over the per-block limit");
+  if constexpr (RES == 0 && (MODE == STATS || MODE == DLOGITS))
+    if (g.kb <= kResKb) return launch<MODE, T, kResKb>(ta, tb, tc, tx, g, dtype, tiles, s);
+  auto kern = ce_gemm_kernel<MODE, T, RES>;
+  if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
   const int pairs = tiles < kPairs ? (int)tiles : kPairs;
-  rk_host::launch_k(kern, 2 * pairs, kCeThreads, ce_smem(MODE), s, ta, tb, tc, tx, g,
+  rk_host::launch_k(kern, 2 * pairs, kCeThreads, smem, s, ta, tb, tc, tx, g,
                     idesc_f16(kTile, kTile, dtype == RK_BF16 ? 1 : 0, a_mn ? 1 : 0, b_mn ? 1 : 0));
   return rk_host::launch_status();
 }
