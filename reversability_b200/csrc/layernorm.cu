@@ -440,7 +440,7 @@ using namespace rk;
 
 namespace {
 
-constexpr int kMaxWidth = 16384;  // 32 elements a thread, 512 threads
+constexpr int kMaxWidth = 16384;  // 32 elements a thread, 512 threads (from the boundary before a row to the one behind)
 constexpr int kWarpWidth = 1024;  // 32 elements a lane
 constexpr int kCtaWidth = 8192;   // 16 elements a thread, 512 threads
 
@@ -578,6 +578,7 @@ extern "C" int rk_layernorm_fwd(const void* x, int x_dtype, int64_t ldx, const v
   a.rows = rows;
   a.width = (int)width;
   a.span = row_span(x, ldx, x_dtype, rows, width);
+  if (a.span > kMaxWidth) return RK_ERR_UNSUPPORTED;
   a.eps = eps;
   a.s = static_cast<cudaStream_t>(stream);
   return dispatch_types(a, x_dtype, y_dtype);
@@ -620,6 +621,7 @@ extern "C" int rk_layernorm_bwd(const void* x, int x_dtype, int64_t ldx, const v
     a.rows = rows;
     a.width = (int)width;
     a.span = row_span(x, ldx, x_dtype, rows, width);
+    if (a.span > kMaxWidth) return RK_ERR_UNSUPPORTED;
     a.s = s;
     parts = (int)bwd_ctas(rows, a.span);
     const int st = dispatch_types(a, x_dtype, dy_dtype);

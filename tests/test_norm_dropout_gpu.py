@@ -19,7 +19,8 @@ E = 2.0 ** -24
 # (rows, width): one element, warp, vector and CTA edges, more rows than the backward has CTAs, the widest
 SHAPES = [(1, 1), (3, 2), (5, 7), (9, 8), (17, 31), (33, 256), (70, 257), (10, 1000), (6, 1024), (5, 1025), (3, 4097),
           (3, 8192), (2, 16384), (5000, 333), (7000, 64), (1500, 768), (700, 1536),
-          (100, 1017), (100, 1019), (1400, 1501), (310, 5003), (160, 8191), (150, 10007)]
+          (100, 1017), (100, 1019), (1400, 1501), (310, 5003), (160, 8191), (150, 10007),
+          (3, 16377), (300, 8185)]
 
 
 def _rows(rows, width, dtype, layout="plain", seed=0, shift=0.5):
@@ -204,8 +205,9 @@ def test_layer_norm_refusals():
                        (lambda: fx.layer_norm(x, w.cpu()), "CUDA")):
         with pytest.raises(ValueError, match=match):
             bad()
-    with pytest.raises(RuntimeError, match="rk_layernorm_fwd"):
-        fx.layer_norm(torch.randn(2, 16385, device=DEV))
+    for width in (16385, 16383):  # the second reaches over more than 16384 elements between boundaries
+        with pytest.raises(RuntimeError, match="rk_layernorm_fwd"):
+            fx.layer_norm(torch.randn(2, width, device=DEV, dtype=BF16))
 
 
 def test_enable_layernorm_routes_modules():
