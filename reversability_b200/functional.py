@@ -514,7 +514,7 @@ def _linear_ce_check(hidden, weight, labels, reduction):
         raise ValueError("the head loss takes hidden [..., d] and a non-empty weight [vocabulary, d]")
     if hidden.dtype != weight.dtype or hidden.dtype not in _lib.DTYPE_CODE:
         raise ValueError("hidden and weight must share a type: fp32, bf16 or fp16")
-    if labels.dtype != torch.int64 or labels.shape != hidden.shape[:-1]:
+    if labels.dtype is not torch.int64 or labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels must be int64 of shape {tuple(hidden.shape[:-1])}")
     _on_current_device(hidden, "hidden", weight, labels)
 
@@ -561,8 +561,10 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
     """(d hidden, d weight) for the loss's gradient (a device scalar; one a row with reduction "none"), in the inputs'
     types unless others are given; None where not wanted."""
     V, K = weight.shape
-    grad = grad.detach().float().contiguous()
-    if grad.device != hidden.device or grad.numel() != (hidden.shape[:-1].numel() if reduction == "none" else 1):
+    if grad.dtype is not torch.float32 or not grad.is_contiguous():
+        grad = grad.detach().float().contiguous()
+    if grad.get_device() != hidden.get_device() or \
+            grad.numel() != (hidden.shape[:-1].numel() if reduction == "none" else 1):
         raise ValueError("the loss's gradient must be on hidden's device, one number or one a row")
     dx = _new(hidden, dx_dtype or hidden.dtype) if want_dx else None
     dw = _new(weight, dw_dtype or weight.dtype) if want_dw else None
@@ -572,7 +574,7 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
     x, M, _, ld = even_rows(hidden)
     w, ldw, copy_w = _head_weight(weight)
     n_ws = _linear_ce_bytes(M, V, K, copy_w)[2]
-    ws = torch.empty(n_ws, device=hidden.device, dtype=torch.uint8)
+    ws = hidden.new_empty(n_ws, dtype=torch.uint8)
     _lib.call("rk_linear_ce_bwd", x.data_ptr(), ld, w.data_ptr(), ldw, kept.data_ptr(), M, V, K,
               _lib.code(hidden.dtype), _REDUCTIONS[reduction], grad.data_ptr(), _lib.ptr(dx), K,
               _lib.code(dx.dtype) if want_dx else 0, _lib.ptr(dw), K, _lib.code(dw.dtype) if want_dw else 0,
