@@ -24,13 +24,15 @@
 // warps a CTA. The gradient products keep the tensor pipe 86 to 88 % busy; at
 // K = 256 the two with exponentials in their epilogue keep it and the
 // exponential unit, both with 2048 cycles of work a tile, 65 and 53 % busy
-// (292 us forward, 393 us for dz at 14848 x 50257). Sums over sliced reductions
-// are added in a fixed order: no atomics, the same bits every run.
+// (290 us forward, 390 us for dz at 14848 x 50257). Not faster there: two groups
+// of warps on alternate tiles (300), a part of the exponentials as polynomials
+// on the FMA pipes (311 to 328). Sums over sliced reductions are added in a
+// fixed order: no atomics, the same bits every run.
 //
-// Whole passes, forward and backward: 14848 x 50257 x 256 bf16 1.56 ms (1.53
-// TFLOP with the logits formed twice: 980 TFLOP/s), 32768 x 50257 x 1024 10.9
+// Whole passes, forward and backward: 14848 x 50257 x 256 bf16 1.57 ms (1.53
+// TFLOP with the logits formed twice: 975 TFLOP/s), 32768 x 50257 x 1024 10.9
 // ms (1237 TFLOP/s under the power cap, where plain products reach 1391), 3001 x
-// 32003 x 328 fp16 with half of the rows ignored 0.23 ms, one row forward 25 us.
+// 32003 x 328 fp16 with half of the rows ignored 0.23 ms, one row forward 23 us.
 #include <cudaTypedefs.h>
 #include <mutex>
 #include <type_traits>
@@ -54,7 +56,7 @@ __host__ __device__ constexpr uint32_t ce_out_bytes(int m) {
   return m == STATS ? 0 : (m == ADD || m == OUTER) ? kEpiWarps * 4096 : kEpiWarps * 2048;  // a box of 32 rows of 128 bytes a warp
 }
 // Row tiles of A that stay in shared memory (STATS, DLOGITS, up to `res` k blocks): only the weight streams, half of the
-// bytes from L2, whose 10 TB/s bound these two at K = 256 otherwise.
+// bytes from L2 (14848 x 50257 x 256 1.60 -> 1.57 ms a pass; in short runs, at full clocks, no faster).
 constexpr int kResKb = 4;
 __host__ __device__ constexpr uint32_t ce_stage_bytes(int res) { return res ? kStageBytes / 2 : kStageBytes; }
 __host__ __device__ constexpr uint32_t ce_res_bytes(int res) { return res * (kStageBytes / 2); }
