@@ -2,6 +2,7 @@
 
     python -m reversability_b200.microbench [--only NAME[,NAME...]] [--iters N]
     python -m reversability_b200.microbench --only versus      (cuBLAS / torch SDPA arms beside librevk)
+    python -m reversability_b200.microbench --only lean        (layer norm, dropout, head loss in pieces of the vocabulary)
     python -m reversability_b200.microbench --only api --iters 20   (the reference API's training paths on this package)
     python -m reversability_b200.microbench --only head|attention|swiglu|membound|gemms --profile   (ncu launch sequence)
 
@@ -9,7 +10,8 @@ Workload: 16,896 tokens x width 256 in bf16 (activations N(0,1), weights
 N(0,0.02)); RMSNorm fwd+bwd, SwiGLU fwd+bwd (gate/up 256->1024, i.e. u is
 [N, 2048], h is [N, 1024]), the MLP GEMMs 256->2048->256 forward and backward,
 and the midpoint reconstruct step x_prev = x_next - 2h*F on fp32 residuals
-N(0,1) (2h = 1, fp32 force). Also the cfg2 head GEMM and attention.
+N(0,1) (2h = 1, fp32 force). Also the cfg2 head GEMM and attention, and the
+lean training operators at their own sizes.
 
 Each kernel is launched `iters` times from one captured CUDA graph, cycling
 through enough input/output buffer sets that every launch misses L2 (sets
@@ -252,6 +254,41 @@ def bench_attention(iters):
             ("tensor", "attention_bwd", int(2.5 * flops), time_graph(bwd, 1, iters))]
 
 
+def bench_lean(iters):
+    """Layer norm, dropout and the head loss without logits, each direction on its own: the 20.3M decoder's microbatch
+    (14,848 tokens of width 256, 50,257 words) and the scaled decoder's (32,768 of 1024; MLP width 4096), bf16."""
+    for rows, width, dt in ((14848, 256, torch.float32), (32768, 1024, torch.bfloat16)):
+        size = 4 if dt == torch.float32 else 2
+        n = rows * width
+        ns = sets_for(n * (size + 2))
+        w, b = torch.ones(width, device="cuda"), torch.zeros(width, device="cuda")
+        xs = [torch.randn(rows, width, device="cuda").to(dt) for _ in range(ns)]
+        gs = [torch.randn(rows, width, device="cuda").bfloat16() for _ in range(ns)]
+        stats = [fn.layernorm_fwd(x, w, b, 1e-5, torch.bfloat16)[1] for x in xs]
+        tag = f"{rows}x{width} {str(dt)[6:]} in, bf16 out"
+        yield "hbm", f"layernorm_fwd {tag}", n * (size + 2), time_graph(
+            lambda k: fn.layernorm_fwd(xs[k], w, b, 1e-5, torch.bfloat16), ns, iters)
+        yield "hbm", f"layernorm_bwd {tag}", n * (2 * size + 2), time_graph(
+            lambda k: fn.layernorm_bwd(xs[k], w, stats[k], gs[k]), ns, iters)
+        if dt == torch.float32:
+            yield "hbm", f"dropout of bf16 onto fp32 {rows}x{width}", n * 10, time_graph(
+                lambda k: fn.dropout(gs[k], 0.1, 7, 1, xs[k]), ns, iters)
+        del xs, gs, stats
+    x = [torch.randn(32768, 4096, device="cuda").bfloat16() for _ in range(2)]
+    yield "hbm", "dropout 32768x4096 bf16", 2 * 2 * x[0].numel(), time_graph(lambda k: fn.dropout(x[k], 0.2, 7), 2, iters)
+    del x
+    for M, K in ((14848, 256), (32768, 1024)):
+        V = 50257
+        h = torch.randn(M, K, device="cuda").bfloat16()
+        w = (torch.randn(V, K, device="cuda") * (2 / K ** 0.5)).bfloat16()
+        y = torch.randint(0, V, (M,), device="cuda")
+        kept, one = fn.linear_ce_fwd(h, w, y)[1], torch.ones((), device="cuda")
+        flops, few = 2 * M * V * K, min(iters, 10)
+        yield "tensor", f"linear_ce_fwd {M}x{V}x{K}", flops, time_graph(lambda k: fn.linear_ce_fwd(h, w, y), 1, few)
+        yield "tensor", f"linear_ce_bwd {M}x{V}x{K} (logits again, both gradients)", 3 * flops, time_graph(
+            lambda k: fn.linear_ce_bwd(h, w, kept, one), 1, few)
+
+
 def bench_versus(iters):
     """Same-box comparison arms for the library calls the reference makes at
     these shapes (model.py:37,45,55-56 F.linear -> cuBLAS; model.py:42-44
@@ -330,7 +367,8 @@ def bench_versus(iters):
 
 
 BENCHES = {"rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "reconstruct": bench_reconstruct,
-           "mlp_gemms": bench_mlp_gemms, "head": bench_head, "attention": bench_attention, "versus": bench_versus}
+           "mlp_gemms": bench_mlp_gemms, "head": bench_head, "attention": bench_attention, "lean": bench_lean,
+           "versus": bench_versus}
 
 
 def profile_head():
