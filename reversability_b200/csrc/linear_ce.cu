@@ -592,7 +592,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
             for (int k = 0; k < 32; ++k)
               if (li == k) v[k] -= rc.y;
           }
-          const int valid = g.vocab - (g.v0 + c0);
+          // rows behind the last are zeros also where an infinite weight makes their products something else
+          const int valid = label < 0 ? 0 : g.vocab - (g.v0 + c0);
           if (valid < 32) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)

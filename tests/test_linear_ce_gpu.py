@@ -244,6 +244,26 @@ def test_large_logits():
     _check(x, w, y, torch.ones(300, device=DEV), rows, dx, dw)
 
 
+@pytest.mark.parametrize("rows", [3, 300, 512])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_an_entry_of_minus_infinity(dtype, rows):
+    """An entry whose logits are -inf is as one whose exponentials underflow, also where rows of zeros pad a tile."""
+    x, w, y = _inputs(rows, 600, 64, dtype)
+    x = x.detach()
+    x[:, 0] = 1 + x[:, 0].abs()
+    y = torch.where(y == 5, 6, y)
+    got = []
+    for entry in (-float("inf"), -30000.0):
+        v = w.detach().clone()
+        v[5] = 0
+        v[5, 0] = entry
+        v.requires_grad_()
+        loss = fx.linear_cross_entropy(x, v, y)
+        got.append((loss.detach(), torch.autograd.grad(loss, v)[0]))
+    assert torch.isfinite(got[0][1]).all()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 def test_results_are_the_same_bits_every_run():
     x, w, y = _inputs(3000, 5000, 264, BF16)
     runs = []
