@@ -135,10 +135,10 @@ class LayerNormFn(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """F.layer_norm over the last dimension (at most 16384 wide, 16377 if the width is no multiple of 8): statistics in fp32, weight and bias (each may be
-    None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise (any type for fp32 x, fp32 for
-    16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in its input's type under
-    autocast. The gradients of weight and bias are sums in a fixed order."""
+    """F.layer_norm over the last dimension (at most 16384 wide, 16377 if the width is no multiple of 8): statistics in
+    fp32, weight and bias (each may be None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise
+    (any type for fp32 x, fp32 for 16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in
+    its input's type under autocast. The gradients of weight and bias are sums in a fixed order."""
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
