@@ -4,15 +4,22 @@
 //   dx = s (g w - mean(g w) - n mean(g w n)),  dw = sum_rows g n,  db = sum_rows g
 //
 // Bound by memory: forward x in and y out, backward x and dy in and dx out; a
-// row is read once. Rows of up to 1024 elements belong to a warp, wider ones
-// to a CTA with 16 (from 8192 on 32) elements a thread; warps (CTAs) walk over
-// rows, and each lane copies its own elements of the next rows into shared
-// memory asynchronously while the current row is summed, the mean first and
-// then the squares about it, so a large mean costs no digits. (With rows loaded
-// into registers as they were needed the backward of 32768 x 1024 bf16 took
-// 152 us: eight warps an SM, each waiting for its row.) Arithmetic is on pairs
-// (fp32x2), or instructions would bound it: 16-bit rows leave some 14 of them
-// an element at full bandwidth, forward, and 20 backward.
+// row is read once. Forward, rows of up to 1024 elements belong to a warp,
+// wider ones to a CTA with 16 (from 8192 on 32) elements a thread. Backward, a
+// thread has at most 16 elements up to 8192 wide: a warp's row to 512, two
+// warps' to 1024, four warps' to 2048, then a CTA's; so the column sums, x and
+// dy of a row fit in registers, and a row is not read and formed again after
+// its sums (32768 x 1024 bf16 on one warp and read twice 52 us, on two and kept
+// 40; 512 wide 36 and 26; 8192 x 2048 on CTAs 36, on four warps, which leave
+// half as many partial rows, 27). Forward rows on two or four warps were no
+// faster. Warps (CTAs) walk over rows, and each lane copies its own elements of
+// the next rows into shared memory asynchronously while the current row is
+// summed, the mean first and then the squares about it, so a large mean costs
+// no digits. (With rows loaded into registers as they were needed the backward
+// of 32768 x 1024 bf16 took 152 us: eight warps an SM, each waiting for its
+// row.) Arithmetic is on pairs (fp32x2), or instructions would bound it: 16-bit
+// rows leave some 14 of them an element at full bandwidth, forward, and 20
+// backward, about what a row formed twice takes.
 //
 // A lane's elements are vectors of 16 bytes of x at 16-byte boundaries, also
 // where rows start between those: then the first and last vector of a row are
@@ -23,9 +30,9 @@
 // sums in shared memory, CTAs leave one partial row each and a second kernel
 // adds those in a fixed order: no atomics, the same bits every run.
 //
-// 32768 x 1024 bf16: forward 28 us (4.8 TB/s), backward 52 + 3 us (3.9 TB/s);
-// 14848 x 256 fp32 to bf16: 5.9 and 9.3 + 3.2 us in L2; 2047 x 5001 fp32: 22.7
-// (3.6 TB/s) and 35 + 5.6 us (3.5 TB/s; by single elements 33 and 80 + 5).
+// 32768 x 1024 bf16: forward 27 us (5.0 TB/s), backward with its columns 41 us
+// (4.9 TB/s); 14848 x 256 fp32 to bf16: 5.9 and 11.9 us in L2; 2047 x 5001
+// fp32: 22.9 (3.6 TB/s) and 40 us (3.1 TB/s; by single elements 33 and 85).
 #include "vec.cuh"
 
 namespace rk {
@@ -110,17 +117,32 @@ __device__ __forceinline__ void store_part(T* __restrict__ row, bool edge, int c
   }
 }
 
-// Sums over the row's threads, the same values in all of them. CTA rows: one barrier; `red` is one of several buffers
+// Sums over the row's threads (W warps; 0: the CTA), the same values in all of them. Several warps: one barrier; `red` is one of several buffers
 // used in turn, so a buffer is written again only after a barrier that follows its last read.
-template <bool WARP, bool TWO>
+template <int W, bool TWO>
 __device__ __forceinline__ float2 row_sums(float2 v, float2* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
     if (TWO) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  if (WARP) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if (W == 1) return v;
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) red[warp] = v;
+  if constexpr (W > 1) {  // the row's warps only
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / W), "n"(32 * W) : "memory");
+    if (W == 2) {
+      const float2 o = red[warp ^ 1];
+      return make_float2(o.x + v.x, o.y + v.y);
+    }
+    v = red[warp / W * W];
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      const float2 o = red[warp / W * W + k];
+      v = make_float2(v.x + o.x, v.y + o.y);
+    }
+    return v;
+  }
   __syncthreads();
   v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x & 31] : make_float2(0.f, 0.f);
 #pragma unroll
@@ -139,28 +161,29 @@ __host__ __device__ constexpr int norm_depth(int elements, int bytes_per_element
   const int row = elements * bytes_per_element * (warp ? 256 : 512);
   return !warp && elements > 16 ? 1 : 3 * row <= 100 * 1024 ? 3 : 2;
 }
-// Parameters in registers (CTA rows of 16 elements a thread) or in shared memory, as they meet the lanes' vectors.
+// Forward: parameters in registers (CTA rows of 16 elements a thread) or in shared memory, as they meet the lanes'
+// vectors. Backward: the weight in shared memory; what its registers would hold is the row.
 __host__ __device__ constexpr bool norm_param_regs(int elements, bool warp) { return !warp && elements <= 16; }
 
 // What a thread does in every row that it visits.
-template <typename Tx, int V, int NV, bool WARP>
+template <typename Tx, int V, int NV, int W>
 struct RowWalk {
   int T, t;            // threads of a row, and this one's place
   int ph;              // elements between a row's start and the 16-byte boundary (of x) before it
   int64_t row, step;
   uint32_t edge;       // bit j: vector j lies partly outside the row
   __device__ RowWalk(const Tx* x, int64_t ldx, int width) {
-    T = WARP ? 32 : blockDim.x;
-    t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    if (WARP) {  // a CTA's rows are equal mod 8
-      row = (blockIdx.x & 7) + 8 * ((int64_t)(blockIdx.x >> 3) * 8 + (threadIdx.x >> 5));
-      step = (int64_t)gridDim.x * 8;
+    T = W ? 32 * W : blockDim.x;
+    t = W ? threadIdx.x % (32 * W) : threadIdx.x;
+    if constexpr (W > 0) {  // a CTA's rows are equal mod 8
+      row = (blockIdx.x & 7) + 8 * ((int64_t)(blockIdx.x >> 3) * (8 / W) + threadIdx.x / (32 * W));
+      step = (int64_t)gridDim.x * (8 / W);
     } else {
       row = blockIdx.x;
       step = gridDim.x;
     }
     // the CTA's first row speaks for all that it visits
-    const int64_t first = WARP ? blockIdx.x & 7 : blockIdx.x;
+    const int64_t first = W ? blockIdx.x & 7 : blockIdx.x;
     ph = (int)((reinterpret_cast<uintptr_t>(x + first * ldx) / sizeof(Tx)) % V);
     edge = 0;
 #pragma unroll
@@ -177,17 +200,17 @@ struct RowWalk {
   }
 };
 
-template <typename Tx, typename Ty, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 3) : 1)
+template <typename Tx, typename Ty, int V, int NV, int W>
+__global__ void __launch_bounds__(W ? 256 : 512, W ? (NV * V <= 16 ? 4 : 3) : 1)
     layernorm_fwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const NormParam b,
                          Ty* __restrict__ y, int64_t ldy, float2* __restrict__ stats, int64_t rows, int width,
                          float eps) {
-  constexpr int D = norm_depth(NV * V, (int)sizeof(Tx), WARP), H = V / 2;
-  constexpr bool REGS = norm_param_regs(NV * V, WARP);
+  constexpr int D = norm_depth(NV * V, (int)sizeof(Tx), W), H = V / 2;
+  constexpr bool REGS = norm_param_regs(NV * V, W);
   extern __shared__ uint4 shared[];  // [D][NV][threads] packs of x, then weight and bias, NV * T * V floats each
-  __shared__ float2 red[WARP ? 1 : 4][16];
+  __shared__ float2 red[W == 1 ? 1 : 4][16];
   pdl_wait();  // inputs are the previous kernel's outputs
-  RowWalk<Tx, V, NV, WARP> r(x, ldx, width);
+  RowWalk<Tx, V, NV, W> r(x, ldx, width);
   RowPack<Tx, V>* mine = reinterpret_cast<RowPack<Tx, V>*>(shared) + threadIdx.x;
   float2* params = reinterpret_cast<float2*>(reinterpret_cast<RowPack<Tx, V>*>(shared) + D * NV * blockDim.x);
   auto start = [&](int64_t row, int d) {
@@ -239,7 +262,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 3
 #pragma unroll
       for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][k]);
     }
-    const float mean = row_sums<WARP, false>(make_float2(sum.x + sum.y, 0.f), red[WARP ? 0 : 2 * turn]).x * inv;
+    const float mean = row_sums<W, false>(make_float2(sum.x + sum.y, 0.f), red[W == 1 ? 0 : 2 * turn]).x * inv;
     float2 sq = both(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -256,7 +279,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 3
       for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][k], v[j][k], sq);
     }
     const float rstd =
-        rsqrtf(row_sums<WARP, false>(make_float2(sq.x + sq.y, 0.f), red[WARP ? 0 : 2 * turn + 1]).x * inv + eps);
+        rsqrtf(row_sums<W, false>(make_float2(sq.x + sq.y, 0.f), red[W == 1 ? 0 : 2 * turn + 1]).x * inv + eps);
     if (stats && r.t == 0) stats[row] = make_float2(mean, rstd);
     Ty* dst = y + row * ldy;
 #pragma unroll
@@ -276,18 +299,18 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 16 ? 4 : 3
 }
 
 // partial: [gridDim.x][2][width] fp32 (dw, then db), or null when neither is wanted; dx may be null.
-template <typename Tx, typename Tg, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2) : 1)
+template <typename Tx, typename Tg, int V, int NV, int W>
+__global__ void __launch_bounds__(W ? 256 : 512, W > 1 ? 2 : W ? (NV * V <= 8 ? 3 : 2) : 1)
     layernorm_bwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const float2* __restrict__ stats,
                          const Tg* __restrict__ dy, int64_t lddy, Tx* __restrict__ dx, int64_t lddx,
                          float* __restrict__ partial, int64_t rows, int width) {
-  constexpr int D = norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), WARP), H = V / 2;
-  constexpr bool REGS = norm_param_regs(NV * V, WARP);
-  // [D][NV][threads] packs of x, then of dy, then the weight; at the end (WARP) [8][2][width] column sums
+  constexpr int D = norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), W), H = V / 2;
+  constexpr bool KEEP = NV * V <= 16;  // n and g w stay in registers over the row's sums
+  // [D][NV][threads] packs of x, then of dy, then the weight; at the end (W) [8 / W][2][width] column sums
   extern __shared__ uint4 shared[];
-  __shared__ float2 red[WARP ? 1 : 2][16];
+  __shared__ float2 red[W == 1 ? 1 : 2][16];
   pdl_wait();  // inputs are the previous kernel's outputs
-  RowWalk<Tx, V, NV, WARP> r(x, ldx, width);
+  RowWalk<Tx, V, NV, W> r(x, ldx, width);
   RowPack<Tx, V>* ring_x = reinterpret_cast<RowPack<Tx, V>*>(shared);
   RowPack<Tg, V>* ring_g = reinterpret_cast<RowPack<Tg, V>*>(ring_x + D * NV * blockDim.x);
   float2* params = reinterpret_cast<float2*>(ring_g + D * NV * blockDim.x);
@@ -317,20 +340,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
       }
 #pragma unroll
   for (int d = 0; d < D - 1; ++d) start(r.row + d * r.step, d);
-  float2 wr[REGS ? NV : 1][H];
-  if constexpr (REGS) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < H; ++k) {
-        const int c = r.col(j) + 2 * k;
-        wr[j][k] = make_float2(param_at(w, c, width, 1.f), param_at(w, c + 1, width, 1.f));
-      }
-  } else {
-    for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x)
-      params[i] = make_float2(param_at(w, r.param_col(i), width, 1.f), param_at(w, r.param_col(i) + 1, width, 1.f));
-    __syncthreads();
-  }
+  for (int i = threadIdx.x; i < NV * r.T * H; i += blockDim.x)
+    params[i] = make_float2(param_at(w, r.param_col(i), width, 1.f), param_at(w, r.param_col(i) + 1, width, 1.f));
+  __syncthreads();
   float2 dw[NV][H], db[NV][H];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -346,16 +358,23 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
     copies_wait<D - 1>();
     const float2 rs = both(st.y), mu = both(-st.x);
     float2 s1 = both(0.f), s2 = both(0.f);
+    float2 kept_n[KEEP ? NV : 1][H], kept_g[KEEP ? NV : 1][H];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {  // outside the row g = 0 (and x, but for edges of rows with a mean that is not finite)
       float2 xv[H], gv[H];
+      float2(&nk)[H] = kept_n[KEEP ? j : 0];
+      float2(&gk)[H] = kept_g[KEEP ? j : 0];
       const bool edge = r.edge >> j & 1;
       read_slot<Tx, V>(mine_x + (d * NV + j) * blockDim.x, edge, r.col(j), width, xv);
       read_slot<Tg, V>(mine_g + (d * NV + j) * blockDim.x, edge, r.col(j), width, gv);
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
-        const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[r.param(j, k)]);
+        const float2 gw = __fmul2_rn(gv[k], params[r.param(j, k)]);
+        if (KEEP) {
+          nk[k] = n;
+          gk[k] = gw;
+        }
         s1 = __fadd2_rn(s1, gw);
         s2 = __ffma2_rn(gw, n, s2);
         dw[j][k] = __ffma2_rn(gv[k], n, dw[j][k]);
@@ -363,8 +382,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
       }
     }
     if (dx) {
-      const float2 m = row_sums<WARP, true>(make_float2(s1.x + s1.y, s2.x + s2.y), red[WARP ? 0 : turn]);
-      asm volatile("" ::: "memory");  // the row is read from shared memory again: kept, its registers would spill
+      const float2 m = row_sums<W, true>(make_float2(s1.x + s1.y, s2.x + s2.y), red[W == 1 ? 0 : turn]);
+      if (!KEEP) asm volatile("" ::: "memory");  // the row is read from shared memory again: kept, it would spill
       // dx = s g w - s m1 - s m2 n
       const float2 a = both(-st.y * (m.x * inv)), c2 = both(-st.y * (m.y * inv));
       Tx* dst = dx + row * lddx;
@@ -373,12 +392,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
         if (r.col(j) >= width) break;
         float2 xv[H], gv[H];
         const bool edge = r.edge >> j & 1;
-        read_slot<Tx, V>(mine_x + (d * NV + j) * blockDim.x, false, 0, width, xv);
-        read_slot<Tg, V>(mine_g + (d * NV + j) * blockDim.x, false, 0, width, gv);
+        if (!KEEP) {
+          read_slot<Tx, V>(mine_x + (d * NV + j) * blockDim.x, false, 0, width, xv);
+          read_slot<Tg, V>(mine_g + (d * NV + j) * blockDim.x, false, 0, width, gv);
+        }
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          const float2 n = __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
-          const float2 gw = __fmul2_rn(gv[k], REGS ? wr[j][k] : params[r.param(j, k)]);
+          const float2 n = KEEP ? kept_n[KEEP ? j : 0][k] : __fmul2_rn(__fadd2_rn(xv[k], mu), rs);
+          const float2 gw = KEEP ? kept_g[KEEP ? j : 0][k] : __fmul2_rn(gv[k], params[r.param(j, k)]);
           xv[k] = __ffma2_rn(gw, rs, __ffma2_rn(n, c2, a));
         }
         store_part<Tx, V>(dst, edge, r.col(j), width, xv);
@@ -389,24 +410,24 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, WARP ? (NV * V <= 8 ? 3 : 2)
   copies_wait<0>();
   if (!partial) return;
   float* out = partial + (int64_t)blockIdx.x * 2 * width;
-  float* sums = reinterpret_cast<float*>(shared) + (threadIdx.x >> 5) * 2 * width;
-  if (WARP) __syncthreads();  // ring and weight are not read any more
+  float* sums = reinterpret_cast<float*>(shared) + threadIdx.x / (32 * (W ? W : 1)) * 2 * width;
+  if (W) __syncthreads();  // ring and weight are not read any more
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int c = r.col(j) + e;
       if ((unsigned)c < (unsigned)width) {
-        (WARP ? sums : out)[c] = e & 1 ? dw[j][e / 2].y : dw[j][e / 2].x;
-        (WARP ? sums : out)[width + c] = e & 1 ? db[j][e / 2].y : db[j][e / 2].x;
+        (W ? sums : out)[c] = e & 1 ? dw[j][e / 2].y : dw[j][e / 2].x;
+        (W ? sums : out)[width + c] = e & 1 ? db[j][e / 2].y : db[j][e / 2].x;
       }
     }
-  if (!WARP) return;
+  if (!W) return;
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += reinterpret_cast<float*>(shared)[k * 2 * width + c];
+    for (int k = 0; k < 8 / (W ? W : 1); ++k) s += reinterpret_cast<float*>(shared)[k * 2 * width + c];
     out[c] = s;
   }
 }
@@ -441,22 +462,23 @@ using namespace rk;
 namespace {
 
 constexpr int kMaxWidth = 16384;  // 32 elements a thread, 512 threads (from the boundary before a row to the one behind)
-constexpr int kWarpWidth = 1024;  // 32 elements a lane
 constexpr int kCtaWidth = 8192;   // 16 elements a thread, 512 threads
 
 // Threads of a row's CTA: `per` elements each, whole warps.
 int cta_threads(int64_t elements, int per) { return (int)((elements + per * 32 - 1) / (per * 32) * 32); }
 
-// CTAs for warps' rows, at most `most` of them: a multiple of 8, eight warps each.
-int64_t warp_ctas(int64_t rows, int64_t most) {
-  const int64_t want = (rows + 63) / 64 * 8;
+// CTAs for warps' rows, `at_once` a CTA, at most `most` CTAs: a multiple of 8.
+int64_t warp_ctas(int64_t rows, int64_t most, int at_once) {
+  const int64_t want = (rows + 8 * at_once - 1) / (8 * at_once) * 8;
   return want < most / 8 * 8 ? want : most / 8 * 8;
 }
 
 // CTAs of the backward for rows of `span` elements from boundary to boundary: as many as the SMs hold at once, so
 // partial rows stay few; a multiple of 8 where a CTA visits more than one row.
 int64_t bwd_ctas(int64_t rows, int64_t span) {
-  if (span <= kWarpWidth) return warp_ctas(rows, 148 * (span <= 256 ? 3 : 2));
+  if (span <= 512) return warp_ctas(rows, 148 * (span <= 256 ? 3 : 2), 8);
+  if (span <= 1024) return warp_ctas(rows, 148 * 2, 4);
+  if (span <= 2048) return warp_ctas(rows, 148 * 2, 2);
   const int64_t most = 148 * (span <= 2560 ? 4 : span <= 5120 ? 2 : 1) / 8 * 8;
   return rows < most ? rows : most;
 }
@@ -477,31 +499,36 @@ struct NormArgs {
   cudaStream_t s;
 };
 
-template <typename Tx, typename To, int V, int NV, bool WARP>
-int launch(const NormArgs& a) {
-  const int threads = WARP ? 256 : cta_threads(a.span, NV * V);
-  const size_t params = norm_param_regs(NV * V, WARP) ? 0 : (size_t)NV * V * (WARP ? 32 : threads) * 4;
-  if (!a.backward) {
-    auto kern = layernorm_fwd_kernel<Tx, To, V, NV, WARP>;
-    const int bytes = NV * V * (int)sizeof(Tx);
-    const size_t smem = (size_t)norm_depth(NV * V, (int)sizeof(Tx), WARP) * bytes * threads + 2 * params;
-    if (smem > 46 * 1024)  // beside 1 KB of row sums
-      if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
-    const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (WARP ? NV * V <= 16 ? 1024 : 768 : 512) / threads;
-    const int64_t most = 148 * (fit < held ? fit : held);
-    const int64_t grid = WARP ? warp_ctas(a.rows, most) : a.rows < most ? a.rows : most / 8 * 8;
-    rk_host::launch_k(kern, (unsigned)grid, threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w, a.b,
-                      static_cast<To*>(a.out), a.ldo, a.stats, a.rows, a.width, a.eps);
-    return rk_host::launch_status();
-  }
-  auto kern = layernorm_bwd_kernel<Tx, To, V, NV, WARP>;
-  const int bytes = NV * V * (int)(sizeof(Tx) + sizeof(To));
-  size_t smem = (size_t)norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(To)), WARP) * bytes * threads + params;
-  if (WARP && smem < (size_t)16 * a.width * 4) smem = (size_t)16 * a.width * 4;
+template <typename Tx, typename Ty, int V, int NV, int W>
+int launch_fwd(const NormArgs& a) {
+  const int threads = W ? 256 : cta_threads(a.span, NV * V);
+  const size_t params = norm_param_regs(NV * V, W) ? 0 : (size_t)NV * V * (W ? 32 * W : threads) * 4;
+  auto kern = layernorm_fwd_kernel<Tx, Ty, V, NV, W>;
+  const int bytes = NV * V * (int)sizeof(Tx);
+  const size_t smem = (size_t)norm_depth(NV * V, (int)sizeof(Tx), W) * bytes * threads + 2 * params;
+  if (smem > 46 * 1024)  // beside 1 KB of row sums
+    if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
+  const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (W ? NV * V <= 16 ? 1024 : 768 : 512) / threads;
+  const int64_t most = 148 * (fit < held ? fit : held);
+  const int64_t grid = W ? warp_ctas(a.rows, most, 8) : a.rows < most ? a.rows : most / 8 * 8;
+  rk_host::launch_k(kern, (unsigned)grid, threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w, a.b,
+                    static_cast<Ty*>(a.out), a.ldo, a.stats, a.rows, a.width, a.eps);
+  return rk_host::launch_status();
+}
+
+template <typename Tx, typename Tg, int V, int NV, int W>
+int launch_bwd(const NormArgs& a) {
+  const int threads = W ? 256 : cta_threads(a.span, NV * V);
+  auto kern = layernorm_bwd_kernel<Tx, Tg, V, NV, W>;
+  const int bytes = NV * V * (int)(sizeof(Tx) + sizeof(Tg));
+  size_t smem = (size_t)norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), W) * bytes * threads +
+                (size_t)NV * V * (W ? 32 * W : threads) * 4;
+  const size_t sums = (size_t)(W ? 16 / (W ? W : 1) : 0) * a.width * 4;
+  if (smem < sums) smem = sums;
   if (smem > 46 * 1024)
     if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
   rk_host::launch_k(kern, (unsigned)bwd_ctas(a.rows, a.span), threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w,
-                    a.stats, static_cast<const To*>(a.dy), a.lddy, static_cast<Tx*>(a.out), a.ldo, a.partial, a.rows,
+                    a.stats, static_cast<const Tg*>(a.dy), a.lddy, static_cast<Tx*>(a.out), a.ldo, a.partial, a.rows,
                     a.width);
   return rk_host::launch_status();
 }
@@ -509,13 +536,23 @@ int launch(const NormArgs& a) {
 template <typename Tx, typename To>
 int dispatch(const NormArgs& a) {
   constexpr int V = 16 / (int)sizeof(Tx);
-  if (a.span > kCtaWidth) return launch<Tx, To, V, 32 / V, false>(a);
-  if (a.span > kWarpWidth) return launch<Tx, To, V, 16 / V, false>(a);
-  if (a.span <= 32 * V) return launch<Tx, To, V, 1, true>(a);
-  if (a.span <= 64 * V) return launch<Tx, To, V, 2, true>(a);
+  if (a.backward) {
+    if (a.span <= 32 * V) return launch_bwd<Tx, To, V, 1, 1>(a);
+    if (a.span <= 64 * V) return launch_bwd<Tx, To, V, 2, 1>(a);
+    if constexpr (V == 4)
+      if (a.span <= 128 * V) return launch_bwd<Tx, To, V, 4, 1>(a);
+    if (a.span <= 1024) return launch_bwd<Tx, To, V, 16 / V, 2>(a);
+    if (a.span <= 2048) return launch_bwd<Tx, To, V, 16 / V, 4>(a);
+    if (a.span <= kCtaWidth) return launch_bwd<Tx, To, V, 16 / V, 0>(a);
+    return launch_bwd<Tx, To, V, 32 / V, 0>(a);
+  }
+  if (a.span <= 32 * V) return launch_fwd<Tx, To, V, 1, 1>(a);
+  if (a.span <= 64 * V) return launch_fwd<Tx, To, V, 2, 1>(a);
+  if (a.span <= 128 * V) return launch_fwd<Tx, To, V, 4, 1>(a);
   if constexpr (V == 4)
-    if (a.span > 128 * V) return launch<Tx, To, V, 8, true>(a);
-  return launch<Tx, To, V, 4, true>(a);
+    if (a.span <= 1024) return launch_fwd<Tx, To, V, 8, 1>(a);
+  if (a.span <= kCtaWidth) return launch_fwd<Tx, To, V, 16 / V, 0>(a);
+  return launch_fwd<Tx, To, V, 32 / V, 0>(a);
 }
 
 // x in fp32: the other side in any type; x in 16 bits: the same type or fp32.
