@@ -32,7 +32,7 @@
 //
 // 32768 x 1024 bf16: forward 27 us (5.0 TB/s), backward with its columns 41 us
 // (4.9 TB/s); 14848 x 256 fp32 to bf16: 5.9 and 11.9 us in L2; 2047 x 5001
-// fp32: 22.9 (3.6 TB/s) and 40 us (3.1 TB/s; by single elements 33 and 85).
+// fp32: 16.7 (4.9 TB/s) and 39 us (3.1 TB/s; by single elements 33 and 85).
 #include "vec.cuh"
 
 namespace rk {
@@ -200,8 +200,8 @@ struct RowWalk {
   }
 };
 
-template <typename Tx, typename Ty, int V, int NV, int W>
-__global__ void __launch_bounds__(W ? 256 : 512, W ? (NV * V <= 16 ? 4 : 3) : 1)
+template <typename Tx, typename Ty, int V, int NV, int W, int THREADS>
+__global__ void __launch_bounds__(THREADS, W ? (NV * V <= 16 ? 4 : 3) : 1)
     layernorm_fwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const NormParam b,
                          Ty* __restrict__ y, int64_t ldy, float2* __restrict__ stats, int64_t rows, int width,
                          float eps) {
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(W ? 256 : 512, W ? (NV * V <= 16 ? 4 : 3) : 1)
 }
 
 // partial: [gridDim.x][2][width] fp32 (dw, then db), or null when neither is wanted; dx may be null.
-template <typename Tx, typename Tg, int V, int NV, int W>
-__global__ void __launch_bounds__(W ? 256 : 512, W > 1 ? 2 : W ? (NV * V <= 8 ? 3 : 2) : 1)
+template <typename Tx, typename Tg, int V, int NV, int W, int THREADS>
+__global__ void __launch_bounds__(THREADS, W > 1 ? 2 : W ? (NV * V <= 8 ? 3 : 2) : 1)
     layernorm_bwd_kernel(const Tx* __restrict__ x, int64_t ldx, const NormParam w, const float2* __restrict__ stats,
                          const Tg* __restrict__ dy, int64_t lddy, Tx* __restrict__ dx, int64_t lddx,
                          float* __restrict__ partial, int64_t rows, int width) {
@@ -473,13 +473,19 @@ int64_t warp_ctas(int64_t rows, int64_t most, int at_once) {
   return want < most / 8 * 8 ? want : most / 8 * 8;
 }
 
+// Threads that an SM holds at 96 registers, where that is another CTA of rows than at the 128 that CTA rows of 16
+// elements a thread would rather have (2047 x 5001 fp32 forward 16.7 us, at 128 registers 22.8; 8192 x 4096 bf16, two CTAs
+// either way, 33.0 and 31.3, and backward 65 and 52).
+constexpr int kHeld = 640;
+bool held_pays(int threads) { return kHeld / threads > 512 / threads; }
+
 // CTAs of the backward for rows of `span` elements from boundary to boundary: as many as the SMs hold at once, so
 // partial rows stay few; a multiple of 8 where a CTA visits more than one row.
 int64_t bwd_ctas(int64_t rows, int64_t span) {
   if (span <= 512) return warp_ctas(rows, 148 * (span <= 256 ? 3 : 2), 8);
   if (span <= 1024) return warp_ctas(rows, 148 * 2, 4);
   if (span <= 2048) return warp_ctas(rows, 148 * 2, 2);
-  const int64_t most = 148 * (span <= 2560 ? 4 : span <= 5120 ? 2 : 1) / 8 * 8;
+  const int64_t most = 148 * (span <= kCtaWidth ? kHeld / cta_threads(span, 16) : 1) / 8 * 8;
   return rows < most ? rows : most;
 }
 
@@ -499,16 +505,18 @@ struct NormArgs {
   cudaStream_t s;
 };
 
-template <typename Tx, typename Ty, int V, int NV, int W>
+template <typename Tx, typename Ty, int V, int NV, int W, int THREADS = W ? 256 : 512>
 int launch_fwd(const NormArgs& a) {
-  const int threads = W ? 256 : cta_threads(a.span, NV * V);
+  const int threads = W ? THREADS : cta_threads(a.span, NV * V);
+  if constexpr (W == 0 && NV * V == 16 && THREADS != kHeld)
+    if (held_pays(threads)) return launch_fwd<Tx, Ty, V, NV, 0, kHeld>(a);
   const size_t params = norm_param_regs(NV * V, W) ? 0 : (size_t)NV * V * (W ? 32 * W : threads) * 4;
-  auto kern = layernorm_fwd_kernel<Tx, Ty, V, NV, W>;
+  auto kern = layernorm_fwd_kernel<Tx, Ty, V, NV, W, THREADS>;
   const int bytes = NV * V * (int)sizeof(Tx);
   const size_t smem = (size_t)norm_depth(NV * V, (int)sizeof(Tx), W) * bytes * threads + 2 * params;
   if (smem > 46 * 1024)  // beside 1 KB of row sums
     if (const int e = rk_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return e;
-  const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (W ? NV * V <= 16 ? 1024 : 768 : 512) / threads;
+  const int64_t fit = 227 * 1024 / (int64_t)(smem + 2048), held = (W ? NV * V <= 16 ? 1024 : 768 : THREADS) / threads;
   const int64_t most = 148 * (fit < held ? fit : held);
   const int64_t grid = W ? warp_ctas(a.rows, most, 8) : a.rows < most ? a.rows : most / 8 * 8;
   rk_host::launch_k(kern, (unsigned)grid, threads, smem, a.s, static_cast<const Tx*>(a.x), a.ldx, a.w, a.b,
@@ -516,10 +524,12 @@ int launch_fwd(const NormArgs& a) {
   return rk_host::launch_status();
 }
 
-template <typename Tx, typename Tg, int V, int NV, int W>
+template <typename Tx, typename Tg, int V, int NV, int W, int THREADS = W ? 256 : 512>
 int launch_bwd(const NormArgs& a) {
-  const int threads = W ? 256 : cta_threads(a.span, NV * V);
-  auto kern = layernorm_bwd_kernel<Tx, Tg, V, NV, W>;
+  const int threads = W ? THREADS : cta_threads(a.span, NV * V);
+  if constexpr (W == 0 && NV * V == 16 && THREADS != kHeld)
+    if (held_pays(threads)) return launch_bwd<Tx, Tg, V, NV, 0, kHeld>(a);
+  auto kern = layernorm_bwd_kernel<Tx, Tg, V, NV, W, THREADS>;
   const int bytes = NV * V * (int)(sizeof(Tx) + sizeof(Tg));
   size_t smem = (size_t)norm_depth(NV * V, (int)(sizeof(Tx) + sizeof(Tg)), W) * bytes * threads +
                 (size_t)NV * V * (W ? 32 * W : threads) * 4;

@@ -95,13 +95,14 @@ def test_layer_norm_of_strided_and_unaligned_rows(layout, rows, width, dtype):
     _check(x, w, b, 1e-3, y, g, *torch.autograd.grad(y, (x, w, b), g))
 
 
-@pytest.mark.parametrize("width", [248, 257, 505, 512, 513, 999, 1024, 1031, 1536, 2041, 2048, 2055])
+@pytest.mark.parametrize("rows,width", [(4099, k) for k in (248, 257, 505, 512, 513, 999, 1024, 1031, 1536, 2041, 2048, 2055)] +
+                         [(1301, k) for k in (2553, 2560, 2561, 3401, 4096, 5105, 5120, 5127, 8192, 8199)])
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F32, F16), (F16, F32)])
-def test_layer_norm_gradients_of_many_rows_at_the_borders_of_rows_threads(width, dtype, out):
-    x = _rows(4099, width, dtype).requires_grad_()
+def test_layer_norm_gradients_of_many_rows_at_the_borders_of_rows_threads(rows, width, dtype, out):
+    x = _rows(rows, width, dtype).requires_grad_()
     w, b = _params(width, F32)
     y = fx.layer_norm(x, w, b, out_dtype=out)
-    g = _rows(4099, width, out, seed=1, shift=0.1)
+    g = _rows(rows, width, out, seed=1, shift=0.1)
     grads = torch.autograd.grad(y, (x, w, b), g, retain_graph=True)
     _check(x, w, b, 1e-5, y, g, *grads)
     for one, again in zip(grads, torch.autograd.grad(y, (x, w, b), g)):
