@@ -144,10 +144,9 @@ def _fast_rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, int, int, int]:
     return _norm_rows(t, per)
 
 
-def layernorm_fwd_rows(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+def layernorm_fwd_kept(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
                        out_dtype: torch.dtype | None = None, want_stats: bool = True):
-    """layernorm_fwd that also returns what its backward can use again: (y, stats, weight, (rows of x, their number,
-    width, stride, dtype code, parameters' dtype code))."""
+    """layernorm_fwd that also returns what its backward can use again: (y, stats, x in rows it can read, weight)."""
     require_cuda(x, weight, bias, what="layer norm kernels")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("layer norm needs a non-empty last dimension")
@@ -158,18 +157,17 @@ def layernorm_fwd_rows(x: torch.Tensor, weight: torch.Tensor | None, bias: torch
     _on_current_device(x, "the input", weight, bias)
     weight, bias, pcode = _norm_params(x, weight, bias)
     xr, rows, width, ld = _fast_rows(x, 16 // x.element_size())
-    xcode = _lib.code(x.dtype)
     y = _new(x, out_dtype)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
-    _lib.call("rk_layernorm_fwd", xr.data_ptr(), xcode, ld, _lib.ptr(weight), _lib.ptr(bias), pcode, y.data_ptr(),
-              _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, eps, _lib.stream_ptr())
-    return y, stats, weight, (xr, rows, width, ld, xcode, pcode)
+    _lib.call("rk_layernorm_fwd", xr.data_ptr(), _lib.code(x.dtype), ld, _lib.ptr(weight), _lib.ptr(bias), pcode,
+              y.data_ptr(), _lib.code(out_dtype), width, _lib.ptr(stats), rows, width, eps, _lib.stream_ptr())
+    return y, stats, xr, weight
 
 
 def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
                   out_dtype: torch.dtype | None = None, want_stats: bool = True):
     """y = (x - mean) * rsqrt(var + eps) * weight + bias over the last dim; returns (y, stats [rows, 2] or None)."""
-    return layernorm_fwd_rows(x, weight, bias, float(eps), out_dtype, want_stats)[:2]
+    return layernorm_fwd_kept(x, weight, bias, float(eps), out_dtype, want_stats)[:2]
 
 
 @functools.lru_cache(maxsize=64)
@@ -177,36 +175,30 @@ def _layernorm_workspace(rows: int, width: int) -> int:
     return _lib.lib().rk_layernorm_bwd_workspace(rows, width)
 
 
-def layernorm_bwd_rows(x_rows: tuple, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
-                       param_dtype: torch.dtype, want_dx: bool, want_dw: bool, want_db: bool):
-    """layernorm_bwd from layernorm_fwd_rows' results, which were checked there."""
-    xr, rows, width, ldx, xcode, pcode = x_rows
-    dyr, _, _, lddy = _fast_rows(dy, 16 // xr.element_size())
-    dx = _new(xr, xr.dtype) if want_dx else None
-    dw = (xr.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_dw else None
-    db = (xr.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_db else None
-    n_ws = _layernorm_workspace(rows, width) if want_dw or want_db else 0
-    ws = stats.new_empty(n_ws // 4) if n_ws else None
-    _lib.call("rk_layernorm_bwd", xr.data_ptr(), xcode, ldx, _lib.ptr(weight), pcode, stats.data_ptr(), dyr.data_ptr(),
-              _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), n_ws, rows, width,
-              _lib.stream_ptr())
-    return dx, dw, db
-
-
 def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
                   param_dtype: torch.dtype = torch.float32, want_dx: bool = True, want_dw: bool = True,
                   want_db: bool = True):
-    """(dx in x's type, dweight, dbias in param_dtype; None where not wanted) of layernorm_fwd."""
+    """(dx in x's type, dweight, dbias in param_dtype; None where not wanted) of layernorm_fwd. Rows, strides and types are
+    those of the tensors given: hooks on saved tensors need not hand back the strides that the forward saw."""
     require_cuda(x, weight, stats, dy, what="layer norm kernels")
     _on_current_device(x, "the input", weight, stats, dy)
     weight, _, _ = _norm_params(x, weight, None)
     if weight is not None and weight.dtype != param_dtype:
         raise ValueError("parameter gradients come in the weight's type")
-    xr, rows, width, ldx = _norm_rows(x, 16 // x.element_size())
+    per = 16 // x.element_size()
+    xr, rows, width, ldx = _fast_rows(x, per)
     if dy.shape != x.shape or stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("layer norm backward takes dy of the input's shape and the forward's stats")
-    x_rows = (xr, rows, width, ldx, _lib.code(x.dtype), _lib.code(param_dtype))
-    return layernorm_bwd_rows(x_rows, weight, stats, dy, param_dtype, want_dx, want_dw, want_db)
+    dyr, _, _, lddy = _fast_rows(dy, per)
+    dx = _new(xr, x.dtype) if want_dx else None
+    dw = (x.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_dw else None
+    db = (x.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_db else None
+    n_ws = _layernorm_workspace(rows, width) if want_dw or want_db else 0
+    ws = stats.new_empty(n_ws // 4) if n_ws else None
+    _lib.call("rk_layernorm_bwd", xr.data_ptr(), _lib.code(x.dtype), ldx, _lib.ptr(weight), _lib.code(param_dtype),
+              stats.data_ptr(), dyr.data_ptr(), _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw), _lib.ptr(db),
+              _lib.ptr(ws), n_ws, rows, width, _lib.stream_ptr())
+    return dx, dw, db
 
 
 # ------------------------------------------------------------------ dropout

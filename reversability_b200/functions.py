@@ -119,7 +119,7 @@ class LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, eps, out_dtype):
-        y, stats, weight, (xr, *ctx.rows) = fn.layernorm_fwd_rows(x, w, b, eps, out_dtype)
+        y, stats, xr, weight = fn.layernorm_fwd_kept(x, w, b, eps, out_dtype)
         ctx.save_for_backward(xr, weight, stats)
         ctx.param_dtype = torch.float32 if w is None and b is None else (b if w is None else w).dtype
         return y
@@ -129,7 +129,7 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, gy):
         xr, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = fn.layernorm_bwd_rows((xr, *ctx.rows), weight, stats, gy, ctx.param_dtype, need[0], need[1], need[2])
+        dx, dw, db = fn.layernorm_bwd(xr, weight, stats, gy, ctx.param_dtype, need[0], need[1], need[2])
         return dx, dw, db, None, None
 
 
@@ -142,7 +142,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
-    return fn.layernorm_fwd_rows(x, weight, bias, float(eps), out_dtype, False)[0]
+    return fn.layernorm_fwd_kept(x, weight, bias, float(eps), out_dtype, False)[0]
 
 
 class DropoutFn(torch.autograd.Function):

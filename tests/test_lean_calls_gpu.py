@@ -1,0 +1,45 @@
+"""Layer norm, dropout and the head loss in the calls around them: saved-tensor hooks, forward-mode derivatives, labels and
+gradients that are not numbers to count with, several pieces of the vocabulary."""
+import pytest
+import torch
+
+from reversability_b200 import _lib, functional as fn, functions as fx
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width,pitch", [(300, 256, 768), (37, 1000, 1024), (9, 20, 24)])
+def test_layer_norm_of_spaced_rows_offloaded_to_the_host(rows, width, pitch, dtype):
+    """What is saved comes back from the host with rows side by side: the same gradients as without the detour."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(rows, pitch, generator=g, device=DEV).to(dtype)[:, :width].requires_grad_()
+    w = torch.randn(width, generator=g, device=DEV).requires_grad_()
+    b = torch.randn(width, generator=g, device=DEV).requires_grad_()
+    dy = torch.randn(rows, width, generator=g, device=DEV).to(dtype)
+    y = fx.layer_norm(x, w, b)
+    want = torch.autograd.grad(y, (x, w, b), dy)
+    with torch.autograd.graph.save_on_cpu():
+        z = fx.layer_norm(x, w, b)
+    got = torch.autograd.grad(z, (x, w, b), dy)
+    assert torch.equal(y, z) and all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_head_loss_and_dropout_offloaded_to_the_host(dtype):
+    """The same for the other two: wide hidden rows, a transposed weight, a seed on the device."""
+    x = torch.randn(70, 96, device=DEV).to(dtype)[:, :64].requires_grad_()
+    w = torch.randn(64, 500, device=DEV).to(dtype).t().requires_grad_()
+    y = torch.randint(0, 500, (70,), device=DEV)
+    seed = torch.tensor(3, device=DEV)
+
+    def step():
+        loss = fx.linear_cross_entropy(fx.dropout(x, 0.3, seed), w, y)
+        return loss
+    want = torch.autograd.grad(step(), (x, w))
+    with torch.autograd.graph.save_on_cpu():
+        loss = step()
+    assert all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(loss, (x, w)), want))
+    assert fn is not None and _lib.device_status() == 0
