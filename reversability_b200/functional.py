@@ -10,6 +10,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,6 +21,13 @@ def require_cuda(*tensors: torch.Tensor, what: str = "librevk kernels") -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError(f"{what} require CUDA tensors; no CPU fallback exists")
+
+
+def carries_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether one of the tensors is a dual number of forward-mode differentiation."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open (asking each tensor takes 0.6 us)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _row_major_2d(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:

@@ -114,6 +114,16 @@ def once(backward):
     return run
 
 
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether a derivative of these is to be had: one of them requires a gradient, or carries a tangent of forward-mode
+    differentiation (which a Function refuses; past it, the result would have lost the tangent without a word)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return fn.carries_tangent(*tensors)
+
+
 class LayerNormFn(torch.autograd.Function):
     """Keeps the input and two numbers a row."""
 
@@ -139,8 +149,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     fp32, weight and bias (each may be None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise
     (any type for fp32 x, fp32 for 16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in
     its input's type under autocast. The gradients of weight and bias are sums in a fixed order."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if differentiated(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
     return fn.layernorm_fwd_kept(x, weight, bias, float(eps), out_dtype, False)[0]
 
@@ -178,7 +187,7 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, *, offset: int 
     change it in place only after the backward. What is dropped is not used: NaN there does not spread."""
     if not training:
         p = 0.0
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if differentiated(x, residual):
         return DropoutFn.apply(x, residual, float(p), seed, offset)
     return fn.dropout(x, float(p), seed, offset, residual)
 
@@ -233,6 +242,6 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     if low is not None:
         with torch.autocast("cuda", enabled=False):
             hidden, weight = hidden.to(low), weight.to(low)
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if differentiated(hidden, weight):
         return LinearCrossEntropyFn.apply(hidden, weight, labels, int(ignore_index), reduction)
     return fn.linear_ce_fwd(hidden, weight, labels, int(ignore_index), reduction)[0]

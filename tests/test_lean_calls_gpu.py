@@ -2,6 +2,7 @@
 gradients that are not numbers to count with, several pieces of the vocabulary."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from reversability_b200 import _lib, functional as fn, functions as fx
 
@@ -43,3 +44,20 @@ def test_head_loss_and_dropout_offloaded_to_the_host(dtype):
         loss = step()
     assert all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(loss, (x, w)), want))
     assert fn is not None and _lib.device_status() == 0
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is not dropped without a word, with gradients recorded or not, whichever input carries it."""
+    x, w, y = torch.randn(4, 16, device=DEV), torch.ones(16, device=DEV), torch.randint(0, 9, (4,), device=DEV)
+    head, b16 = torch.randn(9, 16, device=DEV), x.to(BF16)
+    for calls, like in (((lambda t: fx.layer_norm(t, w), lambda t: fx.dropout(t, 0.5, 3), lambda t: fx.dropout(x, 0.5, 3, residual=t),
+                          lambda t: fx.linear_cross_entropy(t, head, y)), x),
+                        ((lambda t: fx.linear_cross_entropy(t, head.to(BF16), y),), b16),
+                        ((lambda t: fx.layer_norm(x, t), lambda t: fx.layer_norm(x, w, t)), w),
+                        ((lambda t: fx.linear_cross_entropy(x, t, y),), head)):
+        for call in calls:
+            for mode in (torch.enable_grad, torch.no_grad):
+                with forward_ad.dual_level(), mode():
+                    call(like)  # without a tangent: as ever
+                    with pytest.raises(RuntimeError, match="forward"):
+                        call(forward_ad.make_dual(like, torch.ones_like(like)))
