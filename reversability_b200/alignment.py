@@ -29,6 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import functional as fn
+from .functions import differentiated
 from .optimized import _accumulate_grad, amp_context, compute_dtype, hidden_states
 
 
@@ -58,7 +59,7 @@ def _check_rows(temperature: float, ignore_index: int) -> None:
 
 def _check_constants(**tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if differentiated(t):
             raise ValueError(f"{name} is a constant of the loss; detach it")
 
 
@@ -90,7 +91,7 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: f
     the pair (log-probabilities, entropies of the rows). Differentiable with respect to the logits."""
     _check_rows(temperature, ignore_index)
     fn.require_cuda(logits, labels, what="token log-probabilities")
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not differentiated(logits):
         lp, h, _ = fn.token_logprob_fwd(logits, labels, temperature, ignore_index, entropy, want_stats=False)
         return (lp, h) if entropy else lp
     return _TokenLogprobs.apply(logits, labels, float(temperature), int(ignore_index), bool(entropy))
@@ -146,7 +147,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprobs: torch
     _check_constants(old_logprobs=old_logprobs, advantages=advantages, ref_logprobs=ref_logprobs, weights=weights,
                      denominator=denominator)
     fn.require_cuda(logits, actions, old_logprobs, advantages, what="the policy loss")
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not differentiated(logits):
         loss, clip, lp, kl, h, _, _ = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False, **args)
         return PolicyLoss(loss, lp, kl, h, clip)
     loss, clip, lp, kl, h, _, pairs = fn.policy_loss(logits, actions, old_logprobs, advantages, want_grad=False,
@@ -218,7 +219,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logprobs: to
     args = _preference_args(kind, beta, label_smoothing, average, temperature, ignore_index)
     _check_constants(ref_logprobs=ref_logprobs)
     fn.require_cuda(logits, labels, ref_logprobs, what="the preference loss")
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not differentiated(logits):
         loss, lp, rewards, _, _ = fn.preference_loss(logits, labels, ref_logprobs, want_grad=False, **args)
         return PreferenceLoss(loss, rewards, lp)
     loss, lp, rewards, _, rows = fn.preference_loss(logits, labels, ref_logprobs, want_grad=False, **args)

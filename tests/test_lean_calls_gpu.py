@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from reversability_b200 import _lib, functional as fn, functions as fx
+from reversability_b200 import _lib, alignment, functional as fn, functions as fx
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -61,3 +61,17 @@ def test_forward_mode_derivatives_are_refused():
                     call(like)  # without a tangent: as ever
                     with pytest.raises(RuntimeError, match="forward"):
                         call(forward_ad.make_dual(like, torch.ones_like(like)))
+
+
+def test_forward_mode_derivatives_of_token_losses_are_refused():
+    """The same for the losses on token log-probabilities: a tangent on the logits or on a constant."""
+    z, y, ref = torch.randn(4, 6, 20, device=DEV), torch.randint(0, 20, (4, 6), device=DEV), torch.randn(4, 6, device=DEV)
+    for call, like, match in ((lambda t: alignment.token_logprobs(t, y), z, "forward"),
+                              (lambda t: alignment.policy_loss(t, y, ref, ref), z, "forward"),
+                              (lambda t: alignment.policy_loss(z, y, ref, t), ref, "constant"),
+                              (lambda t: alignment.preference_loss(t, y, ref), z, "forward"),
+                              (lambda t: alignment.preference_loss(z, y, t), ref, "constant")):
+        with forward_ad.dual_level(), torch.no_grad():
+            call(like)
+            with pytest.raises((RuntimeError, ValueError), match=match):
+                call(forward_ad.make_dual(like, torch.ones_like(like)))
