@@ -595,12 +595,14 @@ def _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss):
     """fp32 parity configuration: pieces of the rows, on the CUDA-core GEMM and the token-loss kernels."""
     V = weight.shape[0]
     x, y = hidden.reshape(-1, hidden.shape[-1]), labels.view(-1)
-    valid = (y != ignore_index) & (y >= 0) & (y < V)
+    ignored = y == ignore_index
+    valid = ~ignored & (y >= 0) & (y < V)
+    marks = torch.where(valid, y, torch.where(ignored, -100, -1))  # -1: outside the vocabulary, whatever ignore_index is
     rows = torch.empty(y.shape, device=x.device, dtype=torch.float32)
     w = weight.contiguous()
     for s, n, logits in _f32_chunks(x, y, V):
         linear_fwd(x[s:s + n].contiguous(), w, out=logits[:n])
-        rows[s:s + n] = token_logprob_fwd(logits[:n], torch.where(valid[s:s + n], y[s:s + n], -100), want_stats=False)[0]
+        rows[s:s + n] = token_logprob_fwd(logits[:n], marks[s:s + n], want_stats=False)[0]
     rows.neg_()
     if reduction == "none":
         loss.copy_(rows.view(loss.shape))

@@ -234,10 +234,12 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
                          reduction: str = "mean") -> torch.Tensor:
     """F.cross_entropy(F.linear(hidden, weight), labels) without the logits (model.py:104, train_baseline.py:262): hidden
     [..., d], weight [V, d] of one type, int64 labels [...]; the loss in fp32, 'mean' over the labels that count (0 if
-    none does), 'sum', or 'none' (one a label). Rows labelled ignore_index cost nothing, are not read and get zero
-    gradients; a label outside [0, V) sets the library's device status and counts as ignored. The gradients come in the
-    inputs' types, rounded once from fp32 sums over 16-bit softmax terms (fp16: scaled inside, so a mean over many rows
-    does not underflow before the gradients themselves do). Under autocast both inputs are cast as F.linear's are."""
+    none does), 'sum', or 'none' (one a label). What lies in a row labelled ignore_index does not spread and its gradients
+    are zero; in 16 bits such rows are not read and cost nothing. A label outside [0, V) sets the library's device status
+    and counts as ignored. The gradients come in the inputs' types, rounded once from fp32 sums over 16-bit softmax terms
+    (fp16: scaled inside, so a mean over many rows does not underflow before the gradients themselves do; with 'none' one
+    power of two serves all rows, and a row whose gradient is 2^-k of the largest keeps terms down to 2^(k - 37)). fp32
+    inputs stay fp32 throughout, in pieces of the rows. Under autocast both inputs are cast as F.linear's are."""
     low = autocast_dtype("cuda")
     if low is not None:
         with torch.autocast("cuda", enabled=False):

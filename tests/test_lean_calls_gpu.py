@@ -75,3 +75,25 @@ def test_forward_mode_derivatives_of_token_losses_are_refused():
             call(like)
             with pytest.raises((RuntimeError, ValueError), match=match):
                 call(forward_ad.make_dual(like, torch.ones_like(like)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("ignore,bad", [(-100, (100, -3)), (7, (-100, 1 << 40)), (-1, (-100, -2))])
+def test_labels_outside_the_vocabulary_set_the_status(dtype, ignore, bad):
+    """In every type, whichever number is the ignored one; the ignored one alone sets nothing."""
+    x = torch.randn(200, 16, device=DEV).to(dtype).requires_grad_()
+    w = torch.randn(100, 16, device=DEV).to(dtype).requires_grad_()
+    y = torch.randint(0, 100, (200,), device=DEV)
+    y[3] = y[60] = ignore
+    wrong = y.clone()
+    wrong[9], wrong[150] = bad
+    y[9] = y[150] = ignore
+    assert _lib.device_status() == 0
+    want = fx.linear_cross_entropy(x, w, y, ignore_index=ignore)
+    assert _lib.device_status() == 0
+    got = fx.linear_cross_entropy(x, w, wrong, ignore_index=ignore)
+    assert _lib.device_status() == 4  # RK_DEV_CE_LABEL
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, (x, w)), torch.autograd.grad(want, (x, w))):
+        assert torch.equal(a, b)
+    assert _lib.device_status() == 0
