@@ -625,7 +625,8 @@ def _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw):
         stats = token_logprob_fwd(z, kept[s:s + n])[2]
         d = token_logprob_bwd(z, kept[s:s + n], stats, up[s:s + n].contiguous(), out=z)
         if dx is not None:
-            dx.view(-1, K)[s:s + n] = linear_dgrad(d, w)
+            part = linear_dgrad(d, w)
+            dx.view(-1, K)[s:s + n] = part.masked_fill_(~valid[s:s + n, None], 0.0)  # 0 times an infinite weight is none
         if total is not None:
             linear_wgrad(d, xc, dw=total, accumulate=True)
     return dx, total if dw is None or dw.dtype == torch.float32 else total.to(dw.dtype)

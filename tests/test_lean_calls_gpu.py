@@ -97,3 +97,14 @@ def test_labels_outside_the_vocabulary_set_the_status(dtype, ignore, bad):
     for a, b in zip(torch.autograd.grad(got, (x, w)), torch.autograd.grad(want, (x, w))):
         assert torch.equal(a, b)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_ignored_rows_have_zero_gradients_under_an_infinite_weight(dtype):
+    x = torch.randn(70, 32, device=DEV).to(dtype).requires_grad_()
+    w = torch.randn(90, 32, device=DEV).to(dtype)
+    w[5, 0], w[6, 1] = float("inf"), -float("inf")
+    y = torch.randint(10, 90, (70,), device=DEV)
+    y[::3] = -100
+    dx, = torch.autograd.grad(fx.linear_cross_entropy(x, w, y), x)
+    assert not dx[::3].any()
