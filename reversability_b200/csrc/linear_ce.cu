@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const uint16_t* __restri
     float each = f.boost;
     if (f.reduction == 0) each = 1.f / *f.scale;
     else if (blockIdx.x == 0 && threadIdx.x == 0)
-      *f.scale = (f.reduction == 2 ? f.grad[0] / (float)(count > 0 ? count : 1) : f.grad[0]) / f.boost;
+      *f.scale = count ? (f.reduction == 2 ? f.grad[0] / (float)count : f.grad[0]) / f.boost : 0.f;  // no rows: zeros
     for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256)
       f.rowc[i] = make_float2(-f.lse[i] * kLog2e, f.reduction == 0 ? f.grad[rows_of[i]] * each : each);
   }

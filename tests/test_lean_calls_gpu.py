@@ -108,3 +108,15 @@ def test_ignored_rows_have_zero_gradients_under_an_infinite_weight(dtype):
     y[::3] = -100
     dx, = torch.autograd.grad(fx.linear_cross_entropy(x, w, y), x)
     assert not dx[::3].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("K", [32, 27])
+def test_no_row_counts_under_a_gradient_that_is_no_number(dtype, reduction, K):
+    """Zeros, as there is nothing to multiply (a weight gradient stored at once, and one from slices)."""
+    x, w = torch.randn(300, K, device=DEV).to(dtype).requires_grad_(), torch.randn(90, K, device=DEV).to(dtype).requires_grad_()
+    y = torch.full((300,), -100, device=DEV)
+    for bad in (float("inf"), float("nan")):
+        loss = fx.linear_cross_entropy(x, w, y, reduction=reduction)
+        assert not any(t.any() for t in torch.autograd.grad(loss, (x, w), torch.full_like(loss, bad)))
