@@ -816,7 +816,7 @@ struct FactorArgs {
 // Listed rows side by side, `pitch` apart, and zeros up to the next multiple of 256 rows; not if all rows are listed and
 // the GEMMs can read them where they are. For the backward also the rows' factors: rowc[i] = (-lse log2 e, f_i) with
 // dz = scale f_i (softmax - onehot). One gradient for all rows: f = boost and scale is that gradient (over the count for
-// a mean) / boost. One a row: scale is a power of two near the largest of them / boost and f_i = g_i / scale, exactly. In
+// a mean) / boost. One a row: scale is a power of two near the largest finite one / boost and f_i = g_i / scale, exactly. In
 // fp16 `boost` is a power of two above 1, so that probabilities down to 2^-37 are held.
 __global__ void __launch_bounds__(256) ce_gather_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t rows, int width,
                                                         int64_t pitch, const int* __restrict__ head,
@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float2* __restrict
   }
 }
 
-// The scale of the backward when each row has a gradient: a power of two near the largest of them, over boost.
+// The scale of the backward when each row has a gradient: a power of two near the largest finite one, over boost.
 __global__ void __launch_bounds__(1024) ce_scale_kernel(const int* __restrict__ head, const int* __restrict__ rows_of,
                                                         const float* __restrict__ grad, float boost,
                                                         float* __restrict__ scale) {
@@ -940,7 +940,10 @@ __global__ void __launch_bounds__(1024) ce_scale_kernel(const int* __restrict__ 
   const int lane = threadIdx.x & 31;
   float m = 0.f;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < count; i += 1024) m = fmaxf(m, fabsf(grad[rows_of[i]]));
+  for (int i = threadIdx.x; i < count; i += 1024) {
+    const float a = fabsf(grad[rows_of[i]]);
+    if (a < INFINITY) m = fmaxf(m, a);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) top[threadIdx.x >> 5] = m;
@@ -950,7 +953,7 @@ __global__ void __launch_bounds__(1024) ce_scale_kernel(const int* __restrict__ 
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (threadIdx.x == 0) {
     float unit = 1.f;
-    if (m > 0.f && m < INFINITY) {
+    if (m > 0.f) {
       int e;
       frexpf(m, &e);
       unit = ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);  // the scale and its reciprocal are normal numbers

@@ -120,3 +120,16 @@ def test_no_row_counts_under_a_gradient_that_is_no_number(dtype, reduction, K):
     for bad in (float("inf"), float("nan")):
         loss = fx.linear_cross_entropy(x, w, y, reduction=reduction)
         assert not any(t.any() for t in torch.autograd.grad(loss, (x, w), torch.full_like(loss, bad)))
+
+
+def test_an_infinite_gradient_of_one_row_leaves_the_others():
+    """fp16, a gradient a row: the common scale is that of the finite ones, so theirs do not overflow beside an infinite one."""
+    x, w = torch.randn(40, 32, device=DEV).to(F16).requires_grad_(), torch.randn(50, 32, device=DEV).to(F16).requires_grad_()
+    y = torch.randint(0, 50, (40,), device=DEV)
+    g = torch.full((40,), 300.0, device=DEV)
+    want, = torch.autograd.grad(fx.linear_cross_entropy(x, w, y, reduction="none"), x, g)
+    for bad in (float("inf"), float("nan")):
+        g[7] = bad
+        dx, = torch.autograd.grad(fx.linear_cross_entropy(x, w, y, reduction="none"), x, g)
+        rest = torch.arange(40, device=DEV) != 7
+        assert torch.equal(dx[rest], want[rest]) and not torch.isfinite(dx[7]).any()
