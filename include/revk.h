@@ -98,8 +98,9 @@ RK_API int rk_rmsnorm_bwd(const void* x, int x_dtype, int64_t ldx, const float* 
  * in any type, or x in 16 bits with y in the same type or fp32. w, b: [width]
  * in param_dtype, each may be NULL (1 and 0). stats (may be NULL): fp32 pairs
  * (mu, s) per row, 8-byte aligned. width <= 16384 (rows that start between
- * 16-byte boundaries: 16377 covers every case). Up to 15 bytes in front of
- * a row and behind it are read where other rows of the same array surround it. */
+ * 16-byte boundaries: 16377 covers every case). Only what lies between the
+ * first row's start and the last row's end is read; there, up to seven elements
+ * (three, for fp32 x) in front of a row and behind it. */
 RK_API int rk_layernorm_fwd(const void* x, int x_dtype, int64_t ldx, const void* w, const void* b, int param_dtype,
                             void* y, int y_dtype, int64_t ldy, float* stats, int64_t rows, int64_t width, float eps,
                             void* stream);

@@ -73,7 +73,9 @@ __device__ __forceinline__ void copies_wait() {
 }
 
 // Starts the copy of V elements of a row from column c on into this lane's slot. `whole`: all of them lie in the
-// matrix, those of an edge vector outside the row too; else what is outside the row is not touched.
+// matrix, those of an edge vector outside the row too; else what is outside the row is not touched. An edge vector, up to
+// V - 1 elements in front of its row and behind it, lies in the matrix if there is a row before and one behind and rows are
+// at least V elements apart: its start is then behind the first row's, its end before the last row's.
 template <typename T, int V>
 __device__ __forceinline__ void fetch(RowPack<T, V>* slot, const T* __restrict__ row, int c, int width, bool whole) {
   if (whole) {
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, W ? (NV * V <= 16 ? 4 : 3) : 1)
   auto start = [&](int64_t row, int d) {
     if (row < rows) {
       const Tx* src = x + row * ldx;
-      const bool inner = row > 0 && row + 1 < rows;
+      const bool inner = row > 0 && row + 1 < rows && ldx >= V;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (r.col(j) < width)
@@ -320,12 +322,12 @@ __global__ void __launch_bounds__(THREADS, W > 1 ? 2 : W ? (NV * V <= 8 ? 3 : 2)
     if (row < rows) {
       const Tx* src = x + row * ldx;
       const Tg* src_g = dy + row * lddy;
-      const bool inner = row > 0 && row + 1 < rows;
+      const bool middle = row > 0 && row + 1 < rows, inner = middle && ldx >= V, inner_g = middle && lddy >= V;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (r.col(j) < width) {
           fetch<Tx, V>(mine_x + (d * NV + j) * blockDim.x, src, r.col(j), width, inner || !(r.edge >> j & 1));
-          fetch<Tg, V>(mine_g + (d * NV + j) * blockDim.x, src_g, r.col(j), width, inner || !(r.edge >> j & 1));
+          fetch<Tg, V>(mine_g + (d * NV + j) * blockDim.x, src_g, r.col(j), width, inner_g || !(r.edge >> j & 1));
         }
     }
     copies_commit();

@@ -2,6 +2,7 @@
 gradients that are not numbers to count with, several pieces of the vocabulary."""
 import pytest
 import torch
+from test_norm_dropout_gpu import _check as _check_norm  # with the tolerances derived there
 from torch.autograd import forward_ad
 
 from reversability_b200 import _lib, alignment, functional as fn, functions as fx
@@ -133,3 +134,33 @@ def test_an_infinite_gradient_of_one_row_leaves_the_others():
         dx, = torch.autograd.grad(fx.linear_cross_entropy(x, w, y, reduction="none"), x, g)
         rest = torch.arange(40, device=DEV) != 7
         assert torch.equal(dx[rest], want[rest]) and not torch.isfinite(dx[7]).any()
+
+
+@pytest.mark.parametrize("rows,width,ld,at", [(3, 1, 1, 0), (3, 1, 1, 5), (4, 1, 9, 7), (5, 3, 3, 2), (7, 2, 5, 1), (2, 5, 6, 3),
+                                              (9, 7, 7, 6), (1, 3, 3, 4), (40, 6, 8, 1), (700, 4, 7, 3), (700, 9, 9, 5)])
+@pytest.mark.parametrize("xt,yt", [(F32, F32), (F32, BF16), (BF16, BF16), (BF16, F32), (F16, F32)])
+def test_layer_norm_entries_on_narrow_rows_at_any_address(rows, width, ld, at, xt, yt):
+    """Rows shorter than a vector, closer together than one, starting anywhere: the entries against 64 bits, and what lies
+    around the arrays untouched."""
+    g = torch.Generator(device=DEV).manual_seed(rows + width)
+
+    def array(dtype, fill=float("nan")):
+        store = torch.full((at + rows * ld + 40,), fill, device=DEV, dtype=dtype)
+        return store, store[at:at + rows * ld].view(rows, ld)[:, :width]
+    (_, x), (_, dy) = array(xt), array(yt)
+    x.copy_(torch.randn(rows, width, generator=g, device=DEV)), dy.copy_(torch.randn(rows, width, generator=g, device=DEV))
+    (ys, y), (dxs, dx) = array(yt, -7.0), array(xt, -7.0)
+    w = torch.randn(width, generator=g, device=DEV)
+    b, dw, db = torch.randn(width, generator=g, device=DEV), torch.empty(width, device=DEV), torch.empty(width, device=DEV)
+    stats = torch.empty(rows, 2, device=DEV)
+    n_ws = _lib.lib().rk_layernorm_bwd_workspace(rows, width)
+    ws = torch.empty(n_ws // 4, device=DEV)
+    xc, yc, s = _lib.code(xt), _lib.code(yt), _lib.stream_ptr()
+    _lib.call("rk_layernorm_fwd", x.data_ptr(), xc, ld, w.data_ptr(), b.data_ptr(), 0, y.data_ptr(), yc, ld, stats.data_ptr(),
+              rows, width, 1e-3, s)
+    _lib.call("rk_layernorm_bwd", x.data_ptr(), xc, ld, w.data_ptr(), 0, stats.data_ptr(), dy.data_ptr(), yc, ld,
+              dx.data_ptr(), ld, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n_ws, rows, width, s)
+    _check_norm(x, w, b, 1e-3, y, dy, dx, dw, db)
+    for store, part in ((ys, y), (dxs, dx)):
+        part.fill_(-7.0)
+        assert (store == -7.0).all()
