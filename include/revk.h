@@ -358,12 +358,17 @@ RK_API int rk_token_logprob_bwd(const void* logits, int64_t ld, int64_t vocab, c
  * kept (rk_linear_ce_kept(M) bytes, 16-byte aligned) carries the listed rows
  * and their log-sum-exps to the backward, which does not write it. Workspaces
  * are 256-byte aligned; the backward's holds dz of one piece of the vocabulary
- * (up to 512 MB, one 256-column tile at least). copy_w: whether w is copied
+ * (up to 512 MB, one 256-column tile at least), fp32 sums of dx (M x K for each
+ * slice of the reduction) and fp32 tiles of dw on their way out (up to 128 MB,
+ * 512 MB with slices, one tile of rows at least). copy_w: whether w is copied
  * into the workspace, which it is unless it is 16-byte aligned with ldw a
- * multiple of 8. */
+ * multiple of 8. The backward's query takes 1 for that, plus the flags below
+ * for gradients that the call leaves out. */
+#define RK_LINEAR_CE_NO_DX 2
+#define RK_LINEAR_CE_NO_DW 4
 RK_API int64_t rk_linear_ce_kept(int64_t M);
 RK_API int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w);
-RK_API int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w);
+RK_API int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int flags);
 RK_API int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
                             int64_t ignore_index, int64_t M, int64_t V, int64_t K, int dtype, int reduction, float* loss,
                             void* kept, void* workspace, int64_t workspace_bytes, void* stream);

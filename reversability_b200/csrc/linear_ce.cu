@@ -1039,6 +1039,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // dz of one piece. Pieces that stay in L2 cost more in kernels' ends than they save in memory: 64, 128, 256, 512 and 1024
 // MB took 1.99, 1.80, 1.68, 1.59 and 1.62 ms at 14848 x 50257 x 256, 13.5, 12.0, 11.3, 10.8 and 10.9 at 32768 x 50257 x 1024.
 constexpr int64_t kPieceBytes = 512ll << 20;
+// fp32 tiles of dW on their way to another type or to rows that TMA cannot write: a step of the piece's rows at a time, and
+// with slices of the reduction the piece (within kPieceBytes). With few rows a piece is the whole vocabulary, and its
+// tiles at once would be an fp32 copy of the weight (4 GB at 256 x 128256 x 8192).
+constexpr int64_t kStagedBytes = 128ll << 20;
 
 // How the work of (M rows, V, K) is cut. Pure arithmetic, the same for the workspace queries and the calls.
 struct CePlan {
@@ -1047,6 +1051,7 @@ struct CePlan {
   int units;        // row tiles x segments of the forward, at most
   int piece_tiles;  // vocabulary tiles of a piece
   int dx_slices, dw_slices;
+  int dw_step;      // vocabulary tiles of dW staged at a time
 };
 
 // Model of the work in microseconds, for choosing among cuts: a k block of a 256 x 256 tile takes a pair about 0.35, a
@@ -1055,6 +1060,7 @@ double waves_us(int64_t tiles, int64_t slices, int64_t kb) {
   return (double)ceil_div(tiles * slices, kPairs) * (0.35 * (double)ceil_div(kb, slices) + 1.5) + 3.0;
 }
 double moved_us(double bytes) { return bytes / 5e6 + 3.0; }
+int64_t staged_bytes(int64_t tiles, int64_t pitch) { return tiles * kTile * pitch * 4; }
 
 CePlan make_plan(int64_t M, int64_t V, int64_t K) {
   static thread_local CePlan p{};  // of the last sizes asked for: the choice takes some microseconds
@@ -1080,7 +1086,7 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
   for (int n = fewest; n <= fewest + 4 && n <= p.tiles_v; ++n) {
     const int tiles = (int)ceil_div(p.tiles_v, n);
     const int whole = (int)ceil_div(p.tiles_v, tiles) - 1, rest = p.tiles_v - whole * tiles;
-    for (int s = 1; s <= 16 && (s == 1 || kb_rows / s >= 16); ++s) {
+    for (int s = 1; s <= 16 && (s == 1 || (kb_rows / s >= 16 && s * staged_bytes(tiles, p.Kq) <= kPieceBytes)); ++s) {
       double t = 0;
       for (int last = 0; last < 2; ++last) {
         const int64_t v = last ? rest : tiles;
@@ -1095,6 +1101,11 @@ CePlan make_plan(int64_t M, int64_t V, int64_t K) {
         p.dw_slices = s;
       }
     }
+  }
+  p.dw_step = p.piece_tiles;
+  if (p.dw_slices == 1) {  // equal steps
+    const int64_t most = kStagedBytes / staged_bytes(1, p.Kq), steps = ceil_div(p.piece_tiles, most > 1 ? most : 1);
+    p.dw_step = (int)ceil_div(p.piece_tiles, steps);
   }
   best = 1e30;
   const int kb_piece = p.piece_tiles * (kTile / kKb), pieces = (int)ceil_div(p.tiles_v, p.piece_tiles);
@@ -1154,15 +1165,15 @@ struct BwdSpace {
 bool dw_direct(const CePlan& p, const void* dw, int64_t lddw, int dw_dtype, int dtype) {
   return p.dw_slices == 1 && dw_dtype == dtype && rk_host::aligned(dw, 16) && (lddw * 2) % 16 == 0;
 }
-int64_t bwd_space(const CePlan& p, bool copy_w, char* base, BwdSpace* b) {
+int64_t bwd_space(const CePlan& p, bool copy_w, bool dx, bool dw, char* base, BwdSpace* b) {
   Arena a{base, 0};
   b->w = a.take(copy_w ? p.V * p.Kp * 2 : 0);
   b->x = a.take(p.Mp * p.Kp * 2);
   b->dz = a.take(p.Mp * p.piece_tiles * kTile * 2);
   b->rowc = static_cast<float2*>(a.take(p.M * 8));
   b->scale = static_cast<float*>(a.take(4));
-  b->dx = static_cast<float*>(a.take((int64_t)p.dx_slices * p.Mp * p.Kq * 4));
-  b->dw = static_cast<float*>(a.take((int64_t)p.dw_slices * p.piece_tiles * kTile * p.Kq * 4));
+  b->dx = static_cast<float*>(a.take(dx ? (int64_t)p.dx_slices * p.Mp * p.Kq * 4 : 0));
+  b->dw = static_cast<float*>(a.take(dw ? p.dw_slices * staged_bytes(p.dw_step, p.Kq) : 0));
   return a.at;
 }
 
@@ -1263,10 +1274,10 @@ extern "C" int64_t rk_linear_ce_fwd_workspace(int64_t M, int64_t V, int64_t K, i
   return fwd_space(make_plan(M, V, K), copy_w != 0, nullptr, &f);
 }
 
-extern "C" int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int copy_w) {
+extern "C" int64_t rk_linear_ce_bwd_workspace(int64_t M, int64_t V, int64_t K, int flags) {
   if (!sizes_ok(M, V, K) || M == 0) return 0;
   BwdSpace b;
-  return bwd_space(make_plan(M, V, K), copy_w != 0, nullptr, &b);
+  return bwd_space(make_plan(M, V, K), flags & 1, !(flags & RK_LINEAR_CE_NO_DX), !(flags & RK_LINEAR_CE_NO_DW), nullptr, &b);
 }
 
 extern "C" int rk_linear_ce_fwd(const void* hidden, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
@@ -1356,9 +1367,9 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   const CePlan p = make_plan(M, V, K);
   BwdSpace b;
   const bool copy_w = !w_ready(w, ldw, V);
-  if (!workspace || workspace_bytes < bwd_space(p, copy_w, nullptr, &b)) return RK_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < bwd_space(p, copy_w, dx, dw, nullptr, &b)) return RK_ERR_WORKSPACE;
   if (!rk_host::aligned(workspace, 256)) return RK_ERR_ALIGN;
-  bwd_space(p, copy_w, static_cast<char*>(workspace), &b);
+  bwd_space(p, copy_w, dx, dw, static_cast<char*>(workspace), &b);
   const CeKept k = kept_of(const_cast<int*>(static_cast<const int*>(kept)), M);
   float* scale = b.scale;
   const bool in_place = readable(hidden, ldh, p);
@@ -1372,13 +1383,12 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   if ((st = weight_rows(w, ldw, p, b.w, s)) != RK_OK) return st;
   const int64_t pitch = (int64_t)p.piece_tiles * kTile;  // of dz
   const bool direct = dw && dw_direct(p, dw, lddw, dw_dtype, dtype);
-  CUtensorMap x_k, x_mn, in_k, in_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out, dw_out;
+  CUtensorMap x_k, x_mn, in_k, in_mn, w_k, w_mn, dz_out, dz_k, dz_mn, dx_out{}, dw_out{};
   if (!tensor_map(&x_k, b.x, K, p.Mp, p.Kp, dtype, kKb, kHalf) || !tensor_map(&x_mn, b.x, K, p.Mp, p.Kp, dtype, 64, kKb) ||
       !tensor_map(&w_k, w, K, V, ldw, dtype, kKb, kHalf) || !tensor_map(&w_mn, w, K, V, ldw, dtype, 64, kKb) ||
       !tensor_map(&dz_out, b.dz, pitch, p.Mp, pitch, dtype, 32, 32) ||
       !tensor_map(&dz_k, b.dz, pitch, p.Mp, pitch, dtype, kKb, kHalf) ||
-      !tensor_map(&dz_mn, b.dz, pitch, p.Mp, pitch, dtype, 64, kKb) ||
-      !tensor_map(&dx_out, b.dx, K, (int64_t)p.dx_slices * p.Mp, p.Kq, RK_F32, 32, 32))
+      (dx && !tensor_map(&dx_out, b.dx, K, (int64_t)p.dx_slices * p.Mp, p.Kq, RK_F32, 32, 32)))
     return RK_ERR_LAUNCH;
   in_k = x_k;
   in_mn = x_mn;
@@ -1386,8 +1396,9 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
   if (in_place && (!tensor_map(&in_k, hidden, K, M, ldi, dtype, kKb, kHalf) ||
                    !tensor_map(&in_mn, hidden, K, M, ldi, dtype, 64, kKb)))
     return RK_ERR_LAUNCH;
-  if (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dtype, 32, 32)
-             : !tensor_map(&dw_out, b.dw, K, (int64_t)p.dw_slices * pitch, p.Kq, RK_F32, 32, 32))
+  const int step = direct ? p.piece_tiles : p.dw_step;  // vocabulary tiles of a launch for dW
+  if (dw && (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dtype, 32, 32)
+                    : !tensor_map(&dw_out, b.dw, K, (int64_t)p.dw_slices * step * kTile, p.Kq, RK_F32, 32, 32)))
     return RK_ERR_LAUNCH;
   CeArgs g{};
   g.in_place_rows = in_place ? (int)M : -1;
@@ -1420,19 +1431,25 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
       st = launch<ADD, float>(dz_k, w_mn, dx_out, dz_k, g, dtype, (int64_t)p.tiles_m * p.tiles_k * p.dx_slices, s);
       if (st != RK_OK) return st;
     }
-    if (dw) {
+    for (int r0 = 0; dw && r0 < tiles; r0 += step) {
+      const int n_tiles = tiles - r0 < step ? tiles - r0 : step;
+      const int64_t first = (int64_t)r0 * kTile;  // of the piece's rows of dW, and columns of dz
+      if (!tensor_map(&dz_mn, static_cast<uint16_t*>(b.dz) + first, pitch - first, p.Mp, pitch, dtype, 64, kKb))
+        return RK_ERR_LAUNCH;
       g.tiles_n = p.tiles_k;
-      g.row_tiles = tiles;
+      g.row_tiles = n_tiles;
       g.slices = p.dw_slices;
-      g.slice_rows = direct ? 0 : (int)pitch;
-      const int64_t n = (int64_t)tiles * p.tiles_k * p.dw_slices;
+      g.slice_rows = direct ? 0 : step * kTile;
+      const int64_t n = (int64_t)n_tiles * p.tiles_k * p.dw_slices;
       if (!direct) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       else if (dtype == RK_BF16) st = launch<OUTER_T, __nv_bfloat16>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       else st = launch<OUTER_T, __half>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       if (st != RK_OK) return st;
       if (!direct) {
-        char* out = static_cast<char*>(dw) + v0 * lddw * (int64_t)rk_host::dtype_size(dw_dtype);
-        if ((st = reduce(b.dw, p.dw_slices, pitch, p.Kq, nullptr, scale, out, lddw, live, K, dw_dtype, s)) != RK_OK)
+        char* out = static_cast<char*>(dw) + (v0 + first) * lddw * (int64_t)rk_host::dtype_size(dw_dtype);
+        const int64_t left = live - first, rows = left < (int64_t)n_tiles * kTile ? left : (int64_t)n_tiles * kTile;
+        if ((st = reduce(b.dw, p.dw_slices, (int64_t)step * kTile, p.Kq, nullptr, scale, out, lddw, rows, K, dw_dtype, s)) !=
+            RK_OK)
           return st;
       }
     }

@@ -520,10 +520,15 @@ def _linear_ce_check(hidden, weight, labels, reduction):
 
 
 @functools.lru_cache(maxsize=64)
-def _linear_ce_bytes(M: int, V: int, K: int, copy_w: bool) -> tuple[int, int, int]:
+def _linear_ce_bytes(M: int, V: int, K: int, copy_w: bool) -> tuple[int, int]:
     lib = _lib.lib()
-    return (lib.rk_linear_ce_kept(M), lib.rk_linear_ce_fwd_workspace(M, V, K, copy_w),
-            lib.rk_linear_ce_bwd_workspace(M, V, K, copy_w))
+    return lib.rk_linear_ce_kept(M), lib.rk_linear_ce_fwd_workspace(M, V, K, copy_w)
+
+
+@functools.lru_cache(maxsize=64)
+def _linear_ce_bwd_bytes(M: int, V: int, K: int, copy_w: bool, dx: bool, dw: bool) -> int:
+    flags = copy_w + (0 if dx else 2) + (0 if dw else 4)  # RK_LINEAR_CE_NO_DX, RK_LINEAR_CE_NO_DW
+    return _lib.lib().rk_linear_ce_bwd_workspace(M, V, K, flags)
 
 
 def _head_weight(weight: torch.Tensor) -> tuple[torch.Tensor, int, bool]:
@@ -546,7 +551,7 @@ def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
         return _linear_ce_fwd_f32(hidden, weight, labels, ignore_index, reduction, loss)
     x, M, _, ld = even_rows(hidden)
     w, ldw, copy_w = _head_weight(weight)
-    n_kept, n_ws, _ = _linear_ce_bytes(M, V, K, copy_w)
+    n_kept, n_ws = _linear_ce_bytes(M, V, K, copy_w)
     kept = labels.new_empty(n_kept // 4, dtype=torch.int32)
     ws = labels.new_empty(n_ws, dtype=torch.uint8)
     _lib.call("rk_linear_ce_fwd", x.data_ptr(), ld, w.data_ptr(), ldw, labels.data_ptr(), int(ignore_index), M, V, K,
@@ -573,7 +578,7 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
     _on_current_device(hidden, "hidden", weight, kept)
     x, M, _, ld = even_rows(hidden)
     w, ldw, copy_w = _head_weight(weight)
-    n_ws = _linear_ce_bytes(M, V, K, copy_w)[2]
+    n_ws = _linear_ce_bwd_bytes(M, V, K, copy_w, want_dx, want_dw)
     ws = hidden.new_empty(n_ws, dtype=torch.uint8)
     _lib.call("rk_linear_ce_bwd", x.data_ptr(), ld, w.data_ptr(), ldw, kept.data_ptr(), M, V, K,
               _lib.code(hidden.dtype), _REDUCTIONS[reduction], grad.data_ptr(), _lib.ptr(dx), K,

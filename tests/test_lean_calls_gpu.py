@@ -164,3 +164,37 @@ def test_layer_norm_entries_on_narrow_rows_at_any_address(rows, width, ld, at, x
     for store, part in ((ys, y), (dxs, dx)):
         part.fill_(-7.0)
         assert (store == -7.0).all()
+
+
+@pytest.mark.parametrize("M,V,K", [(300, 9000, 8200), (40, 5000, 16384), (700, 20011, 2056)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_weight_gradients_staged_a_step_at_a_time(M, V, K, dtype):
+    """An fp32 weight gradient, whose tiles leave through a buffer of some of them: what the 16-bit one is rounded from; and
+    each gradient alone, in a workspace without the other's part."""
+    g = torch.Generator(device=DEV).manual_seed(K)
+    w = (torch.randn(V, K, generator=g, device=DEV) * (2 / K ** 0.5)).to(dtype)
+    y = torch.randint(0, V, (M,), generator=g, device=DEV)
+    x = (torch.randn(M, K, generator=g, device=DEV) + w[y].float()).to(dtype)
+    y[::5] = -100
+    _, kept = fn.linear_ce_fwd(x, w, y)
+    up = torch.tensor(64.0, device=DEV)
+    dx, dw = fn.linear_ce_bwd(x, w, kept, up)
+    dx32, dw32 = fn.linear_ce_bwd(x, w, kept, up, dx_dtype=F32, dw_dtype=F32)
+    assert torch.equal(dw32.to(dtype), dw) and torch.equal(dx32.to(dtype), dx)
+    assert torch.equal(fn.linear_ce_bwd(x, w, kept, up, want_dx=False, dw_dtype=F32)[1], dw32)
+    assert torch.equal(fn.linear_ce_bwd(x, w, kept, up, want_dw=False, dx_dtype=F32)[0], dx32)
+    X, live = x.double(), y >= 0
+    some = torch.randint(0, V, (97,), generator=g, device=DEV)
+    some[0], some[1] = 0, V - 1
+    z = torch.cat([X @ w[s:s + 2000].double().T for s in range(0, V, 2000)], 1)
+    p = (torch.softmax(z, 1) - torch.nn.functional.one_hot(y.clamp(min=0), V)) * live[:, None] * (64 / live.sum())
+    part = p[:, some]
+    want = part.T @ X
+    # as in test_linear_ce_gpu: logits off by (K / 16 + 16) 2e sum|x w|, terms rounded to 16 bits one by one, fp32 sums
+    e, h = 2.0 ** -24, {BF16: 2.0 ** -8, F16: 2.0 ** -11}[dtype]
+    q = 2 * (K / 16 + 16) * 2 * e * (X.abs() @ w.double().abs().amax(0)) + 4e-6
+    soft = part + torch.nn.functional.one_hot(y.clamp(min=0), V)[:, some] * live[:, None] * (64 / live.sum())
+    tol = 7 * h * (part.square().T @ X.square()).sqrt() + (soft * q[:, None]).T @ X.abs() + \
+        (M / 16 + 64) * 2 * e * (part.abs().T @ X.abs()) + 2.0 ** -38 * 64 * X.abs().sum(0)
+    assert ((dw32[some].double() - want).abs() <= tol + 1e-12).all()
+    assert _lib.device_status() == 0

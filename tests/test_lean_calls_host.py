@@ -42,3 +42,19 @@ def test_layer_norm_backward_refuses_saved_tensors_of_other_sizes(recorded):
     with pytest.raises(ValueError):
         y.backward(torch.zeros_like(y))
     assert recorded[-1][0] == "rk_layernorm_fwd"
+
+
+def test_head_loss_workspace_holds_what_the_call_writes():
+    """dz of a piece and the gathered rows; sums of dx only with dx; tiles of dW only with dW, and not the whole of it."""
+    lib, MB, NO_DX, NO_DW = _lib.lib(), 1 << 20, 2, 4
+    for M, V, K in ((256, 128256, 8192), (1024, 151936, 4096), (4096, 131072, 4096), (14848, 50257, 256), (32768, 50257, 1024)):
+        both, no_dx, no_dw, none = (lib.rk_linear_ce_bwd_workspace(M, V, K, f) for f in (0, NO_DX, NO_DW, NO_DX | NO_DW))
+        rows, tiles = -(-M // 256) * 256, -(-V // 256)
+        dz = min(512 * MB, rows * tiles * 512)
+        gathered = rows * K * 2
+        assert none <= dz + gathered + rows * 8 + MB
+        assert 0 < both - no_dx == no_dw - none <= 16 * rows * K * 4  # whole slices of dx
+        assert (both - no_dx) % (rows * K * 4) == 0
+        assert 0 < both - no_dw == no_dx - none <= 128 * MB or (both - no_dw) % (256 * K * 4) == 0 and both - no_dw <= 512 * MB
+        assert lib.rk_linear_ce_bwd_workspace(M, V, K, 1) == both + V * K * 2 + -V * K * 2 % 1024
+    assert lib.rk_linear_ce_bwd_workspace(256, 128256, 8192, 0) < 256 * MB  # where dW itself takes 2 GB
