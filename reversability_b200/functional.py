@@ -506,14 +506,18 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _PIECE_BYTES = 512 << 20  # fp32: logits of the rows taken at a time
 
 
-def _linear_ce_check(hidden, weight, labels, reduction):
-    require_cuda(hidden, weight, labels, what="the head loss")
+def _linear_ce_check_inputs(hidden, weight, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
     if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or 0 in weight.shape:
         raise ValueError("the head loss takes hidden [..., d] and a non-empty weight [vocabulary, d]")
     if hidden.dtype != weight.dtype or hidden.dtype not in _lib.DTYPE_CODE:
         raise ValueError("hidden and weight must share a type: fp32, bf16 or fp16")
+
+
+def _linear_ce_check(hidden, weight, labels, reduction):
+    require_cuda(hidden, weight, labels, what="the head loss")
+    _linear_ce_check_inputs(hidden, weight, reduction)
     if labels.dtype is not torch.int64 or labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels must be int64 of shape {tuple(hidden.shape[:-1])}")
     _on_current_device(hidden, "hidden", weight, labels)
@@ -565,17 +569,21 @@ def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor
                   dx_dtype: torch.dtype | None = None, dw_dtype: torch.dtype | None = None):
     """(d hidden, d weight) for the loss's gradient (a device scalar; one a row with reduction "none"), in the inputs'
     types unless others are given; None where not wanted."""
+    _linear_ce_check_inputs(hidden, weight, reduction)
     V, K = weight.shape
+    rows, f32 = hidden.shape[:-1].numel(), hidden.dtype is torch.float32
+    if kept.dtype is not (torch.int64 if f32 else torch.int32) or kept.numel() != (rows if f32 else 4 + 4 * rows) or \
+            not kept.is_contiguous():
+        raise ValueError("kept must be what linear_ce_fwd returned for hidden")
     if grad.dtype is not torch.float32 or not grad.is_contiguous():
         grad = grad.detach().float().contiguous()
-    if grad.get_device() != hidden.get_device() or \
-            grad.numel() != (hidden.shape[:-1].numel() if reduction == "none" else 1):
+    if grad.get_device() != hidden.get_device() or grad.numel() != (rows if reduction == "none" else 1):
         raise ValueError("the loss's gradient must be on hidden's device, one number or one a row")
+    _on_current_device(hidden, "hidden", weight, kept)
     dx = _new(hidden, dx_dtype or hidden.dtype) if want_dx else None
     dw = _new(weight, dw_dtype or weight.dtype) if want_dw else None
     if hidden.dtype == torch.float32:
         return _linear_ce_bwd_f32(hidden, weight, kept, grad, reduction, dx, dw)
-    _on_current_device(hidden, "hidden", weight, kept)
     x, M, _, ld = even_rows(hidden)
     w, ldw, copy_w = _head_weight(weight)
     n_ws = _linear_ce_bwd_bytes(M, V, K, copy_w, want_dx, want_dw)

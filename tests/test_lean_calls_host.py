@@ -58,3 +58,24 @@ def test_head_loss_workspace_holds_what_the_call_writes():
         assert 0 < both - no_dw == no_dx - none <= 128 * MB or (both - no_dw) % (256 * K * 4) == 0 and both - no_dw <= 512 * MB
         assert lib.rk_linear_ce_bwd_workspace(M, V, K, 1) == both + V * K * 2 + -V * K * 2 % 1024
     assert lib.rk_linear_ce_bwd_workspace(256, 128256, 8192, 0) < 256 * MB  # where dW itself takes 2 GB
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_head_loss_backward_refuses_what_the_forward_did_not_keep(recorded, dtype):
+    """kept, weight and gradient of other sizes would be read behind their ends."""
+    x, w, up = torch.zeros(6, 8, dtype=dtype), torch.zeros(11, 8, dtype=dtype), torch.ones(())
+    kept = torch.zeros(6, dtype=torch.int64) if dtype == torch.float32 else torch.zeros(4 + 4 * 6, dtype=torch.int32)
+    for bad, match in ((lambda: fn.linear_ce_bwd(x, w, kept[:-1], up), "kept"),
+                       (lambda: fn.linear_ce_bwd(x, w, kept.float(), up), "kept"),
+                       (lambda: fn.linear_ce_bwd(x[:5], w, kept, up), "kept"),
+                       (lambda: fn.linear_ce_bwd(x, w[:, :4], kept, up), "weight"),
+                       (lambda: fn.linear_ce_bwd(x, w.double(), kept, up), "share a type"),
+                       (lambda: fn.linear_ce_bwd(x, w, kept, up, "max"), "reduction"),
+                       (lambda: fn.linear_ce_bwd(x, w, kept, up, "none"), "one a row"),
+                       (lambda: fn.linear_ce_bwd(x, w, kept, torch.ones(6)), "one number")):
+        with pytest.raises(ValueError, match=match):
+            bad()
+    assert not recorded
+    if dtype != torch.float32:
+        fn.linear_ce_bwd(x, w, kept, up)
+        assert recorded[-1][0] == "rk_linear_ce_bwd"
