@@ -3,9 +3,10 @@ gradients that are not numbers to count with, several pieces of the vocabulary."
 import pytest
 import torch
 from test_norm_dropout_gpu import _check as _check_norm  # with the tolerances derived there
+from test_linear_ce_gpu import E, HALF_ULP, _check as _check_head, _inputs  # the same
 from torch.autograd import forward_ad
 
-from reversability_b200 import _lib, alignment, functional as fn, functions as fx
+from reversability_b200 import ModelConfig, ReversibleLM, _lib, alignment, functional as fn, functions as fx, optimized, optimized_v3
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -198,3 +199,116 @@ def test_weight_gradients_staged_a_step_at_a_time(M, V, K, dtype):
         (M / 16 + 64) * 2 * e * (part.abs().T @ X.abs()) + 2.0 ** -38 * 64 * X.abs().sum(0)
     assert ((dw32[some].double() - want).abs() <= tol + 1e-12).all()
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("M,V,K", [(16500, 48500, 24), (16500, 49500, 264), (120000, 5000, 40)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_several_pieces_of_the_vocabulary(M, V, K, dtype):
+    """Three pieces and more, the last one shorter and ending inside a tile, over many row tiles with ignored rows: both
+    gradients against 64 bits, a chunk of rows at a time, with the tolerances of test_linear_ce_gpu."""
+    Mp = -(-M // 256) * 256
+    assert _lib.lib().rk_linear_ce_bwd_workspace(M, V, K, 6) < Mp * -(-V // 256) * 512 / 2  # dz of less than half of the tiles
+    x, w, y = _inputs(M, V, K, dtype)
+    rows = fx.linear_cross_entropy(x, w, y, reduction="none")
+    up = torch.rand(M, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)) - 0.5
+    dx, dw = torch.autograd.grad(rows, (x, w), up)
+    W, h = w.detach().double(), HALF_ULP[dtype]
+    sums = [torch.zeros(V, K, device=DEV, dtype=torch.float64) for _ in range(4)]
+    live = y >= 0
+    assert not rows[~live].any() and not dx[~live].any()
+    top = up[live].abs().max().double()
+    for s in range(0, M, 3000):
+        n = torch.arange(s, min(s + 3000, M), device=DEV)
+        n = n[live[n]]
+        X, t, u = x.detach()[n].double(), y[n][:, None], up[n].double()[:, None]
+        z = X @ W.T
+        size = (X.abs() @ W.abs().T).amax(1)
+        dz = ((K / 16 + 16) * 2 * E * size)[:, None]
+        want = torch.logsumexp(z, 1) - z.gather(1, t)[:, 0]
+        assert ((rows[n].double() - want).abs() <= 2 * dz[:, 0] + 4e-6 + 4 * E * z.abs().amax(1)).all()
+        p = torch.softmax(z, 1)
+        err = p * (2 * dz + 4e-6) * u.abs()
+        d = p.scatter_add(1, t, torch.full_like(p[:, :1], -1.0)) * u
+        err += 2 * E * d.abs() + 2.0 ** -38 * top
+        want = d @ W
+        tol = 7 * h * (d.square() @ W.square()).sqrt() + err @ W.abs() + (V / 16 + 64) * 2 * E * (d.abs() @ W.abs()) + h * want.abs()
+        assert ((dx[n].double() - want).abs() <= tol + 3e-8).all()
+        for total, part in zip(sums, (d.T @ X, d.square().T @ X.square(), err.T @ X.abs(), d.abs().T @ X.abs())):
+            total += part
+    want, square, flat, total = sums
+    tol = 7 * h * square.sqrt() + flat + (M / 16 + 64) * 2 * E * total + h * want.abs()
+    assert ((dw.double() - want).abs() <= tol + 3e-8).all()
+    again = torch.autograd.grad(fx.linear_cross_entropy(x, w, y, reduction="none"), (x, w), up)
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("compute", [BF16, F16])
+def test_pieces_backward_under_a_loss_scaler(compute):
+    """fp32 gradients of fp32 hidden states with the scaler's factor in them, from operands of 16 bits."""
+    x, w, y = _inputs(900, 1100, 72, F32)
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 16)
+    total, dx, dw = optimized.head_pieces_backward(x.detach(), w, y, 640, compute, scaler)
+    lx, lw = x.detach().to(compute), w.detach().to(compute)
+    rows = fx.linear_cross_entropy(lx, lw, y, reduction="none")
+    assert dx.dtype == dw.dtype == F32 and abs(total.double() - rows.double().sum()) <= E * total.abs()
+    _check_head(lx, lw, y, torch.full((900,), 1 / 640, device=DEV), rows, dx, dw, 2.0 ** 16)
+
+
+@pytest.mark.parametrize("call", [optimized.chunked_backward, optimized_v3.cached_head_backward])
+def test_pieces_as_a_loss_backend_in_fp16_with_a_scaler(call):
+    """The explicit training step under a loss scaler: 'pieces' against the chunked softmax head, whose logits are fp16
+    (|z| < 2: off by 2^-11 each) and whose hidden gradients are, once more, an eighth of what bf16 may differ by."""
+    ids = torch.randint(0, 997, (4, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(0))
+    labels = ids.roll(-1, 1).clone()
+    labels[:, -1], labels[0, :40] = -100, -100
+    grads = {}
+    for backend in ("cuda", "pieces"):
+        torch.manual_seed(3)
+        model = ReversibleLM(ModelConfig(vocab_size=997, max_sequence_length=64, n_layers=2, n_heads=4, d_model=128, d_ff=256),
+                             "midpoint").to(DEV)
+        scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 12)
+        loss = call(model, ids, labels, 200, 96, scaler=scaler, precision="fp16", loss_backend=backend)
+        grads[backend] = [loss] + [p.grad for p in model.parameters()]
+    for a, b in zip(grads["cuda"], grads["pieces"]):
+        assert torch.isfinite(b).all() and (a - b).norm() <= 2.0 ** -9 * a.norm()
+
+
+def _philox(counter, key):
+    """Philox 4x32, 10 rounds, in Python's whole numbers."""
+    c, k = list(counter), list(key)
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [b >> 32 ^ c[1] ^ k[0], b & 0xFFFFFFFF, a >> 32 ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def test_the_generator_at_its_known_answers():
+    """The published vectors, of all-zero and all-one counters and keys and of digits of pi, pin the restatement; the masks
+    pin the kernel to it under the keys of the second and third."""
+    ones = 0xFFFFFFFF
+    assert _philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert _philox([ones] * 4, [ones] * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    pi = [0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0]
+    assert _philox(*pi) == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    x = torch.ones(8, device=DEV)
+    for offset, key in (([ones, ones], [ones, ones]), (pi[0][2:], pi[1])):
+        words = [v for block in range(2) for v in _philox([block, 0, *offset], key)]
+        seed, at = key[0] + (key[1] << 32), offset[0] + (offset[1] << 32)
+        for i, word in enumerate(words):
+            assert [bool(fx.dropout(x, b / 2 ** 32, seed, offset=at)[i]) for b in (word, word + 1)] == [True, False]
+
+
+def test_dropout_past_the_lower_half_of_the_block_number():
+    """More than 2^34 elements: from there on the block number's upper 32 bits count."""
+    torch.cuda.empty_cache()
+    n = (1 << 34) + 4099
+    x = torch.ones(n, device=DEV, dtype=BF16)
+    y = fx.dropout(x, 0.5, 21, offset=2)
+    del x
+    for first, last in (((1 << 34) - 4096, (1 << 34) + 4096), ((1 << 34) + 4096, n)):  # whole tiles on both sides, the rest
+        words = [v for b in range(first // 4, (last + 3) // 4) for v in _philox([b & 0xFFFFFFFF, b >> 32, 2, 0], [21, 0])]
+        assert torch.equal(y[first:last] != 0, torch.tensor(words[:last - first], device=DEV) >= 1 << 31)
+    del y
+    torch.cuda.empty_cache()
