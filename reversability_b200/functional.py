@@ -10,7 +10,6 @@ from __future__ import annotations
 import functools
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -21,13 +20,6 @@ def require_cuda(*tensors: torch.Tensor, what: str = "librevk kernels") -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError(f"{what} require CUDA tensors; no CPU fallback exists")
-
-
-def carries_tangent(*tensors: torch.Tensor | None) -> bool:
-    """Whether one of the tensors is a dual number of forward-mode differentiation."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open (asking each tensor takes 0.6 us)
-        return False
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _row_major_2d(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
@@ -183,20 +175,18 @@ def _layernorm_workspace(rows: int, width: int) -> int:
     return _lib.lib().rk_layernorm_bwd_workspace(rows, width)
 
 
-def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
-                  param_dtype: torch.dtype = torch.float32, want_dx: bool = True, want_dw: bool = True,
-                  want_db: bool = True):
-    """(dx in x's type, dweight, dbias in param_dtype; None where not wanted) of layernorm_fwd. Rows, strides and types are
-    those of the tensors given: hooks on saved tensors need not hand back the strides that the forward saw."""
-    require_cuda(x, weight, stats, dy, what="layer norm kernels")
-    _on_current_device(x, "the input", weight, stats, dy)
-    weight, _, _ = _norm_params(x, weight, None)
-    if weight is not None and weight.dtype != param_dtype:
-        raise ValueError("parameter gradients come in the weight's type")
-    per = 16 // x.element_size()
+def layernorm_bwd_kept(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+                       param_dtype: torch.dtype, want_dx: bool, want_dw: bool, want_db: bool):
+    """layernorm_bwd of what layernorm_fwd_kept returned. Rows, strides, sizes and devices are looked at anew: hooks on saved
+    tensors need not hand back the strides that the forward saw."""
+    per, device = 16 // x.element_size(), dy.get_device()
     xr, rows, width, ldx = _fast_rows(x, per)
-    if dy.shape != x.shape or stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+    if dy.numel() != x.numel() or stats.numel() != 2 * rows or stats.dtype is not torch.float32 or \
+            not stats.is_contiguous() or x.get_device() != device or stats.get_device() != device:
         raise ValueError("layer norm backward takes dy of the input's shape and the forward's stats")
+    if weight is not None and (weight.numel() != width or weight.dtype is not param_dtype or not weight.is_contiguous() or
+                               weight.get_device() != device):
+        raise ValueError("layer norm backward takes the forward's weight")
     dyr, _, _, lddy = _fast_rows(dy, per)
     dx = _new(xr, x.dtype) if want_dx else None
     dw = (x.new_empty(width, dtype=param_dtype) if weight is None else torch.empty_like(weight)) if want_dw else None
@@ -207,6 +197,20 @@ def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Ten
               stats.data_ptr(), dyr.data_ptr(), _lib.code(dy.dtype), lddy, _lib.ptr(dx), width, _lib.ptr(dw), _lib.ptr(db),
               _lib.ptr(ws), n_ws, rows, width, _lib.stream_ptr())
     return dx, dw, db
+
+
+def layernorm_bwd(x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+                  param_dtype: torch.dtype = torch.float32, want_dx: bool = True, want_dw: bool = True,
+                  want_db: bool = True):
+    """(dx in x's type, dweight, dbias in param_dtype; None where not wanted) of layernorm_fwd."""
+    require_cuda(x, weight, stats, dy, what="layer norm kernels")
+    _on_current_device(x, "the input", weight, stats, dy)
+    weight, _, _ = _norm_params(x, weight, None)
+    if weight is not None and weight.dtype != param_dtype:
+        raise ValueError("parameter gradients come in the weight's type")
+    if dy.shape != x.shape:
+        raise ValueError("layer norm backward takes dy of the input's shape and the forward's stats")
+    return layernorm_bwd_kept(x, weight, stats, dy, param_dtype, want_dx, want_dw, want_db)
 
 
 # ------------------------------------------------------------------ dropout
