@@ -46,7 +46,8 @@ constexpr int kKb = 64;     // reduction elements of a stage
 constexpr float kLog2e = 1.4426950408889634f;
 
 // STATS: running (max, sum exp) per row; DLOGITS: dz of a piece, 16 bits; ADD: fp32 tiles stored or added, A K-major
-// (dx); OUTER: the same with A MN-major (slices of dW); OUTER_T: A MN-major, scaled and stored in 16 bits (dW).
+// (dx); OUTER: fp32 with A MN-major (dW: slices of it, or scaled to where it belongs); OUTER_T: A MN-major, scaled and
+// stored in 16 bits (dW).
 enum { STATS = 0, DLOGITS = 1, ADD = 2, OUTER = 3, OUTER_T = 4 };
 
 constexpr int kEpiWarps = 16;
@@ -84,7 +85,8 @@ struct CeArgs {
   float* xlabel;     // STATS: logit at the label, per listed row
   const int* label;  // labels of the listed rows
   const float2* rowc;  // DLOGITS: per listed row (-lse log2 e, factor of dz)
-  const float* scale;  // OUTER_T
+  const float* scale;  // OUTER_T, OUTER to dW itself
+  int to_weight;       // OUTER: the output is dW, not a buffer of its tiles
   unsigned int* status;
   // STATS with loss set (few rows): the last CTA to finish joins the rows and writes lse and loss
   int* head;
@@ -523,7 +525,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
     float run_m = -INFINITY, run_s = 0.f;  // STATS: reference and sum of exp(z - reference), z in units of log 2
     int label = -1;
     float2 rc = make_float2(0.f, 0.f);
-    const float scale = MODE == OUTER_T ? *g.scale : 1.f;
+    const bool to_weight = MODE == OUTER_T || (MODE == OUTER && g.to_weight);
+    const float scale = to_weight ? *g.scale : 1.f;
     for (CeWalk<MODE> w(g, pair, pairs); w.more(); w.next(g)) {
       if ((MODE == STATS || MODE == DLOGITS) && w.first) {
         const int row = w.m0 + local;
@@ -599,7 +602,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
             for (int k = 0; k < 32; ++k)
               if (k >= valid) v[k] = 0.f;
           }
-        } else if constexpr (MODE == OUTER_T) {
+        } else if constexpr (A_MN) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] *= scale;
         }
@@ -622,8 +625,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          const int yy = MODE == OUTER_T ? g.v0 + y : y;
-          if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && (MODE != OUTER_T || yy < g.vocab)))) {
+          const int yy = to_weight ? g.v0 + y : y;
+          if (lane == 0 && (MODE == DLOGITS || (c0 < g.width && (!to_weight || yy < g.vocab)))) {
             if (MODE == ADD && g.add) reduce_add_2d(&tmC, smem_u32(buf), c0, yy);
             else store_2d(&tmC, smem_u32(buf), c0, yy);
             stores_commit();
@@ -1039,9 +1042,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // dz of one piece. Pieces that stay in L2 cost more in kernels' ends than they save in memory: 64, 128, 256, 512 and 1024
 // MB took 1.99, 1.80, 1.68, 1.59 and 1.62 ms at 14848 x 50257 x 256, 13.5, 12.0, 11.3, 10.8 and 10.9 at 32768 x 50257 x 1024.
 constexpr int64_t kPieceBytes = 512ll << 20;
-// fp32 tiles of dW on their way to another type or to rows that TMA cannot write: a step of the piece's rows at a time, and
-// with slices of the reduction the piece (within kPieceBytes). With few rows a piece is the whole vocabulary, and its
-// tiles at once would be an fp32 copy of the weight (4 GB at 256 x 128256 x 8192).
+// fp32 tiles of dW on their way to rows that TMA cannot write (or the other 16-bit type): a step of the piece's rows at a
+// time, and with slices of the reduction the piece (within kPieceBytes). With few rows a piece is the whole vocabulary, and
+// its tiles at once would be an fp32 copy of the weight (4 GB at 256 x 128256 x 8192).
 constexpr int64_t kStagedBytes = 128ll << 20;
 
 // How the work of (M rows, V, K) is cut. Pure arithmetic, the same for the workspace queries and the calls.
@@ -1161,9 +1164,10 @@ struct BwdSpace {
   float2* rowc;
   float *scale, *dx, *dw;
 };
-// fp32 slices of dW are used unless each tile can leave in the weight's type at once.
+// Tiles of dW are stored in fp32 and converted after that unless each can leave at once, in the operands' type or fp32.
 bool dw_direct(const CePlan& p, const void* dw, int64_t lddw, int dw_dtype, int dtype) {
-  return p.dw_slices == 1 && dw_dtype == dtype && rk_host::aligned(dw, 16) && (lddw * 2) % 16 == 0;
+  return p.dw_slices == 1 && (dw_dtype == dtype || dw_dtype == RK_F32) && rk_host::aligned(dw, 16) &&
+         lddw * (int64_t)rk_host::dtype_size(dw_dtype) % 16 == 0;
 }
 int64_t bwd_space(const CePlan& p, bool copy_w, bool dx, bool dw, char* base, BwdSpace* b) {
   Arena a{base, 0};
@@ -1397,7 +1401,7 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
                    !tensor_map(&in_mn, hidden, K, M, ldi, dtype, 64, kKb)))
     return RK_ERR_LAUNCH;
   const int step = direct ? p.piece_tiles : p.dw_step;  // vocabulary tiles of a launch for dW
-  if (dw && (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dtype, 32, 32)
+  if (dw && (direct ? !tensor_map(&dw_out, dw, K, V, lddw, dw_dtype, 32, 32)
                     : !tensor_map(&dw_out, b.dw, K, (int64_t)p.dw_slices * step * kTile, p.Kq, RK_F32, 32, 32)))
     return RK_ERR_LAUNCH;
   CeArgs g{};
@@ -1441,7 +1445,8 @@ extern "C" int rk_linear_ce_bwd(const void* hidden, int64_t ldh, const void* w, 
       g.slices = p.dw_slices;
       g.slice_rows = direct ? 0 : step * kTile;
       const int64_t n = (int64_t)n_tiles * p.tiles_k * p.dw_slices;
-      if (!direct) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
+      g.to_weight = direct;
+      if (!direct || dw_dtype == RK_F32) st = launch<OUTER, float>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       else if (dtype == RK_BF16) st = launch<OUTER_T, __nv_bfloat16>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       else st = launch<OUTER_T, __half>(dz_mn, x_mn, dw_out, in_mn, g, dtype, n, s);
       if (st != RK_OK) return st;

@@ -167,11 +167,13 @@ def test_layer_norm_entries_on_narrow_rows_at_any_address(rows, width, ld, at, x
         assert (store == -7.0).all()
 
 
-@pytest.mark.parametrize("M,V,K", [(300, 9000, 8200), (40, 5000, 16384), (700, 20011, 2056)])
+@pytest.mark.parametrize("M,V,K", [(300, 9000, 8200), (40, 5000, 16384), (700, 20011, 2056), (90, 6001, 8197), (300, 9000, 8196), (6, 1, 1),
+                                   (6, 1, 5), (6, 300, 33), (6, 257, 12)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_weight_gradients_staged_a_step_at_a_time(M, V, K, dtype):
-    """An fp32 weight gradient, whose tiles leave through a buffer of some of them: what the 16-bit one is rounded from; and
-    each gradient alone, in a workspace without the other's part."""
+    """A weight gradient in the other 16-bit type, or of a width whose rows TMA cannot write, leaves through a buffer of some
+    of its tiles; one in the operands' type or fp32 at once: all are the fp32 one, rounded. And each gradient alone, in a
+    workspace without the other's part."""
     g = torch.Generator(device=DEV).manual_seed(K)
     w = (torch.randn(V, K, generator=g, device=DEV) * (2 / K ** 0.5)).to(dtype)
     y = torch.randint(0, V, (M,), generator=g, device=DEV)
@@ -182,6 +184,8 @@ def test_weight_gradients_staged_a_step_at_a_time(M, V, K, dtype):
     dx, dw = fn.linear_ce_bwd(x, w, kept, up)
     dx32, dw32 = fn.linear_ce_bwd(x, w, kept, up, dx_dtype=F32, dw_dtype=F32)
     assert torch.equal(dw32.to(dtype), dw) and torch.equal(dx32.to(dtype), dx)
+    other = F16 if dtype == BF16 else BF16
+    assert torch.equal(fn.linear_ce_bwd(x, w, kept, up, dw_dtype=other)[1], dw32.to(other))
     assert torch.equal(fn.linear_ce_bwd(x, w, kept, up, want_dx=False, dw_dtype=F32)[1], dw32)
     assert torch.equal(fn.linear_ce_bwd(x, w, kept, up, want_dw=False, dx_dtype=F32)[0], dx32)
     X, live = x.double(), y >= 0
