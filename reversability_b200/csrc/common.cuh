@@ -251,10 +251,15 @@ __device__ __forceinline__ float rms_rstd(float ss, int width, float eps) {
 // previous kernel on the stream drains. pdl_wait() blocks until that kernel
 // has completed and its writes are visible; a kernel calls it before its first
 // read of inputs or write of outputs; it is a no-op when the launch had no PDL
-// attribute. No kernel triggers its dependents explicitly: the next grid starts
+// attribute. Most kernels do not trigger their dependents: the next grid starts
 // launching as this grid's blocks exit, so its prologue and launch latency
 // overlap this grid's tail without taking SM slots from this grid's main loop
-// (an explicit trigger at kernel entry measured slower).
+// (an explicit trigger at kernel entry measured slower there). Those of
+// linear_ce.cu trigger early, some before their own wait, so a kernel may be
+// resident while the one before its predecessor still runs. Order holds along
+// such a chain only because EVERY kernel of the library executes pdl_wait()
+// before it touches global memory and before it ends: a kernel that ended
+// without it would let its successor run ahead of what came before both.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 }  // namespace rk

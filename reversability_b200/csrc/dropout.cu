@@ -8,10 +8,12 @@
 //            as 1, 2, 3", SC 2011);
 //   kept  iff word i >= round(p 2^32);  y_i = residual_i + (kept ? x_i / (1 - p) : 0)
 //
-// Bound by memory for fp32 and with a residual; in 16 bits without one, where
-// an element moves 4 bytes, by the integer pipes: 20 instructions an element, a
-// quarter of them wide multiplies, half of the rest on the half-rate logic
-// pipe. 134M bf16 elements take 115 us (4.7 TB/s; 163 us with one vector after
+// Bound by memory for fp32 (134M elements 170 us, 6.3 TB/s) and with a residual;
+// in 16 bits without one, where an element moves 4 bytes, by the multipliers: 20
+// instructions an element, a quarter of them wide multiplies, which only one of
+// the two FMA pipes takes (it is busy 80 % of the time, warps stall on it first,
+// 2.4 of 10 to 1.0 on memory), half of the rest on the half-rate logic pipe (57
+// %). 134M bf16 elements take 115 us (4.7 TB/s; 163 us with one vector after
 // the other and nothing shared): what is the same for all blocks of a thread
 // (round keys, the second counter word's first product, the first word's
 // second) is formed once, pairs are scaled and rounded by one instruction, and

@@ -32,7 +32,10 @@
 //
 // 32768 x 1024 bf16: forward 27 us (5.0 TB/s), backward with its columns 41 us
 // (4.9 TB/s); 14848 x 256 fp32 to bf16: 5.9 and 11.9 us in L2; 2047 x 5001
-// fp32: 16.7 (4.9 TB/s) and 39 us (3.1 TB/s; by single elements 33 and 85).
+// fp32: 16.7 (4.9 TB/s) and 39 us (3.1 TB/s; by single elements 33 and 85): a CTA
+// has seven rows there, and 296 partial rows of 40 KB are written and read
+// beside 123 MB of rows. Of twice the rows the backward kernel alone takes 53 us
+// (4.6 TB/s) and waits for its loads first (3.5 warps of 11.5; barriers 0.9).
 #include "vec.cuh"
 
 namespace rk {
@@ -119,8 +122,8 @@ __device__ __forceinline__ void store_part(T* __restrict__ row, bool edge, int c
   }
 }
 
-// Sums over the row's threads (W warps; 0: the CTA), the same values in all of them. Several warps: one barrier; `red` is one of several buffers
-// used in turn, so a buffer is written again only after a barrier that follows its last read.
+// Sums over the row's threads (W warps; 0: the CTA), the same values in all of them. Several warps: one barrier; `red` is
+// one of several buffers used in turn, so a buffer is written again only after a barrier that follows its last read.
 template <int W, bool TWO>
 __device__ __forceinline__ float2 row_sums(float2 v, float2* red) {
 #pragma unroll

@@ -7,13 +7,21 @@
 // Rows whose label is ignored are left out before anything is multiplied: the
 // others are listed and gathered (a padded or masked row costs nothing, and
 // what lies in it cannot spread). Forward: one GEMM over the whole vocabulary
-// whose epilogue keeps a running maximum and sum of exponentials in registers
-// and writes no logits; a row keeps one number, its log-sum-exp. Backward, for
-// each piece of the vocabulary: the logits again, turned in the epilogue into
-// dz / scale (16 bits; the scale of the loss, with which fp16 would underflow, is
-// applied to the fp32 results) in a workspace of rows x
-// piece; then the two gradient GEMMs read it: dx adds up over the pieces in
-// fp32, dW of the piece is final and leaves in the weight's type.
+// whose epilogue keeps a row's sum of exponentials in registers, against a
+// reference that an earlier logit set (fp32 holds terms of up to 2^64 of it; at
+// exponents of that size a term is off by 4e-6, which is what a loss may be off
+// by), and writes no logits; a row keeps one number, its log-sum-exp. Backward,
+// for each piece of the vocabulary: the logits again, turned in the epilogue
+// into dz / scale (16 bits; the scale of the loss, with which fp16 would
+// underflow, is applied to the fp32 results) in a workspace of rows x piece;
+// then the two gradient GEMMs read it: dx adds up over the pieces in fp32, dW of
+// the piece is final and leaves in its type.
+//
+// dz is held in 16 bits because the tensor cores take it so, and half the bytes
+// of fp32 pass between the products. Its terms round independently, so sums of
+// many gain little: bf16 gradients of 14848 rows are 0.0018 off their 64-bit
+// values where their own rounding leaves 0.0017. dW of a handful of rows has only
+// as many terms and is off by up to 0.0025. What needs more takes fp32 inputs.
 //
 // Bound by the tensor cores: 2 M V K operations forward, 6 M V K backward (one
 // third of it the logits again). All four GEMMs are one kernel: CTA pairs
@@ -45,7 +53,7 @@ constexpr int kHalf = 128;  // of them a CTA's rows of A and rows of B
 constexpr int kKb = 64;     // reduction elements of a stage
 constexpr float kLog2e = 1.4426950408889634f;
 
-// STATS: running (max, sum exp) per row; DLOGITS: dz of a piece, 16 bits; ADD: fp32 tiles stored or added, A K-major
+// STATS: running (reference, sum exp) per row; DLOGITS: dz of a piece, 16 bits; ADD: fp32 tiles stored or added, A K-major
 // (dx); OUTER: fp32 with A MN-major (dW: slices of it, or scaled to where it belongs); OUTER_T: A MN-major, scaled and
 // stored in 16 bits (dW).
 enum { STATS = 0, DLOGITS = 1, ADD = 2, OUTER = 3, OUTER_T = 4 };

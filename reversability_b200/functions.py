@@ -150,8 +150,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """F.layer_norm over the last dimension (at most 16384 wide, 16377 if the width is no multiple of 8): statistics in
     fp32, weight and bias (each may be None) in fp32 or x's type, the output in x's type unless out_dtype says otherwise
-    (any type for fp32 x, fp32 for 16-bit x). Rows an even distance apart need no copy. Like the other norms it runs in
-    its input's type under autocast. The gradients of weight and bias are sums in a fixed order."""
+    (any type for fp32 x, fp32 for 16-bit x). Rows of unit stride, an even distance apart, are read where they lie if they
+    start as far from 16-byte boundaries as rows side by side would (x[..., :width] of wider rows, both widths multiples of
+    8, do); others are copied. Like the other norms it runs in its input's type under autocast. The gradients of weight
+    and bias are sums in a fixed order."""
     if differentiated(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, float(eps), out_dtype)
     return fn.layernorm_fwd_kept(x, weight, bias, float(eps), out_dtype, False)[0]
