@@ -59,7 +59,7 @@ def _check_rows(temperature: float, ignore_index: int) -> None:
 
 def _check_constants(**tensors) -> None:
     for name, t in tensors.items():
-        if differentiated(t):
+        if t is not None and differentiated(t):
             raise ValueError(f"{name} is a constant of the loss; detach it")
 
 

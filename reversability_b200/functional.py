@@ -138,9 +138,10 @@ def _norm_params(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tenso
 
 
 def _fast_rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, int, int, int]:
-    if t.is_contiguous() and t.data_ptr() % 32 == 0 and t.shape[-1]:
-        width = t.shape[-1]
-        return t, t.numel() // width, width, width
+    if t.is_contiguous() and t.data_ptr() % 32 == 0:
+        width = t.size(-1)
+        if width:
+            return t, t.numel() // width, width, width
     return _norm_rows(t, per)
 
 
@@ -181,7 +182,7 @@ def layernorm_bwd_kept(x: torch.Tensor, weight: torch.Tensor | None, stats: torc
     tensors need not hand back the strides that the forward saw."""
     per, device = 16 // x.element_size(), dy.get_device()
     xr, rows, width, ldx = _fast_rows(x, per)
-    if dy.numel() != x.numel() or stats.numel() != 2 * rows or stats.dtype is not torch.float32 or \
+    if dy.numel() != rows * width or stats.numel() != 2 * rows or stats.dtype is not torch.float32 or \
             not stats.is_contiguous() or x.get_device() != device or stats.get_device() != device:
         raise ValueError("layer norm backward takes dy of the input's shape and the forward's stats")
     if weight is not None and (weight.numel() != width or weight.dtype is not param_dtype or not weight.is_contiguous() or
